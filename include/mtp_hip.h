@@ -1,12 +1,15 @@
 /*
  * mtp_hip.h -- C-ABI of the MI355X (gfx950) hot path of mlx-train-perf.
  *
- * Two parts, each replacing the reference's mx.fast.metal_kernel launch layer:
+ * Two parts that replace the reference's mx.fast.metal_kernel launch layer:
  *   (A) fused linear cross-entropy (LCE): logit-free forward (per-token NLL, log-sum-exp,
  *       target logit) and the dL/dH backward that recomputes vocab tiles, over a dense bf16 or a
  *       4-bit affine group-quantized (group size 64) head;
  *   (B) flash attention forward and backward with GQA, causal and packed-segment masks, saving
- *       only O and the per-row log-sum-exp L.
+ *       only O and the per-row log-sum-exp L;
+ * and two that the reference lacks:
+ *   (C) attention with capped scores, a bias by distance and key spans;
+ *   (D) preference and policy losses over the per-token losses of (A).
  *
  * Conventions (all entry points):
  *   - Plain pointers and sizes; the caller allocates every tensor and the workspace and owns the
@@ -277,6 +280,96 @@ int mtp_attn_bwd_f32(const float* q, const float* k, const float* v, const float
                      int64_t s, int64_t dh, float scale, int32_t causal, const int32_t* seg_id,
                      const int32_t* seg_start, float* d_q, float* d_k, float* d_v, void* workspace,
                      size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * (C) Attention with capped scores, a bias by distance and key spans (no counterpart in the reference)
+ *
+ * As (B), with the softmax over  cap(scale q_i . k_j) - slopes[h] |i - j|:
+ *   softcap > 0: cap(x) = softcap tanh(x / softcap); 0: cap(x) = x.
+ *   slopes: fp32 [hq], or NULL: no bias. They get no gradient.
+ *   span_start, span_end: int32 [b][s], or both NULL. Key j is visible to query i iff
+ *     span_start[i] <= j < span_end[i]; neither may decrease along a row, and a query whose span holds nothing
+ *     gets o = 0, lse = +inf and no gradient. Spans are the whole mask (causal must be 0). Values outside the
+ *     row are clamped into it; spans that decrease give some wrong rows, never an access out of range.
+ * scale must be positive. At least one of the three must be given (else: mtp_attn_fwd).
+ * ------------------------------------------------------------------------------------------- */
+int mtp_attn_scored_fwd(const void* q, const void* k, const void* v, int64_t b, int64_t hq, int64_t hkv,
+                        int64_t s, int64_t dh, float scale, int32_t causal, float softcap,
+                        const float* slopes, const int32_t* span_start, const int32_t* span_end, void* o,
+                        float* lse, void* stream);
+
+/* Workspace bytes of mtp_attn_scored_bwd, each part padded to 256 bytes: D (fp32 [b][hq][s]), the fp32 dK/dV
+ * partials where the dK/dV pass is split (as mtp_attn_bwd's), and for spans the int32 work orders of the two
+ * passes and the int32 range of queries that see each key (2 x [b][s]). */
+size_t mtp_attn_scored_bwd_workspace_bytes(int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh);
+
+int mtp_attn_scored_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse,
+                        const void* d_o, int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh,
+                        float scale, int32_t causal, float softcap, const float* slopes,
+                        const int32_t* span_start, const int32_t* span_end, void* d_q, void* d_k, void* d_v,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* The same with fp32 tensors; the backward's workspace is mtp_attn_bwd_f32_workspace_bytes. */
+int mtp_attn_scored_fwd_f32(const float* q, const float* k, const float* v, int64_t b, int64_t hq,
+                            int64_t hkv, int64_t s, int64_t dh, float scale, int32_t causal, float softcap,
+                            const float* slopes, const int32_t* span_start, const int32_t* span_end, float* o,
+                            float* lse, void* stream);
+int mtp_attn_scored_bwd_f32(const float* q, const float* k, const float* v, const float* o, const float* lse,
+                            const float* d_o, int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh,
+                            float scale, int32_t causal, float softcap, const float* slopes,
+                            const int32_t* span_start, const int32_t* span_end, float* d_q, float* d_k,
+                            float* d_v, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * (D) Preference and policy losses over per-token losses (no counterpart in the reference)
+ *
+ * nll, old_nll, ref_nll: fp32 [n], the per-token losses of the model and of frozen ones (mtp_lce_fwd's nll).
+ * Sequences: offsets int64 [sequences + 1], sequence r being the tokens [offsets[r], offsets[r + 1]); they
+ * never decrease and lie in [0, n]; tokens of no sequence count nowhere and get a gradient of 0. NULL: the n
+ * tokens are rows of one length. mask: uint8 [n], or NULL; tokens with 0 count nowhere, whatever the tensors
+ * hold there. Sums are in 64 bits, joined in a fixed order.
+ * ------------------------------------------------------------------------------------------- */
+#define MTP_PREF_SIGMOID 0
+#define MTP_PREF_HINGE 1
+#define MTP_PREF_IPO 2
+#define MTP_REDUCE_NONE 0
+#define MTP_REDUCE_MEAN 1
+#define MTP_REDUCE_SUM 2
+#define MTP_REDUCE_SEQUENCES 3
+
+size_t mtp_pref_workspace_bytes(int64_t pairs, int64_t n);
+
+/* Preference loss of 2 pairs sequences, p chosen and pairs + p rejected. With the log ratio
+ * g_r = sum_t (ref_nll - nll) (ipo: its mean), rewards[r] = beta g_r and d = rewards[p] - rewards[pairs + p]:
+ *   sigmoid: -(1 - e) log sigmoid(d) - e log sigmoid(-d), e = label_smoothing; hinge: max(0, 1 - d);
+ *   ipo: (d / beta - 1 / (2 beta))^2.
+ * loss: fp32 [pairs] (none) or [1] (mean, sum); rewards, coef: fp32 [2 pairs]; coef is for mtp_pref_bwd. */
+int mtp_pref_fwd(const float* nll, const float* ref_nll, const uint8_t* mask, const int64_t* offsets,
+                 int64_t pairs, int64_t n, int32_t kind, double beta, double label_smoothing,
+                 int32_t reduction, float* loss, float* rewards, float* coef, void* workspace,
+                 size_t workspace_bytes, void* stream);
+/* d_nll [n] from d_loss [pairs] (none) or [1] and the forward's coef. */
+int mtp_pref_bwd(const float* d_loss, const float* coef, const uint8_t* mask, const int64_t* offsets,
+                 int64_t pairs, int64_t n, int32_t reduction, float* d_nll, void* stream);
+
+size_t mtp_policy_workspace_bytes(int64_t rows, int64_t n);
+
+/* Clipped policy loss of `rows` sequences: with the ratio u = exp(old_nll - nll), an advantage A per sequence
+ * ([rows]) or token (adv_per_token, [n]) and d = nll - ref_nll,
+ *   loss_t = -min(u A, clip(u, 1 - clip_low, 1 + clip_high) A) + kl_coef (e^d - d - 1).
+ * reduction none: loss [n] (0 where a token counts nowhere); mean: over the tokens that count; sequences: the
+ * mean over the sequences with such tokens of each one's mean. stats: fp32 [2], the mean of e^d - d - 1 (0
+ * without ref_nll) and the share of clipped tokens; weight: fp32 [rows], for mtp_policy_bwd. ref_nll may be NULL
+ * where kl_coef is 0. No token that counts: loss 0. */
+int mtp_policy_fwd(const float* nll, const float* old_nll, const float* ref_nll, const float* advantages,
+                   int32_t adv_per_token, const uint8_t* mask, const int64_t* offsets, int64_t rows, int64_t n,
+                   double clip_low, double clip_high, double kl_coef, int32_t reduction, float* loss,
+                   float* stats, float* weight, void* workspace, size_t workspace_bytes, void* stream);
+/* d_nll [n] from d_loss [n] (none) or [1] and the forward's weight. */
+int mtp_policy_bwd(const float* d_loss, const float* nll, const float* old_nll, const float* ref_nll,
+                   const float* advantages, int32_t adv_per_token, const uint8_t* mask, const int64_t* offsets,
+                   int64_t rows, int64_t n, double clip_low, double clip_high, double kl_coef,
+                   int32_t reduction, const float* weight, float* d_nll, void* stream);
 
 #ifdef __cplusplus
 }

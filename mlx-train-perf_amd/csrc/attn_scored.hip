@@ -1,0 +1,114 @@
+// Attention with capped scores, a bias by distance and key spans: the plan of a call, and the work orders and key
+// ranges that a span backward needs. The kernels are attn_core.hpp's.
+#include "attn_scored.hpp"
+
+namespace mtp {
+
+// Workgroup 0 orders the B npb query blocks of the dQ pass (P queries each), workgroup 1 the B nkb 128-key blocks of
+// the dK/dV pass, most tiles first; the others fill, for each key j, the queries [col_begin, col_end) that see it:
+// as start and end do not decrease along a row, those from the first with end > j to the first with start > j.
+__global__ __launch_bounds__(1024) void attn_span_sched_kernel(const int32_t* __restrict__ start, const int32_t* __restrict__ end,
+                                                              int B, int S, int P, int32_t* __restrict__ q_order,
+                                                              int32_t* __restrict__ kv_order, int32_t* __restrict__ col_begin,
+                                                              int32_t* __restrict__ col_end) {
+  if (blockIdx.x >= 2) {
+    const long i = (long)(blockIdx.x - 2) * 1024 + threadIdx.x;
+    if (i < (long)B * S) {
+      const int b = (int)(i / S), pos = (int)(i % S);
+      col_begin[i] = first_above(end + (long)b * S, 0, S, pos);
+      col_end[i] = first_above(start + (long)b * S, 0, S, pos);
+    }
+    return;
+  }
+  const bool kv = blockIdx.x == 1;
+  const int nblk = kv ? (S + 127) / 128 : (S + P - 1) / P;
+  const int shift = sched_shift(S);
+  auto tiles = [&](int from, int to) { return to > from ? (to - from / kKT * kKT + kKT - 1) / kKT : 0; };
+  auto in_row = [&](int x) { return x < 0 ? 0 : x < S ? x : S; };
+  auto cost = [&](int i) {
+    const int b = i / nblk, blk = i % nblk;
+    const int32_t *sst = start + (long)b * S, *snd = end + (long)b * S;
+    if (kv) {
+      const int k0 = blk * 128, klast = (k0 + 127 < S) ? k0 + 127 : S - 1;
+      return tiles(first_above(snd, 0, S, k0), first_above(sst, 0, S, klast)) >> shift;
+    }
+    const int q0 = blk * P, q1 = (q0 + P < S) ? q0 + P : S;
+    return tiles(in_row(sst[q0]), in_row(snd[q1 - 1])) >> shift;
+  };
+  sched_sort(B * nblk, cost, kv ? kv_order : q_order);
+}
+
+namespace {
+size_t round256(size_t x) { return (x + 255) / 256 * 256; }
+// Heads of a forward or dQ workgroup's group, and its query positions.
+int wg_heads(int hq, int hkv) {
+  const int G = hq / hkv;
+  return (G % 4 == 0) ? 4 : ((G % 2 == 0) ? 2 : 1);
+}
+int wg_rows(int hq, int hkv) { return 32 * (4 / wg_heads(hq, hkv)); }
+int q_grid(const AttnShape& sh) {
+  const int P = wg_rows(sh.hq, sh.hkv);
+  return (sh.s + P - 1) / P * sh.b * (sh.hq / wg_heads(sh.hq, sh.hkv));
+}
+// Splits of the dK/dV pass: the size table of the causal mask, also for spans, whose layout is on the device.
+int scored_nsplit(const AttnShape& sh, bool span) { return attn_dkv_nsplit(sh.b, sh.hq, sh.hkv, sh.s, sh.dh, span ? 1 : sh.causal); }
+// The parts of a workspace from `base` (null: sizes alone), with room for the larger split of the two masks; returns the bytes.
+size_t carve(int b, int hq, int hkv, int s, int dh, char* base, ScoredWorkspace* ws) {
+  const int ns1 = attn_dkv_nsplit(b, hq, hkv, s, dh, 1), ns0 = attn_dkv_nsplit(b, hq, hkv, s, dh, 0);
+  const int ns = ns1 > ns0 ? ns1 : ns0, P = wg_rows(hq, hkv);
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    char* p = base + at;
+    at += round256(bytes);
+    return p;
+  };
+  ws->dvec = reinterpret_cast<float*>(take((size_t)b * hq * s * sizeof(float)));
+  ws->part = reinterpret_cast<float*>(take(ns > 1 ? (size_t)ns * 2 * b * hkv * s * dh * sizeof(float) : 0));
+  ws->q_order = reinterpret_cast<int32_t*>(take((size_t)b * ((s + P - 1) / P) * 4));
+  ws->kv_order = reinterpret_cast<int32_t*>(take((size_t)b * ((s + 127) / 128) * 4));
+  ws->col_begin = reinterpret_cast<int32_t*>(take((size_t)b * s * 4));
+  ws->col_end = reinterpret_cast<int32_t*>(take((size_t)b * s * 4));
+  return at;
+}
+}  // namespace
+
+size_t attn_scored_bwd_workspace(int b, int hq, int hkv, int s, int dh) {
+  ScoredWorkspace ws;
+  return carve(b, hq, hkv, s, dh, nullptr, &ws);
+}
+
+hipError_t launch_attn_scored_fwd(const AttnShape& sh, const AttnScore& sc, const bf16_t* q, const bf16_t* k,
+                                  const bf16_t* v, bf16_t* o, float* lse, hipStream_t st) {
+  switch (sh.dh) {
+    case 64: return scored_fwd<64>(sh, sc, q, k, v, o, lse, q_grid(sh), st);
+    case 96: return scored_fwd<96>(sh, sc, q, k, v, o, lse, q_grid(sh), st);
+    case 128: return scored_fwd<128>(sh, sc, q, k, v, o, lse, q_grid(sh), st);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+hipError_t launch_attn_scored_bwd(const AttnShape& sh, const AttnScore& sc, const bf16_t* q, const bf16_t* k,
+                                  const bf16_t* v, const bf16_t* o, const float* lse, const bf16_t* d_o, bf16_t* dq,
+                                  bf16_t* dk, bf16_t* dv, void* workspace, hipStream_t st) {
+  ScoredWorkspace ws;
+  carve(sh.b, sh.hq, sh.hkv, sh.s, sh.dh, static_cast<char*>(workspace), &ws);
+  ws.nsplit = scored_nsplit(sh, sc.start != nullptr);
+  hipError_t e = hipSuccess;
+  if (sc.start) {
+    const unsigned fill = (unsigned)(((long)sh.b * sh.s + 1023) / 1024);
+    hipLaunchKernelGGL(attn_span_sched_kernel, dim3(2 + fill), dim3(1024), 0, st, sc.start, sc.end, sh.b, sh.s,
+                       wg_rows(sh.hq, sh.hkv), ws.q_order, ws.kv_order, ws.col_begin, ws.col_end);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  switch (sh.dh) {
+    case 64: e = scored_bwd<64>(sh, sc, ws, q, k, v, o, lse, d_o, dq, dk, dv, q_grid(sh), st); break;
+    case 96: e = scored_bwd<96>(sh, sc, ws, q, k, v, o, lse, d_o, dq, dk, dv, q_grid(sh), st); break;
+    case 128: e = scored_bwd<128>(sh, sc, ws, q, k, v, o, lse, d_o, dq, dk, dv, q_grid(sh), st); break;
+    default: return hipErrorInvalidValue;
+  }
+  if (e != hipSuccess || ws.nsplit == 1) return e;
+  return launch_attn_dkv_reduce(ws.part, ws.nsplit, (long)sh.b * sh.hkv * sh.s * sh.dh, dk, dv, st);
+}
+
+}  // namespace mtp

@@ -1,0 +1,82 @@
+// Attention with capped scores, a bias by distance and key spans: the launches of one head_dim over the
+// kernels of attn_core.hpp, instantiated by attn_scored_<head_dim>.hip and called from attn_scored.hip.
+#pragma once
+#include "attn_core.hpp"
+
+namespace mtp {
+
+// A backward call's workspace, in order: D, the fp32 partials of a split dK/dV pass, and for spans the two work
+// orders and the queries [col_begin, col_end) that see each key.
+struct ScoredWorkspace {
+  float* dvec;
+  float* part;
+  int32_t *q_order, *kv_order, *col_begin, *col_end;
+  int nsplit;
+};
+
+template <int DH>
+hipError_t scored_fwd(const AttnShape& sh, const AttnScore& sc, const bf16_t* q, const bf16_t* k, const bf16_t* v,
+                      bf16_t* o, float* lse, int grid, hipStream_t st);
+template <int DH>
+hipError_t scored_bwd(const AttnShape& sh, const AttnScore& sc, const ScoredWorkspace& ws, const bf16_t* q,
+                      const bf16_t* k, const bf16_t* v, const bf16_t* o, const float* lse, const bf16_t* d_o,
+                      bf16_t* dq, bf16_t* dk, bf16_t* dv, int grid, hipStream_t st);
+
+// f(std::integral_constant<int, MOD>) for the call's score form.
+template <class F>
+hipError_t with_mod(const AttnScore& sc, F&& f) {
+  if (sc.cap > 0.f) {
+    if (sc.slopes) return f(std::integral_constant<int, kModBoth>{});
+    return f(std::integral_constant<int, kModCap>{});
+  }
+  if (sc.slopes) return f(std::integral_constant<int, kModSlope>{});
+  return f(std::integral_constant<int, kModNone>{});
+}
+
+#ifdef MTP_SCORED_DH
+template <>
+hipError_t scored_fwd<MTP_SCORED_DH>(const AttnShape& sh, const AttnScore& sc, const bf16_t* q, const bf16_t* k,
+                                     const bf16_t* v, bf16_t* o, float* lse, int grid, hipStream_t st) {
+  constexpr int DH = MTP_SCORED_DH;
+  return with_mod(sc, [&](auto m) {
+    constexpr int MOD = decltype(m)::value;
+    auto launch = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, st, q, k, v, nullptr, nullptr, nullptr, nullptr, sc.end,
+                         sc.start, o, lse, sh.b, sh.hq, sh.hkv, sh.s, sh.scale * kLog2e, sh.scale, sh.causal, nullptr,
+                         sc.cap, sc.slopes);
+      return hipGetLastError();
+    };
+    if (sc.start) return launch(attn_kv_kernel<DH, kMaskSpan, false, MOD>);
+    if constexpr (MOD != kModNone) return launch(attn_kv_kernel<DH, kMaskPlain, false, MOD>);
+    return hipErrorInvalidValue;
+  });
+}
+
+template <>
+hipError_t scored_bwd<MTP_SCORED_DH>(const AttnShape& sh, const AttnScore& sc, const ScoredWorkspace& ws,
+                                     const bf16_t* q, const bf16_t* k, const bf16_t* v, const bf16_t* o,
+                                     const float* lse, const bf16_t* d_o, bf16_t* dq, bf16_t* dk, bf16_t* dv, int grid,
+                                     hipStream_t st) {
+  constexpr int DH = MTP_SCORED_DH;
+  return with_mod(sc, [&](auto m) {
+    constexpr int MOD = decltype(m)::value;
+    auto launch = [&](auto dq_kernel, auto dkv_kernel) {
+      hipLaunchKernelGGL(dq_kernel, dim3(grid), dim3(256), 0, st, q, k, v, d_o, o, lse, ws.dvec, sc.end, sc.start, dq,
+                         nullptr, sh.b, sh.hq, sh.hkv, sh.s, sh.scale * kLog2e, sh.scale, sh.causal, ws.q_order, sc.cap,
+                         sc.slopes);
+      hipError_t e = hipGetLastError();
+      if (e != hipSuccess) return e;
+      hipLaunchKernelGGL(dkv_kernel, dim3((sh.s + 127) / 128 * sh.b * sh.hkv * ws.nsplit), dim3(512), 0, st, q, k, v, d_o,
+                         lse, ws.dvec, ws.col_end, dk, dv, sh.b, sh.hq, sh.hkv, sh.s, sh.scale * kLog2e, sh.scale,
+                         sh.causal, ws.nsplit, ws.part, ws.kv_order, ws.col_begin, sc.cap, sc.slopes);
+      return hipGetLastError();
+    };
+    if (sc.start) return launch(attn_kv_kernel<DH, kMaskSpan, true, MOD>, attn_bwd_dkv_ab_kernel<DH, kMaskSpan, MOD>);
+    if constexpr (MOD != kModNone)
+      return launch(attn_kv_kernel<DH, kMaskPlain, true, MOD>, attn_bwd_dkv_ab_kernel<DH, kMaskPlain, MOD>);
+    return hipErrorInvalidValue;
+  });
+}
+#endif
+
+}  // namespace mtp

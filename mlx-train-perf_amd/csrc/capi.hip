@@ -2,6 +2,7 @@
 // Every function validates shapes, alignment and workspace before any launch and reports a
 // negative MTP_ERR_* code with a thread-local message; nothing here allocates device memory or
 // synchronizes the host.
+#include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
 
@@ -91,6 +92,42 @@ int check_attn(const void* q, const void* k, const void* v, int64_t b, int64_t h
   if (seg_id && !causal) return fail(MTP_ERR_UNSUPPORTED, "segments (packed attention) require causal=1; packing composes on top of the causal triangle");
   if (!q || !k || !v) return fail(MTP_ERR_INPUT, "q, k, v must be non-null");
   if (!aligned16(q) || !aligned16(k) || !aligned16(v)) return fail(MTP_ERR_UNSUPPORTED, "q, k, v must be 16-byte aligned");
+  return MTP_OK;
+}
+
+int check_scored(const void* q, const void* k, const void* v, int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh,
+                 float scale, int32_t causal, float softcap, const float* slopes, const int32_t* span_start,
+                 const int32_t* span_end) {
+  const int rc = check_attn(q, k, v, b, hq, hkv, s, dh, causal, nullptr, nullptr);
+  if (rc) return rc;
+  // Distances exact in fp32, and the byte count of a row's keys within 32 bits.
+  if (s >= (int64_t(1) << 23)) return fail(MTP_ERR_INPUT, "s must be < 2^23 with softcap, slopes or spans (got %lld)", (long long)s);
+  if (!(scale > 0.f) || !(scale < HUGE_VALF)) return fail(MTP_ERR_INPUT, "scale must be positive and finite (got %g)", (double)scale);
+  if (!(softcap >= 0.f) || !(softcap < HUGE_VALF)) return fail(MTP_ERR_INPUT, "softcap must be finite and >= 0, 0 for none (got %g)", (double)softcap);
+  if ((span_start == nullptr) != (span_end == nullptr)) return fail(MTP_ERR_INPUT, "span_start and span_end must be both given or both null");
+  if (span_start && causal) return fail(MTP_ERR_INPUT, "spans are the whole mask: causal must be 0 with them");
+  if (!span_start && !slopes && softcap == 0.f) return fail(MTP_ERR_INPUT, "no softcap, slopes or spans given: use mtp_attn_fwd / mtp_attn_bwd");
+  return MTP_OK;
+}
+
+// Rows and tokens of a preference or policy loss.
+int check_rows(int64_t rows, int64_t n, const int64_t* offsets) {
+  if (rows < 1 || n < 1) return fail(MTP_ERR_INPUT, "the loss needs at least one sequence and one token (got %lld sequences, %lld tokens)", (long long)rows, (long long)n);
+  if (rows > (int64_t(1) << 24) || n > kMaxDim) return fail(MTP_ERR_INPUT, "at most 2^24 sequences and 2^31 - 1 tokens");
+  if (!offsets && n % rows) return fail(MTP_ERR_INPUT, "without offsets the %lld tokens must be %lld rows of one length", (long long)n, (long long)rows);
+  return MTP_OK;
+}
+
+int policy_params(mtp::PolicyLoss* p, const float* ref_nll, int32_t adv_per_token, double clip_low, double clip_high,
+                  double kl_coef, int32_t reduction) {
+  if (!(clip_low >= 0.0 && clip_low <= 1.0)) return fail(MTP_ERR_INPUT, "clip_low must be in [0, 1] (got %g)", clip_low);
+  if (!(clip_high >= 0.0 && clip_high < HUGE_VAL)) return fail(MTP_ERR_INPUT, "clip_high must be finite and >= 0 (got %g)", clip_high);
+  if (!(kl_coef >= 0.0 && kl_coef < HUGE_VAL)) return fail(MTP_ERR_INPUT, "kl_coef must be finite and >= 0 (got %g)", kl_coef);
+  if (kl_coef != 0.0 && !ref_nll) return fail(MTP_ERR_INPUT, "kl_coef needs ref_nll");
+  if (reduction != MTP_REDUCE_NONE && reduction != MTP_REDUCE_MEAN && reduction != MTP_REDUCE_SEQUENCES)
+    return fail(MTP_ERR_INPUT, "unknown reduction %d of a policy loss", (int)reduction);
+  *p = mtp::PolicyLoss{reduction, ref_nll != nullptr, adv_per_token != 0, log1p(-clip_low), log1p(clip_high),
+                       (float)(1.0 - clip_low), (float)(1.0 + clip_high), (float)kl_coef};
   return MTP_OK;
 }
 
@@ -569,6 +606,179 @@ int mtp_attn_bwd_f32(const float* q, const float* k, const float* v, const float
   hipError_t e = mtp::launch_attn32_bwd(sh, q, k, v, o, lse, d_o, seg_start, d_q, d_k, d_v,
                                         static_cast<float*>(workspace), ns, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return fail(MTP_ERR_RUNTIME, "fp32 attention backward launch failed: %s", hipGetErrorString(e));
+  return ok();
+}
+
+// ---------------------------------------------------------------------------------------------
+// Attention with capped scores, a bias by distance and key spans
+// ---------------------------------------------------------------------------------------------
+
+int mtp_attn_scored_fwd(const void* q, const void* k, const void* v, int64_t b, int64_t hq, int64_t hkv, int64_t s,
+                        int64_t dh, float scale, int32_t causal, float softcap, const float* slopes,
+                        const int32_t* span_start, const int32_t* span_end, void* o, float* lse, void* stream) {
+  int rc = check_scored(q, k, v, b, hq, hkv, s, dh, scale, causal, softcap, slopes, span_start, span_end);
+  if (rc) return rc;
+  if (!o || !lse) return fail(MTP_ERR_INPUT, "o and lse must be non-null");
+  if (!aligned16(o)) return fail(MTP_ERR_UNSUPPORTED, "o must be 16-byte aligned");
+  mtp::AttnShape sh{(int)b, (int)hq, (int)hkv, (int)s, (int)dh, scale, (int)causal};
+  mtp::AttnScore sc{softcap, slopes, span_start, span_end};
+  hipError_t e = mtp::launch_attn_scored_fwd(sh, sc, static_cast<const mtp::bf16_t*>(q), static_cast<const mtp::bf16_t*>(k),
+                                             static_cast<const mtp::bf16_t*>(v), static_cast<mtp::bf16_t*>(o), lse,
+                                             static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(MTP_ERR_RUNTIME, "scored attention forward launch failed: %s", hipGetErrorString(e));
+  return ok();
+}
+
+int mtp_attn_scored_fwd_f32(const float* q, const float* k, const float* v, int64_t b, int64_t hq, int64_t hkv, int64_t s,
+                            int64_t dh, float scale, int32_t causal, float softcap, const float* slopes,
+                            const int32_t* span_start, const int32_t* span_end, float* o, float* lse, void* stream) {
+  int rc = check_scored(q, k, v, b, hq, hkv, s, dh, scale, causal, softcap, slopes, span_start, span_end);
+  if (rc) return rc;
+  if (!o || !lse) return fail(MTP_ERR_INPUT, "o and lse must be non-null");
+  if (!aligned16(o)) return fail(MTP_ERR_UNSUPPORTED, "o must be 16-byte aligned");
+  mtp::AttnShape sh{(int)b, (int)hq, (int)hkv, (int)s, (int)dh, scale, (int)causal};
+  mtp::AttnScore sc{softcap, slopes, span_start, span_end};
+  hipError_t e = mtp::launch_attn32_scored_fwd(sh, sc, q, k, v, o, lse, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(MTP_ERR_RUNTIME, "fp32 scored attention forward launch failed: %s", hipGetErrorString(e));
+  return ok();
+}
+
+size_t mtp_attn_scored_bwd_workspace_bytes(int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh) {
+  if (b < 1 || hq < 1 || hkv < 1 || s < 1 || hq % hkv || b * hq * s > kMaxDim) return 0;
+  return mtp::attn_scored_bwd_workspace((int)b, (int)hq, (int)hkv, (int)s, (int)dh);
+}
+
+int mtp_attn_scored_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* d_o,
+                        int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh, float scale, int32_t causal,
+                        float softcap, const float* slopes, const int32_t* span_start, const int32_t* span_end, void* d_q,
+                        void* d_k, void* d_v, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_scored(q, k, v, b, hq, hkv, s, dh, scale, causal, softcap, slopes, span_start, span_end);
+  if (rc) return rc;
+  if (!o || !lse || !d_o || !d_q || !d_k || !d_v) return fail(MTP_ERR_INPUT, "o, lse, d_o, d_q, d_k, d_v must be non-null");
+  if (!aligned16(o) || !aligned16(d_o) || !aligned16(d_q) || !aligned16(d_k) || !aligned16(d_v))
+    return fail(MTP_ERR_UNSUPPORTED, "o, d_o, d_q, d_k, d_v must be 16-byte aligned");
+  const size_t need = mtp_attn_scored_bwd_workspace_bytes(b, hq, hkv, s, dh);
+  if (!workspace || workspace_bytes < need)
+    return fail(MTP_ERR_WORKSPACE, "scored attention backward needs a workspace of %zu bytes (got %zu)", need, workspace ? workspace_bytes : (size_t)0);
+  if (!aligned16(workspace)) return fail(MTP_ERR_UNSUPPORTED, "workspace must be 16-byte aligned");
+  mtp::AttnShape sh{(int)b, (int)hq, (int)hkv, (int)s, (int)dh, scale, (int)causal};
+  mtp::AttnScore sc{softcap, slopes, span_start, span_end};
+  hipError_t e = mtp::launch_attn_scored_bwd(sh, sc, static_cast<const mtp::bf16_t*>(q), static_cast<const mtp::bf16_t*>(k),
+                                             static_cast<const mtp::bf16_t*>(v), static_cast<const mtp::bf16_t*>(o), lse,
+                                             static_cast<const mtp::bf16_t*>(d_o), static_cast<mtp::bf16_t*>(d_q),
+                                             static_cast<mtp::bf16_t*>(d_k), static_cast<mtp::bf16_t*>(d_v), workspace,
+                                             static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(MTP_ERR_RUNTIME, "scored attention backward launch failed: %s", hipGetErrorString(e));
+  return ok();
+}
+
+int mtp_attn_scored_bwd_f32(const float* q, const float* k, const float* v, const float* o, const float* lse,
+                            const float* d_o, int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh, float scale,
+                            int32_t causal, float softcap, const float* slopes, const int32_t* span_start,
+                            const int32_t* span_end, float* d_q, float* d_k, float* d_v, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+  int rc = check_scored(q, k, v, b, hq, hkv, s, dh, scale, causal, softcap, slopes, span_start, span_end);
+  if (rc) return rc;
+  if (!o || !lse || !d_o || !d_q || !d_k || !d_v) return fail(MTP_ERR_INPUT, "o, lse, d_o, d_q, d_k, d_v must be non-null");
+  if (!aligned16(o) || !aligned16(d_o) || !aligned16(d_q) || !aligned16(d_k) || !aligned16(d_v))
+    return fail(MTP_ERR_UNSUPPORTED, "o, d_o, d_q, d_k, d_v must be 16-byte aligned");
+  // D is all it needs; a workspace without room for the split's partials runs the dK/dV pass unsplit.
+  const size_t need = mtp::attn32_bwd_workspace((int)b, (int)hq, (int)hkv, (int)s, (int)dh, 1);
+  if (!workspace || workspace_bytes < need)
+    return fail(MTP_ERR_WORKSPACE, "fp32 scored attention backward needs a workspace of %zu bytes (got %zu)", need, workspace ? workspace_bytes : (size_t)0);
+  mtp::AttnShape sh{(int)b, (int)hq, (int)hkv, (int)s, (int)dh, scale, (int)causal};
+  mtp::AttnScore sc{softcap, slopes, span_start, span_end};
+  const bool split = workspace_bytes >= mtp_attn_bwd_f32_workspace_bytes(b, hq, hkv, s, dh);
+  const int ns = split ? mtp::attn32_dkv_splits(sh.b, sh.hq, sh.hkv, sh.s, sh.dh) : 1;
+  hipError_t e = mtp::launch_attn32_scored_bwd(sh, sc, q, k, v, o, lse, d_o, d_q, d_k, d_v, static_cast<float*>(workspace), ns,
+                                               static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(MTP_ERR_RUNTIME, "fp32 scored attention backward launch failed: %s", hipGetErrorString(e));
+  return ok();
+}
+
+// ---------------------------------------------------------------------------------------------
+// Preference and policy losses
+// ---------------------------------------------------------------------------------------------
+
+size_t mtp_pref_workspace_bytes(int64_t pairs, int64_t n) {
+  return pairs < 1 || pairs > (int64_t(1) << 23) || n < 1 || n > kMaxDim ? 0 : mtp::pref_workspace((long)pairs, (long)n);
+}
+
+int mtp_pref_fwd(const float* nll, const float* ref_nll, const uint8_t* mask, const int64_t* offsets, int64_t pairs, int64_t n,
+                 int32_t kind, double beta, double label_smoothing, int32_t reduction, float* loss, float* rewards,
+                 float* coef, void* workspace, size_t workspace_bytes, void* stream) {
+  if (pairs < 1) return fail(MTP_ERR_INPUT, "pairs must be >= 1 (got %lld)", (long long)pairs);
+  int rc = check_rows(pairs > (int64_t(1) << 24) ? pairs : 2 * pairs, n, offsets);
+  if (rc) return rc;
+  if (!nll || !ref_nll || !loss || !rewards || !coef) return fail(MTP_ERR_INPUT, "nll, ref_nll, loss, rewards and coef must be non-null");
+  if (kind < MTP_PREF_SIGMOID || kind > MTP_PREF_IPO) return fail(MTP_ERR_INPUT, "unknown kind %d of a preference loss", (int)kind);
+  if (!(beta > 0.0 && beta < HUGE_VAL)) return fail(MTP_ERR_INPUT, "beta must be positive and finite (got %g)", beta);
+  if (!(label_smoothing >= 0.0 && label_smoothing < 0.5)) return fail(MTP_ERR_INPUT, "label_smoothing must be in [0, 0.5) (got %g)", label_smoothing);
+  if (label_smoothing != 0.0 && kind != MTP_PREF_SIGMOID) return fail(MTP_ERR_INPUT, "label_smoothing belongs to the sigmoid loss");
+  if (reduction != MTP_REDUCE_NONE && reduction != MTP_REDUCE_MEAN && reduction != MTP_REDUCE_SUM)
+    return fail(MTP_ERR_INPUT, "unknown reduction %d of a preference loss", (int)reduction);
+  const size_t need = mtp_pref_workspace_bytes(pairs, n);
+  if (!workspace || workspace_bytes < need)
+    return fail(MTP_ERR_WORKSPACE, "the preference loss needs a workspace of %zu bytes (got %zu)", need, workspace ? workspace_bytes : (size_t)0);
+  if (!aligned16(workspace)) return fail(MTP_ERR_UNSUPPORTED, "workspace must be 16-byte aligned");
+  hipError_t e = mtp::launch_pref_fwd(nll, ref_nll, mask, offsets, (long)pairs, (long)n,
+                                      mtp::PrefLoss{kind, reduction, beta, label_smoothing}, loss, rewards, coef, workspace,
+                                      static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(MTP_ERR_RUNTIME, "preference loss launch failed: %s", hipGetErrorString(e));
+  return ok();
+}
+
+int mtp_pref_bwd(const float* d_loss, const float* coef, const uint8_t* mask, const int64_t* offsets, int64_t pairs, int64_t n,
+                 int32_t reduction, float* d_nll, void* stream) {
+  if (pairs < 1) return fail(MTP_ERR_INPUT, "pairs must be >= 1 (got %lld)", (long long)pairs);
+  int rc = check_rows(pairs > (int64_t(1) << 24) ? pairs : 2 * pairs, n, offsets);
+  if (rc) return rc;
+  if (!d_loss || !coef || !d_nll) return fail(MTP_ERR_INPUT, "d_loss, coef and d_nll must be non-null");
+  hipError_t e = mtp::launch_pref_bwd(d_loss, coef, mask, offsets, (long)pairs, (long)n, reduction == MTP_REDUCE_NONE, d_nll,
+                                      static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(MTP_ERR_RUNTIME, "preference loss backward launch failed: %s", hipGetErrorString(e));
+  return ok();
+}
+
+size_t mtp_policy_workspace_bytes(int64_t rows, int64_t n) {
+  return rows < 1 || rows > (int64_t(1) << 24) || n < 1 || n > kMaxDim ? 0 : mtp::policy_workspace((long)rows, (long)n);
+}
+
+int mtp_policy_fwd(const float* nll, const float* old_nll, const float* ref_nll, const float* advantages,
+                   int32_t adv_per_token, const uint8_t* mask, const int64_t* offsets, int64_t rows, int64_t n,
+                   double clip_low, double clip_high, double kl_coef, int32_t reduction, float* loss, float* stats,
+                   float* weight, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_rows(rows, n, offsets);
+  if (rc) return rc;
+  if (!nll || !old_nll || !advantages || !loss || !stats || !weight)
+    return fail(MTP_ERR_INPUT, "nll, old_nll, advantages, loss, stats and weight must be non-null");
+  mtp::PolicyLoss p;
+  rc = policy_params(&p, ref_nll, adv_per_token, clip_low, clip_high, kl_coef, reduction);
+  if (rc) return rc;
+  const size_t need = mtp_policy_workspace_bytes(rows, n);
+  if (!workspace || workspace_bytes < need)
+    return fail(MTP_ERR_WORKSPACE, "the policy loss needs a workspace of %zu bytes (got %zu)", need, workspace ? workspace_bytes : (size_t)0);
+  if (!aligned16(workspace)) return fail(MTP_ERR_UNSUPPORTED, "workspace must be 16-byte aligned");
+  hipError_t e = mtp::launch_policy_fwd(nll, old_nll, ref_nll, advantages, mask, offsets, (long)rows, (long)n, p, loss, stats,
+                                        weight, workspace, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(MTP_ERR_RUNTIME, "policy loss launch failed: %s", hipGetErrorString(e));
+  return ok();
+}
+
+int mtp_policy_bwd(const float* d_loss, const float* nll, const float* old_nll, const float* ref_nll, const float* advantages,
+                   int32_t adv_per_token, const uint8_t* mask, const int64_t* offsets, int64_t rows, int64_t n,
+                   double clip_low, double clip_high, double kl_coef, int32_t reduction, const float* weight, float* d_nll,
+                   void* stream) {
+  int rc = check_rows(rows, n, offsets);
+  if (rc) return rc;
+  if (!d_loss || !nll || !old_nll || !advantages || !weight || !d_nll)
+    return fail(MTP_ERR_INPUT, "d_loss, nll, old_nll, advantages, weight and d_nll must be non-null");
+  mtp::PolicyLoss p;
+  rc = policy_params(&p, ref_nll, adv_per_token, clip_low, clip_high, kl_coef, reduction);
+  if (rc) return rc;
+  hipError_t e = mtp::launch_policy_bwd(d_loss, nll, old_nll, ref_nll, advantages, mask, offsets, (long)rows, (long)n, p, weight,
+                                        d_nll, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(MTP_ERR_RUNTIME, "policy loss backward launch failed: %s", hipGetErrorString(e));
   return ok();
 }
 

@@ -28,6 +28,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kNegInf = -__builtin_huge_valf();
 
+// Masks and score forms of the attention kernels (attn_core.hpp).
+enum { kMaskPlain = 0, kMaskPacked = 1, kMaskSpan = 2 };
+enum { kModNone = 0, kModCap = 1, kModSlope = 2, kModBoth = 3 };
+
 __device__ __forceinline__ f32x16 mfma32(const bf16x8& a, const bf16x8& b, const f32x16& c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }

@@ -85,6 +85,30 @@ hipError_t launch_attn_bwd(const AttnShape& sh, const bf16_t* q, const bf16_t* k
                            const int32_t* seg_start, bf16_t* dq, bf16_t* dk, bf16_t* dv, float* dvec,
                            hipStream_t stream);
 
+// Sum of the fp32 partials of a split dK/dV pass; plane: elements of dK.
+hipError_t launch_attn_dkv_reduce(const float* part, int ns, long plane, bf16_t* dk, bf16_t* dv, hipStream_t stream);
+
+// Scores and masks beyond the plain ones (attn_scored.hip): cap > 0: cap tanh(x / cap) in the place of a
+// scaled score x; slopes [hq]: minus slope |i - j|; start and end [b][s]: key j visible to query i iff
+// start[i] <= j < end[i] (both given or neither; AttnShape.causal is then 0).
+struct AttnScore {
+  float cap;
+  const float* slopes;
+  const int32_t* start;
+  const int32_t* end;
+};
+size_t attn_scored_bwd_workspace(int b, int hq, int hkv, int s, int dh);
+hipError_t launch_attn_scored_fwd(const AttnShape& sh, const AttnScore& sc, const bf16_t* q, const bf16_t* k,
+                                  const bf16_t* v, bf16_t* o, float* lse, hipStream_t stream);
+hipError_t launch_attn_scored_bwd(const AttnShape& sh, const AttnScore& sc, const bf16_t* q, const bf16_t* k,
+                                  const bf16_t* v, const bf16_t* o, const float* lse, const bf16_t* d_o, bf16_t* dq,
+                                  bf16_t* dk, bf16_t* dv, void* workspace, hipStream_t stream);
+hipError_t launch_attn32_scored_fwd(const AttnShape& sh, const AttnScore& sc, const float* q, const float* k,
+                                    const float* v, float* o, float* lse, hipStream_t stream);
+hipError_t launch_attn32_scored_bwd(const AttnShape& sh, const AttnScore& sc, const float* q, const float* k,
+                                    const float* v, const float* o, const float* lse, const float* d_o, float* dq,
+                                    float* dk, float* dv, float* dvec, int nsplit, hipStream_t stream);
+
 // fp32 inputs (f32_kernels.hip): fp32 MFMA products, fp32 outputs and gradients.
 struct LceHead32 {
   int q4;                 // 0: dense fp32 [V][D]; 1: 4-bit affine, group size 64, fp32 scales/biases
@@ -103,6 +127,7 @@ hipError_t launch_lce32_bwd(const LceHead32& h, const float* H, const int64_t* t
                             float* dW, float* Gbuf, hipStream_t stream);
 hipError_t launch_attn32_fwd(const AttnShape& sh, const float* q, const float* k, const float* v,
                              const int32_t* seg_start, float* o, float* lse, hipStream_t stream);
+hipError_t launch_attn32_dkv_reduce(const float* part, int ns, long plane, float* dk, float* dv, hipStream_t stream);
 // Splits of the fp32 dK/dV pass (1: none), and the backward's workspace with them: D, then the partials.
 int attn32_dkv_splits(int b, int hq, int hkv, int s, int dh);
 size_t attn32_bwd_workspace(int b, int hq, int hkv, int s, int dh, int nsplit);
@@ -110,5 +135,34 @@ size_t attn32_bwd_workspace(int b, int hq, int hkv, int s, int dh, int nsplit);
 hipError_t launch_attn32_bwd(const AttnShape& sh, const float* q, const float* k, const float* v, const float* o,
                              const float* lse, const float* d_o, const int32_t* seg_start, float* dq, float* dk,
                              float* dv, float* dvec, int nsplit, hipStream_t stream);
+
+// Preference and policy losses (preference_kernels.hip).
+enum { kPrefSigmoid = 0, kPrefHinge = 1, kPrefIpo = 2 };
+enum { kReduceNone = 0, kReduceMean = 1, kReduceSum = 2, kReduceSequences = 3 };
+struct PrefLoss {
+  int kind, reduction;
+  double beta, smoothing;
+};
+struct PolicyLoss {
+  int reduction;      // none: per token; mean over the tokens; sequences: mean of each sequence's mean
+  int has_ref, adv_per_token;
+  double log_low, log_high;   // log(1 - clip_low), log(1 + clip_high)
+  float edge_low, edge_high;  // 1 - clip_low, 1 + clip_high
+  float kl_coef;
+};
+size_t pref_workspace(long pairs, long n);
+size_t policy_workspace(long rows, long n);
+// reduction none: loss [pairs], else [1]; reward, coef [2 pairs]. offsets [2 pairs + 1], or null: rows of n / (2 pairs).
+hipError_t launch_pref_fwd(const float* nll, const float* ref, const uint8_t* mask, const int64_t* offsets, long pairs, long n,
+                           const PrefLoss& p, float* loss, float* reward, float* coef, void* ws, hipStream_t stream);
+hipError_t launch_pref_bwd(const float* d_loss, const float* coef, const uint8_t* mask, const int64_t* offsets, long pairs,
+                           long n, int per_pair, float* d_nll, hipStream_t stream);
+// reduction none: loss [n], else [1]; stats [2], weight [rows].
+hipError_t launch_policy_fwd(const float* nll, const float* old, const float* ref, const float* adv, const uint8_t* mask,
+                             const int64_t* offsets, long rows, long n, const PolicyLoss& p, float* loss, float* stats,
+                             float* weight, void* ws, hipStream_t stream);
+hipError_t launch_policy_bwd(const float* d_loss, const float* nll, const float* old, const float* ref, const float* adv,
+                             const uint8_t* mask, const int64_t* offsets, long rows, long n, const PolicyLoss& p,
+                             const float* weight, float* d_nll, hipStream_t stream);
 
 }  // namespace mtp

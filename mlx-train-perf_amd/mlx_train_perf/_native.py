@@ -50,6 +50,7 @@ _c_void_p = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int32
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 _size = ctypes.c_size_t
 
 # name -> (restype, argtypes); the single source of truth for the Python side of the ABI.
@@ -101,6 +102,25 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "mtp_attn_bwd_f32": (ctypes.c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                                         _i64, _i64, _i64, _i64, _i64, _f32, _i32, _c_void_p, _c_void_p,
                                         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _size, _c_void_p]),
+    # capped scores, a bias by distance, key spans
+    **{name: (ctypes.c_int, [_c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _i64, _f32, _i32, _f32, _c_void_p,
+                             _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p])
+       for name in ("mtp_attn_scored_fwd", "mtp_attn_scored_fwd_f32")},
+    "mtp_attn_scored_bwd_workspace_bytes": (_size, [_i64, _i64, _i64, _i64, _i64]),
+    **{name: (ctypes.c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _i64,
+                             _f32, _i32, _f32, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
+                             _size, _c_void_p])
+       for name in ("mtp_attn_scored_bwd", "mtp_attn_scored_bwd_f32")},
+    # preference and policy losses
+    "mtp_pref_workspace_bytes": (_size, [_i64, _i64]),
+    "mtp_pref_fwd": (ctypes.c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i32, _f64, _f64, _i32, _c_void_p,
+                                    _c_void_p, _c_void_p, _c_void_p, _size, _c_void_p]),
+    "mtp_pref_bwd": (ctypes.c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i32, _c_void_p, _c_void_p]),
+    "mtp_policy_workspace_bytes": (_size, [_i64, _i64]),
+    "mtp_policy_fwd": (ctypes.c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _c_void_p, _c_void_p, _i64, _i64,
+                                      _f64, _f64, _f64, _i32, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _size, _c_void_p]),
+    "mtp_policy_bwd": (ctypes.c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _c_void_p, _c_void_p,
+                                      _i64, _i64, _f64, _f64, _f64, _i32, _c_void_p, _c_void_p, _c_void_p]),
 }
 
 _lock = threading.Lock()

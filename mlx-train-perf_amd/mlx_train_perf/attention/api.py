@@ -8,17 +8,23 @@ with fp32 outputs and gradients; head_dim in {64, 96, 128}; causal with optional
 or non-causal -- an extension: the reference kernel refuses causal=False, api.py:109-113). `impl="reference"`: the materialized oracle with the hand-written
 FlashAttention backward over full tensors -- an explicit opt-in, O(N^2) memory, small N only.
 No silent fallback: unsupported configs raise the reference's typed errors.
+
+Beyond the reference: `softcap` (scores capped by a tanh), `slopes` (a bias by distance) and `spans` (a range of
+keys for each query), on both impls and both dtypes, forward and backward; the kernel impl serves them by the
+mtp_attn_scored_* entry points.
 """
 from __future__ import annotations
 
+import math
 import weakref
 from typing import Literal
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from mlx_train_perf import _compat, _native
-from mlx_train_perf.attention.reference import flash_attention_reference, kv_head_for
-from mlx_train_perf.attention.segments import PackedMask, layout_violation, segment_allowed
+from mlx_train_perf.attention.reference import flash_attention_reference, hide, kv_head_for, scores_of
+from mlx_train_perf.attention.segments import PackedMask, SpanMask, layout_violation, packed_as_spans, span_violation
 from mlx_train_perf.errors import AttentionInputError, UnsupportedAttentionError
 
 _KERNEL_DTYPES = (torch.bfloat16, torch.float32)   # the reference kernel's T (api.py:41-43)
@@ -81,10 +87,41 @@ def _validate_segments(q: torch.Tensor, segments: PackedMask, *, check_layout: b
         _CHECKED_LAYOUTS[id(sid)] = (weakref.ref(sid), weakref.ref(sst), (sid._version, sst._version))
 
 
+def _validate_score(q: torch.Tensor, softcap: float | None, slopes: torch.Tensor | None, spans: SpanMask | None,
+                    segments: PackedMask | None, *, check_spans: bool) -> None:
+    b, hq, n, _ = q.shape
+    if softcap is not None and not (math.isfinite(softcap) and softcap > 0):
+        raise AttentionInputError(f"softcap must be a positive finite number, or None for none; got {softcap!r}")
+    if slopes is not None:
+        if tuple(slopes.shape) != (hq,) or not slopes.dtype.is_floating_point:
+            raise AttentionInputError(f"slopes must be {hq} floating-point values, one per query head; got {slopes.dtype} "
+                                      f"of shape {tuple(slopes.shape)}")
+        if slopes.device != q.device:
+            raise AttentionInputError(f"slopes are on {slopes.device}, q on {q.device}")
+        if slopes.requires_grad and torch.is_grad_enabled():
+            raise AttentionInputError("slopes get no gradient: detach them")
+    if spans is not None:
+        if segments is not None:
+            raise AttentionInputError("give segments or spans, not both: spans are the whole mask")
+        for name, t in (("start", spans.start), ("end", spans.end)):
+            if tuple(t.shape) != (b, n):
+                raise AttentionInputError(f"spans.{name} must have shape (B, N)=({b}, {n}); got {tuple(t.shape)}")
+            if t.dtype.is_floating_point or t.dtype == torch.bool or t.dtype.is_complex:
+                raise AttentionInputError(f"spans.{name} must be an integer tensor; got {t.dtype}")
+        if check_spans:
+            problem = span_violation(spans)
+            if problem is not None:
+                raise AttentionInputError(f"spans violate their contract: {problem}")
+
+
 def resolve_attention_impl(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, impl: str, causal: bool = True,
-                           segments: PackedMask | None = None, validate_segments: bool = False) -> str:
+                           segments: PackedMask | None = None, validate_segments: bool = False,
+                           softcap: float | None = None, slopes: torch.Tensor | None = None,
+                           spans: SpanMask | None = None) -> str:
     """api.py:75-123: "reference" is always allowed; "auto"/"kernel" run the kernel-support gate."""
     _validate_shapes(q, k, v)
+    if softcap is not None or slopes is not None or spans is not None:
+        _validate_score(q, softcap, slopes, spans, segments, check_spans=validate_segments)
     if segments is not None:
         _validate_segments(q, segments, check_layout=validate_segments)
         if not causal:
@@ -121,7 +158,8 @@ def _kv_gather(x: torch.Tensor, *, hq: int, hkv: int) -> torch.Tensor:
     return x.index_select(1, idx)
 
 
-def _flash_attention_backward(q, k, v, o, lse, d_o, *, scale, causal, segments=None):
+def _flash_attention_backward(q, k, v, o, lse, d_o, *, scale, causal, segments=None, softcap=None, slopes=None,
+                              spans=None):
     """Hand-written FlashAttention backward over full tensors, fp32 (api.py:140-194)."""
     b, hq, n, dd = q.shape
     hkv = k.shape[1]
@@ -132,13 +170,13 @@ def _flash_attention_backward(q, k, v, o, lse, d_o, *, scale, causal, segments=N
     d = _bwd_D(d_o, o)
     do32 = d_o.to(torch.float32)
     s = (q32 @ k_g.transpose(-1, -2).contiguous()) * scale
-    if segments is not None:
-        s = s.masked_fill(~segment_allowed(segments.seg_id), float("-inf"))
-    if causal:
-        s = s.masked_fill(torch.ones(n, n, dtype=torch.bool, device=q.device).triu(1), float("-inf"))
+    s, bend = scores_of(s, softcap=softcap, slopes=slopes)
+    s = hide(s, causal=causal, segments=segments, spans=spans)
     p = torch.exp(s - lse.to(torch.float32)[..., None])
     d_p = do32 @ v_g.transpose(-1, -2).contiguous()
     d_s = p * (d_p - d[..., None])
+    if bend is not None:
+        d_s = d_s * bend
     d_q = scale * (d_s @ k_g)
     d_v = (p.transpose(-1, -2).contiguous() @ do32).reshape(b, hkv, group, n, dd).sum(2)
     d_k = (scale * (d_s.transpose(-1, -2).contiguous() @ q32)).reshape(b, hkv, group, n, dd).sum(2)
@@ -147,9 +185,10 @@ def _flash_attention_backward(q, k, v, o, lse, d_o, *, scale, causal, segments=N
 
 class _ReferenceAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, seg_id, seg_start, scale, causal):
+    def forward(ctx, q, k, v, seg_id, seg_start, scale, causal, score=None):
         segments = None if seg_id is None else PackedMask(seg_id=seg_id, seg_start=seg_start)
-        o, lse = flash_attention_reference(q, k, v, scale=scale, causal=causal, segments=segments)
+        ctx.score = score or {}   # softcap, slopes, spans
+        o, lse = flash_attention_reference(q, k, v, scale=scale, causal=causal, segments=segments, **ctx.score)
         ctx.save_for_backward(q, k, v, o, lse)
         ctx.segments = segments
         ctx.scale, ctx.causal = scale, causal
@@ -161,8 +200,8 @@ class _ReferenceAttention(torch.autograd.Function):
         VJP_CALLS["flash_attention"] = VJP_CALLS.get("flash_attention", 0) + 1
         q, k, v, o, lse = ctx.saved_tensors
         dq, dk, dv = _flash_attention_backward(q, k, v, o, lse, d_o, scale=ctx.scale, causal=ctx.causal,
-                                               segments=ctx.segments)
-        return dq, dk, dv, None, None, None, None
+                                               segments=ctx.segments, **ctx.score)
+        return dq, dk, dv, None, None, None, None, None
 
 
 def _seg_args(q, seg_id, seg_start):
@@ -233,9 +272,83 @@ class _KernelAttention(torch.autograd.Function):
         return dq, dk, dv, None, None, None, None
 
 
+def scored_forward(q, k, v, slopes, start, end, *, scale: float, causal: bool, softcap: float | None):
+    """(O, L) from mtp_attn_scored_fwd (_f32 for fp32 inputs); contiguous tensors on the GPU."""
+    lib = _native.load()
+    b, hq, n, dh = q.shape
+    o = torch.empty_like(q)
+    lse = torch.empty((b, hq, n), dtype=torch.float32, device=q.device)
+    fwd = lib.mtp_attn_scored_fwd_f32 if q.dtype == torch.float32 else lib.mtp_attn_scored_fwd
+    with _native.on_device(q):
+        rc = fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), b, hq, k.shape[1], n, dh, scale, int(causal), softcap or 0.0,
+                 _native.ptr(slopes), _native.ptr(start), _native.ptr(end), o.data_ptr(), lse.data_ptr(),
+                 _native.stream_of(q))
+    _native.check(rc, domain="attention")
+    return o, lse
+
+
+def scored_backward(q, k, v, o, lse, d_o, slopes, start, end, *, scale: float, causal: bool, softcap: float | None):
+    """(dQ, dK, dV) from mtp_attn_scored_bwd (_f32 for fp32 inputs)."""
+    lib = _native.load()
+    b, hq, n, dh = q.shape
+    hkv = k.shape[1]
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    f32 = q.dtype == torch.float32
+    ws_bytes = (lib.mtp_attn_bwd_f32_workspace_bytes if f32 else lib.mtp_attn_scored_bwd_workspace_bytes)(b, hq, hkv, n, dh)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+    bwd = lib.mtp_attn_scored_bwd_f32 if f32 else lib.mtp_attn_scored_bwd
+    with _native.on_device(q):
+        rc = bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), d_o.data_ptr(), b, hq, hkv, n, dh,
+                 scale, int(causal), softcap or 0.0, _native.ptr(slopes), _native.ptr(start), _native.ptr(end),
+                 dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), ws_bytes, _native.stream_of(q))
+    _native.check(rc, domain="attention")
+    return dq, dk, dv
+
+
+class _ScoredAttention(torch.autograd.Function):
+    """Attention with softcap, slopes or spans; the residuals are _KernelAttention's."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, slopes, start, end, scale, causal, softcap):
+        o, lse = scored_forward(q, k, v, slopes, start, end, scale=scale, causal=causal, softcap=softcap)
+        ctx.save_for_backward(q, k, v, o, lse, slopes, start, end)
+        ctx.scale, ctx.causal, ctx.softcap = scale, causal, softcap
+        ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
+        return o, lse
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, d_o, _d_l):
+        VJP_CALLS["flash_attention"] = VJP_CALLS.get("flash_attention", 0) + 1
+        VJP_CALLS["flash_attention_kernel_bwd"] = VJP_CALLS.get("flash_attention_kernel_bwd", 0) + 1
+        q, k, v, o, lse, slopes, start, end = ctx.saved_tensors
+        d_o = torch.zeros_like(o) if d_o is None else d_o.contiguous()
+        dq, dk, dv = scored_backward(q, k, v, o, lse, d_o, slopes, start, end, scale=ctx.scale, causal=ctx.causal,
+                                     softcap=ctx.softcap)
+        return dq, dk, dv, None, None, None, None, None, None
+
+
+def _scored_attention(q, k, v, *, scale, causal, segments, softcap, slopes, spans):
+    """The kernel impl of a call with softcap, slopes or spans. Packed segments go as spans."""
+    if segments is not None:
+        spans = packed_as_spans(segments)
+    start = end = None
+    if spans is not None:
+        causal = False
+        start, end = (t.to(device=q.device, dtype=torch.int32).contiguous() for t in (spans.start, spans.end))
+    if slopes is not None:
+        slopes = slopes.detach().to(torch.float32).contiguous()
+    args = (q.contiguous(), k.contiguous(), v.contiguous(), slopes, start, end, float(scale), bool(causal),
+            None if softcap is None else float(softcap))
+    return _ScoredAttention.apply(*args)[0]
+
+
 def flash_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: float, causal: bool = True,
                     impl: Literal["auto", "kernel", "reference"] = "auto",
-                    segments: PackedMask | None = None, validate_segments: bool = True) -> torch.Tensor:
+                    segments: PackedMask | None = None, validate_segments: bool = True,
+                    softcap: float | None = None, slopes: torch.Tensor | None = None,
+                    spans: SpanMask | None = None) -> torch.Tensor:
     """softmax(scale * Q K^T + mask) V with GQA (api.py:281-439). Only O is returned; L stays internal.
 
     `segments` (requires causal=True) switches on packed block-diagonal-causal attention; the
@@ -243,9 +356,19 @@ def flash_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale:
     its own layout. `validate_segments` checks the layout contract of `PackedMask` (seg_id from 0 in
     steps of 0 or 1, seg_start the first position of each segment) and raises AttentionInputError
     on a violation; the check costs one host sync per distinct mask (a model's layers share it).
-    Pass False on a trusted path, like the loss's `validate_targets`."""
+    Pass False on a trusted path, like the loss's `validate_targets`.
+
+    `softcap`: scores become softcap * tanh(score / softcap). `slopes`: (Hq,) values, slopes[h] * |i - j| is taken
+    from the score of query i and key j (after the cap); they get no gradient. `spans`: a `SpanMask`, the keys that
+    each query sees; it is the whole mask, so `causal` has no say beside it and `segments` may not be given (cap and
+    slopes go with either). A query that sees nothing gets zeros and no gradient. `validate_segments` checks the
+    contract of `spans` too, at one host sync a call."""
     resolved = resolve_attention_impl(q, k, v, impl=impl, causal=causal, segments=segments,
-                                      validate_segments=validate_segments)
+                                      validate_segments=validate_segments, softcap=softcap, slopes=slopes, spans=spans)
+    scored = softcap is not None or slopes is not None or spans is not None
+    if scored and resolved == "kernel":
+        return _scored_attention(q, k, v, scale=scale, causal=causal, segments=segments, softcap=softcap, slopes=slopes,
+                                 spans=spans)
     seg_id, seg_start = (None, None) if segments is None else _seg_args(q, segments.seg_id, segments.seg_start)
     if resolved == "kernel":
         args = (q.contiguous(), k.contiguous(), v.contiguous(), seg_id, seg_start, float(scale), bool(causal))
@@ -254,5 +377,8 @@ def flash_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale:
             return nodes.attention(*args)
         o, _ = _KernelAttention.apply(*args)
         return o
-    o, _ = _ReferenceAttention.apply(q, k, v, seg_id, seg_start, float(scale), causal)
+    if spans is not None:
+        spans = SpanMask(start=spans.start.to(q.device), end=spans.end.to(q.device))
+    score = {"softcap": softcap, "slopes": slopes, "spans": spans} if scored else None
+    o, _ = _ReferenceAttention.apply(q, k, v, seg_id, seg_start, float(scale), causal, score)
     return o
