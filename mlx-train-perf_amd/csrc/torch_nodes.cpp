@@ -1,5 +1,6 @@
-// The autograd nodes of flash_attention and linear_cross_entropy on plain tensors: the forward and backward of
-// attention/api.py's _KernelAttention and core/loss.py's _KernelLCE, planned and launched from C++.
+// The autograd nodes of flash_attention, linear_cross_entropy, preference_loss and policy_loss on plain tensors: the
+// forward and backward of attention/api.py's _KernelAttention and _ScoredAttention, core/loss.py's _KernelLCE and
+// core/preference.py's _Preference and _Policy, planned and launched from C++.
 // Autograd runs a backward on a thread of its own; a Python node there holds the interpreter lock for the
 // whole of it and pulls the interpreter's state to that thread's core, and the next forward pulls it back.
 // A node here takes the lock for a moment: once to count the backward, and in a loss also for the workspace
@@ -41,6 +42,17 @@ struct Entries {
   decltype(&mtp_lce_bwd_f32_chunk) lce_chunk32 = nullptr;
   decltype(&mtp_lce_mean) lce_mean = nullptr;
   decltype(&mtp_lce_mean_bwd) lce_mean_bwd = nullptr;
+  decltype(&mtp_attn_scored_fwd) scored_fwd = nullptr;
+  decltype(&mtp_attn_scored_bwd) scored_bwd = nullptr;
+  decltype(&mtp_attn_scored_bwd_workspace_bytes) scored_ws = nullptr;
+  decltype(&mtp_attn_scored_fwd_f32) scored_fwd32 = nullptr;
+  decltype(&mtp_attn_scored_bwd_f32) scored_bwd32 = nullptr;
+  decltype(&mtp_pref_fwd) pref_fwd = nullptr;
+  decltype(&mtp_pref_bwd) pref_bwd = nullptr;
+  decltype(&mtp_pref_workspace_bytes) pref_ws = nullptr;
+  decltype(&mtp_policy_fwd) policy_fwd = nullptr;
+  decltype(&mtp_policy_bwd) policy_bwd = nullptr;
+  decltype(&mtp_policy_workspace_bytes) policy_ws = nullptr;
 };
 Entries g_api;
 // Python: the typed error of a return code (_native.check), the call counters of the attention and the
@@ -49,6 +61,7 @@ Entries g_api;
 PyObject* g_check = nullptr;
 PyObject* g_attn_calls = nullptr;
 PyObject* g_lce_calls = nullptr;
+PyObject* g_pref_calls = nullptr;
 PyObject* g_transposed_head = nullptr;
 PyObject* g_budget = nullptr;
 PyObject* g_env = nullptr;
@@ -141,6 +154,172 @@ struct KernelAttention : torch::autograd::Function<KernelAttention> {
       check(g_api.bwd(ptr(q), ptr(k), ptr(v), ptr(o), ptr<float>(lse), ptr(d_o), b, hq, hkv, s, dh, scale, causal,
                       ints(seg_id), ints(seg_start), ptr(dq), ptr(dk), ptr(dv), ptr(ws), bytes, stream_of(q)));
     return {dq, dk, dv, at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+// Scores and masks beyond the plain ones: not inputs of the node either.
+struct Score {
+  double softcap;  // 0: none
+  at::Tensor slopes, start, end;
+};
+const float* floats(const at::Tensor& t) { return t.defined() ? t.const_data_ptr<float>() : nullptr; }
+
+struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k,
+                            const at::Tensor& v, const Score& score, double scale, bool causal) {
+    const c10::DeviceGuard device(q.device());
+    const int64_t b = q.size(0), hq = q.size(1), s = q.size(2), dh = q.size(3), hkv = k.size(1);
+    const at::Tensor o = at::empty_like(q), lse = at::empty({b, hq, s}, q.options().dtype(at::kFloat));
+    const float cap = (float)score.softcap;
+    if (q.scalar_type() == at::kFloat)
+      check(g_api.scored_fwd32(ptr<float>(q), ptr<float>(k), ptr<float>(v), b, hq, hkv, s, dh, (float)scale, causal, cap,
+                               floats(score.slopes), ints(score.start), ints(score.end), ptr<float>(o), ptr<float>(lse),
+                               stream_of(q)));
+    else
+      check(g_api.scored_fwd(ptr(q), ptr(k), ptr(v), b, hq, hkv, s, dh, (float)scale, causal, cap, floats(score.slopes),
+                             ints(score.start), ints(score.end), ptr(o), ptr<float>(lse), stream_of(q)));
+    ctx->save_for_backward({q, k, v, o, lse, score.slopes, score.start, score.end});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["softcap"] = score.softcap;
+    ctx->set_materialize_grads(false);
+    return o;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    count_backward(g_attn_calls, {"flash_attention", "flash_attention_kernel_bwd"});
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &o = saved[3], &lse = saved[4];
+    const at::Tensor &slopes = saved[5], &start = saved[6], &end = saved[7];
+    const float scale = (float)ctx->saved_data["scale"].toDouble(), cap = (float)ctx->saved_data["softcap"].toDouble();
+    const bool causal = ctx->saved_data["causal"].toBool();
+    const c10::DeviceGuard device(q.device());
+    const at::Tensor d_o = grads[0].defined() ? grads[0].contiguous() : at::zeros_like(o);
+    const int64_t b = q.size(0), hq = q.size(1), s = q.size(2), dh = q.size(3), hkv = k.size(1);
+    const bool f32 = q.scalar_type() == at::kFloat;
+    const at::Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v);
+    const size_t bytes = (f32 ? g_api.ws32 : g_api.scored_ws)(b, hq, hkv, s, dh);
+    const at::Tensor ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+    if (f32)
+      check(g_api.scored_bwd32(ptr<float>(q), ptr<float>(k), ptr<float>(v), ptr<float>(o), ptr<float>(lse), ptr<float>(d_o), b,
+                               hq, hkv, s, dh, scale, causal, cap, floats(slopes), ints(start), ints(end), ptr<float>(dq),
+                               ptr<float>(dk), ptr<float>(dv), ptr(ws), bytes, stream_of(q)));
+    else
+      check(g_api.scored_bwd(ptr(q), ptr(k), ptr(v), ptr(o), ptr<float>(lse), ptr(d_o), b, hq, hkv, s, dh, scale, causal, cap,
+                             floats(slopes), ints(start), ints(end), ptr(dq), ptr(dk), ptr(dv), ptr(ws), bytes, stream_of(q)));
+    return {dq, dk, dv, at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+// Preference and policy losses: what a call has beside nll, none of it an input of the node.
+struct Rows {
+  at::Tensor mask, offsets;  // uint8, int64; may be missing
+  int64_t rows;
+};
+const uint8_t* bytes_of(const at::Tensor& t) { return t.defined() ? t.const_data_ptr<uint8_t>() : nullptr; }
+const int64_t* longs(const at::Tensor& t) { return t.defined() ? t.const_data_ptr<int64_t>() : nullptr; }
+struct PreferenceCall {
+  at::Tensor ref;
+  Rows rows;
+  int64_t kind, reduction;
+  double beta, smoothing;
+};
+
+struct Preference : torch::autograd::Function<Preference> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& nll,
+                                                const PreferenceCall& c) {
+    const c10::DeviceGuard device(nll.device());
+    const int64_t n = nll.numel(), pairs = c.rows.rows / 2;
+    const auto opt = nll.options();
+    const at::Tensor loss = c.reduction == MTP_REDUCE_NONE ? at::empty({pairs}, opt) : at::empty({}, opt);
+    const at::Tensor rewards = at::empty({2, pairs}, opt);
+    // The factors that the backward reads, then (16-byte aligned) the workspace.
+    const size_t bytes = g_api.pref_ws(pairs, n);
+    const int64_t at = (2 * pairs + 3) / 4 * 4;
+    const at::Tensor coef = at::empty({at + (int64_t)(bytes + 3) / 4}, opt);
+    check(g_api.pref_fwd(ptr<float>(nll), ptr<float>(c.ref), bytes_of(c.rows.mask), longs(c.rows.offsets), pairs, n, (int)c.kind,
+                         c.beta, c.smoothing, (int)c.reduction, ptr<float>(loss), ptr<float>(rewards), ptr<float>(coef),
+                         ptr<float>(coef) + at, bytes, stream_of(nll)),
+          "loss");
+    ctx->save_for_backward({coef, c.rows.mask, c.rows.offsets});
+    ctx->saved_data["shape"] = nll.sizes().vec();
+    ctx->saved_data["pairs"] = pairs;
+    ctx->saved_data["reduction"] = c.reduction;
+    const at::Tensor chosen = rewards.select(0, 0), rejected = rewards.select(0, 1);
+    ctx->mark_non_differentiable({chosen, rejected});
+    ctx->set_materialize_grads(false);
+    return {loss, chosen, rejected};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    count_backward(g_pref_calls, {"preference"});
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &coef = saved[0], &mask = saved[1], &offsets = saved[2];
+    const c10::DeviceGuard device(coef.device());
+    const auto shape = ctx->saved_data["shape"].toIntVector();
+    if (!grads[0].defined()) return {at::zeros(shape, coef.options()), at::Tensor()};
+    const at::Tensor d_loss = grads[0].to(at::kFloat).contiguous(), d_nll = at::empty(shape, coef.options());
+    check(g_api.pref_bwd(ptr<float>(d_loss), ptr<float>(coef), bytes_of(mask), longs(offsets), ctx->saved_data["pairs"].toInt(),
+                         d_nll.numel(), (int)ctx->saved_data["reduction"].toInt(), ptr<float>(d_nll), stream_of(coef)),
+          "loss");
+    return {d_nll, at::Tensor()};
+  }
+};
+
+struct PolicyCall {
+  at::Tensor old, ref, adv;  // ref may be missing
+  Rows rows;
+  int64_t reduction;
+  double clip_low, clip_high, kl_coef;
+};
+
+struct Policy : torch::autograd::Function<Policy> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& nll,
+                                                const PolicyCall& c) {
+    const c10::DeviceGuard device(nll.device());
+    const int64_t n = nll.numel(), rows = c.rows.rows;
+    const auto opt = nll.options();
+    const at::Tensor loss = c.reduction == MTP_REDUCE_NONE ? at::empty(nll.sizes(), opt) : at::empty({}, opt);
+    const at::Tensor stats = at::empty({2}, opt);
+    const size_t bytes = g_api.policy_ws(rows, n);
+    const int64_t at = (rows + 3) / 4 * 4;
+    const at::Tensor weight = at::empty({at + (int64_t)(bytes + 3) / 4}, opt);
+    check(g_api.policy_fwd(ptr<float>(nll), ptr<float>(c.old), floats(c.ref), ptr<float>(c.adv), c.adv.sizes() == nll.sizes(),
+                           bytes_of(c.rows.mask), longs(c.rows.offsets), rows, n, c.clip_low, c.clip_high, c.kl_coef,
+                           (int)c.reduction, ptr<float>(loss), ptr<float>(stats), ptr<float>(weight), ptr<float>(weight) + at,
+                           bytes, stream_of(nll)),
+          "loss");
+    ctx->save_for_backward({nll, c.old, c.ref, c.adv, c.rows.mask, c.rows.offsets, weight});
+    auto& sd = ctx->saved_data;
+    sd["rows"] = rows;
+    sd["reduction"] = c.reduction;
+    sd["clip_low"] = c.clip_low;
+    sd["clip_high"] = c.clip_high;
+    sd["kl_coef"] = c.kl_coef;
+    const at::Tensor kl = stats.select(0, 0), share = stats.select(0, 1);
+    ctx->mark_non_differentiable({kl, share});
+    ctx->set_materialize_grads(false);
+    return {loss, kl, share};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    count_backward(g_pref_calls, {"policy"});
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &nll = saved[0], &old = saved[1], &ref = saved[2], &adv = saved[3], &mask = saved[4], &offsets = saved[5];
+    const at::Tensor& weight = saved[6];
+    const c10::DeviceGuard device(nll.device());
+    if (!grads[0].defined()) return {at::zeros_like(nll), at::Tensor()};
+    const at::Tensor d_loss = grads[0].to(at::kFloat).contiguous(), d_nll = at::empty_like(nll);
+    auto& sd = ctx->saved_data;
+    check(g_api.policy_bwd(ptr<float>(d_loss), ptr<float>(nll), ptr<float>(old), floats(ref), ptr<float>(adv),
+                           adv.sizes() == nll.sizes(), bytes_of(mask), longs(offsets), sd["rows"].toInt(), nll.numel(),
+                           sd["clip_low"].toDouble(), sd["clip_high"].toDouble(), sd["kl_coef"].toDouble(),
+                           (int)sd["reduction"].toInt(), ptr<float>(weight), ptr<float>(d_nll), stream_of(nll)),
+          "loss");
+    return {d_nll, at::Tensor()};
   }
 };
 
@@ -291,7 +470,7 @@ struct KernelLoss : torch::autograd::Function<KernelLoss> {
 
 // The node's result for a Python caller: typed errors as they are.
 template <class F>
-at::Tensor apply_node(F&& f) {
+auto apply_node(F&& f) {
   try {
     py::gil_scoped_release no_gil;
     return f();
@@ -321,6 +500,32 @@ at::Tensor attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor&
   });
 }
 
+at::Tensor scored_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const std::optional<at::Tensor>& slopes,
+                            const std::optional<at::Tensor>& start, const std::optional<at::Tensor>& end, double scale, bool causal,
+                            double softcap) {
+  const at::Tensor none;
+  const Score score{softcap, slopes.value_or(none), start.value_or(none), end.value_or(none)};
+  return apply_node([&] { return ScoredAttention::apply(q, k, v, score, scale, causal); });
+}
+
+std::vector<at::Tensor> preference(const at::Tensor& nll, const at::Tensor& ref, const std::optional<at::Tensor>& mask,
+                                   const std::optional<at::Tensor>& offsets, int64_t pairs, int64_t kind, double beta,
+                                   double smoothing, int64_t reduction) {
+  const at::Tensor none;
+  const PreferenceCall call{ref, Rows{mask.value_or(none), offsets.value_or(none), 2 * pairs}, kind, reduction, beta, smoothing};
+  return apply_node([&] { return Preference::apply(nll, call); });
+}
+
+std::vector<at::Tensor> policy(const at::Tensor& nll, const at::Tensor& old, const std::optional<at::Tensor>& ref,
+                               const at::Tensor& adv, const std::optional<at::Tensor>& mask,
+                               const std::optional<at::Tensor>& offsets, int64_t rows, double clip_low, double clip_high,
+                               double kl_coef, int64_t reduction) {
+  const at::Tensor none;
+  const PolicyCall call{old, ref.value_or(none), adv, Rows{mask.value_or(none), offsets.value_or(none), rows}, reduction,
+                        clip_low, clip_high, kl_coef};
+  return apply_node([&] { return Policy::apply(nll, call); });
+}
+
 void bind(const py::dict& entries, py::object check_fn) {
   auto set = [&](auto& f, const char* name) {
     f = reinterpret_cast<std::remove_reference_t<decltype(f)>>(entries[name].cast<uintptr_t>());
@@ -345,9 +550,21 @@ void bind(const py::dict& entries, py::object check_fn) {
   set(g_api.lce_chunk32, "mtp_lce_bwd_f32_chunk");
   set(g_api.lce_mean, "mtp_lce_mean");
   set(g_api.lce_mean_bwd, "mtp_lce_mean_bwd");
+  set(g_api.scored_fwd, "mtp_attn_scored_fwd");
+  set(g_api.scored_bwd, "mtp_attn_scored_bwd");
+  set(g_api.scored_ws, "mtp_attn_scored_bwd_workspace_bytes");
+  set(g_api.scored_fwd32, "mtp_attn_scored_fwd_f32");
+  set(g_api.scored_bwd32, "mtp_attn_scored_bwd_f32");
+  set(g_api.pref_fwd, "mtp_pref_fwd");
+  set(g_api.pref_bwd, "mtp_pref_bwd");
+  set(g_api.pref_ws, "mtp_pref_workspace_bytes");
+  set(g_api.policy_fwd, "mtp_policy_fwd");
+  set(g_api.policy_bwd, "mtp_policy_bwd");
+  set(g_api.policy_ws, "mtp_policy_workspace_bytes");
   g_check = check_fn.release().ptr();
 }
 void bind_attention(py::object calls) { g_attn_calls = calls.release().ptr(); }
+void bind_preference(py::object calls) { g_pref_calls = calls.release().ptr(); }
 void bind_loss(py::object calls, py::object transposed_head, py::object budget, py::object env) {
   g_lce_calls = calls.release().ptr();
   g_transposed_head = transposed_head.release().ptr();
@@ -363,4 +580,8 @@ PYBIND11_MODULE(_mtp_torch, m) {
   m.def("bind_loss", &bind_loss);
   m.def("loss", &loss);
   m.def("attention", &attention);
+  m.def("bind_preference", &bind_preference);
+  m.def("scored_attention", &scored_attention);
+  m.def("preference", &preference);
+  m.def("policy", &policy);
 }

@@ -272,7 +272,7 @@ class _KernelAttention(torch.autograd.Function):
         return dq, dk, dv, None, None, None, None
 
 
-def scored_forward(q, k, v, slopes, start, end, *, scale: float, causal: bool, softcap: float | None):
+def scored_forward(q, k, v, slopes, start, end, *, scale: float, causal: bool, softcap: float):
     """(O, L) from mtp_attn_scored_fwd (_f32 for fp32 inputs); contiguous tensors on the GPU."""
     lib = _native.load()
     b, hq, n, dh = q.shape
@@ -280,14 +280,14 @@ def scored_forward(q, k, v, slopes, start, end, *, scale: float, causal: bool, s
     lse = torch.empty((b, hq, n), dtype=torch.float32, device=q.device)
     fwd = lib.mtp_attn_scored_fwd_f32 if q.dtype == torch.float32 else lib.mtp_attn_scored_fwd
     with _native.on_device(q):
-        rc = fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), b, hq, k.shape[1], n, dh, scale, int(causal), softcap or 0.0,
+        rc = fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), b, hq, k.shape[1], n, dh, scale, int(causal), softcap,
                  _native.ptr(slopes), _native.ptr(start), _native.ptr(end), o.data_ptr(), lse.data_ptr(),
                  _native.stream_of(q))
     _native.check(rc, domain="attention")
     return o, lse
 
 
-def scored_backward(q, k, v, o, lse, d_o, slopes, start, end, *, scale: float, causal: bool, softcap: float | None):
+def scored_backward(q, k, v, o, lse, d_o, slopes, start, end, *, scale: float, causal: bool, softcap: float):
     """(dQ, dK, dV) from mtp_attn_scored_bwd (_f32 for fp32 inputs)."""
     lib = _native.load()
     b, hq, n, dh = q.shape
@@ -299,14 +299,14 @@ def scored_backward(q, k, v, o, lse, d_o, slopes, start, end, *, scale: float, c
     bwd = lib.mtp_attn_scored_bwd_f32 if f32 else lib.mtp_attn_scored_bwd
     with _native.on_device(q):
         rc = bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), d_o.data_ptr(), b, hq, hkv, n, dh,
-                 scale, int(causal), softcap or 0.0, _native.ptr(slopes), _native.ptr(start), _native.ptr(end),
+                 scale, int(causal), softcap, _native.ptr(slopes), _native.ptr(start), _native.ptr(end),
                  dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), ws_bytes, _native.stream_of(q))
     _native.check(rc, domain="attention")
     return dq, dk, dv
 
 
 class _ScoredAttention(torch.autograd.Function):
-    """Attention with softcap, slopes or spans; the residuals are _KernelAttention's."""
+    """Attention with softcap (0: none), slopes or spans: the general path, as _KernelAttention, whose residuals it has."""
 
     @staticmethod
     def forward(ctx, q, k, v, slopes, start, end, scale, causal, softcap):
@@ -339,8 +339,10 @@ def _scored_attention(q, k, v, *, scale, causal, segments, softcap, slopes, span
         start, end = (t.to(device=q.device, dtype=torch.int32).contiguous() for t in (spans.start, spans.end))
     if slopes is not None:
         slopes = slopes.detach().to(torch.float32).contiguous()
-    args = (q.contiguous(), k.contiguous(), v.contiguous(), slopes, start, end, float(scale), bool(causal),
-            None if softcap is None else float(softcap))
+    args = (q.contiguous(), k.contiguous(), v.contiguous(), slopes, start, end, float(scale), bool(causal), float(softcap or 0.0))
+    nodes = _native.nodes() if _native.plain(q, k, v) else None
+    if nodes is not None:
+        return nodes.scored_attention(*args)
     return _ScoredAttention.apply(*args)[0]
 
 

@@ -111,7 +111,8 @@ def _count(name: str) -> None:
 
 
 class _Preference(torch.autograd.Function):
-    """(loss, rewards) from mtp_pref_fwd; the backward spreads each sequence's factor over its tokens."""
+    """(loss, rewards) from mtp_pref_fwd; the backward spreads each sequence's factor over its tokens. The general path:
+    plain tensors take the C++ node of the same calls."""
 
     @staticmethod
     def forward(ctx, nll, ref_nll, mask, offsets, pairs, kind, beta, smoothing, reduction):
@@ -151,7 +152,8 @@ class _Preference(torch.autograd.Function):
 
 
 class _Policy(torch.autograd.Function):
-    """(loss, stats) from mtp_policy_fwd; the backward forms each token's gradient again from the inputs."""
+    """(loss, stats) from mtp_policy_fwd; the backward forms each token's gradient again from the inputs. The general
+    path, as _Preference."""
 
     @staticmethod
     def forward(ctx, nll, old_nll, ref_nll, adv, mask, offsets, rows, clip_low, clip_high, kl_coef, reduction):
@@ -305,8 +307,12 @@ def preference_loss(nll: torch.Tensor, ref_nll: torch.Tensor, *, offsets: torch.
     if _resolve(nll, {"ref_nll": ref_nll, "offsets": offsets, "mask": mask}, impl) == "reference":
         return _reference_preference(nll, ref_nll.detach(), offsets, mask, rows, kind, beta, label_smoothing, reduction)
     pairs = rows // 2
-    loss, rewards = _Preference.apply(nll.contiguous(), ref_nll.detach().contiguous(), _plain_mask(mask), _plain_offsets(offsets),
-                                      pairs, _KINDS[kind], beta, label_smoothing, _REDUCTIONS[reduction])
+    args = (nll.contiguous(), ref_nll.detach().contiguous(), _plain_mask(mask), _plain_offsets(offsets), pairs, _KINDS[kind], beta,
+            label_smoothing, _REDUCTIONS[reduction])
+    nodes = _native.nodes() if _native.plain(nll, ref_nll) else None
+    if nodes is not None:
+        return PreferenceLoss(*nodes.preference(*args))
+    loss, rewards = _Preference.apply(*args)
     return PreferenceLoss(loss, rewards[:pairs], rewards[pairs:])
 
 
@@ -339,6 +345,9 @@ def policy_loss(nll: torch.Tensor, old_nll: torch.Tensor, advantages: torch.Tens
         return _reference_policy(nll, old_nll.detach(), ref, advantages.detach(), offsets, mask, rows, clip_low, clip_high,
                                  kl_coef, reduction)
     old, ref, adv = (None if t is None else t.detach().contiguous() for t in (old_nll, ref_nll, advantages))
-    loss, stats = _Policy.apply(nll.contiguous(), old, ref, adv, _plain_mask(mask), _plain_offsets(offsets), rows, clip_low,
-                                clip_high, kl_coef, _REDUCTIONS[reduction])
+    args = (old, ref, adv, _plain_mask(mask), _plain_offsets(offsets), rows, clip_low, clip_high, kl_coef, _REDUCTIONS[reduction])
+    nodes = _native.nodes() if _native.plain(nll, *(t for t in (old_nll, ref_nll, advantages) if t is not None)) else None
+    if nodes is not None:
+        return PolicyLoss(*nodes.policy(nll.contiguous(), *args))
+    loss, stats = _Policy.apply(nll.contiguous(), *args)
     return PolicyLoss(loss, stats[0], stats[1])
