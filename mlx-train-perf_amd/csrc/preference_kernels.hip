@@ -15,49 +15,152 @@
 //   d loss_t / d nll_t = [not clipped] e^s A + kl_coef (e^d - 1)
 // clipped: A > 0 and e^s > 1 + high, or A < 0 and e^s < 1 - low.
 //
-// Both are bound by their launches until some hundred thousand tokens, then by reading 8 to 17 bytes a token. Sums are in
-// 64 bits: a log ratio is the small difference of long sums. Every sequence is cut into `chunks` equal parts, a workgroup
-// each, whose partial sums one workgroup joins in order, so a result does not depend on scheduling.
+// Both read 8 to 17 bytes a token and are bound by launches and latency up to some hundred thousand tokens. So each wave
+// takes 512 consecutive tokens, whatever sequences they belong to (sequences dealt to workgroups made the longest of a
+// ragged batch the whole time), and has all its loads in flight at once: eight tokens a lane. For every sequence r that
+// wave w touches it leaves one part at slot w + r; as w and r never decrease along the tokens no two parts share a slot,
+// so nwaves + rows slots hold them. A join, one workgroup, adds each sequence's parts in order. Sums are in 64 bits, since
+// a log ratio is the small difference of long sums, and no result depends on scheduling. Up to kOneTokens tokens one
+// workgroup does both in one launch.
 #include "mtp_common.hpp"
 #include "mtp_launch.hpp"
 
 namespace mtp {
 
 namespace {
-constexpr int kPrefThreads = 256;
-constexpr int kJoinThreads = 1024;
+constexpr int kLaneTokens = 8, kWaveTokens = 64 * kLaneTokens;
+constexpr int kThreads = 256;        // a workgroup of the large grid
+constexpr int kJoinThreads = 1024;   // the join's, and that of the one-launch form
+constexpr int kOneTokens = 16384;
 
-struct Span {
-  long begin, end;
-};
-__device__ __forceinline__ Span sequence_of(const int64_t* offsets, long rows, long n, long r) {
-  if (!offsets) {
-    const long t = n / rows;
-    return Span{r * t, (r + 1) * t};
+struct Seqs {
+  const int64_t* offsets;
+  int rows, n, t;  // t: tokens of a row, without offsets
+  __device__ __forceinline__ int clamp(long x) const { return x < 0 ? 0 : x < n ? (int)x : n; }
+  __device__ __forceinline__ int begin(int r) const { return offsets ? clamp(offsets[r]) : r * t; }
+  __device__ __forceinline__ int end(int r) const { return offsets ? clamp(offsets[r + 1]) : (r + 1) * t; }
+  // The first sequence that ends past token s (rows if none), the same in every lane: a search by 64 probes at a time.
+  __device__ __forceinline__ int first(int s) const {
+    if (!offsets) return s / t;
+    int lo = 0, hi = rows;
+    while (lo < hi) {
+      const int step = (hi - lo + 63) / 64, probe = lo + ((int)(threadIdx.x & 63) + 1) * step - 1;
+      const uint64_t past = __builtin_amdgcn_ballot_w64(probe >= hi || offsets[probe + 1] > s);
+      if (past == 0) return hi;
+      lo += __builtin_ctzll(past) * step;
+      hi = lo + step - 1 < hi ? lo + step - 1 : hi;
+    }
+    return lo;
   }
-  long a = offsets[r], b = offsets[r + 1];
-  a = a < 0 ? 0 : a < n ? a : n;
-  b = b < a ? a : b < n ? b : n;
-  return Span{a, b};
+};
+
+// A lane's tokens of wave-tile w are w kWaveTokens + token(k) for k = 0 .. 7: two runs of four.
+__device__ __forceinline__ int token(int k) { return 256 * (k >> 2) + 4 * (int)(threadIdx.x & 63) + (k & 3); }
+
+// The lane's eight values of src (tokens from n on: not read). VEC: src is 16-byte aligned.
+template <bool VEC>
+__device__ __forceinline__ void load8(const float* __restrict__ src, int s, int n, float (&x)[kLaneTokens]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int t = s + token(4 * h);
+    if (VEC && t + 3 < n) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(src + t);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[4 * h + j] = v[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[4 * h + j] = t + j < n ? src[t + j] : 0.f;
+    }
+  }
 }
-__device__ __forceinline__ Span part_of(const Span& s, int c, int chunks) {
-  const long len = s.end - s.begin;
-  return Span{s.begin + len * c / chunks, s.begin + len * (c + 1) / chunks};
+template <bool VEC>
+__device__ __forceinline__ void store8(float* __restrict__ dst, int s, int n, const float (&x)[kLaneTokens]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int t = s + token(4 * h);
+    if (VEC && t + 3 < n) {
+      *reinterpret_cast<f32x4*>(dst + t) = f32x4{x[4 * h], x[4 * h + 1], x[4 * h + 2], x[4 * h + 3]};
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (t + j < n) dst[t + j] = x[4 * h + j];
+    }
+  }
+}
+// Bit k: token k counts (VEC: mask is 4-byte aligned).
+template <bool VEC>
+__device__ __forceinline__ uint32_t keep8(const uint8_t* __restrict__ mask, int s, int n) {
+  if (!mask) return 0xff;
+  uint32_t keep = 0;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int t = s + token(4 * h);
+    if (VEC && t + 3 < n) {
+      const uint32_t m = *reinterpret_cast<const uint32_t*>(mask + t);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) keep |= ((m >> (8 * j)) & 0xffu) ? 1u << (4 * h + j) : 0u;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) keep |= (t + j < n && mask[t + j]) ? 1u << (4 * h + j) : 0u;
+    }
+  }
+  return keep;
+}
+// f(r, part) for every sequence r of tile w, in order: bit k of `part` tells whether token k is one of it.
+template <class F>
+__device__ __forceinline__ void each_sequence(const Seqs& q, int w, F&& f) {
+  const int s = w * kWaveTokens, e = s + kWaveTokens < q.n ? s + kWaveTokens : q.n;
+  for (int r = q.first(s); r < q.rows; ++r) {
+    const int a = q.begin(r), b = q.end(r);
+    if (a >= e) break;
+    uint32_t part = 0;
+#pragma unroll
+    for (int k = 0; k < kLaneTokens; ++k) {
+      const int t = s + token(k);
+      part |= (t >= a && t < b) ? 1u << k : 0u;  // b <= n
+    }
+    f(r, part);
+  }
 }
 
-// Sum over the workgroup's threads, in every thread: within a wave by halves, then the waves in order.
-template <int THREADS, class T>
-__device__ __forceinline__ T block_sum(T x) {
-  __shared__ T part[THREADS / 64];
+template <class T>
+__device__ __forceinline__ T wave_add(T x) {
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o, 64);
+  return x;
+}
+// Sum over the join's threads, in every thread: within a wave by halves, then the 16 waves' by halves.
+template <class T>
+__device__ __forceinline__ T block_add(T x) {
+  constexpr int kWaves = kJoinThreads / 64;
+  __shared__ T part[kWaves];
+  x = wave_add(x);
   __syncthreads();  // the last use of part is over
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
   __syncthreads();
-  T s = part[0];
+  x = part[threadIdx.x % kWaves];
 #pragma unroll
-  for (int w = 1; w < THREADS / 64; ++w) s += part[w];
-  return s;
+  for (int o = kWaves / 2; o >= 1; o >>= 1) x += __shfl_xor(x, o, 64);
+  return x;
+}
+
+// The join gives every item (a pair, a sequence) a group of lanes, as many as there are threads for (a power of two, 64 at
+// most), and a lane of the group every group-th part.
+__device__ __forceinline__ int join_group(int items) {
+  int g = 64;
+  while (g > 1 && g * items > kJoinThreads) g >>= 1;
+  return g;
+}
+template <class T>
+__device__ __forceinline__ T group_add(T x, int group) {
+  for (int o = group >> 1; o >= 1; o >>= 1) x += __shfl_xor(x, o, 64);
+  return x;
+}
+// Tiles [first, last] with a part of sequence r; none for an empty one.
+__device__ __forceinline__ void tiles_of(const Seqs& q, int r, int& first, int& last) {
+  const int a = q.begin(r), b = q.end(r);
+  first = a / kWaveTokens;
+  last = b > a ? (b - 1) / kWaveTokens : first - 1;
 }
 
 struct PrefPart {
@@ -65,49 +168,59 @@ struct PrefPart {
   long count;
 };
 
-__global__ __launch_bounds__(kPrefThreads) void pref_sums_kernel(const float* __restrict__ nll, const float* __restrict__ ref,
-                                                                 const uint8_t* __restrict__ mask,
-                                                                 const int64_t* __restrict__ offsets, long rows, long n,
-                                                                 int chunks, PrefPart* __restrict__ part) {
-  const long r = blockIdx.x / chunks;
-  const Span s = part_of(sequence_of(offsets, rows, n, r), blockIdx.x % chunks, chunks);
-  double gap = 0;
-  int count = 0;
-  for (long t = s.begin + threadIdx.x; t < s.end; t += kPrefThreads) {
-    if (mask && !mask[t]) continue;
-    gap += (double)ref[t] - (double)nll[t];
-    ++count;
-  }
-  gap = block_sum<kPrefThreads>(gap);
-  count = block_sum<kPrefThreads>(count);
-  if (threadIdx.x == 0) part[blockIdx.x] = PrefPart{gap, count};
+template <bool VEC>
+__device__ __forceinline__ void pref_tile(const float* __restrict__ nll, const float* __restrict__ ref,
+                                          const uint8_t* __restrict__ mask, const Seqs& q, int w, PrefPart* __restrict__ part) {
+  const int s = w * kWaveTokens;
+  float x[kLaneTokens], y[kLaneTokens];
+  load8<VEC>(nll, s, q.n, x);
+  load8<VEC>(ref, s, q.n, y);
+  const uint32_t keep = keep8<VEC>(mask, s, q.n);
+  each_sequence(q, w, [&](int r, uint32_t mine) {
+    mine &= keep;
+    double gap = 0;
+#pragma unroll
+    for (int k = 0; k < kLaneTokens; ++k)
+      if ((mine >> k) & 1) gap += (double)y[k] - (double)x[k];
+    gap = wave_add(gap);
+    const int count = wave_add(__builtin_popcount(mine));
+    if ((threadIdx.x & 63) == 0) part[w + r] = PrefPart{gap, count};
+  });
 }
 
-__device__ __forceinline__ double softplus(double x) { return fmax(x, 0.0) + log1p(exp(-fabs(x))); }
+// softplus and the logistic of a difference that is already exact to 2^-53: fp32 results need no more than fp32 functions.
+__device__ __forceinline__ float softplus(float x) { return fmaxf(x, 0.f) + log1pf(expf(-fabsf(x))); }
 
-// Joins the parts of each sequence; loss [pairs] (reduction none) or [1], reward and coef [2 pairs].
-__global__ __launch_bounds__(kJoinThreads) void pref_join_kernel(const PrefPart* __restrict__ part, long pairs, int chunks,
-                                                                 PrefLoss p, float* __restrict__ loss,
-                                                                 float* __restrict__ reward, float* __restrict__ coef) {
-  auto sum = [&](long r, double& weight) {
+__device__ __forceinline__ void pref_join(const PrefPart* part, const Seqs& q, const PrefLoss& p, float* __restrict__ loss,
+                                          float* __restrict__ reward, float* __restrict__ coef) {
+  const int pairs = q.rows / 2, group = join_group(pairs), lane = threadIdx.x % group;
+  auto sum = [&](int r, double& weight) {
+    int first, last;
+    tiles_of(q, r, first, last);
     double gap = 0;
     long count = 0;
-    for (int c = 0; c < chunks; ++c) {
-      gap += part[r * chunks + c].gap;
-      count += part[r * chunks + c].count;
+    for (int w = first + lane; w <= last; w += group) {
+      gap += part[w + r].gap;
+      count += part[w + r].count;
     }
+    gap = group_add(gap, group);
+    count = group_add(count, group);
     weight = p.kind == kPrefIpo ? 1.0 / (double)(count > 1 ? count : 1) : 1.0;
     return gap * weight * p.beta;
   };
   const double share = p.reduction == kReduceMean ? 1.0 / (double)pairs : 1.0;
   double total = 0;
-  for (long i = threadIdx.x; i < pairs; i += kJoinThreads) {
+  for (int i0 = 0; i0 < pairs; i0 += kJoinThreads / group) {  // whole groups stay together for group_add
+    const int i = i0 + (int)threadIdx.x / group;
+    const bool live = i < pairs;
     double wc, wr;
-    const double chosen = sum(i, wc), rejected = sum(pairs + i, wr), d = chosen - rejected;
+    const double chosen = sum(live ? i : 0, wc), rejected = sum(pairs + (live ? i : 0), wr), d = chosen - rejected;
+    if (!live || lane != 0) continue;
     double l, slope;
     if (p.kind == kPrefSigmoid) {
-      l = (1.0 - p.smoothing) * softplus(-d) + p.smoothing * softplus(d);
-      slope = p.smoothing - 1.0 / (1.0 + exp(d));
+      const float x = (float)d;
+      l = (1.0 - p.smoothing) * softplus(-x) + p.smoothing * softplus(x);
+      slope = p.smoothing - 1.f / (1.f + expf(x));
     } else if (p.kind == kPrefHinge) {
       l = d < 1.0 ? 1.0 - d : d >= 1.0 ? 0.0 : d;  // NaN stays
       slope = d < 1.0 ? -1.0 : d >= 1.0 ? 0.0 : d;
@@ -124,32 +237,50 @@ __global__ __launch_bounds__(kJoinThreads) void pref_join_kernel(const PrefPart*
     total += l;
   }
   if (p.reduction == kReduceNone) return;
-  total = block_sum<kJoinThreads>(total);
+  total = block_add(total);
   if (threadIdx.x == 0) loss[0] = (float)(total * share);
 }
 
-// The gradient of tokens of no sequence: before the first offset (row 0's workgroups) and behind the last.
-__device__ __forceinline__ void zero_outside(const int64_t* offsets, long rows, long n, long r, const Span& s, int c, float* out) {
-  if (!offsets || c != 0) return;
-  if (r == 0)
-    for (long t = threadIdx.x; t < s.begin; t += kPrefThreads) out[t] = 0.f;
-  if (r == rows - 1)
-    for (long t = s.end + threadIdx.x; t < n; t += kPrefThreads) out[t] = 0.f;
+// Tiles [first, ntiles) by steps of `step` of a wave, or (ONE) all tiles by one workgroup and the join behind them.
+template <bool VEC, bool ONE>
+__global__ __launch_bounds__(ONE ? kJoinThreads : kThreads) void pref_fwd_kernel(
+    const float* __restrict__ nll, const float* __restrict__ ref, const uint8_t* __restrict__ mask, Seqs q, PrefLoss p,
+    PrefPart* part, float* __restrict__ loss, float* __restrict__ reward, float* __restrict__ coef) {
+  constexpr int kWaves = (ONE ? kJoinThreads : kThreads) / 64;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ntiles = (q.n + kWaveTokens - 1) / kWaveTokens;
+  for (int w = ONE ? wave : (int)blockIdx.x * kWaves + wave; w < ntiles; w += ONE ? kWaves : ntiles)
+    pref_tile<VEC>(nll, ref, mask, q, w, part);
+  if constexpr (ONE) {
+    __syncthreads();
+    pref_join(part, q, p, loss, reward, coef);
+  }
+}
+__global__ __launch_bounds__(kJoinThreads) void pref_join_kernel(const PrefPart* __restrict__ part, Seqs q, PrefLoss p,
+                                                                 float* __restrict__ loss, float* __restrict__ reward,
+                                                                 float* __restrict__ coef) {
+  pref_join(part, q, p, loss, reward, coef);
 }
 
-__global__ __launch_bounds__(kPrefThreads) void pref_bwd_kernel(const float* __restrict__ d_loss, const float* __restrict__ coef,
-                                                                const uint8_t* __restrict__ mask,
-                                                                const int64_t* __restrict__ offsets, long pairs, long n,
-                                                                int chunks, int per_pair, float* __restrict__ d_nll) {
-  const long rows = 2 * pairs, r = blockIdx.x / chunks;
-  const Span whole = sequence_of(offsets, rows, n, r), s = part_of(whole, blockIdx.x % chunks, chunks);
-  const float g = coef[r] * d_loss[per_pair ? r % pairs : 0];
-  for (long t = s.begin + threadIdx.x; t < s.end; t += kPrefThreads) d_nll[t] = (!mask || mask[t]) ? g : 0.f;
-  zero_outside(offsets, rows, n, r, whole, blockIdx.x % chunks, d_nll);
+template <bool VEC>
+__global__ __launch_bounds__(kThreads) void pref_bwd_kernel(const float* __restrict__ d_loss, const float* __restrict__ coef,
+                                                            const uint8_t* __restrict__ mask, Seqs q, int per_pair,
+                                                            float* __restrict__ d_nll) {
+  const int w = (int)blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), s = w * kWaveTokens;
+  if (s >= q.n) return;
+  const uint32_t keep = keep8<VEC>(mask, s, q.n);
+  const int pairs = q.rows / 2;
+  float g[kLaneTokens] = {};  // tokens of no sequence: 0
+  each_sequence(q, w, [&](int r, uint32_t mine) {
+    mine &= keep;
+    const float c = coef[r] * d_loss[per_pair ? (r < pairs ? r : r - pairs) : 0];
+#pragma unroll
+    for (int k = 0; k < kLaneTokens; ++k) g[k] = ((mine >> k) & 1) ? c : g[k];
+  });
+  store8<VEC>(d_nll, s, q.n, g);
 }
 
 // e^d - d - 1 without the cancellation near 0: its series there.
-__device__ __forceinline__ float kl_of(float d) {
+__device__ __forceinline__ float kl_of(float d, float em1) {
   if (fabsf(d) < 0.5f) {
     // d^2 / 2 (1 + d / 3 (1 + d / 4 (1 + ...))), up to d^9 / 10!: 2^-26 of the sum at 0.5.
     float p = 1.f;
@@ -157,7 +288,7 @@ __device__ __forceinline__ float kl_of(float d) {
     for (int k = 10; k >= 3; --k) p = __builtin_fmaf(d * (1.f / (float)k), p, 1.f);
     return 0.5f * d * d * p;
   }
-  return expm1f(d) - d;
+  return em1 - d;
 }
 
 struct PolicyToken {
@@ -175,11 +306,11 @@ __device__ __forceinline__ PolicyToken policy_token(const PolicyLoss& p, float n
   k.slope = k.clipped ? 0.f : ratio * adv;
   k.kl = 0.f;
   if (p.has_ref) {
-    const float d = nll - ref;
-    k.kl = kl_of(d);
+    const float d = nll - ref, em1 = expm1f(d);
+    k.kl = kl_of(d, em1);
     if (p.kl_coef != 0.f) {  // 0: the KL is reported alone, and may be infinite
       k.loss += p.kl_coef * k.kl;
-      k.slope += p.kl_coef * expm1f(d);
+      k.slope += p.kl_coef * em1;
     }
   }
   return k;
@@ -187,158 +318,228 @@ __device__ __forceinline__ PolicyToken policy_token(const PolicyLoss& p, float n
 
 struct PolicyPart {
   double loss, kl;
-  long count, clipped;
+  int count, clipped;
 };
 
-__global__ __launch_bounds__(kPrefThreads) void policy_sums_kernel(const float* __restrict__ nll, const float* __restrict__ old,
-                                                                   const float* __restrict__ ref, const float* __restrict__ adv,
-                                                                   const uint8_t* __restrict__ mask,
-                                                                   const int64_t* __restrict__ offsets, long rows, long n,
-                                                                   int chunks, PolicyLoss p, PolicyPart* __restrict__ part,
-                                                                   float* __restrict__ loss) {
-  const long r = blockIdx.x / chunks;
-  const Span whole = sequence_of(offsets, rows, n, r), s = part_of(whole, blockIdx.x % chunks, chunks);
-  const float a_row = p.adv_per_token ? 0.f : adv[r];
-  double sum = 0, kl = 0;
-  int count = 0, clipped = 0;
-  for (long t = s.begin + threadIdx.x; t < s.end; t += kPrefThreads) {
-    float l = 0.f;
-    if (!mask || mask[t]) {
-      const PolicyToken k = policy_token(p, nll[t], old[t], p.has_ref ? ref[t] : 0.f, p.adv_per_token ? adv[t] : a_row);
-      l = k.loss;
-      sum += k.loss;
-      kl += k.kl;
-      ++count;
-      clipped += k.clipped;
-    }
-    if (p.reduction == kReduceNone) loss[t] = l;
+// The tokens of a tile in registers.
+template <bool VEC>
+struct PolicyTile {
+  float x[kLaneTokens], o[kLaneTokens], r[kLaneTokens], a[kLaneTokens];
+  uint32_t keep;
+  __device__ __forceinline__ void load(const float* __restrict__ nll, const float* __restrict__ old, const float* __restrict__ ref,
+                                       const float* __restrict__ adv, const uint8_t* __restrict__ mask, const PolicyLoss& p, int s,
+                                       int n) {
+    load8<VEC>(nll, s, n, x);
+    load8<VEC>(old, s, n, o);
+#pragma unroll
+    for (int k = 0; k < kLaneTokens; ++k) r[k] = a[k] = 0.f;
+    if (p.has_ref) load8<VEC>(ref, s, n, r);
+    if (p.adv_per_token) load8<VEC>(adv, s, n, a);
+    keep = keep8<VEC>(mask, s, n);
   }
-  sum = block_sum<kPrefThreads>(sum);
-  kl = block_sum<kPrefThreads>(kl);
-  count = block_sum<kPrefThreads>(count);
-  clipped = block_sum<kPrefThreads>(clipped);
-  if (threadIdx.x == 0) part[blockIdx.x] = PolicyPart{sum, kl, count, clipped};
-  if (p.reduction == kReduceNone) zero_outside(offsets, rows, n, r, whole, blockIdx.x % chunks, loss);
+};
+
+template <bool VEC>
+__device__ __forceinline__ void policy_tile(const float* __restrict__ nll, const float* __restrict__ old,
+                                            const float* __restrict__ ref, const float* __restrict__ adv,
+                                            const uint8_t* __restrict__ mask, const Seqs& q, const PolicyLoss& p, int w,
+                                            PolicyPart* __restrict__ part, float* __restrict__ loss) {
+  const int s = w * kWaveTokens;
+  PolicyTile<VEC> t;
+  t.load(nll, old, ref, adv, mask, p, s, q.n);
+  float each[kLaneTokens] = {};
+  each_sequence(q, w, [&](int r, uint32_t mine) {
+    mine &= t.keep;
+    const float a_row = p.adv_per_token ? 0.f : adv[r];
+    double sum = 0, kl = 0;
+    int count = 0;  // and, from bit 16 on, the clipped ones
+#pragma unroll
+    for (int k = 0; k < kLaneTokens; ++k)
+      if ((mine >> k) & 1) {
+        const PolicyToken y = policy_token(p, t.x[k], t.o[k], t.r[k], p.adv_per_token ? t.a[k] : a_row);
+        sum += y.loss;
+        kl += y.kl;
+        count += y.clipped ? 0x10001 : 1;
+        each[k] = y.loss;
+      }
+    sum = wave_add(sum);
+    if (p.has_ref) kl = wave_add(kl);
+    count = wave_add(count);
+    if ((threadIdx.x & 63) == 0) part[w + r] = PolicyPart{sum, kl, count & 0xffff, count >> 16};
+  });
+  if (p.reduction == kReduceNone) store8<VEC>(loss, s, q.n, each);
 }
 
-// Joins the parts: stats = (mean KL, share of clipped tokens), weight [rows] the factor of a sequence's tokens in the
-// loss, and the loss unless it is per token.
-__global__ __launch_bounds__(kJoinThreads) void policy_join_kernel(const PolicyPart* __restrict__ part, long rows, int chunks,
-                                                                   PolicyLoss p, float* __restrict__ loss,
-                                                                   float* __restrict__ stats, float* __restrict__ weight) {
+// stats = (mean KL, share of clipped tokens), weight [rows] the factor of a sequence's tokens in the loss, and the loss
+// unless it is per token.
+__device__ __forceinline__ void policy_join(const PolicyPart* part, const Seqs& q, const PolicyLoss& p,
+                                            float* __restrict__ loss, float* __restrict__ stats, float* __restrict__ weight) {
+  const int group = join_group(q.rows), lane = threadIdx.x % group;
   double sum = 0, kl = 0, means = 0;
-  long count = 0, clipped = 0, filled = 0;
-  for (long r = threadIdx.x; r < rows; r += kJoinThreads) {
+  long count = 0, clipped = 0;
+  int filled = 0;
+  for (int r0 = 0; r0 < q.rows; r0 += kJoinThreads / group) {
+    const int r = r0 + (int)threadIdx.x / group;
     double s = 0;
     long n = 0;
-    for (int c = 0; c < chunks; ++c) {
-      const PolicyPart& x = part[r * chunks + c];
-      s += x.loss;
-      n += x.count;
-      kl += x.kl;
-      clipped += x.clipped;
+    if (r < q.rows) {
+      int first, last;
+      tiles_of(q, r, first, last);
+      for (int w = first + lane; w <= last; w += group) {
+        const PolicyPart x = part[w + r];
+        s += x.loss;
+        n += x.count;
+        kl += x.kl;
+        clipped += x.clipped;
+      }
     }
     sum += s;
     count += n;
-    filled += n > 0;
-    if (n > 0) means += s / (double)n;
+    if (p.reduction == kReduceSequences) {
+      s = group_add(s, group);
+      n = group_add(n, group);
+      if (lane == 0 && r < q.rows) {
+        if (n > 0) {
+          means += s / (double)n;
+          ++filled;
+        }
+        weight[r] = (float)(n > 1 ? n : 1);  // below: its reciprocal over the sequences
+      }
+    }
   }
-  sum = block_sum<kJoinThreads>(sum);
-  kl = block_sum<kJoinThreads>(kl);
-  means = block_sum<kJoinThreads>(means);
-  count = block_sum<kJoinThreads>(count);
-  clipped = block_sum<kJoinThreads>(clipped);
-  filled = block_sum<kJoinThreads>(filled);
-  const double tokens = (double)(count > 1 ? count : 1), seqs = (double)(filled > 1 ? filled : 1);
+  kl = block_add(kl);
+  count = block_add(count);
+  clipped = block_add(clipped);
+  const double tokens = (double)(count > 1 ? count : 1);
+  double seqs = 1;
+  if (p.reduction == kReduceMean) sum = block_add(sum);
+  if (p.reduction == kReduceSequences) {
+    means = block_add(means);
+    filled = block_add(filled);
+    seqs = (double)(filled > 1 ? filled : 1);
+  }
   if (threadIdx.x == 0) {
     stats[0] = (float)(kl / tokens);
     stats[1] = (float)((double)clipped / tokens);
     if (p.reduction == kReduceMean) loss[0] = (float)(sum / tokens);
     if (p.reduction == kReduceSequences) loss[0] = (float)(means / seqs);
   }
-  for (long r = threadIdx.x; r < rows; r += kJoinThreads) {
-    double w = 1.0;
-    if (p.reduction == kReduceMean) w = 1.0 / tokens;
-    if (p.reduction == kReduceSequences) {
-      long n = 0;
-      for (int c = 0; c < chunks; ++c) n += part[r * chunks + c].count;
-      w = 1.0 / ((double)(n > 1 ? n : 1) * seqs);
-    }
-    weight[r] = (float)w;
-  }
+  // (block_add's barriers lie between the weights' two steps)
+  for (int r = threadIdx.x; r < q.rows; r += kJoinThreads)
+    weight[r] = p.reduction == kReduceMean ? (float)(1.0 / tokens) : p.reduction == kReduceNone ? 1.f
+                                           : (float)(1.0 / ((double)weight[r] * seqs));
 }
 
-__global__ __launch_bounds__(kPrefThreads) void policy_bwd_kernel(const float* __restrict__ d_loss, const float* __restrict__ nll,
-                                                                  const float* __restrict__ old, const float* __restrict__ ref,
-                                                                  const float* __restrict__ adv,
-                                                                  const uint8_t* __restrict__ mask,
-                                                                  const int64_t* __restrict__ offsets, long rows, long n,
-                                                                  int chunks, PolicyLoss p, const float* __restrict__ weight,
-                                                                  float* __restrict__ d_nll) {
-  const long r = blockIdx.x / chunks;
-  const Span whole = sequence_of(offsets, rows, n, r), s = part_of(whole, blockIdx.x % chunks, chunks);
-  const float a_row = p.adv_per_token ? 0.f : adv[r];
-  const float w = p.reduction == kReduceNone ? 1.f : weight[r] * d_loss[0];
-  for (long t = s.begin + threadIdx.x; t < s.end; t += kPrefThreads) {
-    float g = 0.f;
-    if (!mask || mask[t]) {
-      g = policy_token(p, nll[t], old[t], p.has_ref ? ref[t] : 0.f, p.adv_per_token ? adv[t] : a_row).slope * w;
-      if (p.reduction == kReduceNone) g *= d_loss[t];
-    }
-    d_nll[t] = g;
+template <bool VEC, bool ONE>
+__global__ __launch_bounds__(ONE ? kJoinThreads : kThreads) void policy_fwd_kernel(
+    const float* __restrict__ nll, const float* __restrict__ old, const float* __restrict__ ref, const float* __restrict__ adv,
+    const uint8_t* __restrict__ mask, Seqs q, PolicyLoss p, PolicyPart* part, float* __restrict__ loss,
+    float* __restrict__ stats, float* weight) {
+  constexpr int kWaves = (ONE ? kJoinThreads : kThreads) / 64;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ntiles = (q.n + kWaveTokens - 1) / kWaveTokens;
+  for (int w = ONE ? wave : (int)blockIdx.x * kWaves + wave; w < ntiles; w += ONE ? kWaves : ntiles)
+    policy_tile<VEC>(nll, old, ref, adv, mask, q, p, w, part, loss);
+  if constexpr (ONE) {
+    __syncthreads();
+    policy_join(part, q, p, loss, stats, weight);
   }
-  zero_outside(offsets, rows, n, r, whole, blockIdx.x % chunks, d_nll);
+}
+__global__ __launch_bounds__(kJoinThreads) void policy_join_kernel(const PolicyPart* __restrict__ part, Seqs q, PolicyLoss p,
+                                                                   float* __restrict__ loss, float* __restrict__ stats,
+                                                                   float* weight) {
+  policy_join(part, q, p, loss, stats, weight);
 }
 
-// Parts of a sequence: about 4096 tokens each on average, at most 64.
-int chunks_of(long rows, long n) {
-  const long c = (n / rows + 4095) / 4096;
-  return c < 1 ? 1 : c > 64 ? 64 : (int)c;
+template <bool VEC>
+__global__ __launch_bounds__(kThreads) void policy_bwd_kernel(const float* __restrict__ d_loss, const float* __restrict__ nll,
+                                                              const float* __restrict__ old, const float* __restrict__ ref,
+                                                              const float* __restrict__ adv, const uint8_t* __restrict__ mask,
+                                                              Seqs q, PolicyLoss p, const float* __restrict__ weight,
+                                                              float* __restrict__ d_nll) {
+  const int w = (int)blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), s = w * kWaveTokens;
+  if (s >= q.n) return;
+  PolicyTile<VEC> t;
+  t.load(nll, old, ref, adv, mask, p, s, q.n);
+  float up[kLaneTokens], g[kLaneTokens] = {};
+  const bool each = p.reduction == kReduceNone;
+  if (each) load8<VEC>(d_loss, s, q.n, up);
+  const float one = each ? 1.f : d_loss[0];
+  each_sequence(q, w, [&](int r, uint32_t mine) {
+    mine &= t.keep;
+    const float a_row = p.adv_per_token ? 0.f : adv[r], f = each ? 1.f : weight[r] * one;
+#pragma unroll
+    for (int k = 0; k < kLaneTokens; ++k)
+      if ((mine >> k) & 1)
+        g[k] = policy_token(p, t.x[k], t.o[k], t.r[k], p.adv_per_token ? t.a[k] : a_row).slope * (each ? up[k] : f);
+  });
+  store8<VEC>(d_nll, s, q.n, g);
 }
+
+int tiles(long n) { return (int)((n + kWaveTokens - 1) / kWaveTokens); }
+dim3 tile_grid(long n) { return dim3((unsigned)((tiles(n) + kThreads / 64 - 1) / (kThreads / 64))); }
+Seqs seqs(const int64_t* offsets, long rows, long n) { return Seqs{offsets, (int)rows, (int)n, offsets ? 0 : (int)(n / rows)}; }
+bool aligned(const void* p, unsigned bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
 }  // namespace
 
-size_t pref_workspace(long pairs, long n) { return (size_t)(2 * pairs) * chunks_of(2 * pairs, n) * sizeof(PrefPart); }
-size_t policy_workspace(long rows, long n) { return (size_t)rows * chunks_of(rows, n) * sizeof(PolicyPart); }
+size_t pref_workspace(long pairs, long n) { return (size_t)(tiles(n) + 2 * pairs) * sizeof(PrefPart); }
+size_t policy_workspace(long rows, long n) { return (size_t)(tiles(n) + rows) * sizeof(PolicyPart); }
+
+// One workgroup for a whole loss up to kOneTokens tokens (and a join's worth of sequences): a launch less.
+static bool one_launch(long rows, long n) { return n <= kOneTokens && rows <= kOneTokens / 2; }
 
 hipError_t launch_pref_fwd(const float* nll, const float* ref, const uint8_t* mask, const int64_t* offsets, long pairs, long n,
                            const PrefLoss& p, float* loss, float* reward, float* coef, void* ws, hipStream_t st) {
-  const int chunks = chunks_of(2 * pairs, n);
   PrefPart* part = static_cast<PrefPart*>(ws);
-  hipLaunchKernelGGL(pref_sums_kernel, dim3((unsigned)(2 * pairs * chunks)), dim3(kPrefThreads), 0, st, nll, ref, mask, offsets,
-                     2 * pairs, n, chunks, part);
-  hipError_t e = hipGetLastError();
+  const Seqs q = seqs(offsets, 2 * pairs, n);
+  const bool vec = aligned(nll, 16) && aligned(ref, 16) && aligned(mask, 4);
+  if (one_launch(2 * pairs, n)) {
+    auto k = vec ? pref_fwd_kernel<true, true> : pref_fwd_kernel<false, true>;
+    hipLaunchKernelGGL(k, dim3(1), dim3(kJoinThreads), 0, st, nll, ref, mask, q, p, part, loss, reward, coef);
+    return hipGetLastError();
+  }
+  auto k = vec ? pref_fwd_kernel<true, false> : pref_fwd_kernel<false, false>;
+  hipLaunchKernelGGL(k, tile_grid(n), dim3(kThreads), 0, st, nll, ref, mask, q, p, part, loss, reward, coef);
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(pref_join_kernel, dim3(1), dim3(kJoinThreads), 0, st, part, pairs, chunks, p, loss, reward, coef);
+  hipLaunchKernelGGL(pref_join_kernel, dim3(1), dim3(kJoinThreads), 0, st, part, q, p, loss, reward, coef);
   return hipGetLastError();
 }
 
 hipError_t launch_pref_bwd(const float* d_loss, const float* coef, const uint8_t* mask, const int64_t* offsets, long pairs,
                            long n, int per_pair, float* d_nll, hipStream_t st) {
-  const int chunks = chunks_of(2 * pairs, n);
-  hipLaunchKernelGGL(pref_bwd_kernel, dim3((unsigned)(2 * pairs * chunks)), dim3(kPrefThreads), 0, st, d_loss, coef, mask,
-                     offsets, pairs, n, chunks, per_pair, d_nll);
+  auto k = aligned(d_nll, 16) && aligned(mask, 4) ? pref_bwd_kernel<true> : pref_bwd_kernel<false>;
+  hipLaunchKernelGGL(k, tile_grid(n), dim3(kThreads), 0, st, d_loss, coef, mask, seqs(offsets, 2 * pairs, n), per_pair, d_nll);
   return hipGetLastError();
 }
 
 hipError_t launch_policy_fwd(const float* nll, const float* old, const float* ref, const float* adv, const uint8_t* mask,
                              const int64_t* offsets, long rows, long n, const PolicyLoss& p, float* loss, float* stats,
                              float* weight, void* ws, hipStream_t st) {
-  const int chunks = chunks_of(rows, n);
   PolicyPart* part = static_cast<PolicyPart*>(ws);
-  hipLaunchKernelGGL(policy_sums_kernel, dim3((unsigned)(rows * chunks)), dim3(kPrefThreads), 0, st, nll, old, ref, adv, mask,
-                     offsets, rows, n, chunks, p, part, loss);
-  hipError_t e = hipGetLastError();
+  const Seqs q = seqs(offsets, rows, n);
+  const bool vec = aligned(nll, 16) && aligned(old, 16) && aligned(ref, 16) && (!p.adv_per_token || aligned(adv, 16)) &&
+                   aligned(mask, 4) && (p.reduction != kReduceNone || aligned(loss, 16));
+  if (one_launch(rows, n)) {
+    auto k = vec ? policy_fwd_kernel<true, true> : policy_fwd_kernel<false, true>;
+    hipLaunchKernelGGL(k, dim3(1), dim3(kJoinThreads), 0, st, nll, old, ref, adv, mask, q, p, part, loss, stats, weight);
+    return hipGetLastError();
+  }
+  auto k = vec ? policy_fwd_kernel<true, false> : policy_fwd_kernel<false, false>;
+  hipLaunchKernelGGL(k, tile_grid(n), dim3(kThreads), 0, st, nll, old, ref, adv, mask, q, p, part, loss, stats, weight);
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(policy_join_kernel, dim3(1), dim3(kJoinThreads), 0, st, part, rows, chunks, p, loss, stats, weight);
+  hipLaunchKernelGGL(policy_join_kernel, dim3(1), dim3(kJoinThreads), 0, st, part, q, p, loss, stats, weight);
   return hipGetLastError();
 }
 
 hipError_t launch_policy_bwd(const float* d_loss, const float* nll, const float* old, const float* ref, const float* adv,
                              const uint8_t* mask, const int64_t* offsets, long rows, long n, const PolicyLoss& p,
                              const float* weight, float* d_nll, hipStream_t st) {
-  const int chunks = chunks_of(rows, n);
-  hipLaunchKernelGGL(policy_bwd_kernel, dim3((unsigned)(rows * chunks)), dim3(kPrefThreads), 0, st, d_loss, nll, old, ref, adv,
-                     mask, offsets, rows, n, chunks, p, weight, d_nll);
+  const bool vec = aligned(nll, 16) && aligned(old, 16) && aligned(ref, 16) && (!p.adv_per_token || aligned(adv, 16)) &&
+                   aligned(mask, 4) && aligned(d_nll, 16) && (p.reduction != kReduceNone || aligned(d_loss, 16));
+  auto k = vec ? policy_bwd_kernel<true> : policy_bwd_kernel<false>;
+  hipLaunchKernelGGL(k, tile_grid(n), dim3(kThreads), 0, st, d_loss, nll, old, ref, adv, mask, seqs(offsets, rows, n), p, weight,
+                     d_nll);
   return hipGetLastError();
 }
 

@@ -61,7 +61,6 @@ Entries g_api;
 PyObject* g_check = nullptr;
 PyObject* g_attn_calls = nullptr;
 PyObject* g_lce_calls = nullptr;
-PyObject* g_pref_calls = nullptr;
 PyObject* g_transposed_head = nullptr;
 PyObject* g_budget = nullptr;
 PyObject* g_env = nullptr;
@@ -254,7 +253,6 @@ struct Preference : torch::autograd::Function<Preference> {
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
-    count_backward(g_pref_calls, {"preference"});
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &coef = saved[0], &mask = saved[1], &offsets = saved[2];
     const c10::DeviceGuard device(coef.device());
@@ -306,7 +304,6 @@ struct Policy : torch::autograd::Function<Policy> {
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
-    count_backward(g_pref_calls, {"policy"});
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &nll = saved[0], &old = saved[1], &ref = saved[2], &adv = saved[3], &mask = saved[4], &offsets = saved[5];
     const at::Tensor& weight = saved[6];
@@ -564,7 +561,6 @@ void bind(const py::dict& entries, py::object check_fn) {
   g_check = check_fn.release().ptr();
 }
 void bind_attention(py::object calls) { g_attn_calls = calls.release().ptr(); }
-void bind_preference(py::object calls) { g_pref_calls = calls.release().ptr(); }
 void bind_loss(py::object calls, py::object transposed_head, py::object budget, py::object env) {
   g_lce_calls = calls.release().ptr();
   g_transposed_head = transposed_head.release().ptr();
@@ -580,7 +576,6 @@ PYBIND11_MODULE(_mtp_torch, m) {
   m.def("bind_loss", &bind_loss);
   m.def("loss", &loss);
   m.def("attention", &attention);
-  m.def("bind_preference", &bind_preference);
   m.def("scored_attention", &scored_attention);
   m.def("preference", &preference);
   m.def("policy", &policy);

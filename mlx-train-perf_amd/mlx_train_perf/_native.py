@@ -181,17 +181,16 @@ def _bind_nodes(lib):
             warnings.warn(f"{path} cannot be loaded ({e}); calls take the Python autograd functions. Run "
                           "`python -c \"import __graft_entry__ as g; g.build()\"` from the repository root.", stacklevel=2)
         return False
-    if not hasattr(_mtp_torch, "bind_preference"):   # an older build, which grows by new nodes
+    if not hasattr(_mtp_torch, "preference"):   # an older build, which grows by new nodes
         warnings.warn(f"{_mtp_torch.__file__} is from older sources; calls take the Python autograd functions. Run "
                       "`python -c \"import __graft_entry__ as g; g.build()\"` from the repository root.", stacklevel=2)
         return False
     from mlx_train_perf.attention import api
-    from mlx_train_perf.core import loss, preference
+    from mlx_train_perf.core import loss
     from mlx_train_perf.plan import launch
 
     _mtp_torch.bind({name: ctypes.cast(getattr(lib, name), _c_void_p).value for name in SIGNATURES}, check)
     _mtp_torch.bind_attention(api.VJP_CALLS)
-    _mtp_torch.bind_preference(preference.VJP_CALLS)
     _mtp_torch.bind_loss(loss.VJP_CALLS, loss._transposed_head, launch.lce_bwd_budget_bytes, os.environ.get)
     return _mtp_torch
 

@@ -25,8 +25,6 @@ from mlx_train_perf.errors import LossInputError, UnsupportedHeadError
 _KINDS = {"sigmoid": 0, "hinge": 1, "ipo": 2}
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2, "token": 1, "sequence": 3}
 
-VJP_CALLS: dict[str, int] = {}
-
 
 class PreferenceLoss(NamedTuple):
     """`chosen_rewards` and `rejected_rewards` are beta times the log ratios, (pairs,), without a gradient."""
@@ -106,10 +104,6 @@ def _plain_offsets(offsets: torch.Tensor | None) -> torch.Tensor | None:
     return None if offsets is None else offsets.to(torch.int64).contiguous()
 
 
-def _count(name: str) -> None:
-    VJP_CALLS[name] = VJP_CALLS.get(name, 0) + 1
-
-
 class _Preference(torch.autograd.Function):
     """(loss, rewards) from mtp_pref_fwd; the backward spreads each sequence's factor over its tokens. The general path:
     plain tensors take the C++ node of the same calls."""
@@ -137,7 +131,6 @@ class _Preference(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, d_loss, _d_rewards):
-        _count("preference")
         lib = _native.load()
         coef, mask, offsets = ctx.saved_tensors
         d_nll = torch.empty(ctx.shape, dtype=torch.float32, device=coef.device)
@@ -180,7 +173,6 @@ class _Policy(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, d_loss, _d_stats):
-        _count("policy")
         lib = _native.load()
         nll, old_nll, ref_nll, adv, mask, offsets, weight = ctx.saved_tensors
         d_nll = torch.empty_like(nll)
