@@ -37,34 +37,50 @@ constexpr int kKT = 64;  // positions (keys or queries) per LDS tile
 // tile's maximum exceeds it by more than this, so unnormalized probabilities stay <= 2^8.
 constexpr float kRescaleLog2 = 8.f;
 
-// Scores in the log2 domain, cap2 tanh(x / cap) - slope2 |i - j|, in two steps with the mask between them, each in
-// the place of the raw products (the registers have no room for a second array): raw(s) is r = 1 / (1 + e^(2x/cap))
-// with a cap, since tanh(t) = 1 - 2 / (1 + e^2t), or scale2 s without; of(v, d) is the score of what raw gave at
-// distance d, and bend(r) the cap's derivative 1 - tanh^2 = 4 r (1 - r). Both ends are exact (r = 0 or 1); elsewhere
-// r is off by about 2^-22, 2e-5 of a score at a cap of 50, far below the step of the bf16 probability formed from it.
-// kHidden in the place of raw's value gives the score -inf and, by the clamp, a bend of 0.
+// Scores in the log2 domain, cap2 tanh(x / cap) - slope2 |i - j|, formed in the place of the raw products s (the
+// registers have no room for a second array) so that the last step is the plain score's one multiply-add,
+// score = v mul + add, with mul > 0, and a maximum of v is one of the scores:
+//   raw: v = -1 / (1 + e^(2x/cap)) with a cap, as tanh(t) = 1 - 2 / (1 + e^2t): mul = 2 cap2, add = cap2; else v = s,
+//     mul = scale2. Both ends of the cap are exact; between them v is off by about 2^-22, 2e-5 of a score at a cap of 50
+//     and 4e-4 at 1000, the largest allowed: below the step of the bf16 probability formed from it.
+//   slant: v -= slope2 / mul |rel - c| for the element at distance |rel - c|, c a constant and rel the lane's and tile's.
+//     Where all of a wave's tile lies on one side of its positions that is one multiply-add by c, the rest (rel) in add.
+//   bend(v): -v - v^2 = (1 - tanh^2) / 4, the cap's derivative, negated and without its 4, which the gradients' last
+//     multiplier has (-4 scale).
+// A hidden pair has v = hidden<BWD>(): its score is -inf or so low that its probability is 0; in the backward it stays
+// finite under a cap, so that probability times bend is 0 as well.
 template <int MOD>
 struct Score {
-  static constexpr bool kCap = MOD & kModCap;
-  static constexpr float kHidden = kCap ? __builtin_huge_valf() : -__builtin_huge_valf();
-  float scale2;  // scale log2 e (no cap)
-  float in2;     // 2 log2 e scale / cap
-  float cap2;    // cap log2 e
-  float slope2;  // slope log2 e of the head at hand
-  __device__ __forceinline__ float raw(float s) const {
-    return kCap ? __builtin_amdgcn_rcpf(1.f + fast_exp2(s * in2)) : s * scale2;
+  static constexpr bool kCap = MOD & kModCap, kSlope = MOD & kModSlope;
+  float in2, mul, add, slope2, ratio;
+  __device__ __forceinline__ Score(float scale_log2, float cap)
+      : in2(kCap ? 2.f * scale_log2 / cap : 0.f), mul(kCap ? 2.f * cap * kLog2e : scale_log2), add(kCap ? cap * kLog2e : 0.f),
+        slope2(0.f), ratio(0.f) {}
+  __device__ __forceinline__ void set_slope(float slope) {
+    slope2 = slope * kLog2e;
+    ratio = slope2 / mul;
   }
-  __device__ __forceinline__ float of(float v, float d) const {
-    float y = kCap ? __builtin_fmaf(-2.f * cap2, v, cap2) : v;
-    if (MOD & kModSlope) y = __builtin_fmaf(-slope2, __builtin_fabsf(d), y);
-    return y;
+  template <bool BWD>
+  static __device__ __forceinline__ float hidden() { return BWD && kCap ? -1e15f : -__builtin_huge_valf(); }
+  __device__ __forceinline__ float raw(float s) const { return kCap ? __builtin_amdgcn_rcpf(-1.f - fast_exp2(s * in2)) : s; }
+  // side: 1 where rel >= c for every pair of the wave's tile that is not hidden, -1 where rel <= c, 0 where neither.
+  __device__ __forceinline__ void slant(f32x16& v, int half, int side, float rel) const {
+    if (side != 0) {
+      const float k = side > 0 ? ratio : -ratio;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) v[r] = __builtin_fmaf(k, (float)(32 * half + 8 * (r >> 2) + (r & 3)), v[r]);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        v[r] = __builtin_fmaf(-ratio, __builtin_fabsf(rel - (float)(32 * half + 8 * (r >> 2) + (r & 3))), v[r]);
+      }
+    }
   }
-  static __device__ __forceinline__ float bend(float r) { return __builtin_amdgcn_fmed3f(4.f * r * (1.f - r), 0.f, 1.f); }
+  // add of a slanted tile.
+  __device__ __forceinline__ float slant_add(int side, float rel) const { return add - (float)side * slope2 * rel; }
+  static __device__ __forceinline__ float bend(float v) { return __builtin_fmaf(v, v, v); }
 };
-template <int MOD>
-__device__ __forceinline__ Score<MOD> make_score(float scale_log2, float cap) {
-  return Score<MOD>{scale_log2, (MOD & kModCap) ? 2.f * scale_log2 / cap : 0.f, cap * kLog2e, 0.f};
-}
+
 
 // Compiler-visible waits: an inline-asm s_waitcnt is opaque to the compiler's own wait insertion,
 // which then keeps earlier loads outstanding and waits for them again later (and for every copy
@@ -345,7 +361,7 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
     my_beg = kvalid ? cbeg[kj] : S;
     w_beg = kw0 < S ? __builtin_amdgcn_readfirstlane(cbeg[kw0 + 31 < S ? kw0 + 31 : S - 1]) : 0;
   }
-  Score<MOD> score = make_score<MOD>(scale_log2, cap);
+  Score<MOD> score(scale_log2, cap);
   const int ntq = (q_end > q_begin) ? (q_end - q_begin + kKT - 1) / kKT : 0;
   const int niter = G * ntq;
   // This workgroup's share of the key block's (head, query tile) items: [it0, it0 + nloc).
@@ -470,12 +486,22 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
       const int thr = kvalid ? (SPAN ? my_beg - q0 - 4 * hf : causal ? kj - q0 - 4 * hf : -(1 << 20)) : (1 << 20);
       const int lim = my_lim - q0 - 4 * hf;
       const bool need_mask = (causal && q0 < kw0 + 31) || (q0 + kKT > S) || (PACKED && q0 + kKT > w_lim) || (SPAN && q0 < w_beg);
+      // With a cap and slopes bend needs v as raw left it, so that the bias comes after (mixed).
+      constexpr bool kMixed = MOD == kModBoth;
+      float add = score.add;
+      const float rel = (float)(kj - q0 - 4 * hf);
+      if constexpr (MOD & kModSlope) score.set_slope(slopes ? slopes[kvh * G + (it0 + it) / ntq] : 0.f);
       if constexpr (MOD != kModNone) {
-        if (MOD & kModSlope) score.slope2 = slopes[kvh * G + (it0 + it) / ntq] * kLog2e;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int r = 0; r < 16; ++r) a1[h][r] = score.raw(a1[h][r]);
+        if constexpr (MOD == kModSlope) {
+          const int side = (causal || q0 >= kw0 + 31) ? -1 : q0 + kKT - 1 <= kw0 ? 1 : 0;
+          score.slant(a1[0], 0, side, rel);
+          score.slant(a1[1], 1, side, rel);
+          add = score.slant_add(side, rel);
+        }
       }
       if (need_mask) {
 #pragma unroll
@@ -483,11 +509,10 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int c = 32 * h + 8 * (r >> 2) + (r & 3);
-            a1[h][r] = (c >= thr && c < lim) ? a1[h][r] : Score<MOD>::kHidden;
+            a1[h][r] = (c >= thr && c < lim) ? a1[h][r] : Score<MOD>::template hidden<true>();
           }
       }
       const float* ls = reinterpret_cast<const float*>(st + 2 * kTile);
-      const float rel = (float)(kj - q0 - 4 * hf);
       bf16x8 pf[2][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -500,7 +525,9 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
             if constexpr (MOD == kModNone) {
               pf[h][r >> 3][r & 7] = (__bf16)fast_exp2(__builtin_fmaf(a1[h][r], scale_log2, -l4[u] * kLog2e));
             } else {
-              const float p = fast_exp2(score.of(a1[h][r], rel - (float)(32 * h + 8 * rq + u)) - l4[u] * kLog2e);
+              float y = __builtin_fmaf(a1[h][r], score.mul, __builtin_fmaf(-kLog2e, l4[u], add));
+              if constexpr (kMixed) y = __builtin_fmaf(-score.slope2, __builtin_fabsf(rel - (float)(32 * h + 8 * rq + u)), y);
+              const float p = fast_exp2(y);
               if constexpr (CAP) pown[h][r >> 3][r & 7] = (__bf16)p;
               pf[h][r >> 3][r & 7] = (__bf16)(CAP ? p * Score<MOD>::bend(a1[h][r]) : p);
             }
@@ -645,7 +672,7 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
   }
 
   if (kvalid) {
-    const float mul = pwave ? 1.f : scale;
+    const float mul = pwave ? 1.f : CAP ? -4.f * scale : scale;  // (Score::bend)
     if (nsplit == 1) {
       bf16_t* o = (pwave ? dv : dk) + (krow + kj) * DH;
 #pragma unroll
@@ -779,10 +806,16 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
     w_end_first = in_row(__builtin_amdgcn_readfirstlane(wave_has ? snd[qw0] : 0));
     w_end_last = in_row(__builtin_amdgcn_readfirstlane(wave_has ? snd[wq_last] : 0));
   }
-  Score<MOD> score = make_score<MOD>(scale_log2, cap);
-  if (MOD & kModSlope) score.slope2 = slopes[head] * kLog2e;
+  Score<MOD> score(scale_log2, cap);
+  if constexpr (MOD & kModSlope) score.set_slope(slopes ? slopes[head] : 0.f);
+  // The side of its queries that a tile's keys lie on (Score::slant).
+  auto side_of = [&](int kv0) { return (causal || kv0 + kKT - 1 <= qw0) ? 1 : kv0 >= qw0 + 31 ? -1 : 0; };
 
-  float m = kNegInf, l = 0.f;
+  // Forward with a cap alone (kFixedMax, up to kFixedCap): no score exceeds the cap and none is below its negative, so
+  // probabilities are formed against 0: at most 2^80, summed over a row and times a value below 2^24 still in fp32's
+  // range, and at least 2^-80. That saves the running maximum, its exchange and every rescale.
+  constexpr bool kFixedMax = !DQ && MOD == kModCap;
+  float m = kFixedMax ? 0.f : kNegInf, l = 0.f;
   f32x16 acc[kDB];
 #pragma unroll
   for (int db = 0; db < kDB; ++db)
@@ -924,28 +957,34 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
         if (PACKED) ok = ok && (c >= lo);
         return ok;
       };
+      // The bias comes after, at an operation more than Score::slant: bend needs v as raw left it, and slant's two cases
+      // of 32 scores each do not fit beside dP (14 spilled registers at head_dim 128).
+      constexpr bool kMixed = MOD & kModSlope;
+      float add = score.add;
+      const float rel = (float)(qi - kv0 - 4 * hf);
       if constexpr (MOD != kModNone) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
           for (int r = 0; r < 16; ++r) sacc[kb][r] = score.raw(sacc[kb][r]);
+        add -= l2q;
       }
       if (need_mask) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) sacc[kb][r] = visible(kb, r) ? sacc[kb][r] : Score<MOD>::kHidden;
+          for (int r = 0; r < 16; ++r) sacc[kb][r] = visible(kb, r) ? sacc[kb][r] : Score<MOD>::template hidden<true>();
       }
       bf16x8 pf[4];
       // dS = P (dP - D) (1 - tanh^2), P = exp2(scale log2(e) S - L log2(e)).
-      const float rel = (float)(qi - kv0 - 4 * hf);
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          const float p = fast_exp2(MOD == kModNone ? __builtin_fmaf(sacc[kb][r], scale_log2, -l2q)
-                                                    : score.of(sacc[kb][r], rel - (float)(32 * kb + 8 * (r >> 2) + (r & 3))) - l2q);
-          const float ds = p * (pacc[kb][r] - dq_row);
+          float y = MOD == kModNone ? __builtin_fmaf(sacc[kb][r], scale_log2, -l2q) : __builtin_fmaf(sacc[kb][r], score.mul, add);
+          if constexpr (kMixed)
+            y = __builtin_fmaf(-score.slope2, __builtin_fabsf(rel - (float)(32 * kb + 8 * (r >> 2) + (r & 3))), y);
+          const float ds = fast_exp2(y) * (pacc[kb][r] - dq_row);
           pf[2 * kb + (r >> 3)][r & 7] = (__bf16)(CAP ? ds * Score<MOD>::bend(sacc[kb][r]) : ds);
         }
       // dQ^T += K^T dS^T: contraction over the 64 keys in 16-key slabs.
@@ -1045,21 +1084,24 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
         };
         // Probability r of half kb against the row bias nb into pf[2 kb + r / 8]; returns it.
         bf16x8 pf[4];
-        auto form = [&](f32x16& sc, int kb) {  // raw products into scores
+        const int side = (MOD & kModSlope) ? side_of(kv0) : 0;
+        const float rel = (float)(qi - kv0 - 4 * hf);
+        const float add = (MOD & kModSlope) ? score.slant_add(side, rel) : score.add;
+        auto form = [&](f32x16& sc, int kb) {  // raw products into v (Score)
           if constexpr (MOD != kModNone) {
-            const float rel = (float)(qi - kv0 - 4 * hf);
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-              sc[r] = score.of(score.raw(sc[r]), rel - (float)(32 * kb + 8 * (r >> 2) + (r & 3)));
+            for (int r = 0; r < 16; ++r) sc[r] = score.raw(sc[r]);
+            if constexpr (MOD & kModSlope) score.slant(sc, kb, side, rel);
           }
         };
+        auto bias = [&]() { return MOD == kModNone ? ((m == kNegInf) ? 0.f : -m) : kFixedMax ? add : ((m == kNegInf) ? 0.f : -m) + add; };
         auto prob = [&](const f32x16& sc, int kb, int r, float nb) {
-          const float p = fast_exp2(MOD == kModNone ? __builtin_fmaf(sc[r], scale_log2, nb) : sc[r] + nb);
+          const float p = fast_exp2(__builtin_fmaf(sc[r], MOD == kModNone ? scale_log2 : score.mul, nb));
           pf[2 * kb + (r >> 3)][r & 7] = (__bf16)p;
           return p;
         };
         // m = -inf only while every key seen by this row is masked; then p = exp2(-inf) = 0.
-        float nb = (m == kNegInf) ? 0.f : -m;
+        float nb = bias();
         form(s0, 0);
         mask(s0, 0);
         // Chain 1, each product followed by an even share of half 0's 16 probabilities (written in
@@ -1083,11 +1125,12 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
         tr_slab<1, kDB, kRowB>(a0, a1, tf);
         form(s1, 1);
         mask(s1, 1);
+        if constexpr (!kFixedMax) {
         float mx = kNegInf;
 #pragma unroll
         for (int r = 0; r < 16; r += 2) mx = fmaxf(fmaxf(mx, s0[r]), fmaxf(s1[r], fmaxf(s0[r + 1], s1[r + 1])));
         const float mt = MOD == kModNone ? max_xhalf(mx) * scale_log2  // scale_log2 > 0: the max of the scaled scores
-                                         : max_xhalf(mx);
+                                         : max_xhalf(__builtin_fmaf(mx, score.mul, add));  // add differs by lane half
         // A row raises m only when the tile maximum exceeds it by more than kRescaleLog2: its O and
         // l are then rescaled together and half 0 recomputed; otherwise probabilities up to
         // 2^kRescaleLog2 accumulate against the old m. O / l and L = m + log2(l) are the same
@@ -1105,10 +1148,11 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
           for (int db = 0; db < kDB; ++db)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[db][r] *= alpha;
-          nb = (m == kNegInf) ? 0.f : -m;
+          nb = bias();
           l0 = 0.f;
 #pragma unroll
           for (int r = 0; r < 16; ++r) l0 += prob(s0, 0, r, nb);
+        }
         }
         l += l0;
         // O^T += V^T P^T: half 0's two 16-key slabs, each product followed by an even share of half
@@ -1149,7 +1193,7 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
     }
   }
 
-  float mul = scale, lt = 0.f;
+  float mul = (DQ && CAP) ? -4.f * scale : scale, lt = 0.f;  // (Score::bend)
   if constexpr (!DQ) {
     lt = l + __shfl_xor(l, 32, 64);
     mul = (lt > 0.f) ? 1.f / lt : 0.f;

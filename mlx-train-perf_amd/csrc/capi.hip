@@ -104,6 +104,7 @@ int check_scored(const void* q, const void* k, const void* v, int64_t b, int64_t
   if (s >= (int64_t(1) << 23)) return fail(MTP_ERR_INPUT, "s must be < 2^23 with softcap, slopes or spans (got %lld)", (long long)s);
   if (!(scale > 0.f) || !(scale < HUGE_VALF)) return fail(MTP_ERR_INPUT, "scale must be positive and finite (got %g)", (double)scale);
   if (!(softcap >= 0.f) || !(softcap < HUGE_VALF)) return fail(MTP_ERR_INPUT, "softcap must be finite and >= 0, 0 for none (got %g)", (double)softcap);
+  if (softcap != 0.f && !(softcap >= 1e-3f && softcap <= 1e3f)) return fail(MTP_ERR_UNSUPPORTED, "kernel impl serves a softcap in [1e-3, 1e3] (got %g); use impl='reference'", (double)softcap);
   if ((span_start == nullptr) != (span_end == nullptr)) return fail(MTP_ERR_INPUT, "span_start and span_end must be both given or both null");
   if (span_start && causal) return fail(MTP_ERR_INPUT, "spans are the whole mask: causal must be 0 with them");
   if (!span_start && !slopes && softcap == 0.f) return fail(MTP_ERR_INPUT, "no softcap, slopes or spans given: use mtp_attn_fwd / mtp_attn_bwd");
