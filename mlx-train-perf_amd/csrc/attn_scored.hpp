@@ -22,13 +22,13 @@ hipError_t scored_bwd(const AttnShape& sh, const AttnScore& sc, const ScoredWork
                       const bf16_t* k, const bf16_t* v, const bf16_t* o, const float* lse, const bf16_t* d_o,
                       bf16_t* dq, bf16_t* dk, bf16_t* dv, int grid, hipStream_t st);
 
-// f(std::integral_constant<int, MOD>) for the call's score form. The forward of a cap alone runs against a fixed
-// maximum up to a cap of 80 ln 2 = 55.4 (attn_kv_kernel), above it as a cap with slopes of none.
+// The forward under a cap of at most 80 ln 2 runs against a fixed maximum (attn_kv_kernel).
 constexpr float kFixedCap = 55.4f;
+// f(std::integral_constant<int, MOD>) for the call's score form.
 template <class F>
-hipError_t with_mod(const AttnScore& sc, bool fwd, F&& f) {
+hipError_t with_mod(const AttnScore& sc, F&& f) {
   if (sc.cap > 0.f) {
-    if (sc.slopes || (fwd && sc.cap > kFixedCap)) return f(std::integral_constant<int, kModBoth>{});
+    if (sc.slopes) return f(std::integral_constant<int, kModBoth>{});
     return f(std::integral_constant<int, kModCap>{});
   }
   if (sc.slopes) return f(std::integral_constant<int, kModSlope>{});
@@ -40,7 +40,7 @@ template <>
 hipError_t scored_fwd<MTP_SCORED_DH>(const AttnShape& sh, const AttnScore& sc, const bf16_t* q, const bf16_t* k,
                                      const bf16_t* v, bf16_t* o, float* lse, int grid, hipStream_t st) {
   constexpr int DH = MTP_SCORED_DH;
-  return with_mod(sc, true, [&](auto m) {
+  return with_mod(sc, [&](auto m) {
     constexpr int MOD = decltype(m)::value;
     auto launch = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, st, q, k, v, nullptr, nullptr, nullptr, nullptr, sc.end,
@@ -48,8 +48,18 @@ hipError_t scored_fwd<MTP_SCORED_DH>(const AttnShape& sh, const AttnScore& sc, c
                          sc.cap, sc.slopes);
       return hipGetLastError();
     };
-    if (sc.start) return launch(attn_kv_kernel<DH, kMaskSpan, false, MOD>);
-    if constexpr (MOD != kModNone) return launch(attn_kv_kernel<DH, kMaskPlain, false, MOD>);
+    // A cap above kFixedCap runs as a cap with slopes of none; spans may hide a query's own key, whose bias of 0 the
+    // fixed maximum counts on.
+    constexpr int RUN = MOD == kModCap ? kModBoth : MOD;
+    const bool fixed = sc.cap <= kFixedCap;
+    if (sc.start) {
+      if constexpr (MOD == kModCap)
+        if (fixed) return launch(attn_kv_kernel<DH, kMaskSpan, false, MOD, true>);
+      return launch(attn_kv_kernel<DH, kMaskSpan, false, RUN>);
+    }
+    if constexpr (MOD & kModCap)
+      if (fixed) return launch(attn_kv_kernel<DH, kMaskPlain, false, MOD, true>);
+    if constexpr (MOD != kModNone) return launch(attn_kv_kernel<DH, kMaskPlain, false, RUN>);
     return hipErrorInvalidValue;
   });
 }
@@ -60,7 +70,7 @@ hipError_t scored_bwd<MTP_SCORED_DH>(const AttnShape& sh, const AttnScore& sc, c
                                      const float* lse, const bf16_t* d_o, bf16_t* dq, bf16_t* dk, bf16_t* dv, int grid,
                                      hipStream_t st) {
   constexpr int DH = MTP_SCORED_DH;
-  return with_mod(sc, false, [&](auto m) {
+  return with_mod(sc, [&](auto m) {
     constexpr int MOD = decltype(m)::value;
     auto launch = [&](auto dq_kernel, auto dkv_kernel) {
       hipLaunchKernelGGL(dq_kernel, dim3(grid), dim3(256), 0, st, q, k, v, d_o, o, lse, ws.dvec, sc.end, sc.start, dq,
