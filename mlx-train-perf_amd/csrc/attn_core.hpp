@@ -44,7 +44,8 @@ constexpr float kRescaleLog2 = 8.f;
 //     mul = scale2. Both ends of the cap are exact; between them v is off by about 2^-22, 2e-5 of a score at a cap of 50
 //     and 4e-4 at 1000, the largest allowed: below the step of the bf16 probability formed from it.
 //   slant: v -= slope2 / mul |rel - c| for the element at distance |rel - c|, c a constant and rel the lane's and tile's.
-//     Where all of a wave's tile lies on one side of its positions that is one multiply-add by c, the rest (rel) in add.
+//     Where all of a wave's tile lies on one side of its positions that is a term in c, the rest (rel) in add: one
+//     multiply-add, or none where the product began from the term (ramp, a cap aside) instead of from 0.
 //   bend(v): -v - v^2 = (1 - tanh^2) / 4, the cap's derivative, negated and without its 4, which the gradients' last
 //     multiplier has (-4 scale).
 // A hidden pair has v = hidden<BWD>(): its score is -inf or so low that its probability is 0; in the backward it stays
@@ -63,21 +64,39 @@ struct Score {
   template <bool BWD>
   static __device__ __forceinline__ float hidden() { return BWD && kCap ? -1e15f : -__builtin_huge_valf(); }
   __device__ __forceinline__ float raw(float s) const { return kCap ? __builtin_amdgcn_rcpf(-1.f - fast_exp2(s * in2)) : s; }
-  // side: 1 where rel >= c for every pair of the wave's tile that is not hidden, -1 where rel <= c, 0 where neither.
+  static __device__ __forceinline__ constexpr float at(int half, int r) { return (float)(32 * half + 8 * (r >> 2) + (r & 3)); }
+  // SIGN ratio c: what a product begins from.
+  template <int SIGN>
+  __device__ __forceinline__ void set_ramp(f32x16 (&ramp)[2]) const {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) ramp[h][r] = SIGN * ratio * at(h, r);
+  }
+  // side: 1 where rel >= c for every pair of the wave's tile that is not hidden, -1 where rel <= c, 0 where neither; SIGN
+  // the usual one, whose term (a ramp's) a tile of neither keeps and corrects.
+  template <int SIGN, bool RAMP>
   __device__ __forceinline__ void slant(f32x16& v, int half, int side, float rel) const {
-    if (side != 0) {
-      const float k = side > 0 ? ratio : -ratio;
+    if constexpr (RAMP) {
+      if (side == -SIGN) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) v[r] = __builtin_fmaf(k, (float)(32 * half + 8 * (r >> 2) + (r & 3)), v[r]);
-    } else {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        v[r] = __builtin_fmaf(-ratio, __builtin_fabsf(rel - (float)(32 * half + 8 * (r >> 2) + (r & 3))), v[r]);
+        for (int r = 0; r < 16; ++r) v[r] = __builtin_fmaf(-2 * SIGN * ratio, at(half, r), v[r]);
       }
+    } else {
+      const float k = side == -SIGN ? -SIGN * ratio : SIGN * ratio;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) v[r] = __builtin_fmaf(k, at(half, r), v[r]);
+    }
+    if (side == 0) {  // -|d| = -SIGN d + 2 min(SIGN d, 0)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) v[r] = __builtin_fmaf(2.f * ratio, fminf(SIGN * (rel - at(half, r)), 0.f), v[r]);
     }
   }
   // add of a slanted tile.
-  __device__ __forceinline__ float slant_add(int side, float rel) const { return add - (float)side * slope2 * rel; }
+  template <int SIGN>
+  __device__ __forceinline__ float slant_add(int side, float rel) const {
+    return add - (side == -SIGN ? -SIGN : SIGN) * slope2 * rel;
+  }
   static __device__ __forceinline__ float bend(float v) { return __builtin_fmaf(v, v, v); }
 };
 
@@ -445,6 +464,10 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
   // Start of tile `it` (stage `st`): the first product of both halves into a1; the P wave then
   // forms P (hidden pairs 0) and writes it to `pb`.
   f32x16 a1[2];
+  // With slopes alone the P wave's products begin from the bias' ramp of the head at hand, where it fits the registers.
+  constexpr bool kRamp = MOD == kModSlope && DH <= 96;
+  f32x16 ramp[2];
+  int ramp_head = -1;
   // With a cap the P wave hands its partner P (1 - tanh^2), which dS is formed from, and keeps P itself in
   // registers for its own second product.
   bf16x8 pown[CAP ? 2 : 1][2];
@@ -462,6 +485,18 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int r = 0; r < 16; ++r) a1[h][r] = 0.f;
+      if constexpr (kRamp) {
+        if (pwave) {
+          const int hh = (it0 + it) / ntq;
+          if (hh != ramp_head) {
+            ramp_head = hh;
+            score.set_slope(slopes ? slopes[kvh * G + hh] : 0.f);
+            score.template set_ramp<-1>(ramp);
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) a1[h] = ramp[h];
+        }
+      }
       issue_scal(cx, sx);
       rd(0);
       rd(1);
@@ -490,7 +525,7 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
       constexpr bool kMixed = MOD == kModBoth;
       float add = score.add;
       const float rel = (float)(kj - q0 - 4 * hf);
-      if constexpr (MOD & kModSlope) score.set_slope(slopes ? slopes[kvh * G + (it0 + it) / ntq] : 0.f);
+      if constexpr ((MOD & kModSlope) && !kRamp) score.set_slope(slopes ? slopes[kvh * G + (it0 + it) / ntq] : 0.f);
       if constexpr (MOD != kModNone) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -498,9 +533,9 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
           for (int r = 0; r < 16; ++r) a1[h][r] = score.raw(a1[h][r]);
         if constexpr (MOD == kModSlope) {
           const int side = (causal || q0 >= kw0 + 31) ? -1 : q0 + kKT - 1 <= kw0 ? 1 : 0;
-          score.slant(a1[0], 0, side, rel);
-          score.slant(a1[1], 1, side, rel);
-          add = score.slant_add(side, rel);
+          score.template slant<-1, kRamp>(a1[0], 0, side, rel);
+          score.template slant<-1, kRamp>(a1[1], 1, side, rel);
+          add = score.template slant_add<-1>(side, rel);
         }
       }
       if (need_mask) {
@@ -811,6 +846,11 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
   // The side of its queries that a tile's keys lie on (Score::slant).
   auto side_of = [&](int kv0) { return (causal || kv0 + kKT - 1 <= qw0) ? 1 : kv0 >= qw0 + 31 ? -1 : 0; };
 
+  // Slopes alone: the products K Q^T begin from the bias' ramp where it fits the registers.
+  constexpr bool kRamp = MOD == kModSlope && (!DQ || DH <= 96);
+  f32x16 ramp[2];
+  if constexpr (kRamp) score.template set_ramp<1>(ramp);
+
   // Forward with a fixed maximum (FIXED): under a cap of at most kFixedCap no score exceeds the cap, and of every row
   // that sees anything some score (with slopes, in the masks that show a query its own key, that key's) is at least its
   // negative. So probabilities are formed against 0: at most 2^80, summed over a row and times a value below 2^24 still
@@ -921,7 +961,7 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        sacc[kb][r] = 0.f;
+        sacc[kb][r] = kRamp ? ramp[kb][r] : 0.f;
         pacc[kb][r] = 0.f;
       }
     constexpr int RA = 1;
@@ -969,9 +1009,7 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
         if (PACKED) ok = ok && (c >= lo);
         return ok;
       };
-      // The bias comes after, at an operation more than Score::slant: bend needs v as raw left it, and slant's two cases
-      // of 32 scores each do not fit beside dP (14 spilled registers at head_dim 128).
-      constexpr bool kMixed = MOD & kModSlope;
+      constexpr bool kMixed = MOD == kModBoth;  // bend needs v as raw left it: the bias comes after
       float add = score.add;
       const float rel = (float)(qi - kv0 - 4 * hf);
       if constexpr (MOD != kModNone) {
@@ -979,6 +1017,12 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
           for (int r = 0; r < 16; ++r) sacc[kb][r] = score.raw(sacc[kb][r]);
+        if constexpr (MOD == kModSlope) {
+          const int side = side_of(kv0);
+          score.template slant<1, kRamp>(sacc[0], 0, side, rel);
+          score.template slant<1, kRamp>(sacc[1], 1, side, rel);
+          add = score.template slant_add<1>(side, rel);
+        }
         add -= l2q;
       }
       if (need_mask) {
@@ -1052,8 +1096,8 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
     f32x16 s0, s1;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      s0[r] = 0.f;
-      s1[r] = 0.f;
+      s0[r] = kRamp ? ramp[0][r] : 0.f;
+      s1[r] = kRamp ? ramp[1][r] : 0.f;
     }
     // Step i of the 2 kDK products: chain i / kDK, k16 step i % kDK; row fragments two steps ahead.
     constexpr int RA = 2;
@@ -1098,12 +1142,12 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
         bf16x8 pf[4];
         const int side = (MOD & kModSlope) ? side_of(kv0) : 0;
         const float rel = (float)(qi - kv0 - 4 * hf);
-        const float add = (MOD & kModSlope) ? score.slant_add(side, rel) : score.add;
+        const float add = (MOD & kModSlope) ? score.template slant_add<1>(side, rel) : score.add;
         auto form = [&](f32x16& sc, int kb) {  // raw products into v (Score)
           if constexpr (MOD != kModNone) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) sc[r] = score.raw(sc[r]);
-            if constexpr (MOD & kModSlope) score.slant(sc, kb, side, rel);
+            if constexpr (MOD & kModSlope) score.template slant<1, kRamp>(sc, kb, side, rel);
           }
         };
         auto bias = [&]() { return MOD == kModNone ? ((m == kNegInf) ? 0.f : -m) : FIXED ? add : ((m == kNegInf) ? 0.f : -m) + add; };
