@@ -567,8 +567,6 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
               pf[h][r >> 3][r & 7] = (__bf16)(CAP ? p * Score<MOD>::bend(a1[h][r]) : p);
             }
           }
-          // Four at a time: the scheduler would otherwise hold more of them in flight than there are registers.
-          if constexpr (CAP) __builtin_amdgcn_sched_barrier(0);
         }
       // Chunk j of every lane is one contiguous KiB of this key group's P.
 #pragma unroll
