@@ -19,9 +19,9 @@
 // takes 512 consecutive tokens, whatever sequences they belong to (sequences dealt to workgroups made the longest of a
 // ragged batch the whole time), and has all its loads in flight at once: eight tokens a lane. For every sequence r that
 // wave w touches it leaves one part at slot w + r; as w and r never decrease along the tokens no two parts share a slot,
-// so nwaves + rows slots hold them. A join, one workgroup, adds each sequence's parts in order. Sums are in 64 bits, since
-// a log ratio is the small difference of long sums, and no result depends on scheduling. Up to kOneTokens tokens one
-// workgroup does both in one launch.
+// so nwaves + rows slots hold them. A join, one workgroup, adds each sequence's parts in a fixed order. Sums are in 64 bits,
+// since a log ratio is the small difference of long sums, and no result depends on scheduling. Up to kOneTokens tokens of
+// kOneRows sequences one workgroup does both in one launch, the parts in LDS.
 #include "mtp_common.hpp"
 #include "mtp_launch.hpp"
 
@@ -31,7 +31,8 @@ namespace {
 constexpr int kLaneTokens = 8, kWaveTokens = 64 * kLaneTokens;
 constexpr int kThreads = 256;        // a workgroup of the large grid
 constexpr int kJoinThreads = 1024;   // the join's, and that of the one-launch form
-constexpr int kOneTokens = 16384;
+constexpr int kOneTokens = 16384, kOneRows = 512;
+constexpr int kOneParts = kOneTokens / kWaveTokens + kOneRows;
 
 struct Seqs {
   const int64_t* offsets;
@@ -123,25 +124,52 @@ __device__ __forceinline__ void each_sequence(const Seqs& q, int w, F&& f) {
   }
 }
 
+// x of another lane of the same 16, by the DPP control CTRL: lanes 1 or 2 away, or mirrored within 8 or 16.
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kMirror8 = 0x141, kMirror16 = 0x140;
+template <int CTRL, class T>
+__device__ __forceinline__ T dpp(T x) {
+  static_assert(sizeof(T) % 4 == 0);
+  struct Words {
+    int w[sizeof(T) / 4];
+  };
+  Words v = __builtin_bit_cast(Words, x);
+#pragma unroll
+  for (unsigned i = 0; i < sizeof(T) / 4; ++i) v.w[i] = __builtin_amdgcn_update_dpp(0, v.w[i], CTRL, 0xf, 0xf, true);
+  return __builtin_bit_cast(T, v);
+}
+template <class T>
+__device__ __forceinline__ T read_lane(T x, int lane) {
+  struct Words {
+    int w[sizeof(T) / 4];
+  };
+  Words v = __builtin_bit_cast(Words, x);
+#pragma unroll
+  for (unsigned i = 0; i < sizeof(T) / 4; ++i) v.w[i] = __builtin_amdgcn_readlane(v.w[i], lane);
+  return __builtin_bit_cast(T, v);
+}
+// Sum over each 16 lanes, in all of them; a quarter of the time of exchanges through LDS.
+template <class T>
+__device__ __forceinline__ T row_add(T x) {
+  x += dpp<kXor1>(x);
+  x += dpp<kXor2>(x);
+  x += dpp<kMirror8>(x);
+  return x + dpp<kMirror16>(x);
+}
 template <class T>
 __device__ __forceinline__ T wave_add(T x) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o, 64);
-  return x;
+  x = row_add(x);
+  return ((read_lane(x, 0) + read_lane(x, 16)) + read_lane(x, 32)) + read_lane(x, 48);
 }
-// Sum over the join's threads, in every thread: within a wave by halves, then the 16 waves' by halves.
+// Sum over the join's threads, in every thread.
 template <class T>
 __device__ __forceinline__ T block_add(T x) {
-  constexpr int kWaves = kJoinThreads / 64;
-  __shared__ T part[kWaves];
+  static_assert(kJoinThreads == 16 * 64);
+  __shared__ T part[16];
   x = wave_add(x);
   __syncthreads();  // the last use of part is over
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
   __syncthreads();
-  x = part[threadIdx.x % kWaves];
-#pragma unroll
-  for (int o = kWaves / 2; o >= 1; o >>= 1) x += __shfl_xor(x, o, 64);
-  return x;
+  return row_add(part[threadIdx.x % 16]);
 }
 
 // The join gives every item (a pair, a sequence) a group of lanes, as many as there are threads for (a power of two, 64 at
@@ -153,7 +181,12 @@ __device__ __forceinline__ int join_group(int items) {
 }
 template <class T>
 __device__ __forceinline__ T group_add(T x, int group) {
-  for (int o = group >> 1; o >= 1; o >>= 1) x += __shfl_xor(x, o, 64);
+  if (group >= 2) x += dpp<kXor1>(x);
+  if (group >= 4) x += dpp<kXor2>(x);
+  if (group >= 8) x += dpp<kMirror8>(x);
+  if (group >= 16) x += dpp<kMirror16>(x);
+  if (group >= 32) x += __shfl_xor(x, 16, 64);
+  if (group >= 64) x += __shfl_xor(x, 32, 64);
   return x;
 }
 // Tiles [first, last] with a part of sequence r; none for an empty one.
@@ -170,7 +203,7 @@ struct PrefPart {
 
 template <bool VEC>
 __device__ __forceinline__ void pref_tile(const float* __restrict__ nll, const float* __restrict__ ref,
-                                          const uint8_t* __restrict__ mask, const Seqs& q, int w, PrefPart* __restrict__ part) {
+                                          const uint8_t* __restrict__ mask, const Seqs& q, int w, PrefPart* part) {
   const int s = w * kWaveTokens;
   float x[kLaneTokens], y[kLaneTokens];
   load8<VEC>(nll, s, q.n, x);
@@ -245,7 +278,9 @@ __device__ __forceinline__ void pref_join(const PrefPart* part, const Seqs& q, c
 template <bool VEC, bool ONE>
 __global__ __launch_bounds__(ONE ? kJoinThreads : kThreads) void pref_fwd_kernel(
     const float* __restrict__ nll, const float* __restrict__ ref, const uint8_t* __restrict__ mask, Seqs q, PrefLoss p,
-    PrefPart* part, float* __restrict__ loss, float* __restrict__ reward, float* __restrict__ coef) {
+    PrefPart* ws, float* __restrict__ loss, float* __restrict__ reward, float* __restrict__ coef) {
+  __shared__ PrefPart lds[ONE ? kOneParts : 1];
+  PrefPart* part = ONE ? lds : ws;
   constexpr int kWaves = (ONE ? kJoinThreads : kThreads) / 64;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ntiles = (q.n + kWaveTokens - 1) / kWaveTokens;
   for (int w = ONE ? wave : (int)blockIdx.x * kWaves + wave; w < ntiles; w += ONE ? kWaves : ntiles)
@@ -343,7 +378,7 @@ template <bool VEC>
 __device__ __forceinline__ void policy_tile(const float* __restrict__ nll, const float* __restrict__ old,
                                             const float* __restrict__ ref, const float* __restrict__ adv,
                                             const uint8_t* __restrict__ mask, const Seqs& q, const PolicyLoss& p, int w,
-                                            PolicyPart* __restrict__ part, float* __restrict__ loss) {
+                                            PolicyPart* part, float* __restrict__ loss) {
   const int s = w * kWaveTokens;
   PolicyTile<VEC> t;
   t.load(nll, old, ref, adv, mask, p, s, q.n);
@@ -433,8 +468,10 @@ __device__ __forceinline__ void policy_join(const PolicyPart* part, const Seqs& 
 template <bool VEC, bool ONE>
 __global__ __launch_bounds__(ONE ? kJoinThreads : kThreads) void policy_fwd_kernel(
     const float* __restrict__ nll, const float* __restrict__ old, const float* __restrict__ ref, const float* __restrict__ adv,
-    const uint8_t* __restrict__ mask, Seqs q, PolicyLoss p, PolicyPart* part, float* __restrict__ loss,
+    const uint8_t* __restrict__ mask, Seqs q, PolicyLoss p, PolicyPart* ws, float* __restrict__ loss,
     float* __restrict__ stats, float* weight) {
+  __shared__ PolicyPart lds[ONE ? kOneParts : 1];
+  PolicyPart* part = ONE ? lds : ws;
   constexpr int kWaves = (ONE ? kJoinThreads : kThreads) / 64;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ntiles = (q.n + kWaveTokens - 1) / kWaveTokens;
   for (int w = ONE ? wave : (int)blockIdx.x * kWaves + wave; w < ntiles; w += ONE ? kWaves : ntiles)
@@ -484,8 +521,8 @@ bool aligned(const void* p, unsigned bytes) { return ((uintptr_t)p & (bytes - 1)
 size_t pref_workspace(long pairs, long n) { return (size_t)(tiles(n) + 2 * pairs) * sizeof(PrefPart); }
 size_t policy_workspace(long rows, long n) { return (size_t)(tiles(n) + rows) * sizeof(PolicyPart); }
 
-// One workgroup for a whole loss up to kOneTokens tokens (and a join's worth of sequences): a launch less.
-static bool one_launch(long rows, long n) { return n <= kOneTokens && rows <= kOneTokens / 2; }
+// One workgroup for a whole loss: a launch less.
+static bool one_launch(long rows, long n) { return n <= kOneTokens && rows <= kOneRows; }
 
 hipError_t launch_pref_fwd(const float* nll, const float* ref, const uint8_t* mask, const int64_t* offsets, long pairs, long n,
                            const PrefLoss& p, float* loss, float* reward, float* coef, void* ws, hipStream_t st) {
