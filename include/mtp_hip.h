@@ -309,11 +309,15 @@ int mtp_attn_scored_bwd(const void* q, const void* k, const void* v, const void*
                         const int32_t* span_start, const int32_t* span_end, void* d_q, void* d_k, void* d_v,
                         void* workspace, size_t workspace_bytes, void* stream);
 
-/* The same with fp32 tensors; the backward's workspace is mtp_attn_bwd_f32_workspace_bytes. */
+/* The same with fp32 tensors. Where few workgroups would run, the passes are split over the keys and their parts
+ * joined in order: the workspaces hold them (the forward's may be NULL, the backward's needs D, fp32 [b][hq][s], at
+ * least; a pass without room for its parts runs unsplit). */
+size_t mtp_attn_scored_fwd_f32_workspace_bytes(int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh);
 int mtp_attn_scored_fwd_f32(const float* q, const float* k, const float* v, int64_t b, int64_t hq,
                             int64_t hkv, int64_t s, int64_t dh, float scale, int32_t causal, float softcap,
                             const float* slopes, const int32_t* span_start, const int32_t* span_end, float* o,
-                            float* lse, void* stream);
+                            float* lse, void* workspace, size_t workspace_bytes, void* stream);
+size_t mtp_attn_scored_bwd_f32_workspace_bytes(int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh);
 int mtp_attn_scored_bwd_f32(const float* q, const float* k, const float* v, const float* o, const float* lse,
                             const float* d_o, int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh,
                             float scale, int32_t causal, float softcap, const float* slopes,

@@ -222,17 +222,24 @@ void attn32_q_kernel(const float* __restrict__ q, const float* __restrict__ k, c
                      const float* __restrict__ d_o, const float* __restrict__ o_in, const float* __restrict__ lse_in,
                      float* __restrict__ dvec, const int32_t* __restrict__ seg_start, float* __restrict__ out,
                      float* __restrict__ lse_out, int B, int Hq, int Hkv, int S, float scale, int causal,
-                     const int32_t* __restrict__ span_end, float cap, const float* __restrict__ slopes) {
+                     const int32_t* __restrict__ span_end, float cap, const float* __restrict__ slopes, int nsplit,
+                     float* __restrict__ part) {
   // seg_start: the first key that each query sees (packed: its segment's start; span: its span's).
+  // Scored calls of few workgroups are split (attn32_q_splits): workgroup `split` of a pair of blocks takes every
+  // nsplit-th key tile from tile `split` on, and writes its dQ, or its unnormalized O, maximum and sum, to
+  // part[split] ([b][hq][s][dh], the forward's maxima and sums [split][b][hq][s][2] behind all of them).
   constexpr bool PACKED = MASK != kMaskPlain, SPAN = MASK == kMaskSpan, CAP = MOD & kModCap;
+  constexpr bool SPLIT = SPAN || MOD != kModNone;
   using L = ALay<DH>;
   __shared__ __attribute__((aligned(1024))) char lds0[2 * L::kTile];  // K, V
   __shared__ __attribute__((aligned(1024))) char lds1[2 * L::kTile];
   const int G = Hq / Hkv, hpw = q_heads32(G), R = 16 * (4 / hpw);
   const int nqb = (S + R - 1) / R, hgb = Hq / hpw, nhg = B * hgb;
-  const int hg = blockIdx.x % nhg, b = hg / hgb, h0 = (hg % hgb) * hpw, kvh = h0 / G;
+  const int ns = SPLIT ? nsplit : 1, split = SPLIT ? blockIdx.x % ns : 0;
+  const unsigned wg = SPLIT ? blockIdx.x / ns : blockIdx.x;
+  const int hg = wg % nhg, b = hg / hgb, h0 = (hg % hgb) * hpw, kvh = h0 / G;
   int pa, pb;
-  pair_blocks((int)(blockIdx.x / nhg), nqb, causal && !PACKED, pa, pb);
+  pair_blocks((int)(wg / nhg), nqb, causal && !PACKED, pa, pb);
   ALane<DH> ln;
   ln.init();
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), u = w & 3;
@@ -263,7 +270,7 @@ void attn32_q_kernel(const float* __restrict__ q, const float* __restrict__ k, c
 #pragma unroll
       for (int s = 0; s < 4; ++s) dp = __builtin_fmaf(dx[c][s], ox[c][s], dp);
     dq_row = col_sum(dp);
-    if (qvalid && ln.g == 0) dvec[qrow + qi] = dq_row;
+    if (qvalid && ln.g == 0 && split == 0) dvec[qrow + qi] = dq_row;
     l2q = qvalid ? lse_in[qrow + qi] * kLog2e : 0.f;
   }
   // Keys of the workgroup: those of its last block (the latest queries) and, packed, from its first
@@ -285,8 +292,8 @@ void attn32_q_kernel(const float* __restrict__ q, const float* __restrict__ k, c
   f32x4 acc[L::kB];
 #pragma unroll
   for (int i = 0; i < L::kB; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  ln.copy(kh, kv_begin, S, lds0, ntiles > 0);  // no tile (a segment start past the queries): nothing read
-  ln.copy(vh, kv_begin, S, lds0 + L::kTile, ntiles > 0);
+  ln.copy(kh, kv_begin + split * kPos, S, lds0, ntiles > split);  // no tile (a segment start past the queries): nothing read
+  ln.copy(vh, kv_begin + split * kPos, S, lds0 + L::kTile, ntiles > split);
   copies_landed();
   // The row loads are complete here: tell the compiler, which would wait for them (and for the copies
   // in flight) at their first use.
@@ -298,8 +305,8 @@ void attn32_q_kernel(const float* __restrict__ q, const float* __restrict__ k, c
 
   auto body = [&](int t, const char* cur, char* nxt) __attribute__((always_inline)) {
     const int kv0 = kv_begin + t * kPos;
-    ln.copy(kh, kv0 + kPos, S, nxt, t + 1 < ntiles);
-    ln.copy(vh, kv0 + kPos, S, nxt + L::kTile, t + 1 < ntiles);
+    ln.copy(kh, kv0 + ns * kPos, S, nxt, t + ns < ntiles);
+    ln.copy(vh, kv0 + ns * kPos, S, nxt + L::kTile, t + ns < ntiles);
     if (wave_has && !(causal && kv0 > wq_last) && !(PACKED && kv0 + kPos - 1 < w_sst_first) && !(SPAN && kv0 >= w_end_last)) {
       f32x4 sc[2];
       ln.dot_rows(cur, qx, sc);  // S^T = K Q^T
@@ -377,22 +384,30 @@ void attn32_q_kernel(const float* __restrict__ q, const float* __restrict__ k, c
     }
     copies_landed();
   };
-  for (int t = 0; t < ntiles; t += 2) {
+  for (int t = split; t < ntiles; t += 2 * ns) {
     body(t, lds0, lds1);
-    if (t + 1 < ntiles) body(t + 1, lds1, lds0);
+    if (t + ns < ntiles) body(t + ns, lds1, lds0);
   }
+  const long rows = (long)B * Hq * S;
   if constexpr (DQ) {
+    if (SPLIT && ns > 1) out = part + split * rows * DH;
     if (qvalid) ln.store_row(out + (qrow + qi) * DH, acc, scale);
   } else {
     const float lt = col_sum(l);
     if (!qvalid) return;
+    if (SPLIT && ns > 1) {
+      if (ln.g == 0) *reinterpret_cast<f32x2*>(part + ns * rows * DH + 2 * (split * rows + qrow + qi)) = f32x2{m, lt};
+      ln.store_row(part + (split * rows + qrow + qi) * DH, acc, 1.f);
+      asm volatile("s_nop 0");  // (below)
+      return;
+    }
     // A query that sees nothing: +inf with spans, so that the backward's exp(S - L) is 0.
     if (ln.g == 0) lse_out[qrow + qi] = (lt > 0.f) ? (m + fast_log2(lt)) * kLn2 : SPAN ? -kNegInf : kNegInf;
     ln.store_row(out + (qrow + qi) * DH, acc, lt > 0.f ? 1.f / lt : 0.f);
-    // Keeps the last store apart from the block that the compiler places behind the program's end, which writes the
-    // store's data registers (never run after it, but alike to the listing check of such pairs).
-    if constexpr (SPAN) asm volatile("s_nop 0");
   }
+  // The padding behind a program's end reads as a write of v0, which the listing check of stores whose data the next
+  // instructions write would hold against a last store of v0.
+  if constexpr (SPLIT) asm volatile("s_nop 0");
 }
 
 // dK, dV: a half-workgroup holds a block of 64 keys of one kv head, each wave 16 of them with their K

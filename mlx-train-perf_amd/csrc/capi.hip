@@ -632,16 +632,28 @@ int mtp_attn_scored_fwd(const void* q, const void* k, const void* v, int64_t b, 
 
 int mtp_attn_scored_fwd_f32(const float* q, const float* k, const float* v, int64_t b, int64_t hq, int64_t hkv, int64_t s,
                             int64_t dh, float scale, int32_t causal, float softcap, const float* slopes,
-                            const int32_t* span_start, const int32_t* span_end, float* o, float* lse, void* stream) {
+                            const int32_t* span_start, const int32_t* span_end, float* o, float* lse, void* workspace,
+                            size_t workspace_bytes, void* stream) {
   int rc = check_scored(q, k, v, b, hq, hkv, s, dh, scale, causal, softcap, slopes, span_start, span_end);
   if (rc) return rc;
   if (!o || !lse) return fail(MTP_ERR_INPUT, "o and lse must be non-null");
   if (!aligned16(o)) return fail(MTP_ERR_UNSUPPORTED, "o must be 16-byte aligned");
   mtp::AttnShape sh{(int)b, (int)hq, (int)hkv, (int)s, (int)dh, scale, (int)causal};
   mtp::AttnScore sc{softcap, slopes, span_start, span_end};
-  hipError_t e = mtp::launch_attn32_scored_fwd(sh, sc, q, k, v, o, lse, static_cast<hipStream_t>(stream));
+  if (!aligned16(workspace)) return fail(MTP_ERR_UNSUPPORTED, "workspace must be 16-byte aligned");
+  hipError_t e = mtp::launch_attn32_scored_fwd(sh, sc, q, k, v, o, lse, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return fail(MTP_ERR_RUNTIME, "fp32 scored attention forward launch failed: %s", hipGetErrorString(e));
   return ok();
+}
+
+size_t mtp_attn_scored_fwd_f32_workspace_bytes(int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh) {
+  if (b < 1 || hq < 1 || hkv < 1 || s < 1 || hq % hkv || b * hq * s > kMaxDim) return 0;
+  return mtp::attn32_scored_fwd_workspace((int)b, (int)hq, (int)hkv, (int)s, (int)dh);
+}
+
+size_t mtp_attn_scored_bwd_f32_workspace_bytes(int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh) {
+  if (b < 1 || hq < 1 || hkv < 1 || s < 1 || hq % hkv || b * hq * s > kMaxDim) return 0;
+  return mtp::attn32_scored_bwd_workspace((int)b, (int)hq, (int)hkv, (int)s, (int)dh);
 }
 
 size_t mtp_attn_scored_bwd_workspace_bytes(int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh) {
@@ -683,15 +695,14 @@ int mtp_attn_scored_bwd_f32(const float* q, const float* k, const float* v, cons
   if (!o || !lse || !d_o || !d_q || !d_k || !d_v) return fail(MTP_ERR_INPUT, "o, lse, d_o, d_q, d_k, d_v must be non-null");
   if (!aligned16(o) || !aligned16(d_o) || !aligned16(d_q) || !aligned16(d_k) || !aligned16(d_v))
     return fail(MTP_ERR_UNSUPPORTED, "o, d_o, d_q, d_k, d_v must be 16-byte aligned");
-  // D is all it needs; a workspace without room for the split's partials runs the dK/dV pass unsplit.
-  const size_t need = mtp::attn32_bwd_workspace((int)b, (int)hq, (int)hkv, (int)s, (int)dh, 1);
+  // D is all it needs; a pass without room for its partials runs unsplit.
+  const size_t need = (size_t)b * hq * s * sizeof(float);
   if (!workspace || workspace_bytes < need)
     return fail(MTP_ERR_WORKSPACE, "fp32 scored attention backward needs a workspace of %zu bytes (got %zu)", need, workspace ? workspace_bytes : (size_t)0);
+  if (!aligned16(workspace)) return fail(MTP_ERR_UNSUPPORTED, "workspace must be 16-byte aligned");
   mtp::AttnShape sh{(int)b, (int)hq, (int)hkv, (int)s, (int)dh, scale, (int)causal};
   mtp::AttnScore sc{softcap, slopes, span_start, span_end};
-  const bool split = workspace_bytes >= mtp_attn_bwd_f32_workspace_bytes(b, hq, hkv, s, dh);
-  const int ns = split ? mtp::attn32_dkv_splits(sh.b, sh.hq, sh.hkv, sh.s, sh.dh) : 1;
-  hipError_t e = mtp::launch_attn32_scored_bwd(sh, sc, q, k, v, o, lse, d_o, d_q, d_k, d_v, static_cast<float*>(workspace), ns,
+  hipError_t e = mtp::launch_attn32_scored_bwd(sh, sc, q, k, v, o, lse, d_o, d_q, d_k, d_v, workspace, workspace_bytes,
                                                static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return fail(MTP_ERR_RUNTIME, "fp32 scored attention backward launch failed: %s", hipGetErrorString(e));
   return ok();

@@ -741,8 +741,8 @@ template <int DH>
 hipError_t fwd32_dh(const AttnShape& sh, const float* q, const float* k, const float* v, const int32_t* sst, float* o,
                     float* lse, hipStream_t st) {
   const dim3 grid = grid32_q(sh), block(512);
-  if (sst) hipLaunchKernelGGL((attn32_q_kernel<DH, kMaskPacked, false>), grid, block, 0, st, q, k, v, nullptr, nullptr, nullptr, nullptr, sst, o, lse, sh.b, sh.hq, sh.hkv, sh.s, sh.scale, sh.causal, nullptr, 0.f, nullptr);
-  else hipLaunchKernelGGL((attn32_q_kernel<DH, kMaskPlain, false>), grid, block, 0, st, q, k, v, nullptr, nullptr, nullptr, nullptr, sst, o, lse, sh.b, sh.hq, sh.hkv, sh.s, sh.scale, sh.causal, nullptr, 0.f, nullptr);
+  if (sst) hipLaunchKernelGGL((attn32_q_kernel<DH, kMaskPacked, false>), grid, block, 0, st, q, k, v, nullptr, nullptr, nullptr, nullptr, sst, o, lse, sh.b, sh.hq, sh.hkv, sh.s, sh.scale, sh.causal, nullptr, 0.f, nullptr, 1, nullptr);
+  else hipLaunchKernelGGL((attn32_q_kernel<DH, kMaskPlain, false>), grid, block, 0, st, q, k, v, nullptr, nullptr, nullptr, nullptr, sst, o, lse, sh.b, sh.hq, sh.hkv, sh.s, sh.scale, sh.causal, nullptr, 0.f, nullptr, 1, nullptr);
   return hipGetLastError();
 }
 template <int DH>
@@ -750,8 +750,8 @@ hipError_t bwd32_dh(const AttnShape& sh, const float* q, const float* k, const f
                     const float* lse, const float* d_o, const int32_t* sst, float* dq, float* dk, float* dv,
                     float* dvec, int ns, hipStream_t st) {
   const dim3 qgrid = grid32_q(sh), block(512);
-  if (sst) hipLaunchKernelGGL((attn32_q_kernel<DH, kMaskPacked, true>), qgrid, block, 0, st, q, k, v, d_o, o, lse, dvec, sst, dq, nullptr, sh.b, sh.hq, sh.hkv, sh.s, sh.scale, sh.causal, nullptr, 0.f, nullptr);
-  else hipLaunchKernelGGL((attn32_q_kernel<DH, kMaskPlain, true>), qgrid, block, 0, st, q, k, v, d_o, o, lse, dvec, sst, dq, nullptr, sh.b, sh.hq, sh.hkv, sh.s, sh.scale, sh.causal, nullptr, 0.f, nullptr);
+  if (sst) hipLaunchKernelGGL((attn32_q_kernel<DH, kMaskPacked, true>), qgrid, block, 0, st, q, k, v, d_o, o, lse, dvec, sst, dq, nullptr, sh.b, sh.hq, sh.hkv, sh.s, sh.scale, sh.causal, nullptr, 0.f, nullptr, 1, nullptr);
+  else hipLaunchKernelGGL((attn32_q_kernel<DH, kMaskPlain, true>), qgrid, block, 0, st, q, k, v, d_o, o, lse, dvec, sst, dq, nullptr, sh.b, sh.hq, sh.hkv, sh.s, sh.scale, sh.causal, nullptr, 0.f, nullptr, 1, nullptr);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   float* part = reinterpret_cast<float*>(((uintptr_t)(dvec + (size_t)sh.b * sh.hq * sh.s) + 255) / 256 * 256);

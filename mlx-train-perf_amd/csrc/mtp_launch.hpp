@@ -103,11 +103,14 @@ hipError_t launch_attn_scored_fwd(const AttnShape& sh, const AttnScore& sc, cons
 hipError_t launch_attn_scored_bwd(const AttnShape& sh, const AttnScore& sc, const bf16_t* q, const bf16_t* k,
                                   const bf16_t* v, const bf16_t* o, const float* lse, const bf16_t* d_o, bf16_t* dq,
                                   bf16_t* dk, bf16_t* dv, void* workspace, hipStream_t stream);
+// Workspaces of the fp32 passes; less than that (the backward: at least D) runs what lacks room unsplit.
+size_t attn32_scored_fwd_workspace(int b, int hq, int hkv, int s, int dh);
+size_t attn32_scored_bwd_workspace(int b, int hq, int hkv, int s, int dh);
 hipError_t launch_attn32_scored_fwd(const AttnShape& sh, const AttnScore& sc, const float* q, const float* k,
-                                    const float* v, float* o, float* lse, hipStream_t stream);
+                                    const float* v, float* o, float* lse, void* workspace, size_t bytes, hipStream_t stream);
 hipError_t launch_attn32_scored_bwd(const AttnShape& sh, const AttnScore& sc, const float* q, const float* k,
                                     const float* v, const float* o, const float* lse, const float* d_o, float* dq,
-                                    float* dk, float* dv, float* dvec, int nsplit, hipStream_t stream);
+                                    float* dk, float* dv, void* workspace, size_t bytes, hipStream_t stream);
 
 // fp32 inputs (f32_kernels.hip): fp32 MFMA products, fp32 outputs and gradients.
 struct LceHead32 {

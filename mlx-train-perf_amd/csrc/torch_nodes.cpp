@@ -45,6 +45,7 @@ struct Entries {
   decltype(&mtp_attn_scored_fwd) scored_fwd = nullptr;
   decltype(&mtp_attn_scored_bwd) scored_bwd = nullptr;
   decltype(&mtp_attn_scored_bwd_workspace_bytes) scored_ws = nullptr;
+  decltype(&mtp_attn_scored_fwd_f32_workspace_bytes) scored_fwd_ws32 = nullptr, scored_bwd_ws32 = nullptr;
   decltype(&mtp_attn_scored_fwd_f32) scored_fwd32 = nullptr;
   decltype(&mtp_attn_scored_bwd_f32) scored_bwd32 = nullptr;
   decltype(&mtp_pref_fwd) pref_fwd = nullptr;
@@ -170,13 +171,16 @@ struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
     const int64_t b = q.size(0), hq = q.size(1), s = q.size(2), dh = q.size(3), hkv = k.size(1);
     const at::Tensor o = at::empty_like(q), lse = at::empty({b, hq, s}, q.options().dtype(at::kFloat));
     const float cap = (float)score.softcap;
-    if (q.scalar_type() == at::kFloat)
+    if (q.scalar_type() == at::kFloat) {
+      const size_t bytes = g_api.scored_fwd_ws32(b, hq, hkv, s, dh);
+      const at::Tensor ws = bytes ? at::empty({(int64_t)bytes}, q.options().dtype(at::kByte)) : at::Tensor();
       check(g_api.scored_fwd32(ptr<float>(q), ptr<float>(k), ptr<float>(v), b, hq, hkv, s, dh, (float)scale, causal, cap,
                                floats(score.slopes), ints(score.start), ints(score.end), ptr<float>(o), ptr<float>(lse),
-                               stream_of(q)));
-    else
+                               opt_ptr(ws), bytes, stream_of(q)));
+    } else {
       check(g_api.scored_fwd(ptr(q), ptr(k), ptr(v), b, hq, hkv, s, dh, (float)scale, causal, cap, floats(score.slopes),
                              ints(score.start), ints(score.end), ptr(o), ptr<float>(lse), stream_of(q)));
+    }
     ctx->save_for_backward({q, k, v, o, lse, score.slopes, score.start, score.end});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["causal"] = causal;
@@ -198,7 +202,7 @@ struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
     const int64_t b = q.size(0), hq = q.size(1), s = q.size(2), dh = q.size(3), hkv = k.size(1);
     const bool f32 = q.scalar_type() == at::kFloat;
     const at::Tensor dq = at::empty_like(q), dk = at::empty_like(k), dv = at::empty_like(v);
-    const size_t bytes = (f32 ? g_api.ws32 : g_api.scored_ws)(b, hq, hkv, s, dh);
+    const size_t bytes = (f32 ? g_api.scored_bwd_ws32 : g_api.scored_ws)(b, hq, hkv, s, dh);
     const at::Tensor ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
     if (f32)
       check(g_api.scored_bwd32(ptr<float>(q), ptr<float>(k), ptr<float>(v), ptr<float>(o), ptr<float>(lse), ptr<float>(d_o), b,
@@ -550,6 +554,8 @@ void bind(const py::dict& entries, py::object check_fn) {
   set(g_api.scored_fwd, "mtp_attn_scored_fwd");
   set(g_api.scored_bwd, "mtp_attn_scored_bwd");
   set(g_api.scored_ws, "mtp_attn_scored_bwd_workspace_bytes");
+  set(g_api.scored_fwd_ws32, "mtp_attn_scored_fwd_f32_workspace_bytes");
+  set(g_api.scored_bwd_ws32, "mtp_attn_scored_bwd_f32_workspace_bytes");
   set(g_api.scored_fwd32, "mtp_attn_scored_fwd_f32");
   set(g_api.scored_bwd32, "mtp_attn_scored_bwd_f32");
   set(g_api.pref_fwd, "mtp_pref_fwd");

@@ -278,11 +278,16 @@ def scored_forward(q, k, v, slopes, start, end, *, scale: float, causal: bool, s
     b, hq, n, dh = q.shape
     o = torch.empty_like(q)
     lse = torch.empty((b, hq, n), dtype=torch.float32, device=q.device)
-    fwd = lib.mtp_attn_scored_fwd_f32 if q.dtype == torch.float32 else lib.mtp_attn_scored_fwd
+    shape = (b, hq, k.shape[1], n, dh)
+    args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), *shape, scale, int(causal), softcap, _native.ptr(slopes), _native.ptr(start),
+            _native.ptr(end), o.data_ptr(), lse.data_ptr())
     with _native.on_device(q):
-        rc = fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), b, hq, k.shape[1], n, dh, scale, int(causal), softcap,
-                 _native.ptr(slopes), _native.ptr(start), _native.ptr(end), o.data_ptr(), lse.data_ptr(),
-                 _native.stream_of(q))
+        if q.dtype == torch.float32:
+            ws_bytes = lib.mtp_attn_scored_fwd_f32_workspace_bytes(*shape)
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+            rc = lib.mtp_attn_scored_fwd_f32(*args, _native.ptr(ws), ws_bytes, _native.stream_of(q))
+        else:
+            rc = lib.mtp_attn_scored_fwd(*args, _native.stream_of(q))
     _native.check(rc, domain="attention")
     return o, lse
 
@@ -294,7 +299,7 @@ def scored_backward(q, k, v, o, lse, d_o, slopes, start, end, *, scale: float, c
     hkv = k.shape[1]
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
     f32 = q.dtype == torch.float32
-    ws_bytes = (lib.mtp_attn_bwd_f32_workspace_bytes if f32 else lib.mtp_attn_scored_bwd_workspace_bytes)(b, hq, hkv, n, dh)
+    ws_bytes = (lib.mtp_attn_scored_bwd_f32_workspace_bytes if f32 else lib.mtp_attn_scored_bwd_workspace_bytes)(b, hq, hkv, n, dh)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
     bwd = lib.mtp_attn_scored_bwd_f32 if f32 else lib.mtp_attn_scored_bwd
     with _native.on_device(q):

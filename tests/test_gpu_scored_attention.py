@@ -261,3 +261,38 @@ def test_offsets_past_32_bits():
     for name, a, x in zip(("o", "dq", "dk", "dv"), (o, dq, dk, dv), want):
         assert S.rel(a[:, -1:, -tail:], x[:, :, -tail:]) <= 1e-2, name
     assert not dq[:, :-1].any() and not dk[:, :-1].any() and not dq[:, -1, :-tail].any()
+
+
+@pytest.mark.parametrize("dh", [64, 96, 128])
+@pytest.mark.parametrize(("mask", "cap", "biased"), [("causal", 30.0, True), ("full", None, True), ("docs", 9.0, False),
+                                                     ("ragged", None, False), ("window", 80.0, True)])
+def test_fp32_passes_split_over_the_keys(dh, mask, cap, biased):
+    """Few workgroups: the forward and dQ are split, and their parts (some without a key of a row) joined."""
+    from mlx_train_perf import _native
+
+    assert _native.load().mtp_attn_scored_fwd_f32_workspace_bytes(1, 4, 2, 777, dh) > 0
+    _check(1, 4, 2, 777, dh, mask=mask, cap=cap, biased=biased, dtype=torch.float32, seed=dh)
+
+
+def test_fp32_without_room_for_parts():
+    """No workspace in the forward, D's alone in the backward: unsplit, the same sums in another order."""
+    from mlx_train_perf import _native
+    from mlx_train_perf.attention.api import scored_backward, scored_forward
+
+    lib = _native.load()
+    b, hq, hkv, s, dh = 1, 4, 2, 600, 64
+    q, k, v, d_o = (x.cuda() for x in S.inputs(b, hq, hkv, s, dh, torch.float32, 3))
+    slopes = S.slopes_of(hq).cuda()
+    args = {"scale": 0.125, "causal": True, "softcap": 9.0}
+    o, lse = scored_forward(q, k, v, slopes, None, None, **args)
+    grads = scored_backward(q, k, v, o, lse, d_o, slopes, None, None, **args)
+    o1, lse1 = torch.empty_like(o), torch.empty_like(lse)
+    outs = [torch.empty_like(x) for x in (q, k, v)]
+    ws = torch.empty(b * hq * s, device="cuda")
+    st = _native.stream_of(q)
+    common = (b, hq, hkv, s, dh, 0.125, 1, 9.0, slopes.data_ptr(), None, None)
+    assert lib.mtp_attn_scored_fwd_f32(q.data_ptr(), k.data_ptr(), v.data_ptr(), *common, o1.data_ptr(), lse1.data_ptr(), None, 0, st) == 0
+    assert lib.mtp_attn_scored_bwd_f32(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), d_o.data_ptr(), *common,
+                                       *(x.data_ptr() for x in outs), ws.data_ptr(), ws.numel() * 4, st) == 0
+    for a, c in zip((o1, lse1, *outs), (o, lse, *grads)):
+        assert S.rel(a, c) <= 2 * BAR[torch.float32]

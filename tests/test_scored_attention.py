@@ -136,7 +136,8 @@ def test_c_abi_refusals():
     p, none, shape = 1 << 20, None, (1, 2, 1, 8, 64)
 
     def fwd(scale=1.0, causal=0, cap=1.0, slopes=none, start=none, end=none, q=p, o=p, shape=shape, lib_fn=lib.mtp_attn_scored_fwd):
-        return lib_fn(q, p, p, *shape, scale, causal, cap, slopes, start, end, o, p, none)
+        ws = (none, 0) if lib_fn is lib.mtp_attn_scored_fwd_f32 else ()
+        return lib_fn(q, p, p, *shape, scale, causal, cap, slopes, start, end, o, p, *ws, none)
 
     bad, un = _native.MTP_ERR_INPUT, _native.MTP_ERR_UNSUPPORTED
     for fn in (lib.mtp_attn_scored_fwd, lib.mtp_attn_scored_fwd_f32):
@@ -159,3 +160,8 @@ def test_c_abi_refusals():
     assert bwd(ws - 1) == _native.MTP_ERR_WORKSPACE and bwd(ws, workspace=none) == _native.MTP_ERR_WORKSPACE
     assert bwd(ws, workspace=p + 4) == un and bwd(ws, d_o=none) == bad
     assert bwd(8, fn=lib.mtp_attn_scored_bwd_f32) == _native.MTP_ERR_WORKSPACE
+    # fp32: parts of 4 splits of one pair of 64-query blocks of 8 heads (64 workgroups), 33 tiles of 32 keys
+    assert lib.mtp_attn_scored_fwd_f32_workspace_bytes(1, 8, 2, 1000, 128) == 4 * 8 * 1000 * 130 * 4
+    assert lib.mtp_attn_scored_fwd_f32_workspace_bytes(1, 32, 8, 8192, 128) == 0    # enough workgroups
+    assert lib.mtp_attn_scored_fwd_f32_workspace_bytes(1, 1, 1, 100, 64) == 0       # too few tiles
+    assert lib.mtp_attn_scored_bwd_f32_workspace_bytes(1, 8, 2, 1000, 128) >= 8000 * 4 + 4 * 8 * 1000 * 128 * 4
