@@ -1,5 +1,6 @@
 """Trainer adapter for torch causal LMs: `split_model`, `make_loss_fn`, `make_packed_loss_fn`
-(the torch counterpart of src/mlx_train_perf/adapters/mlx_lm.py:140-297).
+(the torch counterpart of src/mlx_train_perf/adapters/mlx_lm.py:140-297), and beyond the reference
+`make_token_nll_fn`, `make_preference_loss_fn` and `make_policy_loss_fn` for steps on preferences and rewards.
 
 Loss contract (the mlx-lm trainer's `default_loss`, quoted at adapters/mlx_lm.py:5-20):
 inputs = batch[:, :-1], targets = batch[:, 1:], steps = 1..T, mask = (steps >= lengths[:, 0]) &
@@ -22,8 +23,9 @@ from typing import Any, Literal
 import torch
 from torch import nn
 
-from mlx_train_perf.attention.segments import PackedMask
+from mlx_train_perf.attention.segments import PackedMask, SpanMask
 from mlx_train_perf.core.loss import DenseHead, HeadRef, linear_cross_entropy, resolve_impl, tied_head
+from mlx_train_perf.core.preference import PolicyLoss, PreferenceLoss, policy_loss, preference_loss
 from mlx_train_perf.errors import AdapterError
 
 _Impl = Literal["auto", "kernel", "chunked", "naive"]
@@ -109,5 +111,73 @@ def make_packed_loss_fn(model: Any, *, impl: _Impl = "auto", allow_unverified_ml
         ntoks = loss_mask.sum()
         loss = (nll * loss_mask).to(torch.float32).sum() / ntoks
         return loss, ntoks
+
+    return loss_fn
+
+
+def make_token_nll_fn(model: Any, *, impl: _Impl = "auto",
+                      allow_unverified_mlx: bool = False) -> Callable[..., torch.Tensor]:
+    """`nll(model, batch, spans=None) -> (B, T)`, the per-token losses of the targets batch[:, 1:]: what the losses
+    below take from frozen models (call it under `torch.no_grad()` for those). `spans`: a `SpanMask` over the inputs
+    batch[:, :-1], handed to every attention call; requires `enable_flash_attention(model)`."""
+    from mlx_train_perf.attention.wrapper import is_enabled  # noqa: PLC0415
+
+    split_model(model)
+    cfg = getattr(model, "config", None)
+    if getattr(cfg, "final_logit_softcapping", None) is not None:
+        raise AdapterError("the fused loss does not cap logits (config.final_logit_softcapping is set)")
+
+    def nll_fn(model_arg: Any, batch: torch.Tensor, spans: SpanMask | None = None) -> torch.Tensor:
+        trunk, head = split_model(model_arg)
+        if spans is not None and not is_enabled(model_arg):
+            raise AdapterError("spans require enable_flash_attention(model) first")
+        hidden = trunk(batch[:, :-1], **({} if spans is None else {"mtp_spans": spans}))
+        return linear_cross_entropy(hidden, head, batch[:, 1:], impl=impl, reduction="none", validate_targets=False,
+                                    allow_unverified_mlx=allow_unverified_mlx).to(torch.float32)
+
+    return nll_fn
+
+
+def _target_mask(lengths: torch.Tensor, t: int) -> torch.Tensor:
+    """The trainer's mask of `make_loss_fn`: targets at steps offset .. length of each row."""
+    steps = torch.arange(1, t + 1, device=lengths.device)
+    return (steps >= lengths[:, 0:1]) & (steps <= lengths[:, 1:])
+
+
+def _row_loss_impl(impl: str) -> Literal["auto", "reference"]:
+    return "reference" if impl in ("naive", "chunked") else "auto"
+
+
+def make_preference_loss_fn(model: Any, *, beta: float = 0.1, kind: Literal["sigmoid", "hinge", "ipo"] = "sigmoid",
+                            label_smoothing: float = 0.0, impl: _Impl = "auto",
+                            allow_unverified_mlx: bool = False) -> Callable[..., PreferenceLoss]:
+    """`loss(model, batch, lengths, ref_nll, spans=None) -> PreferenceLoss`: `batch` (2P, T + 1) holds the P chosen
+    answers, then the P rejected ones; `lengths` (2P, 2) as in `make_loss_fn` (the answer's first and last step);
+    `ref_nll` (2P, T) is the reference model's `make_token_nll_fn` of the same batch."""
+    nll_fn = make_token_nll_fn(model, impl=impl, allow_unverified_mlx=allow_unverified_mlx)
+
+    def loss_fn(model_arg: Any, batch: torch.Tensor, lengths: torch.Tensor, ref_nll: torch.Tensor,
+                spans: SpanMask | None = None) -> PreferenceLoss:
+        nll = nll_fn(model_arg, batch, spans)
+        return preference_loss(nll, ref_nll, mask=_target_mask(lengths, nll.shape[1]), beta=beta, kind=kind,
+                               label_smoothing=label_smoothing, impl=_row_loss_impl(impl))
+
+    return loss_fn
+
+
+def make_policy_loss_fn(model: Any, *, clip_low: float = 0.2, clip_high: float = 0.2, kl_coef: float = 0.0,
+                        reduction: Literal["token", "sequence"] = "token", impl: _Impl = "auto",
+                        allow_unverified_mlx: bool = False) -> Callable[..., PolicyLoss]:
+    """`loss(model, batch, lengths, old_nll, advantages, ref_nll=None, spans=None) -> PolicyLoss`: `old_nll` (B, T) is
+    the sampling model's `make_token_nll_fn` of the batch, `advantages` (B,) or (B, T), `lengths` as in
+    `make_loss_fn`."""
+    nll_fn = make_token_nll_fn(model, impl=impl, allow_unverified_mlx=allow_unverified_mlx)
+
+    def loss_fn(model_arg: Any, batch: torch.Tensor, lengths: torch.Tensor, old_nll: torch.Tensor, advantages: torch.Tensor,
+                ref_nll: torch.Tensor | None = None, spans: SpanMask | None = None) -> PolicyLoss:
+        nll = nll_fn(model_arg, batch, spans)
+        return policy_loss(nll, old_nll, advantages, ref_nll=ref_nll, mask=_target_mask(lengths, nll.shape[1]),
+                           clip_low=clip_low, clip_high=clip_high, kl_coef=kl_coef, reduction=reduction,
+                           impl=_row_loss_impl(impl))
 
     return loss_fn

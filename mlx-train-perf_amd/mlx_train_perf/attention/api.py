@@ -24,7 +24,7 @@ from torch.autograd.function import once_differentiable
 
 from mlx_train_perf import _compat, _native
 from mlx_train_perf.attention.reference import flash_attention_reference, hide, kv_head_for, scores_of
-from mlx_train_perf.attention.segments import PackedMask, SpanMask, layout_violation, packed_as_spans, span_violation
+from mlx_train_perf.attention.segments import PackedMask, SpanMask, layout_violation, packed_as_spans
 from mlx_train_perf.errors import AttentionInputError, UnsupportedAttentionError
 
 _KERNEL_DTYPES = (torch.bfloat16, torch.float32)   # the reference kernel's T (api.py:41-43)
@@ -109,7 +109,7 @@ def _validate_score(q: torch.Tensor, softcap: float | None, slopes: torch.Tensor
             if t.dtype.is_floating_point or t.dtype == torch.bool or t.dtype.is_complex:
                 raise AttentionInputError(f"spans.{name} must be an integer tensor; got {t.dtype}")
         if check_spans:
-            problem = span_violation(spans)
+            problem = spans.violation()
             if problem is not None:
                 raise AttentionInputError(f"spans violate their contract: {problem}")
 
@@ -369,7 +369,7 @@ def flash_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale:
     from the score of query i and key j (after the cap); they get no gradient. `spans`: a `SpanMask`, the keys that
     each query sees; it is the whole mask, so `causal` has no say beside it and `segments` may not be given (cap and
     slopes go with either). A query that sees nothing gets zeros and no gradient. `validate_segments` checks the
-    contract of `spans` too, at one host sync a call."""
+    contract of `spans` too, at one host sync a mask."""
     resolved = resolve_attention_impl(q, k, v, impl=impl, causal=causal, segments=segments,
                                       validate_segments=validate_segments, softcap=softcap, slopes=slopes, spans=spans)
     scored = softcap is not None or slopes is not None or spans is not None

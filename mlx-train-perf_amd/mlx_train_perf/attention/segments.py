@@ -3,7 +3,7 @@ src/mlx_train_perf/attention/segments.py:9-29), plus the checks of its layout co
 gives every query a range of keys (prompts as prefixes, whole documents, windows), with its builders."""
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import torch
 
@@ -68,9 +68,23 @@ class SpanMask:
 
     Neither tensor may decrease along a row, and both lie in [0, N]. A query whose range holds nothing (padding)
     gets an output of zeros and takes part in no gradient. A window of w keys is start = i - w + 1, end = i + 1.
+
+    A mask remembers that its contract was checked (a host sync), for as long as neither tensor is written to, so that
+    a model's layers check the mask of a step once.
     """
     start: torch.Tensor
     end: torch.Tensor
+    _checked: list = field(default_factory=list, init=False, repr=False, compare=False)
+
+    def violation(self) -> str | None:
+        """`span_violation` of this mask, unless it was found to be none before."""
+        versions = [self.start._version, self.end._version]
+        if self._checked == versions:
+            return None
+        problem = span_violation(self)
+        if problem is None:
+            self._checked[:] = versions
+        return problem
 
 
 def _lengths(values: torch.Tensor | list[int], device: torch.device | None) -> torch.Tensor:

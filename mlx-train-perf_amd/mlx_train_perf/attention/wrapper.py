@@ -8,11 +8,13 @@ Two model shapes are served:
   and selected on the model config. Every decoder layer keeps its own projections, rotary
   embedding and (Qwen3) q/k norms; only the single attention call changes, exactly the seam the
   reference swaps (wrapper.py:126-157). A packed batch passes its `PackedMask` as the
-  `mtp_segments=` keyword of the model call; transformers forwards it to every layer.
+  `mtp_segments=` keyword of the model call, prompts as prefixes or other ranges of keys a `SpanMask` as
+  `mtp_spans=`; transformers forwards them to every layer. A layer that caps its scores passes the cap itself.
 - **mlx-lm-style modules**: layers whose `self_attn` has `q_proj/k_proj/v_proj/o_proj`, a `rope`
   callable, `n_heads`, `n_kv_heads`, `scale` (and optionally `q_norm/k_norm`) are wrapped in
   `FlashAttentionWrapper`, which holds the original submodules under their original names (so
-  LoRA injection by module path keeps working, wrapper.py:17-31) and reproduces the stock call.
+  LoRA injection by module path keeps working, wrapper.py:17-31) and reproduces the stock call, with the
+  module's `attn_logit_softcapping` where it has one.
 
 Refusals (`UnsupportedAttentionError`, at enable time): sliding-window or mixed `layer_types`,
 configured attention dropout, head_dim outside {64, 96, 128}, an unrecognised model shape.
@@ -28,7 +30,7 @@ import torch
 from torch import nn
 
 from mlx_train_perf.attention.api import flash_attention
-from mlx_train_perf.attention.segments import PackedMask
+from mlx_train_perf.attention.segments import PackedMask, SpanMask
 from mlx_train_perf.errors import AttentionInputError, UnsupportedAttentionError
 from mlx_train_perf.plan import launch as _plan
 
@@ -36,10 +38,10 @@ _KERNEL_HEAD_DIMS: tuple[int, ...] = (64, 96, 128)
 IMPL_NAME = "mtp_hip_attention"  # no "flash" in the name: transformers routes such names to its kernel hub
 
 
-def _resolve_mask(mask: Any) -> bool | PackedMask:
+def _resolve_mask(mask: Any) -> bool | PackedMask | SpanMask:
     """Map a caller's mask onto `flash_attention` (wrapper.py:72-96): "causal"/None -> causal,
-    a PackedMask passes through, anything else (array / additive / sliding masks) is refused."""
-    if isinstance(mask, PackedMask):
+    a PackedMask or SpanMask passes through, anything else (array / additive / sliding masks) is refused."""
+    if isinstance(mask, (PackedMask, SpanMask)):
         return mask
     if isinstance(mask, str):
         if mask == "causal":
@@ -92,9 +94,10 @@ def _hf_mask(batch_size: int, q_length: int, kv_length: int, q_offset: int = 0, 
 
 def _hf_flash_attention(module: nn.Module, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
                         attention_mask: Any, scaling: float, dropout: float = 0.0,
-                        mtp_segments: PackedMask | None = None, **kwargs: Any):
+                        mtp_segments: PackedMask | None = None, mtp_spans: SpanMask | None = None,
+                        softcap: float | None = None, **kwargs: Any):
     """transformers attention-interface function: q (B,Hq,S,D), k/v (B,Hkv,S,D) post-RoPE;
-    returns (output (B,S,Hq,D), None)."""
+    returns (output (B,S,Hq,D), None). `softcap`: what layers with capped scores pass."""
     if dropout:
         raise UnsupportedAttentionError("flash-attention training path does not support attention dropout")
     if attention_mask is not None:
@@ -104,7 +107,8 @@ def _hf_flash_attention(module: nn.Module, query: torch.Tensor, key: torch.Tenso
             "an explicit attention mask was given"
         raise AttentionInputError(f"the flash-attention path cannot honour this mask: {reason}")
     impl = getattr(module.config, "_mtp_flash_impl", "auto")
-    out = flash_attention(query, key, value, scale=float(scaling), causal=True, impl=impl, segments=mtp_segments)
+    out = flash_attention(query, key, value, scale=float(scaling), causal=True, impl=impl, segments=mtp_segments,
+                          softcap=softcap, spans=mtp_spans)
     return out.transpose(1, 2).contiguous(), None
 
 
@@ -127,6 +131,7 @@ class FlashAttentionWrapper(nn.Module):
         self.n_heads = original.n_heads
         self.n_kv_heads = original.n_kv_heads
         self.scale = original.scale
+        self.softcap = getattr(original, "attn_logit_softcapping", None)
         self._impl = impl
 
     def forward(self, x: torch.Tensor, mask: Any = None, cache: Any = None) -> torch.Tensor:
@@ -146,8 +151,9 @@ class FlashAttentionWrapper(nn.Module):
         keys = self.rope(keys)
         resolved = _resolve_mask(mask)
         segments = resolved if isinstance(resolved, PackedMask) else None
-        out = flash_attention(queries, keys, values, scale=self.scale, causal=True, segments=segments,
-                              impl=self._impl)  # type: ignore[arg-type]
+        spans = resolved if isinstance(resolved, SpanMask) else None
+        out = flash_attention(queries, keys, values, scale=self.scale, causal=True, segments=segments, spans=spans,
+                              softcap=self.softcap, impl=self._impl)  # type: ignore[arg-type]
         return self.o_proj(out.transpose(1, 2).reshape(b, length, -1))
 
 
@@ -196,7 +202,7 @@ def _model_device_dtype(model: Any) -> tuple[torch.device, torch.dtype] | None:
 
 
 def _prewarm(model: Any, *, impl: str, seq_len: int, batch_size: int, hq: int, hkv: int, head_dim: int,
-             packed: bool) -> None:
+             packed: bool, softcap: float | None = None) -> None:
     """One zeros forward + backward at the training shape (the counterpart of the reference's
     `_prewarm_rate_caches`, wrapper.py:170-202), so the first training step does not pay for loading
     the kernels' code objects; with `packed`, a second one with a single-segment `PackedMask`, which
@@ -214,7 +220,8 @@ def _prewarm(model: Any, *, impl: str, seq_len: int, batch_size: int, hq: int, h
         z = torch.zeros((batch_size, seq_len), dtype=torch.int32, device=dev)
         masks.append(PackedMask(seg_id=z, seg_start=z))
     for seg in masks:
-        out = flash_attention(q, k, v, scale=1.0 / head_dim ** 0.5, causal=True, impl=impl, segments=seg)  # type: ignore[arg-type]
+        out = flash_attention(q, k, v, scale=1.0 / head_dim ** 0.5, causal=True, impl=impl, segments=seg,  # type: ignore[arg-type]
+                              softcap=softcap)
         out.backward(torch.zeros_like(out))
 
 
@@ -265,7 +272,7 @@ def enable_flash_attention(model: Any, *, impl: str = "auto", seq_len: int | Non
         head_dim = _head_dim(cfg)
         _plan.attn_plan(b=batch_size, hq=hq, hkv=hkv, s=seq_len, dh=head_dim)
         _prewarm(model, impl=impl, seq_len=seq_len, batch_size=batch_size, hq=hq, hkv=hkv, head_dim=head_dim,
-                 packed=packed)
+                 packed=packed, softcap=getattr(cfg, "attn_logit_softcapping", None))
 
 
 def is_enabled(model: Any) -> bool:
