@@ -329,7 +329,7 @@ int mtp_attn_scored_bwd_f32(const float* q, const float* k, const float* v, cons
  *
  * nll, old_nll, ref_nll: fp32 [n], the per-token losses of the model and of frozen ones (mtp_lce_fwd's nll).
  * Sequences: offsets int64 [sequences + 1], sequence r being the tokens [offsets[r], offsets[r + 1]); they
- * never decrease and lie in [0, n]; tokens of no sequence count nowhere and get a gradient of 0. NULL: the n
+ * never decrease and lie in [0, n], n <= 2^31 - 2048; tokens of no sequence count nowhere and get a gradient of 0. NULL: the n
  * tokens are rows of one length. mask: uint8 [n], or NULL; tokens with 0 count nowhere, whatever the tensors
  * hold there. Sums are in 64 bits, joined in a fixed order.
  * ------------------------------------------------------------------------------------------- */

@@ -39,6 +39,7 @@ int ok() {
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 constexpr int64_t kMaxDim = (int64_t(1) << 31) - 1;
+constexpr int64_t kMaxLossTokens = (int64_t(1) << 31) - 2048;  // a whole workgroup's tokens end below 2^31
 constexpr int64_t kTile = 256;
 
 size_t lce_fwd_ws(int64_t n, int64_t v) {
@@ -114,7 +115,7 @@ int check_scored(const void* q, const void* k, const void* v, int64_t b, int64_t
 // Rows and tokens of a preference or policy loss.
 int check_rows(int64_t rows, int64_t n, const int64_t* offsets) {
   if (rows < 1 || n < 1) return fail(MTP_ERR_INPUT, "the loss needs at least one sequence and one token (got %lld sequences, %lld tokens)", (long long)rows, (long long)n);
-  if (rows > (int64_t(1) << 24) || n > kMaxDim) return fail(MTP_ERR_INPUT, "at most 2^24 sequences and 2^31 - 1 tokens");
+  if (rows > (int64_t(1) << 24) || n > kMaxLossTokens) return fail(MTP_ERR_INPUT, "at most 2^24 sequences and 2^31 - 2048 tokens");
   if (!offsets && n % rows) return fail(MTP_ERR_INPUT, "without offsets the %lld tokens must be %lld rows of one length", (long long)n, (long long)rows);
   return MTP_OK;
 }
@@ -713,7 +714,7 @@ int mtp_attn_scored_bwd_f32(const float* q, const float* k, const float* v, cons
 // ---------------------------------------------------------------------------------------------
 
 size_t mtp_pref_workspace_bytes(int64_t pairs, int64_t n) {
-  return pairs < 1 || pairs > (int64_t(1) << 23) || n < 1 || n > kMaxDim ? 0 : mtp::pref_workspace((long)pairs, (long)n);
+  return pairs < 1 || pairs > (int64_t(1) << 23) || n < 1 || n > kMaxLossTokens ? 0 : mtp::pref_workspace((long)pairs, (long)n);
 }
 
 int mtp_pref_fwd(const float* nll, const float* ref_nll, const uint8_t* mask, const int64_t* offsets, int64_t pairs, int64_t n,
@@ -753,7 +754,7 @@ int mtp_pref_bwd(const float* d_loss, const float* coef, const uint8_t* mask, co
 }
 
 size_t mtp_policy_workspace_bytes(int64_t rows, int64_t n) {
-  return rows < 1 || rows > (int64_t(1) << 24) || n < 1 || n > kMaxDim ? 0 : mtp::policy_workspace((long)rows, (long)n);
+  return rows < 1 || rows > (int64_t(1) << 24) || n < 1 || n > kMaxLossTokens ? 0 : mtp::policy_workspace((long)rows, (long)n);
 }
 
 int mtp_policy_fwd(const float* nll, const float* old_nll, const float* ref_nll, const float* advantages,

@@ -169,3 +169,16 @@ def test_c_abi_refusals():
         assert policy(**kw) == bad, kw
     assert policy(ws=0) == ws_rc
     assert lib.mtp_policy_bwd(p, p, p, None, p, 0, None, None, 4, 8, 0.2, 0.2, 0.1, 1, p, p, None) == bad
+
+
+def test_c_abi_refuses_tokens_that_end_past_32_bits():
+    """A workgroup takes 2048 tokens and counts them in 32 bits, those behind the last one too."""
+    lib = _native.load()
+    p, n, rows = 1 << 20, (1 << 31) - 2048, 1 << 10
+    assert lib.mtp_pref_workspace_bytes(rows // 2, n) > 0 and lib.mtp_policy_workspace_bytes(rows, n) > 0
+    for more in (n + rows, (1 << 31) - rows):
+        assert lib.mtp_pref_workspace_bytes(rows // 2, more) == 0 and lib.mtp_policy_workspace_bytes(rows, more) == 0
+        assert lib.mtp_pref_fwd(p, p, None, None, rows // 2, more, 0, 0.1, 0.0, 1, p, p, p, p, 1 << 40, None) == _native.MTP_ERR_INPUT
+        assert lib.mtp_pref_bwd(p, p, None, None, rows // 2, more, 1, p, None) == _native.MTP_ERR_INPUT
+        assert lib.mtp_policy_fwd(p, p, None, p, 0, None, None, rows, more, 0.2, 0.2, 0.0, 1, p, p, p, p, 1 << 40, None) == _native.MTP_ERR_INPUT
+        assert lib.mtp_policy_bwd(p, p, p, None, p, 0, None, None, rows, more, 0.2, 0.2, 0.0, 1, p, p, None) == _native.MTP_ERR_INPUT
