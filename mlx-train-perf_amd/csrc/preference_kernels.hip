@@ -252,7 +252,8 @@ __device__ __forceinline__ void pref_join(const PrefPart* part, const Seqs& q, c
     double l, slope;
     if (p.kind == kPrefSigmoid) {
       const float x = (float)d;
-      l = (1.0 - p.smoothing) * softplus(-x) + p.smoothing * softplus(x);
+      l = (1.0 - p.smoothing) * softplus(-x);
+      if (p.smoothing != 0.0) l += p.smoothing * softplus(x);  // 0 of an infinite one is 0
       slope = p.smoothing - 1.f / (1.f + expf(x));
     } else if (p.kind == kPrefHinge) {
       l = d < 1.0 ? 1.0 - d : d >= 1.0 ? 0.0 : d;  // NaN stays
@@ -337,8 +338,10 @@ __device__ __forceinline__ PolicyToken policy_token(const PolicyLoss& p, float n
   const double s = (double)old - (double)nll;
   const float ratio = expf((float)s);
   k.clipped = adv > 0.f ? s > p.log_high : adv < 0.f ? s < p.log_low : false;
-  k.loss = -(k.clipped ? (adv > 0.f ? p.edge_high : p.edge_low) : ratio) * adv;
-  k.slope = k.clipped ? 0.f : ratio * adv;
+  // An advantage of 0 leaves nothing of a ratio that overflows either.
+  const bool flat = k.clipped || adv == 0.f;
+  k.loss = -(flat ? (adv > 0.f ? p.edge_high : p.edge_low) : ratio) * adv;
+  k.slope = flat ? 0.f : ratio * adv;
   k.kl = 0.f;
   if (p.has_ref) {
     const float d = nll - ref, em1 = expm1f(d);

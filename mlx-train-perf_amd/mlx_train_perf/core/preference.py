@@ -225,7 +225,9 @@ def _reference_preference(nll, ref_nll, offsets, mask, rows, kind, beta, smoothi
     chosen, rejected = (beta * ratio).reshape(2, -1)
     d = chosen - rejected
     if kind == "sigmoid":
-        loss = (1 - smoothing) * torch.nn.functional.softplus(-d) + smoothing * torch.nn.functional.softplus(d)
+        loss = (1 - smoothing) * torch.nn.functional.softplus(-d)
+        if smoothing:   # 0 of an infinite one is 0
+            loss = loss + smoothing * torch.nn.functional.softplus(d)
     elif kind == "hinge":
         loss = torch.relu(1 - d)
     else:
@@ -245,11 +247,11 @@ def _reference_policy(nll, old_nll, ref_nll, adv, offsets, mask, rows, clip_low,
     x = at(flat)
     a = at(adv) if adv.shape == nll.shape else torch.where(keep, adv.double()[owner.clamp(max=rows - 1)], 0.0)
     step = at(old_nll) - x
-    ratio = torch.exp(step)
     clipped = torch.where(a > 0, step > math.log1p(clip_high),
                           step < (math.log1p(-clip_low) if clip_low < 1 else -math.inf)) & (a != 0)
     edge = torch.where(a > 0, torch.full_like(a, 1 + clip_high), 1 - clip_low)
-    loss = -torch.where(clipped, edge, ratio) * a
+    flat = clipped | (a == 0)   # nothing is left of the ratio, also of an infinite one
+    loss = -torch.where(flat, edge, torch.exp(torch.where(flat, 0.0, step))) * a
     kl = torch.zeros_like(loss)
     if ref_nll is not None:
         gap = x - at(ref_nll)

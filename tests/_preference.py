@@ -3,6 +3,7 @@ from __future__ import annotations
 
 import math
 
+import pytest
 import torch
 
 
@@ -117,3 +118,27 @@ def layout(name, seqs, t, seed):
 
 
 LAYOUTS = ("batch", "masked", "packed", "gaps")
+
+
+def check_infinite(place, **kw):
+    """Losses and gradients where a ratio is infinite or 0; `place` puts a tensor where `kw`'s impl wants it."""
+    from mlx_train_perf import policy_loss, preference_loss
+
+    inf = math.inf
+    # the rejected answer (then the chosen one) has a token that the policy rules out
+    for nll, want, slope in (([[1.0, 2.0], [1.0, inf]], 0.0, 0.0), ([[1.0, inf], [1.0, 2.0]], inf, 0.1)):
+        x = place(torch.tensor(nll)).requires_grad_(True)
+        r = preference_loss(x, place(torch.ones(2, 2)), **kw)
+        (d,) = torch.autograd.grad(r.loss, x)
+        assert float(r.loss.detach()) == want
+        assert torch.allclose(d.double().cpu(), torch.tensor([[slope] * 2, [-slope] * 2], dtype=torch.float64), atol=1e-9)
+    # old = inf: a ratio of infinity; advantages that clip it, drop it and leave it. nll = inf: a ratio of 0
+    old = torch.tensor([[inf, inf, inf, 1.0, 1.0, 1.0]])
+    nll = torch.tensor([[1.0, 1.0, 1.0, inf, inf, inf]])
+    adv = torch.tensor([[1.0, 0.0, -1.0, 1.0, 0.0, -1.0]])
+    x = place(nll).requires_grad_(True)
+    r = policy_loss(x, place(old), place(adv), reduction="none", **kw)
+    (d,) = torch.autograd.grad(r.loss, x, torch.ones_like(r.loss))
+    assert r.loss.detach().tolist()[0] == pytest.approx([-1.2, 0.0, inf, 0.0, 0.0, 0.8])
+    assert d.tolist()[0] == [0.0, 0.0, -inf, 0.0, 0.0, 0.0]
+    assert float(r.clip_fraction) == pytest.approx(2 / 6)

@@ -222,3 +222,12 @@ def test_captured_steps(packed):
             g.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(out, fn(new))), (turn, n)
+
+
+@pytest.mark.parametrize("node", [True, False])
+def test_infinite_ratios(node, monkeypatch):
+    from mlx_train_perf import _native
+
+    if not node:
+        monkeypatch.setattr(_native, "nodes", lambda: None)
+    P.check_infinite(lambda t: t.cuda())

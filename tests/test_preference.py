@@ -182,3 +182,9 @@ def test_c_abi_refuses_tokens_that_end_past_32_bits():
         assert lib.mtp_pref_bwd(p, p, None, None, rows // 2, more, 1, p, None) == _native.MTP_ERR_INPUT
         assert lib.mtp_policy_fwd(p, p, None, p, 0, None, None, rows, more, 0.2, 0.2, 0.0, 1, p, p, p, p, 1 << 40, None) == _native.MTP_ERR_INPUT
         assert lib.mtp_policy_bwd(p, p, p, None, p, 0, None, None, rows, more, 0.2, 0.2, 0.0, 1, p, p, None) == _native.MTP_ERR_INPUT
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+def test_infinite_ratios(dtype):
+    """A token that one model rules out: what the formulas leave of it is finite where a factor of 0 or a border stands."""
+    P.check_infinite(lambda t: t.to(dtype), impl="reference")
