@@ -853,7 +853,12 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
   // that sees anything some score (with slopes, in the masks that show a query its own key, that key's) is at least its
   // negative. So probabilities are formed against 0: at most 2^80, summed over a row and times a value below 2^24 still
   // in fp32's range, and their sum is at least 2^-80. That saves the running maximum, its exchange and every rescale.
+  // A slope below 0 raises far keys: there the bias of a query's farthest key takes the place of 0.
   static_assert(!FIXED || (!DQ && CAP));
+  auto fixed_top = [&]() {
+    return (MOD & kModSlope) ? fmaxf(-score.slope2, 0.f) * (float)(causal || qi > S - 1 - qi ? qi : S - 1 - qi) : 0.f;
+  };
+  if constexpr (FIXED) score.add -= fixed_top();
   float m = FIXED ? 0.f : kNegInf, l = 0.f;
   f32x16 acc[kDB];
 #pragma unroll
@@ -1254,7 +1259,7 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
   }
   if constexpr (!DQ) {
     // A query that sees nothing: L = +inf, so that the backward's probabilities exp(S - L) are 0.
-    if (qvalid && hf == 0) lse_out[qrow + qi] = (SPAN && !(lt > 0.f)) ? -kNegInf : (m + fast_log2(lt)) * kLn2;
+    if (qvalid && hf == 0) lse_out[qrow + qi] = (SPAN && !(lt > 0.f)) ? -kNegInf : ((FIXED ? fixed_top() : m) + fast_log2(lt)) * kLn2;
   }
   auto quad = [&](int db, int rq) __attribute__((always_inline)) {  // dims 32 db + 8 rq + 4 hf .. + 3
     return u32x2{pack_bf16x2(acc[db][4 * rq] * mul, acc[db][4 * rq + 1] * mul),

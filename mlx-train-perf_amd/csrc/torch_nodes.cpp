@@ -12,9 +12,11 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <string>
 
 #include "../../include/mtp_hip.h"
@@ -157,6 +159,20 @@ struct KernelAttention : torch::autograd::Function<KernelAttention> {
   }
 };
 
+// The gradients of a backward whose own derivative does not exist: asked for (create_graph) it raises, as behind
+// once_differentiable, and is not taken for 0.
+torch::autograd::variable_list once(const torch::autograd::variable_list& cotangents, torch::autograd::variable_list grads) {
+  const auto asked = [](const at::Tensor& t) { return t.defined() && t.requires_grad(); };
+  if (!at::GradMode::is_enabled() || std::none_of(cotangents.begin(), cotangents.end(), asked)) return grads;
+  for (at::Tensor& g : grads) {
+    if (!g.defined()) continue;
+    const auto error = std::make_shared<torch::autograd::DelayedError>(
+        "trying to differentiate twice a function that was marked with @once_differentiable", 1);
+    g = (*error)({g.detach().set_requires_grad(true)})[0];
+  }
+  return grads;
+}
+
 // Scores and masks beyond the plain ones: not inputs of the node either.
 struct Score {
   double softcap;  // 0: none
@@ -211,7 +227,7 @@ struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
     else
       check(g_api.scored_bwd(ptr(q), ptr(k), ptr(v), ptr(o), ptr<float>(lse), ptr(d_o), b, hq, hkv, s, dh, scale, causal, cap,
                              floats(slopes), ints(start), ints(end), ptr(dq), ptr(dk), ptr(dv), ptr(ws), bytes, stream_of(q)));
-    return {dq, dk, dv, at::Tensor(), at::Tensor(), at::Tensor()};
+    return once(grads, {dq, dk, dv, at::Tensor(), at::Tensor(), at::Tensor()});
   }
 };
 
@@ -266,7 +282,7 @@ struct Preference : torch::autograd::Function<Preference> {
     check(g_api.pref_bwd(ptr<float>(d_loss), ptr<float>(coef), bytes_of(mask), longs(offsets), ctx->saved_data["pairs"].toInt(),
                          d_nll.numel(), (int)ctx->saved_data["reduction"].toInt(), ptr<float>(d_nll), stream_of(coef)),
           "loss");
-    return {d_nll, at::Tensor()};
+    return once(grads, {d_nll, at::Tensor()});
   }
 };
 
@@ -320,7 +336,7 @@ struct Policy : torch::autograd::Function<Policy> {
                            sd["clip_low"].toDouble(), sd["clip_high"].toDouble(), sd["kl_coef"].toDouble(),
                            (int)sd["reduction"].toInt(), ptr<float>(weight), ptr<float>(d_nll), stream_of(nll)),
           "loss");
-    return {d_nll, at::Tensor()};
+    return once(grads, {d_nll, at::Tensor()});
   }
 };
 

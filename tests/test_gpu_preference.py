@@ -231,3 +231,47 @@ def test_infinite_ratios(node, monkeypatch):
     if not node:
         monkeypatch.setattr(_native, "nodes", lambda: None)
     P.check_infinite(lambda t: t.cuda())
+
+
+def _both(x, ref, adv, offsets, mask, kw):
+    from mlx_train_perf import policy_loss, preference_loss
+
+    r = preference_loss(x, ref, offsets=offsets, mask=mask)
+    p = policy_loss(x, ref, adv, ref_nll=ref, kl_coef=0.1, offsets=offsets, mask=mask, **kw)
+    return r, p
+
+
+@pytest.mark.parametrize("layout", P.LAYOUTS)
+def test_node_and_function_agree(layout, monkeypatch):
+    """The C++ nodes and the Python Functions are the same calls, to the bit."""
+    from mlx_train_perf import _native
+
+    shape, offsets, mask = P.layout(layout, 6, 300, 2)
+    nll, ref, _ = (t.cuda() for t in P.tensors(shape, 2))
+    adv = torch.randn(6, generator=torch.Generator().manual_seed(2)).cuda()
+
+    def step():
+        out = []
+        for kw in ({}, {"reduction": "sequence"}, {"reduction": "none"}):
+            x = nll.detach().requires_grad_(True)
+            r, p = _both(x, ref, adv, _cuda(offsets), _cuda(mask), kw)
+            out += [*(v.detach() for v in (*r, *p)), torch.autograd.grad(r.loss + p.loss.sum(), x)[0]]
+        return out
+
+    assert _native.nodes() is not None
+    with_node = step()
+    monkeypatch.setattr(_native, "nodes", lambda: None)
+    assert all(torch.equal(a, b) for a, b in zip(with_node, step()))
+
+
+@pytest.mark.parametrize("node", [True, False])
+def test_second_derivative_is_refused(node, monkeypatch):
+    from mlx_train_perf import _native
+
+    if not node:
+        monkeypatch.setattr(_native, "nodes", lambda: None)
+    x = torch.rand(4, 5, device="cuda", requires_grad=True)
+    for loss in _both(x, torch.rand(4, 5, device="cuda"), torch.randn(4, device="cuda"), None, None, {}):
+        (d,) = torch.autograd.grad(loss.loss.square(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            (d.square().sum() + x.sum()).backward()

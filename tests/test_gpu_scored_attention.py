@@ -28,11 +28,11 @@ def _call(q, k, v, d_o, *, mask, spans, **kw):
     return [o.detach(), *torch.autograd.grad(o, qs, d_o.cuda())]
 
 
-def _check(b, hq, hkv, s, dh, *, mask, cap, biased, dtype, seed=0, std=2.0, spans=None):
+def _check(b, hq, hkv, s, dh, *, mask, cap, biased, dtype, seed=0, std=2.0, spans=None, slopes=None, more_bar=0.0):
     print(f"[scored] b={b} hq={hq} hkv={hkv} s={s} dh={dh} {mask} cap={cap} biased={biased} {dtype}", flush=True)
     q, k, v, d_o = S.inputs(b, hq, hkv, s, dh, dtype, seed, std)
     spans = S.spans_of(mask, b, s, seed) if spans is None else spans
-    slopes = S.slopes_of(hq).cuda() if biased else None
+    slopes = None if not biased else S.slopes_of(hq).cuda() if slopes is None else slopes.cuda()
     scale = dh ** -0.5
     got = _call(q, k, v, d_o, mask=mask, spans=spans, scale=scale, softcap=cap, slopes=slopes)
     see = S.visible(mask, spans, b, s, "cuda")
@@ -45,7 +45,7 @@ def _check(b, hq, hkv, s, dh, *, mask, cap, biased, dtype, seed=0, std=2.0, span
             assert not a.transpose(1, 2)[empty].any(), f"{name}: a query that sees nothing"
         if name in ("dk", "dv"):
             assert not a.transpose(1, 2)[~see.any(1)].any(), f"{name}: a key that nothing sees"
-        assert S.off(a, w) <= BAR[dtype] * float(w.norm()) + more.get(name, 0.0), (name, S.rel(a, w), more)
+        assert S.off(a, w) <= (BAR[dtype] + more_bar) * float(w.norm()) + more.get(name, 0.0), (name, S.rel(a, w), more)
     return got
 
 
@@ -296,3 +296,69 @@ def test_fp32_without_room_for_parts():
                                        *(x.data_ptr() for x in outs), ws.data_ptr(), ws.numel() * 4, st) == 0
     for a, c in zip((o1, lse1, *outs), (o, lse, *grads)):
         assert S.rel(a, c) <= 2 * BAR[torch.float32]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("cap", [20.0, 100.0, None])
+@pytest.mark.parametrize("mask", ["causal", "full", "ragged", "window"])
+@pytest.mark.parametrize(("s", "dh"), [(1, 64), (70, 96), (300, 64), (300, 128)])
+def test_slopes_of_either_sign(s, dh, mask, cap, dtype):
+    """Slopes below 0 raise far keys: biases of up to 75, past fp32's largest exponential when a cap of 20 is added. A
+    score is then the last of four roundings (slope times distance, the two sums, L) of at most 75: 4 * 75 * 2^-24 on top."""
+    slopes = torch.tensor([0.25, -0.25, 0.0, -0.01])
+    _check(1, 4, 2, s, dh, mask=mask, cap=cap, biased=True, dtype=dtype, seed=s, slopes=slopes, more_bar=4 * 75 * 2 ** -24)
+
+
+@pytest.mark.parametrize("mask", ["causal", "window"])
+def test_values_of_every_size(mask):
+    """Scores at a cap of 50 (probabilities against a fixed maximum span 2^144): V times a power of 2 gives O times it."""
+    q, k, v, d_o = S.inputs(1, 4, 2, 200, 64, torch.bfloat16, 4, std=40.0)
+    spans = S.spans_of(mask, 1, 200, 4)
+    base = _call(q, k, v, d_o, mask=mask, spans=spans, scale=1.0, softcap=50.0)[0]
+    assert torch.isfinite(base).all()
+    for power in (24, 10, -30):
+        o = _call(q, k, v * 2.0 ** power, d_o, mask=mask, spans=spans, scale=1.0, softcap=50.0)[0]
+        assert S.rel(o * 2.0 ** -power, base.double()) <= 1e-6, power
+
+
+def _forms():
+    from mlx_train_perf.attention import SpanMask
+
+    sp = SpanMask(*(t.cuda() for t in S.spans_of("prefix", 2, 150, 3)))
+    return [{"softcap": 9.0}, {"slopes": S.slopes_of(4).cuda(), "softcap": 80.0, "spans": sp}, {"spans": sp}]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_node_and_function_agree(dtype, monkeypatch):
+    """The C++ node and the Python Function are the same calls, to the bit."""
+    from mlx_train_perf import _native
+    from mlx_train_perf.attention import flash_attention
+
+    x = [t.cuda() for t in S.inputs(2, 4, 2, 150, 64, dtype, 6)]
+
+    def step(kw):
+        qs = [t.detach().requires_grad_(True) for t in x[:3]]
+        o = flash_attention(*qs, scale=0.125, **kw)
+        return [o.detach(), *torch.autograd.grad(o, qs, x[3])]
+
+    assert _native.nodes() is not None
+    with_node = [step(kw) for kw in _forms()]
+    monkeypatch.setattr(_native, "nodes", lambda: None)
+    for kw, a in zip(_forms(), with_node):
+        assert all(torch.equal(p, r) for p, r in zip(a, step(kw)))
+
+
+@pytest.mark.parametrize("node", [True, False])
+def test_second_derivative_is_refused(node, monkeypatch):
+    from mlx_train_perf import _native
+    from mlx_train_perf.attention import flash_attention
+
+    if not node:
+        monkeypatch.setattr(_native, "nodes", lambda: None)
+    q, k, v, d_o = (t.cuda().requires_grad_(True) for t in S.inputs(1, 2, 1, 40, 64, torch.float32, 6))
+    o = flash_attention(q, k, v, scale=0.125, softcap=9.0)
+    dq, dk = torch.autograd.grad(o, (q, k), d_o, create_graph=True)
+    want = torch.autograd.grad(flash_attention(q, k, v, scale=0.125, softcap=9.0), (q, k), d_o.detach())
+    assert torch.equal(dq, want[0]) and torch.equal(dk, want[1])
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        (dq.square().sum() + o.sum()).backward()
