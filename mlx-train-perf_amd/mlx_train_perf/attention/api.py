@@ -29,6 +29,7 @@ from mlx_train_perf.errors import AttentionInputError, UnsupportedAttentionError
 
 _KERNEL_DTYPES = (torch.bfloat16, torch.float32)   # the reference kernel's T (api.py:41-43)
 _KERNEL_HEAD_DIMS = (64, 96, 128)
+_KERNEL_CAPS = (1e-3, 1e3)   # beyond it fp32 has no tanh of the scores, or none that bends them
 
 VJP_CALLS: dict[str, int] = {}
 
@@ -141,6 +142,11 @@ def resolve_attention_impl(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *,
     if head_dim not in _KERNEL_HEAD_DIMS:
         raise UnsupportedAttentionError(
             f"kernel impl only supports head_dim in {_KERNEL_HEAD_DIMS} (got {head_dim}); use impl='reference'."
+        )
+    # (here, not in the library, which sees a cap that rounds to an fp32 0 as none)
+    if softcap is not None and not _KERNEL_CAPS[0] <= softcap <= _KERNEL_CAPS[1]:
+        raise UnsupportedAttentionError(
+            f"kernel impl only supports a softcap in {list(_KERNEL_CAPS)} (got {softcap}); use impl='reference'."
         )
     _compat.check_device_verified(allow_unverified=False, error=UnsupportedAttentionError)
     _compat.require_gpu_tensor(q, error=UnsupportedAttentionError)
@@ -369,7 +375,10 @@ def flash_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale:
     from the score of query i and key j (after the cap); they get no gradient. `spans`: a `SpanMask`, the keys that
     each query sees; it is the whole mask, so `causal` has no say beside it and `segments` may not be given (cap and
     slopes go with either). A query that sees nothing gets zeros and no gradient. `validate_segments` checks the
-    contract of `spans` too, at one host sync a mask."""
+    contract of `spans` too, at one host sync a mask.
+    The kernel impl takes a softcap in [1e-3, 1e3], with any of the three a scale above 0, and slopes of either sign of
+    up to some hundreds. As in a plain product, a hidden V (and in the backward a hidden K or dO) must be finite: 0 is
+    what it is multiplied by. These calls differentiate once."""
     resolved = resolve_attention_impl(q, k, v, impl=impl, causal=causal, segments=segments,
                                       validate_segments=validate_segments, softcap=softcap, slopes=slopes, spans=spans)
     scored = softcap is not None or slopes is not None or spans is not None

@@ -70,7 +70,7 @@ class SpanMask:
     gets an output of zeros and takes part in no gradient. A window of w keys is start = i - w + 1, end = i + 1.
 
     A mask remembers that its contract was checked (a host sync), for as long as neither tensor is written to, so that
-    a model's layers check the mask of a step once.
+    a model's layers check the mask of a step once (tensors made in inference mode do not tell of writes: checked each time).
     """
     start: torch.Tensor
     end: torch.Tensor
@@ -78,11 +78,12 @@ class SpanMask:
 
     def violation(self) -> str | None:
         """`span_violation` of this mask, unless it was found to be none before."""
-        versions = [self.start._version, self.end._version]
-        if self._checked == versions:
+        tells = not (self.start.is_inference() or self.end.is_inference())
+        versions = [self.start._version, self.end._version] if tells else []
+        if tells and self._checked == versions:
             return None
         problem = span_violation(self)
-        if problem is None:
+        if problem is None and tells:
             self._checked[:] = versions
         return problem
 

@@ -315,7 +315,8 @@ def policy_loss(nll: torch.Tensor, old_nll: torch.Tensor, advantages: torch.Tens
                 clip_high: float = 0.2, kl_coef: float = 0.0, reduction: Literal["token", "sequence", "none"] = "token",
                 impl: Literal["auto", "kernel", "reference"] = "auto", validate_offsets: bool = True) -> PolicyLoss:
     """Clipped policy loss with a KL term. With u = exp(old_nll - nll), the advantage A of the token (`advantages` of
-    nll's shape) or of its sequence ((sequences,)), and d = nll - ref_nll, a token's loss is
+    nll's shape) or of its sequence ((sequences,); where that is nll's shape too, they are the tokens'), and
+    d = nll - ref_nll, a token's loss is
       -min(u A, clip(u, 1 - clip_low, 1 + clip_high) A) + kl_coef (e^d - d - 1).
     `reduction`: "token", the mean over the tokens that count; "sequence", the mean over the sequences that have such
     tokens of each one's mean; "none", per token (0 where it counts nowhere). With no token that counts the loss is 0.

@@ -129,6 +129,10 @@ def test_refusals():
         call(spans=SpanMask(start=z.float(), end=z))
     with pytest.raises(UnsupportedAttentionError):   # the kernel gate, as without a cap
         resolve_attention_impl(q.half(), q.half(), q.half(), impl="kernel", softcap=1.0)
+    for cap in (1e-50, 9e-4, 1001.0):   # the first is an fp32 0
+        assert call(softcap=cap) == "reference"
+        with pytest.raises(UnsupportedAttentionError, match="softcap in"):
+            resolve_attention_impl(q, q, q, impl="kernel", softcap=cap, slopes=torch.zeros(4))
 
 
 def test_c_abi_refusals():
@@ -144,7 +148,7 @@ def test_c_abi_refusals():
         for kw, rc, what in [({"scale": 0.0}, bad, "scale"), ({"scale": math.nan}, bad, "scale"), ({"scale": -1.0}, bad, "scale"),
                              ({"cap": -1.0}, bad, "softcap"), ({"cap": math.inf}, bad, "softcap"), ({"cap": math.nan}, bad, "softcap"),
                              ({"start": p}, bad, "span_start and span_end"), ({"start": p, "end": p, "causal": 1}, bad, "causal must be 0"),
-                             ({"cap": 0.0}, bad, "no softcap"), ({"q": none}, bad, "non-null"), ({"o": none}, bad, "non-null"),
+                             ({"cap": 0.0}, bad, "no softcap"), ({"cap": 9e-4}, un, "softcap"), ({"cap": 1001.0}, un, "softcap"), ({"q": none}, bad, "non-null"), ({"o": none}, bad, "non-null"),
                              ({"q": p + 2}, un, "aligned"), ({"shape": (1, 3, 2, 8, 64)}, bad, "multiple"),
                              ({"shape": (1, 2, 1, 8, 80)}, un, "head_dim"), ({"shape": (1, 2, 1, 1 << 23, 64)}, bad, "2\\^23"),
                              ({"causal": 2}, bad, "causal")]:
@@ -165,3 +169,17 @@ def test_c_abi_refusals():
     assert lib.mtp_attn_scored_fwd_f32_workspace_bytes(1, 32, 8, 8192, 128) == 0    # enough workgroups
     assert lib.mtp_attn_scored_fwd_f32_workspace_bytes(1, 1, 1, 100, 64) == 0       # too few tiles
     assert lib.mtp_attn_scored_bwd_f32_workspace_bytes(1, 8, 2, 1000, 128) >= 8000 * 4 + 4 * 8 * 1000 * 128 * 4
+
+
+def test_spans_of_inference_mode():
+    """Tensors made in inference mode have no version: their contract is checked at every call."""
+    with torch.inference_mode():
+        q = torch.randn(1, 2, 5, 64)
+        end = torch.arange(1, 6, dtype=torch.int32)[None]
+        sp = SpanMask(start=torch.zeros_like(end), end=end)
+        for _ in range(2):
+            o = flash_attention(q, q, q, scale=1.0, impl="reference", spans=sp)
+        assert torch.allclose(o, flash_attention(q, q, q, scale=1.0, impl="reference"), atol=1e-6)
+        end.fill_(6)
+        with pytest.raises(AttentionInputError, match="end must lie"):
+            flash_attention(q, q, q, scale=1.0, impl="reference", spans=sp)
