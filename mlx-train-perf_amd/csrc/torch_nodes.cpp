@@ -233,10 +233,10 @@ struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
 
 // Preference and policy losses: what a call has beside nll, none of it an input of the node.
 struct Rows {
-  at::Tensor mask, offsets;  // uint8, int64; may be missing
+  at::Tensor mask, offsets;  // uint8 or bool, int64; may be missing
   int64_t rows;
 };
-const uint8_t* bytes_of(const at::Tensor& t) { return t.defined() ? t.const_data_ptr<uint8_t>() : nullptr; }
+const uint8_t* bytes_of(const at::Tensor& t) { return t.defined() ? static_cast<const uint8_t*>(t.const_data_ptr()) : nullptr; }
 const int64_t* longs(const at::Tensor& t) { return t.defined() ? t.const_data_ptr<int64_t>() : nullptr; }
 struct PreferenceCall {
   at::Tensor ref;

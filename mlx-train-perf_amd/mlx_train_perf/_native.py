@@ -203,8 +203,10 @@ def plain(*tensors: torch.Tensor) -> bool:
     """Ordinary tensors outside function transforms, tracing and dispatch modes, without a forward-mode
     tangent: the calls that the C++ nodes take. The others keep the Python Functions, which refuse or
     serve them as they always did (a node sees no tangent of a tensor that is not its input)."""
-    return (all(type(t) in (torch.Tensor, torch.nn.Parameter) for t in tensors)
-            and not torch._C._are_functorch_transforms_active() and torch._C._get_tracing_state() is None
+    for t in tensors:
+        if type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:
+            return False
+    return (not torch._C._are_functorch_transforms_active() and torch._C._get_tracing_state() is None
             and not torch.compiler.is_compiling() and torch._C._len_torch_dispatch_stack() == 0
             and (forward_ad._current_level < 0 or all(forward_ad.unpack_dual(t).tangent is None for t in tensors)))
 

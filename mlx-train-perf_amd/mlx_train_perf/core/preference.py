@@ -50,25 +50,26 @@ def _number(name: str, x: float, ok: bool, what: str) -> float:
 def _sequences(nll: torch.Tensor, frozen: dict[str, torch.Tensor | None], offsets: torch.Tensor | None,
                mask: torch.Tensor | None, validate_offsets: bool) -> int:
     """The number of sequences, after the checks that both losses share."""
+    shape = nll.shape
     if not nll.dtype.is_floating_point:
         raise LossInputError(f"nll must be floating-point; got {nll.dtype}")
     if nll.numel() < 1:
-        raise LossInputError(f"nll must hold at least one token; got shape {tuple(nll.shape)}")
+        raise LossInputError(f"nll must hold at least one token; got shape {tuple(shape)}")
     for name, t in frozen.items():
         if t is None:
             continue
-        if t.shape != nll.shape:
-            raise LossInputError(f"{name} must have nll's shape {tuple(nll.shape)}; got {tuple(t.shape)}")
+        if t.shape != shape:
+            raise LossInputError(f"{name} must have nll's shape {tuple(shape)}; got {tuple(t.shape)}")
         if not t.dtype.is_floating_point:
             raise LossInputError(f"{name} must be floating-point; got {t.dtype}")
         if t.requires_grad and torch.is_grad_enabled():
             raise LossInputError(f"{name} belongs to a frozen model and gets no gradient: detach it")
-    if mask is not None and (mask.shape != nll.shape or mask.dtype not in (torch.bool, torch.uint8)):
-        raise LossInputError(f"mask must be bool or uint8 of nll's shape {tuple(nll.shape)}; got {mask.dtype} {tuple(mask.shape)}")
+    if mask is not None and (mask.shape != shape or mask.dtype not in (torch.bool, torch.uint8)):
+        raise LossInputError(f"mask must be bool or uint8 of nll's shape {tuple(shape)}; got {mask.dtype} {tuple(mask.shape)}")
     if offsets is None:
-        if nll.dim() != 2:
-            raise LossInputError(f"nll must be (sequences, T), or (N,) with offsets; got shape {tuple(nll.shape)}")
-        return nll.shape[0]
+        if len(shape) != 2:
+            raise LossInputError(f"nll must be (sequences, T), or (N,) with offsets; got shape {tuple(shape)}")
+        return shape[0]
     if nll.dim() != 1:
         raise LossInputError(f"with offsets nll must be (N,); got shape {tuple(nll.shape)}")
     if offsets.dim() != 1 or offsets.numel() < 2 or offsets.dtype not in (torch.int32, torch.int64):
@@ -84,20 +85,27 @@ def _resolve(nll: torch.Tensor, others: dict[str, torch.Tensor | None], impl: st
         return impl
     if impl not in ("auto", "kernel"):
         raise LossInputError(f"unknown impl {impl!r}; expected one of 'auto', 'kernel', 'reference'")
+    others = {name: t for name, t in others.items() if t is not None}
     for name, t in {"nll": nll, **others}.items():
-        if t is not None and t.dtype.is_floating_point and t.dtype != torch.float32:
-            raise UnsupportedHeadError(f"kernel impl reads fp32 tensors (got {name} of {t.dtype}); use impl='reference'.")
+        dtype = t.dtype
+        if dtype is not torch.float32 and dtype.is_floating_point:
+            raise UnsupportedHeadError(f"kernel impl reads fp32 tensors (got {name} of {dtype}); use impl='reference'.")
     _compat.check_device_verified(allow_unverified=False, error=UnsupportedHeadError)
     _compat.require_gpu_tensor(nll, error=UnsupportedHeadError)
+    device = nll.device
     for name, t in others.items():
-        if t is not None and t.device != nll.device:
-            raise LossInputError(f"{name} is on {t.device} but nll is on {nll.device}; the kernel impl needs every "
+        if t.device != device:
+            raise LossInputError(f"{name} is on {t.device} but nll is on {device}; the kernel impl needs every "
                                  "input on the same GPU")
     return "kernel"
 
 
+def _frozen(t: torch.Tensor | None) -> torch.Tensor | None:
+    return None if t is None else (t.detach() if t.requires_grad else t).contiguous()
+
+
 def _plain_mask(mask: torch.Tensor | None) -> torch.Tensor | None:
-    return None if mask is None else mask.contiguous().view(torch.uint8)
+    return None if mask is None else mask.contiguous()   # bool or uint8: bytes either way
 
 
 def _plain_offsets(offsets: torch.Tensor | None) -> torch.Tensor | None:
@@ -301,7 +309,7 @@ def preference_loss(nll: torch.Tensor, ref_nll: torch.Tensor, *, offsets: torch.
     if _resolve(nll, {"ref_nll": ref_nll, "offsets": offsets, "mask": mask}, impl) == "reference":
         return _reference_preference(nll, ref_nll.detach(), offsets, mask, rows, kind, beta, label_smoothing, reduction)
     pairs = rows // 2
-    args = (nll.contiguous(), ref_nll.detach().contiguous(), _plain_mask(mask), _plain_offsets(offsets), pairs, _KINDS[kind], beta,
+    args = (nll.contiguous(), _frozen(ref_nll), _plain_mask(mask), _plain_offsets(offsets), pairs, _KINDS[kind], beta,
             label_smoothing, _REDUCTIONS[reduction])
     nodes = _native.nodes() if _native.plain(nll, ref_nll) else None
     if nodes is not None:
@@ -339,8 +347,7 @@ def policy_loss(nll: torch.Tensor, old_nll: torch.Tensor, advantages: torch.Tens
         ref = None if ref_nll is None else ref_nll.detach()
         return _reference_policy(nll, old_nll.detach(), ref, advantages.detach(), offsets, mask, rows, clip_low, clip_high,
                                  kl_coef, reduction)
-    old, ref, adv = (None if t is None else t.detach().contiguous() for t in (old_nll, ref_nll, advantages))
-    args = (old, ref, adv, _plain_mask(mask), _plain_offsets(offsets), rows, clip_low, clip_high, kl_coef, _REDUCTIONS[reduction])
+    args = (_frozen(old_nll), _frozen(ref_nll), _frozen(advantages), _plain_mask(mask), _plain_offsets(offsets), rows, clip_low, clip_high, kl_coef, _REDUCTIONS[reduction])
     nodes = _native.nodes() if _native.plain(nll, *(t for t in (old_nll, ref_nll, advantages) if t is not None)) else None
     if nodes is not None:
         return PolicyLoss(*nodes.policy(nll.contiguous(), *args))
