@@ -291,20 +291,23 @@ int mtp_attn_bwd_f32(const float* q, const float* k, const float* v, const float
  *     span_start[i] <= j < span_end[i]; neither may decrease along a row, and a query whose span holds nothing
  *     gets o = 0, lse = +inf and no gradient. Spans are the whole mask (causal must be 0). Values outside the
  *     row are clamped into it; spans that decrease give some wrong rows, never an access out of range.
- * scale must be positive. At least one of the three must be given (else: mtp_attn_fwd).
+ * scale must be positive, softcap 0 or in [1e-3, 1e3], slopes of either sign. At least one of the three must be
+ * given (else: mtp_attn_fwd). What a query does not see must be finite all the same: v, and in the backward k and d_o.
+ * o_low: int8 [b][hq][s][dh], the 8 bits of the output below its bf16 ones (bits of x = bits of bf16(x) + 2^8 o_low), for
+ * the backward's D = rowsum(d_o o); NULL in a forward without a backward.
  * ------------------------------------------------------------------------------------------- */
 int mtp_attn_scored_fwd(const void* q, const void* k, const void* v, int64_t b, int64_t hq, int64_t hkv,
                         int64_t s, int64_t dh, float scale, int32_t causal, float softcap,
                         const float* slopes, const int32_t* span_start, const int32_t* span_end, void* o,
-                        float* lse, void* stream);
+                        int8_t* o_low, float* lse, void* stream);
 
 /* Workspace bytes of mtp_attn_scored_bwd, each part padded to 256 bytes: D (fp32 [b][hq][s]), the fp32 dK/dV
  * partials where the dK/dV pass is split (as mtp_attn_bwd's), and for spans the int32 work orders of the two
  * passes and the int32 range of queries that see each key (2 x [b][s]). */
 size_t mtp_attn_scored_bwd_workspace_bytes(int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh);
 
-int mtp_attn_scored_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse,
-                        const void* d_o, int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh,
+int mtp_attn_scored_bwd(const void* q, const void* k, const void* v, const void* o, const int8_t* o_low,
+                        const float* lse, const void* d_o, int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh,
                         float scale, int32_t causal, float softcap, const float* slopes,
                         const int32_t* span_start, const int32_t* span_end, void* d_q, void* d_k, void* d_v,
                         void* workspace, size_t workspace_bytes, void* stream);

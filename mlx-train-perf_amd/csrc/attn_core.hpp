@@ -421,10 +421,11 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
       tro[t][db] = rl * kRowB + ((c ^ swt) << 4) + 8 * (lane & 1);
     }
   }
-  // With a cap P's two copies leave no room for these 16 offsets: each is then formed at its use from the first of
-  // its kind (2 ks touches chunk bits 1-3, 4 db bits 2-3, of an XOR-swizzled chunk index).
-  auto row_off = [&](int base, int ks) __attribute__((always_inline)) { return CAP ? base ^ (ks << 5) : ro[ks]; };
-  auto tr_off = [&](int base, int t, int db) __attribute__((always_inline)) { return CAP ? base ^ (db << 6) : tro[t][db]; };
+  // With a cap (or slopes' ramp at head_dim 96) P's two copies leave no room for these 16 offsets: each is then formed at
+  // its use from the first of its kind (2 ks touches chunk bits 1-3, 4 db bits 2-3, of an XOR-swizzled chunk index).
+  constexpr bool kForm = CAP || (MOD == kModSlope && DH == 96);
+  auto row_off = [&](int base, int ks) __attribute__((always_inline)) { return kForm ? base ^ (ks << 5) : ro[ks]; };
+  auto tr_off = [&](int base, int t, int db) __attribute__((always_inline)) { return kForm ? base ^ (db << 6) : tro[t][db]; };
   // The P wave reads Q rows and dO^T; the dS wave dO rows and Q^T.
   const int row_src = pwave ? 0 : kTile;
   const int tr_src = pwave ? kTile : 0;
@@ -468,15 +469,19 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
   constexpr bool kRamp = MOD == kModSlope && DH <= 96;
   f32x16 ramp[2];
   int ramp_head = -1;
-  // With a cap the P wave hands its partner P (1 - tanh^2), which dS is formed from, and keeps P itself in
-  // registers for its own second product.
-  bf16x8 pown[CAP ? 2 : 1][2];
+  // HALF: the P wave hands its partner P (with a cap P (1 - tanh^2)), which dS is formed from, in fp16, and keeps P in bf16
+  // in registers for its own second product: bf16 there made dK's error 2.9e-3 of its norm instead of 2.4e-3. P is formed
+  // 2^15 times as large, so that fp16 holds it to the last bit down to 2^-29; the last multipliers of dV and dK take the
+  // factor back.
+  constexpr bool HALF = SPAN || MOD != kModNone;
+  constexpr float kUp = HALF ? 15.f : 0.f, kDown = HALF ? 0x1p-15f : 1.f;
+  bf16x8 pown[HALF ? 2 : 1][2];
   auto start = [&](int it, const char* st, char* pb, const CopySrc& cx, char* sx) __attribute__((always_inline)) {
     {
       // Row fragments read two k16 steps ahead of their products.
       bf16x8 rf[3][2];
       int rbase = ro[0];
-      if constexpr (CAP) asm volatile("" : "+v"(rbase));
+      if constexpr (kForm) asm volatile("" : "+v"(rbase));
       auto rd = [&](int ks) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) rf[ks % 3][h] = as_bf16x8(lds_read16(st + row_src, 32 * h * kRowB + row_off(rbase, ks)));
@@ -523,7 +528,7 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
       const bool need_mask = (causal && q0 < kw0 + 31) || (q0 + kKT > S) || (PACKED && q0 + kKT > w_lim) || (SPAN && q0 < w_beg);
       // With a cap and slopes bend needs v as raw left it, so that the bias comes after (mixed).
       constexpr bool kMixed = MOD == kModBoth;
-      float add = score.add;
+      float add = score.add + kUp;
       const float rel = (float)(kj - q0 - 4 * hf);
       if constexpr ((MOD & kModSlope) && !kRamp) score.set_slope(slopes ? slopes[kvh * G + (it0 + it) / ntq] : 0.f);
       if constexpr (MOD != kModNone) {
@@ -535,7 +540,7 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
           const int side = (causal || q0 >= kw0 + 31) ? -1 : q0 + kKT - 1 <= kw0 ? 1 : 0;
           score.template slant<-1, kRamp>(a1[0], 0, side, rel);
           score.template slant<-1, kRamp>(a1[1], 1, side, rel);
-          add = score.template slant_add<-1>(side, rel);
+          add = score.template slant_add<-1>(side, rel) + kUp;
         }
       }
       if (need_mask) {
@@ -548,7 +553,7 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
           }
       }
       const float* ls = reinterpret_cast<const float*>(st + 2 * kTile);
-      bf16x8 pf[2][2];
+      std::conditional_t<HALF, f16x8, bf16x8> pf[2][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -557,14 +562,14 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             const int r = 4 * rq + u;
-            if constexpr (MOD == kModNone) {
+            if constexpr (!HALF) {
               pf[h][r >> 3][r & 7] = (__bf16)fast_exp2(__builtin_fmaf(a1[h][r], scale_log2, -l4[u] * kLog2e));
             } else {
               float y = __builtin_fmaf(a1[h][r], score.mul, __builtin_fmaf(-kLog2e, l4[u], add));
               if constexpr (kMixed) y = __builtin_fmaf(-score.slope2, __builtin_fabsf(rel - (float)(32 * h + 8 * rq + u)), y);
               const float p = fast_exp2(y);
-              if constexpr (CAP) pown[h][r >> 3][r & 7] = (__bf16)p;
-              pf[h][r >> 3][r & 7] = (__bf16)(CAP ? p * Score<MOD>::bend(a1[h][r]) : p);
+              pown[h][r >> 3][r & 7] = (__bf16)p;
+              pf[h][r >> 3][r & 7] = (_Float16)(CAP ? p * Score<MOD>::bend(a1[h][r]) : p);
             }
           }
         }
@@ -580,12 +585,12 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
   // The transposed reads of the first two 16-query slabs are issued first, in flight while P is read
   // (and dS formed); each slab's products wait for its reads (lgkmcnt counts LDS reads in issue
   // order) while the slab after next is read.
-  auto finish = [&](const char* st, const char* pb, const bf16x8 (&pold)[CAP ? 2 : 1][2]) __attribute__((always_inline)) {
+  auto finish = [&](const char* st, const char* pb, const bf16x8 (&pold)[HALF ? 2 : 1][2]) __attribute__((always_inline)) {
     uint32_t ta0[4], ta1[4];
     {
       const uint32_t b = lds_addr(st + tr_src);
       int t0 = tro[0][0], t1 = tro[1][0];
-      if constexpr (CAP) asm volatile("" : "+v"(t0), "+v"(t1));
+      if constexpr (kForm) asm volatile("" : "+v"(t0), "+v"(t1));
 #pragma unroll
       for (int db = 0; db < kDB; ++db) {
         ta0[db] = b + tr_off(t0, 0, db);
@@ -600,12 +605,13 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        if (CAP && pwave) bo[h][j] = pold[CAP ? h : 0][j];
+        if (HALF && pwave) bo[h][j] = pold[HALF ? h : 0][j];
         else bo[h][j] = as_bf16x8(*reinterpret_cast<const u32x4*>(pb + pmine + 1024 * (2 * h + j) + 16 * lane));
       }
     if (!pwave) {
       // dS = P (dP - D).
       const float* ds_ = reinterpret_cast<const float*>(st + 2 * kTile) + 64;
+      bf16x8 ds;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -614,7 +620,13 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             const int r = 4 * rq + u;
-            bo[h][r >> 3][r & 7] = (__bf16)((float)bo[h][r >> 3][r & 7] * (a1[h][r] - d4[u]));
+            if constexpr (HALF) {
+              const float p = (float)__builtin_bit_cast(f16x8, bo[h][r >> 3])[r & 7];
+              ds[r & 7] = (__bf16)__builtin_fmaf(p, a1[h][r] - d4[u], 0.f);  // (a conversion less than a product)
+              if ((r & 7) == 7) bo[h][r >> 3] = ds;
+            } else {
+              bo[h][r >> 3][r & 7] = (__bf16)((float)bo[h][r >> 3][r & 7] * (a1[h][r] - d4[u]));
+            }
           }
         }
     }
@@ -669,8 +681,8 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
     constexpr bool PW = decltype(pw)::value;
     auto step = [&](int t, const char* sc, const char* pc, const char* sn, char* pn, char* sx) __attribute__((always_inline)) {
       if constexpr (PW) {
-        bf16x8 pold[CAP ? 2 : 1][2];
-        if constexpr (CAP) {
+        bf16x8 pold[HALF ? 2 : 1][2];
+        if constexpr (HALF) {
 #pragma unroll
           for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -705,7 +717,7 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
   }
 
   if (kvalid) {
-    const float mul = pwave ? 1.f : CAP ? -4.f * scale : scale;  // (Score::bend)
+    const float mul = kDown * (pwave ? 1.f : CAP ? -4.f * scale : scale);  // (Score::bend)
     if (nsplit == 1) {
       bf16_t* o = (pwave ? dv : dk) + (krow + kj) * DH;
 #pragma unroll
@@ -747,8 +759,13 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
                     float* __restrict__ dvec, const int32_t* __restrict__ span_end,
                     const int32_t* __restrict__ seg_start, bf16_t* __restrict__ out, float* __restrict__ lse_out,
                     int B, int Hq, int Hkv, int S, float scale_log2, float scale, int causal,
-                    const int32_t* __restrict__ order, float cap, const float* __restrict__ slopes) {
+                    const int32_t* __restrict__ order, float cap, const float* __restrict__ slopes,
+                    int8_t* __restrict__ o_low) {
   // seg_start: the first key that each query sees (packed: its segment's start; span: its span's).
+  // o_low (spans, caps and biases): the 8 bits of O below bf16's, written by the forward where given, read with O for
+  // D = rowsum(dO o O). dS = P (dP - D) is a difference that all but cancels where one probability is nearly 1, and
+  // D of the rounded O was the largest part of dQ's and dK's error there (3.6e-3 of the norm against 2.4e-3: 4 x 16 heads,
+  // 2048 positions, slopes). A value x is its bf16 plus o_low in units of 2^8 of its bits' value, whatever the exponent.
   constexpr bool PACKED = MASK != kMaskPlain, SPAN = MASK == kMaskSpan, CAP = MOD & kModCap;
   using L = kvdma::Lay<DH>;
   constexpr int kRowB = L::kRowB, kTile = L::kTile, kStage = L::kStage;
@@ -800,7 +817,9 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
   const int32_t* snd = SPAN ? span_end + (long)bidx * S : nullptr;
   const int32_t* sst = PACKED ? seg_start + (long)bidx * S : nullptr;
 
+  constexpr bool LOW = SPAN || MOD != kModNone;
   bf16x8 qf[kDK], df[DQ ? kDK : 1], of[DQ ? kDK : 1];
+  u32x2 low[DQ && LOW ? kDK : 1];
 #pragma unroll
   for (int ks = 0; ks < kDK; ++ks)
     qf[ks] = qvalid ? as_bf16x8(*reinterpret_cast<const u32x4*>(q + (qrow + qi) * DH + 16 * ks + 8 * hf)) : as_bf16x8(zero4());
@@ -813,6 +832,11 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
 #pragma unroll
     for (int ks = 0; ks < kDK; ++ks)
       of[ks] = qvalid ? as_bf16x8(*reinterpret_cast<const u32x4*>(o_in + (qrow + qi) * DH + 16 * ks + 8 * hf)) : as_bf16x8(zero4());
+    if constexpr (LOW) {
+#pragma unroll
+      for (int ks = 0; ks < kDK; ++ks)
+        low[ks] = qvalid ? *reinterpret_cast<const u32x2*>(o_low + (qrow + qi) * DH + 16 * ks + 8 * hf) : u32x2{0, 0};
+    }
   }
 
   const int wg_q0 = pb * P;
@@ -860,6 +884,14 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
   };
   if constexpr (FIXED) score.add -= fixed_top();
   float m = FIXED ? 0.f : kNegInf, l = 0.f;
+  // Spans, caps and biases: O is divided by the sum of the bf16 probabilities that it was formed from, L is of the exact
+  // sum. The probabilities' roundings then shift O, and D with it, only by what dP differs between keys, which is what dS is
+  // made of: with the exact sum dQ's and dK's error grew to 5.9e-3 of the norm in rows of 2 to 8 keys, and is 3.0e-3 at most.
+  float lr = 0.f;
+  auto add_rounded = [&](const bf16x8& p) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) lr = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{p[j], p[j + 1]}, bf16x2{(__bf16)1.f, (__bf16)1.f}, lr, false);
+  };
   f32x16 acc[kDB];
 #pragma unroll
   for (int db = 0; db < kDB; ++db)
@@ -932,8 +964,14 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
 #pragma unroll
     for (int ks = 0; ks < kDK; ++ks) {
       asm volatile("" : "+v"(df[ks]), "+v"(of[ks]));
+      if constexpr (LOW) asm volatile("" : "+v"(low[ks]));
 #pragma unroll
-      for (int j = 0; j < 8; ++j) dp = __builtin_fmaf((float)df[ks][j], (float)of[ks][j], dp);
+      for (int j = 0; j < 8; ++j) {
+        float x = (float)of[ks][j];
+        if constexpr (LOW)
+          x = __builtin_bit_cast(float, __builtin_bit_cast(int, x) + (((int)(low[ks][j >> 2] << (24 - 8 * (j & 3))) >> 24) << 8));
+        dp = __builtin_fmaf((float)df[ks][j], x, dp);
+      }
     }
     dq_row = sum_xhalf(dp);
     if (qvalid && hf == 0) dvec[qrow + qi] = dq_row;
@@ -1203,6 +1241,7 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
           const float alpha = up ? fast_exp2(m - mt) : 1.f;  // m = -inf: alpha = 0 (O, l are 0)
           m = up ? mt : m;
           l *= alpha;
+          lr *= alpha;
 #pragma unroll
           for (int db = 0; db < kDB; ++db)
 #pragma unroll
@@ -1214,6 +1253,10 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
         }
         }
         l += l0;
+        if constexpr (LOW) {
+          add_rounded(pf[0]);
+          add_rounded(pf[1]);
+        }
         // O^T += V^T P^T: half 0's two 16-key slabs, each product followed by an even share of half
         // 1's probabilities, then half 1's slabs.
         slab_wait<0, kDB>(tf[0]);
@@ -1235,6 +1278,10 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
         for (int ks = 2; ks < 4; ++ks)
 #pragma unroll
           for (int db = 0; db < kDB; ++db) acc[db] = mfma32(tf[ks][db], pf[ks], acc[db]);
+        if constexpr (LOW) {
+          add_rounded(pf[2]);
+          add_rounded(pf[3]);
+        }
       }
     }
     // This wave's copies of tile t+1 landed; after the barrier nobody reads `cur`, which takes t+2.
@@ -1255,7 +1302,8 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
   float mul = (DQ && CAP) ? -4.f * scale : scale, lt = 0.f;  // (Score::bend)
   if constexpr (!DQ) {
     lt = l + __shfl_xor(l, 32, 64);
-    mul = (lt > 0.f) ? 1.f / lt : 0.f;
+    const float by = LOW ? lr + __shfl_xor(lr, 32, 64) : lt;
+    mul = (by > 0.f) ? 1.f / by : 0.f;
   }
   if constexpr (!DQ) {
     // A query that sees nothing: L = +inf, so that the backward's probabilities exp(S - L) are 0.
@@ -1265,6 +1313,33 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
     return u32x2{pack_bf16x2(acc[db][4 * rq] * mul, acc[db][4 * rq + 1] * mul),
                  pack_bf16x2(acc[db][4 * rq + 2] * mul, acc[db][4 * rq + 3] * mul)};
   };
+  if constexpr (LOW && !DQ) {
+    if (o_low != nullptr && wave_has) {
+      // As O's below, through this wave's quarter of stage 1, rows of DH bytes 16 apart.
+      char* ob = lds1 + w * (32 * (DH + 16));
+#pragma unroll
+      for (int db = 0; db < kDB; ++db)
+#pragma unroll
+        for (int rq = 0; rq < 4; ++rq) {
+          const u32x2 x = quad(db, rq);
+          uint32_t bytes = 0;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int top = (int)((u & 1) ? x[u >> 1] & 0xffff0000u : x[u >> 1] << 16);
+            const int rest = (__builtin_bit_cast(int, acc[db][4 * rq + u] * mul) - top + 0x80) >> 8;  // in [-128, 128]
+            bytes |= (uint32_t)((rest < 127 ? rest : 127) & 0xff) << (8 * u);
+          }
+          *reinterpret_cast<uint32_t*>(ob + col * (DH + 16) + 32 * db + 8 * rq + 4 * hf) = bytes;
+        }
+      int8_t* lh = o_low + (qrow + qw0) * DH;
+#pragma unroll
+      for (int p = 0; p < DH / 32; ++p) {
+        const int id = lane + 64 * p, row = id / (DH / 16), c = id % (DH / 16);
+        const u32x4 x = *reinterpret_cast<const u32x4*>(ob + row * (DH + 16) + 16 * c);
+        if (qw0 + row < S) *reinterpret_cast<u32x4*>(lh + row * DH + 16 * c) = x;
+      }
+    }
+  }
   if constexpr (DH == 96) {
     // Rows of 192 bytes, a line and a half: through LDS measured the same (88.8 and 89.0 us at
     // 2 x 16/4 x 2050, not causal).

@@ -108,18 +108,19 @@ size_t attn_scored_bwd_workspace(int b, int hq, int hkv, int s, int dh) {
 }
 
 hipError_t launch_attn_scored_fwd(const AttnShape& sh, const AttnScore& sc, const bf16_t* q, const bf16_t* k,
-                                  const bf16_t* v, bf16_t* o, float* lse, hipStream_t st) {
+                                  const bf16_t* v, bf16_t* o, int8_t* o_low, float* lse, hipStream_t st) {
   switch (sh.dh) {
-    case 64: return scored_fwd<64>(sh, sc, q, k, v, o, lse, q_grid(sh), st);
-    case 96: return scored_fwd<96>(sh, sc, q, k, v, o, lse, q_grid(sh), st);
-    case 128: return scored_fwd<128>(sh, sc, q, k, v, o, lse, q_grid(sh), st);
+    case 64: return scored_fwd<64>(sh, sc, q, k, v, o, o_low, lse, q_grid(sh), st);
+    case 96: return scored_fwd<96>(sh, sc, q, k, v, o, o_low, lse, q_grid(sh), st);
+    case 128: return scored_fwd<128>(sh, sc, q, k, v, o, o_low, lse, q_grid(sh), st);
     default: return hipErrorInvalidValue;
   }
 }
 
 hipError_t launch_attn_scored_bwd(const AttnShape& sh, const AttnScore& sc, const bf16_t* q, const bf16_t* k,
-                                  const bf16_t* v, const bf16_t* o, const float* lse, const bf16_t* d_o, bf16_t* dq,
-                                  bf16_t* dk, bf16_t* dv, void* workspace, hipStream_t st) {
+                                  const bf16_t* v, const bf16_t* o, const int8_t* o_low, const float* lse,
+                                  const bf16_t* d_o, bf16_t* dq, bf16_t* dk, bf16_t* dv, void* workspace,
+                                  hipStream_t st) {
   ScoredWorkspace ws;
   carve(sh.b, sh.hq, sh.hkv, sh.s, sh.dh, static_cast<char*>(workspace), &ws);
   ws.nsplit = scored_nsplit(sh, sc.start != nullptr);
@@ -132,9 +133,9 @@ hipError_t launch_attn_scored_bwd(const AttnShape& sh, const AttnScore& sc, cons
     if (e != hipSuccess) return e;
   }
   switch (sh.dh) {
-    case 64: e = scored_bwd<64>(sh, sc, ws, q, k, v, o, lse, d_o, dq, dk, dv, q_grid(sh), st); break;
-    case 96: e = scored_bwd<96>(sh, sc, ws, q, k, v, o, lse, d_o, dq, dk, dv, q_grid(sh), st); break;
-    case 128: e = scored_bwd<128>(sh, sc, ws, q, k, v, o, lse, d_o, dq, dk, dv, q_grid(sh), st); break;
+    case 64: e = scored_bwd<64>(sh, sc, ws, q, k, v, o, o_low, lse, d_o, dq, dk, dv, q_grid(sh), st); break;
+    case 96: e = scored_bwd<96>(sh, sc, ws, q, k, v, o, o_low, lse, d_o, dq, dk, dv, q_grid(sh), st); break;
+    case 128: e = scored_bwd<128>(sh, sc, ws, q, k, v, o, o_low, lse, d_o, dq, dk, dv, q_grid(sh), st); break;
     default: return hipErrorInvalidValue;
   }
   if (e != hipSuccess || ws.nsplit == 1) return e;

@@ -16,11 +16,11 @@ struct ScoredWorkspace {
 
 template <int DH>
 hipError_t scored_fwd(const AttnShape& sh, const AttnScore& sc, const bf16_t* q, const bf16_t* k, const bf16_t* v,
-                      bf16_t* o, float* lse, int grid, hipStream_t st);
+                      bf16_t* o, int8_t* o_low, float* lse, int grid, hipStream_t st);
 template <int DH>
 hipError_t scored_bwd(const AttnShape& sh, const AttnScore& sc, const ScoredWorkspace& ws, const bf16_t* q,
-                      const bf16_t* k, const bf16_t* v, const bf16_t* o, const float* lse, const bf16_t* d_o,
-                      bf16_t* dq, bf16_t* dk, bf16_t* dv, int grid, hipStream_t st);
+                      const bf16_t* k, const bf16_t* v, const bf16_t* o, const int8_t* o_low, const float* lse,
+                      const bf16_t* d_o, bf16_t* dq, bf16_t* dk, bf16_t* dv, int grid, hipStream_t st);
 
 // The forward under a cap of at most 80 ln 2 runs against a fixed maximum (attn_kv_kernel).
 constexpr float kFixedCap = 55.4f;
@@ -38,14 +38,15 @@ hipError_t with_mod(const AttnScore& sc, F&& f) {
 #ifdef MTP_SCORED_DH
 template <>
 hipError_t scored_fwd<MTP_SCORED_DH>(const AttnShape& sh, const AttnScore& sc, const bf16_t* q, const bf16_t* k,
-                                     const bf16_t* v, bf16_t* o, float* lse, int grid, hipStream_t st) {
+                                     const bf16_t* v, bf16_t* o, int8_t* o_low, float* lse, int grid,
+                                     hipStream_t st) {
   constexpr int DH = MTP_SCORED_DH;
   return with_mod(sc, [&](auto m) {
     constexpr int MOD = decltype(m)::value;
     auto launch = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, st, q, k, v, nullptr, nullptr, nullptr, nullptr, sc.end,
                          sc.start, o, lse, sh.b, sh.hq, sh.hkv, sh.s, sh.scale * kLog2e, sh.scale, sh.causal, nullptr,
-                         sc.cap, sc.slopes);
+                         sc.cap, sc.slopes, o_low);
       return hipGetLastError();
     };
     // A cap above kFixedCap runs as a cap with slopes of none; spans may hide a query's own key, whose bias of 0 the
@@ -67,7 +68,7 @@ hipError_t scored_fwd<MTP_SCORED_DH>(const AttnShape& sh, const AttnScore& sc, c
 template <>
 hipError_t scored_bwd<MTP_SCORED_DH>(const AttnShape& sh, const AttnScore& sc, const ScoredWorkspace& ws,
                                      const bf16_t* q, const bf16_t* k, const bf16_t* v, const bf16_t* o,
-                                     const float* lse, const bf16_t* d_o, bf16_t* dq, bf16_t* dk, bf16_t* dv, int grid,
+                                     const int8_t* o_low, const float* lse, const bf16_t* d_o, bf16_t* dq, bf16_t* dk, bf16_t* dv, int grid,
                                      hipStream_t st) {
   constexpr int DH = MTP_SCORED_DH;
   return with_mod(sc, [&](auto m) {
@@ -75,7 +76,7 @@ hipError_t scored_bwd<MTP_SCORED_DH>(const AttnShape& sh, const AttnScore& sc, c
     auto launch = [&](auto dq_kernel, auto dkv_kernel) {
       hipLaunchKernelGGL(dq_kernel, dim3(grid), dim3(256), 0, st, q, k, v, d_o, o, lse, ws.dvec, sc.end, sc.start, dq,
                          nullptr, sh.b, sh.hq, sh.hkv, sh.s, sh.scale * kLog2e, sh.scale, sh.causal, ws.q_order, sc.cap,
-                         sc.slopes);
+                         sc.slopes, const_cast<int8_t*>(o_low));
       hipError_t e = hipGetLastError();
       if (e != hipSuccess) return e;
       hipLaunchKernelGGL(dkv_kernel, dim3((sh.s + 127) / 128 * sh.b * sh.hkv * ws.nsplit), dim3(512), 0, st, q, k, v, d_o,

@@ -177,6 +177,7 @@ torch::autograd::variable_list once(const torch::autograd::variable_list& cotang
 struct Score {
   double softcap;  // 0: none
   at::Tensor slopes, start, end;
+  bool train;
 };
 const float* floats(const at::Tensor& t) { return t.defined() ? t.const_data_ptr<float>() : nullptr; }
 
@@ -187,6 +188,7 @@ struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
     const int64_t b = q.size(0), hq = q.size(1), s = q.size(2), dh = q.size(3), hkv = k.size(1);
     const at::Tensor o = at::empty_like(q), lse = at::empty({b, hq, s}, q.options().dtype(at::kFloat));
     const float cap = (float)score.softcap;
+    at::Tensor low;  // the bits of O below its bf16 ones, for the backward
     if (q.scalar_type() == at::kFloat) {
       const size_t bytes = g_api.scored_fwd_ws32(b, hq, hkv, s, dh);
       const at::Tensor ws = bytes ? at::empty({(int64_t)bytes}, q.options().dtype(at::kByte)) : at::Tensor();
@@ -194,10 +196,11 @@ struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
                                floats(score.slopes), ints(score.start), ints(score.end), ptr<float>(o), ptr<float>(lse),
                                opt_ptr(ws), bytes, stream_of(q)));
     } else {
+      if (score.train) low = at::empty_like(q, q.options().dtype(at::kChar));
       check(g_api.scored_fwd(ptr(q), ptr(k), ptr(v), b, hq, hkv, s, dh, (float)scale, causal, cap, floats(score.slopes),
-                             ints(score.start), ints(score.end), ptr(o), ptr<float>(lse), stream_of(q)));
+                             ints(score.start), ints(score.end), ptr(o), opt_ptr<int8_t>(low), ptr<float>(lse), stream_of(q)));
     }
-    ctx->save_for_backward({q, k, v, o, lse, score.slopes, score.start, score.end});
+    ctx->save_for_backward({q, k, v, o, low, lse, score.slopes, score.start, score.end});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["softcap"] = score.softcap;
@@ -209,8 +212,8 @@ struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
                                                  torch::autograd::variable_list grads) {
     count_backward(g_attn_calls, {"flash_attention", "flash_attention_kernel_bwd"});
     const auto saved = ctx->get_saved_variables();
-    const at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &o = saved[3], &lse = saved[4];
-    const at::Tensor &slopes = saved[5], &start = saved[6], &end = saved[7];
+    const at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &o = saved[3], &low = saved[4], &lse = saved[5];
+    const at::Tensor &slopes = saved[6], &start = saved[7], &end = saved[8];
     const float scale = (float)ctx->saved_data["scale"].toDouble(), cap = (float)ctx->saved_data["softcap"].toDouble();
     const bool causal = ctx->saved_data["causal"].toBool();
     const c10::DeviceGuard device(q.device());
@@ -225,7 +228,7 @@ struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
                                hq, hkv, s, dh, scale, causal, cap, floats(slopes), ints(start), ints(end), ptr<float>(dq),
                                ptr<float>(dk), ptr<float>(dv), ptr(ws), bytes, stream_of(q)));
     else
-      check(g_api.scored_bwd(ptr(q), ptr(k), ptr(v), ptr(o), ptr<float>(lse), ptr(d_o), b, hq, hkv, s, dh, scale, causal, cap,
+      check(g_api.scored_bwd(ptr(q), ptr(k), ptr(v), ptr(o), ptr<int8_t>(low), ptr<float>(lse), ptr(d_o), b, hq, hkv, s, dh, scale, causal, cap,
                              floats(slopes), ints(start), ints(end), ptr(dq), ptr(dk), ptr(dv), ptr(ws), bytes, stream_of(q)));
     return once(grads, {dq, dk, dv, at::Tensor(), at::Tensor(), at::Tensor()});
   }
@@ -521,7 +524,8 @@ at::Tensor scored_attention(const at::Tensor& q, const at::Tensor& k, const at::
                             const std::optional<at::Tensor>& start, const std::optional<at::Tensor>& end, double scale, bool causal,
                             double softcap) {
   const at::Tensor none;
-  const Score score{softcap, slopes.value_or(none), start.value_or(none), end.value_or(none)};
+  const Score score{softcap, slopes.value_or(none), start.value_or(none), end.value_or(none),
+                    at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad())};
   return apply_node([&] { return ScoredAttention::apply(q, k, v, score, scale, causal); });
 }
 

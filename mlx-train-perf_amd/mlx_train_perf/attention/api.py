@@ -278,27 +278,30 @@ class _KernelAttention(torch.autograd.Function):
         return dq, dk, dv, None, None, None, None
 
 
-def scored_forward(q, k, v, slopes, start, end, *, scale: float, causal: bool, softcap: float):
-    """(O, L) from mtp_attn_scored_fwd (_f32 for fp32 inputs); contiguous tensors on the GPU."""
+def scored_forward(q, k, v, slopes, start, end, *, scale: float, causal: bool, softcap: float, train: bool = True):
+    """(O, L, low) from mtp_attn_scored_fwd (_f32 for fp32 inputs); contiguous tensors on the GPU. low: the bits of a bf16
+    O's values that the backward needs beside it (None for fp32, and without `train`)."""
     lib = _native.load()
     b, hq, n, dh = q.shape
     o = torch.empty_like(q)
     lse = torch.empty((b, hq, n), dtype=torch.float32, device=q.device)
     shape = (b, hq, k.shape[1], n, dh)
     args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), *shape, scale, int(causal), softcap, _native.ptr(slopes), _native.ptr(start),
-            _native.ptr(end), o.data_ptr(), lse.data_ptr())
+            _native.ptr(end), o.data_ptr())
+    low = None
     with _native.on_device(q):
         if q.dtype == torch.float32:
             ws_bytes = lib.mtp_attn_scored_fwd_f32_workspace_bytes(*shape)
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-            rc = lib.mtp_attn_scored_fwd_f32(*args, _native.ptr(ws), ws_bytes, _native.stream_of(q))
+            rc = lib.mtp_attn_scored_fwd_f32(*args, lse.data_ptr(), _native.ptr(ws), ws_bytes, _native.stream_of(q))
         else:
-            rc = lib.mtp_attn_scored_fwd(*args, _native.stream_of(q))
+            low = torch.empty_like(q, dtype=torch.int8) if train else None
+            rc = lib.mtp_attn_scored_fwd(*args, _native.ptr(low), lse.data_ptr(), _native.stream_of(q))
     _native.check(rc, domain="attention")
-    return o, lse
+    return o, lse, low
 
 
-def scored_backward(q, k, v, o, lse, d_o, slopes, start, end, *, scale: float, causal: bool, softcap: float):
+def scored_backward(q, k, v, o, low, lse, d_o, slopes, start, end, *, scale: float, causal: bool, softcap: float):
     """(dQ, dK, dV) from mtp_attn_scored_bwd (_f32 for fp32 inputs)."""
     lib = _native.load()
     b, hq, n, dh = q.shape
@@ -308,8 +311,9 @@ def scored_backward(q, k, v, o, lse, d_o, slopes, start, end, *, scale: float, c
     ws_bytes = (lib.mtp_attn_scored_bwd_f32_workspace_bytes if f32 else lib.mtp_attn_scored_bwd_workspace_bytes)(b, hq, hkv, n, dh)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
     bwd = lib.mtp_attn_scored_bwd_f32 if f32 else lib.mtp_attn_scored_bwd
+    out = (o.data_ptr(),) if f32 else (o.data_ptr(), low.data_ptr())
     with _native.on_device(q):
-        rc = bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), d_o.data_ptr(), b, hq, hkv, n, dh,
+        rc = bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), *out, lse.data_ptr(), d_o.data_ptr(), b, hq, hkv, n, dh,
                  scale, int(causal), softcap, _native.ptr(slopes), _native.ptr(start), _native.ptr(end),
                  dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), ws_bytes, _native.stream_of(q))
     _native.check(rc, domain="attention")
@@ -321,8 +325,9 @@ class _ScoredAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, slopes, start, end, scale, causal, softcap):
-        o, lse = scored_forward(q, k, v, slopes, start, end, scale=scale, causal=causal, softcap=softcap)
-        ctx.save_for_backward(q, k, v, o, lse, slopes, start, end)
+        o, lse, low = scored_forward(q, k, v, slopes, start, end, scale=scale, causal=causal, softcap=softcap,
+                                     train=any(ctx.needs_input_grad))
+        ctx.save_for_backward(q, k, v, o, low, lse, slopes, start, end)
         ctx.scale, ctx.causal, ctx.softcap = scale, causal, softcap
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
@@ -333,9 +338,9 @@ class _ScoredAttention(torch.autograd.Function):
     def backward(ctx, d_o, _d_l):
         VJP_CALLS["flash_attention"] = VJP_CALLS.get("flash_attention", 0) + 1
         VJP_CALLS["flash_attention_kernel_bwd"] = VJP_CALLS.get("flash_attention_kernel_bwd", 0) + 1
-        q, k, v, o, lse, slopes, start, end = ctx.saved_tensors
+        q, k, v, o, low, lse, slopes, start, end = ctx.saved_tensors
         d_o = torch.zeros_like(o) if d_o is None else d_o.contiguous()
-        dq, dk, dv = scored_backward(q, k, v, o, lse, d_o, slopes, start, end, scale=ctx.scale, causal=ctx.causal,
+        dq, dk, dv = scored_backward(q, k, v, o, low, lse, d_o, slopes, start, end, scale=ctx.scale, causal=ctx.causal,
                                      softcap=ctx.softcap)
         return dq, dk, dv, None, None, None, None, None, None
 

@@ -120,8 +120,9 @@ def test_large_scores_and_far_keys(dtype):
 
 
 def test_spans_equal_the_masks_they_describe():
-    """A causal triangle, everything, and packed documents given as spans: the same visible pairs give the plain
-    kernels' results to the bit in O (the tiles walked are the same)."""
+    """A causal triangle, everything, and packed documents given as spans are the plain kernels' masks. Their O and the
+    span kernels' (which divide by the sum of the rounded probabilities) have two roundings each, of rms
+    2^-8 / sqrt(3) at most: 4.5e-3 together."""
     from mlx_train_perf.attention import PackedMask, SpanMask, document_spans, flash_attention
     from oracle import attention as oatt
 
@@ -131,11 +132,11 @@ def test_spans_equal_the_masks_they_describe():
     zero = torch.zeros_like(i)
     for causal, spans in ((True, SpanMask(start=zero, end=i + 1)), (False, SpanMask(start=zero, end=zero + s))):
         a = flash_attention(q, k, v, scale=0.1, causal=causal)
-        assert torch.equal(a, flash_attention(q, k, v, scale=0.1, spans=spans))
+        assert S.rel(flash_attention(q, k, v, scale=0.1, spans=spans), a.double()) <= 4.5e-3
     sid, sst = (t[None].cuda() for t in oatt.segments_from_lengths([100, 1, 77, 155]))
     seg = PackedMask(seg_id=sid, seg_start=sst)
     a = flash_attention(q, k, v, scale=0.1, segments=seg)
-    assert torch.equal(a, flash_attention(q, k, v, scale=0.1, spans=document_spans(seg)))
+    assert S.rel(flash_attention(q, k, v, scale=0.1, spans=document_spans(seg)), a.double()) <= 4.5e-3
     capped = flash_attention(q, k, v, scale=0.1, segments=seg, softcap=7.0)
     assert torch.equal(capped, flash_attention(q, k, v, scale=0.1, spans=document_spans(seg), softcap=7.0))
 
@@ -284,8 +285,9 @@ def test_fp32_without_room_for_parts():
     q, k, v, d_o = (x.cuda() for x in S.inputs(b, hq, hkv, s, dh, torch.float32, 3))
     slopes = S.slopes_of(hq).cuda()
     args = {"scale": 0.125, "causal": True, "softcap": 9.0}
-    o, lse = scored_forward(q, k, v, slopes, None, None, **args)
-    grads = scored_backward(q, k, v, o, lse, d_o, slopes, None, None, **args)
+    o, lse, low = scored_forward(q, k, v, slopes, None, None, **args)
+    assert low is None   # bf16's alone
+    grads = scored_backward(q, k, v, o, low, lse, d_o, slopes, None, None, **args)
     o1, lse1 = torch.empty_like(o), torch.empty_like(lse)
     outs = [torch.empty_like(x) for x in (q, k, v)]
     ws = torch.empty(b * hq * s, device="cuda")
@@ -362,3 +364,23 @@ def test_second_derivative_is_refused(node, monkeypatch):
     assert torch.equal(dq, want[0]) and torch.equal(dk, want[1])
     with pytest.raises(RuntimeError, match="differentiate twice"):
         (dq.square().sum() + o.sum()).backward()
+
+
+@pytest.mark.parametrize(("cap", "biased"), [(None, True), (20.0, False), (20.0, True), (None, False)])
+@pytest.mark.parametrize(("s", "w"), [(17, 2), (200, 3), (200, 6)])
+@pytest.mark.parametrize("dh", [64, 96, 128])
+def test_gradients_of_rows_with_few_keys(dh, s, w, cap, biased):
+    """dS = P (dP - D) all but cancels here, so that an error of D shows: D comes from more bits of O than bf16's, and O is
+    divided by the sum of the rounded probabilities. What is left in dq and dk are the roundings of those (by
+    sum_j dP_j (P_j' - P_j), which is of dS's own size as both sum to 1), of dS and of the output, each of rms
+    2^-8 / sqrt(3) at most: 3.9e-3 together."""
+    hq, hkv = 4, 2
+    q, k, v, d_o = (x.cuda() for x in S.inputs(1, hq, hkv, s, dh, torch.bfloat16, w))
+    i = torch.arange(s, dtype=torch.int32)[None]
+    spans = ((i - w + 1).clamp(min=0).to(torch.int32), i + 1)
+    slopes = torch.tensor([0.7, 0.3, 0.1, 0.01]).cuda() if biased else None
+    got = _call(q, k, v, d_o, mask="window", spans=spans, scale=dh ** -0.5, softcap=cap, slopes=slopes)
+    see = S.visible("window", spans, 1, s, "cuda")
+    want = S.attention(q, k, v, d_o, scale=dh ** -0.5, see=see, softcap=cap, slopes=slopes)
+    for name, a, x in zip(("dq", "dk"), got[1:], want[1:]):
+        assert S.rel(a, x) <= 4e-3, name
