@@ -292,7 +292,7 @@ int mtp_attn_bwd_f32(const float* q, const float* k, const float* v, const float
  *     gets o = 0, lse = +inf and no gradient. Spans are the whole mask (causal must be 0). Values outside the
  *     row are clamped into it; spans that decrease give some wrong rows, never an access out of range.
  * scale must be positive, softcap 0 or in [1e-3, 1e3], slopes of either sign. At least one of the three must be
- * given (else: mtp_attn_fwd). What a query does not see must be finite all the same: v, and in the backward k and d_o.
+ * given (else: mtp_attn_fwd). What the mask hides must be finite all the same, padding too: v, and in the backward q, k and d_o.
  * o_low: int8 [b][hq][s][dh], the 8 bits of the output below its bf16 ones (bits of x = bits of bf16(x) + 2^8 o_low), for
  * the backward's D = rowsum(d_o o); NULL in a forward without a backward.
  * ------------------------------------------------------------------------------------------- */

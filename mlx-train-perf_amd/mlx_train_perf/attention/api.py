@@ -382,8 +382,8 @@ def flash_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale:
     slopes go with either). A query that sees nothing gets zeros and no gradient. `validate_segments` checks the
     contract of `spans` too, at one host sync a mask.
     The kernel impl takes a softcap in [1e-3, 1e3], with any of the three a scale above 0, and slopes of either sign of
-    up to some hundreds. As in a plain product, a hidden V (and in the backward a hidden K or dO) must be finite: 0 is
-    what it is multiplied by. These calls differentiate once."""
+    up to some hundreds. As in a plain product, what the mask hides must be finite, padding too (V; in the backward Q,
+    K and dO): 0 is what it is multiplied by. These calls differentiate once."""
     resolved = resolve_attention_impl(q, k, v, impl=impl, causal=causal, segments=segments,
                                       validate_segments=validate_segments, softcap=softcap, slopes=slopes, spans=spans)
     scored = softcap is not None or slopes is not None or spans is not None

@@ -67,7 +67,7 @@ class SpanMask:
     start[b, i] <= j < end[b, i], whether they come before it or after.
 
     Neither tensor may decrease along a row, and both lie in [0, N]. A query whose range holds nothing (padding)
-    gets an output of zeros and takes part in no gradient. A window of w keys is start = i - w + 1, end = i + 1.
+    gets an output of zeros and takes part in no gradient. A window of w keys is start = max(0, i - w + 1), end = i + 1.
 
     A mask remembers that its contract was checked (a host sync), for as long as neither tensor is written to, so that
     a model's layers check the mask of a step once (tensors made in inference mode do not tell of writes: checked each time).
