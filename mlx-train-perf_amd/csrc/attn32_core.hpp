@@ -225,7 +225,7 @@ void attn32_q_kernel(const float* __restrict__ q, const float* __restrict__ k, c
                      const int32_t* __restrict__ span_end, float cap, const float* __restrict__ slopes, int nsplit,
                      float* __restrict__ part) {
   // seg_start: the first key that each query sees (packed: its segment's start; span: its span's).
-  // Scored calls of few workgroups are split (attn32_q_splits): workgroup `split` of a pair of blocks takes every
+  // Scored calls of few workgroups are split (q_splits, attn32_scored.hip): workgroup `split` of a pair of blocks takes every
   // nsplit-th key tile from tile `split` on, and writes its dQ, or its unnormalized O, maximum and sum, to
   // part[split] ([b][hq][s][dh], the forward's maxima and sums [split][b][hq][s][2] behind all of them).
   constexpr bool PACKED = MASK != kMaskPlain, SPAN = MASK == kMaskSpan, CAP = MOD & kModCap;
