@@ -80,11 +80,20 @@ int q_grid(const AttnShape& sh) {
   const int P = wg_rows(sh.hq, sh.hkv);
   return (sh.s + P - 1) / P * sh.b * (sh.hq / wg_heads(sh.hq, sh.hkv));
 }
-// Splits of the dK/dV pass: the size table of the causal mask, also for spans, whose layout is on the device.
-int scored_nsplit(const AttnShape& sh, bool span) { return attn_dkv_nsplit(sh.b, sh.hq, sh.hkv, sh.s, sh.dh, span ? 1 : sh.causal); }
+// Splits of the dK/dV pass: as many as the plain kernels' table has (for spans, whose layout is on the device, the causal
+// mask's), but a split of a key block has at least 2 of its (head, query tile) items where all workgroups run at once, and
+// 16 where they take turns: below that its start and the sum of the parts outweigh the shorter walk. A whole step, split
+// 8, 4, 2 and 1 times: 4 x 16/4 x 509 x 128 89, 79, 90 and 113 us (4 taken); 2 x 8/8 x 700 x 64 71, 60, 59 and 60 (2);
+// 2 x 8/2 x 300 x 128 59, 62, 70 and 86 (8); 1 x 16/8 x 4000 x 128 400 split twice, 472 not at all (2).
+int scored_nsplit(int b, int hq, int hkv, int s, int dh, int causal) {
+  int ns = attn_dkv_nsplit(b, hq, hkv, s, dh, causal);
+  const long wgs = (long)(s + 127) / 128 * b * hkv, items = (long)hq / hkv * ((s + 63) / 64);
+  while (ns > 1 && items < ns * (wgs * ns <= kNumCU + kNumCU / 4 ? 2 : 16)) ns /= 2;
+  return ns;
+}
 // The parts of a workspace from `base` (null: sizes alone), with room for the larger split of the two masks; returns the bytes.
 size_t carve(int b, int hq, int hkv, int s, int dh, char* base, ScoredWorkspace* ws) {
-  const int ns1 = attn_dkv_nsplit(b, hq, hkv, s, dh, 1), ns0 = attn_dkv_nsplit(b, hq, hkv, s, dh, 0);
+  const int ns1 = scored_nsplit(b, hq, hkv, s, dh, 1), ns0 = scored_nsplit(b, hq, hkv, s, dh, 0);
   const int ns = ns1 > ns0 ? ns1 : ns0, P = wg_rows(hq, hkv);
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -123,7 +132,7 @@ hipError_t launch_attn_scored_bwd(const AttnShape& sh, const AttnScore& sc, cons
                                   hipStream_t st) {
   ScoredWorkspace ws;
   carve(sh.b, sh.hq, sh.hkv, sh.s, sh.dh, static_cast<char*>(workspace), &ws);
-  ws.nsplit = scored_nsplit(sh, sc.start != nullptr);
+  ws.nsplit = scored_nsplit(sh.b, sh.hq, sh.hkv, sh.s, sh.dh, sc.start ? 1 : sh.causal);
   hipError_t e = hipSuccess;
   if (sc.start) {
     const unsigned fill = (unsigned)(((long)sh.b * sh.s + 1023) / 1024);

@@ -384,3 +384,10 @@ def test_gradients_of_rows_with_few_keys(dh, s, w, cap, biased):
     want = S.attention(q, k, v, d_o, scale=dh ** -0.5, see=see, softcap=cap, slopes=slopes)
     for name, a, x in zip(("dq", "dk"), got[1:], want[1:]):
         assert S.rel(a, x) <= 4e-3, name
+
+
+@pytest.mark.parametrize(("b", "hq", "hkv", "s", "dh"), [(1, 4, 4, 100, 64), (1, 8, 8, 700, 64), (2, 16, 4, 509, 128), (2, 8, 2, 300, 96)])
+@pytest.mark.parametrize(("mask", "cap", "biased"), [("causal", 20.0, False), ("prefix", None, False), ("full", None, True)])
+def test_splits_of_the_key_blocks(b, hq, hkv, s, dh, mask, cap, biased):
+    """dK/dV of a key block by one workgroup, and by two, four and eight."""
+    _check(b, hq, hkv, s, dh, mask=mask, cap=cap, biased=biased, dtype=torch.bfloat16, seed=s)
