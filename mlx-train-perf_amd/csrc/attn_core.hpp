@@ -237,6 +237,27 @@ __device__ __forceinline__ int first_above(const int32_t* a, int lo, int hi, int
   return lo;
 }
 
+// The queries [begin, end) that see keys x to y: as start and end do not decrease along a row, those from the first with
+// end > x to the first with start > y. The two searches run side by side: each is a chain of dependent loads, a quarter
+// of a microsecond a link.
+__device__ __forceinline__ void queries_of(const int32_t* start, const int32_t* end, int S, int x, int y, int& qb, int& qe) {
+  int lo0 = 0, hi0 = S, lo1 = 0, hi1 = S;
+  while (lo0 < hi0 || lo1 < hi1) {
+    const int m0 = (lo0 + hi0) >> 1, m1 = (lo1 + hi1) >> 1;
+    const int v0 = end[m0 < S ? m0 : S - 1], v1 = start[m1 < S ? m1 : S - 1];
+    if (lo0 < hi0) {
+      if (v0 > x) hi0 = m0;
+      else lo0 = m0 + 1;
+    }
+    if (lo1 < hi1) {
+      if (v1 > y) hi1 = m1;
+      else lo1 = m1 + 1;
+    }
+  }
+  qb = lo0;
+  qe = lo1;
+}
+
 // Counting sort of the work items 0 .. n - 1 of one workgroup of 1024 threads by cost(i) < kSchedBuckets,
 // highest first: order[r] is the item of rank r. Items of one cost land in any order.
 constexpr int kSchedBuckets = 2048;
@@ -769,7 +790,7 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
                     const int32_t* __restrict__ seg_start, bf16_t* __restrict__ out, float* __restrict__ lse_out,
                     int B, int Hq, int Hkv, int S, float scale_log2, float scale, int causal,
                     const int32_t* __restrict__ order, float cap, const float* __restrict__ slopes,
-                    int8_t* __restrict__ o_low) {
+                    int8_t* __restrict__ o_low, int32_t* __restrict__ col_begin, int32_t* __restrict__ col_end) {
   // seg_start: the first key that each query sees (packed: its segment's start; span: its span's).
   // o_low (spans, caps and biases): the 8 bits of O below bf16's, written by the forward where given, read with O for
   // D = rowsum(dO o O). dS = P (dP - D) is a difference that all but cancels where one probability is nearly 1, and
@@ -827,6 +848,17 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
   const int32_t* sst = PACKED ? seg_start + (long)bidx * S : nullptr;
 
   constexpr bool LOW = SPAN || MOD != kModNone;
+  // A span backward without work orders: the queries that see each key, for the dK/dV pass (attn_scored.hip), each by the
+  // workgroup of the first heads whose queries stand where the key does.
+  if constexpr (SPAN && DQ) {
+    if (col_begin != nullptr && h0 == 0 && tid < P && pb * P + tid < S) {
+      int qb, qe;
+      queries_of(sst, snd, S, pb * P + tid, pb * P + tid, qb, qe);
+      col_begin[(long)bidx * S + pb * P + tid] = qb;
+      col_end[(long)bidx * S + pb * P + tid] = qe;
+    }
+  }
+
   bf16x8 qf[kDK], df[DQ ? kDK : 1], of[DQ ? kDK : 1];
   u32x2 low[DQ && LOW ? kDK : 1];
 #pragma unroll

@@ -4,27 +4,6 @@
 
 namespace mtp {
 
-// The queries [begin, end) that see keys x to y: as start and end do not decrease along a row, those from the first with
-// end > x to the first with start > y. The two searches run side by side: each is a chain of dependent loads, a quarter
-// of a microsecond a link.
-__device__ __forceinline__ void queries_of(const int32_t* start, const int32_t* end, int S, int x, int y, int& qb, int& qe) {
-  int lo0 = 0, hi0 = S, lo1 = 0, hi1 = S;
-  while (lo0 < hi0 || lo1 < hi1) {
-    const int m0 = (lo0 + hi0) >> 1, m1 = (lo1 + hi1) >> 1;
-    const int v0 = end[m0 < S ? m0 : S - 1], v1 = start[m1 < S ? m1 : S - 1];
-    if (lo0 < hi0) {
-      if (v0 > x) hi0 = m0;
-      else lo0 = m0 + 1;
-    }
-    if (lo1 < hi1) {
-      if (v1 > y) hi1 = m1;
-      else lo1 = m1 + 1;
-    }
-  }
-  qb = lo0;
-  qe = lo1;
-}
-
 // Workgroup 0 orders the B npb query blocks of the dQ pass (P queries each), workgroup 1 the B nkb 128-key blocks of
 // the dK/dV pass, most tiles first; the others fill, for each key, the queries [col_begin, col_end) that see it. Costs are
 // looked up twice by the sort, so the first kSchedCosts are kept: 7.3 us at 8192 positions (12.9 with the two searches one
@@ -134,7 +113,12 @@ hipError_t launch_attn_scored_bwd(const AttnShape& sh, const AttnScore& sc, cons
   carve(sh.b, sh.hq, sh.hkv, sh.s, sh.dh, static_cast<char*>(workspace), &ws);
   ws.nsplit = scored_nsplit(sh.b, sh.hq, sh.hkv, sh.s, sh.dh, sc.start ? 1 : sh.causal);
   hipError_t e = hipSuccess;
-  if (sc.start) {
+  // Where all workgroups of both passes run at once their order is of no account, and the dQ pass fills the key ranges
+  // that the dK/dV pass reads: a launch less (a step of 4 x 16/8 x 509 x 64: 63.2 against
+  // 67.5 us of GPU time, 1 x 8/8 x 100 x 128 37.0 against 41.2).
+  const bool ordered = q_grid(sh) > 2 * kNumCU || (long)(sh.s + 127) / 128 * sh.b * sh.hkv * ws.nsplit > kNumCU;
+  if (sc.start && !ordered) ws.q_order = ws.kv_order = nullptr;
+  if (sc.start && ordered) {
     const unsigned fill = (unsigned)(((long)sh.b * sh.s + 1023) / 1024);
     hipLaunchKernelGGL(attn_span_sched_kernel, dim3(2 + fill), dim3(1024), 0, st, sc.start, sc.end, sh.b, sh.s,
                        wg_rows(sh.hq, sh.hkv), ws.q_order, ws.kv_order, ws.col_begin, ws.col_end);

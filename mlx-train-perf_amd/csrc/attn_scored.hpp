@@ -6,7 +6,7 @@
 namespace mtp {
 
 // A backward call's workspace, in order: D, the fp32 partials of a split dK/dV pass, and for spans the two work
-// orders and the queries [col_begin, col_end) that see each key.
+// orders (null: none) and the queries [col_begin, col_end) that see each key.
 struct ScoredWorkspace {
   float* dvec;
   float* part;
@@ -46,7 +46,7 @@ hipError_t scored_fwd<MTP_SCORED_DH>(const AttnShape& sh, const AttnScore& sc, c
     auto launch = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, st, q, k, v, nullptr, nullptr, nullptr, nullptr, sc.end,
                          sc.start, o, lse, sh.b, sh.hq, sh.hkv, sh.s, sh.scale * kLog2e, sh.scale, sh.causal, nullptr,
-                         sc.cap, sc.slopes, o_low);
+                         sc.cap, sc.slopes, o_low, nullptr, nullptr);
       return hipGetLastError();
     };
     // A cap above kFixedCap runs as a cap with slopes of none; spans may hide a query's own key, whose bias of 0 the
@@ -76,7 +76,8 @@ hipError_t scored_bwd<MTP_SCORED_DH>(const AttnShape& sh, const AttnScore& sc, c
     auto launch = [&](auto dq_kernel, auto dkv_kernel) {
       hipLaunchKernelGGL(dq_kernel, dim3(grid), dim3(256), 0, st, q, k, v, d_o, o, lse, ws.dvec, sc.end, sc.start, dq,
                          nullptr, sh.b, sh.hq, sh.hkv, sh.s, sh.scale * kLog2e, sh.scale, sh.causal, ws.q_order, sc.cap,
-                         sc.slopes, const_cast<int8_t*>(o_low));
+                         sc.slopes, const_cast<int8_t*>(o_low), ws.q_order ? nullptr : ws.col_begin,
+                         ws.q_order ? nullptr : ws.col_end);
       hipError_t e = hipGetLastError();
       if (e != hipSuccess) return e;
       hipLaunchKernelGGL(dkv_kernel, dim3((sh.s + 127) / 128 * sh.b * sh.hkv * ws.nsplit), dim3(512), 0, st, q, k, v, d_o,

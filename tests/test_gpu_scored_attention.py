@@ -386,8 +386,10 @@ def test_gradients_of_rows_with_few_keys(dh, s, w, cap, biased):
         assert S.rel(a, x) <= 4e-3, name
 
 
-@pytest.mark.parametrize(("b", "hq", "hkv", "s", "dh"), [(1, 4, 4, 100, 64), (1, 8, 8, 700, 64), (2, 16, 4, 509, 128), (2, 8, 2, 300, 96)])
+@pytest.mark.parametrize(("b", "hq", "hkv", "s", "dh"), [(1, 4, 4, 100, 64), (1, 8, 8, 700, 64), (2, 16, 4, 509, 128), (2, 8, 2, 300, 96),
+                                                    (4, 32, 8, 900, 64)])
 @pytest.mark.parametrize(("mask", "cap", "biased"), [("causal", 20.0, False), ("prefix", None, False), ("full", None, True)])
 def test_splits_of_the_key_blocks(b, hq, hkv, s, dh, mask, cap, biased):
-    """dK/dV of a key block by one workgroup, and by two, four and eight."""
+    """dK/dV of a key block by one workgroup, and by two, four and eight; more workgroups than run at once, in work orders
+    under spans."""
     _check(b, hq, hkv, s, dh, mask=mask, cap=cap, biased=biased, dtype=torch.bfloat16, seed=s)
