@@ -847,7 +847,7 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
   const int32_t* snd = SPAN ? span_end + (long)bidx * S : nullptr;
   const int32_t* sst = PACKED ? seg_start + (long)bidx * S : nullptr;
 
-  constexpr bool LOW = SPAN || MOD != kModNone;
+  constexpr bool SCORED = SPAN || MOD != kModNone;
   // A span backward without work orders: the queries that see each key, for the dK/dV pass (attn_scored.hip), each by the
   // workgroup of the first heads whose queries stand where the key does.
   if constexpr (SPAN && DQ) {
@@ -860,7 +860,7 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
   }
 
   bf16x8 qf[kDK], df[DQ ? kDK : 1], of[DQ ? kDK : 1];
-  u32x2 low[DQ && LOW ? kDK : 1];
+  u32x2 low[DQ && SCORED ? kDK : 1];
 #pragma unroll
   for (int ks = 0; ks < kDK; ++ks)
     qf[ks] = qvalid ? as_bf16x8(*reinterpret_cast<const u32x4*>(q + (qrow + qi) * DH + 16 * ks + 8 * hf)) : as_bf16x8(zero4());
@@ -873,7 +873,7 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
 #pragma unroll
     for (int ks = 0; ks < kDK; ++ks)
       of[ks] = qvalid ? as_bf16x8(*reinterpret_cast<const u32x4*>(o_in + (qrow + qi) * DH + 16 * ks + 8 * hf)) : as_bf16x8(zero4());
-    if constexpr (LOW) {
+    if constexpr (SCORED) {
 #pragma unroll
       for (int ks = 0; ks < kDK; ++ks)
         low[ks] = qvalid ? *reinterpret_cast<const u32x2*>(o_low + (qrow + qi) * DH + 16 * ks + 8 * hf) : u32x2{0, 0};
@@ -1005,11 +1005,11 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
 #pragma unroll
     for (int ks = 0; ks < kDK; ++ks) {
       asm volatile("" : "+v"(df[ks]), "+v"(of[ks]));
-      if constexpr (LOW) asm volatile("" : "+v"(low[ks]));
+      if constexpr (SCORED) asm volatile("" : "+v"(low[ks]));
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         float x = (float)of[ks][j];
-        if constexpr (LOW)
+        if constexpr (SCORED)
           x = __builtin_bit_cast(float, __builtin_bit_cast(int, x) + (((int)(low[ks][j >> 2] << (24 - 8 * (j & 3))) >> 24) << 8));
         dp = __builtin_fmaf((float)df[ks][j], x, dp);
       }
@@ -1294,7 +1294,7 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
         }
         }
         l += l0;
-        if constexpr (LOW) {
+        if constexpr (SCORED) {
           add_rounded(pf[0]);
           add_rounded(pf[1]);
         }
@@ -1319,7 +1319,7 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
         for (int ks = 2; ks < 4; ++ks)
 #pragma unroll
           for (int db = 0; db < kDB; ++db) acc[db] = mfma32(tf[ks][db], pf[ks], acc[db]);
-        if constexpr (LOW) {
+        if constexpr (SCORED) {
           add_rounded(pf[2]);
           add_rounded(pf[3]);
         }
@@ -1343,7 +1343,7 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
   float mul = (DQ && CAP) ? -4.f * scale : scale, lt = 0.f;  // (Score::bend)
   if constexpr (!DQ) {
     lt = l + __shfl_xor(l, 32, 64);
-    const float by = LOW ? lr + __shfl_xor(lr, 32, 64) : lt;
+    const float by = SCORED ? lr + __shfl_xor(lr, 32, 64) : lt;
     mul = (by > 0.f) ? 1.f / by : 0.f;
   }
   if constexpr (!DQ) {
@@ -1354,7 +1354,7 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
     return u32x2{pack_bf16x2(acc[db][4 * rq] * mul, acc[db][4 * rq + 1] * mul),
                  pack_bf16x2(acc[db][4 * rq + 2] * mul, acc[db][4 * rq + 3] * mul)};
   };
-  if constexpr (LOW && !DQ) {
+  if constexpr (SCORED && !DQ) {
     if (o_low != nullptr && wave_has) {
       // As O's below, through this wave's quarter of stage 1, rows of DH bytes 16 apart.
       char* ob = lds1 + w * (32 * (DH + 16));

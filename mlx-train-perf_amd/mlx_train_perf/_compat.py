@@ -5,6 +5,8 @@ architecture (unless `allow_unverified=True`), instead of failing inside a launc
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 VERIFIED_ARCHS = ("gfx950",)
@@ -15,13 +17,16 @@ def device_arch(device: torch.device | int | None = None) -> str:
     return getattr(props, "gcnArchName", "").split(":")[0]
 
 
+_arch_of = functools.lru_cache(maxsize=None)(device_arch)   # by index: a GPU does not change (1 us a call)
+
+
 def check_device_verified(*, allow_unverified: bool, error: type[Exception]) -> None:
     if not torch.cuda.is_available():
         raise error("kernel impl requires an MI355X (gfx950) GPU; none is visible. Use impl='chunked' / "
                     "impl='reference' on CPU.")
     if allow_unverified:
         return
-    arch = device_arch()
+    arch = _arch_of(torch.cuda.current_device())
     if arch not in VERIFIED_ARCHS:
         raise error(f"kernel impl is built for {VERIFIED_ARCHS}; device reports {arch!r} "
                     "(pass allow_unverified_mlx=True to try anyway)")
