@@ -105,9 +105,9 @@ def _validate_score(q: torch.Tensor, softcap: float | None, slopes: torch.Tensor
         if segments is not None:
             raise AttentionInputError("give segments or spans, not both: spans are the whole mask")
         for name, t in (("start", spans.start), ("end", spans.end)):
-            if tuple(t.shape) != (b, n):
+            if t.shape != (b, n):
                 raise AttentionInputError(f"spans.{name} must have shape (B, N)=({b}, {n}); got {tuple(t.shape)}")
-            if t.dtype.is_floating_point or t.dtype == torch.bool or t.dtype.is_complex:
+            if t.dtype is not torch.int32 and (t.dtype.is_floating_point or t.dtype == torch.bool or t.dtype.is_complex):
                 raise AttentionInputError(f"spans.{name} must be an integer tensor; got {t.dtype}")
         if check_spans:
             problem = spans.violation()
@@ -345,6 +345,12 @@ class _ScoredAttention(torch.autograd.Function):
         return dq, dk, dv, None, None, None, None, None, None
 
 
+def _int32_on(t: torch.Tensor, device: torch.device) -> torch.Tensor:
+    if t.dtype is not torch.int32 or t.device != device:   # (asked first: a call that changes nothing costs 1 us)
+        t = t.to(device=device, dtype=torch.int32)
+    return t.contiguous()
+
+
 def _scored_attention(q, k, v, *, scale, causal, segments, softcap, slopes, spans):
     """The kernel impl of a call with softcap, slopes or spans. Packed segments go as spans."""
     if segments is not None:
@@ -352,7 +358,7 @@ def _scored_attention(q, k, v, *, scale, causal, segments, softcap, slopes, span
     start = end = None
     if spans is not None:
         causal = False
-        start, end = (t.to(device=q.device, dtype=torch.int32).contiguous() for t in (spans.start, spans.end))
+        start, end = _int32_on(spans.start, q.device), _int32_on(spans.end, q.device)
     if slopes is not None:
         slopes = slopes.detach().to(torch.float32).contiguous()
     args = (q.contiguous(), k.contiguous(), v.contiguous(), slopes, start, end, float(scale), bool(causal), float(softcap or 0.0))

@@ -78,12 +78,14 @@ class SpanMask:
 
     def violation(self) -> str | None:
         """`span_violation` of this mask, unless it was found to be none before."""
-        tells = not (self.start.is_inference() or self.end.is_inference())
-        versions = [self.start._version, self.end._version] if tells else []
-        if tells and self._checked == versions:
+        start, end = self.start, self.end
+        if start.is_inference() or end.is_inference():
+            return span_violation(self)
+        versions = [start._version, end._version]
+        if self._checked == versions:
             return None
         problem = span_violation(self)
-        if problem is None and tells:
+        if problem is None:
             self._checked[:] = versions
         return problem
 
