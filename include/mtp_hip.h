@@ -301,7 +301,7 @@ int mtp_attn_scored_fwd(const void* q, const void* k, const void* v, int64_t b, 
                         const float* slopes, const int32_t* span_start, const int32_t* span_end, void* o,
                         int8_t* o_low, float* lse, void* stream);
 
-/* Workspace bytes of mtp_attn_scored_bwd, each part padded to 256 bytes: D (fp32 [b][hq][s]), the fp32 dK/dV
+/* Workspace bytes of mtp_attn_scored_bwd, each part padded to 256 bytes: D and a logarithm (fp32 [2][b][hq][s]), the fp32 dK/dV
  * partials where the dK/dV pass is split, and for spans the int32 work orders of the two
  * passes and the int32 range of queries that see each key (2 x [b][s]). */
 size_t mtp_attn_scored_bwd_workspace_bytes(int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh);

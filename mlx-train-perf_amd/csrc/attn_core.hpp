@@ -595,7 +595,9 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
             if constexpr (!HALF) {
               pf[h][r >> 3][r & 7] = (__bf16)fast_exp2(__builtin_fmaf(a1[h][r], scale_log2, -l4[u] * kLog2e));
             } else {
-              float y = __builtin_fmaf(a1[h][r], score.mul, __builtin_fmaf(-kLog2e, l4[u], add));
+              // Without slopes what is added to a query's scores is one number, which the dQ pass left in the place of L
+              // (8192 positions, 32/8 heads, head_dim 128, cap 50: 1177 against 1190 us).
+              float y = __builtin_fmaf(a1[h][r], score.mul, (MOD & kModSlope) ? __builtin_fmaf(-kLog2e, l4[u], add) : l4[u]);
               if constexpr (kMixed) y = __builtin_fmaf(-score.slope2, __builtin_fabsf(rel - (float)(32 * h + 8 * rq + u)), y);
               const float p = fast_exp2(y);
               pown[h][r >> 3][r & 7] = (__bf16)p;
@@ -1015,7 +1017,10 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
       }
     }
     dq_row = sum_xhalf(dp);
-    if (qvalid && hf == 0) dvec[qrow + qi] = dq_row;
+    if (qvalid && hf == 0) {
+      dvec[qrow + qi] = dq_row;
+      if constexpr (SCORED && !(MOD & kModSlope)) dvec[(long)B * Hq * S + qrow + qi] = score.add + 15.f - l2q;  // (kUp there)
+    }
   }
 
   // dQ pass, tile t from stage cur; the copies of tile t+1 go to stage nxt (free since the barrier

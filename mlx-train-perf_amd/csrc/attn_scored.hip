@@ -80,7 +80,7 @@ size_t carve(int b, int hq, int hkv, int s, int dh, char* base, ScoredWorkspace*
     at += round256(bytes);
     return p;
   };
-  ws->dvec = reinterpret_cast<float*>(take((size_t)b * hq * s * sizeof(float)));
+  ws->dvec = reinterpret_cast<float*>(take((size_t)2 * b * hq * s * sizeof(float)));
   ws->part = reinterpret_cast<float*>(take(ns > 1 ? (size_t)ns * 2 * b * hkv * s * dh * sizeof(float) : 0));
   ws->q_order = reinterpret_cast<int32_t*>(take((size_t)b * ((s + P - 1) / P) * 4));
   ws->kv_order = reinterpret_cast<int32_t*>(take((size_t)b * ((s + 127) / 128) * 4));

@@ -5,7 +5,7 @@
 
 namespace mtp {
 
-// A backward call's workspace, in order: D, the fp32 partials of a split dK/dV pass, and for spans the two work
+// A backward call's workspace, in order: D, without slopes the logarithms in the P waves' form, the fp32 partials of a split dK/dV pass, and for spans the two work
 // orders (null: none) and the queries [col_begin, col_end) that see each key.
 struct ScoredWorkspace {
   float* dvec;
@@ -81,7 +81,7 @@ hipError_t scored_bwd<MTP_SCORED_DH>(const AttnShape& sh, const AttnScore& sc, c
       hipError_t e = hipGetLastError();
       if (e != hipSuccess) return e;
       hipLaunchKernelGGL(dkv_kernel, dim3((sh.s + 127) / 128 * sh.b * sh.hkv * ws.nsplit), dim3(512), 0, st, q, k, v, d_o,
-                         lse, ws.dvec, ws.col_end, dk, dv, sh.b, sh.hq, sh.hkv, sh.s, sh.scale * kLog2e, sh.scale,
+                         (MOD & kModSlope) ? lse : ws.dvec + (long)sh.b * sh.hq * sh.s, ws.dvec, ws.col_end, dk, dv, sh.b, sh.hq, sh.hkv, sh.s, sh.scale * kLog2e, sh.scale,
                          sh.causal, ws.nsplit, ws.part, ws.kv_order, ws.col_begin, sc.cap, sc.slopes);
       return hipGetLastError();
     };
