@@ -295,11 +295,14 @@ int mtp_attn_bwd_f32(const float* q, const float* k, const float* v, const float
  * given (else: mtp_attn_fwd). What the mask hides must be finite all the same, padding too: v, and in the backward q, k and d_o.
  * o_low: int8 [b][hq][s][dh], the 8 bits of the output below its bf16 ones (bits of x = bits of bf16(x) + 2^8 o_low), for
  * the backward's D = rowsum(d_o o); NULL in a forward without a backward.
+ * plan: mtp_attn_scored_plan_bytes, with spans what a forward works out for itself and its backward (the work orders, the
+ * queries that see each key); NULL in either: the forward goes without, the backward works it out. 0 bytes: NULL in both.
  * ------------------------------------------------------------------------------------------- */
+size_t mtp_attn_scored_plan_bytes(int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh);
 int mtp_attn_scored_fwd(const void* q, const void* k, const void* v, int64_t b, int64_t hq, int64_t hkv,
                         int64_t s, int64_t dh, float scale, int32_t causal, float softcap,
                         const float* slopes, const int32_t* span_start, const int32_t* span_end, void* o,
-                        int8_t* o_low, float* lse, void* stream);
+                        int8_t* o_low, int32_t* plan, float* lse, void* stream);
 
 /* Workspace bytes of mtp_attn_scored_bwd, each part padded to 256 bytes: D and a logarithm (fp32 [2][b][hq][s]), the fp32 dK/dV
  * partials where the dK/dV pass is split, and for spans the int32 work orders of the two
@@ -307,7 +310,7 @@ int mtp_attn_scored_fwd(const void* q, const void* k, const void* v, int64_t b, 
 size_t mtp_attn_scored_bwd_workspace_bytes(int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh);
 
 int mtp_attn_scored_bwd(const void* q, const void* k, const void* v, const void* o, const int8_t* o_low,
-                        const float* lse, const void* d_o, int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh,
+                        const int32_t* plan, const float* lse, const void* d_o, int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh,
                         float scale, int32_t causal, float softcap, const float* slopes,
                         const int32_t* span_start, const int32_t* span_end, void* d_q, void* d_k, void* d_v,
                         void* workspace, size_t workspace_bytes, void* stream);

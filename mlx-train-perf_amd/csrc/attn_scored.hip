@@ -70,23 +70,43 @@ int scored_nsplit(int b, int hq, int hkv, int s, int dh, int causal) {
   while (ns > 1 && items < ns * (wgs * ns <= kNumCU + kNumCU / 4 ? 2 : 16)) ns /= 2;
   return ns;
 }
-// The parts of a workspace from `base` (null: sizes alone), with room for the larger split of the two masks; returns the bytes.
+// Whether the workgroups of a span backward's passes take turns, so that their order counts.
+bool ordered(int b, int hq, int hkv, int s, int dh) {
+  const AttnShape sh{b, hq, hkv, s, dh, 0.f, 0};
+  return q_grid(sh) > 2 * kNumCU || (long)(s + 127) / 128 * b * hkv * scored_nsplit(b, hq, hkv, s, dh, 1) > kNumCU;
+}
+struct Carver {
+  char* base;  // null: sizes alone
+  size_t at = 0;
+  template <class T>
+  void take(T*& p, size_t n) {
+    p = reinterpret_cast<T*>(base + at);
+    at += round256(n * sizeof(T));
+  }
+};
+// What spans add to a backward: its work orders and the queries that see each key.
+void carve_plan(Carver& c, int b, int hq, int hkv, int s, ScoredWorkspace* ws) {
+  const int P = wg_rows(hq, hkv);
+  c.take(ws->q_order, (size_t)b * ((s + P - 1) / P));
+  c.take(ws->kv_order, (size_t)b * ((s + 127) / 128));
+  c.take(ws->col_begin, (size_t)b * s);
+  c.take(ws->col_end, (size_t)b * s);
+}
+// The parts of a workspace from `base`, with room for the larger split of the two masks; returns the bytes.
 size_t carve(int b, int hq, int hkv, int s, int dh, char* base, ScoredWorkspace* ws) {
   const int ns1 = scored_nsplit(b, hq, hkv, s, dh, 1), ns0 = scored_nsplit(b, hq, hkv, s, dh, 0);
-  const int ns = ns1 > ns0 ? ns1 : ns0, P = wg_rows(hq, hkv);
-  size_t at = 0;
-  auto take = [&](size_t bytes) {
-    char* p = base + at;
-    at += round256(bytes);
-    return p;
-  };
-  ws->dvec = reinterpret_cast<float*>(take((size_t)2 * b * hq * s * sizeof(float)));
-  ws->part = reinterpret_cast<float*>(take(ns > 1 ? (size_t)ns * 2 * b * hkv * s * dh * sizeof(float) : 0));
-  ws->q_order = reinterpret_cast<int32_t*>(take((size_t)b * ((s + P - 1) / P) * 4));
-  ws->kv_order = reinterpret_cast<int32_t*>(take((size_t)b * ((s + 127) / 128) * 4));
-  ws->col_begin = reinterpret_cast<int32_t*>(take((size_t)b * s * 4));
-  ws->col_end = reinterpret_cast<int32_t*>(take((size_t)b * s * 4));
-  return at;
+  const int ns = ns1 > ns0 ? ns1 : ns0;
+  Carver c{base};
+  c.take(ws->dvec, (size_t)2 * b * hq * s);
+  c.take(ws->part, ns > 1 ? (size_t)ns * 2 * b * hkv * s * dh : 0);
+  carve_plan(c, b, hq, hkv, s, ws);
+  return c.at;
+}
+hipError_t launch_sched(const AttnShape& sh, const AttnScore& sc, const ScoredWorkspace& ws, hipStream_t st) {
+  const unsigned fill = (unsigned)(((long)sh.b * sh.s + 1023) / 1024);
+  hipLaunchKernelGGL(attn_span_sched_kernel, dim3(2 + fill), dim3(1024), 0, st, sc.start, sc.end, sh.b, sh.s,
+                     wg_rows(sh.hq, sh.hkv), ws.q_order, ws.kv_order, ws.col_begin, ws.col_end);
+  return hipGetLastError();
 }
 }  // namespace
 
@@ -95,19 +115,38 @@ size_t attn_scored_bwd_workspace(int b, int hq, int hkv, int s, int dh) {
   return carve(b, hq, hkv, s, dh, nullptr, &ws);
 }
 
+size_t attn_scored_plan(int b, int hq, int hkv, int s, int dh) {
+  if (!ordered(b, hq, hkv, s, dh)) return 0;
+  ScoredWorkspace ws;
+  Carver c{nullptr};
+  carve_plan(c, b, hq, hkv, s, &ws);
+  return c.at;
+}
+
 hipError_t launch_attn_scored_fwd(const AttnShape& sh, const AttnScore& sc, const bf16_t* q, const bf16_t* k,
-                                  const bf16_t* v, bf16_t* o, int8_t* o_low, float* lse, hipStream_t st) {
+                                  const bf16_t* v, bf16_t* o, int8_t* o_low, int32_t* plan, float* lse, hipStream_t st) {
+  // The forward of a training step makes the backward's plan, and goes by its order of query blocks too (documents of 64
+  // to 2048 in 8192 positions, 16/4 heads, head_dim 128: 62 against 76 us).
+  const int32_t* order = nullptr;
+  if (plan && sc.start && ordered(sh.b, sh.hq, sh.hkv, sh.s, sh.dh)) {
+    ScoredWorkspace ws;
+    Carver c{reinterpret_cast<char*>(plan)};
+    carve_plan(c, sh.b, sh.hq, sh.hkv, sh.s, &ws);
+    const hipError_t e = launch_sched(sh, sc, ws, st);
+    if (e != hipSuccess) return e;
+    order = ws.q_order;
+  }
   switch (sh.dh) {
-    case 64: return scored_fwd<64>(sh, sc, q, k, v, o, o_low, lse, q_grid(sh), st);
-    case 96: return scored_fwd<96>(sh, sc, q, k, v, o, o_low, lse, q_grid(sh), st);
-    case 128: return scored_fwd<128>(sh, sc, q, k, v, o, o_low, lse, q_grid(sh), st);
+    case 64: return scored_fwd<64>(sh, sc, q, k, v, o, o_low, order, lse, q_grid(sh), st);
+    case 96: return scored_fwd<96>(sh, sc, q, k, v, o, o_low, order, lse, q_grid(sh), st);
+    case 128: return scored_fwd<128>(sh, sc, q, k, v, o, o_low, order, lse, q_grid(sh), st);
     default: return hipErrorInvalidValue;
   }
 }
 
 hipError_t launch_attn_scored_bwd(const AttnShape& sh, const AttnScore& sc, const bf16_t* q, const bf16_t* k,
-                                  const bf16_t* v, const bf16_t* o, const int8_t* o_low, const float* lse,
-                                  const bf16_t* d_o, bf16_t* dq, bf16_t* dk, bf16_t* dv, void* workspace,
+                                  const bf16_t* v, const bf16_t* o, const int8_t* o_low, const int32_t* plan,
+                                  const float* lse, const bf16_t* d_o, bf16_t* dq, bf16_t* dk, bf16_t* dv, void* workspace,
                                   hipStream_t st) {
   ScoredWorkspace ws;
   carve(sh.b, sh.hq, sh.hkv, sh.s, sh.dh, static_cast<char*>(workspace), &ws);
@@ -116,13 +155,13 @@ hipError_t launch_attn_scored_bwd(const AttnShape& sh, const AttnScore& sc, cons
   // Where all workgroups of both passes run at once their order is of no account, and the dQ pass fills the key ranges
   // that the dK/dV pass reads: a launch less (a step of 4 x 16/8 x 509 x 64: 63.2 against
   // 67.5 us of GPU time, 1 x 8/8 x 100 x 128 37.0 against 41.2).
-  const bool ordered = q_grid(sh) > 2 * kNumCU || (long)(sh.s + 127) / 128 * sh.b * sh.hkv * ws.nsplit > kNumCU;
-  if (sc.start && !ordered) ws.q_order = ws.kv_order = nullptr;
-  if (sc.start && ordered) {
-    const unsigned fill = (unsigned)(((long)sh.b * sh.s + 1023) / 1024);
-    hipLaunchKernelGGL(attn_span_sched_kernel, dim3(2 + fill), dim3(1024), 0, st, sc.start, sc.end, sh.b, sh.s,
-                       wg_rows(sh.hq, sh.hkv), ws.q_order, ws.kv_order, ws.col_begin, ws.col_end);
-    e = hipGetLastError();
+  if (sc.start && !ordered(sh.b, sh.hq, sh.hkv, sh.s, sh.dh)) {
+    ws.q_order = ws.kv_order = nullptr;
+  } else if (sc.start && plan) {
+    Carver c{reinterpret_cast<char*>(const_cast<int32_t*>(plan))};
+    carve_plan(c, sh.b, sh.hq, sh.hkv, sh.s, &ws);
+  } else if (sc.start) {
+    e = launch_sched(sh, sc, ws, st);
     if (e != hipSuccess) return e;
   }
   switch (sh.dh) {

@@ -16,7 +16,7 @@ struct ScoredWorkspace {
 
 template <int DH>
 hipError_t scored_fwd(const AttnShape& sh, const AttnScore& sc, const bf16_t* q, const bf16_t* k, const bf16_t* v,
-                      bf16_t* o, int8_t* o_low, float* lse, int grid, hipStream_t st);
+                      bf16_t* o, int8_t* o_low, const int32_t* order, float* lse, int grid, hipStream_t st);
 template <int DH>
 hipError_t scored_bwd(const AttnShape& sh, const AttnScore& sc, const ScoredWorkspace& ws, const bf16_t* q,
                       const bf16_t* k, const bf16_t* v, const bf16_t* o, const int8_t* o_low, const float* lse,
@@ -38,14 +38,14 @@ hipError_t with_mod(const AttnScore& sc, F&& f) {
 #ifdef MTP_SCORED_DH
 template <>
 hipError_t scored_fwd<MTP_SCORED_DH>(const AttnShape& sh, const AttnScore& sc, const bf16_t* q, const bf16_t* k,
-                                     const bf16_t* v, bf16_t* o, int8_t* o_low, float* lse, int grid,
-                                     hipStream_t st) {
+                                     const bf16_t* v, bf16_t* o, int8_t* o_low, const int32_t* order,
+                                     float* lse, int grid, hipStream_t st) {
   constexpr int DH = MTP_SCORED_DH;
   return with_mod(sc, [&](auto m) {
     constexpr int MOD = decltype(m)::value;
     auto launch = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, st, q, k, v, nullptr, nullptr, nullptr, nullptr, sc.end,
-                         sc.start, o, lse, sh.b, sh.hq, sh.hkv, sh.s, sh.scale * kLog2e, sh.scale, sh.causal, nullptr,
+                         sc.start, o, lse, sh.b, sh.hq, sh.hkv, sh.s, sh.scale * kLog2e, sh.scale, sh.causal, order,
                          sc.cap, sc.slopes, o_low, nullptr, nullptr);
       return hipGetLastError();
     };

@@ -617,16 +617,16 @@ int mtp_attn_bwd_f32(const float* q, const float* k, const float* v, const float
 
 int mtp_attn_scored_fwd(const void* q, const void* k, const void* v, int64_t b, int64_t hq, int64_t hkv, int64_t s,
                         int64_t dh, float scale, int32_t causal, float softcap, const float* slopes,
-                        const int32_t* span_start, const int32_t* span_end, void* o, int8_t* o_low, float* lse,
-                        void* stream) {
+                        const int32_t* span_start, const int32_t* span_end, void* o, int8_t* o_low, int32_t* plan,
+                        float* lse, void* stream) {
   int rc = check_scored(q, k, v, b, hq, hkv, s, dh, scale, causal, softcap, slopes, span_start, span_end);
   if (rc) return rc;
   if (!o || !lse) return fail(MTP_ERR_INPUT, "o and lse must be non-null");
-  if (!aligned16(o) || !aligned16(o_low)) return fail(MTP_ERR_UNSUPPORTED, "o and o_low must be 16-byte aligned");
+  if (!aligned16(o) || !aligned16(o_low) || !aligned16(plan)) return fail(MTP_ERR_UNSUPPORTED, "o, o_low and plan must be 16-byte aligned");
   mtp::AttnShape sh{(int)b, (int)hq, (int)hkv, (int)s, (int)dh, scale, (int)causal};
   mtp::AttnScore sc{softcap, slopes, span_start, span_end};
   hipError_t e = mtp::launch_attn_scored_fwd(sh, sc, static_cast<const mtp::bf16_t*>(q), static_cast<const mtp::bf16_t*>(k),
-                                             static_cast<const mtp::bf16_t*>(v), static_cast<mtp::bf16_t*>(o), o_low, lse,
+                                             static_cast<const mtp::bf16_t*>(v), static_cast<mtp::bf16_t*>(o), o_low, plan, lse,
                                              static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return fail(MTP_ERR_RUNTIME, "scored attention forward launch failed: %s", hipGetErrorString(e));
   return ok();
@@ -658,20 +658,25 @@ size_t mtp_attn_scored_bwd_f32_workspace_bytes(int64_t b, int64_t hq, int64_t hk
   return mtp::attn32_scored_bwd_workspace((int)b, (int)hq, (int)hkv, (int)s, (int)dh);
 }
 
+size_t mtp_attn_scored_plan_bytes(int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh) {
+  if (b < 1 || hq < 1 || hkv < 1 || s < 1 || hq % hkv || b * hq * s > kMaxDim) return 0;
+  return mtp::attn_scored_plan((int)b, (int)hq, (int)hkv, (int)s, (int)dh);
+}
+
 size_t mtp_attn_scored_bwd_workspace_bytes(int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh) {
   if (b < 1 || hq < 1 || hkv < 1 || s < 1 || hq % hkv || b * hq * s > kMaxDim) return 0;
   return mtp::attn_scored_bwd_workspace((int)b, (int)hq, (int)hkv, (int)s, (int)dh);
 }
 
 int mtp_attn_scored_bwd(const void* q, const void* k, const void* v, const void* o, const int8_t* o_low,
-                        const float* lse, const void* d_o, int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh, float scale, int32_t causal,
+                        const int32_t* plan, const float* lse, const void* d_o, int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh, float scale, int32_t causal,
                         float softcap, const float* slopes, const int32_t* span_start, const int32_t* span_end, void* d_q,
                         void* d_k, void* d_v, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_scored(q, k, v, b, hq, hkv, s, dh, scale, causal, softcap, slopes, span_start, span_end);
   if (rc) return rc;
   if (!o || !o_low || !lse || !d_o || !d_q || !d_k || !d_v) return fail(MTP_ERR_INPUT, "o, o_low, lse, d_o, d_q, d_k, d_v must be non-null");
-  if (!aligned16(o) || !aligned16(o_low) || !aligned16(d_o) || !aligned16(d_q) || !aligned16(d_k) || !aligned16(d_v))
-    return fail(MTP_ERR_UNSUPPORTED, "o, o_low, d_o, d_q, d_k, d_v must be 16-byte aligned");
+  if (!aligned16(o) || !aligned16(o_low) || !aligned16(plan) || !aligned16(d_o) || !aligned16(d_q) || !aligned16(d_k) || !aligned16(d_v))
+    return fail(MTP_ERR_UNSUPPORTED, "o, o_low, plan, d_o, d_q, d_k, d_v must be 16-byte aligned");
   const size_t need = mtp_attn_scored_bwd_workspace_bytes(b, hq, hkv, s, dh);
   if (!workspace || workspace_bytes < need)
     return fail(MTP_ERR_WORKSPACE, "scored attention backward needs a workspace of %zu bytes (got %zu)", need, workspace ? workspace_bytes : (size_t)0);
@@ -679,7 +684,7 @@ int mtp_attn_scored_bwd(const void* q, const void* k, const void* v, const void*
   mtp::AttnShape sh{(int)b, (int)hq, (int)hkv, (int)s, (int)dh, scale, (int)causal};
   mtp::AttnScore sc{softcap, slopes, span_start, span_end};
   hipError_t e = mtp::launch_attn_scored_bwd(sh, sc, static_cast<const mtp::bf16_t*>(q), static_cast<const mtp::bf16_t*>(k),
-                                             static_cast<const mtp::bf16_t*>(v), static_cast<const mtp::bf16_t*>(o), o_low, lse,
+                                             static_cast<const mtp::bf16_t*>(v), static_cast<const mtp::bf16_t*>(o), o_low, plan, lse,
                                              static_cast<const mtp::bf16_t*>(d_o), static_cast<mtp::bf16_t*>(d_q),
                                              static_cast<mtp::bf16_t*>(d_k), static_cast<mtp::bf16_t*>(d_v), workspace,
                                              static_cast<hipStream_t>(stream));

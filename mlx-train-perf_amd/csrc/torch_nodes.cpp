@@ -46,6 +46,7 @@ struct Entries {
   decltype(&mtp_lce_mean_bwd) lce_mean_bwd = nullptr;
   decltype(&mtp_attn_scored_fwd) scored_fwd = nullptr;
   decltype(&mtp_attn_scored_bwd) scored_bwd = nullptr;
+  decltype(&mtp_attn_scored_plan_bytes) scored_plan = nullptr;
   decltype(&mtp_attn_scored_bwd_workspace_bytes) scored_ws = nullptr;
   decltype(&mtp_attn_scored_fwd_f32_workspace_bytes) scored_fwd_ws32 = nullptr, scored_bwd_ws32 = nullptr;
   decltype(&mtp_attn_scored_fwd_f32) scored_fwd32 = nullptr;
@@ -188,7 +189,7 @@ struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
     const int64_t b = q.size(0), hq = q.size(1), s = q.size(2), dh = q.size(3), hkv = k.size(1);
     const at::Tensor o = at::empty_like(q), lse = at::empty({b, hq, s}, q.options().dtype(at::kFloat));
     const float cap = (float)score.softcap;
-    at::Tensor low;  // the bits of O below its bf16 ones, for the backward
+    at::Tensor low, plan;  // the bits of O below its bf16 ones, and the spans' plan, for the backward
     if (q.scalar_type() == at::kFloat) {
       const size_t bytes = g_api.scored_fwd_ws32(b, hq, hkv, s, dh);
       const at::Tensor ws = bytes ? at::empty({(int64_t)bytes}, q.options().dtype(at::kByte)) : at::Tensor();
@@ -196,11 +197,16 @@ struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
                                floats(score.slopes), ints(score.start), ints(score.end), ptr<float>(o), ptr<float>(lse),
                                opt_ptr(ws), bytes, stream_of(q)));
     } else {
-      if (score.train) low = at::empty_like(q, q.options().dtype(at::kChar));
+      if (score.train) {
+        low = at::empty_like(q, q.options().dtype(at::kChar));
+        const size_t bytes = score.start.defined() ? g_api.scored_plan(b, hq, hkv, s, dh) : 0;
+        if (bytes) plan = at::empty({(int64_t)bytes / 4}, q.options().dtype(at::kInt));
+      }
       check(g_api.scored_fwd(ptr(q), ptr(k), ptr(v), b, hq, hkv, s, dh, (float)scale, causal, cap, floats(score.slopes),
-                             ints(score.start), ints(score.end), ptr(o), opt_ptr<int8_t>(low), ptr<float>(lse), stream_of(q)));
+                             ints(score.start), ints(score.end), ptr(o), opt_ptr<int8_t>(low), opt_ptr<int32_t>(plan), ptr<float>(lse),
+                             stream_of(q)));
     }
-    ctx->save_for_backward({q, k, v, o, low, lse, score.slopes, score.start, score.end});
+    ctx->save_for_backward({q, k, v, o, low, plan, lse, score.slopes, score.start, score.end});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["softcap"] = score.softcap;
@@ -212,8 +218,8 @@ struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
                                                  torch::autograd::variable_list grads) {
     count_backward(g_attn_calls, {"flash_attention", "flash_attention_kernel_bwd"});
     const auto saved = ctx->get_saved_variables();
-    const at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &o = saved[3], &low = saved[4], &lse = saved[5];
-    const at::Tensor &slopes = saved[6], &start = saved[7], &end = saved[8];
+    const at::Tensor &q = saved[0], &k = saved[1], &v = saved[2], &o = saved[3], &low = saved[4];
+    const at::Tensor &plan = saved[5], &lse = saved[6], &slopes = saved[7], &start = saved[8], &end = saved[9];
     const float scale = (float)ctx->saved_data["scale"].toDouble(), cap = (float)ctx->saved_data["softcap"].toDouble();
     const bool causal = ctx->saved_data["causal"].toBool();
     const c10::DeviceGuard device(q.device());
@@ -228,7 +234,7 @@ struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
                                hq, hkv, s, dh, scale, causal, cap, floats(slopes), ints(start), ints(end), ptr<float>(dq),
                                ptr<float>(dk), ptr<float>(dv), ptr(ws), bytes, stream_of(q)));
     else
-      check(g_api.scored_bwd(ptr(q), ptr(k), ptr(v), ptr(o), ptr<int8_t>(low), ptr<float>(lse), ptr(d_o), b, hq, hkv, s, dh, scale, causal, cap,
+      check(g_api.scored_bwd(ptr(q), ptr(k), ptr(v), ptr(o), ptr<int8_t>(low), ints(plan), ptr<float>(lse), ptr(d_o), b, hq, hkv, s, dh, scale, causal, cap,
                              floats(slopes), ints(start), ints(end), ptr(dq), ptr(dk), ptr(dv), ptr(ws), bytes, stream_of(q)));
     return once(grads, {dq, dk, dv, at::Tensor(), at::Tensor(), at::Tensor()});
   }
@@ -573,6 +579,7 @@ void bind(const py::dict& entries, py::object check_fn) {
   set(g_api.lce_mean_bwd, "mtp_lce_mean_bwd");
   set(g_api.scored_fwd, "mtp_attn_scored_fwd");
   set(g_api.scored_bwd, "mtp_attn_scored_bwd");
+  set(g_api.scored_plan, "mtp_attn_scored_plan_bytes");
   set(g_api.scored_ws, "mtp_attn_scored_bwd_workspace_bytes");
   set(g_api.scored_fwd_ws32, "mtp_attn_scored_fwd_f32_workspace_bytes");
   set(g_api.scored_bwd_ws32, "mtp_attn_scored_bwd_f32_workspace_bytes");

@@ -279,8 +279,9 @@ class _KernelAttention(torch.autograd.Function):
 
 
 def scored_forward(q, k, v, slopes, start, end, *, scale: float, causal: bool, softcap: float, train: bool = True):
-    """(O, L, low) from mtp_attn_scored_fwd (_f32 for fp32 inputs); contiguous tensors on the GPU. low: the bits of a bf16
-    O's values that the backward needs beside it (None for fp32, and without `train`)."""
+    """(O, L, low, plan) from mtp_attn_scored_fwd (_f32 for fp32 inputs); contiguous tensors on the GPU. low and plan are for
+    the backward of bf16 inputs (None for fp32, and without `train`): the bits of O's values below its own, and what
+    spans have to be known of (None where that is of no use)."""
     lib = _native.load()
     b, hq, n, dh = q.shape
     o = torch.empty_like(q)
@@ -288,7 +289,7 @@ def scored_forward(q, k, v, slopes, start, end, *, scale: float, causal: bool, s
     shape = (b, hq, k.shape[1], n, dh)
     args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), *shape, scale, int(causal), softcap, _native.ptr(slopes), _native.ptr(start),
             _native.ptr(end), o.data_ptr())
-    low = None
+    low = plan = None
     with _native.on_device(q):
         if q.dtype == torch.float32:
             ws_bytes = lib.mtp_attn_scored_fwd_f32_workspace_bytes(*shape)
@@ -296,12 +297,14 @@ def scored_forward(q, k, v, slopes, start, end, *, scale: float, causal: bool, s
             rc = lib.mtp_attn_scored_fwd_f32(*args, lse.data_ptr(), _native.ptr(ws), ws_bytes, _native.stream_of(q))
         else:
             low = torch.empty_like(q, dtype=torch.int8) if train else None
-            rc = lib.mtp_attn_scored_fwd(*args, _native.ptr(low), lse.data_ptr(), _native.stream_of(q))
+            plan_bytes = lib.mtp_attn_scored_plan_bytes(*shape) if train and start is not None else 0
+            plan = torch.empty(plan_bytes // 4, dtype=torch.int32, device=q.device) if plan_bytes else None
+            rc = lib.mtp_attn_scored_fwd(*args, _native.ptr(low), _native.ptr(plan), lse.data_ptr(), _native.stream_of(q))
     _native.check(rc, domain="attention")
-    return o, lse, low
+    return o, lse, low, plan
 
 
-def scored_backward(q, k, v, o, low, lse, d_o, slopes, start, end, *, scale: float, causal: bool, softcap: float):
+def scored_backward(q, k, v, o, low, plan, lse, d_o, slopes, start, end, *, scale: float, causal: bool, softcap: float):
     """(dQ, dK, dV) from mtp_attn_scored_bwd (_f32 for fp32 inputs)."""
     lib = _native.load()
     b, hq, n, dh = q.shape
@@ -311,7 +314,7 @@ def scored_backward(q, k, v, o, low, lse, d_o, slopes, start, end, *, scale: flo
     ws_bytes = (lib.mtp_attn_scored_bwd_f32_workspace_bytes if f32 else lib.mtp_attn_scored_bwd_workspace_bytes)(b, hq, hkv, n, dh)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
     bwd = lib.mtp_attn_scored_bwd_f32 if f32 else lib.mtp_attn_scored_bwd
-    out = (o.data_ptr(),) if f32 else (o.data_ptr(), low.data_ptr())
+    out = (o.data_ptr(),) if f32 else (o.data_ptr(), low.data_ptr(), _native.ptr(plan))
     with _native.on_device(q):
         rc = bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), *out, lse.data_ptr(), d_o.data_ptr(), b, hq, hkv, n, dh,
                  scale, int(causal), softcap, _native.ptr(slopes), _native.ptr(start), _native.ptr(end),
@@ -325,9 +328,9 @@ class _ScoredAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, slopes, start, end, scale, causal, softcap):
-        o, lse, low = scored_forward(q, k, v, slopes, start, end, scale=scale, causal=causal, softcap=softcap,
-                                     train=any(ctx.needs_input_grad))
-        ctx.save_for_backward(q, k, v, o, low, lse, slopes, start, end)
+        o, lse, low, plan = scored_forward(q, k, v, slopes, start, end, scale=scale, causal=causal, softcap=softcap,
+                                           train=any(ctx.needs_input_grad))
+        ctx.save_for_backward(q, k, v, o, low, plan, lse, slopes, start, end)
         ctx.scale, ctx.causal, ctx.softcap = scale, causal, softcap
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
@@ -338,9 +341,9 @@ class _ScoredAttention(torch.autograd.Function):
     def backward(ctx, d_o, _d_l):
         VJP_CALLS["flash_attention"] = VJP_CALLS.get("flash_attention", 0) + 1
         VJP_CALLS["flash_attention_kernel_bwd"] = VJP_CALLS.get("flash_attention_kernel_bwd", 0) + 1
-        q, k, v, o, low, lse, slopes, start, end = ctx.saved_tensors
+        q, k, v, o, low, plan, lse, slopes, start, end = ctx.saved_tensors
         d_o = torch.zeros_like(o) if d_o is None else d_o.contiguous()
-        dq, dk, dv = scored_backward(q, k, v, o, low, lse, d_o, slopes, start, end, scale=ctx.scale, causal=ctx.causal,
+        dq, dk, dv = scored_backward(q, k, v, o, low, plan, lse, d_o, slopes, start, end, scale=ctx.scale, causal=ctx.causal,
                                      softcap=ctx.softcap)
         return dq, dk, dv, None, None, None, None, None, None
 

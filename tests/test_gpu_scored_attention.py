@@ -285,9 +285,9 @@ def test_fp32_without_room_for_parts():
     q, k, v, d_o = (x.cuda() for x in S.inputs(b, hq, hkv, s, dh, torch.float32, 3))
     slopes = S.slopes_of(hq).cuda()
     args = {"scale": 0.125, "causal": True, "softcap": 9.0}
-    o, lse, low = scored_forward(q, k, v, slopes, None, None, **args)
-    assert low is None   # bf16's alone
-    grads = scored_backward(q, k, v, o, low, lse, d_o, slopes, None, None, **args)
+    o, lse, low, plan = scored_forward(q, k, v, slopes, None, None, **args)
+    assert low is None and plan is None   # bf16's alone
+    grads = scored_backward(q, k, v, o, low, plan, lse, d_o, slopes, None, None, **args)
     o1, lse1 = torch.empty_like(o), torch.empty_like(lse)
     outs = [torch.empty_like(x) for x in (q, k, v)]
     ws = torch.empty(b * hq * s, device="cuda")
@@ -393,3 +393,20 @@ def test_splits_of_the_key_blocks(b, hq, hkv, s, dh, mask, cap, biased):
     """dK/dV of a key block by one workgroup, and by two, four and eight; more workgroups than run at once, in work orders
     under spans."""
     _check(b, hq, hkv, s, dh, mask=mask, cap=cap, biased=biased, dtype=torch.bfloat16, seed=s)
+
+
+def test_with_and_without_a_plan():
+    """Spans of many workgroups: the forward's plan (its order of work, and the backward's) changes no bit."""
+    from mlx_train_perf.attention.api import scored_backward, scored_forward
+
+    b, hq, hkv, s, dh = 4, 32, 8, 900, 64
+    q, k, v, d_o = (x.cuda() for x in S.inputs(b, hq, hkv, s, dh, torch.bfloat16, 3))
+    start, end = (t.cuda() for t in S.spans_of("docs", b, s, 3))
+    args = {"scale": 0.125, "causal": False, "softcap": 0.0}
+    o, lse, low, plan = scored_forward(q, k, v, None, start, end, **args)
+    assert plan is not None
+    bare = scored_forward(q, k, v, None, start, end, train=False, **args)
+    assert bare[2] is None and bare[3] is None and torch.equal(o, bare[0]) and torch.equal(lse, bare[1])
+    a = scored_backward(q, k, v, o, low, plan, lse, d_o, None, start, end, **args)
+    c = scored_backward(q, k, v, o, low, None, lse, d_o, None, start, end, **args)
+    assert all(torch.equal(x, y) for x, y in zip(a, c))

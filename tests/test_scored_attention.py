@@ -141,7 +141,7 @@ def test_c_abi_refusals():
 
     def fwd(scale=1.0, causal=0, cap=1.0, slopes=none, start=none, end=none, q=p, o=p, shape=shape, lib_fn=lib.mtp_attn_scored_fwd):
         f32 = lib_fn is lib.mtp_attn_scored_fwd_f32
-        return lib_fn(q, p, p, *shape, scale, causal, cap, slopes, start, end, o, *(() if f32 else (none,)), p,
+        return lib_fn(q, p, p, *shape, scale, causal, cap, slopes, start, end, o, *(() if f32 else (none, none)), p,
                       *((none, 0) if f32 else ()), none)
 
     bad, un = _native.MTP_ERR_INPUT, _native.MTP_ERR_UNSUPPORTED
@@ -159,13 +159,14 @@ def test_c_abi_refusals():
     assert ws > 0 and lib.mtp_attn_scored_bwd_workspace_bytes(1, 3, 2, 8, 64) == 0
     assert ws % 256 == 0 and ws >= 2 * 8 * 4 + 2 * 8 * 4
 
-    def bwd(bytes_, workspace=p, d_o=p, low=p, fn=lib.mtp_attn_scored_bwd):
-        out = (p,) if fn is lib.mtp_attn_scored_bwd_f32 else (p, low)
+    def bwd(bytes_, workspace=p, d_o=p, low=p, plan=none, fn=lib.mtp_attn_scored_bwd):
+        out = (p,) if fn is lib.mtp_attn_scored_bwd_f32 else (p, low, plan)
         return fn(p, p, p, *out, p, d_o, *shape, 1.0, 0, 1.0, none, none, none, p, p, p, workspace, bytes_, none)
 
     assert bwd(ws - 1) == _native.MTP_ERR_WORKSPACE and bwd(ws, workspace=none) == _native.MTP_ERR_WORKSPACE
     assert bwd(ws, workspace=p + 4) == un and bwd(ws, d_o=none) == bad
-    assert bwd(ws, low=none) == bad and bwd(ws, low=p + 8) == un
+    assert bwd(ws, low=none) == bad and bwd(ws, low=p + 8) == un and bwd(ws, plan=p + 8) == un
+    assert lib.mtp_attn_scored_plan_bytes(*shape) == 0 and lib.mtp_attn_scored_plan_bytes(1, 16, 4, 8192, 128) >= 2 * 8192 * 4
     assert bwd(8, fn=lib.mtp_attn_scored_bwd_f32) == _native.MTP_ERR_WORKSPACE
     # fp32: parts of 4 splits of one pair of 64-query blocks of 8 heads (64 workgroups), 33 tiles of 32 keys
     assert lib.mtp_attn_scored_fwd_f32_workspace_bytes(1, 8, 2, 1000, 128) == 4 * 8 * 1000 * 130 * 4
