@@ -410,3 +410,35 @@ def test_with_and_without_a_plan():
     a = scored_backward(q, k, v, o, low, plan, lse, d_o, None, start, end, **args)
     c = scored_backward(q, k, v, o, low, None, lse, d_o, None, start, end, **args)
     assert all(torch.equal(x, y) for x, y in zip(a, c))
+
+
+def test_captured_step_with_a_plan():
+    """The plan belongs to the captured step: replays with new spans work out theirs, between eager steps."""
+    from mlx_train_perf import _native
+    from mlx_train_perf.attention import SpanMask, flash_attention
+
+    b, hq, hkv, s, dh = 4, 32, 8, 700, 64
+    assert _native.load().mtp_attn_scored_plan_bytes(b, hq, hkv, s, dh) > 0
+    x = [t.cuda() for t in S.inputs(b, hq, hkv, s, dh, torch.bfloat16, 1)]
+    sp = [t.cuda() for t in S.spans_of("docs", b, s, 1)]
+
+    def step(spans):
+        qs = [t.detach().requires_grad_(True) for t in x[:3]]
+        o = flash_attention(*qs, scale=0.125, softcap=30.0, spans=SpanMask(*spans), validate_segments=False)
+        return [o.detach(), *torch.autograd.grad(o, qs, x[3])]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(sp)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step(sp)
+    for turn, mask in enumerate(("docs", "ragged", "window", "nothing", "prefix")):
+        new = [t.cuda() for t in S.spans_of(mask, b, s, turn + 7)]
+        for old, t in zip(sp, new):
+            old.copy_(t)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, w) for a, w in zip(out, step(new))), mask
