@@ -784,8 +784,14 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
 // read transposed fragments of the same tiles. Two LDS stages, one barrier per key tile.
 // ------------------------------------------------------------------------------------------
 
+// Waves a SIMD: at head_dim 64 a forward with spans, a cap or slopes fits three (without the bias' ramp), whose exponentials
+// and products overlap more than two waves': 2 x 32/8 x 4096 causal with a cap 250 us against 262, 4 x 16/16 x 2048 with
+// slopes, not causal, 122 against 135, causal 72 against 75; a round of workgroups or two (2 x 16 x 1024) 25.6 against 25.2.
+// The dQ pass would spill.
+template <int DH, int MASK, bool DQ, int MOD>
+constexpr int kv_waves() { return DH == 64 && !DQ && (MASK == kMaskSpan || MOD != kModNone) ? 3 : 2; }
 template <int DH, int MASK, bool DQ, int MOD = kModNone, bool FIXED = false>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kv_waves<DH, MASK, DQ, MOD>(), kv_waves<DH, MASK, DQ, MOD>())))
 void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, const bf16_t* __restrict__ v,
                     const bf16_t* __restrict__ d_o, const bf16_t* __restrict__ o_in, const float* __restrict__ lse_in,
                     float* __restrict__ dvec, const int32_t* __restrict__ span_end,
@@ -911,8 +917,8 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
   // The side of its queries that a tile's keys lie on (Score::slant).
   auto side_of = [&](int kv0) { return (causal || kv0 + kKT - 1 <= qw0) ? 1 : kv0 >= qw0 + 31 ? -1 : 0; };
 
-  // Slopes alone: the products K Q^T begin from the bias' ramp where it fits the registers.
-  constexpr bool kRamp = MOD == kModSlope && (!DQ || DH <= 96);
+  // Slopes alone: the products K Q^T begin from the bias' ramp where it fits the registers (kv_waves).
+  constexpr bool kRamp = MOD == kModSlope && (DQ ? DH <= 96 : DH != 64);
   f32x16 ramp[2];
   if constexpr (kRamp) score.template set_ramp<1>(ramp);
 
