@@ -19,9 +19,9 @@
 // in the dK/dV kernel), which leaves errors of 2.0e-3 of the norm in O, 2.3e-3 in dV and 2.4e-3 to 3.0e-3 in dQ and dK.
 //
 // Bound by the SIMDs' issue, matrix and vector instructions together: with a cap the matrix pipe is busy for 0.44 to 0.55
-// of the time (8192 positions, 32/8 heads, head_dim 128: forward 640 us, dQ 833, dK/dV 1191; without a cap 515, 690 and
+// of the time (8192 positions, 32/8 heads, head_dim 128: forward 641 us, dQ 835, dK/dV 1174; without a cap 515, 690 and
 // 1010), as a score costs an exponential and a reciprocal more. With slopes alone the products begin from the bias and the
-// times are the plain kernels' (4 x 16 heads x 2048 x 64: 61, 67 and 95 us).
+// times are the plain kernels' (4 x 16 heads x 2048 x 64: 60, 68 and 98 us).
 //
 // Kernel structure (all MFMA 32x32x16 bf16, fp32 accumulate):
 //   attn_kv_kernel<DH, MASK, DQ, MOD> (forward, and the dQ pass, which also forms D): a wave owns 32
