@@ -297,12 +297,16 @@ int mtp_attn_bwd_f32(const float* q, const float* k, const float* v, const float
  * the backward's D = rowsum(d_o o); NULL in a forward without a backward.
  * plan: mtp_attn_scored_plan_bytes, with spans what a forward works out for itself and its backward (the work orders, the
  * queries that see each key); NULL in either: the forward goes without, the backward works it out. 0 bytes: NULL in both.
+ * Where few workgroups would run, the forward and dQ passes are split over the keys and their parts joined in order: the
+ * forward's workspace holds them (0 bytes: not split; NULL or too small: it runs unsplit).
  * ------------------------------------------------------------------------------------------- */
+size_t mtp_attn_scored_fwd_workspace_bytes(int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh);
 size_t mtp_attn_scored_plan_bytes(int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh);
 int mtp_attn_scored_fwd(const void* q, const void* k, const void* v, int64_t b, int64_t hq, int64_t hkv,
                         int64_t s, int64_t dh, float scale, int32_t causal, float softcap,
                         const float* slopes, const int32_t* span_start, const int32_t* span_end, void* o,
-                        int8_t* o_low, int32_t* plan, float* lse, void* stream);
+                        int8_t* o_low, int32_t* plan, float* lse, void* workspace, size_t workspace_bytes,
+                        void* stream);
 
 /* Workspace bytes of mtp_attn_scored_bwd, each part padded to 256 bytes: D and a logarithm (fp32 [2][b][hq][s]), the fp32 dK/dV
  * partials where the dK/dV pass is split, and for spans the int32 work orders of the two
@@ -315,9 +319,8 @@ int mtp_attn_scored_bwd(const void* q, const void* k, const void* v, const void*
                         const int32_t* span_start, const int32_t* span_end, void* d_q, void* d_k, void* d_v,
                         void* workspace, size_t workspace_bytes, void* stream);
 
-/* The same with fp32 tensors. Where few workgroups would run, the passes are split over the keys and their parts
- * joined in order: the workspaces hold them (the forward's may be NULL, the backward's needs D, fp32 [b][hq][s], at
- * least; a pass without room for its parts runs unsplit). */
+/* The same with fp32 tensors. The workspaces hold the parts of split passes (the forward's may be NULL, the backward's
+ * needs D, fp32 [b][hq][s], at least; a pass without room for its parts runs unsplit). */
 size_t mtp_attn_scored_fwd_f32_workspace_bytes(int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh);
 int mtp_attn_scored_fwd_f32(const float* q, const float* k, const float* v, int64_t b, int64_t hq,
                             int64_t hkv, int64_t s, int64_t dh, float scale, int32_t causal, float softcap,

@@ -227,6 +227,12 @@ struct Lanes {
 };
 }  // namespace kvdma
 
+// The 8 bits of x below those of its bf16, `top` its bits, as a byte (attn_kv_kernel's o_low).
+__device__ __forceinline__ uint32_t below_bf16(float x, uint32_t top) {
+  const int rest = (__builtin_bit_cast(int, x) - (int)top + 0x80) >> 8;  // in [-128, 128]
+  return (uint32_t)(rest < 127 ? rest : 127) & 0xff;
+}
+
 // First index i in [lo, hi) with a[i] > x (hi if none); a is non-decreasing.
 __device__ __forceinline__ int first_above(const int32_t* a, int lo, int hi, int x) {
   while (lo < hi) {
@@ -798,10 +804,15 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
                     const int32_t* __restrict__ seg_start, bf16_t* __restrict__ out, float* __restrict__ lse_out,
                     int B, int Hq, int Hkv, int S, float scale_log2, float scale, int causal,
                     const int32_t* __restrict__ order, float cap, const float* __restrict__ slopes,
-                    int8_t* __restrict__ o_low, int32_t* __restrict__ col_begin, int32_t* __restrict__ col_end) {
+                    int8_t* __restrict__ o_low, int32_t* __restrict__ col_begin, int32_t* __restrict__ col_end, int nsplit,
+                    float* __restrict__ part) {
   // seg_start: the first key that each query sees (packed: its segment's start; span: its span's).
   // o_low (spans, caps and biases): the 8 bits of O below bf16's, written by the forward where given, read with O for
-  // D = rowsum(dO o O). dS = P (dP - D) is a difference that all but cancels where one probability is nearly 1, and
+  // D = rowsum(dO o O).
+  // nsplit > 1 (the same): workgroup `split` of a query block takes every nsplit-th key tile of its walk from tile `split`
+  // on, and writes its dQ, or its O before the division, to part[split] ([b][hq][s][dh]; the forward's maximum and sums
+  // [split][b][hq][s][4] behind all of them): attn_scored.hip joins them.
+  // dS = P (dP - D) is a difference that all but cancels where one probability is nearly 1, and
   // D of the rounded O was the largest part of dQ's and dK's error there (3.6e-3 of the norm against 2.4e-3: 4 x 16 heads,
   // 2048 positions, slopes). A value x is its bf16 plus o_low in units of 2^8 of its bits' value, whatever the exponent.
   constexpr bool PACKED = MASK != kMaskPlain, SPAN = MASK == kMaskSpan, CAP = MOD & kModCap;
@@ -819,7 +830,9 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
   const int npb = (S + P - 1) / P;
   const int hgb = Hq / hpw;
   const int nhg = B * hgb;
-  const int g = blockIdx.x;
+  constexpr bool SCORED = SPAN || MOD != kModNone;
+  const int ns = SCORED ? nsplit : 1, split = SCORED ? (int)blockIdx.x % ns : 0;
+  const int g = SCORED ? (int)blockIdx.x / ns : blockIdx.x;
   // Heaviest query blocks first: the latest under the causal mask; packed, with a work order, item
   // order[g / hgb] (batch row item / npb, query block item % npb), its head groups consecutive.
   int pb, bidx, h0;
@@ -855,11 +868,10 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
   const int32_t* snd = SPAN ? span_end + (long)bidx * S : nullptr;
   const int32_t* sst = PACKED ? seg_start + (long)bidx * S : nullptr;
 
-  constexpr bool SCORED = SPAN || MOD != kModNone;
   // A span backward without work orders: the queries that see each key, for the dK/dV pass (attn_scored.hip), each by the
   // workgroup of the first heads whose queries stand where the key does.
   if constexpr (SPAN && DQ) {
-    if (col_begin != nullptr && h0 == 0 && tid < P && pb * P + tid < S) {
+    if (col_begin != nullptr && h0 == 0 && split == 0 && tid < P && pb * P + tid < S) {
       int qb, qe;
       queries_of(sst, snd, S, pb * P + tid, pb * P + tid, qb, qe);
       col_begin[(long)bidx * S + pb * P + tid] = qb;
@@ -895,7 +907,8 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
   int kv_begin = 0;
   if (SPAN) kv_begin = (in_row(__builtin_amdgcn_readfirstlane(sst[wg_q0])) / kKT) * kKT;
   else if (PACKED) kv_begin = (sst[wg_q0] / kKT) * kKT;
-  const int ntiles = (SPAN && wg_q1 <= kv_begin) ? 0 : (wg_q1 - kv_begin + kKT - 1) / kKT;
+  const int nwalk = (SPAN && wg_q1 <= kv_begin) ? 0 : (wg_q1 - kv_begin + kKT - 1) / kKT;
+  const int ntiles = !SCORED ? nwalk : nwalk > split ? (nwalk - split + ns - 1) / ns : 0;  // this workgroup's
 
   // Packed: with contiguous, gapless segments, key j shares query i's segment and j <= i iff
   // seg_start[i] <= j <= i, so the mask is a range test on this lane's seg_start.
@@ -918,7 +931,7 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
   auto side_of = [&](int kv0) { return (causal || kv0 + kKT - 1 <= qw0) ? 1 : kv0 >= qw0 + 31 ? -1 : 0; };
 
   // Slopes alone: the products K Q^T begin from the bias' ramp where it fits the registers (kv_waves).
-  constexpr bool kRamp = MOD == kModSlope && (DQ ? DH <= 96 : DH != 64);
+  constexpr bool kRamp = MOD == kModSlope && (DQ ? DH <= 96 : DH == 96 || (DH == 128 && !SPAN));
   f32x16 ramp[2];
   if constexpr (kRamp) score.template set_ramp<1>(ramp);
 
@@ -979,9 +992,10 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
   constexpr bool kNearFirst = !DQ && (MOD & kModSlope) && !FIXED;
   const int near = kNearFirst ? (wg_q0 / kKT * kKT <= kv_begin ? 0 : (wg_q0 / kKT * kKT - kv_begin) / kKT) : 0;
   auto tile_at = [&](int t) {
+    if constexpr (SCORED) t = split + t * ns;
     if constexpr (!kNearFirst) return kv_begin + t * kKT;
-    int i = (near < ntiles ? near : ntiles - 1) - t;
-    if (i < 0) i += ntiles;
+    int i = (near < nwalk ? near : nwalk - 1) - t;
+    if (i < 0) i += nwalk;
     return kv_begin + i * kKT;
   };
   auto issue_one = [&](int t, char* st, int j) __attribute__((always_inline)) {
@@ -1023,7 +1037,7 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
       }
     }
     dq_row = sum_xhalf(dp);
-    if (qvalid && hf == 0) {
+    if (qvalid && hf == 0 && split == 0) {
       dvec[qrow + qi] = dq_row;
       if constexpr (SCORED && !(MOD & kModSlope)) dvec[(long)B * Hq * S + qrow + qi] = score.add + 15.f - l2q;  // (kUp there)
     }
@@ -1032,7 +1046,7 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
   // dQ pass, tile t from stage cur; the copies of tile t+1 go to stage nxt (free since the barrier
   // that ended tile t-1).
   auto body = [&](int t, const char* cur, char* nxt) __attribute__((always_inline)) {
-    const int kv0 = kv_begin + t * kKT;
+    const int kv0 = tile_at(t);
     const bool skip = !wave_has || (causal && kv0 > wq_last) || (PACKED && kv0 + kKT - 1 < w_sst_first) ||
                       (SPAN && kv0 >= w_end_last);
     const char* kt = cur;
@@ -1352,6 +1366,31 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
   }
 
   float mul = (DQ && CAP) ? -4.f * scale : scale, lt = 0.f;  // (Score::bend)
+  if constexpr (SCORED) {
+    if (ns > 1) {
+      const long rows = (long)B * Hq * S;
+      if constexpr (!DQ) {
+        lt = l + __shfl_xor(l, 32, 64);
+        const float ltr = lr + __shfl_xor(lr, 32, 64);
+        if (qvalid && hf == 0)
+          *reinterpret_cast<f32x4*>(part + ns * rows * DH + 4 * (split * rows + qrow + qi)) = f32x4{FIXED ? fixed_top() : m, lt, ltr, 0.f};
+        mul = 1.f;
+      }
+      if (qvalid) {
+        float* ph = part + (split * rows + qrow + qi) * DH;
+#pragma unroll
+        for (int db = 0; db < kDB; ++db)
+#pragma unroll
+          for (int rq = 0; rq < 4; ++rq)
+            *reinterpret_cast<f32x4*>(ph + 32 * db + 8 * rq + 4 * hf) =
+                f32x4{acc[db][4 * rq] * mul, acc[db][4 * rq + 1] * mul, acc[db][4 * rq + 2] * mul, acc[db][4 * rq + 3] * mul};
+      }
+      // The padding behind a program's end reads as a write of v0, which the listing check of stores whose data the next
+      // instructions write would hold against a last store of v0.
+      asm volatile("s_nop 0");
+      return;
+    }
+  }
   if constexpr (!DQ) {
     lt = l + __shfl_xor(l, 32, 64);
     const float by = SCORED ? lr + __shfl_xor(lr, 32, 64) : lt;
@@ -1377,9 +1416,8 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
           uint32_t bytes = 0;
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            const int top = (int)((u & 1) ? x[u >> 1] & 0xffff0000u : x[u >> 1] << 16);
-            const int rest = (__builtin_bit_cast(int, acc[db][4 * rq + u] * mul) - top + 0x80) >> 8;  // in [-128, 128]
-            bytes |= (uint32_t)((rest < 127 ? rest : 127) & 0xff) << (8 * u);
+            const uint32_t top = (u & 1) ? x[u >> 1] & 0xffff0000u : x[u >> 1] << 16;
+            bytes |= below_bf16(acc[db][4 * rq + u] * mul, top) << (8 * u);
           }
           *reinterpret_cast<uint32_t*>(ob + col * (DH + 16) + 32 * db + 8 * rq + 4 * hf) = bytes;
         }

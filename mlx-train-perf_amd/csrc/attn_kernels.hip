@@ -138,8 +138,8 @@ hipError_t fwd_dh(const AttnShape& sh, const bf16_t* q, const bf16_t* k, const b
                   const int32_t* sst, bf16_t* o, float* lse, hipStream_t st) {
   const float sl2 = sh.scale * kLog2e;
   dim3 grid(fwd_grid(sh)), block(256);
-  if (sid) hipLaunchKernelGGL((attn_kv_kernel<DH, kMaskPacked, false>), grid, block, 0, st, q, k, v, nullptr, nullptr, nullptr, nullptr, nullptr, sst, o, lse, sh.b, sh.hq, sh.hkv, sh.s, sl2, sh.scale, sh.causal, nullptr, 0.f, nullptr, nullptr, nullptr, nullptr);
-  else hipLaunchKernelGGL((attn_kv_kernel<DH, kMaskPlain, false>), grid, block, 0, st, q, k, v, nullptr, nullptr, nullptr, nullptr, nullptr, sst, o, lse, sh.b, sh.hq, sh.hkv, sh.s, sl2, sh.scale, sh.causal, nullptr, 0.f, nullptr, nullptr, nullptr, nullptr);
+  if (sid) hipLaunchKernelGGL((attn_kv_kernel<DH, kMaskPacked, false>), grid, block, 0, st, q, k, v, nullptr, nullptr, nullptr, nullptr, nullptr, sst, o, lse, sh.b, sh.hq, sh.hkv, sh.s, sl2, sh.scale, sh.causal, nullptr, 0.f, nullptr, nullptr, nullptr, nullptr, 1, nullptr);
+  else hipLaunchKernelGGL((attn_kv_kernel<DH, kMaskPlain, false>), grid, block, 0, st, q, k, v, nullptr, nullptr, nullptr, nullptr, nullptr, sst, o, lse, sh.b, sh.hq, sh.hkv, sh.s, sl2, sh.scale, sh.causal, nullptr, 0.f, nullptr, nullptr, nullptr, nullptr, 1, nullptr);
   return hipGetLastError();
 }
 
@@ -168,8 +168,8 @@ hipError_t bwd_dh(const AttnShape& sh, const bf16_t* q, const bf16_t* k, const b
     if (e != hipSuccess) return e;
   }
   dim3 qgrid(fwd_grid(sh));
-  if (sid) hipLaunchKernelGGL((attn_kv_kernel<DH, kMaskPacked, true>), qgrid, block, 0, st, q, k, v, d_o, o, lse, dvec, nullptr, sst, dq, nullptr, sh.b, sh.hq, sh.hkv, sh.s, sl2, sh.scale, sh.causal, q_order, 0.f, nullptr, nullptr, nullptr, nullptr);
-  else hipLaunchKernelGGL((attn_kv_kernel<DH, kMaskPlain, true>), qgrid, block, 0, st, q, k, v, d_o, o, lse, dvec, nullptr, sst, dq, nullptr, sh.b, sh.hq, sh.hkv, sh.s, sl2, sh.scale, sh.causal, nullptr, 0.f, nullptr, nullptr, nullptr, nullptr);
+  if (sid) hipLaunchKernelGGL((attn_kv_kernel<DH, kMaskPacked, true>), qgrid, block, 0, st, q, k, v, d_o, o, lse, dvec, nullptr, sst, dq, nullptr, sh.b, sh.hq, sh.hkv, sh.s, sl2, sh.scale, sh.causal, q_order, 0.f, nullptr, nullptr, nullptr, nullptr, 1, nullptr);
+  else hipLaunchKernelGGL((attn_kv_kernel<DH, kMaskPlain, true>), qgrid, block, 0, st, q, k, v, d_o, o, lse, dvec, nullptr, sst, dq, nullptr, sh.b, sh.hq, sh.hkv, sh.s, sl2, sh.scale, sh.causal, nullptr, 0.f, nullptr, nullptr, nullptr, nullptr, 1, nullptr);
   e = hipGetLastError();
   if (e != hipSuccess) return e;
   // Split key blocks write fp32 partials after the D vector in the workspace; the reduce sums them.

@@ -70,6 +70,70 @@ int scored_nsplit(int b, int hq, int hkv, int s, int dh, int causal) {
   while (ns > 1 && items < ns * (wgs * ns <= kNumCU + kNumCU / 4 ? 2 : 16)) ns /= 2;
   return ns;
 }
+// Splits of the forward and dQ passes over the keys (1: none): as many as give every CU a workgroup with four tiles of the
+// longest walk, or both its places one with eight (spans, whose walks are mostly shorter: sixteen). GPU time of a step,
+// unsplit, for one workgroup a CU and for two: 1 x 2/1 x 2932 x 128 211, 106 and 106 us; 1 x 4/1 x 4000 x 64 226, 159 and
+// 132; 4 x 16/8 x 509 x 64 (256 workgroups) 61, 61 and 72; windows of 500 in 2 x 4/4 x 4000 x 64 83, 83 and 93, prefixes 197,
+// 197 and 163.
+int q_splits(int b, int hq, int hkv, int s, bool span) {
+  const AttnShape sh{b, hq, hkv, s, 0, 0.f, 0};
+  const int wgs = q_grid(sh), tiles = (s + kKT - 1) / kKT;
+  auto least = [](int x, int y) { return x < y ? x : y; };
+  const int one = least(kNumCU / wgs, tiles / 4), two = least(2 * kNumCU / wgs, tiles / (span ? 16 : 8));
+  const int ns = one > two ? one : two;
+  return ns < 1 ? 1 : ns > 8 ? 8 : ns;
+}
+size_t fwd_part_bytes(int b, int hq, int s, int dh, int ns) { return ns > 1 ? (size_t)ns * b * hq * s * (dh + 4) * 4 : 0; }
+
+// O, its bits below bf16 and L from the parts of a split forward: with M the largest maximum,
+// O = sum 2^(m - M) O_part / sum 2^(m - M) lr_part. Eight values of a row a thread.
+__global__ __launch_bounds__(256) void attn_join_kernel(const float* __restrict__ part, int ns, long rows, int dh, int span,
+                                                        bf16_t* __restrict__ o, int8_t* __restrict__ o_low,
+                                                        float* __restrict__ lse) {
+  const long e = ((long)blockIdx.x * 256 + threadIdx.x) * 8, row = e / dh;
+  if (row >= rows) return;
+  const f32x4* ml = reinterpret_cast<const f32x4*>(part + ns * rows * dh);
+  float top = kNegInf, l = 0.f, lr = 0.f;
+  for (int sp = 0; sp < ns; ++sp) top = fmaxf(top, ml[sp * rows + row][0]);
+  const float base = top == kNegInf ? 0.f : top;
+  f32x4 x[2] = {};
+  for (int sp = 0; sp < ns; ++sp) {
+    const f32x4 v = ml[sp * rows + row];
+    const float w = fast_exp2(v[0] - base);  // a part without keys: 2^-inf
+    l += w * v[1];
+    lr += w * v[2];
+    const f32x4* p = reinterpret_cast<const f32x4*>(part + sp * rows * dh + e);
+    x[0] += w * p[0];
+    x[1] += w * p[1];
+  }
+  const float mul = lr > 0.f ? 1.f / lr : 0.f;
+  u32x4 hi;
+  uint32_t low[2] = {0, 0};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float a = x[j >> 1][2 * (j & 1)] * mul, c = x[j >> 1][2 * (j & 1) + 1] * mul;
+    hi[j] = pack_bf16x2(a, c);
+    low[j >> 1] |= (below_bf16(a, hi[j] << 16) | below_bf16(c, hi[j] & 0xffff0000u) << 8) << (16 * (j & 1));
+  }
+  *reinterpret_cast<u32x4*>(o + e) = hi;
+  if (o_low) *reinterpret_cast<u32x2*>(o_low + e) = u32x2{low[0], low[1]};
+  if (e % dh == 0) lse[row] = l > 0.f ? (top + fast_log2(l)) * kLn2 : span ? -kNegInf : kNegInf;
+}
+// dQ = the sum of the parts of a split pass, in order.
+__global__ __launch_bounds__(256) void attn_dq_sum_kernel(const float* __restrict__ part, int ns, long plane, bf16_t* __restrict__ dq) {
+  const long e = ((long)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (e >= plane) return;
+  f32x4 x[2] = {};
+  for (int sp = 0; sp < ns; ++sp) {
+    const f32x4* p = reinterpret_cast<const f32x4*>(part + sp * plane + e);
+    x[0] += p[0];
+    x[1] += p[1];
+  }
+  *reinterpret_cast<u32x4*>(dq + e) = u32x4{pack_bf16x2(x[0][0], x[0][1]), pack_bf16x2(x[0][2], x[0][3]),
+                                            pack_bf16x2(x[1][0], x[1][1]), pack_bf16x2(x[1][2], x[1][3])};
+}
+dim3 eights_grid(long values) { return dim3((unsigned)((values / 8 + 255) / 256)); }
+
 // Whether the workgroups of a span backward's passes take turns, so that their order counts.
 bool ordered(int b, int hq, int hkv, int s, int dh) {
   const AttnShape sh{b, hq, hkv, s, dh, 0.f, 0};
@@ -98,7 +162,9 @@ size_t carve(int b, int hq, int hkv, int s, int dh, char* base, ScoredWorkspace*
   const int ns = ns1 > ns0 ? ns1 : ns0;
   Carver c{base};
   c.take(ws->dvec, (size_t)2 * b * hq * s);
-  c.take(ws->part, ns > 1 ? (size_t)ns * 2 * b * hkv * s * dh : 0);
+  const int nq = q_splits(b, hq, hkv, s, false);  // (spans: no more)
+  const size_t kv_part = ns > 1 ? (size_t)ns * 2 * b * hkv * s * dh : 0, q_part = nq > 1 ? (size_t)nq * b * hq * s * dh : 0;
+  c.take(ws->part, kv_part > q_part ? kv_part : q_part);
   carve_plan(c, b, hq, hkv, s, ws);
   return c.at;
 }
@@ -115,6 +181,14 @@ size_t attn_scored_bwd_workspace(int b, int hq, int hkv, int s, int dh) {
   return carve(b, hq, hkv, s, dh, nullptr, &ws);
 }
 
+size_t attn_scored_fwd_workspace(int b, int hq, int hkv, int s, int dh) {
+  return fwd_part_bytes(b, hq, s, dh, q_splits(b, hq, hkv, s, false));
+}
+hipError_t launch_attn_dq_sum(const float* part, int ns, long plane, bf16_t* dq, hipStream_t st) {
+  hipLaunchKernelGGL(attn_dq_sum_kernel, eights_grid(plane), dim3(256), 0, st, part, ns, plane, dq);
+  return hipGetLastError();
+}
+
 size_t attn_scored_plan(int b, int hq, int hkv, int s, int dh) {
   if (!ordered(b, hq, hkv, s, dh)) return 0;
   ScoredWorkspace ws;
@@ -124,7 +198,8 @@ size_t attn_scored_plan(int b, int hq, int hkv, int s, int dh) {
 }
 
 hipError_t launch_attn_scored_fwd(const AttnShape& sh, const AttnScore& sc, const bf16_t* q, const bf16_t* k,
-                                  const bf16_t* v, bf16_t* o, int8_t* o_low, int32_t* plan, float* lse, hipStream_t st) {
+                                  const bf16_t* v, bf16_t* o, int8_t* o_low, int32_t* plan, float* lse,
+                                  void* workspace, size_t bytes, hipStream_t st) {
   // The forward of a training step makes the backward's plan, and goes by its order of query blocks too (documents of 64
   // to 2048 in 8192 positions, 16/4 heads, head_dim 128: 62 against 76 us).
   const int32_t* order = nullptr;
@@ -136,12 +211,21 @@ hipError_t launch_attn_scored_fwd(const AttnShape& sh, const AttnScore& sc, cons
     if (e != hipSuccess) return e;
     order = ws.q_order;
   }
+  int ns = q_splits(sh.b, sh.hq, sh.hkv, sh.s, sc.start != nullptr);
+  if (!workspace || bytes < fwd_part_bytes(sh.b, sh.hq, sh.s, sh.dh, ns)) ns = 1;
+  float* part = static_cast<float*>(workspace);
+  hipError_t e = hipErrorInvalidValue;
   switch (sh.dh) {
-    case 64: return scored_fwd<64>(sh, sc, q, k, v, o, o_low, order, lse, q_grid(sh), st);
-    case 96: return scored_fwd<96>(sh, sc, q, k, v, o, o_low, order, lse, q_grid(sh), st);
-    case 128: return scored_fwd<128>(sh, sc, q, k, v, o, o_low, order, lse, q_grid(sh), st);
-    default: return hipErrorInvalidValue;
+    case 64: e = scored_fwd<64>(sh, sc, q, k, v, o, o_low, order, lse, q_grid(sh), ns, part, st); break;
+    case 96: e = scored_fwd<96>(sh, sc, q, k, v, o, o_low, order, lse, q_grid(sh), ns, part, st); break;
+    case 128: e = scored_fwd<128>(sh, sc, q, k, v, o, o_low, order, lse, q_grid(sh), ns, part, st); break;
+    default: break;
   }
+  if (e != hipSuccess || ns == 1) return e;
+  const long rows = (long)sh.b * sh.hq * sh.s;
+  hipLaunchKernelGGL(attn_join_kernel, eights_grid(rows * sh.dh), dim3(256), 0, st, part, ns, rows, sh.dh, sc.start != nullptr,
+                     o, o_low, lse);
+  return hipGetLastError();
 }
 
 hipError_t launch_attn_scored_bwd(const AttnShape& sh, const AttnScore& sc, const bf16_t* q, const bf16_t* k,
@@ -151,6 +235,7 @@ hipError_t launch_attn_scored_bwd(const AttnShape& sh, const AttnScore& sc, cons
   ScoredWorkspace ws;
   carve(sh.b, sh.hq, sh.hkv, sh.s, sh.dh, static_cast<char*>(workspace), &ws);
   ws.nsplit = scored_nsplit(sh.b, sh.hq, sh.hkv, sh.s, sh.dh, sc.start ? 1 : sh.causal);
+  ws.nq = q_splits(sh.b, sh.hq, sh.hkv, sh.s, sc.start != nullptr);
   hipError_t e = hipSuccess;
   // Where all workgroups of both passes run at once their order is of no account, and the dQ pass fills the key ranges
   // that the dK/dV pass reads: a launch less (a step of 4 x 16/8 x 509 x 64: 63.2 against

@@ -5,18 +5,21 @@
 
 namespace mtp {
 
-// A backward call's workspace, in order: D, without slopes the logarithms in the P waves' form, the fp32 partials of a split dK/dV pass, and for spans the two work
+// A backward call's workspace, in order: D, without slopes the logarithms in the P waves' form, the fp32 parts of a split
+// dQ, then dK/dV pass, and for spans the two work
 // orders (null: none) and the queries [col_begin, col_end) that see each key.
 struct ScoredWorkspace {
   float* dvec;
   float* part;
   int32_t *q_order, *kv_order, *col_begin, *col_end;
-  int nsplit;
+  int nsplit, nq;  // of the dK/dV pass, of the dQ pass
 };
+hipError_t launch_attn_dq_sum(const float* part, int ns, long plane, bf16_t* dq, hipStream_t st);
 
 template <int DH>
 hipError_t scored_fwd(const AttnShape& sh, const AttnScore& sc, const bf16_t* q, const bf16_t* k, const bf16_t* v,
-                      bf16_t* o, int8_t* o_low, const int32_t* order, float* lse, int grid, hipStream_t st);
+                      bf16_t* o, int8_t* o_low, const int32_t* order, float* lse, int grid, int nsplit, float* part,
+                      hipStream_t st);
 template <int DH>
 hipError_t scored_bwd(const AttnShape& sh, const AttnScore& sc, const ScoredWorkspace& ws, const bf16_t* q,
                       const bf16_t* k, const bf16_t* v, const bf16_t* o, const int8_t* o_low, const float* lse,
@@ -39,14 +42,14 @@ hipError_t with_mod(const AttnScore& sc, F&& f) {
 template <>
 hipError_t scored_fwd<MTP_SCORED_DH>(const AttnShape& sh, const AttnScore& sc, const bf16_t* q, const bf16_t* k,
                                      const bf16_t* v, bf16_t* o, int8_t* o_low, const int32_t* order,
-                                     float* lse, int grid, hipStream_t st) {
+                                     float* lse, int grid, int nsplit, float* part, hipStream_t st) {
   constexpr int DH = MTP_SCORED_DH;
   return with_mod(sc, [&](auto m) {
     constexpr int MOD = decltype(m)::value;
     auto launch = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, st, q, k, v, nullptr, nullptr, nullptr, nullptr, sc.end,
+      hipLaunchKernelGGL(kernel, dim3(grid * nsplit), dim3(256), 0, st, q, k, v, nullptr, nullptr, nullptr, nullptr, sc.end,
                          sc.start, o, lse, sh.b, sh.hq, sh.hkv, sh.s, sh.scale * kLog2e, sh.scale, sh.causal, order,
-                         sc.cap, sc.slopes, o_low, nullptr, nullptr);
+                         sc.cap, sc.slopes, o_low, nullptr, nullptr, nsplit, part);
       return hipGetLastError();
     };
     // A cap above kFixedCap runs as a cap with slopes of none; spans may hide a query's own key, whose bias of 0 the
@@ -74,12 +77,14 @@ hipError_t scored_bwd<MTP_SCORED_DH>(const AttnShape& sh, const AttnScore& sc, c
   return with_mod(sc, [&](auto m) {
     constexpr int MOD = decltype(m)::value;
     auto launch = [&](auto dq_kernel, auto dkv_kernel) {
-      hipLaunchKernelGGL(dq_kernel, dim3(grid), dim3(256), 0, st, q, k, v, d_o, o, lse, ws.dvec, sc.end, sc.start, dq,
+      hipLaunchKernelGGL(dq_kernel, dim3(grid * ws.nq), dim3(256), 0, st, q, k, v, d_o, o, lse, ws.dvec, sc.end, sc.start, dq,
                          nullptr, sh.b, sh.hq, sh.hkv, sh.s, sh.scale * kLog2e, sh.scale, sh.causal, ws.q_order, sc.cap,
                          sc.slopes, const_cast<int8_t*>(o_low), ws.q_order ? nullptr : ws.col_begin,
-                         ws.q_order ? nullptr : ws.col_end);
+                         ws.q_order ? nullptr : ws.col_end, ws.nq, ws.part);
       hipError_t e = hipGetLastError();
+      if (e == hipSuccess && ws.nq > 1) e = launch_attn_dq_sum(ws.part, ws.nq, (long)sh.b * sh.hq * sh.s * sh.dh, dq, st);
       if (e != hipSuccess) return e;
+      // (the parts of dQ are read: those of dK and dV take their place)
       hipLaunchKernelGGL(dkv_kernel, dim3((sh.s + 127) / 128 * sh.b * sh.hkv * ws.nsplit), dim3(512), 0, st, q, k, v, d_o,
                          (MOD & kModSlope) ? lse : ws.dvec + (long)sh.b * sh.hq * sh.s, ws.dvec, ws.col_end, dk, dv, sh.b, sh.hq, sh.hkv, sh.s, sh.scale * kLog2e, sh.scale,
                          sh.causal, ws.nsplit, ws.part, ws.kv_order, ws.col_begin, sc.cap, sc.slopes);

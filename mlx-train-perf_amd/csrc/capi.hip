@@ -618,16 +618,16 @@ int mtp_attn_bwd_f32(const float* q, const float* k, const float* v, const float
 int mtp_attn_scored_fwd(const void* q, const void* k, const void* v, int64_t b, int64_t hq, int64_t hkv, int64_t s,
                         int64_t dh, float scale, int32_t causal, float softcap, const float* slopes,
                         const int32_t* span_start, const int32_t* span_end, void* o, int8_t* o_low, int32_t* plan,
-                        float* lse, void* stream) {
+                        float* lse, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_scored(q, k, v, b, hq, hkv, s, dh, scale, causal, softcap, slopes, span_start, span_end);
   if (rc) return rc;
   if (!o || !lse) return fail(MTP_ERR_INPUT, "o and lse must be non-null");
-  if (!aligned16(o) || !aligned16(o_low) || !aligned16(plan)) return fail(MTP_ERR_UNSUPPORTED, "o, o_low and plan must be 16-byte aligned");
+  if (!aligned16(o) || !aligned16(o_low) || !aligned16(plan) || !aligned16(workspace)) return fail(MTP_ERR_UNSUPPORTED, "o, o_low, plan and workspace must be 16-byte aligned");
   mtp::AttnShape sh{(int)b, (int)hq, (int)hkv, (int)s, (int)dh, scale, (int)causal};
   mtp::AttnScore sc{softcap, slopes, span_start, span_end};
   hipError_t e = mtp::launch_attn_scored_fwd(sh, sc, static_cast<const mtp::bf16_t*>(q), static_cast<const mtp::bf16_t*>(k),
                                              static_cast<const mtp::bf16_t*>(v), static_cast<mtp::bf16_t*>(o), o_low, plan, lse,
-                                             static_cast<hipStream_t>(stream));
+                                             workspace, workspace_bytes, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return fail(MTP_ERR_RUNTIME, "scored attention forward launch failed: %s", hipGetErrorString(e));
   return ok();
 }
@@ -656,6 +656,11 @@ size_t mtp_attn_scored_fwd_f32_workspace_bytes(int64_t b, int64_t hq, int64_t hk
 size_t mtp_attn_scored_bwd_f32_workspace_bytes(int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh) {
   if (b < 1 || hq < 1 || hkv < 1 || s < 1 || hq % hkv || b * hq * s > kMaxDim) return 0;
   return mtp::attn32_scored_bwd_workspace((int)b, (int)hq, (int)hkv, (int)s, (int)dh);
+}
+
+size_t mtp_attn_scored_fwd_workspace_bytes(int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh) {
+  if (b < 1 || hq < 1 || hkv < 1 || s < 1 || hq % hkv || b * hq * s > kMaxDim) return 0;
+  return mtp::attn_scored_fwd_workspace((int)b, (int)hq, (int)hkv, (int)s, (int)dh);
 }
 
 size_t mtp_attn_scored_plan_bytes(int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh) {

@@ -98,10 +98,11 @@ struct AttnScore {
   const int32_t* end;
 };
 size_t attn_scored_bwd_workspace(int b, int hq, int hkv, int s, int dh);
+size_t attn_scored_fwd_workspace(int b, int hq, int hkv, int s, int dh);  // less: unsplit
 size_t attn_scored_plan(int b, int hq, int hkv, int s, int dh);  // bytes; 0: no use for one
 hipError_t launch_attn_scored_fwd(const AttnShape& sh, const AttnScore& sc, const bf16_t* q, const bf16_t* k,
                                   const bf16_t* v, bf16_t* o, int8_t* o_low, int32_t* plan, float* lse,
-                                  hipStream_t stream);
+                                  void* workspace, size_t bytes, hipStream_t stream);
 hipError_t launch_attn_scored_bwd(const AttnShape& sh, const AttnScore& sc, const bf16_t* q, const bf16_t* k,
                                   const bf16_t* v, const bf16_t* o, const int8_t* o_low, const int32_t* plan,
                                   const float* lse, const bf16_t* d_o, bf16_t* dq, bf16_t* dk, bf16_t* dv, void* workspace,

@@ -47,6 +47,7 @@ struct Entries {
   decltype(&mtp_attn_scored_fwd) scored_fwd = nullptr;
   decltype(&mtp_attn_scored_bwd) scored_bwd = nullptr;
   decltype(&mtp_attn_scored_plan_bytes) scored_plan = nullptr;
+  decltype(&mtp_attn_scored_fwd_workspace_bytes) scored_fwd_ws = nullptr;
   decltype(&mtp_attn_scored_bwd_workspace_bytes) scored_ws = nullptr;
   decltype(&mtp_attn_scored_fwd_f32_workspace_bytes) scored_fwd_ws32 = nullptr, scored_bwd_ws32 = nullptr;
   decltype(&mtp_attn_scored_fwd_f32) scored_fwd32 = nullptr;
@@ -190,21 +191,22 @@ struct ScoredAttention : torch::autograd::Function<ScoredAttention> {
     const at::Tensor o = at::empty_like(q), lse = at::empty({b, hq, s}, q.options().dtype(at::kFloat));
     const float cap = (float)score.softcap;
     at::Tensor low, plan;  // the bits of O below its bf16 ones, and the spans' plan, for the backward
-    if (q.scalar_type() == at::kFloat) {
-      const size_t bytes = g_api.scored_fwd_ws32(b, hq, hkv, s, dh);
-      const at::Tensor ws = bytes ? at::empty({(int64_t)bytes}, q.options().dtype(at::kByte)) : at::Tensor();
+    const bool f32 = q.scalar_type() == at::kFloat;
+    const size_t bytes = (f32 ? g_api.scored_fwd_ws32 : g_api.scored_fwd_ws)(b, hq, hkv, s, dh);
+    const at::Tensor ws = bytes ? at::empty({(int64_t)bytes}, q.options().dtype(at::kByte)) : at::Tensor();
+    if (f32) {
       check(g_api.scored_fwd32(ptr<float>(q), ptr<float>(k), ptr<float>(v), b, hq, hkv, s, dh, (float)scale, causal, cap,
                                floats(score.slopes), ints(score.start), ints(score.end), ptr<float>(o), ptr<float>(lse),
                                opt_ptr(ws), bytes, stream_of(q)));
     } else {
       if (score.train) {
         low = at::empty_like(q, q.options().dtype(at::kChar));
-        const size_t bytes = score.start.defined() ? g_api.scored_plan(b, hq, hkv, s, dh) : 0;
-        if (bytes) plan = at::empty({(int64_t)bytes / 4}, q.options().dtype(at::kInt));
+        const size_t size = score.start.defined() ? g_api.scored_plan(b, hq, hkv, s, dh) : 0;
+        if (size) plan = at::empty({(int64_t)size / 4}, q.options().dtype(at::kInt));
       }
       check(g_api.scored_fwd(ptr(q), ptr(k), ptr(v), b, hq, hkv, s, dh, (float)scale, causal, cap, floats(score.slopes),
                              ints(score.start), ints(score.end), ptr(o), opt_ptr<int8_t>(low), opt_ptr<int32_t>(plan), ptr<float>(lse),
-                             stream_of(q)));
+                             opt_ptr(ws), bytes, stream_of(q)));
     }
     ctx->save_for_backward({q, k, v, o, low, plan, lse, score.slopes, score.start, score.end});
     ctx->saved_data["scale"] = scale;
@@ -580,6 +582,7 @@ void bind(const py::dict& entries, py::object check_fn) {
   set(g_api.scored_fwd, "mtp_attn_scored_fwd");
   set(g_api.scored_bwd, "mtp_attn_scored_bwd");
   set(g_api.scored_plan, "mtp_attn_scored_plan_bytes");
+  set(g_api.scored_fwd_ws, "mtp_attn_scored_fwd_workspace_bytes");
   set(g_api.scored_ws, "mtp_attn_scored_bwd_workspace_bytes");
   set(g_api.scored_fwd_ws32, "mtp_attn_scored_fwd_f32_workspace_bytes");
   set(g_api.scored_bwd_ws32, "mtp_attn_scored_bwd_f32_workspace_bytes");

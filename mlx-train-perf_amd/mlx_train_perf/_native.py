@@ -105,12 +105,12 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     # capped scores, a bias by distance, key spans
     "mtp_attn_scored_fwd": (ctypes.c_int, [_c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _i64, _f32, _i32, _f32,
                                            _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
-                                           _c_void_p]),
+                                           _c_void_p, _size, _c_void_p]),
     "mtp_attn_scored_fwd_f32": (ctypes.c_int, [_c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i64, _i64, _i64, _f32, _i32,
                                                _f32, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _size,
                                                _c_void_p]),
     **{name: (_size, [_i64, _i64, _i64, _i64, _i64])
-       for name in ("mtp_attn_scored_plan_bytes", "mtp_attn_scored_bwd_workspace_bytes", "mtp_attn_scored_fwd_f32_workspace_bytes",
+       for name in ("mtp_attn_scored_plan_bytes", "mtp_attn_scored_fwd_workspace_bytes", "mtp_attn_scored_bwd_workspace_bytes", "mtp_attn_scored_fwd_f32_workspace_bytes",
                     "mtp_attn_scored_bwd_f32_workspace_bytes")},
     **{name: (ctypes.c_int, [*[_c_void_p] * tensors, _i64, _i64, _i64, _i64, _i64,
                              _f32, _i32, _f32, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,

@@ -290,16 +290,18 @@ def scored_forward(q, k, v, slopes, start, end, *, scale: float, causal: bool, s
     args = (q.data_ptr(), k.data_ptr(), v.data_ptr(), *shape, scale, int(causal), softcap, _native.ptr(slopes), _native.ptr(start),
             _native.ptr(end), o.data_ptr())
     low = plan = None
+    f32 = q.dtype == torch.float32
+    ws_bytes = (lib.mtp_attn_scored_fwd_f32_workspace_bytes if f32 else lib.mtp_attn_scored_fwd_workspace_bytes)(*shape)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
     with _native.on_device(q):
-        if q.dtype == torch.float32:
-            ws_bytes = lib.mtp_attn_scored_fwd_f32_workspace_bytes(*shape)
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+        if f32:
             rc = lib.mtp_attn_scored_fwd_f32(*args, lse.data_ptr(), _native.ptr(ws), ws_bytes, _native.stream_of(q))
         else:
             low = torch.empty_like(q, dtype=torch.int8) if train else None
             plan_bytes = lib.mtp_attn_scored_plan_bytes(*shape) if train and start is not None else 0
             plan = torch.empty(plan_bytes // 4, dtype=torch.int32, device=q.device) if plan_bytes else None
-            rc = lib.mtp_attn_scored_fwd(*args, _native.ptr(low), _native.ptr(plan), lse.data_ptr(), _native.stream_of(q))
+            rc = lib.mtp_attn_scored_fwd(*args, _native.ptr(low), _native.ptr(plan), lse.data_ptr(), _native.ptr(ws),
+                                         ws_bytes, _native.stream_of(q))
     _native.check(rc, domain="attention")
     return o, lse, low, plan
 

@@ -442,3 +442,33 @@ def test_captured_step_with_a_plan():
         g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, w) for a, w in zip(out, step(new))), mask
+
+
+@pytest.mark.parametrize(("b", "hq", "hkv", "s", "dh"), [(1, 2, 1, 520, 64), (1, 1, 1, 1100, 128), (1, 8, 2, 777, 96), (2, 4, 4, 300, 128),
+                                                    (2, 4, 4, 600, 128)])
+@pytest.mark.parametrize(("mask", "cap", "biased"), [("causal", 20.0, False), ("full", None, True), ("docs", 30.0, True),
+                                                     ("ragged", None, False), ("window", 80.0, False), ("prefix", None, True),
+                                                     ("causal", 20.0, True)])
+def test_passes_split_over_the_keys(b, hq, hkv, s, dh, mask, cap, biased):
+    """Few workgroups: the forward and dQ of bf16 are split, and their parts (some without a key of a row) joined. O, L and
+    the bits below O are those of an unsplit forward but for the order of sums; without a workspace it is unsplit."""
+    from mlx_train_perf import _native
+    from mlx_train_perf.attention.api import scored_forward
+
+    lib = _native.load()
+    assert (lib.mtp_attn_scored_fwd_workspace_bytes(b, hq, hkv, s, dh) > 0) == (s >= 512)   # two splits of four tiles
+    _check(b, hq, hkv, s, dh, mask=mask, cap=cap, biased=biased, dtype=torch.bfloat16, seed=dh)
+    q, k, v, _ = (x.cuda() for x in S.inputs(b, hq, hkv, s, dh, torch.bfloat16, 3))
+    slopes = S.slopes_of(hq).cuda() if biased else None
+    spans = S.spans_of(mask, b, s, 3)
+    start, end = (None, None) if spans is None else (t.cuda() for t in spans)
+    causal = mask == "causal"
+    o, lse, low, _ = scored_forward(q, k, v, slopes, start, end, scale=0.1, causal=causal, softcap=cap or 0.0)
+    o1, low1, lse1 = torch.empty_like(o), torch.empty_like(low), torch.empty_like(lse)
+    assert lib.mtp_attn_scored_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), b, hq, hkv, s, dh, 0.1, int(causal), cap or 0.0,
+                                   _native.ptr(slopes), _native.ptr(start), _native.ptr(end), o1.data_ptr(), low1.data_ptr(), None,
+                                   lse1.data_ptr(), None, 0, _native.stream_of(q)) == 0
+    fine = lambda x, y: (x.float().view(torch.int32) + (y.to(torch.int32) << 8)).view(torch.float32).double()  # noqa: E731
+    seen = torch.isfinite(lse1)
+    assert torch.equal(seen, torch.isfinite(lse)) and torch.allclose(lse[seen], lse1[seen], rtol=2e-6, atol=2e-5)
+    assert S.rel(fine(o, low), fine(o1, low1)) <= 2 ** -8   # another maximum rounds the probabilities elsewhere

@@ -142,7 +142,7 @@ def test_c_abi_refusals():
     def fwd(scale=1.0, causal=0, cap=1.0, slopes=none, start=none, end=none, q=p, o=p, shape=shape, lib_fn=lib.mtp_attn_scored_fwd):
         f32 = lib_fn is lib.mtp_attn_scored_fwd_f32
         return lib_fn(q, p, p, *shape, scale, causal, cap, slopes, start, end, o, *(() if f32 else (none, none)), p,
-                      *((none, 0) if f32 else ()), none)
+                      none, 0, none)
 
     bad, un = _native.MTP_ERR_INPUT, _native.MTP_ERR_UNSUPPORTED
     for fn in (lib.mtp_attn_scored_fwd, lib.mtp_attn_scored_fwd_f32):
