@@ -796,7 +796,7 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
 // The dQ pass would spill.
 template <int DH, int MASK, bool DQ, int MOD>
 constexpr int kv_waves() { return DH == 64 && !DQ && (MASK == kMaskSpan || MOD != kModNone) ? 3 : 2; }
-template <int DH, int MASK, bool DQ, int MOD = kModNone, bool FIXED = false>
+template <int DH, int MASK, bool DQ, int MOD = kModNone, bool FIXED = false, bool SPLIT = false>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(kv_waves<DH, MASK, DQ, MOD>(), kv_waves<DH, MASK, DQ, MOD>())))
 void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, const bf16_t* __restrict__ v,
                     const bf16_t* __restrict__ d_o, const bf16_t* __restrict__ o_in, const float* __restrict__ lse_in,
@@ -809,7 +809,7 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
   // seg_start: the first key that each query sees (packed: its segment's start; span: its span's).
   // o_low (spans, caps and biases): the 8 bits of O below bf16's, written by the forward where given, read with O for
   // D = rowsum(dO o O).
-  // nsplit > 1 (the same): workgroup `split` of a query block takes every nsplit-th key tile of its walk from tile `split`
+  // SPLIT (the same; a variant of its own, as its walk cost the others 2.5%): workgroup `split` of a query block takes every nsplit-th key tile of its walk from tile `split`
   // on, and writes its dQ, or its O before the division, to part[split] ([b][hq][s][dh]; the forward's maximum and sums
   // [split][b][hq][s][4] behind all of them): attn_scored.hip joins them.
   // dS = P (dP - D) is a difference that all but cancels where one probability is nearly 1, and
@@ -831,8 +831,9 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
   const int hgb = Hq / hpw;
   const int nhg = B * hgb;
   constexpr bool SCORED = SPAN || MOD != kModNone;
-  const int ns = SCORED ? nsplit : 1, split = SCORED ? (int)blockIdx.x % ns : 0;
-  const int g = SCORED ? (int)blockIdx.x / ns : blockIdx.x;
+  static_assert(!SPLIT || SCORED);
+  const int ns = SPLIT ? nsplit : 1, split = SPLIT ? (int)blockIdx.x % ns : 0;
+  const int g = SPLIT ? (int)blockIdx.x / ns : blockIdx.x;
   // Heaviest query blocks first: the latest under the causal mask; packed, with a work order, item
   // order[g / hgb] (batch row item / npb, query block item % npb), its head groups consecutive.
   int pb, bidx, h0;
@@ -908,7 +909,7 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
   if (SPAN) kv_begin = (in_row(__builtin_amdgcn_readfirstlane(sst[wg_q0])) / kKT) * kKT;
   else if (PACKED) kv_begin = (sst[wg_q0] / kKT) * kKT;
   const int nwalk = (SPAN && wg_q1 <= kv_begin) ? 0 : (wg_q1 - kv_begin + kKT - 1) / kKT;
-  const int ntiles = !SCORED ? nwalk : nwalk > split ? (nwalk - split + ns - 1) / ns : 0;  // this workgroup's
+  const int ntiles = !SPLIT ? nwalk : nwalk > split ? (nwalk - split + ns - 1) / ns : 0;  // this workgroup's
 
   // Packed: with contiguous, gapless segments, key j shares query i's segment and j <= i iff
   // seg_start[i] <= j <= i, so the mask is a range test on this lane's seg_start.
@@ -931,7 +932,7 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
   auto side_of = [&](int kv0) { return (causal || kv0 + kKT - 1 <= qw0) ? 1 : kv0 >= qw0 + 31 ? -1 : 0; };
 
   // Slopes alone: the products K Q^T begin from the bias' ramp where it fits the registers (kv_waves).
-  constexpr bool kRamp = MOD == kModSlope && (DQ ? DH <= 96 : DH == 96 || (DH == 128 && !SPAN));
+  constexpr bool kRamp = MOD == kModSlope && (DQ ? DH <= 96 : DH == 96 || (DH == 128 && !(SPAN && SPLIT)));
   f32x16 ramp[2];
   if constexpr (kRamp) score.template set_ramp<1>(ramp);
 
@@ -992,7 +993,7 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
   constexpr bool kNearFirst = !DQ && (MOD & kModSlope) && !FIXED;
   const int near = kNearFirst ? (wg_q0 / kKT * kKT <= kv_begin ? 0 : (wg_q0 / kKT * kKT - kv_begin) / kKT) : 0;
   auto tile_at = [&](int t) {
-    if constexpr (SCORED) t = split + t * ns;
+    if constexpr (SPLIT) t = split + t * ns;
     if constexpr (!kNearFirst) return kv_begin + t * kKT;
     int i = (near < nwalk ? near : nwalk - 1) - t;
     if (i < 0) i += nwalk;
@@ -1366,30 +1367,28 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
   }
 
   float mul = (DQ && CAP) ? -4.f * scale : scale, lt = 0.f;  // (Score::bend)
-  if constexpr (SCORED) {
-    if (ns > 1) {
-      const long rows = (long)B * Hq * S;
-      if constexpr (!DQ) {
-        lt = l + __shfl_xor(l, 32, 64);
-        const float ltr = lr + __shfl_xor(lr, 32, 64);
-        if (qvalid && hf == 0)
-          *reinterpret_cast<f32x4*>(part + ns * rows * DH + 4 * (split * rows + qrow + qi)) = f32x4{FIXED ? fixed_top() : m, lt, ltr, 0.f};
-        mul = 1.f;
-      }
-      if (qvalid) {
-        float* ph = part + (split * rows + qrow + qi) * DH;
-#pragma unroll
-        for (int db = 0; db < kDB; ++db)
-#pragma unroll
-          for (int rq = 0; rq < 4; ++rq)
-            *reinterpret_cast<f32x4*>(ph + 32 * db + 8 * rq + 4 * hf) =
-                f32x4{acc[db][4 * rq] * mul, acc[db][4 * rq + 1] * mul, acc[db][4 * rq + 2] * mul, acc[db][4 * rq + 3] * mul};
-      }
-      // The padding behind a program's end reads as a write of v0, which the listing check of stores whose data the next
-      // instructions write would hold against a last store of v0.
-      asm volatile("s_nop 0");
-      return;
+  if constexpr (SPLIT) {
+    const long rows = (long)B * Hq * S;
+    if constexpr (!DQ) {
+      lt = l + __shfl_xor(l, 32, 64);
+      const float ltr = lr + __shfl_xor(lr, 32, 64);
+      if (qvalid && hf == 0)
+        *reinterpret_cast<f32x4*>(part + ns * rows * DH + 4 * (split * rows + qrow + qi)) = f32x4{FIXED ? fixed_top() : m, lt, ltr, 0.f};
+      mul = 1.f;
     }
+    if (qvalid) {
+      float* ph = part + (split * rows + qrow + qi) * DH;
+#pragma unroll
+      for (int db = 0; db < kDB; ++db)
+#pragma unroll
+        for (int rq = 0; rq < 4; ++rq)
+          *reinterpret_cast<f32x4*>(ph + 32 * db + 8 * rq + 4 * hf) =
+              f32x4{acc[db][4 * rq] * mul, acc[db][4 * rq + 1] * mul, acc[db][4 * rq + 2] * mul, acc[db][4 * rq + 3] * mul};
+    }
+    // The padding behind a program's end reads as a write of v0, which the listing check of stores whose data the next
+    // instructions write would hold against a last store of v0.
+    asm volatile("s_nop 0");
+    return;
   }
   if constexpr (!DQ) {
     lt = l + __shfl_xor(l, 32, 64);

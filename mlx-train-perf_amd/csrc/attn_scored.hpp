@@ -46,8 +46,8 @@ hipError_t scored_fwd<MTP_SCORED_DH>(const AttnShape& sh, const AttnScore& sc, c
   constexpr int DH = MTP_SCORED_DH;
   return with_mod(sc, [&](auto m) {
     constexpr int MOD = decltype(m)::value;
-    auto launch = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3(grid * nsplit), dim3(256), 0, st, q, k, v, nullptr, nullptr, nullptr, nullptr, sc.end,
+    auto launch = [&](auto whole, auto split) {
+      hipLaunchKernelGGL(nsplit > 1 ? split : whole, dim3(grid * nsplit), dim3(256), 0, st, q, k, v, nullptr, nullptr, nullptr, nullptr, sc.end,
                          sc.start, o, lse, sh.b, sh.hq, sh.hkv, sh.s, sh.scale * kLog2e, sh.scale, sh.causal, order,
                          sc.cap, sc.slopes, o_low, nullptr, nullptr, nsplit, part);
       return hipGetLastError();
@@ -58,12 +58,12 @@ hipError_t scored_fwd<MTP_SCORED_DH>(const AttnShape& sh, const AttnScore& sc, c
     const bool fixed = sc.cap <= kFixedCap;
     if (sc.start) {
       if constexpr (MOD == kModCap)
-        if (fixed) return launch(attn_kv_kernel<DH, kMaskSpan, false, MOD, true>);
-      return launch(attn_kv_kernel<DH, kMaskSpan, false, RUN>);
+        if (fixed) return launch(attn_kv_kernel<DH, kMaskSpan, false, MOD, true>, attn_kv_kernel<DH, kMaskSpan, false, MOD, true, true>);
+      return launch(attn_kv_kernel<DH, kMaskSpan, false, RUN>, attn_kv_kernel<DH, kMaskSpan, false, RUN, false, true>);
     }
     if constexpr (MOD & kModCap)
-      if (fixed) return launch(attn_kv_kernel<DH, kMaskPlain, false, MOD, true>);
-    if constexpr (MOD != kModNone) return launch(attn_kv_kernel<DH, kMaskPlain, false, RUN>);
+      if (fixed) return launch(attn_kv_kernel<DH, kMaskPlain, false, MOD, true>, attn_kv_kernel<DH, kMaskPlain, false, MOD, true, true>);
+    if constexpr (MOD != kModNone) return launch(attn_kv_kernel<DH, kMaskPlain, false, RUN>, attn_kv_kernel<DH, kMaskPlain, false, RUN, false, true>);
     return hipErrorInvalidValue;
   });
 }
@@ -76,8 +76,8 @@ hipError_t scored_bwd<MTP_SCORED_DH>(const AttnShape& sh, const AttnScore& sc, c
   constexpr int DH = MTP_SCORED_DH;
   return with_mod(sc, [&](auto m) {
     constexpr int MOD = decltype(m)::value;
-    auto launch = [&](auto dq_kernel, auto dkv_kernel) {
-      hipLaunchKernelGGL(dq_kernel, dim3(grid * ws.nq), dim3(256), 0, st, q, k, v, d_o, o, lse, ws.dvec, sc.end, sc.start, dq,
+    auto launch = [&](auto whole, auto split, auto dkv_kernel) {
+      hipLaunchKernelGGL(ws.nq > 1 ? split : whole, dim3(grid * ws.nq), dim3(256), 0, st, q, k, v, d_o, o, lse, ws.dvec, sc.end, sc.start, dq,
                          nullptr, sh.b, sh.hq, sh.hkv, sh.s, sh.scale * kLog2e, sh.scale, sh.causal, ws.q_order, sc.cap,
                          sc.slopes, const_cast<int8_t*>(o_low), ws.q_order ? nullptr : ws.col_begin,
                          ws.q_order ? nullptr : ws.col_end, ws.nq, ws.part);
@@ -90,9 +90,11 @@ hipError_t scored_bwd<MTP_SCORED_DH>(const AttnShape& sh, const AttnScore& sc, c
                          sh.causal, ws.nsplit, ws.part, ws.kv_order, ws.col_begin, sc.cap, sc.slopes);
       return hipGetLastError();
     };
-    if (sc.start) return launch(attn_kv_kernel<DH, kMaskSpan, true, MOD>, attn_bwd_dkv_ab_kernel<DH, kMaskSpan, MOD>);
+    if (sc.start) return launch(attn_kv_kernel<DH, kMaskSpan, true, MOD>, attn_kv_kernel<DH, kMaskSpan, true, MOD, false, true>,
+                    attn_bwd_dkv_ab_kernel<DH, kMaskSpan, MOD>);
     if constexpr (MOD != kModNone)
-      return launch(attn_kv_kernel<DH, kMaskPlain, true, MOD>, attn_bwd_dkv_ab_kernel<DH, kMaskPlain, MOD>);
+      return launch(attn_kv_kernel<DH, kMaskPlain, true, MOD>, attn_kv_kernel<DH, kMaskPlain, true, MOD, false, true>,
+                    attn_bwd_dkv_ab_kernel<DH, kMaskPlain, MOD>);
     return hipErrorInvalidValue;
   });
 }
