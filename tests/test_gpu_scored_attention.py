@@ -472,3 +472,36 @@ def test_passes_split_over_the_keys(b, hq, hkv, s, dh, mask, cap, biased):
     seen = torch.isfinite(lse1)
     assert torch.equal(seen, torch.isfinite(lse)) and torch.allclose(lse[seen], lse1[seen], rtol=2e-6, atol=2e-5)
     assert S.rel(fine(o, low), fine(o1, low1)) <= 2 ** -8   # another maximum rounds the probabilities elsewhere
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_captured_split_step_beside_another_stream(dtype):
+    """A captured step whose passes are split, replayed while an eager step of other tensors runs on a stream of its own:
+    each has its workspaces."""
+    from mlx_train_perf.attention import flash_attention
+
+    b, hq, hkv, s, dh = 1, 4, 2, 900, 64
+    made = [[t.cuda() for t in S.inputs(b, hq, hkv, s, dh, dtype, seed)] for seed in (1, 2)]
+    slopes = S.slopes_of(hq).cuda()
+
+    def step(x, cap):
+        qs = [t.detach().requires_grad_(True) for t in x[:3]]
+        o = flash_attention(*qs, scale=0.125, softcap=cap, slopes=slopes)
+        return [o.detach(), *torch.autograd.grad(o, qs, x[3])]
+
+    want = [step(made[0], 20.0), step(made[1], None)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(made[0], 20.0)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step(made[0], 20.0)
+    for _ in range(3):
+        side.wait_stream(torch.cuda.current_stream())
+        g.replay()
+        with torch.cuda.stream(side):
+            eager = step(made[1], None)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, w) for a, w in zip(out, want[0])) and all(torch.equal(a, w) for a, w in zip(eager, want[1]))
