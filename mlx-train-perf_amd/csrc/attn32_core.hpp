@@ -191,6 +191,9 @@ template <int MOD>
 __device__ __forceinline__ Score32<MOD> make_score32(float scale, float cap) {
   return Score32<MOD>{scale * kLog2e, (MOD & kModCap) ? scale / cap : 0.f, cap * kLog2e, 0.f};
 }
+// 2^y of a probability formed again from L: at most 1, where the rounding of y, a difference of two numbers of the scores'
+// size, may be far above 0 for scores past 2^29. NaN stays.
+__device__ __forceinline__ float prob32(float y) { return fast_exp2(__builtin_elementwise_minimum(y, 0.f)); }
 // Sum and maximum over the four lanes (g = 0..3) of a column.
 __device__ __forceinline__ float col_sum(float x) {
   x += __shfl_xor(x, 16, 64);
@@ -325,10 +328,11 @@ void attn32_q_kernel(const float* __restrict__ q, const float* __restrict__ k, c
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             if constexpr (MOD == kModNone) {
-              sc[half][r] = fast_exp2(__builtin_fmaf(sc[half][r], scale_log2, -l2q));
+              const float y = __builtin_fmaf(sc[half][r], scale_log2, -l2q);
+              sc[half][r] = SPAN ? prob32(y) : fast_exp2(y);
             } else {
               const float v = score.raw(sc[half][r]);
-              sc[half][r] = fast_exp2(score.of(v, rel - (float)(16 * half + r)) - l2q);
+              sc[half][r] = prob32(score.of(v, rel - (float)(16 * half + r)) - l2q);
               if constexpr (CAP) {  // P (1 - tanh^2): dP, D and the mask come after
                 sc[half][r] *= 1.f - v * v;
               }
@@ -524,11 +528,12 @@ void attn32_dkv_kernel(const float* __restrict__ q, const float* __restrict__ k,
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           if constexpr (MOD == kModNone) {
-            p[half][r] = fast_exp2(__builtin_fmaf(p[half][r], scale_log2, -l4[r] * kLog2e));
+            const float y = __builtin_fmaf(p[half][r], scale_log2, -l4[r] * kLog2e);
+            p[half][r] = SPAN ? prob32(y) : fast_exp2(y);
           } else {
             const float v = score.raw(p[half][r]);
             if constexpr (CAP) bend[half][r] = 1.f - v * v;
-            p[half][r] = fast_exp2(score.of(v, rel - (float)(16 * half + r)) - l4[r] * kLog2e);
+            p[half][r] = prob32(score.of(v, rel - (float)(16 * half + r)) - l4[r] * kLog2e);
           }
         }
       }

@@ -605,6 +605,10 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
               // (8192 positions, 32/8 heads, head_dim 128, cap 50: 1177 against 1190 us).
               float y = __builtin_fmaf(a1[h][r], score.mul, (MOD & kModSlope) ? __builtin_fmaf(-kLog2e, l4[u], add) : l4[u]);
               if constexpr (kMixed) y = __builtin_fmaf(-score.slope2, __builtin_fabsf(rel - (float)(32 * h + 8 * rq + u)), y);
+              // P is at most 1, but y is the difference of two numbers of the scores' size: from 2^22 on its rounding alone is
+              // 1, and 2^16 is past fp16; from 2^29 on 2^y may leave fp32. (A cap keeps scores below 2^11. NaN stays. 4 x 16 heads, 2048
+              // positions, head_dim 64, slopes: 111 us instead of 108.)
+              if constexpr (MOD != kModCap) y = __builtin_elementwise_minimum(y, kUp);
               const float p = fast_exp2(y);
               pown[h][r >> 3][r & 7] = (__bf16)p;
               pf[h][r >> 3][r & 7] = (_Float16)(CAP ? p * Score<MOD>::bend(a1[h][r]) : p);
@@ -1148,7 +1152,9 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
           float y = MOD == kModNone ? __builtin_fmaf(sacc[kb][r], scale_log2, -l2q) : __builtin_fmaf(sacc[kb][r], score.mul, add);
           if constexpr (kMixed)
             y = __builtin_fmaf(-score.slope2, __builtin_fabsf(rel - (float)(32 * kb + 8 * (r >> 2) + (r & 3))), y);
-          const float ds = fast_exp2(y) * (pacc[kb][r] - dq_row);
+          // (P <= 1, see the dK/dV pass; a clamp costs nothing, and the NaN that it drops is in D)
+          const float p = SCORED && MOD != kModCap ? __builtin_amdgcn_fmed3f(fast_exp2(y), 0.f, 1.f) : fast_exp2(y);
+          const float ds = p * (pacc[kb][r] - dq_row);
           pf[2 * kb + (r >> 3)][r & 7] = (__bf16)(CAP ? ds * Score<MOD>::bend(sacc[kb][r]) : ds);
         }
       // dQ^T += K^T dS^T: contraction over the 64 keys in 16-key slabs.
