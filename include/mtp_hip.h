@@ -291,6 +291,8 @@ int mtp_attn_bwd_f32(const float* q, const float* k, const float* v, const float
  *     span_start[i] <= j < span_end[i]; neither may decrease along a row, and a query whose span holds nothing
  *     gets o = 0, lse = +inf and no gradient. Spans are the whole mask (causal must be 0). Values outside the
  *     row are clamped into it; spans that decrease give some wrong rows, never an access out of range.
+ * A row's biases count from the highest of the keys that it sees (the nearest key's, with a slope below 0 the farthest's), and
+ * lse with them: the logarithm of the scores' sum of exponentials, less that bias.
  * scale must be positive, softcap 0 or in [1e-3, 1e3], slopes of either sign. At least one of the three must be
  * given (else: mtp_attn_fwd). What the mask hides must be finite all the same, padding too: v, and in the backward q, k and d_o.
  * o_low: int8 [b][hq][s][dh], the 8 bits of the output below its bf16 ones (bits of x = bits of bf16(x) + 2^8 o_low), for
@@ -308,9 +310,9 @@ int mtp_attn_scored_fwd(const void* q, const void* k, const void* v, int64_t b, 
                         int8_t* o_low, int32_t* plan, float* lse, void* workspace, size_t workspace_bytes,
                         void* stream);
 
-/* Workspace bytes of mtp_attn_scored_bwd, each part padded to 256 bytes: D and a logarithm (fp32 [2][b][hq][s]), the fp32 dK/dV
- * partials where the dK/dV pass is split, and for spans the int32 work orders of the two
- * passes and the int32 range of queries that see each key (2 x [b][s]). */
+/* Workspace bytes of mtp_attn_scored_bwd, each part padded to 256 bytes: D, a logarithm and the highest bias' distance (fp32
+ * [3][b][hq][s]), the fp32 parts of a split dQ, then dK/dV pass, and for spans the int32 work orders of the two passes and
+ * the int32 range of queries that see each key (2 x [b][s]). */
 size_t mtp_attn_scored_bwd_workspace_bytes(int64_t b, int64_t hq, int64_t hkv, int64_t s, int64_t dh);
 
 int mtp_attn_scored_bwd(const void* q, const void* k, const void* v, const void* o, const int8_t* o_low,

@@ -176,15 +176,16 @@ struct ALane {
     }
   }
 };
-// Scores in the log2 domain: raw(s) is tanh(x / cap) with a cap, else scale2 s; of(v, d) the score at distance d.
+// Scores in the log2 domain: raw(s) is tanh(x / cap) with a cap, else scale2 s; of(v, d, top) the score at distance |d|, its
+// bias counted from the highest of the row, that of the key at distance top (top_distance, as in the bf16 kernels).
 template <int MOD>
 struct Score32 {
   static constexpr bool kCap = MOD & kModCap;
   float scale2, in, cap2, slope2;
   __device__ __forceinline__ float raw(float s) const { return kCap ? tanhf(s * in) : s * scale2; }
-  __device__ __forceinline__ float of(float v, float d) const {
+  __device__ __forceinline__ float of(float v, float d, float top) const {
     const float y = kCap ? v * cap2 : v;
-    return (MOD & kModSlope) ? __builtin_fmaf(-slope2, __builtin_fabsf(d), y) : y;
+    return (MOD & kModSlope) ? __builtin_fmaf(-slope2, __builtin_fabsf(d) - top, y) : y;
   }
 };
 template <int MOD>
@@ -318,7 +319,14 @@ void attn32_q_kernel(const float* __restrict__ q, const float* __restrict__ k, c
                              (SPAN && kv0 + kPos > w_end_first);
       const int hi = (SPAN ? my_end - 1 : causal ? (qi < S - 1 ? qi : S - 1) : S - 1) - kv0 - 4 * ln.g;
       const int lo = my_sst - kv0 - 4 * ln.g;
-      const float rel = (float)(qi - kv0 - 4 * ln.g);
+      float rel = 0.f, top = 0.f;
+      if constexpr (MOD & kModSlope) {
+        int lane = threadIdx.x;
+        asm volatile("" : "+v"(lane));  // formed in each tile: the registers are full
+        const int i = qw0 + (lane & 15);
+        rel = (float)(i - kv0 - 4 * ((lane >> 4) & 3));
+        top = top_distance(score.slope2, i, SPAN ? in_row(my_sst) : 0, SPAN ? my_end : causal ? i + 1 : S);
+      }
       auto visible = [&](int half, int r) { return 16 * half + r <= hi && (!PACKED || 16 * half + r >= lo); };
       if constexpr (DQ) {
         f32x4 dp[2];
@@ -332,7 +340,7 @@ void attn32_q_kernel(const float* __restrict__ q, const float* __restrict__ k, c
               sc[half][r] = SPAN ? prob32(y) : fast_exp2(y);
             } else {
               const float v = score.raw(sc[half][r]);
-              sc[half][r] = prob32(score.of(v, rel - (float)(16 * half + r)) - l2q);
+              sc[half][r] = prob32(score.of(v, rel - (float)(16 * half + r), top) - l2q);
               if constexpr (CAP) {  // P (1 - tanh^2): dP, D and the mask come after
                 sc[half][r] *= 1.f - v * v;
               }
@@ -356,7 +364,7 @@ void attn32_q_kernel(const float* __restrict__ q, const float* __restrict__ k, c
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             if constexpr (MOD == kModNone) sc[half][r] *= scale_log2;
-            else sc[half][r] = score.of(score.raw(sc[half][r]), rel - (float)(16 * half + r));
+            else sc[half][r] = score.of(score.raw(sc[half][r]), rel - (float)(16 * half + r), top);
           }
         if (need_mask) {
 #pragma unroll
@@ -443,6 +451,8 @@ void attn32_dkv_kernel(const float* __restrict__ q, const float* __restrict__ k,
   const long krow = (long)bh * S;
   const float scale_log2 = scale * kLog2e;
   const int32_t* sst = PACKED ? seg_start + (long)b * S : nullptr;
+  const int32_t* send = SPAN ? span_end + (long)b * S : nullptr;
+  auto in_row = [&](int x) { return x < 0 ? 0 : x < S ? x : S; };
 
   f32x4 kx[L::kC], vx[L::kC];
   ln.load_row(k + (krow + kj) * DH, kvalid, kx);
@@ -464,12 +474,11 @@ void attn32_dkv_kernel(const float* __restrict__ q, const float* __restrict__ k,
     return lo;
   };
   if (SPAN) {
-    const int32_t* snd = span_end + (long)b * S;
-    t0 = __builtin_amdgcn_readfirstlane(first_over(snd, 0, ba * 64)) / kPos;
+    t0 = __builtin_amdgcn_readfirstlane(first_over(send, 0, ba * 64)) / kPos;
     if (wave_has) {
-      my_beg = kvalid ? first_over(snd, 0, kj) : S;
+      my_beg = kvalid ? first_over(send, 0, kj) : S;
       w_beg = __builtin_amdgcn_readfirstlane(my_beg);
-      w_beg_last = __builtin_amdgcn_readfirstlane(first_over(snd, 0, kw0 + 15 < S ? kw0 + 15 : S - 1));
+      w_beg_last = __builtin_amdgcn_readfirstlane(first_over(send, 0, kw0 + 15 < S ? kw0 + 15 : S - 1));
     }
   }
   if (PACKED) {
@@ -513,13 +522,24 @@ void attn32_dkv_kernel(const float* __restrict__ q, const float* __restrict__ k,
     copy(next, nxt);
     const int q0 = x.t * kPos;
     if (wave_has && !(causal && q0 + kPos - 1 < kw0) && !(PACKED && q0 >= w_end) && !(SPAN && q0 + kPos - 1 < w_beg)) {
+      if ((MOD & kModSlope) && slopes) score.slope2 = slopes[kvh * G + x.h] * kLog2e;
+      // The tops of the tile's queries: each formed in a lane, ahead of the products. Without spans 0 for slopes from 0 on.
+      f32x4 top[2] = {};
+      if constexpr (MOD & kModSlope)
+        if (SPAN || score.slope2 < 0.f) {
+          const int qi = q0 + (int)(threadIdx.x & 31), at = qi < S ? qi : S - 1;
+          const float mine = top_distance(score.slope2, qi, SPAN ? in_row(sst[at]) : 0, SPAN ? in_row(send[at]) : causal ? qi + 1 : S);
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) top[half][r] = __shfl(mine, 16 * half + 4 * ln.g + r, 64);
+        }
       f32x4 p[2], ds[2];
       ln.dot_rows(cur, kx, p);              // S = Q K^T (queries x this lane's key)
       ln.dot_rows(cur + L::kTile, vx, ds);  // dP = dO V^T
       const float* sl = reinterpret_cast<const float*>(cur + 2 * L::kTile);
       const bool need_mask = (causal && q0 < kw0 + 15) || q0 + kPos > S || (PACKED && q0 + kPos > w_lim) || (SPAN && q0 < w_beg_last);
       const int lo = SPAN ? my_beg - q0 - 4 * ln.g : causal ? kj - q0 - 4 * ln.g : -kPos, hi = my_lim - q0 - 4 * ln.g;
-      if ((MOD & kModSlope) && slopes) score.slope2 = slopes[kvh * G + x.h] * kLog2e;
       const float rel = (float)(kj - q0 - 4 * ln.g);
       f32x4 bend[2];
 #pragma unroll
@@ -533,7 +553,7 @@ void attn32_dkv_kernel(const float* __restrict__ q, const float* __restrict__ k,
           } else {
             const float v = score.raw(p[half][r]);
             if constexpr (CAP) bend[half][r] = 1.f - v * v;
-            p[half][r] = prob32(score.of(v, rel - (float)(16 * half + r)) - l4[r] * kLog2e);
+            p[half][r] = prob32(score.of(v, rel - (float)(16 * half + r), top[half][r]) - l4[r] * kLog2e);
           }
         }
       }

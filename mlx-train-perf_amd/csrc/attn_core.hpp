@@ -55,6 +55,10 @@ constexpr float kRescaleLog2 = 8.f;
 //   slant: v -= slope2 / mul |rel - c| for the element at distance |rel - c|, c a constant and rel the lane's and tile's.
 //     Where all of a wave's tile lies on one side of its positions that is a term in c, the rest (rel) in add: one
 //     multiply-add, or none where the product began from the term (ramp, a cap aside) instead of from 0.
+//   A row's biases, and with them its L, count from the highest of them, that of the key at distance top (top_distance):
+//     -slope2 (|rel - c| - top), the difference a whole number. Where the slope is below 0, or spans hide the keys nearby, a
+//     bias of slope2 |rel - c| has no digits left for what tells the row's keys apart (slope -4, distances of 60000: P off by
+//     1%; slope -300: by a factor).
 //   bend(v): -v - v^2 = (1 - tanh^2) / 4, the cap's derivative, negated and without its 4, which the gradients' last
 //     multiplier has (-4 scale).
 // A hidden pair has v = hidden<BWD>(): its score is -inf or so low that its probability is 0; in the backward it stays
@@ -64,23 +68,28 @@ struct Score {
   static constexpr bool kCap = MOD & kModCap, kSlope = MOD & kModSlope;
   float in2, mul, add, slope2, ratio;
   __device__ __forceinline__ Score(float scale_log2, float cap)
-      : in2(kCap ? 2.f * scale_log2 / cap : 0.f), mul(kCap ? 2.f * cap * kLog2e : scale_log2), add(kCap ? cap * kLog2e : 0.f),
+      : in2(kCap ? scalar(2.f * scale_log2 / cap) : 0.f), mul(kCap ? scalar(2.f * cap * kLog2e) : scale_log2), add(kCap ? scalar(cap * kLog2e) : 0.f),
         slope2(0.f), ratio(0.f) {}
+  // (the same in every lane: kept in scalar registers, as the vector ones are full)
   __device__ __forceinline__ void set_slope(float slope) {
-    slope2 = slope * kLog2e;
-    ratio = slope2 / mul;
+    slope2 = scalar(slope * kLog2e);
+    ratio = scalar(slope2 / mul);
+  }
+  static __device__ __forceinline__ float scalar(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
   }
   template <bool BWD>
   static __device__ __forceinline__ float hidden() { return BWD && kCap ? -1e15f : -__builtin_huge_valf(); }
   __device__ __forceinline__ float raw(float s) const { return kCap ? __builtin_amdgcn_rcpf(-1.f - fast_exp2(s * in2)) : s; }
   static __device__ __forceinline__ constexpr float at(int half, int r) { return (float)(32 * half + 8 * (r >> 2) + (r & 3)); }
-  // SIGN ratio c: what a product begins from.
+  // SIGN ratio c: what a product begins from (`none`: 0).
   template <int SIGN>
-  __device__ __forceinline__ void set_ramp(f32x16 (&ramp)[2]) const {
+  __device__ __forceinline__ void set_ramp(f32x16 (&ramp)[2], bool none = false) const {
+    const float step = none ? 0.f : SIGN * ratio;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) ramp[h][r] = SIGN * ratio * at(h, r);
+      for (int r = 0; r < 16; ++r) ramp[h][r] = step * at(h, r);
   }
   // side: 1 where rel >= c for every pair of the wave's tile that is not hidden, -1 where rel <= c, 0 where neither; SIGN
   // the usual one, whose term (a ramp's) a tile of neither keeps and corrects.
@@ -101,10 +110,25 @@ struct Score {
       for (int r = 0; r < 16; ++r) v[r] = __builtin_fmaf(2.f * ratio, fminf(SIGN * (rel - at(half, r)), 0.f), v[r]);
     }
   }
+  // The same for keys in lanes, k times c and, where keys lie on both sides, the correction.
+  __device__ __forceinline__ void lean(f32x16 (&v)[2], float k, bool both, float rel) const {
+    if (k != 0.f) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) v[h][r] = __builtin_fmaf(k * ratio, at(h, r), v[h][r]);
+    }
+    if (both) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) v[h][r] = __builtin_fmaf(2.f * ratio, fminf(at(h, r) - rel, 0.f), v[h][r]);
+    }
+  }
   // add of a slanted tile.
   template <int SIGN>
-  __device__ __forceinline__ float slant_add(int side, float rel) const {
-    return add - (side == -SIGN ? -SIGN : SIGN) * slope2 * rel;
+  __device__ __forceinline__ float slant_add(int side, float rel, float top) const {
+    return __builtin_fmaf(-slope2, (side == -SIGN ? -SIGN : SIGN) * rel - top, add);
   }
   static __device__ __forceinline__ float bend(float v) { return __builtin_fmaf(v, v, v); }
 };
@@ -321,9 +345,9 @@ __device__ __forceinline__ void sched_sort(int n, Cost cost, int32_t* order) {
 // statically.
 // ------------------------------------------------------------------------------------------
 namespace dkvab {
-constexpr int kScal = 2 * 256;                  // L and D of the 64 queries
-template <int DH>
-constexpr int kStage = 2 * kvdma::Lay<DH>::kTile + kScal;  // Q, dO, L log2 e, D
+// Q, dO, and of the 64 queries L, D and, with slopes, the top (Score).
+template <int DH, int MOD>
+constexpr int kStage = 2 * kvdma::Lay<DH>::kTile + ((MOD & kModSlope) ? 3 : 2) * 256;
 constexpr int kPBytes = kKT * 32 * 2;           // P of one key group (64 queries x 32 keys, bf16)
 constexpr int kPBuf = 4 * kPBytes;              // P of the workgroup's four key groups
 }  // namespace dkvab
@@ -344,9 +368,9 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
   constexpr int kRowB = L::kRowB, kTile = L::kTile;
   auto sw = [](int r) { return L::sw(r); };
   constexpr int kDK = DH / 16, kDB = DH / 32;
-  __shared__ __attribute__((aligned(1024))) char st0[dkvab::kStage<DH>];
-  __shared__ __attribute__((aligned(1024))) char st1[dkvab::kStage<DH>];
-  __shared__ __attribute__((aligned(1024))) char st2[dkvab::kStage<DH>];
+  __shared__ __attribute__((aligned(1024))) char st0[dkvab::kStage<DH, MOD>];
+  __shared__ __attribute__((aligned(1024))) char st1[dkvab::kStage<DH, MOD>];
+  __shared__ __attribute__((aligned(1024))) char st2[dkvab::kStage<DH, MOD>];
   __shared__ __attribute__((aligned(1024))) char pb0[dkvab::kPBuf];
   __shared__ __attribute__((aligned(1024))) char pb1[dkvab::kPBuf];
   __shared__ __attribute__((aligned(1024))) char pb2[dkvab::kPBuf];
@@ -457,9 +481,10 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
       tro[t][db] = rl * kRowB + ((c ^ swt) << 4) + 8 * (lane & 1);
     }
   }
-  // With a cap (or slopes' ramp at head_dim 96) P's two copies leave no room for these 16 offsets: each is then formed at
-  // its use from the first of its kind (2 ks touches chunk bits 1-3, 4 db bits 2-3, of an XOR-swizzled chunk index).
-  constexpr bool kForm = CAP || (MOD == kModSlope && DH == 96);
+  // With a cap (or slopes' ramp at head_dim 96, slopes and spans at 128) P's two copies leave no room for these 16 offsets:
+  // each is then formed at its use from the first of its kind (2 ks touches chunk bits 1-3, 4 db bits 2-3, of an
+  // XOR-swizzled chunk index).
+  constexpr bool kForm = CAP || (MOD == kModSlope && (DH == 96 || (SPAN && DH == 128)));
   auto row_off = [&](int base, int ks) __attribute__((always_inline)) { return kForm ? base ^ (ks << 5) : ro[ks]; };
   auto tr_off = [&](int base, int t, int db) __attribute__((always_inline)) { return kForm ? base ^ (db << 6) : tro[t][db]; };
   // The P wave reads Q rows and dO^T; the dS wave dO rows and Q^T.
@@ -470,7 +495,8 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
   // Copies of tile `it` into stage `st`: this wave's load j (0-1 Q rows, 2-3 dO rows); zero bytes,
   // no memory access (zeros into a free stage), when not `live`.
   // The per-query scalars L and D of the tile's 64 queries go beside it (waves 0 and 4, one 4-byte
-  // load each).
+  // load each), and with slopes, where they are read, the dQ pass' tops (wave 1).
+  constexpr bool SLOPE = MOD & kModSlope, TOPS = SLOPE && (SPAN || CAP);
   struct CopySrc {
     const bf16_t* qs;
     const bf16_t* ds;
@@ -483,7 +509,7 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
     const long qrow = (long)(bidx * Hq + kvh * G + hh) * S;
     const int q0 = q_begin + tq * kKT;
     const int rows = live ? ((S - q0 < kKT) ? S - q0 : kKT) : 0;
-    return CopySrc{q + (qrow + q0) * DH, d_o + (qrow + q0) * DH, (w < 4 ? lse : dvec) + qrow + q0, rows * 2 * DH, rows * 4};
+    return CopySrc{q + (qrow + q0) * DH, d_o + (qrow + q0) * DH, (TOPS && w == 1 ? dvec + 2L * B * Hq * S : w < 4 ? lse : dvec) + qrow + q0, rows * 2 * DH, rows * 4};
   };
   // The P waves copy for their dS partners too (the dS waves are the longer role): load j of a P wave
   // covers Q (j < 2 kM) or dO rows, piece 8 m + w (m = j % kM) or that of wave w + 4 (j / kM odd),
@@ -495,13 +521,15 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
                coff[m] + (part ? (uint32_t)(4 * kRpp * 2 * DH) : 0u));
   };
   auto issue_scal = [&](const CopySrc& c, char* st) __attribute__((always_inline)) {
-    if (grp == 0) lds_copy4(c.scal, c.sbytes, st + 2 * kTile + (pwave ? 0 : 256), (uint32_t)(4 * lane));
+    if (grp == 0 || (TOPS && w == 1))
+      lds_copy4(c.scal, c.sbytes, st + 2 * kTile + (TOPS && w == 1 ? 512 : pwave ? 0 : 256), (uint32_t)(4 * lane));
   };
 
   // Start of tile `it` (stage `st`): the first product of both halves into a1; the P wave then
   // forms P (hidden pairs 0) and writes it to `pb`.
   f32x16 a1[2];
-  // With slopes alone the P wave's products begin from the bias' ramp of the head at hand, where it fits the registers.
+  // With slopes alone the P wave's products begin from the bias' ramp of the head at hand, where it fits the registers, and
+  // with spans, where tops are not all 0, from the biases themselves, formed one by one.
   constexpr bool kRamp = MOD == kModSlope && DH <= 96;
   f32x16 ramp[2];
   int ramp_head = -1;
@@ -513,6 +541,8 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
   constexpr float kUp = HALF ? 15.f : 0.f, kDown = HALF ? 0x1p-15f : 1.f;
   bf16x8 pown[HALF ? 2 : 1][2];
   auto start = [&](int it, const char* st, char* pb, const CopySrc& cx, char* sx) __attribute__((always_inline)) {
+    const float* tops = reinterpret_cast<const float*>(st + 2 * kTile + 512);
+    bool far = false;  // slopes and spans: some query of the tile has its top at another distance than 0
     {
       // Row fragments read two k16 steps ahead of their products.
       bf16x8 rf[3][2];
@@ -522,30 +552,48 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
 #pragma unroll
         for (int h = 0; h < 2; ++h) rf[ks % 3][h] = as_bf16x8(lds_read16(st + row_src, 32 * h * kRowB + row_off(rbase, ks)));
       };
+      const float mine = SPAN && MOD == kModSlope && pwave ? tops[lane] : 0.f;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int r = 0; r < 16; ++r) a1[h][r] = 0.f;
-      if constexpr (kRamp) {
-        if (pwave) {
-          const int hh = (it0 + it) / ntq;
-          if (hh != ramp_head) {
-            ramp_head = hh;
-            score.set_slope(slopes ? slopes[kvh * G + hh] : 0.f);
-            score.template set_ramp<-1>(ramp);
-          }
-#pragma unroll
-          for (int h = 0; h < 2; ++h) a1[h] = ramp[h];
-        }
-      }
       issue_scal(cx, sx);
       rd(0);
       rd(1);
+      if constexpr (SLOPE) {
+        const int hh = (it0 + it) / ntq;
+        if (pwave && (!kRamp || hh != ramp_head)) {
+          ramp_head = hh;
+          score.set_slope(slopes ? slopes[kvh * G + hh] : 0.f);
+          if constexpr (kRamp) score.template set_ramp<-1>(ramp, !SPAN && score.slope2 < 0.f);
+        }
+        if constexpr (SPAN && MOD == kModSlope) far = pwave && __builtin_amdgcn_ballot_w64(mine != 0.f) != 0;
+      }
 #pragma unroll
       for (int ks = 0; ks < kDK; ++ks) {
         if (ks + 2 < kDK) rd(ks + 2);
+        // (the first products in branches of their own: one behind them would copy what they begin from)
+        auto product = [&](auto&& from) __attribute__((always_inline)) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) a1[h] = mfma32(rf[ks % 3][h], opf[ks], a1[h]);
+          for (int h = 0; h < 2; ++h) a1[h] = mfma32(rf[ks % 3][h], opf[ks], from(h));
+        };
+        if (SPAN && MOD == kModSlope && ks == 0 && far) {
+          const float rel = (float)(kj - (q_begin + ((it0 + it) % ntq) * kKT) - 4 * hf);
+          product([&](int h) {
+            f32x16 x;
+#pragma unroll
+            for (int rq = 0; rq < 4; ++rq) {
+              const f32x4 t4 = *reinterpret_cast<const f32x4*>(tops + 32 * h + 8 * rq + 4 * hf);
+#pragma unroll
+              for (int u = 0; u < 4; ++u) x[4 * rq + u] = -score.ratio * (__builtin_fabsf(rel - (float)(32 * h + 8 * rq + u)) - t4[u]);
+            }
+            return x;
+          });
+        } else if (kRamp && ks == 0 && pwave) {
+          product([&](int h) { return ramp[h]; });
+        } else {
+          product([&](int h) { return a1[h]; });
+        }
         // The copy loads of the tile after next, spread over the k16 steps of the P waves, between
         // products that wait: a copy load holds its wave at issue while the CU's load path serves
         // others.
@@ -566,17 +614,29 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
       constexpr bool kMixed = MOD == kModBoth;
       float add = score.add + kUp;
       const float rel = (float)(kj - q0 - 4 * hf);
-      if constexpr ((MOD & kModSlope) && !kRamp) score.set_slope(slopes ? slopes[kvh * G + (it0 + it) / ntq] : 0.f);
       if constexpr (MOD != kModNone) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int r = 0; r < 16; ++r) a1[h][r] = score.raw(a1[h][r]);
         if constexpr (MOD == kModSlope) {
-          const int side = (causal || q0 >= kw0 + 31) ? -1 : q0 + kKT - 1 <= kw0 ? 1 : 0;
-          score.template slant<-1, kRamp>(a1[0], 0, side, rel);
-          score.template slant<-1, kRamp>(a1[1], 1, side, rel);
-          add = score.template slant_add<-1>(side, rel) + kUp;
+          if (!far) {
+            // |i - j| - top, i the query: i - j or, on the other side, j - i. Without spans and for a slope below 0 top is i, or
+            // without the causal mask S - 1 - i where that is more (a tile's first half then has that correction: mid).
+            const int side = (causal || q0 >= kw0 + 31) ? -1 : q0 + kKT - 1 <= kw0 ? 1 : 0, i0 = q0 + 4 * hf;
+            const bool neg = !SPAN && score.slope2 < 0.f, back = !causal && 2 * (q0 + kKT - 1) <= S - 1;
+            const bool mid = neg && !back && !causal && 2 * q0 < S - 1;
+            const int k = (side == 1 ? 1 : -1) + (neg ? back ? -1 : 1 : kRamp ? 1 : 0);  // how often c is in -(|i - j| - top)
+            score.lean(a1, (float)k, side == 0, rel);
+            if (mid) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                  a1[h][r] = __builtin_fmaf(score.ratio, fmaxf((float)(S - 1 - 2 * i0) - 2.f * Score<MOD>::at(h, r), 0.f), a1[h][r]);
+            }
+            add = __builtin_fmaf(-score.slope2, (side == 1 ? rel : -rel) - (neg ? (float)(back ? S - 1 - i0 : i0) : 0.f), add);
+          }
         }
       }
       if (need_mask) {
@@ -595,20 +655,28 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
 #pragma unroll
         for (int rq = 0; rq < 4; ++rq) {
           const f32x4 l4 = *reinterpret_cast<const f32x4*>(ls + 32 * h + 8 * rq + 4 * hf);
+          f32x4 t4;
+          if constexpr (kMixed) {
+            if constexpr (DH == 128) __builtin_amdgcn_sched_barrier(0);  // (the reads of later ones would spill)
+            t4 = *reinterpret_cast<const f32x4*>(tops + 32 * h + 8 * rq + 4 * hf);
+          }
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             const int r = 4 * rq + u;
             if constexpr (!HALF) {
               pf[h][r >> 3][r & 7] = (__bf16)fast_exp2(__builtin_fmaf(a1[h][r], scale_log2, -l4[u] * kLog2e));
             } else {
-              // Without slopes what is added to a query's scores is one number, which the dQ pass left in the place of L
+              // What is added to a query's scores, but for slopes alone, is one number, which the dQ pass left in the place of L
               // (8192 positions, 32/8 heads, head_dim 128, cap 50: 1177 against 1190 us).
-              float y = __builtin_fmaf(a1[h][r], score.mul, (MOD & kModSlope) ? __builtin_fmaf(-kLog2e, l4[u], add) : l4[u]);
-              if constexpr (kMixed) y = __builtin_fmaf(-score.slope2, __builtin_fabsf(rel - (float)(32 * h + 8 * rq + u)), y);
+              float y = __builtin_fmaf(a1[h][r], score.mul, MOD == kModSlope ? __builtin_fmaf(-kLog2e, l4[u], add) : l4[u]);
+              if constexpr (kMixed) {
+                const float d = __builtin_fabsf(rel - (float)(32 * h + 8 * rq + u));
+                y = __builtin_fmaf(-score.slope2, d - t4[u], y);
+              }
               // P is at most 1, but y is the difference of two numbers of the scores' size: from 2^22 on its rounding alone is
-              // 1, and 2^16 is past fp16; from 2^29 on 2^y may leave fp32. (A cap keeps scores below 2^11. NaN stays. 4 x 16 heads, 2048
+              // 1, and 2^16 is past fp16; from 2^29 on 2^y may leave fp32. (A cap keeps scores below 2^12. NaN stays. 4 x 16 heads, 2048
               // positions, head_dim 64, slopes: 111 us instead of 108.)
-              if constexpr (MOD != kModCap) y = __builtin_elementwise_minimum(y, kUp);
+              if constexpr (!CAP) y = __builtin_elementwise_minimum(y, kUp);
               const float p = fast_exp2(y);
               pown[h][r >> 3][r & 7] = (__bf16)p;
               pf[h][r >> 3][r & 7] = (_Float16)(CAP ? p * Score<MOD>::bend(a1[h][r]) : p);
@@ -931,7 +999,11 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
     w_end_last = in_row(__builtin_amdgcn_readfirstlane(wave_has ? snd[wq_last] : 0));
   }
   Score<MOD> score(scale_log2, cap);
-  if constexpr (MOD & kModSlope) score.set_slope(slopes ? slopes[head] : 0.f);
+  float top = 0.f;
+  if constexpr (MOD & kModSlope) {
+    score.set_slope(slopes ? slopes[head] : 0.f);
+    top = top_distance(score.slope2, qi, SPAN ? in_row(my_sst) : 0, SPAN ? my_end : causal ? qi + 1 : S);
+  }
   // The side of its queries that a tile's keys lie on (Score::slant).
   auto side_of = [&](int kv0) { return (causal || kv0 + kKT - 1 <= qw0) ? 1 : kv0 >= qw0 + 31 ? -1 : 0; };
 
@@ -940,16 +1012,11 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
   f32x16 ramp[2];
   if constexpr (kRamp) score.template set_ramp<1>(ramp);
 
-  // Forward with a fixed maximum (FIXED): under a cap of at most kFixedCap no score exceeds the cap, and of every row
-  // that sees anything some score (with slopes, in the masks that show a query its own key, that key's) is at least its
-  // negative. So probabilities are formed against 0: at most 2^80, summed over a row and times a value below 2^24 still
-  // in fp32's range, and their sum is at least 2^-80. That saves the running maximum, its exchange and every rescale.
-  // A slope below 0 raises far keys: there the bias of a query's farthest key takes the place of 0.
+  // Forward with a fixed maximum (FIXED): under a cap of at most kFixedCap no score exceeds the cap, as biases count from
+  // the row's highest, and of every row that sees anything some score is at least its negative. So probabilities are
+  // formed against 0: at most 2^80, summed over a row and times a value below 2^24 still in fp32's range, and their sum is
+  // at least 2^-80. That saves the running maximum, its exchange and every rescale.
   static_assert(!FIXED || (!DQ && CAP));
-  auto fixed_top = [&]() {
-    return (MOD & kModSlope) ? fmaxf(-score.slope2, 0.f) * (float)(causal || qi > S - 1 - qi ? qi : S - 1 - qi) : 0.f;
-  };
-  if constexpr (FIXED) score.add -= fixed_top();
   float m = FIXED ? 0.f : kNegInf, l = 0.f;
   // Spans, caps and biases: O is divided by the sum of the bf16 probabilities that it was formed from, L is of the exact
   // sum. The probabilities' roundings then shift O, and D with it, only by what dP differs between keys, which is what dS is
@@ -1044,7 +1111,8 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
     dq_row = sum_xhalf(dp);
     if (qvalid && hf == 0 && split == 0) {
       dvec[qrow + qi] = dq_row;
-      if constexpr (SCORED && !(MOD & kModSlope)) dvec[(long)B * Hq * S + qrow + qi] = score.add + 15.f - l2q;  // (kUp there)
+      if constexpr (SCORED && MOD != kModSlope) dvec[(long)B * Hq * S + qrow + qi] = score.add + 15.f - l2q;  // (kUp there)
+      if constexpr ((MOD & kModSlope) && (SPAN || CAP)) dvec[2L * B * Hq * S + qrow + qi] = top;
     }
   }
 
@@ -1123,7 +1191,7 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
       };
       constexpr bool kMixed = MOD == kModBoth;  // bend needs v as raw left it: the bias comes after
       float add = score.add;
-      const float rel = (float)(qi - kv0 - 4 * hf);
+      float rel = (float)(qi - kv0 - 4 * hf), steep = -__builtin_fabsf(score.slope2);
       if constexpr (MOD != kModNone) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
@@ -1133,7 +1201,17 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
           const int side = side_of(kv0);
           score.template slant<1, kRamp>(sacc[0], 0, side, rel);
           score.template slant<1, kRamp>(sacc[1], 1, side, rel);
-          add = score.template slant_add<1>(side, rel);
+          add = score.template slant_add<1>(side, rel, top);
+        }
+        // Of a tile on one side of the queries all distances are one way from top: -slope2 (|d| - top) is -|slope2 (rel -+ top
+        // - c)|. A tile of both sides has only distances below 100, and takes top as a term of its own.
+        if constexpr (kMixed) {
+          const int side = side_of(kv0);
+          if (side == 0) {
+            add = __builtin_fmaf(score.slope2, top, add);
+            steep = -score.slope2;
+          }
+          rel -= (float)side * top;
         }
         add -= l2q;
       }
@@ -1151,9 +1229,9 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
         for (int r = 0; r < 16; ++r) {
           float y = MOD == kModNone ? __builtin_fmaf(sacc[kb][r], scale_log2, -l2q) : __builtin_fmaf(sacc[kb][r], score.mul, add);
           if constexpr (kMixed)
-            y = __builtin_fmaf(-score.slope2, __builtin_fabsf(rel - (float)(32 * kb + 8 * (r >> 2) + (r & 3))), y);
+            y = __builtin_fmaf(steep, __builtin_fabsf(rel - (float)(32 * kb + 8 * (r >> 2) + (r & 3))), y);
           // (P <= 1, see the dK/dV pass; a clamp costs nothing, and the NaN that it drops is in D)
-          const float p = SCORED && MOD != kModCap ? __builtin_amdgcn_fmed3f(fast_exp2(y), 0.f, 1.f) : fast_exp2(y);
+          const float p = SCORED && !CAP ? __builtin_amdgcn_fmed3f(fast_exp2(y), 0.f, 1.f) : fast_exp2(y);
           const float ds = p * (pacc[kb][r] - dq_row);
           pf[2 * kb + (r >> 3)][r & 7] = (__bf16)(CAP ? ds * Score<MOD>::bend(sacc[kb][r]) : ds);
         }
@@ -1256,7 +1334,7 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
         bf16x8 pf[4];
         const int side = (MOD & kModSlope) ? side_of(kv0) : 0;
         const float rel = (float)(qi - kv0 - 4 * hf);
-        const float add = (MOD & kModSlope) ? score.template slant_add<1>(side, rel) : score.add;
+        const float add = (MOD & kModSlope) ? score.template slant_add<1>(side, rel, top) : score.add;
         auto form = [&](f32x16& sc, int kb) {  // raw products into v (Score)
           if constexpr (MOD != kModNone) {
 #pragma unroll
@@ -1379,7 +1457,7 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
       lt = l + __shfl_xor(l, 32, 64);
       const float ltr = lr + __shfl_xor(lr, 32, 64);
       if (qvalid && hf == 0)
-        *reinterpret_cast<f32x4*>(part + ns * rows * DH + 4 * (split * rows + qrow + qi)) = f32x4{FIXED ? fixed_top() : m, lt, ltr, 0.f};
+        *reinterpret_cast<f32x4*>(part + ns * rows * DH + 4 * (split * rows + qrow + qi)) = f32x4{m, lt, ltr, 0.f};
       mul = 1.f;
     }
     if (qvalid) {
@@ -1403,7 +1481,7 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
   }
   if constexpr (!DQ) {
     // A query that sees nothing: L = +inf, so that the backward's probabilities exp(S - L) are 0.
-    if (qvalid && hf == 0) lse_out[qrow + qi] = (SPAN && !(lt > 0.f)) ? -kNegInf : ((FIXED ? fixed_top() : m) + fast_log2(lt)) * kLn2;
+    if (qvalid && hf == 0) lse_out[qrow + qi] = (SPAN && !(lt > 0.f)) ? -kNegInf : (m + fast_log2(lt)) * kLn2;
   }
   auto quad = [&](int db, int rq) __attribute__((always_inline)) {  // dims 32 db + 8 rq + 4 hf .. + 3
     return u32x2{pack_bf16x2(acc[db][4 * rq] * mul, acc[db][4 * rq + 1] * mul),

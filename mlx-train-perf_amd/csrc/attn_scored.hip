@@ -161,7 +161,7 @@ size_t carve(int b, int hq, int hkv, int s, int dh, char* base, ScoredWorkspace*
   const int ns1 = scored_nsplit(b, hq, hkv, s, dh, 1), ns0 = scored_nsplit(b, hq, hkv, s, dh, 0);
   const int ns = ns1 > ns0 ? ns1 : ns0;
   Carver c{base};
-  c.take(ws->dvec, (size_t)2 * b * hq * s);
+  c.take(ws->dvec, (size_t)3 * b * hq * s);
   const int nq = q_splits(b, hq, hkv, s, false);  // (spans: no more)
   const size_t kv_part = ns > 1 ? (size_t)ns * 2 * b * hkv * s * dh : 0, q_part = nq > 1 ? (size_t)nq * b * hq * s * dh : 0;
   c.take(ws->part, kv_part > q_part ? kv_part : q_part);

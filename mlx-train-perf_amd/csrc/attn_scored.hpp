@@ -5,9 +5,9 @@
 
 namespace mtp {
 
-// A backward call's workspace, in order: D, without slopes the logarithms in the P waves' form, the fp32 parts of a split
-// dQ, then dK/dV pass, and for spans the two work
-// orders (null: none) and the queries [col_begin, col_end) that see each key.
+// A backward call's workspace, in order: D, but for slopes alone the logarithms in the P waves' form, with slopes and a cap
+// or spans the tops of the rows' biases (Score), the fp32 parts of a split dQ, then dK/dV pass, and for spans the two work orders (null: none) and
+// the queries [col_begin, col_end) that see each key.
 struct ScoredWorkspace {
   float* dvec;
   float* part;
@@ -52,8 +52,7 @@ hipError_t scored_fwd<MTP_SCORED_DH>(const AttnShape& sh, const AttnScore& sc, c
                          sc.cap, sc.slopes, o_low, nullptr, nullptr, nsplit, part);
       return hipGetLastError();
     };
-    // A cap above kFixedCap runs as a cap with slopes of none; spans may hide a query's own key, whose bias of 0 the
-    // fixed maximum counts on.
+    // A cap above kFixedCap runs as a cap with slopes of none.
     constexpr int RUN = MOD == kModCap ? kModBoth : MOD;
     const bool fixed = sc.cap <= kFixedCap;
     if (sc.start) {
@@ -86,7 +85,7 @@ hipError_t scored_bwd<MTP_SCORED_DH>(const AttnShape& sh, const AttnScore& sc, c
       if (e != hipSuccess) return e;
       // (the parts of dQ are read: those of dK and dV take their place)
       hipLaunchKernelGGL(dkv_kernel, dim3((sh.s + 127) / 128 * sh.b * sh.hkv * ws.nsplit), dim3(512), 0, st, q, k, v, d_o,
-                         (MOD & kModSlope) ? lse : ws.dvec + (long)sh.b * sh.hq * sh.s, ws.dvec, ws.col_end, dk, dv, sh.b, sh.hq, sh.hkv, sh.s, sh.scale * kLog2e, sh.scale,
+                         MOD == kModSlope ? lse : ws.dvec + (long)sh.b * sh.hq * sh.s, ws.dvec, ws.col_end, dk, dv, sh.b, sh.hq, sh.hkv, sh.s, sh.scale * kLog2e, sh.scale,
                          sh.causal, ws.nsplit, ws.part, ws.kv_order, ws.col_begin, sc.cap, sc.slopes);
       return hipGetLastError();
     };

@@ -33,6 +33,14 @@ constexpr float kNegInf = -__builtin_huge_valf();
 enum { kMaskPlain = 0, kMaskPacked = 1, kMaskSpan = 2 };
 enum { kModNone = 0, kModCap = 1, kModSlope = 2, kModBoth = 3 };
 
+// The distance from query i to the key whose bias is its row's highest: of the keys [start, end) that it sees the nearest,
+// the farthest for a slope below 0 (none: 0).
+__device__ __forceinline__ float top_distance(float slope2, int i, int start, int end) {
+  const int first = i - start, last = end - 1 - i;  // how far before i the range begins, and behind it ends
+  const int nearest = first < 0 ? -first : last < 0 ? -last : 0, farthest = first > last ? first : last;
+  return end <= start ? 0.f : (float)(slope2 < 0.f ? farthest : nearest);
+}
+
 __device__ __forceinline__ f32x16 mfma32(const bf16x8& a, const bf16x8& b, const f32x16& c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
