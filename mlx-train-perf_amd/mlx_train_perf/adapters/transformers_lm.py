@@ -124,7 +124,7 @@ def make_token_nll_fn(model: Any, *, impl: _Impl = "auto",
 
     split_model(model)
     cfg = getattr(model, "config", None)
-    if getattr(cfg, "final_logit_softcapping", None) is not None:
+    if getattr(cfg, "final_logit_softcapping", None):   # (0, like None: no cap)
         raise AdapterError("the fused loss does not cap logits (config.final_logit_softcapping is set)")
 
     def nll_fn(model_arg: Any, batch: torch.Tensor, spans: SpanMask | None = None) -> torch.Tensor:

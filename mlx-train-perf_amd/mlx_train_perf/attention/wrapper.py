@@ -57,6 +57,11 @@ def _resolve_mask(mask: Any) -> bool | PackedMask | SpanMask:
     )
 
 
+def _cap(softcap: float | None) -> float | None:
+    """A layer's or configuration's cap; both None and 0 say that there is none."""
+    return softcap or None
+
+
 class _UnsupportedMask:
     """What `_hf_mask` hands to the layers for a mask pattern the causal kernels cannot honour; the
     attention call then refuses with `reason` instead of silently attending causally."""
@@ -97,7 +102,7 @@ def _hf_flash_attention(module: nn.Module, query: torch.Tensor, key: torch.Tenso
                         mtp_segments: PackedMask | None = None, mtp_spans: SpanMask | None = None,
                         softcap: float | None = None, **kwargs: Any):
     """transformers attention-interface function: q (B,Hq,S,D), k/v (B,Hkv,S,D) post-RoPE;
-    returns (output (B,S,Hq,D), None). `softcap`: what layers with capped scores pass."""
+    returns (output (B,S,Hq,D), None). `softcap`: what layers with capped scores pass (0 or None: none)."""
     if dropout:
         raise UnsupportedAttentionError("flash-attention training path does not support attention dropout")
     if attention_mask is not None:
@@ -108,7 +113,7 @@ def _hf_flash_attention(module: nn.Module, query: torch.Tensor, key: torch.Tenso
         raise AttentionInputError(f"the flash-attention path cannot honour this mask: {reason}")
     impl = getattr(module.config, "_mtp_flash_impl", "auto")
     out = flash_attention(query, key, value, scale=float(scaling), causal=True, impl=impl, segments=mtp_segments,
-                          softcap=softcap, spans=mtp_spans)
+                          softcap=_cap(softcap), spans=mtp_spans)
     return out.transpose(1, 2).contiguous(), None
 
 
@@ -153,7 +158,7 @@ class FlashAttentionWrapper(nn.Module):
         segments = resolved if isinstance(resolved, PackedMask) else None
         spans = resolved if isinstance(resolved, SpanMask) else None
         out = flash_attention(queries, keys, values, scale=self.scale, causal=True, segments=segments, spans=spans,
-                              softcap=self.softcap, impl=self._impl)  # type: ignore[arg-type]
+                              softcap=_cap(self.softcap), impl=self._impl)  # type: ignore[arg-type]
         return self.o_proj(out.transpose(1, 2).reshape(b, length, -1))
 
 
@@ -272,7 +277,7 @@ def enable_flash_attention(model: Any, *, impl: str = "auto", seq_len: int | Non
         head_dim = _head_dim(cfg)
         _plan.attn_plan(b=batch_size, hq=hq, hkv=hkv, s=seq_len, dh=head_dim)
         _prewarm(model, impl=impl, seq_len=seq_len, batch_size=batch_size, hq=hq, hkv=hkv, head_dim=head_dim,
-                 packed=packed, softcap=getattr(cfg, "attn_logit_softcapping", None))
+                 packed=packed, softcap=_cap(getattr(cfg, "attn_logit_softcapping", None)))
 
 
 def is_enabled(model: Any) -> bool:
