@@ -20,8 +20,8 @@
 // ragged batch the whole time), and has all its loads in flight at once: eight tokens a lane. For every sequence r that
 // wave w touches it leaves one part at slot w + r; as w and r never decrease along the tokens no two parts share a slot,
 // so nwaves + rows slots hold them. A join, one workgroup, adds each sequence's parts in a fixed order. Sums are in 64 bits,
-// since a log ratio is the small difference of long sums, and no result depends on scheduling. Up to kOneTokens tokens of
-// kOneRows sequences one workgroup does both in one launch, the parts in LDS.
+// since a log ratio is the small difference of long sums, and no result depends on scheduling. Small batches take one
+// launch of one workgroup that does both, the parts in LDS (one_launch).
 //
 // Measured, 512 packed sequences of 2048 tokens, four tensors read (16.8 MB): policy forward 9.5 us (1.8 TB/s), join 8.0,
 // backward 8.4 (21 MB: 2.5 TB/s; a large copy reaches 4.9); 16 x 1024 padded tokens: preference forward and join 8.0 us in
@@ -36,8 +36,11 @@ namespace {
 constexpr int kLaneTokens = 8, kWaveTokens = 64 * kLaneTokens;
 constexpr int kThreads = 256;        // a workgroup of the large grid
 constexpr int kJoinThreads = 1024;   // the join's, and that of the one-launch form
-constexpr int kOneTokens = 16384, kOneRows = 512;
-constexpr int kOneParts = kOneTokens / kWaveTokens + kOneRows;
+// Bounds of the one-launch form: tokens of a preference and of a policy loss with up to kFewRows sequences, and with up to
+// kOneRows.
+constexpr int kPrefTokens = 16384, kPolicyTokens = 8192, kFewRows = 64, kRowTokens = 4096, kOneRows = 512;
+constexpr int kOneParts = kRowTokens / kWaveTokens + kOneRows;
+static_assert(kPrefTokens / kWaveTokens + kFewRows <= kOneParts && kPolicyTokens <= kPrefTokens);
 
 struct Seqs {
   const int64_t* offsets;
@@ -323,7 +326,7 @@ __global__ __launch_bounds__(kThreads) void pref_bwd_kernel(const float* __restr
 // e^d - d - 1 without the cancellation near 0: its series there.
 __device__ __forceinline__ float kl_of(float d, float em1) {
   if (fabsf(d) < 0.5f) {
-    // d^2 / 2 (1 + d / 3 (1 + d / 4 (1 + ...))), up to d^9 / 10!: 2^-26 of the sum at 0.5.
+    // d^2 / 2 (1 + d / 3 (1 + d / 4 (1 + ...))), up to d^10 / 10!: what follows is 2^-33 of the sum at 0.5.
     float p = 1.f;
 #pragma unroll
     for (int k = 10; k >= 3; --k) p = __builtin_fmaf(d * (1.f / (float)k), p, 1.f);
@@ -529,15 +532,19 @@ bool aligned(const void* p, unsigned bytes) { return ((uintptr_t)p & (bytes - 1)
 size_t pref_workspace(long pairs, long n) { return (size_t)(tiles(n) + 2 * pairs) * sizeof(PrefPart); }
 size_t policy_workspace(long rows, long n) { return (size_t)(tiles(n) + rows) * sizeof(PolicyPart); }
 
-// One workgroup for a whole loss: a launch less.
-static bool one_launch(long rows, long n) { return n <= kOneTokens && rows <= kOneRows; }
+// One workgroup for a whole loss: a launch less (4 us and more of host time, 4 of GPU time for the join), but its 16 waves
+// alone form the parts, of which there are as many as tiles and sequences. us in one launch | in two, without the gap between
+// them: 16 sequences, preference 6.1 | 7.1 at 8192 tokens, 7.9 | 7.7 at 16384, 12 | 8.5 at 32768; policy 10.2 | 9.1,
+// 16.1 | 9.3, 28 | 10.1. 64 sequences of 16384 in all: 10.0 | 9.2, 18.5 | 10.2 (policy, 8192: 14.2 | 11.9). 512: preference
+// 38 | 36 at 4096, 31 | 22 at 8192, policy 71 | 68, 54 | 40.
+static bool one_launch(long rows, long n, long tokens) { return n <= (rows <= kFewRows ? tokens : kRowTokens) && rows <= kOneRows; }
 
 hipError_t launch_pref_fwd(const float* nll, const float* ref, const uint8_t* mask, const int64_t* offsets, long pairs, long n,
                            const PrefLoss& p, float* loss, float* reward, float* coef, void* ws, hipStream_t st) {
   PrefPart* part = static_cast<PrefPart*>(ws);
   const Seqs q = seqs(offsets, 2 * pairs, n);
   const bool vec = aligned(nll, 16) && aligned(ref, 16) && aligned(mask, 4);
-  if (one_launch(2 * pairs, n)) {
+  if (one_launch(2 * pairs, n, kPrefTokens)) {
     auto k = vec ? pref_fwd_kernel<true, true> : pref_fwd_kernel<false, true>;
     hipLaunchKernelGGL(k, dim3(1), dim3(kJoinThreads), 0, st, nll, ref, mask, q, p, part, loss, reward, coef);
     return hipGetLastError();
@@ -564,7 +571,7 @@ hipError_t launch_policy_fwd(const float* nll, const float* old, const float* re
   const Seqs q = seqs(offsets, rows, n);
   const bool vec = aligned(nll, 16) && aligned(old, 16) && aligned(ref, 16) && (!p.adv_per_token || aligned(adv, 16)) &&
                    aligned(mask, 4) && (p.reduction != kReduceNone || aligned(loss, 16));
-  if (one_launch(rows, n)) {
+  if (one_launch(rows, n, kPolicyTokens)) {
     auto k = vec ? policy_fwd_kernel<true, true> : policy_fwd_kernel<false, true>;
     hipLaunchKernelGGL(k, dim3(1), dim3(kJoinThreads), 0, st, nll, old, ref, adv, mask, q, p, part, loss, stats, weight);
     return hipGetLastError();

@@ -1,5 +1,5 @@
-"""GPU: the preference and policy losses on batches that take two launches (more than 16384 tokens or 512 sequences), at the
-borders between one launch and two, and on views off a 16-byte boundary, against their definition in 64 bits, vectorized.
+"""GPU: the preference and policy losses on batches that take two launches, at the borders between one launch and two, and on
+views off a 16-byte boundary, against their definition in 64 bits, vectorized.
 
 Tolerance: as test_gpu_preference.py, whose per-token errors do not grow with the number of tokens: sums are in 64 bits."""
 from __future__ import annotations
@@ -14,9 +14,9 @@ from tests import _preference as P
 pytestmark = pytest.mark.gpu
 
 TOL = 2e-6
-# one launch; two for the tokens' sake; one with 512 sequences; two for the sequences' sake; more pairs than join threads;
-# many parts of a sequence
-SIZES = [(2, 8192), (2, 8193), (512, 32), (514, 31), (40, 1500), (1300, 40), (2600, 9), (4, 30011)]
+# Few sequences: one launch up to 8192 tokens (policy), 16384 (preference). More than 64 sequences: up to 4096, of 512 sequences
+# at most. Then many parts of a sequence, and more pairs than join threads.
+SIZES = [(2, 4097), (2, 8192), (2, 8193), (64, 80), (66, 80), (512, 9), (514, 7), (40, 1500), (2600, 20), (4, 30011)]
 
 
 def _keep(shape, offsets, mask):
