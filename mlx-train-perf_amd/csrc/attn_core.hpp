@@ -68,8 +68,8 @@ struct Score {
   static constexpr bool kCap = MOD & kModCap, kSlope = MOD & kModSlope;
   float in2, mul, add, slope2, ratio;
   __device__ __forceinline__ Score(float scale_log2, float cap)
-      : in2(kCap ? scalar(2.f * scale_log2 / cap) : 0.f), mul(kCap ? scalar(2.f * cap * kLog2e) : scale_log2), add(kCap ? scalar(cap * kLog2e) : 0.f),
-        slope2(0.f), ratio(0.f) {}
+      : in2(kCap ? scalar(2.f * scale_log2 / cap) : 0.f), mul(kCap ? scalar(2.f * cap * kLog2e) : scale_log2),
+        add(kCap ? scalar(cap * kLog2e) : 0.f), slope2(0.f), ratio(0.f) {}
   // (the same in every lane: kept in scalar registers, as the vector ones are full)
   __device__ __forceinline__ void set_slope(float slope) {
     slope2 = scalar(slope * kLog2e);
@@ -91,26 +91,30 @@ struct Score {
 #pragma unroll
       for (int r = 0; r < 16; ++r) ramp[h][r] = step * at(h, r);
   }
-  // side: 1 where rel >= c for every pair of the wave's tile that is not hidden, -1 where rel <= c, 0 where neither; SIGN
-  // the usual one, whose term (a ramp's) a tile of neither keeps and corrects.
-  template <int SIGN, bool RAMP>
+  // Queries in lanes. side: 1 where rel >= c (no key behind its query) for every pair of the wave's tile that is not hidden,
+  // -1 where rel <= c, 0 where neither: such a tile keeps the usual term (a ramp's, rel >= c) and corrects it.
+  template <bool RAMP>
   __device__ __forceinline__ void slant(f32x16& v, int half, int side, float rel) const {
     if constexpr (RAMP) {
-      if (side == -SIGN) {
+      if (side == -1) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) v[r] = __builtin_fmaf(-2 * SIGN * ratio, at(half, r), v[r]);
+        for (int r = 0; r < 16; ++r) v[r] = __builtin_fmaf(-2 * ratio, at(half, r), v[r]);
       }
     } else {
-      const float k = side == -SIGN ? -SIGN * ratio : SIGN * ratio;
+      const float k = side == -1 ? -ratio : ratio;
 #pragma unroll
       for (int r = 0; r < 16; ++r) v[r] = __builtin_fmaf(k, at(half, r), v[r]);
     }
-    if (side == 0) {  // -|d| = -SIGN d + 2 min(SIGN d, 0)
+    if (side == 0) {  // -|d| = -d + 2 min(d, 0)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) v[r] = __builtin_fmaf(2.f * ratio, fminf(SIGN * (rel - at(half, r)), 0.f), v[r]);
+      for (int r = 0; r < 16; ++r) v[r] = __builtin_fmaf(2.f * ratio, fminf(rel - at(half, r), 0.f), v[r]);
     }
   }
-  // The same for keys in lanes, k times c and, where keys lie on both sides, the correction.
+  // add of such a tile.
+  __device__ __forceinline__ float slant_add(int side, float rel, float top) const {
+    return __builtin_fmaf(-slope2, (side == -1 ? -rel : rel) - top, add);
+  }
+  // Keys in lanes: k times c and, where keys lie on both sides, the correction (the usual term is that of rel <= c).
   __device__ __forceinline__ void lean(f32x16 (&v)[2], float k, bool both, float rel) const {
     if (k != 0.f) {
 #pragma unroll
@@ -124,11 +128,6 @@ struct Score {
 #pragma unroll
         for (int r = 0; r < 16; ++r) v[h][r] = __builtin_fmaf(2.f * ratio, fminf(at(h, r) - rel, 0.f), v[h][r]);
     }
-  }
-  // add of a slanted tile.
-  template <int SIGN>
-  __device__ __forceinline__ float slant_add(int side, float rel, float top) const {
-    return __builtin_fmaf(-slope2, (side == -SIGN ? -SIGN : SIGN) * rel - top, add);
   }
   static __device__ __forceinline__ float bend(float v) { return __builtin_fmaf(v, v, v); }
 };
@@ -880,13 +879,13 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
                     float* __restrict__ part) {
   // seg_start: the first key that each query sees (packed: its segment's start; span: its span's).
   // o_low (spans, caps and biases): the 8 bits of O below bf16's, written by the forward where given, read with O for
-  // D = rowsum(dO o O).
-  // SPLIT (the same; a variant of its own, as its walk cost the others 2.5%): workgroup `split` of a query block takes every nsplit-th key tile of its walk from tile `split`
-  // on, and writes its dQ, or its O before the division, to part[split] ([b][hq][s][dh]; the forward's maximum and sums
-  // [split][b][hq][s][4] behind all of them): attn_scored.hip joins them.
-  // dS = P (dP - D) is a difference that all but cancels where one probability is nearly 1, and
+  // D = rowsum(dO o O). dS = P (dP - D) is a difference that all but cancels where one probability is nearly 1, and
   // D of the rounded O was the largest part of dQ's and dK's error there (3.6e-3 of the norm against 2.4e-3: 4 x 16 heads,
   // 2048 positions, slopes). A value x is its bf16 plus o_low in units of 2^8 of its bits' value, whatever the exponent.
+  // SPLIT (spans, caps and biases; a variant of its own, as its walk cost the others 2.5%): workgroup `split` of a query
+  // block takes every nsplit-th key tile of its walk from tile `split` on, and writes its dQ, or its O before the division,
+  // to part[split] ([b][hq][s][dh]; the forward's maximum and sums [split][b][hq][s][4] behind all of them):
+  // attn_scored.hip joins them.
   constexpr bool PACKED = MASK != kMaskPlain, SPAN = MASK == kMaskSpan, CAP = MOD & kModCap;
   using L = kvdma::Lay<DH>;
   constexpr int kRowB = L::kRowB, kTile = L::kTile, kStage = L::kStage;
@@ -1199,9 +1198,9 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
           for (int r = 0; r < 16; ++r) sacc[kb][r] = score.raw(sacc[kb][r]);
         if constexpr (MOD == kModSlope) {
           const int side = side_of(kv0);
-          score.template slant<1, kRamp>(sacc[0], 0, side, rel);
-          score.template slant<1, kRamp>(sacc[1], 1, side, rel);
-          add = score.template slant_add<1>(side, rel, top);
+          score.template slant<kRamp>(sacc[0], 0, side, rel);
+          score.template slant<kRamp>(sacc[1], 1, side, rel);
+          add = score.slant_add(side, rel, top);
         }
         // Of a tile on one side of the queries all distances are one way from top: -slope2 (|d| - top) is -|slope2 (rel -+ top
         // - c)|. A tile of both sides has only distances below 100, and takes top as a term of its own.
@@ -1334,12 +1333,12 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
         bf16x8 pf[4];
         const int side = (MOD & kModSlope) ? side_of(kv0) : 0;
         const float rel = (float)(qi - kv0 - 4 * hf);
-        const float add = (MOD & kModSlope) ? score.template slant_add<1>(side, rel, top) : score.add;
+        const float add = (MOD & kModSlope) ? score.slant_add(side, rel, top) : score.add;
         auto form = [&](f32x16& sc, int kb) {  // raw products into v (Score)
           if constexpr (MOD != kModNone) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) sc[r] = score.raw(sc[r]);
-            if constexpr (MOD & kModSlope) score.template slant<1, kRamp>(sc, kb, side, rel);
+            if constexpr (MOD & kModSlope) score.template slant<kRamp>(sc, kb, side, rel);
           }
         };
         auto bias = [&]() { return MOD == kModNone ? ((m == kNegInf) ? 0.f : -m) : FIXED ? add : ((m == kNegInf) ? 0.f : -m) + add; };
@@ -1374,34 +1373,34 @@ void attn_kv_kernel(const bf16_t* __restrict__ q, const bf16_t* __restrict__ k, 
         form(s1, 1);
         mask(s1, 1);
         if constexpr (!FIXED) {
-        float mx = kNegInf;
+          float mx = kNegInf;
 #pragma unroll
-        for (int r = 0; r < 16; r += 2) mx = fmaxf(fmaxf(mx, s0[r]), fmaxf(s1[r], fmaxf(s0[r + 1], s1[r + 1])));
-        const float mt = MOD == kModNone ? max_xhalf(mx) * scale_log2  // scale_log2 > 0: the max of the scaled scores
-                                         : max_xhalf(__builtin_fmaf(mx, score.mul, add));  // add differs by lane half
-        // A row raises m only when the tile maximum exceeds it by more than kRescaleLog2: its O and
-        // l are then rescaled together and half 0 recomputed; otherwise probabilities up to
-        // 2^kRescaleLog2 accumulate against the old m. O / l and L = m + log2(l) are the same
-        // either way. The branch is taken by the whole wave when any row needs it (most tiles
-        // skip it), but each row decides for itself and the others keep their values bitwise (alpha
-        // 1, half 0 recomputed identically): a row's arithmetic depends only on its own scores, so
-        // rows of other packed segments sharing the wave come out bitwise the same whatever this
-        // row's keys hold.
-        const bool up = mt > m + kRescaleLog2;  // false while mt = -inf (all keys hidden)
-        if (__builtin_amdgcn_ballot_w64(up) != 0) {
-          const float alpha = up ? fast_exp2(m - mt) : 1.f;  // m = -inf: alpha = 0 (O, l are 0)
-          m = up ? mt : m;
-          l *= alpha;
-          lr *= alpha;
+          for (int r = 0; r < 16; r += 2) mx = fmaxf(fmaxf(mx, s0[r]), fmaxf(s1[r], fmaxf(s0[r + 1], s1[r + 1])));
+          const float mt = MOD == kModNone ? max_xhalf(mx) * scale_log2  // scale_log2 > 0: the max of the scaled scores
+                                           : max_xhalf(__builtin_fmaf(mx, score.mul, add));  // add differs by lane half
+          // A row raises m only when the tile maximum exceeds it by more than kRescaleLog2: its O and
+          // l are then rescaled together and half 0 recomputed; otherwise probabilities up to
+          // 2^kRescaleLog2 accumulate against the old m. O / l and L = m + log2(l) are the same
+          // either way. The branch is taken by the whole wave when any row needs it (most tiles
+          // skip it), but each row decides for itself and the others keep their values bitwise (alpha
+          // 1, half 0 recomputed identically): a row's arithmetic depends only on its own scores, so
+          // rows of other packed segments sharing the wave come out bitwise the same whatever this
+          // row's keys hold.
+          const bool up = mt > m + kRescaleLog2;  // false while mt = -inf (all keys hidden)
+          if (__builtin_amdgcn_ballot_w64(up) != 0) {
+            const float alpha = up ? fast_exp2(m - mt) : 1.f;  // m = -inf: alpha = 0 (O, l are 0)
+            m = up ? mt : m;
+            l *= alpha;
+            lr *= alpha;
 #pragma unroll
-          for (int db = 0; db < kDB; ++db)
+            for (int db = 0; db < kDB; ++db)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[db][r] *= alpha;
-          nb = bias();
-          l0 = 0.f;
+              for (int r = 0; r < 16; ++r) acc[db][r] *= alpha;
+            nb = bias();
+            l0 = 0.f;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) l0 += prob(s0, 0, r, nb);
-        }
+            for (int r = 0; r < 16; ++r) l0 += prob(s0, 0, r, nb);
+          }
         }
         l += l0;
         if constexpr (SCORED) {
