@@ -393,8 +393,8 @@ def flash_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale:
     slopes go with either). A query that sees nothing gets zeros and no gradient. `validate_segments` checks the
     contract of `spans` too, at one host sync a mask.
     The kernel impl takes a softcap in [1e-3, 1e3], with any of the three a scale above 0, and slopes of either sign. A
-    row's biases count from the highest of the keys that it sees, so that rows of any length keep their digits: what a
-    slope costs is 64 * |slope| * 2^-24 of a probability, 0.2% at 500 (`impl="reference"` forms them in fp32 as they are:
+    row's biases count from the highest of the keys that it sees, so that rows of any length keep their digits; in bf16 a
+    slope costs some 8e-6 * |slope| of a probability, 0.4% at 500 (`impl="reference"` forms biases in fp32 as they are:
     N * |slope| * 2^-24). As in a plain product, what the mask hides must be finite, padding too (V; in the backward Q,
     K and dO): 0 is what it is multiplied by. These calls differentiate once."""
     resolved = resolve_attention_impl(q, k, v, impl=impl, causal=causal, segments=segments,

@@ -134,3 +134,34 @@ def test_gradients_of_scores_above_the_cap(dh, cap, std, biased, dtype):
     # fp32: scores reach 4 std, of which 2^-24 (100: 2.4e-5) is also an error of x in the derivative's 2 x / cap
     more = 0.0 if dtype == torch.bfloat16 else 4 * std * 2 ** -24 * (1 + 2 / cap)
     _compare([x[0] for x in got], want, terms, dtype, BAR[dtype] + more, bend=2 ** -21)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize(("mask", "cap"), [("causal", None), ("full", None), ("ragged", None), ("window", 20.0), ("causal", 20.0), ("full", 90.0)])
+def test_logarithms_count_from_the_highest_bias(mask, cap, dtype):
+    """L of the C entry points is that of the scores less the highest bias of a row's visible keys, +inf where it sees none.
+    Scores of up to 2^5 in four roundings, 4 * 2^5 * 2^-24 = 8e-6, the logarithm's own, and 2^-22 of a cap: 5e-5 is twice that.
+    bf16 kernels: a tile's biases are slope * c, c < 64, and a term of the tile: the product begins from the former (one
+    rounding), adds up over dh / 16 = 4 steps, is multiplied and added to the latter, itself rounded (2), and L once: 8
+    roundings of at most 2^-24 of up to 64 * |slope|."""
+    from mlx_train_perf.attention.api import scored_forward
+
+    hq, hkv, s, dh = 4, 2, 301, 64
+    q, k, v, _ = (x.cuda() for x in S.inputs(1, hq, hkv, s, dh, dtype, 8))
+    slopes = torch.tensor([0.3, -0.3, -5.0, 60.0])
+    spans = S.spans_of(mask, 1, s, 4)
+    start, end = (None, None) if spans is None else (t.cuda() for t in spans)
+    _, lse, _, _ = scored_forward(q, k, v, slopes.cuda(), start, end, scale=dh ** -0.5, causal=mask == "causal", softcap=cap or 0.0)
+    see = S.visible(mask, spans, 1, s, "cuda")[0]
+    i = torch.arange(s, device="cuda")
+    away = (i[:, None] - i[None]).abs().double()
+    for h in range(hq):
+        x = dh ** -0.5 * (q[0, h].double() @ k[0, h // 2].double().T)
+        if cap is not None:
+            x = cap * torch.tanh(x / cap)
+        bias = torch.where(see, -float(slopes[h]) * away, -torch.inf)
+        want = torch.logsumexp(x + bias, 1) - bias.amax(1)
+        seen = see.any(1)
+        assert torch.isposinf(lse[0, h, ~seen]).all()
+        steps = 8 * 64 * abs(float(slopes[h])) * 2 ** -24 if dtype == torch.bfloat16 else 0.0
+        assert float((lse[0, h].double() - want)[seen].abs().max()) <= 5e-5 + steps, h
