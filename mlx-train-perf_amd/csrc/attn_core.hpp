@@ -19,9 +19,9 @@
 // in the dK/dV kernel), which leaves errors of 2.0e-3 of the norm in O, 2.3e-3 in dV and 2.4e-3 to 3.0e-3 in dQ and dK.
 //
 // Bound by the SIMDs' issue, matrix and vector instructions together: with a cap the matrix pipe is busy for 0.44 to 0.55
-// of the time (8192 positions, 32/8 heads, head_dim 128: forward 641 us, dQ 835, dK/dV 1174; without a cap 515, 690 and
+// of the time (8192 positions, 32/8 heads, head_dim 128: forward 637 us, dQ 828, dK/dV 1166; without a cap 515, 690 and
 // 1010), as a score costs an exponential and a reciprocal more. With slopes alone the products begin from the bias and the
-// times are the plain kernels' (4 x 16 heads x 2048 x 64: 60, 68 and 98 us).
+// forward and dQ take the plain kernels' times (4 x 16 heads x 2048 x 64: 59 and 68 us); dK/dV 101, 3% more (kUp).
 //
 // Kernel structure (all MFMA 32x32x16 bf16, fp32 accumulate):
 //   attn_kv_kernel<DH, MASK, DQ, MOD> (forward, and the dQ pass, which also forms D): a wave owns 32
@@ -673,8 +673,8 @@ void attn_bwd_dkv_ab_kernel(const bf16_t* __restrict__ q, const bf16_t* __restri
                 y = __builtin_fmaf(-score.slope2, d - t4[u], y);
               }
               // P is at most 1, but y is the difference of two numbers of the scores' size: from 2^22 on its rounding alone is
-              // 1, and 2^16 is past fp16; from 2^29 on 2^y may leave fp32. (A cap keeps scores below 2^12. NaN stays. 4 x 16 heads, 2048
-              // positions, head_dim 64, slopes: 111 us instead of 108.)
+              // 1, and 2^16 is past fp16; from 2^29 on 2^y may leave fp32. (A cap keeps scores below 2^12. NaN stays. 3% of the pass
+              // at 4 x 16 heads, 2048 positions, head_dim 64, slopes.)
               if constexpr (!CAP) y = __builtin_elementwise_minimum(y, kUp);
               const float p = fast_exp2(y);
               pown[h][r >> 3][r & 7] = (__bf16)p;

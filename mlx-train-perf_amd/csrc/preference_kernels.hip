@@ -23,9 +23,9 @@
 // since a log ratio is the small difference of long sums, and no result depends on scheduling. Small batches take one
 // launch of one workgroup that does both, the parts in LDS (one_launch).
 //
-// Measured, 512 packed sequences of 2048 tokens, four tensors read (16.8 MB): policy forward 9.5 us (1.8 TB/s), join 8.0,
-// backward 8.4 (21 MB: 2.5 TB/s; a large copy reaches 4.9); 16 x 1024 padded tokens: preference forward and join 8.0 us in
-// one launch (9.6 in two, with a sequence's parts found by exchanges through LDS), backward 3.5. The host takes 60 us for
+// Measured, 512 packed sequences of 2048 tokens, four tensors read (16.8 MB): policy forward 9.3 us (1.8 TB/s), join 8.1,
+// backward 8.7 (21 MB: 2.4 TB/s; a large copy reaches 4.9); 16 x 1024 padded tokens: preference forward and join 8.0 us in
+// one launch (7.7 in two and the gap between them), backward 3.4. The host takes 60 us for
 // such a step, so that what is left here does not show.
 #include "mtp_common.hpp"
 #include "mtp_launch.hpp"

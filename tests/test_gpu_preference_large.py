@@ -14,9 +14,9 @@ from tests import _preference as P
 pytestmark = pytest.mark.gpu
 
 TOL = 2e-6
-# Few sequences: one launch up to 8192 tokens (policy), 16384 (preference). More than 64 sequences: up to 4096, of 512 sequences
-# at most. Then many parts of a sequence, and more pairs than join threads.
-SIZES = [(2, 4097), (2, 8192), (2, 8193), (64, 80), (66, 80), (512, 9), (514, 7), (40, 1500), (2600, 20), (4, 30011)]
+# 64 sequences or fewer: one launch up to 8192 tokens (policy), 16384 (preference); more: up to 4096 tokens of 512 sequences.
+# Then more pairs than join threads, and many parts of a sequence.
+SIZES = [(2, 8193), (64, 80), (66, 80), (512, 8), (2600, 20), (4, 30011)]
 
 
 def _keep(shape, offsets, mask):
