@@ -7,9 +7,10 @@
  *       4-bit affine group-quantized (group size 64) head;
  *   (B) flash attention forward and backward with GQA, causal and packed-segment masks, saving
  *       only O and the per-row log-sum-exp L;
- * and two that the reference lacks:
+ * and three that the reference lacks:
  *   (C) attention with capped scores, a bias by distance and key spans;
- *   (D) preference and policy losses over the per-token losses of (A).
+ *   (D) preference and policy losses over the per-token losses of (A);
+ *   (E) token scoring (log probabilities, entropy, top alternatives) and distillation over a head.
  *
  * Conventions (all entry points):
  *   - Plain pointers and sizes; the caller allocates every tensor and the workspace and owns the
@@ -385,6 +386,88 @@ int mtp_policy_bwd(const float* d_loss, const float* nll, const float* old_nll, 
                    const float* advantages, int32_t adv_per_token, const uint8_t* mask, const int64_t* offsets,
                    int64_t rows, int64_t n, double clip_low, double clip_high, double kl_coef,
                    int32_t reduction, const float* weight, float* d_nll, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * (E) Token scoring and distillation over a head (no counterpart in the reference)
+ *
+ * hidden, head, n, d, v, head_kind: as (A), v <= 2^21. With x = hidden . w / temperature, lse = logsumexp x,
+ * p = exp(x - lse). temperature in [1e-3, 1e3]. The _f32 forms take fp32 hidden states and heads.
+ * A forward's head_kind MTP_HEAD_Q4_STAGED dequantizes the whole head into the workspace; a backward's kinds, chunk,
+ * row_block and w_t are mtp_lce_bwd's (mtp_lce_bwd_f32's).
+ * Rows that are left out (an ignored target; a mask of 0; an empty list) may hold anything, NaN too, and get gradients of 0.
+ * ------------------------------------------------------------------------------------------- */
+#define MTP_SCORE_MAX 128 /* most alternatives, and longest teacher's list */
+
+size_t mtp_logprobs_fwd_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t top);
+size_t mtp_logprobs_fwd_f32_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t top);
+
+/* Per token: logprobs = x_y - lse of the target y (targets NULL: no targets, and logprobs and tgt may be NULL; a target outside
+ * [0, v) counts as a logit of 0, as in mtp_lce_fwd), entropy = lse - sum p x, and the `top` largest logits (0 to
+ * min(v, MTP_SCORE_MAX)), the lowest index first among equal ones: top_ids int64 [n][top], top_logprobs fp32 [n][top]. An
+ * ignored target's row: 0, 0, ids -1, log probabilities -inf. lse, tgt (the target's logit before the temperature): fp32 [n],
+ * for the backward. */
+int mtp_logprobs_fwd(const void* hidden, const void* w, const uint32_t* w_q, const void* scales, const void* biases,
+                     const int64_t* targets, int64_t n, int64_t d, int64_t v, int32_t head_kind, int64_t ignore_index,
+                     int32_t top, double temperature, float* logprobs, float* entropy, float* top_logprobs,
+                     int64_t* top_ids, float* lse, float* tgt, void* workspace, size_t workspace_bytes, void* stream);
+int mtp_logprobs_fwd_f32(const float* hidden, const float* w, const uint32_t* w_q, const float* scales, const float* biases,
+                         const int64_t* targets, int64_t n, int64_t d, int64_t v, int32_t head_kind,
+                         int64_t ignore_index, int32_t top, double temperature, float* logprobs, float* entropy,
+                         float* top_logprobs, int64_t* top_ids, float* lse, float* tgt, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* Workspace of the backwards below: mtp_lce_bwd's, then the factors of the gradient (k columns a row: 1 for scoring, the list's
+ * length for distillation) and, for a trainable head, a copy of the hidden states. */
+size_t mtp_score_bwd_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int64_t chunk, int64_t row_block,
+                                     int32_t k, int32_t trainable);
+size_t mtp_score_bwd_f32_workspace_bytes(int64_t n, int64_t d, int64_t v, int64_t chunk, int32_t k, int32_t trainable);
+
+/* dL/dx = d_logprobs ([v = y] - p) - d_entropy p (x - lse + entropy); either gradient may be NULL (0). */
+int mtp_logprobs_bwd(const void* hidden, const void* w, const void* w_t, const uint32_t* w_q, const void* scales,
+                     const void* biases, const int64_t* targets, int64_t n, int64_t d, int64_t v, int32_t head_kind,
+                     int64_t ignore_index, double temperature, const float* lse, const float* entropy,
+                     const float* tgt, const float* d_logprobs, const float* d_entropy, void* d_hidden, void* d_w,
+                     int64_t chunk, int64_t row_block, void* workspace, size_t workspace_bytes, void* stream);
+int mtp_logprobs_bwd_f32(const float* hidden, const float* w, const uint32_t* w_q, const float* scales, const float* biases,
+                         const int64_t* targets, int64_t n, int64_t d, int64_t v, int32_t head_kind,
+                         int64_t ignore_index, double temperature, const float* lse, const float* entropy,
+                         const float* tgt, const float* d_logprobs, const float* d_entropy, float* d_hidden, float* d_w,
+                         int64_t chunk, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Divergence of a teacher's list from p, per token: ids int64 [n][k], 1 <= k <= MTP_SCORE_MAX, and the log probabilities
+ * teacher fp32 [n][k]. A slot is empty with an id outside [0, v), a log probability of -inf, or an id that an earlier slot of the
+ * row has. All outcomes outside the list count as one, of the mass 1 - sum (at least 1e-6) under either model;
+ * renormalize: the teacher has none there, t = softmax(teacher / temperature) over the list (not with reverse).
+ *   forward: KL(t | q); reverse: KL(q | t); jsd: beta KL(t | m) + (1 - beta) KL(q | m), m = beta t + (1 - beta) q, beta in (0, 1).
+ * mask: uint8 [n], or NULL. reduction none: loss [n] (0 for a row left out); mean: over the rows that are not; sum.
+ * scale [1] (unused with none), lse, rest [n], coef fp32 and columns int32 [n][k]: for the backward. */
+#define MTP_DISTILL_FORWARD 0
+#define MTP_DISTILL_REVERSE 1
+#define MTP_DISTILL_JSD 2
+
+size_t mtp_distill_fwd_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t k);
+size_t mtp_distill_fwd_f32_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t k);
+int mtp_distill_fwd(const void* hidden, const void* w, const uint32_t* w_q, const void* scales, const void* biases,
+                    const int64_t* ids, const float* teacher, const uint8_t* mask, int64_t n, int64_t d, int64_t v,
+                    int32_t head_kind, int32_t k, int32_t kind, double beta, double temperature, int32_t renormalize,
+                    int32_t reduction, float* loss, float* scale, float* lse, float* rest, float* coef,
+                    int32_t* columns, void* workspace, size_t workspace_bytes, void* stream);
+int mtp_distill_fwd_f32(const float* hidden, const float* w, const uint32_t* w_q, const float* scales, const float* biases,
+                        const int64_t* ids, const float* teacher, const uint8_t* mask, int64_t n, int64_t d, int64_t v,
+                        int32_t head_kind, int32_t k, int32_t kind, double beta, double temperature,
+                        int32_t renormalize, int32_t reduction, float* loss, float* scale, float* lse, float* rest,
+                        float* coef, int32_t* columns, void* workspace, size_t workspace_bytes, void* stream);
+/* From d_loss [n] (none) or [1] and what the forward left. */
+int mtp_distill_bwd(const void* hidden, const void* w, const void* w_t, const uint32_t* w_q, const void* scales,
+                    const void* biases, int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t k, double temperature,
+                    int32_t reduction, const float* d_loss, const float* scale, const float* lse, const float* rest,
+                    const float* coef, const int32_t* columns, void* d_hidden, void* d_w, int64_t chunk,
+                    int64_t row_block, void* workspace, size_t workspace_bytes, void* stream);
+int mtp_distill_bwd_f32(const float* hidden, const float* w, const uint32_t* w_q, const float* scales, const float* biases,
+                        int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t k, double temperature,
+                        int32_t reduction, const float* d_loss, const float* scale, const float* lse, const float* rest,
+                        const float* coef, const int32_t* columns, float* d_hidden, float* d_w, int64_t chunk,
+                        void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

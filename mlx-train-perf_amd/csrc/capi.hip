@@ -806,4 +806,308 @@ int mtp_policy_bwd(const float* d_loss, const float* nll, const float* old_nll, 
   return ok();
 }
 
+// ---------------------------------------------------------------------------------------------
+// Token scoring and distillation
+// ---------------------------------------------------------------------------------------------
+
+static int check_score(int64_t n, int64_t d, int64_t v, double temperature) {
+  if (v > mtp::kScoreVocab) return fail(MTP_ERR_UNSUPPORTED, "token scoring and distillation serve a vocabulary of at most 2^21 (got v=%lld); use impl='reference'", (long long)v);
+  if (!(temperature >= 1e-3 && temperature <= 1e3)) return fail(MTP_ERR_INPUT, "temperature must be in [1e-3, 1e3] (got %g)", temperature);
+  return MTP_OK;
+}
+
+static int check_list(int32_t k) {
+  if (k < 1 || k > MTP_SCORE_MAX) return fail(MTP_ERR_UNSUPPORTED, "a teacher's list has 1 to %d slots (got k=%d); use impl='reference'", MTP_SCORE_MAX, (int)k);
+  return MTP_OK;
+}
+
+static mtp::ScoreHead score_head(int f32, const void* hidden, const void* w, const uint32_t* w_q, const void* scales,
+                                 const void* biases, int32_t head_kind) {
+  mtp::ScoreHead h{};
+  h.f32 = f32;
+  h.hidden = hidden;
+  if (f32)
+    h.h32 = make_head32(static_cast<const float*>(w), w_q, static_cast<const float*>(scales), static_cast<const float*>(biases), head_kind);
+  else
+    h.h = make_head(w, w_q, scales, biases, head_kind);
+  return h;
+}
+
+// check_lce_common / check_lce32 without a target of each token.
+static int check_score_head(int f32, const void* hidden, const void* w, const uint32_t* w_q, const void* scales,
+                            const void* biases, int64_t n, int64_t d, int64_t v, int32_t head_kind) {
+  static const int64_t any = 0;
+  if (f32)
+    return check_lce32(static_cast<const float*>(hidden), static_cast<const float*>(w), w_q, static_cast<const float*>(scales),
+                       static_cast<const float*>(biases), &any, n, d, v, head_kind);
+  return check_lce_common(hidden, w, w_q, scales, biases, &any, n, d, v, head_kind);
+}
+
+static mtp::ScoreShape score_shape(int64_t n, int64_t d, int64_t v, double temperature, int32_t head_kind) {
+  return mtp::ScoreShape{(long)n, (long)d, (long)v, (float)(1.0 / temperature), head_kind == MTP_HEAD_Q4_STAGED};
+}
+
+static bool q4_kind(int32_t head_kind) { return head_kind == MTP_HEAD_Q4 || head_kind == MTP_HEAD_Q4_STAGED; }
+static bool score_sizes(int64_t n, int64_t d, int64_t v) {
+  return n >= 1 && d >= 1 && v >= 1 && n <= kMaxDim && d <= kMaxDim && v <= mtp::kScoreVocab;
+}
+
+static size_t logprobs_fwd_ws(int f32, int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t top) {
+  if (!score_sizes(n, d, v) || top < 0 || top > MTP_SCORE_MAX) return 0;
+  return mtp::logprobs_fwd_workspace(score_shape(n, d, v, 1.0, head_kind), f32, q4_kind(head_kind), top);
+}
+size_t mtp_logprobs_fwd_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t top) {
+  return logprobs_fwd_ws(0, n, d, v, head_kind, top);
+}
+size_t mtp_logprobs_fwd_f32_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t top) {
+  return logprobs_fwd_ws(1, n, d, v, head_kind, top);
+}
+
+static int logprobs_fwd(int f32, const void* hidden, const void* w, const uint32_t* w_q, const void* scales, const void* biases,
+                        const int64_t* targets, int64_t n, int64_t d, int64_t v, int32_t head_kind, int64_t ignore_index,
+                        int32_t top, double temperature, const mtp::LogprobsOut& out, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+  int rc = check_score_head(f32, hidden, w, w_q, scales, biases, n, d, v, head_kind);
+  if (rc) return rc;
+  rc = check_score(n, d, v, temperature);
+  if (rc) return rc;
+  if (top < 0 || top > v) return fail(MTP_ERR_INPUT, "top must be in [0, v=%lld] (got %d)", (long long)v, (int)top);
+  if (top > MTP_SCORE_MAX) return fail(MTP_ERR_UNSUPPORTED, "at most %d alternatives (got top=%d); use impl='reference'", MTP_SCORE_MAX, (int)top);
+  if (!out.entropy || !out.lse || (targets && (!out.logprobs || !out.tgt)) || (top && (!out.top_logprobs || !out.top_ids)))
+    return fail(MTP_ERR_INPUT, "entropy and lse, with targets logprobs and tgt, with top top_logprobs and top_ids must be non-null");
+  const size_t need = logprobs_fwd_ws(f32, n, d, v, head_kind, top);
+  if (!workspace || workspace_bytes < need)
+    return fail(MTP_ERR_WORKSPACE, "token scoring needs a workspace of %zu bytes (got %zu)", need, workspace ? workspace_bytes : (size_t)0);
+  if (!aligned16(workspace)) return fail(MTP_ERR_UNSUPPORTED, "workspace must be 16-byte aligned");
+  const hipError_t e = mtp::launch_logprobs_fwd(score_head(f32, hidden, w, w_q, scales, biases, head_kind),
+                                                score_shape(n, d, v, temperature, head_kind), targets, (long long)ignore_index,
+                                                (int)top, out, workspace, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(MTP_ERR_RUNTIME, "token scoring launch failed: %s", hipGetErrorString(e));
+  return ok();
+}
+
+int mtp_logprobs_fwd(const void* hidden, const void* w, const uint32_t* w_q, const void* scales, const void* biases,
+                     const int64_t* targets, int64_t n, int64_t d, int64_t v, int32_t head_kind, int64_t ignore_index,
+                     int32_t top, double temperature, float* logprobs, float* entropy, float* top_logprobs,
+                     int64_t* top_ids, float* lse, float* tgt, void* workspace, size_t workspace_bytes, void* stream) {
+  return logprobs_fwd(0, hidden, w, w_q, scales, biases, targets, n, d, v, head_kind, ignore_index, top, temperature,
+                      mtp::LogprobsOut{logprobs, entropy, top_logprobs, top_ids, lse, tgt}, workspace, workspace_bytes, stream);
+}
+int mtp_logprobs_fwd_f32(const float* hidden, const float* w, const uint32_t* w_q, const float* scales, const float* biases,
+                         const int64_t* targets, int64_t n, int64_t d, int64_t v, int32_t head_kind, int64_t ignore_index,
+                         int32_t top, double temperature, float* logprobs, float* entropy, float* top_logprobs,
+                         int64_t* top_ids, float* lse, float* tgt, void* workspace, size_t workspace_bytes, void* stream) {
+  return logprobs_fwd(1, hidden, w, w_q, scales, biases, targets, n, d, v, head_kind, ignore_index, top, temperature,
+                      mtp::LogprobsOut{logprobs, entropy, top_logprobs, top_ids, lse, tgt}, workspace, workspace_bytes, stream);
+}
+
+// After the loss's workspace: alpha [n], beta [n], the columns [n] of scoring, the values [n][k], the cleared hidden states.
+struct ScoreBwd {
+  size_t alpha, beta, columns, value, clean, bytes;
+};
+static ScoreBwd score_bwd_parts(size_t lce, int64_t n, int64_t d, int32_t k, int32_t trainable, size_t elem) {
+  auto pad = [](size_t x) { return (x + 255) / 256 * 256; };
+  ScoreBwd p;
+  p.alpha = pad(lce);
+  p.beta = p.alpha + pad((size_t)n * 4);
+  p.columns = p.beta + pad((size_t)n * 4);
+  p.value = p.columns + pad((size_t)n * 4);
+  p.clean = p.value + pad((size_t)n * k * 4);
+  p.bytes = p.clean + (trainable ? (size_t)n * d * elem : 0);
+  return p;
+}
+size_t mtp_score_bwd_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int64_t chunk, int64_t row_block,
+                                     int32_t k, int32_t trainable) {
+  const size_t lce = mtp_lce_bwd_workspace_bytes(n, d, v, head_kind, chunk, row_block);
+  return !lce || k < 1 || k > MTP_SCORE_MAX ? 0 : score_bwd_parts(lce, n, d, k, trainable, 2).bytes;
+}
+size_t mtp_score_bwd_f32_workspace_bytes(int64_t n, int64_t d, int64_t v, int64_t chunk, int32_t k, int32_t trainable) {
+  const size_t lce = mtp_lce_bwd_f32_workspace_bytes(n, d, v, chunk);
+  return !lce || k < 1 || k > MTP_SCORE_MAX ? 0 : score_bwd_parts(lce, n, d, k, trainable, 4).bytes;
+}
+
+}  // extern "C"
+
+// The shared backward: `factors` launches what fills alpha, beta (or none), columns and value.
+template <class FACTORS>
+static int score_bwd(int f32, const void* hidden, const void* w, const void* w_t, const uint32_t* w_q, const void* scales,
+                     const void* biases, int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t k, double temperature,
+                     const float* lse, const int32_t* columns, void* d_hidden, void* d_w, int64_t chunk, int64_t row_block,
+                     void* workspace, size_t workspace_bytes, hipStream_t stream, const FACTORS& factors) {
+  int rc = check_score_head(f32, hidden, w, w_q, scales, biases, n, d, v, head_kind);
+  if (rc) return rc;
+  rc = check_score(n, d, v, temperature);
+  if (rc) return rc;
+  if (!lse || !d_hidden) return fail(MTP_ERR_INPUT, "lse and d_hidden must be non-null");
+  if (!aligned16(d_hidden) || (d_w && !aligned16(d_w)) || (w_t && !aligned16(w_t)))
+    return fail(MTP_ERR_UNSUPPORTED, "d_hidden, d_w and w_t must be 16-byte aligned");
+  if (d_w && q4_kind(head_kind)) return fail(MTP_ERR_UNSUPPORTED, "a quantized head is frozen: d_w must be null");
+  if (w_t && (f32 || staged_kind(head_kind))) return fail(MTP_ERR_INPUT, "fp32 and the staged head kinds take no w_t");
+  const int64_t tile = f32 ? 128 : kTile;
+  if (chunk < tile || chunk % tile) return fail(MTP_ERR_INPUT, "chunk must be a positive multiple of %lld (got %lld)", (long long)tile, (long long)chunk);
+  if (chunk > round_up(v, tile)) chunk = round_up(v, tile);
+  if (row_block == 0 || row_block > n) row_block = n;
+  if (row_block < n && (f32 || row_block < 0 || row_block % kTile))
+    return fail(MTP_ERR_INPUT, "row_block must be 0, >= n, or (bf16) a positive multiple of 256 (got %lld)", (long long)row_block);
+  if (d_w && row_block < n) return fail(MTP_ERR_INPUT, "a trainable head (d_w) sums over every row: row_block must cover all n=%lld rows", (long long)n);
+  const size_t lce = f32 ? mtp_lce_bwd_f32_workspace_bytes(n, d, v, chunk) : mtp_lce_bwd_workspace_bytes(n, d, v, head_kind, chunk, row_block);
+  const ScoreBwd parts = score_bwd_parts(lce, n, d, k, d_w != nullptr, f32 ? 4 : 2);
+  if (!workspace || workspace_bytes < parts.bytes)
+    return fail(MTP_ERR_WORKSPACE, "the backward needs a workspace of %zu bytes at chunk=%lld, row_block=%lld (got %zu)", parts.bytes, (long long)chunk, (long long)row_block, workspace ? workspace_bytes : (size_t)0);
+  if (!aligned16(workspace)) return fail(MTP_ERR_UNSUPPORTED, "workspace must be 16-byte aligned");
+  char* ws = static_cast<char*>(workspace);
+  float* alpha = reinterpret_cast<float*>(ws + parts.alpha);
+  float* beta = reinterpret_cast<float*>(ws + parts.beta);
+  int* own_columns = reinterpret_cast<int*>(ws + parts.columns);
+  float* value = reinterpret_cast<float*>(ws + parts.value);
+  bool has_beta = false;
+  hipError_t e = factors(alpha, beta, own_columns, value, &has_beta);
+  if (e == hipSuccess && d_w)
+    e = mtp::launch_clean_rows(hidden, alpha, has_beta ? beta : nullptr, (long)n, (long)d * (f32 ? 4 : 2), ws + parts.clean, stream);
+  if (e == hipSuccess) {
+    const float inv_t = (float)(1.0 / temperature);
+    const mtp::AffineGrad grad{{alpha, has_beta ? beta : nullptr, 1.4426950408889634f * inv_t}, columns ? columns : own_columns, value, (int)k, ws + parts.clean};
+    if (f32) {
+      e = mtp::launch_lce32_bwd(score_head(1, hidden, w, w_q, scales, biases, head_kind).h32, static_cast<const float*>(hidden), nullptr,
+                                lse, nullptr, (int)n, (int)d, (int)v, 0, (int)chunk, static_cast<float*>(d_hidden),
+                                static_cast<float*>(d_w), static_cast<float*>(workspace), stream, &grad);
+    } else {
+      mtp::LceHead head = make_head(w, w_q, scales, biases, head_kind);
+      head.wt = static_cast<const mtp::bf16_t*>(w_t);
+      mtp::bf16_t* stage = staged_kind(head_kind) ? reinterpret_cast<mtp::bf16_t*>(ws + lce_bwd_stage_offset(n, d, v, chunk, row_block)) : nullptr;
+      e = mtp::launch_lce_bwd(head, static_cast<const mtp::bf16_t*>(hidden), nullptr, lse, nullptr, (int)n, (int)d, (int)v, 0,
+                              (int)chunk, (int)row_block, static_cast<mtp::bf16_t*>(d_hidden), static_cast<mtp::bf16_t*>(d_w),
+                              static_cast<mtp::bf16_t*>(workspace),
+                              reinterpret_cast<float*>(ws + lce_bwd_acc_offset(chunk, row_block)),
+                              reinterpret_cast<float*>(ws + lce_bwd_parts_offset(d, v, chunk, row_block)), stage, stream, &grad);
+    }
+  }
+  if (e != hipSuccess) return fail(MTP_ERR_RUNTIME, "backward launch failed: %s", hipGetErrorString(e));
+  return ok();
+}
+
+extern "C" {
+
+static int logprobs_bwd(int f32, const void* hidden, const void* w, const void* w_t, const uint32_t* w_q, const void* scales,
+                        const void* biases, const int64_t* targets, int64_t n, int64_t d, int64_t v, int32_t head_kind,
+                        int64_t ignore_index, double temperature, const float* lse, const float* entropy, const float* tgt,
+                        const float* d_logprobs, const float* d_entropy, void* d_hidden, void* d_w, int64_t chunk,
+                        int64_t row_block, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!entropy || (targets && !tgt)) return fail(MTP_ERR_INPUT, "entropy, and with targets tgt, must be non-null");
+  if (d_logprobs && !targets) return fail(MTP_ERR_INPUT, "d_logprobs needs targets");
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  return score_bwd(f32, hidden, w, w_t, w_q, scales, biases, n, d, v, head_kind, 1, temperature, lse, nullptr, d_hidden, d_w, chunk,
+                   row_block, workspace, workspace_bytes, st, [&](float* alpha, float* beta, int* columns, float* value, bool* has_beta) {
+                     *has_beta = d_entropy != nullptr;
+                     return mtp::launch_logprobs_coef(d_logprobs, d_entropy, targets, (long long)ignore_index, lse, entropy, tgt,
+                                                      (long)n, (long)v, (float)(1.0 / temperature), alpha, beta, columns, value, st);
+                   });
+}
+int mtp_logprobs_bwd(const void* hidden, const void* w, const void* w_t, const uint32_t* w_q, const void* scales,
+                     const void* biases, const int64_t* targets, int64_t n, int64_t d, int64_t v, int32_t head_kind,
+                     int64_t ignore_index, double temperature, const float* lse, const float* entropy, const float* tgt,
+                     const float* d_logprobs, const float* d_entropy, void* d_hidden, void* d_w, int64_t chunk,
+                     int64_t row_block, void* workspace, size_t workspace_bytes, void* stream) {
+  return logprobs_bwd(0, hidden, w, w_t, w_q, scales, biases, targets, n, d, v, head_kind, ignore_index, temperature, lse, entropy,
+                      tgt, d_logprobs, d_entropy, d_hidden, d_w, chunk, row_block, workspace, workspace_bytes, stream);
+}
+int mtp_logprobs_bwd_f32(const float* hidden, const float* w, const uint32_t* w_q, const float* scales, const float* biases,
+                         const int64_t* targets, int64_t n, int64_t d, int64_t v, int32_t head_kind, int64_t ignore_index,
+                         double temperature, const float* lse, const float* entropy, const float* tgt, const float* d_logprobs,
+                         const float* d_entropy, float* d_hidden, float* d_w, int64_t chunk, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+  return logprobs_bwd(1, hidden, w, nullptr, w_q, scales, biases, targets, n, d, v, head_kind, ignore_index, temperature, lse, entropy,
+                      tgt, d_logprobs, d_entropy, d_hidden, d_w, chunk, 0, workspace, workspace_bytes, stream);
+}
+
+static size_t distill_fwd_ws(int f32, int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t k) {
+  if (!score_sizes(n, d, v) || k < 1 || k > MTP_SCORE_MAX) return 0;
+  return mtp::distill_fwd_workspace(score_shape(n, d, v, 1.0, head_kind), f32, q4_kind(head_kind), k);
+}
+size_t mtp_distill_fwd_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t k) {
+  return distill_fwd_ws(0, n, d, v, head_kind, k);
+}
+size_t mtp_distill_fwd_f32_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t k) {
+  return distill_fwd_ws(1, n, d, v, head_kind, k);
+}
+
+static int check_reduction(int32_t reduction) {
+  if (reduction != MTP_REDUCE_NONE && reduction != MTP_REDUCE_MEAN && reduction != MTP_REDUCE_SUM)
+    return fail(MTP_ERR_INPUT, "unknown reduction %d of a distillation loss", (int)reduction);
+  return MTP_OK;
+}
+
+static int distill_fwd(int f32, const void* hidden, const void* w, const uint32_t* w_q, const void* scales, const void* biases,
+                       const int64_t* ids, const float* teacher, const uint8_t* mask, int64_t n, int64_t d, int64_t v,
+                       int32_t head_kind, int32_t k, int32_t kind, double beta, double temperature, int32_t renormalize,
+                       int32_t reduction, const mtp::DistillOut& out, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_score_head(f32, hidden, w, w_q, scales, biases, n, d, v, head_kind);
+  if (rc) return rc;
+  if ((rc = check_score(n, d, v, temperature)) || (rc = check_list(k)) || (rc = check_reduction(reduction))) return rc;
+  if (kind < MTP_DISTILL_FORWARD || kind > MTP_DISTILL_JSD) return fail(MTP_ERR_INPUT, "unknown kind %d of a distillation loss", (int)kind);
+  if (kind == MTP_DISTILL_JSD && !(beta > 0.0 && beta < 1.0)) return fail(MTP_ERR_INPUT, "beta must be in (0, 1) (got %g)", beta);
+  if (kind == MTP_DISTILL_REVERSE && renormalize) return fail(MTP_ERR_INPUT, "a renormalized teacher gives nothing to what its list leaves out: the reverse divergence is infinite");
+  if (!ids || !teacher) return fail(MTP_ERR_INPUT, "ids and teacher must be non-null");
+  if (!out.loss || !out.lse || !out.rest || !out.coef || !out.columns || (reduction != MTP_REDUCE_NONE && !out.scale))
+    return fail(MTP_ERR_INPUT, "loss, scale, lse, rest, coef and columns must be non-null");
+  const size_t need = distill_fwd_ws(f32, n, d, v, head_kind, k);
+  if (!workspace || workspace_bytes < need)
+    return fail(MTP_ERR_WORKSPACE, "distillation needs a workspace of %zu bytes (got %zu)", need, workspace ? workspace_bytes : (size_t)0);
+  if (!aligned16(workspace)) return fail(MTP_ERR_UNSUPPORTED, "workspace must be 16-byte aligned");
+  const hipError_t e = mtp::launch_distill_fwd(score_head(f32, hidden, w, w_q, scales, biases, head_kind),
+                                               score_shape(n, d, v, temperature, head_kind), ids, teacher, mask,
+                                               mtp::DistillLoss{(int)k, kind, renormalize != 0, reduction, beta}, out, workspace,
+                                               static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(MTP_ERR_RUNTIME, "distillation launch failed: %s", hipGetErrorString(e));
+  return ok();
+}
+int mtp_distill_fwd(const void* hidden, const void* w, const uint32_t* w_q, const void* scales, const void* biases,
+                    const int64_t* ids, const float* teacher, const uint8_t* mask, int64_t n, int64_t d, int64_t v,
+                    int32_t head_kind, int32_t k, int32_t kind, double beta, double temperature, int32_t renormalize,
+                    int32_t reduction, float* loss, float* scale, float* lse, float* rest, float* coef, int32_t* columns,
+                    void* workspace, size_t workspace_bytes, void* stream) {
+  return distill_fwd(0, hidden, w, w_q, scales, biases, ids, teacher, mask, n, d, v, head_kind, k, kind, beta, temperature, renormalize,
+                     reduction, mtp::DistillOut{loss, scale, lse, rest, coef, columns}, workspace, workspace_bytes, stream);
+}
+int mtp_distill_fwd_f32(const float* hidden, const float* w, const uint32_t* w_q, const float* scales, const float* biases,
+                        const int64_t* ids, const float* teacher, const uint8_t* mask, int64_t n, int64_t d, int64_t v,
+                        int32_t head_kind, int32_t k, int32_t kind, double beta, double temperature, int32_t renormalize,
+                        int32_t reduction, float* loss, float* scale, float* lse, float* rest, float* coef, int32_t* columns,
+                        void* workspace, size_t workspace_bytes, void* stream) {
+  return distill_fwd(1, hidden, w, w_q, scales, biases, ids, teacher, mask, n, d, v, head_kind, k, kind, beta, temperature, renormalize,
+                     reduction, mtp::DistillOut{loss, scale, lse, rest, coef, columns}, workspace, workspace_bytes, stream);
+}
+
+static int distill_bwd(int f32, const void* hidden, const void* w, const void* w_t, const uint32_t* w_q, const void* scales,
+                       const void* biases, int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t k, double temperature,
+                       int32_t reduction, const float* d_loss, const float* scale, const float* lse, const float* rest,
+                       const float* coef, const int32_t* columns, void* d_hidden, void* d_w, int64_t chunk, int64_t row_block,
+                       void* workspace, size_t workspace_bytes, void* stream) {
+  int rc;
+  if ((rc = check_list(k)) || (rc = check_reduction(reduction))) return rc;
+  if (!d_loss || !rest || !coef || !columns || (reduction != MTP_REDUCE_NONE && !scale))
+    return fail(MTP_ERR_INPUT, "d_loss, scale, rest, coef and columns must be non-null");
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  return score_bwd(f32, hidden, w, w_t, w_q, scales, biases, n, d, v, head_kind, k, temperature, lse, columns, d_hidden, d_w, chunk,
+                   row_block, workspace, workspace_bytes, st, [&](float* alpha, float*, int*, float* value, bool*) {
+                     return mtp::launch_distill_coef(d_loss, reduction == MTP_REDUCE_NONE, scale, rest, coef, (long)n, (int)k, alpha, value, st);
+                   });
+}
+int mtp_distill_bwd(const void* hidden, const void* w, const void* w_t, const uint32_t* w_q, const void* scales,
+                    const void* biases, int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t k, double temperature,
+                    int32_t reduction, const float* d_loss, const float* scale, const float* lse, const float* rest,
+                    const float* coef, const int32_t* columns, void* d_hidden, void* d_w, int64_t chunk, int64_t row_block,
+                    void* workspace, size_t workspace_bytes, void* stream) {
+  return distill_bwd(0, hidden, w, w_t, w_q, scales, biases, n, d, v, head_kind, k, temperature, reduction, d_loss, scale, lse, rest, coef,
+                     columns, d_hidden, d_w, chunk, row_block, workspace, workspace_bytes, stream);
+}
+int mtp_distill_bwd_f32(const float* hidden, const float* w, const uint32_t* w_q, const float* scales, const float* biases,
+                        int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t k, double temperature, int32_t reduction,
+                        const float* d_loss, const float* scale, const float* lse, const float* rest, const float* coef,
+                        const int32_t* columns, float* d_hidden, float* d_w, int64_t chunk, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+  return distill_bwd(1, hidden, w, nullptr, w_q, scales, biases, n, d, v, head_kind, k, temperature, reduction, d_loss, scale, lse, rest,
+                     coef, columns, d_hidden, d_w, chunk, 0, workspace, workspace_bytes, stream);
+}
+
 }  // extern "C"

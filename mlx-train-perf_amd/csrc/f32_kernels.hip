@@ -19,6 +19,7 @@
 // reads consecutive k of its row: the register-staged core k = 8 h + s of 16, the copied one
 // 8 c + 4 h + s of 32. The 16x16x4 layout stands at the attention kernels.
 #include "attn32_core.hpp"
+#include "score_gather.hpp"
 
 namespace mtp {
 namespace f32k {
@@ -327,14 +328,18 @@ constexpr int kStage1 = KIND == kCopied ? 2 * kOpB : 16;
 // LCE forward: workgroup (128-token tile, vocab split) walks the split's 128-column vocab tiles;
 // C[v][t] = W_v . H_t, so each lane owns token columns and keeps an online (max, sum of exp2) per
 // token, merged with lane ^ 32 and the other vocab-half wave at the end into part_m/part_s
-// [split][N] (log2 domain), which the finalize merges.
+// [split][N] (log2 domain), which the finalize merges. STAT as in lce_fwd_kernel (lce_kernels.hip).
 // ------------------------------------------------------------------------------------------
-template <int KIND>
+template <int KIND, int STAT = 0>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void lce32_fwd_kernel(const float* __restrict__ H, const float* __restrict__ W,
                                                         const uint32_t* __restrict__ Wq, const float* __restrict__ Sc,
                                                         const float* __restrict__ Bi, int N, int D, int V, int nsplit,
-                                                        float* __restrict__ part_m, float* __restrict__ part_s) {
+                                                        float* __restrict__ part_m, float* __restrict__ part_s, float scale2,
+                                                        float* __restrict__ part_u, float* __restrict__ gmax, int ldg) {
+  const float c2 = STAT ? scale2 : kLog2e;
+  constexpr float kHidden = (STAT & kStatEntropy) ? -1e30f : kNegInf;
+  __shared__ float gx[(STAT & kStatGroups) ? kT : 1];
   __shared__ __attribute__((aligned(1024))) char s0[kStage0<KIND>];
   __shared__ __attribute__((aligned(1024))) char s1[kStage1<KIND>];
   float* lds = reinterpret_cast<float*>(s0);
@@ -344,7 +349,7 @@ void lce32_fwd_kernel(const float* __restrict__ H, const float* __restrict__ W,
   const int vt0 = split * per, vt1 = (vt0 + per < vtiles) ? vt0 + per : vtiles;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, wa = w & 1, wb = w >> 1, h = lane >> 5;
   RowSrc hb{H + (long)t0 * D, D, N - t0, D, aligned16(H) && D % 4 == 0};
-  float m[2] = {kNegInf, kNegInf}, s[2] = {0.f, 0.f};
+  float m[2] = {kNegInf, kNegInf}, s[2] = {0.f, 0.f}, u[2] = {0.f, 0.f};
   for (int vt = vt0; vt < vt1; ++vt) {
     const int v0 = vt * kT;
     f32x16 acc[2][2];
@@ -365,30 +370,50 @@ void lce32_fwd_kernel(const float* __restrict__ H, const float* __restrict__ W,
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int v = v0 + 64 * wa + 32 * i + rrow(r, h);
-          if (v >= V) acc[i][j][r] = kNegInf;
+          if (v >= V) acc[i][j][r] = kHidden;
           mz = fmaxf(mz, acc[i][j][r]);
         }
-      const float mn = fmaxf(m[j], mz * kLog2e);
-      const float base = (mn == kNegInf) ? 0.f : mn;
-      float sum = 0.f;
+      if constexpr (STAT & kStatGroups) {  // the tile's maximum of each token: of both halves of both waves
+        const float both = fmaxf(mz, __shfl_xor(mz, 32, 64));
+        const int tl = 64 * wb + 32 * j + (lane & 31);
+        if (wa == 1 && h == 0) gx[tl] = both;
+        __syncthreads();
+        if (wa == 0 && h == 0 && t0 + tl < N) gmax[(long)(t0 + tl) * ldg + vt] = fmaxf(both, gx[tl]);
+      }
+      const float mn = fmaxf(m[j], mz * c2);
+      const float base = (STAT & kStatEntropy) ? fmaxf(mn, -1e28f) : (mn == kNegInf) ? 0.f : mn;
+      float sum = 0.f, sumu = 0.f;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sum += fast_exp2(__builtin_fmaf(acc[i][j][r], kLog2e, -base));
-      s[j] = s[j] * fast_exp2(m[j] - base) + sum;
+        for (int r = 0; r < 16; ++r) {
+          const float x = __builtin_fmaf(acc[i][j][r], c2, -base);
+          const float e = fast_exp2(x);
+          sum += e;
+          if constexpr (STAT & kStatEntropy) sumu = __builtin_fmaf(e, x, sumu);
+        }
+      const float f = fast_exp2(m[j] - base);
+      if constexpr (STAT & kStatEntropy) u[j] = __builtin_fmaf(s[j], m[j] == kNegInf ? 0.f : m[j] - base, u[j]) * f + sumu;
+      s[j] = s[j] * f + sum;
       m[j] = mn;
     }
   }
 #pragma unroll
-  for (int j = 0; j < 2; ++j) lse2_merge(m[j], s[j], __shfl_xor(m[j], 32, 64), __shfl_xor(s[j], 32, 64));
+  for (int j = 0; j < 2; ++j) {
+    const float mo = __shfl_xor(m[j], 32, 64), so = __shfl_xor(s[j], 32, 64);
+    if constexpr (STAT & kStatEntropy) lse2_merge(m[j], s[j], u[j], mo, so, __shfl_xor(u[j], 32, 64));
+    else lse2_merge(m[j], s[j], mo, so);
+  }
   __syncthreads();
   float* xm = lds;
   float* xs = lds + 128;
+  float* xu = lds + 256;
   if (wa == 1 && h == 0) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       xm[64 * wb + 32 * j + (lane & 31)] = m[j];
       xs[64 * wb + 32 * j + (lane & 31)] = s[j];
+      if constexpr (STAT & kStatEntropy) xu[64 * wb + 32 * j + (lane & 31)] = u[j];
     }
   }
   __syncthreads();
@@ -396,13 +421,46 @@ void lce32_fwd_kernel(const float* __restrict__ H, const float* __restrict__ W,
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int tl = 64 * wb + 32 * j + (lane & 31);
-      lse2_merge(m[j], s[j], xm[tl], xs[tl]);
+      if constexpr (STAT & kStatEntropy) lse2_merge(m[j], s[j], u[j], xm[tl], xs[tl], xu[tl]);
+      else lse2_merge(m[j], s[j], xm[tl], xs[tl]);
       if (t0 + tl < N) {
         part_m[(long)split * N + t0 + tl] = m[j];
         part_s[(long)split * N + t0 + tl] = s[j];
+        if constexpr (STAT & kStatEntropy) part_u[(long)split * N + t0 + tl] = u[j];
       }
     }
   }
+}
+
+// H_t . W_y as an fp32 dot product over the wave (every lane returns the total).
+template <int Q4>
+__device__ __forceinline__ float row_dot32(const float* __restrict__ h, const float* __restrict__ W,
+                                           const uint32_t* __restrict__ Wq, const float* __restrict__ Sc,
+                                           const float* __restrict__ Bi, long long y, int D, int lane) {
+  float dot = 0.f;
+  if constexpr (Q4) {
+    const Q4Geom q{Wq, Sc, Bi, D};
+    for (int d = lane; d < D; d += 64) dot = __builtin_fmaf(h[d], q.w(y, d), dot);
+  } else {
+    const float* wr = W + (long)y * D;
+    for (int d = lane; d < D; d += 64) dot = __builtin_fmaf(h[d], wr[d], dot);
+  }
+  return wave_sum(dot);
+}
+
+// Each token's target logit alone, 0 for a target outside the vocabulary; one wave per token.
+template <int Q4>
+__global__ __launch_bounds__(256) void lce32_target_kernel(const float* __restrict__ H, const float* __restrict__ W,
+                                                           const uint32_t* __restrict__ Wq, const float* __restrict__ Sc,
+                                                           const float* __restrict__ Bi, const int64_t* __restrict__ targets,
+                                                           int N, int D, int V, float* __restrict__ tgt) {
+  const int lane = threadIdx.x & 63;
+  const int t = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (t >= N) return;
+  const long long y = targets[t];
+  float dot = 0.f;
+  if (y >= 0 && y < (long long)V) dot = row_dot32<Q4>(H + (long)t * D, W, Wq, Sc, Bi, y, D, lane);
+  if (lane == 0) tgt[t] = dot;
 }
 
 // Per token (one wave each): merge the splits into lse, tgt = H_t . W_y as an fp32 dot product,
@@ -428,17 +486,7 @@ __global__ __launch_bounds__(256) void lce32_finalize_kernel(const float* __rest
   const bool ignored = y == ignore_index;
   const bool inrange = y >= 0 && y < (long long)V;
   float dot = 0.f;
-  if (!ignored && inrange) {
-    const float* h = H + (long)t * D;
-    if constexpr (Q4) {
-      const Q4Geom q{Wq, Sc, Bi, D};
-      for (int d = lane; d < D; d += 64) dot = __builtin_fmaf(h[d], q.w(y, d), dot);
-    } else {
-      const float* wr = W + (long)y * D;
-      for (int d = lane; d < D; d += 64) dot = __builtin_fmaf(h[d], wr[d], dot);
-    }
-    dot = wave_sum(dot);
-  }
+  if (!ignored && inrange) dot = row_dot32<Q4>(H + (long)t * D, W, Wq, Sc, Bi, y, D, lane);
   if (lane == 0) {
     lse[t] = l;
     tgt[t] = (ignored || !inrange) ? 0.f : dot;
@@ -449,15 +497,16 @@ __global__ __launch_bounds__(256) void lce32_finalize_kernel(const float* __rest
 // Gradient tile of the backward: C[t][v] = H_t . W_v for rows [row0, row0 + nrows) and the chunk's
 // columns [c0, c0 + ncols); G[t][v - c0] = (exp(C - lse_t) - [v == y_t]) * coef_t in fp32, coef_t =
 // d_nll[t] (0 for ignored rows), 0 past the vocab end (up to a multiple of 4 columns, which the dH
-// product reads).
-template <int KIND>
+// product reads). AFFINE as in lce_bwd_g_persist_kernel (lce_kernels.hip).
+template <int KIND, int AFFINE = 0>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void lce32_bwd_g_kernel(const float* __restrict__ H, const float* __restrict__ W,
                                                           const uint32_t* __restrict__ Wq, const float* __restrict__ Sc,
                                                           const float* __restrict__ Bi, const int64_t* __restrict__ targets,
                                                           const float* __restrict__ lse, const float* __restrict__ dnll,
                                                           int D, int V, long long ignore_index, int row0, int nrows,
-                                                          int c0, int ncols, float* __restrict__ G, long ldg) {
+                                                          int c0, int ncols, float* __restrict__ G, long ldg,
+                                                          AffineRows rows) {
   __shared__ __attribute__((aligned(1024))) char s0[kStage0<KIND>];
   __shared__ __attribute__((aligned(1024))) char s1[kStage1<KIND>];
   float* lds = reinterpret_cast<float*>(s0);
@@ -468,8 +517,14 @@ void lce32_bwd_g_kernel(const float* __restrict__ H, const float* __restrict__ W
   // Per row: coefficient, log2-domain lse and the target's column in the chunk (-1: none), fetched ahead
   // of the product (it has barriers between these writes and the reads below).
   __shared__ float rcoef[kT], rl2[kT];
-  __shared__ int ry[kT];
-  if (threadIdx.x < kT) {
+  __shared__ int ry[kT];  // AFFINE: the bits of beta
+  if (AFFINE && threadIdx.x < kT) {
+    const int t = row0 + tt + threadIdx.x;
+    const bool ok = tt + (int)threadIdx.x < nrows;
+    rcoef[threadIdx.x] = ok ? rows.alpha[t] : 0.f;
+    rl2[threadIdx.x] = ok ? lse[t] * kLog2e : 0.f;
+    ry[threadIdx.x] = __builtin_bit_cast(int, ok && rows.beta ? rows.beta[t] : 0.f);
+  } else if (threadIdx.x < kT) {
     const int t = row0 + tt + threadIdx.x;
     const bool ok = tt + (int)threadIdx.x < nrows;
     const long long y = ok ? targets[t] : -1;
@@ -500,13 +555,94 @@ void lce32_bwd_g_kernel(const float* __restrict__ H, const float* __restrict__ W
         const int vl = vv + 64 * wb + 32 * j + (lane & 31);
         if (vl >= ((ncols + 3) & ~3)) continue;
         float g = 0.f;
-        if (c0 + vl < V) {
+        if constexpr (AFFINE) {
+          const float slope = __builtin_bit_cast(float, y);
+          const float p = fast_exp2(__builtin_fmaf(acc[i][j][r], rows.scale2, -l2));
+          if (c0 + vl < V && (coef != 0.f || slope != 0.f)) g = p * __builtin_fmaf(slope, acc[i][j][r], coef);
+        } else if (c0 + vl < V) {
           const float p = fast_exp2(__builtin_fmaf(acc[i][j][r], kLog2e, -l2));
           g = (p - (vl == y ? 1.f : 0.f)) * coef;
         }
         G[(long)tl * ldg + vl] = g;
       }
     }
+}
+
+// A row's listed columns of an affine gradient (column < 0: none), one wave per row.
+__global__ __launch_bounds__(256) void lce32_bwd_g_columns_kernel(const int* __restrict__ columns,
+                                                                  const float* __restrict__ value, int k, int nrows, int c0,
+                                                                  int ncols, float* __restrict__ G, long ldg) {
+  const int t = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (t >= nrows) return;
+  for (int i = threadIdx.x & 63; i < k; i += 64) {
+    const int y = columns[(long)t * k + i];
+    if (y >= c0 && y - c0 < ncols) G[(long)t * ldg + (y - c0)] = value[(long)t * k + i];
+  }
+}
+
+// The rows of a gather's entries as an operand: past the last entry zeros. Offsets from H in 32 bits: a pass has at most
+// kScoreRows tokens, of fewer than 2^15 dims on the copied core.
+struct GatherSrc {
+  static constexpr bool kCol = false;
+  const float* p;
+  const int2* entries;
+  int D, count, K;
+  bool vec;
+  __device__ __forceinline__ float at(const float* row, int k) const { return k < K ? row[k] : 0.f; }
+  __device__ __forceinline__ f32x4 quad(int r, int k) const {
+    if (r >= count) return f32x4{0.f, 0.f, 0.f, 0.f};
+    const float* row = p + (long)entries[r].x * D;
+    if (vec && k + 3 < K) return *reinterpret_cast<const f32x4*>(row + k);
+    return f32x4{at(row, k), at(row, k + 1), at(row, k + 2), at(row, k + 3)};
+  }
+};
+struct GatherOp : RowOp {
+  uint32_t off[4];
+  __device__ __forceinline__ GatherOp(const float* p_, const int2* entries, int count, int D) : RowOp(p_, D, kT, D) {
+    const int first = 8 * (threadIdx.x >> 6) + ((threadIdx.x & 63) >> 3);
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      const int r = first + 32 * m;
+      off[m] = r < count ? 4u * ((uint32_t)entries[r].x * (uint32_t)D + (uint32_t)ck) : 0x80000000u;  // out of any range
+    }
+  }
+  __device__ __forceinline__ void copy(int kt, char* dst) const {
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), left = K - kt * kDK;
+    const bool in = ck < left;
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+      lds_copy16(p + kt * kDK, left > 0 ? 0x7fffffff : 0, dst + 1024 * (4 * m + w), in ? off[m] : 0x80000000u);
+  }
+};
+
+// The logits of a gather's entries (GatherPlan): C[v][entry] = W_v . H_token of one group and up to 128 entries.
+template <int KIND>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void lce32_gather_kernel(const float* __restrict__ H, const float* __restrict__ W, const uint32_t* __restrict__ Wq,
+                         const float* __restrict__ Sc, const float* __restrict__ Bi, int D, int V, GatherPlan plan) {
+  static_assert(kT == kGroup, "a tile is a group");
+  __shared__ __attribute__((aligned(1024))) char s0[kStage0<KIND>];
+  __shared__ __attribute__((aligned(1024))) char s1[kStage1<KIND>];
+  const GatherTile tile = plan.tiles[blockIdx.x];
+  if (tile.count == 0) return;
+  const int2* entries = plan.entries + tile.first;
+  const int v0 = tile.group * kGroup;
+  f32x16 acc[2][2];
+  if constexpr (KIND == kCopied) {
+    gemm128_copied(RowOp(W + (long)v0 * D, D, V - v0, D), GatherOp(H, entries, tile.count, D), D, s0, s1, acc);
+  } else {
+    GatherSrc hs{H, entries, D, tile.count, D, aligned16(H) && D % 4 == 0};
+    float* lds = reinterpret_cast<float*>(s0);
+    if constexpr (KIND == kQ4) {
+      Q4RowSrc ws{Q4Geom{Wq, Sc, Bi, D}, v0, V - v0, D};
+      gemm128(ws, hs, D, lds, acc);
+    } else {
+      RowSrc ws{W + (long)v0 * D, D, V - v0, D, aligned16(W) && D % 4 == 0};
+      gemm128(ws, hs, D, lds, acc);
+    }
+  }
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  store_gathered<2, 2>(acc, plan, entries, tile.count, V - v0, 64 * (w & 1), 64 * (w >> 1), lane);
 }
 
 // Stores (ACC: adds) a product's tile to C[M][N]: blockIdx.x: 128 rows, blockIdx.y: 128 columns. PA, PB: the
@@ -630,17 +766,45 @@ int lce32_fwd_nsplit(long N, long V) {
 // check the bases) and whose 128-row tiles stay below the 31-bit offsets of a copy.
 static bool copied_tiles(long d, long ld) { return d % 4 == 0 && ld % 4 == 0 && d < (1L << 21) && ld < (1L << 21); }
 
+template <int STAT>
+static hipError_t lce32_fwd_tiles(const LceHead32& h, const float* H, int N, int D, int V, float* pm, float* ps, float scale2,
+                                  float* pu, float* gmax, int ldg, hipStream_t st) {
+  const int ns = lce32_fwd_nsplit(N, V);
+  auto kernel = h.q4 ? lce32_fwd_kernel<kQ4, STAT> : copied_tiles(D, D) ? lce32_fwd_kernel<kCopied, STAT> : lce32_fwd_kernel<kDense, STAT>;
+  hipLaunchKernelGGL(kernel, dim3((N + kT - 1) / kT, ns), dim3(256), 0, st, H, h.w, h.wq, h.sc, h.bi, N, D, V, ns, pm, ps,
+                     scale2, pu, gmax, ldg);
+  return hipGetLastError();
+}
+
+hipError_t launch_lce32_stats(const LceHead32& h, const float* H, int N, int D, int V, const ScoreStats& x, hipStream_t st) {
+  if (x.gmax)
+    return lce32_fwd_tiles<kStatScaled | kStatEntropy | kStatGroups>(h, H, N, D, V, x.m, x.s, x.scale2, x.u, x.gmax, x.ldg, st);
+  if (x.u) return lce32_fwd_tiles<kStatScaled | kStatEntropy>(h, H, N, D, V, x.m, x.s, x.scale2, x.u, nullptr, 0, st);
+  return lce32_fwd_tiles<kStatScaled>(h, H, N, D, V, x.m, x.s, x.scale2, nullptr, nullptr, 0, st);
+}
+
+hipError_t launch_lce32_target(const LceHead32& h, const float* H, const int64_t* targets, int N, int D, int V, float* tgt,
+                               hipStream_t st) {
+  auto kernel = h.q4 ? lce32_target_kernel<1> : lce32_target_kernel<0>;
+  hipLaunchKernelGGL(kernel, dim3((N + 3) / 4), dim3(256), 0, st, H, h.w, h.wq, h.sc, h.bi, targets, N, D, V, tgt);
+  return hipGetLastError();
+}
+
+hipError_t launch_lce32_gather(const LceHead32& h, const float* H, int D, int V, const GatherPlan& p, hipStream_t st) {
+  // The product's core is the forward's, so that a logit is the same number in both.
+  auto kernel = h.q4 ? lce32_gather_kernel<kQ4> : copied_tiles(D, D) && D < (1 << 15) ? lce32_gather_kernel<kCopied> : lce32_gather_kernel<kDense>;
+  hipLaunchKernelGGL(kernel, dim3(p.max_tiles), dim3(256), 0, st, H, h.w, h.wq, h.sc, h.bi, D, V, p);
+  return hipGetLastError();
+}
+
 hipError_t launch_lce32_fwd(const LceHead32& h, const float* H, const int64_t* targets, int N, int D, int V,
                             long long ignore_index, float* nll, float* lse, float* tgt, float* ws, hipStream_t st) {
   const int ns = lce32_fwd_nsplit(N, V);
   float* pm = ws;
   float* ps = ws + (long)ns * N;
-  dim3 grid((N + kT - 1) / kT, ns), block(256);
-  if (h.q4) hipLaunchKernelGGL(lce32_fwd_kernel<kQ4>, grid, block, 0, st, H, h.w, h.wq, h.sc, h.bi, N, D, V, ns, pm, ps);
-  else if (copied_tiles(D, D)) hipLaunchKernelGGL(lce32_fwd_kernel<kCopied>, grid, block, 0, st, H, h.w, h.wq, h.sc, h.bi, N, D, V, ns, pm, ps);
-  else hipLaunchKernelGGL(lce32_fwd_kernel<kDense>, grid, block, 0, st, H, h.w, h.wq, h.sc, h.bi, N, D, V, ns, pm, ps);
-  hipError_t e = hipGetLastError();
+  hipError_t e = lce32_fwd_tiles<0>(h, H, N, D, V, pm, ps, 0.f, nullptr, nullptr, 0, st);
   if (e != hipSuccess) return e;
+  const dim3 block(256);
   dim3 fgrid((N + 3) / 4);
   if (h.q4) hipLaunchKernelGGL(lce32_finalize_kernel<1>, fgrid, block, 0, st, H, h.w, h.wq, h.sc, h.bi, targets, N, D, V, ns, pm, ps, ignore_index, nll, lse, tgt);
   else hipLaunchKernelGGL(lce32_finalize_kernel<0>, fgrid, block, 0, st, H, h.w, h.wq, h.sc, h.bi, targets, N, D, V, ns, pm, ps, ignore_index, nll, lse, tgt);
@@ -666,16 +830,20 @@ int lce32_dh_parts(long N, long D, long kcols, int* per) {
 
 hipError_t launch_lce32_bwd(const LceHead32& h, const float* H, const int64_t* targets, const float* lse,
                             const float* dnll, int N, int D, int V, long long ignore_index, int chunk, float* dH,
-                            float* dW, float* Gbuf, hipStream_t st) {
+                            float* dW, float* Gbuf, hipStream_t st, const AffineGrad* affine) {
   const long ldg = (long)chunk + 4;
   const bool copied = copied_tiles(D, ldg);
   dim3 block(256);
   for (int c0 = 0; c0 < V; c0 += chunk) {
     const int kc = (V - c0 < chunk) ? V - c0 : chunk;
     dim3 ggrid((N + kT - 1) / kT, (kc + kT - 1) / kT);
-    if (h.q4) hipLaunchKernelGGL(lce32_bwd_g_kernel<kQ4>, ggrid, block, 0, st, H, h.w, h.wq, h.sc, h.bi, targets, lse, dnll, D, V, ignore_index, 0, N, c0, kc, Gbuf, ldg);
-    else if (copied) hipLaunchKernelGGL(lce32_bwd_g_kernel<kCopied>, ggrid, block, 0, st, H, h.w, h.wq, h.sc, h.bi, targets, lse, dnll, D, V, ignore_index, 0, N, c0, kc, Gbuf, ldg);
-    else hipLaunchKernelGGL(lce32_bwd_g_kernel<kDense>, ggrid, block, 0, st, H, h.w, h.wq, h.sc, h.bi, targets, lse, dnll, D, V, ignore_index, 0, N, c0, kc, Gbuf, ldg);
+    auto gradient = affine ? (h.q4 ? lce32_bwd_g_kernel<kQ4, 1> : copied ? lce32_bwd_g_kernel<kCopied, 1> : lce32_bwd_g_kernel<kDense, 1>)
+                           : (h.q4 ? lce32_bwd_g_kernel<kQ4> : copied ? lce32_bwd_g_kernel<kCopied> : lce32_bwd_g_kernel<kDense>);
+    hipLaunchKernelGGL(gradient, ggrid, block, 0, st, H, h.w, h.wq, h.sc, h.bi, targets, lse, dnll, D, V, ignore_index, 0, N,
+                       c0, kc, Gbuf, ldg, affine ? affine->rows : AffineRows{});
+    if (affine)
+      hipLaunchKernelGGL(lce32_bwd_g_columns_kernel, dim3((N + 3) / 4), block, 0, st, affine->columns, affine->value, affine->k,
+                         N, c0, kc, Gbuf, ldg);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const bool acc = c0 > 0;
@@ -709,8 +877,9 @@ hipError_t launch_lce32_bwd(const LceHead32& h, const float* H, const int64_t* t
     if (e != hipSuccess) return e;
     if (dW) {
       dim3 wgrid((kc + kT - 1) / kT, (D + kT - 1) / kT);
-      if (copied) hipLaunchKernelGGL(lce32_dw_kernel<kCopied>, wgrid, block, 0, st, Gbuf, ldg, H, N, D, kc, dW + (long)c0 * D);
-      else hipLaunchKernelGGL(lce32_dw_kernel<kDense>, wgrid, block, 0, st, Gbuf, ldg, H, N, D, kc, dW + (long)c0 * D);
+      const float* rows = affine ? static_cast<const float*>(affine->clean) : H;
+      if (copied) hipLaunchKernelGGL(lce32_dw_kernel<kCopied>, wgrid, block, 0, st, Gbuf, ldg, rows, N, D, kc, dW + (long)c0 * D);
+      else hipLaunchKernelGGL(lce32_dw_kernel<kDense>, wgrid, block, 0, st, Gbuf, ldg, rows, N, D, kc, dW + (long)c0 * D);
       e = hipGetLastError();
       if (e != hipSuccess) return e;
     }

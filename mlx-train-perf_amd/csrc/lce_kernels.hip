@@ -884,13 +884,21 @@ __device__ __forceinline__ bool xcd_rect_tile(int mtiles, int ntiles, int& m, in
 // token columns, so the vocab reduction is lane-local except for one final exchange. Row r of the
 // dense W holds vocab row wrow0 + r (0 for the whole head, the chunk's first row for a 4-bit head's
 // rows dequantized into a staging buffer, which give the in-register dequantization's values).
+//
+// STAT (mtp_launch.hpp, kStat...) is what token scoring wants beside it: the softmax of z / temperature (scale2 =
+// log2(e) / temperature), the sum of 2^(x - m) (x - m) that the entropy is made of (an fma per logit), and the maximum of
+// every group of kGroup logits, which the tile's own maximum holds already. 0 is the loss as it was.
 // ------------------------------------------------------------------------------------------
-template <int Q4>
+template <int Q4, int STAT = 0>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void lce_fwd_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
                     const uint32_t* __restrict__ Wq, const bf16_t* __restrict__ Sc,
                     const bf16_t* __restrict__ Bi, int N, int D, int V, int nsplit, int split0, int nlocal,
-                    int wrow0, float* __restrict__ part_m, float* __restrict__ part_s) {
+                    int wrow0, float* __restrict__ part_m, float* __restrict__ part_s, float scale2,
+                    float* __restrict__ part_u, float* __restrict__ gmax, int ldg) {
+  const float c2 = STAT ? scale2 : kLog2e;
+  // Hidden rows past V: beyond any logit, but finite where 0 of it has to be 0.
+  constexpr float kHidden = (STAT & kStatEntropy) ? -1e30f : kNegInf;
   __shared__ __attribute__((aligned(16))) char lds[Q4 ? kLdsBytes + kQ4SbBytes : kLdsBytes];
   // Workgroup g runs on XCD g % 8. When the row tiles divide into 8 groups, XCD x owns row tiles
   // [x R/8, (x+1) R/8) for every split, walked split-major: the ~32 workgroups resident on one XCD
@@ -922,11 +930,12 @@ void lce_fwd_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
   const int t0 = rt * kTile;
   const int nk = (D + kBK - 1) / kBK;
 
-  float m[kNJ], s[kNJ];
+  float m[kNJ], s[kNJ], u[kNJ];
 #pragma unroll
   for (int j = 0; j < kNJ; ++j) {
     m[j] = kNegInf;
     s[j] = 0.f;
+    u[j] = 0.f;
   }
 
   // Online (max, sum exp2) update of this lane's token columns with one 256-row vocab tile, in the
@@ -943,16 +952,16 @@ void lce_fwd_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int v = v0 + 128 * wa + 32 * i + 8 * (r >> 2) + 4 * lhalf + (r & 3);
-            if (v >= V) acc[i][j][r] = kNegInf;
+            if (v >= V) acc[i][j][r] = kHidden;
           }
     }
     // Four partial maxima and sums per token column, combined in a fixed order: four short
     // dependency chains instead of one 64 long (forward -1%).
-    float pm[kNJ][4], ps[kNJ][4];
+    float pm[kNJ][4], ps[kNJ][4], pu[kNJ][4];
 #pragma unroll
     for (int j = 0; j < kNJ; ++j)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) pm[j][u] = kNegInf;
+      for (int c = 0; c < 4; ++c) pm[j][c] = kNegInf;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -963,22 +972,37 @@ void lce_fwd_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
 #pragma unroll
     for (int j = 0; j < kNJ; ++j) {
       const float a0 = fmaxf(fmaxf(pm[j][0], pm[j][1]), fmaxf(pm[j][2], pm[j][3]));
-      mn[j] = fmaxf(m[j], a0 * kLog2e);
-      base[j] = (mn[j] == kNegInf) ? 0.f : mn[j];
+      mn[j] = fmaxf(m[j], a0 * c2);
+      // (a lane may have met nothing but hidden rows: they stay far below the base)
+      base[j] = (STAT & kStatEntropy) ? fmaxf(mn[j], -1e28f) : (mn[j] == kNegInf) ? 0.f : mn[j];
+      if constexpr (STAT & kStatGroups) {
+        const float both = fmaxf(a0, __shfl_xor(a0, 32, 64));
+        const int t = t0 + 64 * wb + 32 * j + lcol;
+        if (lhalf == 0 && t < N) gmax[(long)t * ldg + (v0 >> 7) + wa] = both;
+      }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) ps[j][u] = 0.f;
+      for (int c = 0; c < 4; ++c) ps[j][c] = pu[j][c] = 0.f;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int r = 0; r < 16; ++r)
 #pragma unroll
-        for (int j = 0; j < kNJ; ++j)
-          ps[j][r & 3] += fast_exp2(__builtin_fmaf(acc[i][j][r], kLog2e, -base[j]));
+        for (int j = 0; j < kNJ; ++j) {
+          const float x = __builtin_fmaf(acc[i][j][r], c2, -base[j]);
+          const float e = fast_exp2(x);
+          ps[j][r & 3] += e;
+          if constexpr (STAT & kStatEntropy) pu[j][r & 3] = __builtin_fmaf(e, x, pu[j][r & 3]);
+        }
 #pragma unroll
     for (int j = 0; j < kNJ; ++j) {
       const float sum = (ps[j][0] + ps[j][1]) + (ps[j][2] + ps[j][3]);
-      s[j] = s[j] * fast_exp2(m[j] - base[j]) + sum;
+      const float f = fast_exp2(m[j] - base[j]);
+      if constexpr (STAT & kStatEntropy) {
+        const float down = m[j] == kNegInf ? 0.f : m[j] - base[j];
+        u[j] = __builtin_fmaf(s[j], down, u[j]) * f + ((pu[j][0] + pu[j][1]) + (pu[j][2] + pu[j][3]));
+      }
+      s[j] = s[j] * f + sum;
       m[j] = mn[j];
     }
   };
@@ -1086,17 +1110,20 @@ void lce_fwd_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
   for (int j = 0; j < kNJ; ++j) {
     const float mo = __shfl_xor(m[j], 32, 64);
     const float so = __shfl_xor(s[j], 32, 64);
-    lse2_merge(m[j], s[j], mo, so);
+    if constexpr (STAT & kStatEntropy) lse2_merge(m[j], s[j], u[j], mo, so, __shfl_xor(u[j], 32, 64));
+    else lse2_merge(m[j], s[j], mo, so);
   }
   // Merge the two waves sharing the same token columns (wa = 0, 1) through LDS.
   float* xm = reinterpret_cast<float*>(lds);
   float* xs = xm + 256;
+  float* xu = xm + 512;
   if (wa == 1 && lhalf == 0) {
 #pragma unroll
     for (int j = 0; j < kNJ; ++j) {
       const int tl = 64 * wb + 32 * j + lcol;
       xm[tl] = m[j];
       xs[tl] = s[j];
+      if constexpr (STAT & kStatEntropy) xu[tl] = u[j];
     }
   }
   __syncthreads();
@@ -1104,11 +1131,13 @@ void lce_fwd_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
 #pragma unroll
     for (int j = 0; j < kNJ; ++j) {
       const int tl = 64 * wb + 32 * j + lcol;
-      lse2_merge(m[j], s[j], xm[tl], xs[tl]);
+      if constexpr (STAT & kStatEntropy) lse2_merge(m[j], s[j], u[j], xm[tl], xs[tl], xu[tl]);
+      else lse2_merge(m[j], s[j], xm[tl], xs[tl]);
       const int t = t0 + tl;
       if (t < N) {
         part_m[(long)split * N + t] = m[j];
         part_s[(long)split * N + t] = s[j];
+        if constexpr (STAT & kStatEntropy) part_u[(long)split * N + t] = u[j];
       }
     }
   }
@@ -1186,6 +1215,29 @@ __global__ __launch_bounds__(256) void lce_fwd_finalize_kernel(
   }
 }
 
+// Each token's target logit H_t . W_y alone (4-bit weights rounded to bf16, as in the product tiles), 0 for a target outside
+// the vocabulary; one wave per token.
+template <int Q4>
+__global__ __launch_bounds__(256) void lce_target_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
+                                                         const uint32_t* __restrict__ Wq, const bf16_t* __restrict__ Sc,
+                                                         const bf16_t* __restrict__ Bi, const int64_t* __restrict__ targets,
+                                                         int N, int D, int V, float* __restrict__ tgt) {
+  const int lane = threadIdx.x & 63;
+  const int t = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (t >= N) return;
+  const long long y = targets[t];
+  float dot = 0.f;
+  if (y >= 0 && y < (long long)V) dot = row_dot<Q4, true>(H + (long)t * D, W, Wq, Sc, Bi, y, D, lane);
+  if (lane == 0) tgt[t] = dot;
+}
+
+hipError_t launch_lce_target(const LceHead& h, const bf16_t* H, const int64_t* targets, int N, int D, int V, float* tgt,
+                             hipStream_t stream) {
+  auto kernel = h.q4 ? lce_target_kernel<1> : lce_target_kernel<0>;
+  hipLaunchKernelGGL(kernel, dim3((N + 3) / 4), dim3(256), 0, stream, H, h.w, h.wq, h.sc, h.bi, targets, N, D, V, tgt);
+  return hipGetLastError();
+}
+
 // ------------------------------------------------------------------------------------------
 // Backward step 1: G[t][v - v_begin] = bf16((exp(z_tv - lse_t) - [v == y_t]) * coef_t) for one
 // vocab chunk [v_begin, v_end). coef_t = d_nll_t, or 0 for ignored rows. Columns of the padded
@@ -1195,11 +1247,12 @@ __global__ __launch_bounds__(256) void lce_fwd_finalize_kernel(
 // per XCD (workgroup id g runs on XCD g % 8), so concurrently running tiles on one XCD share the
 // same weight rows in L2.
 // ------------------------------------------------------------------------------------------
+template <int AFFINE>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void lce_bwd_g_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
                       const int64_t* __restrict__ targets, const float* __restrict__ lse,
                       const float* __restrict__ dnll, long long ignore_index, int N, int D, int V, int v_begin,
-                      int v_end, int vtiles, int ldg, bf16_t* __restrict__ G) {
+                      int v_end, int vtiles, int ldg, bf16_t* __restrict__ G, AffineRows rows) {
   __shared__ __attribute__((aligned(16))) char lds[kLdsBytes];
   const int rtiles = (N + kTile - 1) / kTile;
   int rt, vtl;
@@ -1234,13 +1287,19 @@ void lce_bwd_g_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W
   for (int j = 0; j < kNJ; ++j) {
     const int tl = 64 * wb + 32 * j + lcol;
     const int t = t0 + tl;
-    float coef = 0.f, l2 = 0.f;
+    float coef = 0.f, l2 = 0.f, slope = 0.f;
     long long y = -1;
     if (t < N) {
-      y = targets[t];
-      coef = (y == ignore_index) ? 0.f : dnll[t];
+      if constexpr (AFFINE) {
+        coef = rows.alpha[t];
+        slope = rows.beta ? rows.beta[t] : 0.f;
+      } else {
+        y = targets[t];
+        coef = (y == ignore_index) ? 0.f : dnll[t];
+      }
       l2 = lse[t] * kLog2e;
     }
+    const bool live = !AFFINE || coef != 0.f || slope != 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -1250,9 +1309,14 @@ void lce_bwd_g_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W
         for (int u = 0; u < 4; ++u) {
           const int r = 4 * q + u;
           const int v = v0 + 128 * wa + 32 * i + 8 * q + 4 * lhalf + u;
-          float p = fast_exp2(acc[i][j][r] * kLog2e - l2);
-          if (v == y) p -= 1.f;
-          gv[u] = (v < vlim) ? p * coef : 0.f;
+          if constexpr (AFFINE) {
+            const float p = fast_exp2(acc[i][j][r] * rows.scale2 - l2);
+            gv[u] = (v < vlim && live) ? p * __builtin_fmaf(slope, acc[i][j][r], coef) : 0.f;
+          } else {
+            float p = fast_exp2(acc[i][j][r] * kLog2e - l2);
+            if (v == y) p -= 1.f;
+            gv[u] = (v < vlim) ? p * coef : 0.f;
+          }
         }
         const int c = 16 * wa + 4 * i + q;  // 16-byte chunk of the 256-wide vocab row
         const int off = tl * 512 + ((c ^ (tl & 31)) << 4) + 8 * lhalf;
@@ -1331,15 +1395,18 @@ __device__ __forceinline__ void store_lines(char* blk, const __amdgpu_buffer_rsr
 // 2048 x 896 x 151936 1133 -> 1055 us, 8192 x 1024 x 50000 1541 -> 1418 us.
 // The blocks lie past the two stages (dense head: 160 KB in all), or in the first stage's head tile, which the
 // 4-bit head's next tile fills only after its first barrier.
+// AFFINE: the gradient of any loss of the softmax that leaves G = p (alpha_t + beta_t z) but for a few columns a row
+// (lce_bwd_g_columns_kernel), p the softmax of z / temperature. Rows with neither factor are written as zeros, whatever their
+// hidden state holds.
 // ------------------------------------------------------------------------------------------
-template <int Q4>
+template <int Q4, int AFFINE = 0>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void lce_bwd_g_persist_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
                               const uint32_t* __restrict__ Wq, const bf16_t* __restrict__ Sc,
                               const bf16_t* __restrict__ Bi, const int64_t* __restrict__ targets,
                               const float* __restrict__ lse, const float* __restrict__ dnll, long long ignore_index,
                               int N, int D, int V, int v_begin, int v_end, int ctiles, int nsplit, int ldg,
-                              int wrow0, bf16_t* __restrict__ G) {
+                              int wrow0, bf16_t* __restrict__ G, AffineRows rows) {
   // One array: with a second one the compiler tracks the copies into LDS by array and waits for all
   // of them (vmcnt(0)) before fragment reads of every stage (flagship 4.09 -> 4.62 ms).
   static_assert(kLdsBytes + (Q4 ? kQ4SbBytes : 8 * kGBlockBytes) <= 160 * 1024, "more than a CU's LDS");
@@ -1370,15 +1437,21 @@ void lce_bwd_g_persist_kernel(const bf16_t* __restrict__ H, const bf16_t* __rest
   const int vlim = v_end < V ? v_end : V;
 
   // Per-thread token rows (fixed for the workgroup): coefficient and log2-domain lse.
-  float coef[kNJ], l2[kNJ];
+  float coef[kNJ], l2[kNJ], slope[kNJ];
 #pragma unroll
   for (int j = 0; j < kNJ; ++j) {
     const int r = 64 * wb + 32 * j + lcol;
     const int t = t0 + r;
     coef[j] = 0.f;
     l2[j] = 0.f;
+    slope[j] = 0.f;
     if (t < N) {
-      coef[j] = targets[t] == ignore_index ? 0.f : dnll[t];
+      if constexpr (AFFINE) {
+        coef[j] = rows.alpha[t];
+        if (rows.beta) slope[j] = rows.beta[t];
+      } else {
+        coef[j] = targets[t] == ignore_index ? 0.f : dnll[t];
+      }
       l2[j] = lse[t] * kLog2e;
     }
   }
@@ -1456,6 +1529,15 @@ void lce_bwd_g_persist_kernel(const bf16_t* __restrict__ H, const bf16_t* __rest
     const int tl = v0 - v_begin;
     auto value = [&](int i, int j, int q) __attribute__((always_inline)) {
       float gv[4];
+      if constexpr (AFFINE) {
+        const uint32_t keep = coef[j] != 0.f || slope[j] != 0.f ? 0xffffffffu : 0u;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const float z = acc[i][j][4 * q + u];
+          gv[u] = fast_exp2(z * rows.scale2 - l2[j]) * __builtin_fmaf(slope[j], z, coef[j]);
+        }
+        return u32x2{pack_bf16x2(gv[0], gv[1]) & keep, pack_bf16x2(gv[2], gv[3]) & keep};
+      }
 #pragma unroll
       for (int u = 0; u < 4; ++u) gv[u] = fast_exp2(acc[i][j][4 * q + u] * kLog2e - l2[j]) * coef[j];
       return u32x2{pack_bf16x2(gv[0], gv[1]), pack_bf16x2(gv[2], gv[3])};
@@ -1490,6 +1572,23 @@ __global__ __launch_bounds__(256) void lce_bwd_g_fix_kernel(
   if (lane == 0) {
     const float p = fast_exp2(z * kLog2e - lse[t] * kLog2e) - 1.f;
     G[(long)t * ldg + (y - v_begin)] = __builtin_bit_cast(bf16_t, (__bf16)(p * dnll[t]));
+  }
+}
+
+// Backward step 1b of an affine gradient, one wave per row of the chunk's G: the columns past the chunk's last vocab row
+// are set to zero, and the row's listed columns (column < 0: none) to their whole gradient, rounded once. No column is listed
+// twice in a row.
+__global__ __launch_bounds__(256) void lce_bwd_g_columns_kernel(const int* __restrict__ columns,
+                                                                const float* __restrict__ value, int k, int N, int vlim,
+                                                                int v_begin, int kc, int ldg, bf16_t* __restrict__ G) {
+  const int lane = threadIdx.x & 63;
+  const int t = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (t >= N) return;
+  bf16_t* row = G + (long)t * ldg;
+  for (int c = vlim - v_begin + lane; c < kc; c += 64) row[c] = 0;
+  for (int i = lane; i < k; i += 64) {
+    const int y = columns[(long)t * k + i];
+    if (y >= v_begin && y < vlim) row[y - v_begin] = __builtin_bit_cast(bf16_t, (__bf16)value[(long)t * k + i]);
   }
 }
 
@@ -2057,12 +2156,11 @@ long lce_fwd_stage_rows_used(long N, long V, long stage_rows) {
   return most;
 }
 
-hipError_t launch_lce_fwd(const LceHead& h, const bf16_t* H, const int64_t* targets, int N, int D, int V,
-                          long long ignore_index, float* nll, float* lse, float* tgt, float* ws,
-                          bf16_t* stage, long stage_rows, hipStream_t stream) {
+// The forward's tiles: partials part_m, part_s (and what STAT adds, else null) [splits][N].
+template <int STAT>
+static hipError_t lce_fwd_tiles(const LceHead& h, const bf16_t* H, int N, int D, int V, float* pm, float* ps, float scale2,
+                                float* pu, float* gmax, int ldg, bf16_t* stage, long stage_rows, hipStream_t stream) {
   const int ns = lce_fwd_nsplit(N, V);
-  float* pm = ws;
-  float* ps = ws + (long)ns * N;
   const int rtiles = (N + kTile - 1) / kTile;
   dim3 block(kThreads);
   if (h.q4 && stage != nullptr && D % kBK == 0) {
@@ -2079,20 +2177,40 @@ hipError_t launch_lce_fwd(const LceHead& h, const bf16_t* H, const int64_t* targ
                          h.wq + r0 * (D >> 3), h.sc + r0 * (D >> 6), h.bi + r0 * (D >> 6), nw, stage);
       hipError_t de = hipGetLastError();
       if (de != hipSuccess) return de;
-      hipLaunchKernelGGL(lce_fwd_kernel<0>, dim3(rtiles * (s1 - s0)), block, 0, stream, H, stage, h.wq, h.sc, h.bi,
-                         N, D, V, ns, s0, s1 - s0, (int)r0, pm, ps);
+      hipLaunchKernelGGL((lce_fwd_kernel<0, STAT>), dim3(rtiles * (s1 - s0)), block, 0, stream, H, stage, h.wq, h.sc, h.bi,
+                         N, D, V, ns, s0, s1 - s0, (int)r0, pm, ps, scale2, pu, gmax, ldg);
       de = hipGetLastError();
       if (de != hipSuccess) return de;
       s0 = s1;
     }
   } else if (h.q4) {
-    hipLaunchKernelGGL(lce_fwd_kernel<1>, dim3(rtiles * ns), block, 0, stream, H, h.w, h.wq, h.sc, h.bi, N, D, V, ns,
-                       0, ns, 0, pm, ps);
+    hipLaunchKernelGGL((lce_fwd_kernel<1, STAT>), dim3(rtiles * ns), block, 0, stream, H, h.w, h.wq, h.sc, h.bi, N, D, V,
+                       ns, 0, ns, 0, pm, ps, scale2, pu, gmax, ldg);
   } else {
-    hipLaunchKernelGGL(lce_fwd_kernel<0>, dim3(rtiles * ns), block, 0, stream, H, h.w, h.wq, h.sc, h.bi, N, D, V, ns,
-                       0, ns, 0, pm, ps);
+    hipLaunchKernelGGL((lce_fwd_kernel<0, STAT>), dim3(rtiles * ns), block, 0, stream, H, h.w, h.wq, h.sc, h.bi, N, D, V,
+                       ns, 0, ns, 0, pm, ps, scale2, pu, gmax, ldg);
   }
-  hipError_t e = hipGetLastError();
+  return hipGetLastError();
+}
+
+hipError_t launch_lce_stats(const LceHead& h, const bf16_t* H, int N, int D, int V, const ScoreStats& st, bf16_t* stage,
+                            long stage_rows, hipStream_t stream) {
+  auto tiles = [&](auto stat) {
+    return lce_fwd_tiles<decltype(stat)::value>(h, H, N, D, V, st.m, st.s, st.scale2, st.u, st.gmax, st.ldg, stage, stage_rows,
+                                                stream);
+  };
+  if (st.gmax) return tiles(std::integral_constant<int, kStatScaled | kStatEntropy | kStatGroups>{});
+  if (st.u) return tiles(std::integral_constant<int, kStatScaled | kStatEntropy>{});
+  return tiles(std::integral_constant<int, kStatScaled>{});
+}
+
+hipError_t launch_lce_fwd(const LceHead& h, const bf16_t* H, const int64_t* targets, int N, int D, int V,
+                          long long ignore_index, float* nll, float* lse, float* tgt, float* ws,
+                          bf16_t* stage, long stage_rows, hipStream_t stream) {
+  const int ns = lce_fwd_nsplit(N, V);
+  float* pm = ws;
+  float* ps = ws + (long)ns * N;
+  hipError_t e = lce_fwd_tiles<0>(h, H, N, D, V, pm, ps, 0.f, nullptr, nullptr, 0, stage, stage_rows, stream);
   if (e != hipSuccess) return e;
   dim3 fgrid((N + 3) / 4), fblock(256);
   if (h.q4) {
@@ -2164,7 +2282,7 @@ hipError_t launch_lce_mean_bwd(const float* d_mean, const float* count, long n, 
 static hipError_t lce_bwd_rows(const LceHead& h, const bf16_t* H, const int64_t* targets, const float* lse,
                                const float* dnll, int N, int D, int V, long long ignore_index, int chunk,
                                bf16_t* dH, bf16_t* dW, bf16_t* Gbuf, float* acc32, float* parts, bf16_t* stage,
-                               hipStream_t stream) {
+                               const AffineGrad* affine, hipStream_t stream) {
   const int rtiles = (N + kTile - 1) / kTile;
   const int dtiles = (D + kTile - 1) / kTile;
   const int nchunks = (V + chunk - 1) / chunk;
@@ -2208,17 +2326,15 @@ static hipError_t lce_bwd_rows(const LceHead& h, const bf16_t* H, const int64_t*
       // One resident workgroup per CU (160 KiB of LDS, all of it, with a dense head; 130 KiB with a 4-bit one).
       const int ns = lce_nsplit(N, (long)ctiles * kTile, 1);
       dim3 pgrid(rtiles * ns);
-      if (gq4) {
-        hipLaunchKernelGGL(lce_bwd_g_persist_kernel<1>, pgrid, block, 0, stream, H, h.w, h.wq, h.sc, h.bi, targets,
-                           lse, dnll, ignore_index, N, D, V, vb, ve, ctiles, ns, ldg, 0, Gbuf);
-      } else {
-        hipLaunchKernelGGL(lce_bwd_g_persist_kernel<0>, pgrid, block, 0, stream, H, gw, h.wq, h.sc, h.bi, targets,
-                           lse, dnll, ignore_index, N, D, V, vb, ve, ctiles, ns, ldg, wrow0, Gbuf);
-      }
+      auto gradient = affine ? (gq4 ? lce_bwd_g_persist_kernel<1, 1> : lce_bwd_g_persist_kernel<0, 1>)
+                             : (gq4 ? lce_bwd_g_persist_kernel<1, 0> : lce_bwd_g_persist_kernel<0, 0>);
+      hipLaunchKernelGGL(gradient, pgrid, block, 0, stream, H, gw, h.wq, h.sc, h.bi, targets, lse, dnll, ignore_index, N, D,
+                         V, vb, ve, ctiles, ns, ldg, wrow0, Gbuf, affine ? affine->rows : AffineRows{});
       hipError_t pe = hipGetLastError();
       if (pe != hipSuccess) return pe;
       dim3 tgrid((N + 3) / 4), tblock(256);
-      if (gq4) {
+      if (affine) {  // (below)
+      } else if (gq4) {
         hipLaunchKernelGGL(lce_bwd_g_fix_kernel<1>, tgrid, tblock, 0, stream, H, h.w, h.wq, h.sc, h.bi, targets,
                            lse, dnll, ignore_index, N, D, V, vb, ve, ctiles * kTile, ldg, 0, Gbuf);
       } else {
@@ -2227,11 +2343,17 @@ static hipError_t lce_bwd_rows(const LceHead& h, const bf16_t* H, const int64_t*
       }
     } else {
       dim3 ggrid(8 * rtiles * ((ctiles + 7) / 8));
-      hipLaunchKernelGGL(lce_bwd_g_kernel, ggrid, block, 0, stream, H, h.w, targets, lse, dnll, ignore_index, N, D, V,
-                         vb, ve, ctiles, ldg, Gbuf);
+      hipLaunchKernelGGL(affine ? lce_bwd_g_kernel<1> : lce_bwd_g_kernel<0>, ggrid, block, 0, stream, H, h.w, targets, lse,
+                         dnll, ignore_index, N, D, V, vb, ve, ctiles, ldg, Gbuf, affine ? affine->rows : AffineRows{});
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
+    if (affine) {
+      hipLaunchKernelGGL(lce_bwd_g_columns_kernel, dim3((N + 3) / 4), dim3(256), 0, stream, affine->columns, affine->value,
+                         affine->k, N, ve, vb, ctiles * kTile, ldg, Gbuf);
+      e = hipGetLastError();
+      if (e != hipSuccess) return e;
+    }
     int mode;
     if (nchunks == 1) mode = 3;
     else if (c == 0) mode = 0;
@@ -2269,7 +2391,8 @@ static hipError_t lce_bwd_rows(const LceHead& h, const bf16_t* H, const int64_t*
     }
     if (dW != nullptr && !h.q4) {
       dim3 wgrid(8 * ctiles * ((dtiles + 7) / 8));
-      hipLaunchKernelGGL(lce_bwd_dw_kernel, wgrid, block, 0, stream, Gbuf, ldg, H, N, D, V, vb, ve, ctiles, dW);
+      const bf16_t* rows = affine ? static_cast<const bf16_t*>(affine->clean) : H;
+      hipLaunchKernelGGL(lce_bwd_dw_kernel, wgrid, block, 0, stream, Gbuf, ldg, rows, N, D, V, vb, ve, ctiles, dW);
       e = hipGetLastError();
       if (e != hipSuccess) return e;
     }
@@ -2283,14 +2406,25 @@ static hipError_t lce_bwd_rows(const LceHead& h, const bf16_t* H, const int64_t*
 hipError_t launch_lce_bwd(const LceHead& h, const bf16_t* H, const int64_t* targets, const float* lse,
                           const float* dnll, int N, int D, int V, long long ignore_index, int chunk, int row_block,
                           bf16_t* dH, bf16_t* dW, bf16_t* Gbuf, float* acc32, float* parts, bf16_t* stage,
-                          hipStream_t stream) {
+                          hipStream_t stream, const AffineGrad* affine) {
   if (dW != nullptr || row_block >= N)
     return lce_bwd_rows(h, H, targets, lse, dnll, N, D, V, ignore_index, chunk, dH, dW, Gbuf, acc32, parts, stage,
-                        stream);
+                        affine, stream);
   for (int r0 = 0; r0 < N; r0 += row_block) {
     const int rows = (N - r0 < row_block) ? N - r0 : row_block;
-    hipError_t e = lce_bwd_rows(h, H + (long)r0 * D, targets + r0, lse + r0, dnll + r0, rows, D, V, ignore_index,
-                                chunk, dH + (long)r0 * D, nullptr, Gbuf, acc32, parts, stage, stream);
+    hipError_t e;
+    if (affine) {
+      AffineGrad a = *affine;
+      a.rows.alpha += r0;
+      if (a.rows.beta) a.rows.beta += r0;
+      a.columns += (long)r0 * a.k;
+      a.value += (long)r0 * a.k;
+      e = lce_bwd_rows(h, H + (long)r0 * D, nullptr, lse + r0, nullptr, rows, D, V, ignore_index, chunk, dH + (long)r0 * D,
+                       nullptr, Gbuf, acc32, parts, stage, &a, stream);
+    } else {
+      e = lce_bwd_rows(h, H + (long)r0 * D, targets + r0, lse + r0, dnll + r0, rows, D, V, ignore_index, chunk,
+                       dH + (long)r0 * D, nullptr, Gbuf, acc32, parts, stage, nullptr, stream);
+    }
     if (e != hipSuccess) return e;
   }
   return hipSuccess;

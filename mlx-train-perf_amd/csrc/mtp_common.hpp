@@ -125,4 +125,15 @@ __device__ __forceinline__ void lse2_merge(float& m, float& s, float mo, float s
   m = mn;
 }
 
+// The same of three: u, the sum of 2^(x - m) (x - m) beside s, moves by s times what the maximum rises.
+__device__ __forceinline__ void lse2_merge(float& m, float& s, float& u, float mo, float so, float uo) {
+  const float mn = fmaxf(m, mo);
+  const float base = (mn == kNegInf) ? 0.f : mn;
+  const float da = m == kNegInf ? 0.f : m - base, db = mo == kNegInf ? 0.f : mo - base;
+  const float fa = fast_exp2(m - base), fb = fast_exp2(mo - base);
+  u = __builtin_fmaf(s, da, u) * fa + __builtin_fmaf(so, db, uo) * fb;
+  s = s * fa + so * fb;
+  m = mn;
+}
+
 }  // namespace mtp

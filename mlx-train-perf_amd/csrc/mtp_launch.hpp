@@ -56,10 +56,40 @@ hipError_t launch_lce_fwd(const LceHead& h, const bf16_t* H, const int64_t* targ
                           long long ignore_index, float* nll, float* lse, float* tgt, float* ws,
                           bf16_t* stage, long stage_rows, hipStream_t stream);
 
+// Token scoring (score_kernels.hip) takes the forward's tiles with more of their statistics. A forward's STAT is a sum of:
+enum { kStatScaled = 1, kStatEntropy = 2, kStatGroups = 4 };
+constexpr int kGroup = 128;  // consecutive logits whose maximum a forward keeps
+struct ScoreStats {
+  float scale2;        // log2(e) / temperature: the partials are of x = z scale2
+  float *m, *s;        // [lce_fwd_nsplit][N] maximum of x, sum of 2^(x - m)
+  float* u;            // the same of 2^(x - m) (x - m), or null
+  float* gmax;         // [N][ldg] the maximum z of each group of kGroup (ldg: an even number of them), or null (with u)
+  int ldg;
+};
+hipError_t launch_lce_stats(const LceHead& h, const bf16_t* H, int N, int D, int V, const ScoreStats& st, bf16_t* stage,
+                            long stage_rows, hipStream_t stream);
+hipError_t launch_lce_target(const LceHead& h, const bf16_t* H, const int64_t* targets, int N, int D, int V, float* tgt,
+                             hipStream_t stream);
+
+// The gradient of a loss of softmax(z / temperature) by the logits z that is p (alpha + beta z) but for k columns a row.
+// Rows with neither factor get zeros, whatever their hidden state holds.
+struct AffineRows {
+  const float *alpha, *beta;  // [N]; beta may be null (0)
+  float scale2;               // log2(e) / temperature
+};
+struct AffineGrad {
+  AffineRows rows;
+  const int* columns;    // [N][k], no column twice in a row; < 0: none
+  const float* value;    // [N][k] the gradient there
+  int k;
+  const void* clean;     // for dW: the hidden states with the rows that get zeros cleared (bf16; fp32 in the fp32 backward)
+};
+
+// affine: that gradient in the place of the loss's (targets, dnll unused).
 hipError_t launch_lce_bwd(const LceHead& h, const bf16_t* H, const int64_t* targets, const float* lse,
                           const float* dnll, int N, int D, int V, long long ignore_index, int chunk, int row_block,
                           bf16_t* dH, bf16_t* dW, bf16_t* Gbuf, float* acc32, float* parts, bf16_t* stage,
-                          hipStream_t stream);
+                          hipStream_t stream, const AffineGrad* affine = nullptr);
 
 hipError_t launch_lce_mean(const float* nll, const int64_t* targets, long n, long long ignore_index, float* mean,
                            float* count, hipStream_t stream);
@@ -131,7 +161,11 @@ hipError_t launch_lce32_fwd(const LceHead32& h, const float* H, const int64_t* t
 // Gbuf: fp32 [N][chunk + 4]; dH fp32 [N][D]; dW (optional, dense head) fp32 [V][D].
 hipError_t launch_lce32_bwd(const LceHead32& h, const float* H, const int64_t* targets, const float* lse,
                             const float* dnll, int N, int D, int V, long long ignore_index, int chunk, float* dH,
-                            float* dW, float* Gbuf, hipStream_t stream);
+                            float* dW, float* Gbuf, hipStream_t stream, const AffineGrad* affine = nullptr);
+hipError_t launch_lce32_stats(const LceHead32& h, const float* H, int N, int D, int V, const ScoreStats& st,
+                              hipStream_t stream);  // [lce32_fwd_nsplit][N]
+hipError_t launch_lce32_target(const LceHead32& h, const float* H, const int64_t* targets, int N, int D, int V, float* tgt,
+                               hipStream_t stream);
 hipError_t launch_attn32_fwd(const AttnShape& sh, const float* q, const float* k, const float* v,
                              const int32_t* seg_start, float* o, float* lse, hipStream_t stream);
 hipError_t launch_attn32_dkv_reduce(const float* part, int ns, long plane, float* dk, float* dv, hipStream_t stream);
@@ -142,6 +176,70 @@ size_t attn32_bwd_workspace(int b, int hq, int hkv, int s, int dh, int nsplit);
 hipError_t launch_attn32_bwd(const AttnShape& sh, const float* q, const float* k, const float* v, const float* o,
                              const float* lse, const float* d_o, const int32_t* seg_start, float* dq, float* dk,
                              float* dv, float* dvec, int nsplit, hipStream_t stream);
+
+// Token scoring and distillation (score_kernels.hip). Logits are recomputed for single tokens and groups of kGroup logits:
+// an entry is a token and what to keep of it, code >= 0: the whole group, to rows[code][kGroup]; code < 0: one logit,
+// column (-1 - code) % kGroup of the group, to picks[(-1 - code) / kGroup]. A tile is up to kGroup entries of one group.
+struct GatherTile {
+  int group, first, count, unused;
+};
+struct GatherPlan {
+  const int2* entries;
+  const GatherTile* tiles;  // [max_tiles], with count 0 past the last
+  int max_tiles;
+  float *rows, *picks;
+};
+hipError_t launch_lce_gather(const LceHead& h, const bf16_t* H, int D, int V, const GatherPlan& p, hipStream_t stream);
+hipError_t launch_lce32_gather(const LceHead32& h, const float* H, int D, int V, const GatherPlan& p, hipStream_t stream);
+
+constexpr long kScoreRows = 16384;   // tokens of one pass of a forward: more are taken in blocks
+constexpr int kScoreTop = 128;       // most alternatives, and longest teacher's list
+constexpr long kScoreVocab = 1 << 21;
+constexpr long kFewTokens = 128;     // tokens up to which a bf16 forward keeps its logits
+constexpr double kTailFloor = 1e-6;  // least mass that the outcomes outside a list count as
+
+// One head of either type; w32 where the hidden states are fp32.
+struct ScoreHead {
+  int f32;
+  LceHead h;
+  LceHead32 h32;
+  const void* hidden;
+};
+struct ScoreShape {
+  long n, d, v;
+  float inv_t;       // 1 / temperature
+  int stage;         // bf16, 4-bit: dequantize the whole head into the workspace first
+};
+struct LogprobsOut {
+  float *logprobs, *entropy, *top_logprobs;
+  int64_t* top_ids;
+  float *lse, *tgt;
+};
+size_t logprobs_fwd_workspace(const ScoreShape& sh, int f32, int q4, int top);
+hipError_t launch_logprobs_fwd(const ScoreHead& h, const ScoreShape& sh, const int64_t* targets, long long ignore_index,
+                               int top, const LogprobsOut& out, void* ws, hipStream_t stream);
+enum { kDistillForward = 0, kDistillReverse = 1, kDistillJsd = 2 };
+struct DistillLoss {
+  int k, kind, renormalize, reduction;
+  double beta;
+};
+struct DistillOut {
+  float *loss, *scale;        // scale [1]: what a row's gradient is multiplied with, 1 / rows that count for a mean
+  float *lse, *rest, *coef;   // [n], [n], [n][k]
+  int* columns;               // [n][k]
+};
+size_t distill_fwd_workspace(const ScoreShape& sh, int f32, int q4, int k);
+hipError_t launch_distill_fwd(const ScoreHead& h, const ScoreShape& sh, const int64_t* ids, const float* teacher,
+                              const uint8_t* mask, const DistillLoss& p, const DistillOut& out, void* ws, hipStream_t stream);
+// What the backwards hand to launch_lce_bwd / launch_lce32_bwd: alpha, beta, columns, value (k = 1).
+hipError_t launch_logprobs_coef(const float* d_logprobs, const float* d_entropy, const int64_t* targets, long long ignore_index,
+                                const float* lse, const float* entropy, const float* tgt, long n, long v, float inv_t,
+                                float* alpha, float* beta, int* columns, float* value, hipStream_t stream);
+hipError_t launch_distill_coef(const float* d_loss, int per_row, const float* scale, const float* rest, const float* coef,
+                               long n, int k, float* alpha, float* value, hipStream_t stream);
+// Hidden states with the rows whose factors are both 0 cleared; row_bytes a multiple of 4.
+hipError_t launch_clean_rows(const void* hidden, const float* alpha, const float* beta, long n, long row_bytes, void* out,
+                             hipStream_t stream);
 
 // Preference and policy losses (preference_kernels.hip).
 enum { kPrefSigmoid = 0, kPrefHinge = 1, kPrefIpo = 2 };

@@ -1,0 +1,1057 @@
+// Token scoring and distillation over a language-model head (gfx950): what a forward keeps of the logits z = H W^T beside or
+// in the place of a target's loss. With x = z / temperature, lse = log sum_v e^x_v and p = e^(x - lse):
+//
+//   scoring (logprobs): log p_y, the entropy lse - sum p x, the `top` largest logits of a token and their log p;
+//   distillation: the divergence of a teacher's list of outcomes (t_k, and the rest as one outcome) from p.
+//
+// The product is the loss's (lce_fwd_kernel, lce32_fwd_kernel): it leaves a maximum and sums per vocab split and, for the
+// alternatives, the maximum of every group of kGroup consecutive logits. The `top` largest logits of a row lie in the
+// groups with the `top` largest maxima (a logit outside them has `top` at least as large ahead of it; equal maxima go to the
+// lower group, so equal logits to the lower index). So: choose those groups, form their logits again (a product over
+// the tokens that want each group: top kGroup / V of the first one, 0.7% for 8 of 151936), choose among them. The logits of a
+// teacher's list are formed the same way, one per entry. The product's k order is the forward's, so a logit has the same bits
+// in both: what is left of 1 after a list's probabilities is exact to fp32 and not to two roundings of a large logit.
+//
+// Up to kFewTokens tokens the logits themselves are kept in the workspace (lce_few_kernel), which leaves two launches.
+#include <math.h>
+
+#include <type_traits>
+
+#include "score_gather.hpp"
+
+namespace mtp {
+namespace {
+
+// ------------------------------------------------------------------------------------------
+// Choice of the K largest keys.
+// ------------------------------------------------------------------------------------------
+constexpr int kPick = 256;  // threads
+
+// fp32 as an unsigned number of the same order; -0 as 0.
+__device__ __forceinline__ uint32_t order_key(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
+
+struct PickScratch {
+  int count[2][kPick / 64];
+  int sum[kPick / 64];
+};
+
+// Sum over the workgroup's threads; every thread gets it.
+__device__ __forceinline__ int block_sum(int mine_wave, PickScratch& s, int step) {
+  const int w = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) s.count[step & 1][w] = mine_wave;
+  __syncthreads();
+  int n = 0;
+#pragma unroll
+  for (int i = 0; i < kPick / 64; ++i) n += s.count[step & 1][i];
+  return n;
+}
+// Sum over the threads before this one.
+__device__ __forceinline__ int block_before(int mine, PickScratch& s) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int run = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int up = __shfl_up(run, o, 64);
+    if (lane >= o) run += up;
+  }
+  __syncthreads();
+  if (lane == 63) s.sum[w] = run;
+  __syncthreads();
+  int before = run - mine;
+  for (int i = 0; i < w; ++i) before += s.sum[i];
+  return before;
+}
+
+// The positions, ascending, of the K largest of M >= K keys in LDS; equal keys go to the lower position. The K-th largest is
+// found bit by bit, 32 counts over the keys, so the time does not depend on their order. Ends with a barrier.
+__device__ __forceinline__ void pick_largest(const uint32_t* key, int M, int K, int* at, PickScratch& s) {
+  const int tid = threadIdx.x;
+  uint32_t least = 0;
+  for (int b = 31; b >= 0; --b) {
+    const uint32_t c = least | (1u << b);
+    int n = 0;
+    for (int base = 0; base < M; base += kPick) {
+      const int i = base + tid;
+      n += __popcll(__ballot(i < M && key[i] >= c));
+    }
+    if (block_sum(n, s, b) >= K) least = c;
+  }
+  int above = 0;
+  for (int base = 0; base < M; base += kPick) {
+    const int i = base + tid;
+    above += __popcll(__ballot(i < M && key[i] > least));
+  }
+  const int equal = K - block_sum(above, s, 1);  // how many of the keys that equal the K-th are taken
+  const int per = (M + kPick - 1) / kPick, lo = tid * per < M ? tid * per : M, hi = lo + per < M ? lo + per : M;
+  int mine = 0;
+  for (int i = lo; i < hi; ++i) mine += key[i] == least;
+  int seen = block_before(mine, s);
+  int taken = 0, rank = seen;
+  for (int i = lo; i < hi; ++i) {
+    if (key[i] > least) ++taken;
+    else if (key[i] == least) taken += rank++ < equal;
+  }
+  int to = block_before(taken, s);
+  for (int i = lo; i < hi; ++i)
+    if (key[i] > least || (key[i] == least && seen++ < equal)) at[to++] = i;
+  __syncthreads();
+}
+
+// ------------------------------------------------------------------------------------------
+// Few tokens (bf16 hidden states): the logits [N][ldz] in fp32, and per group of kGroup of them their maximum and, relative to
+// it, the two sums. The head is read once and bounds it; a workgroup takes one group: 4 waves of 32 vocab rows, the rows'
+// fragments straight from memory to registers a slab of 128 k ahead (8 KiB a wave in flight), the tokens' slab (NB blocks of 32)
+// through LDS, one barrier a slab.
+// ------------------------------------------------------------------------------------------
+constexpr int kSlab = 128;
+
+template <int Q4, int NB>
+__global__ __launch_bounds__(256) void lce_few_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
+                                                      const uint32_t* __restrict__ Wq, const bf16_t* __restrict__ Sc,
+                                                      const bf16_t* __restrict__ Bi, int N, int D, int V, float c2, int ldz,
+                                                      float* __restrict__ Z, float* __restrict__ gmax,
+                                                      float* __restrict__ gs, float* __restrict__ gu) {
+  constexpr int kTok = 32 * NB, kBytes = kTok * 2 * kSlab;  // a slab: two tiles of 64 k, 128 bytes a row
+  __shared__ __attribute__((aligned(16))) char lds[2 * kBytes];
+  __shared__ float xm[4][kTok], xs[4][kTok], xu[4][kTok];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, half = lane >> 5, col = lane & 31;
+  const int v0 = blockIdx.x * kGroup, v = v0 + 32 * w + col;
+  const int vr = v < V ? v : V - 1;  // rows past the end: their logits are replaced
+  const int slabs = (D + kSlab - 1) / kSlab;
+
+  // Fragment j of a slab contracts k chunk (8 values) `2 j + half` of it; with packed words 8 half + j, so that a lane's words
+  // lie together.
+  auto chunk = [&](int j) { return Q4 ? 8 * half + j : 2 * j + half; };
+  u32x4 wa[Q4 ? 2 : 8];
+  uint32_t sb = 0;
+  auto load_head = [&](int slab) {
+    if constexpr (Q4) {
+      const int k = slab * kSlab + 64 * half;
+      if (k < D) {
+        const u32x4* q = reinterpret_cast<const u32x4*>(Wq + (long)vr * (D >> 3) + (k >> 3));
+        wa[0] = q[0];
+        wa[1] = q[1];
+        const long g = (long)vr * (D >> 6) + (k >> 6);
+        sb = (uint32_t)Sc[g] | (uint32_t)Bi[g] << 16;
+      } else {
+        wa[0] = wa[1] = zero4();
+        sb = 0;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int k = slab * kSlab + 8 * chunk(j);
+        wa[j] = k < D ? *reinterpret_cast<const u32x4*>(W + (long)vr * D + k) : zero4();
+      }
+    }
+  };
+  u32x4 ha[2 * NB];
+  auto load_tokens = [&](int slab) {
+#pragma unroll
+    for (int p = 0; p < 2 * NB; ++p) {
+      const int id = tid + 256 * p, row = id >> 4, k = slab * kSlab + 8 * (id & 15);
+      ha[p] = row < N && k < D ? *reinterpret_cast<const u32x4*>(H + (long)row * D + k) : zero4();
+    }
+  };
+  auto put_tokens = [&](char* dst) {
+#pragma unroll
+    for (int p = 0; p < 2 * NB; ++p) {
+      const int id = tid + 256 * p, row = id >> 4, c = id & 15;
+      lds_write16(dst + (c >> 3) * (kTok * 128), lds_off(row, c & 7), ha[p]);
+    }
+  };
+
+  f32x16 acc[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[b][r] = 0.f;
+  load_tokens(0);
+  load_head(0);
+  put_tokens(lds);
+  __syncthreads();
+  for (int s = 0; s < slabs; ++s) {
+    const char* cur = lds + (s & 1) * kBytes;
+    bf16x8 a[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if constexpr (Q4) a[j] = as_bf16x8(dequant8(wa[j >> 2][j & 3], bf16lo(sb), bf16hi(sb)));
+      else a[j] = as_bf16x8(wa[j]);
+    }
+    if (s + 1 < slabs) {
+      load_tokens(s + 1);
+      load_head(s + 1);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int c = chunk(j);
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        const bf16x8 t = as_bf16x8(lds_read16(cur + (c >> 3) * (kTok * 128), lds_off(32 * b + col, c & 7)));
+        acc[b] = mfma32(a[j], t, acc[b]);
+      }
+    }
+    if (s + 1 < slabs) put_tokens(lds + ((s + 1) & 1) * kBytes);
+    __syncthreads();
+  }
+
+  // acc[b][r]: vocab row 32 w + 8 (r / 4) + 4 half + r % 4 of the group, token 32 b + col.
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const int t = 32 * b + col;
+    float top = kNegInf;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int row = 32 * w + 8 * q + 4 * half;
+      f32x4 z;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        z[u] = v0 + row + u < V ? acc[b][4 * q + u] : kNegInf;
+        top = fmaxf(top, z[u]);
+      }
+      if (t < N) *reinterpret_cast<f32x4*>(Z + (long)t * ldz + v0 + row) = z;
+    }
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const float base = top == kNegInf ? 0.f : top * c2;
+    float s = 0.f, u = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      if (v0 + 32 * w + 8 * (r >> 2) + 4 * half + (r & 3) < V) {
+        const float x = __builtin_fmaf(acc[b][r], c2, -base), e = fast_exp2(x);
+        s += e;
+        u = __builtin_fmaf(e, x, u);
+      }
+    s += __shfl_xor(s, 32, 64);
+    u += __shfl_xor(u, 32, 64);
+    if (half == 0) {
+      xm[w][t] = top;
+      xs[w][t] = s;
+      xu[w][t] = u;
+    }
+  }
+  __syncthreads();
+  for (int t = tid; t < N; t += 256) {
+    float top = kNegInf;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = fmaxf(top, xm[i][t]);
+    float m = kNegInf, s = 0.f, u = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) lse2_merge(m, s, u, xm[i][t] == kNegInf ? kNegInf : xm[i][t] * c2, xs[i][t], xu[i][t]);
+    const long o = (long)t * gridDim.x + blockIdx.x;
+    gmax[o] = top;
+    gs[o] = s;
+    gu[o] = u;
+  }
+}
+
+// ------------------------------------------------------------------------------------------
+// The logits of a gather (GatherPlan): C[v][entry] = W_v . H_token, 128 x 128 a workgroup (4 waves of 64 x 64), 64-deep stages
+// through registers, a stage ahead. Bound by the hidden rows it fetches again for every entry (2 D bytes each, out of L2 and
+// the last-level cache).
+// ------------------------------------------------------------------------------------------
+template <int Q4>
+__global__ __launch_bounds__(256) void lce_gather_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
+                                                         const uint32_t* __restrict__ Wq, const bf16_t* __restrict__ Sc,
+                                                         const bf16_t* __restrict__ Bi, int D, int V, GatherPlan plan) {
+  __shared__ __attribute__((aligned(16))) char lds[2][2][16384];
+  const GatherTile tile = plan.tiles[blockIdx.x];
+  if (tile.count == 0) return;
+  const int2* entries = plan.entries + tile.first;
+  const int v0 = tile.group * kGroup;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, half = lane >> 5, col = lane & 31;
+  const int wa = w & 1, wb = w >> 1, c = tid & 7;
+  const int nk = (D + 63) / 64;
+
+  // Thread: 16-byte chunk c of rows tid / 8 + 32 p of both operands.
+  long hrow[4];
+  int vrow[4];
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const int r = (tid >> 3) + 32 * p;
+    hrow[p] = r < tile.count ? (long)entries[r].x * D : -1;
+    vrow[p] = v0 + r < V ? v0 + r : V - 1;  // rows past the end: their logits are replaced
+  }
+  u32x4 a[4], b[4];
+  auto load = [&](int kt) {
+    const int k = 64 * kt + 8 * c;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      b[p] = hrow[p] >= 0 && k < D ? *reinterpret_cast<const u32x4*>(H + hrow[p] + k) : zero4();
+      if constexpr (Q4) {
+        const long g = (long)vrow[p] * (D >> 6) + kt;
+        a[p] = dequant8(Wq[(long)vrow[p] * (D >> 3) + (k >> 3)], bf16_to_f32(Sc[g]), bf16_to_f32(Bi[g]));
+      } else {
+        a[p] = k < D ? *reinterpret_cast<const u32x4*>(W + (long)vrow[p] * D + k) : zero4();
+      }
+    }
+  };
+  auto put = [&](int s) {
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const int r = (tid >> 3) + 32 * p;
+      lds_write16(lds[s][0], lds_off(r, c), a[p]);
+      lds_write16(lds[s][1], lds_off(r, c), b[p]);
+    }
+  };
+  f32x16 acc[2][2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+  load(0);
+  put(0);
+  __syncthreads();
+  for (int kt = 0; kt < nk; ++kt) {
+    const int cur = kt & 1;
+    if (kt + 1 < nk) load(kt + 1);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      bf16x8 x[2], y[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) x[i] = as_bf16x8(lds_read16(lds[cur][0], lds_off(64 * wa + 32 * i + col, 2 * ks + half)));
+#pragma unroll
+      for (int j = 0; j < 2; ++j) y[j] = as_bf16x8(lds_read16(lds[cur][1], lds_off(64 * wb + 32 * j + col, 2 * ks + half)));
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = mfma32(x[i], y[j], acc[i][j]);
+    }
+    if (kt + 1 < nk) put(cur ^ 1);
+    __syncthreads();
+  }
+  store_gathered<2, 2>(acc, plan, entries, tile.count, V - v0, 64 * wa, 64 * wb, lane);
+}
+
+// ------------------------------------------------------------------------------------------
+// Plan of a gather: entries counted by group, dealt into runs of one group each, the runs cut into tiles. The order of a group's
+// entries is that of the atomics and decides nothing: each is a column of its own.
+// ------------------------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void zero_counts_kernel(int* __restrict__ counts, int n) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < n) counts[i] = 0;
+}
+
+// counts -> the first entry of each group (in its place), and the tiles.
+__global__ __launch_bounds__(1024) void gather_tiles_kernel(int* __restrict__ counts, int groups, GatherTile* __restrict__ tiles,
+                                                            int max_tiles) {
+  __shared__ int sum_e[16], sum_t[16];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int per = (groups + 1023) / 1024, lo = tid * per, hi = lo + per < groups ? lo + per : groups;
+  int e = 0, t = 0;
+  for (int g = lo; g < hi; ++g) {
+    e += counts[g];
+    t += (counts[g] + kGroup - 1) / kGroup;
+  }
+  int re = e, rt = t;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int ue = __shfl_up(re, o, 64), ut = __shfl_up(rt, o, 64);
+    if (lane >= o) {
+      re += ue;
+      rt += ut;
+    }
+  }
+  if (lane == 63) {
+    sum_e[w] = re;
+    sum_t[w] = rt;
+  }
+  __syncthreads();
+  int first = re - e, tile = rt - t, all = 0;
+  for (int i = 0; i < 16; ++i) {
+    if (i < w) {
+      first += sum_e[i];
+      tile += sum_t[i];
+    }
+    all += sum_t[i];
+  }
+  for (int g = lo; g < hi; ++g) {
+    const int n = counts[g];
+    counts[g] = first;
+    for (int k = 0; k < n; k += kGroup) tiles[tile++] = GatherTile{g, first + k, n - k < kGroup ? n - k : kGroup, 0};
+    first += n;
+  }
+  for (int i = all + tid; i < max_tiles; i += 1024) tiles[i] = GatherTile{0, 0, 0, 0};
+}
+
+// groups [N][k] (a row's are its chosen ones; < 0: none) to entries that keep whole groups.
+__global__ __launch_bounds__(256) void gather_groups_kernel(const int* __restrict__ groups, long n, int k,
+                                                            int* __restrict__ cursor, int2* __restrict__ entries) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n || groups[i] < 0) return;
+  entries[atomicAdd(&cursor[groups[i]], 1)] = int2{(int)(i / k), (int)i};
+}
+
+// (Loaded and decided apart from the slot's own conditions: with the mask's test among them the compiler dropped the id of
+// every slot of a masked row that counts.)
+__device__ __forceinline__ bool row_counts_by(const uint8_t* mask, long row) { return (mask ? mask[row] : (uint8_t)1) != 0; }
+__device__ __forceinline__ bool listed(long long id, float lp, bool counts, long V) {
+  return (id >= 0) & (id < V) & (lp != kNegInf) & counts;
+}
+// A teacher's list [N][k]: counts (COUNT) and entries of single logits.
+template <bool COUNT>
+__global__ __launch_bounds__(256) void gather_list_kernel(const int64_t* __restrict__ ids, const float* __restrict__ teacher,
+                                                          const uint8_t* __restrict__ mask, long n, int k, long V,
+                                                          int* __restrict__ cursor, int2* __restrict__ entries) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const long long id = ids[i];
+  if (!listed(id, teacher[i], row_counts_by(mask, i / k), V)) return;
+  const int at = atomicAdd(&cursor[id / kGroup], 1);
+  if constexpr (!COUNT) entries[at] = int2{(int)(i / k), (int)(-1 - (i * kGroup + id % kGroup))};
+}
+
+// ------------------------------------------------------------------------------------------
+// Scoring, per token: the statistics of its row, the target's log probability, the groups to look into (and, where the logits
+// were kept, the alternatives themselves). One workgroup a token.
+// ------------------------------------------------------------------------------------------
+// Partials of one row: value i at base[i * stride]. m: of x in the log2 domain, or (few tokens) of z, times c2.
+struct RowParts {
+  const float *m, *s, *u;
+  int count;
+  long stride, row;  // floats between partials, and between rows
+  float m_scale;
+};
+
+// (m, s, u) of a row, in every thread of the workgroup.
+__device__ __forceinline__ void merge_row(const RowParts& p, long t, float& m, float& s, float& u, float (&x)[3][kPick / 64]) {
+  m = kNegInf;
+  s = u = 0.f;
+  const float *pm = p.m + t * p.row, *ps = p.s + t * p.row, *pu = p.u + t * p.row;
+  for (int i = threadIdx.x; i < p.count; i += kPick) {
+    const float mi = pm[i * p.stride];
+    lse2_merge(m, s, u, mi == kNegInf ? kNegInf : mi * p.m_scale, ps[i * p.stride], pu[i * p.stride]);
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    const float mo = __shfl_xor(m, o, 64), so = __shfl_xor(s, o, 64), uo = __shfl_xor(u, o, 64);
+    lse2_merge(m, s, u, mo, so, uo);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    x[0][threadIdx.x >> 6] = m;
+    x[1][threadIdx.x >> 6] = s;
+    x[2][threadIdx.x >> 6] = u;
+  }
+  __syncthreads();
+  m = x[0][0];
+  s = x[1][0];
+  u = x[2][0];
+#pragma unroll
+  for (int i = 1; i < kPick / 64; ++i) lse2_merge(m, s, u, x[0][i], x[1][i], x[2][i]);
+}
+
+// The K largest of a row's candidate logits, M = ngroups kGroup of them in LDS as keys, ordered, with their log
+// probabilities. The groups ascend, so positions ascend with the index. A target among them takes its logit from here.
+__device__ __forceinline__ void write_top(const uint32_t* key, const int* group, int ngroups, int K, int V, float inv_t, float lse,
+                                          long t, long long target, const LogprobsOut& out, int* at, PickScratch& s) {
+  pick_largest(key, ngroups * kGroup, K, at, s);
+  const int i = threadIdx.x;
+  if (i < K) {
+    const uint32_t mine = key[at[i]];
+    int rank = 0;
+    for (int j = 0; j < K; ++j) {
+      const uint32_t other = key[at[j]];
+      rank += other > mine || (other == mine && j < i);
+    }
+    const int id = group[at[i] / kGroup] * kGroup + at[i] % kGroup;
+    const float z = key_value(mine), lp = z * inv_t - lse;
+    out.top_ids[t * K + rank] = id < V ? id : -1;
+    out.top_logprobs[t * K + rank] = lp;
+    if (id == target) {
+      out.tgt[t] = z;
+      out.logprobs[t] = lp;
+    }
+  }
+}
+
+constexpr int kMaxGroups = (int)(kScoreVocab / kGroup);
+
+// KEPT: the logits Z [N][ldz] of few tokens. MG, MC: room for a row's groups and candidates (0: none).
+template <bool KEPT, int MG, int MC>
+__global__ __launch_bounds__(kPick) void score_rows_kernel(RowParts parts, const float* __restrict__ gmax, int ngroups, int ldg,
+                                                           const float* __restrict__ Z, long ldz,
+                                                           const int64_t* __restrict__ targets, long long ignore_index, int V,
+                                                           float inv_t, int K, int take, LogprobsOut out,
+                                                           int* __restrict__ groups, int* __restrict__ counts) {
+  __shared__ float x[3][kPick / 64];
+  __shared__ PickScratch scratch;
+  __shared__ uint32_t key[MG > MC ? MG : MC > 0 ? MC : 1];
+  __shared__ int group[kScoreTop], at[kScoreTop];
+  const long t = blockIdx.x;
+  const int tid = threadIdx.x;
+  const long long y = targets ? targets[t] : 0;
+  const bool dead = targets && y == ignore_index;
+  if (dead) {
+    for (int i = tid; i < K; i += kPick) {
+      out.top_ids[t * K + i] = -1;
+      out.top_logprobs[t * K + i] = kNegInf;
+      if (!KEPT && i < take) groups[t * take + i] = -1;
+    }
+    if (tid == 0) {
+      out.entropy[t] = out.lse[t] = 0.f;
+      if (targets) out.logprobs[t] = out.tgt[t] = 0.f;
+    }
+    return;
+  }
+  float m, s, u;
+  merge_row(parts, t, m, s, u, x);
+  const float lse = (m + fast_log2(s)) * kLn2;
+  const bool in = y >= 0 && y < V;
+  if (tid == 0) {
+    out.lse[t] = lse;
+    out.entropy[t] = (fast_log2(s) - u / s) * kLn2;
+    if (targets) {
+      const float z = KEPT ? (in ? Z[t * ldz + y] : 0.f) : out.tgt[t];
+      out.tgt[t] = z;
+      out.logprobs[t] = in ? z * inv_t - lse : -lse;
+    }
+  }
+  if constexpr (MG > 0) {
+    for (int i = tid; i < ngroups; i += kPick) key[i] = order_key(gmax[t * ldg + i]);
+    __syncthreads();
+    pick_largest(key, ngroups, take, group, scratch);
+    if constexpr (KEPT) {
+      for (int i = tid; i < take * kGroup; i += kPick)
+        key[i] = order_key(Z[t * ldz + (long)group[i / kGroup] * kGroup + i % kGroup]);
+      __syncthreads();
+      write_top(key, group, take, K, V, inv_t, lse, t, targets ? y : -1, out, at, scratch);
+    } else if (tid < take) {
+      groups[t * take + tid] = group[tid];
+      atomicAdd(&counts[group[tid]], 1);
+    }
+  }
+}
+
+// After the gather: the alternatives from the chosen groups' logits [N][take][kGroup].
+template <int MC>
+__global__ __launch_bounds__(kPick) void score_top_kernel(const float* __restrict__ rows, const int* __restrict__ groups,
+                                                          const int64_t* __restrict__ targets, int V, float inv_t, int K,
+                                                          int take, LogprobsOut out) {
+  __shared__ PickScratch scratch;
+  __shared__ uint32_t key[MC];
+  __shared__ int group[kScoreTop], at[kScoreTop];
+  const long t = blockIdx.x;
+  const int tid = threadIdx.x;
+  if (groups[t * take] < 0) return;  // an ignored token
+  for (int i = tid; i < take; i += kPick) group[i] = groups[t * take + i];
+  for (int i = tid; i < take * kGroup; i += kPick) key[i] = order_key(rows[t * take * kGroup + i]);
+  __syncthreads();
+  write_top(key, group, take, K, V, inv_t, out.lse[t], t, targets ? targets[t] : -1, out, at, scratch);
+}
+
+// ------------------------------------------------------------------------------------------
+// Distillation, one wave a token. With q_k = p at the list's ids, R = 1 - sum q, t_k and T = 1 - sum t the teacher's, and
+// f = dL/dq but for a constant (f_R for the rest),
+//   forward  sum t log(t / q) + T log(T / R):        f = -t / q,              f_R = -T / R
+//   reverse  sum q log(q / t) + R log(R / T):        f = log(q / t),          f_R = log(R / T)
+//   jsd      b KL(t | m) + (1 - b) KL(q | m), m = b t + (1 - b) q:  f = (1 - b) log(q / m), f_R = (1 - b) log(R / m_R)
+// the gradient by a logit is p (f_R - F) off the list and q (f - F) on it, F = sum q f + R f_R. R and T (but in F) are at least
+// kTailFloor. All of it in 64 bits: what the list leaves of 1 is a difference, and the products above are what take the time.
+// ------------------------------------------------------------------------------------------
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+__device__ __forceinline__ double wave_max64(double v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v = fmax(v, __shfl_xor(v, o, 64));
+  return v;
+}
+__device__ __forceinline__ double log_add(double a, double b) {
+  const double hi = fmax(a, b);
+  return hi + log1p(exp(fmin(a, b) - hi));
+}
+
+constexpr int kPerLane = kScoreTop / 64;
+constexpr float kLeast = 1.17549435e-38f;
+
+template <int KIND>
+__global__ __launch_bounds__(256) void distill_rows_kernel(RowParts parts, const float* __restrict__ picks,
+                                                           const float* __restrict__ Z, long ldz,
+                                                           const int64_t* __restrict__ ids, const float* __restrict__ teacher,
+                                                           const uint8_t* __restrict__ mask, long n, long V, float inv_t, int k,
+                                                           int renormalize, double beta, float* __restrict__ row_loss,
+                                                           int* __restrict__ row_counts, float* __restrict__ lse_out,
+                                                           float* __restrict__ rest_out, float* __restrict__ coef,
+                                                           int* __restrict__ columns) {
+  const int lane = threadIdx.x & 63;
+  const long t = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (t >= n) return;
+  // Which slots hold an outcome: a column of its own that the teacher gives something to.
+  int id[kPerLane];
+  float lp[kPerLane];
+  bool on[kPerLane];
+  const bool counts = row_counts_by(mask, t);
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) {
+    const int s = lane + 64 * i;
+    const long long y = s < k ? ids[t * k + s] : -1;
+    const float l = s < k ? teacher[t * k + s] : 0.f;
+    on[i] = listed(y, l, counts, V);
+    id[i] = on[i] ? (int)y : -1;
+    lp[i] = on[i] ? l : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i)
+    for (int j = 0; j < 64 && 64 * i + j < k; ++j) {  // a column that an earlier slot has is empty here
+      const int other = __shfl(id[i], j, 64);
+#pragma unroll
+      for (int o = 0; o < kPerLane; ++o)
+        if (64 * i + j < lane + 64 * o && other >= 0 && other == id[o]) on[o] = false;
+    }
+  bool some = false;
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) some |= __any(on[i]);
+  if (!some) {
+    for (int s = lane; s < k; s += 64) {
+      coef[t * k + s] = 0.f;
+      columns[t * k + s] = -1;
+    }
+    if (lane == 0) {
+      row_loss[t] = lse_out[t] = rest_out[t] = 0.f;
+      row_counts[t] = 0;
+    }
+    return;
+  }
+  float m = kNegInf, s = 0.f;
+  for (int i = lane; i < parts.count; i += 64) {
+    const float mi = parts.m[t * parts.row + i * parts.stride];
+    lse2_merge(m, s, mi == kNegInf ? kNegInf : mi * parts.m_scale, parts.s[t * parts.row + i * parts.stride]);
+  }
+  const float top = wave_max(m);
+  const double total = wave_sum64((double)s * (double)fast_exp2(m - top));
+  const double lse = ((double)top + log2(total)) * 0.6931471805599453;
+
+  double lq[kPerLane], lt[kPerLane], q[kPerLane], p[kPerLane];
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) {
+    const long o = t * k + lane + 64 * i;
+    float z = 0.f;
+    if (id[i] >= 0) z = Z ? Z[t * ldz + id[i]] : picks[o];
+    lq[i] = on[i] ? (double)z * (double)inv_t - lse : 0.0;
+    q[i] = on[i] ? exp(lq[i]) : 0.0;
+    lt[i] = (double)lp[i];
+  }
+  if (renormalize) {
+    double hi = -HUGE_VAL, sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+      lt[i] *= (double)inv_t;
+      if (on[i]) hi = fmax(hi, lt[i]);
+    }
+    hi = wave_max64(hi);
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i)
+      if (on[i]) sum += exp(lt[i] - hi);
+    hi += log(wave_sum64(sum));
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) lt[i] -= hi;
+  }
+  double sq = 0.0, st = 0.0;
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) {
+    p[i] = on[i] ? exp(lt[i]) : 0.0;
+    sq += q[i];
+    st += p[i];
+  }
+  const double left = 1.0 - wave_sum64(sq);
+  const double rq = fmax(left, kTailFloor), rt = renormalize ? 0.0 : fmax(1.0 - wave_sum64(st), kTailFloor);
+  double loss = 0.0, qf[kPerLane], sqf = 0.0, frest;
+  if constexpr (KIND == kDistillForward) {
+    frest = -rt / rq;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+      if (on[i]) loss += p[i] * (lt[i] - lq[i]);
+      qf[i] = -p[i];
+      sqf += qf[i];
+    }
+    loss = wave_sum64(loss) + (rt > 0.0 ? rt * log(rt / rq) : 0.0);
+  } else if constexpr (KIND == kDistillReverse) {
+    frest = log(rq / rt);
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+      qf[i] = on[i] ? q[i] * (lq[i] - lt[i]) : 0.0;
+      sqf += qf[i];
+    }
+    loss = wave_sum64(sqf) + rq * frest;
+  } else {
+    const double a = log(beta), b = log1p(-beta), rm = beta * rt + (1.0 - beta) * rq;
+    frest = (1.0 - beta) * log(rq / rm);
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+      qf[i] = 0.0;
+      if (on[i]) {
+        const double lm = log_add(a + lt[i], b + lq[i]);
+        qf[i] = (1.0 - beta) * q[i] * (lq[i] - lm);
+        loss += beta * p[i] * (lt[i] - lm);
+      }
+      sqf += qf[i];
+    }
+    loss = wave_sum64(loss + sqf) + rq * frest + (rt > 0.0 ? beta * rt * log(rt / rm) : 0.0);
+  }
+  const double mean = wave_sum64(sqf) + left * frest;
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) {
+    const int slot = lane + 64 * i;
+    if (slot < k) {
+      coef[t * k + slot] = on[i] ? (float)((qf[i] - q[i] * mean) * (double)inv_t) : 0.f;
+      columns[t * k + slot] = on[i] ? id[i] : -1;
+    }
+  }
+  if (lane == 0) {
+    row_loss[t] = (float)loss;
+    row_counts[t] = 1;
+    lse_out[t] = (float)lse;
+    const float rest = (float)((frest - mean) * (double)inv_t);
+    rest_out[t] = rest == 0.f ? kLeast : rest;  // 0 is a row that gets no gradient
+  }
+}
+
+// The rows' losses as one number, summed in 64 bits in a fixed order, and what a row's gradient is multiplied with. One
+// workgroup.
+__global__ __launch_bounds__(1024) void distill_reduce_kernel(const float* __restrict__ row_loss,
+                                                              const int* __restrict__ row_counts, long n, int mean,
+                                                              float* __restrict__ loss, float* __restrict__ scale) {
+  __shared__ double sums[16];
+  __shared__ long counts[16];
+  double s = 0.0;
+  long c = 0;
+  for (long i = threadIdx.x; i < n; i += 1024) {
+    s += (double)row_loss[i];
+    c += row_counts[i];
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    s += __shfl_xor(s, o, 64);
+    c += __shfl_xor(c, o, 64);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    sums[threadIdx.x >> 6] = s;
+    counts[threadIdx.x >> 6] = c;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 16; ++w) {
+      s += sums[w];
+      c += counts[w];
+    }
+    const double by = mean ? 1.0 / (double)(c > 1 ? c : 1) : 1.0;
+    *loss = (float)(s * by);
+    *scale = (float)by;
+  }
+}
+
+// ------------------------------------------------------------------------------------------
+// Factors of the backward's gradient tiles (AffineGrad).
+// ------------------------------------------------------------------------------------------
+// Scoring: dL/dz = (a [v = y] - p (a + b (log p + entropy))) / temperature, a and b the two gradients.
+__global__ __launch_bounds__(256) void logprobs_coef_kernel(const float* __restrict__ d_logprobs,
+                                                            const float* __restrict__ d_entropy,
+                                                            const int64_t* __restrict__ targets, long long ignore_index,
+                                                            const float* __restrict__ lse, const float* __restrict__ entropy,
+                                                            const float* __restrict__ tgt, long n, long V, float inv_t,
+                                                            float* __restrict__ alpha, float* __restrict__ beta,
+                                                            int* __restrict__ columns, float* __restrict__ value) {
+  const long t = (long)blockIdx.x * 256 + threadIdx.x;
+  if (t >= n) return;
+  const long long y = targets ? targets[t] : -1;
+  const bool dead = targets && y == ignore_index, in = !dead && targets && y >= 0 && y < V;
+  const float a = !dead && d_logprobs ? d_logprobs[t] : 0.f, b = !dead && d_entropy ? d_entropy[t] : 0.f;
+  const float up = lse[t] - entropy[t], l = in ? tgt[t] * inv_t - lse[t] : 0.f;
+  alpha[t] = (b * up - a) * inv_t;
+  beta[t] = -b * inv_t * inv_t;
+  columns[t] = in ? (int)y : -1;
+  value[t] = in ? (-a * expm1f(l) - b * expf(l) * (l + entropy[t])) * inv_t : 0.f;
+}
+
+__global__ __launch_bounds__(256) void distill_coef_kernel(const float* __restrict__ d_loss, int per_row,
+                                                           const float* __restrict__ scale, const float* __restrict__ rest,
+                                                           const float* __restrict__ coef, long n, int k,
+                                                           float* __restrict__ alpha, float* __restrict__ value) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n * k) return;
+  const long t = i / k;
+  const float ct = per_row ? d_loss[t] : d_loss[0] * *scale;
+  const float c = coef[i];
+  value[i] = c == 0.f ? 0.f : c * ct;
+  if (i == t * k) {
+    const float a = rest[t] == 0.f ? 0.f : rest[t] * ct;
+    alpha[t] = a == 0.f && rest[t] != 0.f && ct != 0.f ? kLeast : a;
+  }
+}
+
+// A row whose factors are both 0 gets no gradient and may hold anything, NaN too: in dW = G^T H its zeros would meet that.
+__global__ __launch_bounds__(256) void clean_rows_kernel(const uint32_t* __restrict__ h, const float* __restrict__ alpha,
+                                                         const float* __restrict__ beta, long row_words,
+                                                         uint32_t* __restrict__ out) {
+  const long t = blockIdx.x;
+  const bool live = alpha[t] != 0.f || (beta && beta[t] != 0.f);
+  for (long i = threadIdx.x; i < row_words; i += 256) out[t * row_words + i] = live ? h[t * row_words + i] : 0u;
+}
+
+// ------------------------------------------------------------------------------------------
+// Host side.
+// ------------------------------------------------------------------------------------------
+long ceil_div(long a, long b) { return (a + b - 1) / b; }
+int groups_of(long v) { return (int)ceil_div(v, kGroup); }
+
+// Room in a workspace, in order; every part starts at a 256-byte boundary.
+struct Carver {
+  char* base;
+  size_t used = 0;
+  template <class T>
+  T* take(long count) {
+    T* p = reinterpret_cast<T*>(base + used);
+    used += ((size_t)count * sizeof(T) + 255) / 256 * 256;
+    return p;
+  }
+};
+
+struct Scratch {
+  bool few;
+  int groups, ldg, take, max_tiles;  // ldg: floats between the rows of gmax
+  long rows, ldz, stage_rows;
+  float *m, *s, *u, *gmax, *z, *gs, *gu, *cand, *picks, *row_loss;
+  int *chosen, *counts, *row_counts;
+  int2* entries;
+  GatherTile* tiles;
+  bf16_t* stage;
+};
+
+// k_list: length of a teacher's list (0: scoring, with `top` alternatives).
+Scratch carve(const ScoreShape& sh, int f32, int q4, int top, int k_list, void* ws, size_t* bytes) {
+  Scratch x{};
+  Carver c{static_cast<char*>(ws)};
+  x.few = !f32 && sh.n <= kFewTokens;
+  x.rows = sh.n < kScoreRows ? sh.n : kScoreRows;
+  x.groups = groups_of(sh.v);
+  x.ldg = x.few ? x.groups : (x.groups + 1) / 2 * 2;  // a tile of 256 logits writes both its groups, the last one too
+  x.take = top < x.groups ? top : x.groups;
+  if (x.few) {
+    x.ldz = (long)x.groups * kGroup;
+    x.z = c.take<float>(x.rows * x.ldz);
+    x.gmax = c.take<float>(x.rows * x.groups);
+    x.gs = c.take<float>(x.rows * x.groups);
+    x.gu = c.take<float>(x.rows * x.groups);
+  } else {
+    // (the last block of rows may split the vocabulary into more)
+    const long last = sh.n - (sh.n - 1) / x.rows * x.rows;
+    auto splits = [&](long n) { return (long)(f32 ? lce32_fwd_nsplit(n, sh.v) : lce_fwd_nsplit(n, sh.v)); };
+    const long parts = splits(x.rows) * x.rows > splits(last) * last ? splits(x.rows) * x.rows : splits(last) * last;
+    x.m = c.take<float>(parts);
+    x.s = c.take<float>(parts);
+    if (!k_list) x.u = c.take<float>(parts);
+    if (top) {
+      x.gmax = c.take<float>(x.rows * x.ldg);
+      x.chosen = c.take<int>(x.rows * x.take);
+      x.cand = c.take<float>(x.rows * x.take * kGroup);
+    }
+    const long entries = x.rows * (k_list ? k_list : x.take);
+    if (entries) {
+      x.counts = c.take<int>(x.groups);
+      x.entries = c.take<int2>(entries);
+      x.max_tiles = (int)(x.groups + entries / kGroup);  // each group's last tile may be part of one
+      if (x.max_tiles > entries) x.max_tiles = (int)entries;
+      x.tiles = c.take<GatherTile>(x.max_tiles);
+    }
+    if (k_list) x.picks = c.take<float>(x.rows * k_list);
+    if (q4 && sh.stage) {
+      x.stage_rows = sh.v;
+      x.stage = c.take<bf16_t>(sh.v * sh.d);
+    }
+  }
+  if (k_list) {
+    x.row_loss = c.take<float>(sh.n);
+    x.row_counts = c.take<int>(sh.n);
+  }
+  *bytes = c.used;
+  return x;
+}
+
+#define MTP_LAUNCHED()                        \
+  do {                                        \
+    const hipError_t e = hipGetLastError();   \
+    if (e != hipSuccess) return e;            \
+  } while (0)
+
+hipError_t few_logits(const ScoreHead& h, const ScoreShape& sh, const Scratch& x, float c2, hipStream_t st) {
+  const bf16_t* H = static_cast<const bf16_t*>(h.hidden);
+  const int blocks = (int)ceil_div(sh.n, 32);
+  auto run = [&](auto nb) {
+    constexpr int NB = decltype(nb)::value;
+    auto kernel = h.h.q4 ? lce_few_kernel<1, NB> : lce_few_kernel<0, NB>;
+    hipLaunchKernelGGL(kernel, dim3(x.groups), dim3(256), 0, st, H, h.h.w, h.h.wq, h.h.sc, h.h.bi, (int)sh.n, (int)sh.d,
+                       (int)sh.v, c2, (int)x.ldz, x.z, x.gmax, x.gs, x.gu);
+    return hipGetLastError();
+  };
+  if (blocks == 1) return run(std::integral_constant<int, 1>{});
+  if (blocks == 2) return run(std::integral_constant<int, 2>{});
+  return run(std::integral_constant<int, 4>{});
+}
+
+RowParts row_parts(const Scratch& x, const ScoreHead& h, long n, long v, float c2) {
+  if (x.few) return RowParts{x.gmax, x.gs, x.gu, x.groups, 1, x.groups, c2};
+  const int ns = h.f32 ? lce32_fwd_nsplit(n, v) : lce_fwd_nsplit(n, v);
+  return RowParts{x.m, x.s, x.u ? x.u : x.s, ns, n, 1, 1.f};
+}
+
+// The product over rows [r0, r0 + n) with its statistics.
+hipError_t tile_stats(const ScoreHead& h, const ScoreShape& sh, const Scratch& x, long r0, long n, float c2, hipStream_t st) {
+  const ScoreStats stats{c2, x.m, x.s, x.u, x.gmax, x.ldg};
+  if (h.f32)
+    return launch_lce32_stats(h.h32, static_cast<const float*>(h.hidden) + r0 * sh.d, (int)n, (int)sh.d, (int)sh.v, stats, st);
+  return launch_lce_stats(h.h, static_cast<const bf16_t*>(h.hidden) + r0 * sh.d, (int)n, (int)sh.d, (int)sh.v, stats, x.stage,
+                          x.stage_rows, st);
+}
+
+hipError_t gather(const ScoreHead& h, const ScoreShape& sh, const Scratch& x, long r0, hipStream_t st) {
+  const GatherPlan plan{x.entries, x.tiles, x.max_tiles, x.cand, x.picks};
+  if (h.f32) return launch_lce32_gather(h.h32, static_cast<const float*>(h.hidden) + r0 * sh.d, (int)sh.d, (int)sh.v, plan, st);
+  return launch_lce_gather(h.h, static_cast<const bf16_t*>(h.hidden) + r0 * sh.d, (int)sh.d, (int)sh.v, plan, st);
+}
+
+}  // namespace
+
+hipError_t launch_lce_gather(const LceHead& h, const bf16_t* H, int D, int V, const GatherPlan& p, hipStream_t st) {
+  hipLaunchKernelGGL(h.q4 ? lce_gather_kernel<1> : lce_gather_kernel<0>, dim3(p.max_tiles), dim3(256), 0, st, H, h.w, h.wq, h.sc,
+                     h.bi, D, V, p);
+  return hipGetLastError();
+}
+
+size_t logprobs_fwd_workspace(const ScoreShape& sh, int f32, int q4, int top) {
+  size_t bytes;
+  carve(sh, f32, q4, top, 0, nullptr, &bytes);
+  return bytes;
+}
+
+hipError_t launch_logprobs_fwd(const ScoreHead& h, const ScoreShape& sh, const int64_t* targets, long long ignore_index,
+                               int top, const LogprobsOut& o, void* ws, hipStream_t st) {
+  size_t bytes;
+  const Scratch x = carve(sh, h.f32, h.f32 ? h.h32.q4 : h.h.q4, top, 0, ws, &bytes);
+  const float c2 = kLog2e * sh.inv_t;
+  const int V = (int)sh.v;
+  if (x.few) {
+    const hipError_t e = few_logits(h, sh, x, c2, st);
+    if (e != hipSuccess) return e;
+    auto rows = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)sh.n), dim3(kPick), 0, st, row_parts(x, h, sh.n, sh.v, c2), x.gmax, x.groups, x.ldg, x.z,
+                         x.ldz, targets, ignore_index, V, sh.inv_t, top, x.take, o, nullptr, nullptr);
+      return hipGetLastError();
+    };
+    if (!top) return rows(score_rows_kernel<true, 0, 0>);
+    if (x.take <= 16 && x.groups <= 2048) return rows(score_rows_kernel<true, 2048, 2048>);
+    return rows(score_rows_kernel<true, kMaxGroups, kScoreTop * kGroup>);
+  }
+  for (long r0 = 0; r0 < sh.n; r0 += x.rows) {
+    const long n = sh.n - r0 < x.rows ? sh.n - r0 : x.rows;
+    const LogprobsOut out{o.logprobs ? o.logprobs + r0 : nullptr, o.entropy + r0, top ? o.top_logprobs + r0 * top : nullptr,
+                          top ? o.top_ids + r0 * top : nullptr, o.lse + r0, o.tgt ? o.tgt + r0 : nullptr};
+    const int64_t* y = targets ? targets + r0 : nullptr;
+    hipError_t e = tile_stats(h, sh, x, r0, n, c2, st);
+    if (e != hipSuccess) return e;
+    if (y) {
+      e = h.f32 ? launch_lce32_target(h.h32, static_cast<const float*>(h.hidden) + r0 * sh.d, y, (int)n, (int)sh.d, V, out.tgt, st)
+                : launch_lce_target(h.h, static_cast<const bf16_t*>(h.hidden) + r0 * sh.d, y, (int)n, (int)sh.d, V, out.tgt, st);
+      if (e != hipSuccess) return e;
+    }
+    if (top) {
+      hipLaunchKernelGGL(zero_counts_kernel, dim3((unsigned)ceil_div(x.groups, 256)), dim3(256), 0, st, x.counts, x.groups);
+      MTP_LAUNCHED();
+    }
+    auto rows = !top ? score_rows_kernel<false, 0, 0>
+                     : x.groups <= 2048 ? score_rows_kernel<false, 2048, 0> : score_rows_kernel<false, kMaxGroups, 0>;
+    hipLaunchKernelGGL(rows, dim3((unsigned)n), dim3(kPick), 0, st, row_parts(x, h, n, sh.v, c2), x.gmax, x.groups, x.ldg, nullptr, 0L, y,
+                       ignore_index, V, sh.inv_t, top, x.take, out, x.chosen, x.counts);
+    MTP_LAUNCHED();
+    if (!top) continue;
+    hipLaunchKernelGGL(gather_tiles_kernel, dim3(1), dim3(1024), 0, st, x.counts, x.groups, x.tiles, x.max_tiles);
+    MTP_LAUNCHED();
+    hipLaunchKernelGGL(gather_groups_kernel, dim3((unsigned)ceil_div(n * x.take, 256)), dim3(256), 0, st, x.chosen, n * x.take,
+                       x.take, x.counts, x.entries);
+    MTP_LAUNCHED();
+    e = gather(h, sh, x, r0, st);
+    if (e != hipSuccess) return e;
+    auto best = x.take <= 16 ? score_top_kernel<16 * kGroup> : x.take <= 64 ? score_top_kernel<64 * kGroup> : score_top_kernel<kScoreTop * kGroup>;
+    hipLaunchKernelGGL(best, dim3((unsigned)n), dim3(kPick), 0, st, x.cand, x.chosen, y, V, sh.inv_t, top, x.take, out);
+    MTP_LAUNCHED();
+  }
+  return hipSuccess;
+}
+
+size_t distill_fwd_workspace(const ScoreShape& sh, int f32, int q4, int k) {
+  size_t bytes;
+  carve(sh, f32, q4, 0, k, nullptr, &bytes);
+  return bytes;
+}
+
+hipError_t launch_distill_fwd(const ScoreHead& h, const ScoreShape& sh, const int64_t* ids, const float* teacher,
+                              const uint8_t* mask, const DistillLoss& p, const DistillOut& o, void* ws, hipStream_t st) {
+  size_t bytes;
+  const Scratch x = carve(sh, h.f32, h.f32 ? h.h32.q4 : h.h.q4, 0, p.k, ws, &bytes);
+  const float c2 = kLog2e * sh.inv_t;
+  float* row_loss = p.reduction == kReduceNone ? o.loss : x.row_loss;
+  auto kernel = p.kind == kDistillForward ? distill_rows_kernel<kDistillForward>
+                : p.kind == kDistillReverse ? distill_rows_kernel<kDistillReverse> : distill_rows_kernel<kDistillJsd>;
+  for (long r0 = 0; r0 < sh.n; r0 += x.rows) {
+    const long n = sh.n - r0 < x.rows ? sh.n - r0 : x.rows;
+    const int64_t* id = ids + r0 * p.k;
+    const float* lp = teacher + r0 * p.k;
+    const uint8_t* see = mask ? mask + r0 : nullptr;
+    if (x.few) {
+      const hipError_t e = few_logits(h, sh, x, c2, st);
+      if (e != hipSuccess) return e;
+    } else {
+      hipError_t e = tile_stats(h, sh, x, r0, n, c2, st);
+      if (e != hipSuccess) return e;
+      const dim3 grid((unsigned)ceil_div(n * p.k, 256)), block(256);
+      hipLaunchKernelGGL(zero_counts_kernel, dim3((unsigned)ceil_div(x.groups, 256)), block, 0, st, x.counts, x.groups);
+      MTP_LAUNCHED();
+      hipLaunchKernelGGL(gather_list_kernel<true>, grid, block, 0, st, id, lp, see, n * p.k, p.k, sh.v, x.counts, x.entries);
+      MTP_LAUNCHED();
+      hipLaunchKernelGGL(gather_tiles_kernel, dim3(1), dim3(1024), 0, st, x.counts, x.groups, x.tiles, x.max_tiles);
+      MTP_LAUNCHED();
+      hipLaunchKernelGGL(gather_list_kernel<false>, grid, block, 0, st, id, lp, see, n * p.k, p.k, sh.v, x.counts, x.entries);
+      MTP_LAUNCHED();
+      e = gather(h, sh, x, r0, st);
+      if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(n, 4)), dim3(256), 0, st, row_parts(x, h, n, sh.v, c2), x.picks,
+                       x.few ? x.z : nullptr, x.ldz, id, lp, see, n, sh.v, sh.inv_t, p.k, p.renormalize, p.beta, row_loss + r0,
+                       x.row_counts + r0, o.lse + r0, o.rest + r0, o.coef + r0 * p.k, o.columns + r0 * p.k);
+    MTP_LAUNCHED();
+  }
+  if (p.reduction == kReduceNone) return hipSuccess;
+  hipLaunchKernelGGL(distill_reduce_kernel, dim3(1), dim3(1024), 0, st, row_loss, x.row_counts, sh.n, p.reduction == kReduceMean,
+                     o.loss, o.scale);
+  return hipGetLastError();
+}
+
+hipError_t launch_logprobs_coef(const float* d_logprobs, const float* d_entropy, const int64_t* targets, long long ignore_index,
+                                const float* lse, const float* entropy, const float* tgt, long n, long v, float inv_t,
+                                float* alpha, float* beta, int* columns, float* value, hipStream_t st) {
+  hipLaunchKernelGGL(logprobs_coef_kernel, dim3((unsigned)ceil_div(n, 256)), dim3(256), 0, st, d_logprobs, d_entropy, targets,
+                     ignore_index, lse, entropy, tgt, n, v, inv_t, alpha, beta, columns, value);
+  return hipGetLastError();
+}
+
+hipError_t launch_distill_coef(const float* d_loss, int per_row, const float* scale, const float* rest, const float* coef, long n,
+                               int k, float* alpha, float* value, hipStream_t st) {
+  hipLaunchKernelGGL(distill_coef_kernel, dim3((unsigned)ceil_div(n * k, 256)), dim3(256), 0, st, d_loss, per_row, scale, rest,
+                     coef, n, k, alpha, value);
+  return hipGetLastError();
+}
+
+hipError_t launch_clean_rows(const void* hidden, const float* alpha, const float* beta, long n, long row_bytes, void* out,
+                             hipStream_t st) {
+  hipLaunchKernelGGL(clean_rows_kernel, dim3((unsigned)n), dim3(256), 0, st, static_cast<const uint32_t*>(hidden), alpha, beta,
+                     row_bytes / 4, static_cast<uint32_t*>(out));
+  return hipGetLastError();
+}
+
+}  // namespace mtp

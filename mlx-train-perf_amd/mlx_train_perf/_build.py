@@ -22,7 +22,7 @@ NODE_SRC = CSRC / "torch_nodes.cpp"
 NODE_OUT = PKG_DIR / "_mtp_torch.so"
 OBJ_DIR = PKG_DIR.parent / "_build"
 SOURCES = ("capi.hip", "lce_kernels.hip", "attn_kernels.hip", "attn_scored.hip", "attn_scored_64.hip", "attn_scored_96.hip",
-           "attn_scored_128.hip", "f32_kernels.hip", "attn32_scored.hip", "preference_kernels.hip", "bench_probe.hip")
+           "attn_scored_128.hip", "f32_kernels.hip", "attn32_scored.hip", "preference_kernels.hip", "score_kernels.hip", "bench_probe.hip")
 ARCH = os.environ.get("MTP_OFFLOAD_ARCH", "gfx950")
 
 HIPCC_FLAGS = [
