@@ -35,20 +35,10 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 
 struct PickScratch {
-  int count[2][kPick / 64];
-  int sum[kPick / 64];
+  int4 count[2][kPick / 64];
+  int sum[kPick / 64], listed;
 };
 
-// Sum over the workgroup's threads; every thread gets it.
-__device__ __forceinline__ int block_sum(int mine_wave, PickScratch& s, int step) {
-  const int w = threadIdx.x >> 6;
-  if ((threadIdx.x & 63) == 0) s.count[step & 1][w] = mine_wave;
-  __syncthreads();
-  int n = 0;
-#pragma unroll
-  for (int i = 0; i < kPick / 64; ++i) n += s.count[step & 1][i];
-  return n;
-}
 // Sum over the threads before this one.
 __device__ __forceinline__ int block_before(int mine, PickScratch& s) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -66,26 +56,56 @@ __device__ __forceinline__ int block_before(int mine, PickScratch& s) {
   return before;
 }
 
-// The positions, ascending, of the K largest of M >= K keys in LDS; equal keys go to the lower position. The K-th largest is
-// found bit by bit, 32 counts over the keys, so the time does not depend on their order. Ends with a barrier.
-__device__ __forceinline__ void pick_largest(const uint32_t* key, int M, int K, int* at, PickScratch& s) {
-  const int tid = threadIdx.x;
+// The K-th largest of M >= K keys, key i at thread i % kPick, register i / kPick (0 past the end: below every number's). Found two
+// bits a step, three counts over the keys, so the time does not depend on their order. `above`: how many are larger.
+template <int R>
+__device__ __forceinline__ uint32_t kth_largest(const uint32_t (&key)[R], int K, int& above, PickScratch& s) {
   uint32_t least = 0;
-  for (int b = 31; b >= 0; --b) {
-    const uint32_t c = least | (1u << b);
-    int n = 0;
-    for (int base = 0; base < M; base += kPick) {
-      const int i = base + tid;
-      n += __popcll(__ballot(i < M && key[i] >= c));
+  above = 0;
+  for (int b = 30; b >= 0; b -= 2) {
+    int n1 = 0, n2 = 0, n3 = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      n1 += __popcll(__ballot(key[r] >= (least | 1u << b)));
+      n2 += __popcll(__ballot(key[r] >= (least | 2u << b)));
+      n3 += __popcll(__ballot(key[r] >= (least | 3u << b)));
     }
-    if (block_sum(n, s, b) >= K) least = c;
+    const int w = threadIdx.x >> 6, step = (b >> 1) & 1;
+    if ((threadIdx.x & 63) == 0) s.count[step][w] = int4{n1, n2, n3, 0};
+    __syncthreads();
+    n1 = n2 = n3 = 0;
+#pragma unroll
+    for (int i = 0; i < kPick / 64; ++i) {
+      n1 += s.count[step][i].x;
+      n2 += s.count[step][i].y;
+      n3 += s.count[step][i].z;
+    }
+    if (n3 >= K) {
+      least |= 3u << b;
+    } else if (n2 >= K) {
+      least |= 2u << b;
+      above = n3;
+    } else if (n1 >= K) {
+      least |= 1u << b;
+      above = n2;
+    } else {
+      above = n1;
+    }
   }
-  int above = 0;
-  for (int base = 0; base < M; base += kPick) {
-    const int i = base + tid;
-    above += __popcll(__ballot(i < M && key[i] > least));
-  }
-  const int equal = K - block_sum(above, s, 1);  // how many of the keys that equal the K-th are taken
+  return least;
+}
+
+// The positions, ascending, of the K largest of M >= K keys in LDS; equal keys go to the lower position. Ends with a barrier.
+// R: at least M / kPick. Returns the K-th largest.
+template <int R>
+__device__ __forceinline__ uint32_t pick_largest(const uint32_t* key, int M, int K, int* at, PickScratch& s) {
+  const int tid = threadIdx.x;
+  uint32_t mine_keys[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) mine_keys[r] = r * kPick + tid < M ? key[r * kPick + tid] : 0u;
+  int above;
+  const uint32_t least = kth_largest<R>(mine_keys, K, above, s);
+  const int equal = K - above;  // how many of the keys that equal the K-th are taken
   const int per = (M + kPick - 1) / kPick, lo = tid * per < M ? tid * per : M, hi = lo + per < M ? lo + per : M;
   int mine = 0;
   for (int i = lo; i < hi; ++i) mine += key[i] == least;
@@ -99,68 +119,71 @@ __device__ __forceinline__ void pick_largest(const uint32_t* key, int M, int K, 
   for (int i = lo; i < hi; ++i)
     if (key[i] > least || (key[i] == least && seen++ < equal)) at[to++] = i;
   __syncthreads();
+  return least;
 }
 
 // ------------------------------------------------------------------------------------------
 // Few tokens (bf16 hidden states): the logits [N][ldz] in fp32, and per group of kGroup of them their maximum and, relative to
 // it, the two sums. The head is read once and bounds it; a workgroup takes one group: 4 waves of 32 vocab rows, the rows'
-// fragments straight from memory to registers a slab of 128 k ahead (8 KiB a wave in flight), the tokens' slab (NB blocks of 32)
-// through LDS, one barrier a slab.
+// fragments straight from memory to registers, each loaded for the next slab as soon as its product has gone out (a whole slab in
+// flight a wave, 8 KiB of a dense head, 4 or 2 of a 4-bit one), the tokens' slab (NB blocks of 32) through LDS, one barrier a
+// slab. The registers leave room for 5 workgroups a CU: all 1187 groups of 151936 run at once (with 4 the rest ran alone
+// after them: 262 us a token at 4096 x 151936, now FEWDENSE).
 // ------------------------------------------------------------------------------------------
-constexpr int kSlab = 128;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base, long bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, bytes > 0x7fffffffL ? 0x7fffffff : (int)bytes, 0x00020000);
+}
+__device__ __forceinline__ u32x4 load16(const __amdgpu_buffer_rsrc_t r, uint32_t voff, int soff) {
+  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, voff, soff, 0));
+}
+// LDS written before is seen behind it by the workgroup; loads into registers stay in flight.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-template <int Q4, int NB>
-__global__ __launch_bounds__(256) void lce_few_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
-                                                      const uint32_t* __restrict__ Wq, const bf16_t* __restrict__ Sc,
-                                                      const bf16_t* __restrict__ Bi, int N, int D, int V, float c2, int ldz,
-                                                      float* __restrict__ Z, float* __restrict__ gmax,
-                                                      float* __restrict__ gs, float* __restrict__ gu) {
-  constexpr int kTok = 32 * NB, kBytes = kTok * 2 * kSlab;  // a slab: two tiles of 64 k, 128 bytes a row
+template <int Q4, int NB, int SLAB>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NB == 1 ? 5 : NB == 2 ? 4 : 2)))
+void lce_few_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W, const uint32_t* __restrict__ Wq,
+                    const bf16_t* __restrict__ Sc, const bf16_t* __restrict__ Bi, int N, int D, int V, float c2, int ldz,
+                    float* __restrict__ Z, float* __restrict__ gmax, float* __restrict__ gs, float* __restrict__ gu) {
+  constexpr int kTok = 32 * NB, kBytes = kTok * 2 * SLAB;  // a slab of tokens: tiles of 64 k, 128 bytes a row
+  constexpr int kFrags = SLAB / 16, kParts = kBytes / 4096, kChunks = SLAB / 8;
   __shared__ __attribute__((aligned(16))) char lds[2 * kBytes];
-  __shared__ float xm[4][kTok], xs[4][kTok], xu[4][kTok];
+  float(*xm)[kTok] = reinterpret_cast<float(*)[kTok]>(lds);  // after the product: 4 waves' statistics
+  float(*xs)[kTok] = xm + 4;
+  float(*xu)[kTok] = xm + 8;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, half = lane >> 5, col = lane & 31;
-  const int v0 = blockIdx.x * kGroup, v = v0 + 32 * w + col;
-  const int vr = v < V ? v : V - 1;  // rows past the end: their logits are replaced
-  const int slabs = (D + kSlab - 1) / kSlab;
+  const int v0 = blockIdx.x * kGroup;
+  const int vr = 32 * w + col < V - v0 ? 32 * w + col : V - 1 - v0;  // rows past the end: their logits are replaced
+  const int slabs = (D + SLAB - 1) / SLAB;
 
-  // Fragment j of a slab contracts k chunk (8 values) `2 j + half` of it; with packed words 8 half + j, so that a lane's words
-  // lie together.
-  auto chunk = [&](int j) { return Q4 ? 8 * half + j : 2 * j + half; };
-  u32x4 wa[Q4 ? 2 : 8];
-  uint32_t sb = 0;
-  auto load_head = [&](int slab) {
-    if constexpr (Q4) {
-      const int k = slab * kSlab + 64 * half;
-      if (k < D) {
-        const u32x4* q = reinterpret_cast<const u32x4*>(Wq + (long)vr * (D >> 3) + (k >> 3));
-        wa[0] = q[0];
-        wa[1] = q[1];
-        const long g = (long)vr * (D >> 6) + (k >> 6);
-        sb = (uint32_t)Sc[g] | (uint32_t)Bi[g] << 16;
-      } else {
-        wa[0] = wa[1] = zero4();
-        sb = 0;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int k = slab * kSlab + 8 * chunk(j);
-        wa[j] = k < D ? *reinterpret_cast<const u32x4*>(W + (long)vr * D + k) : zero4();
-      }
-    }
+  // Fragment j of a slab contracts k chunk (8 values) `2 j + half` of it; with packed words kFrags half + j, so that a lane's
+  // words lie together. Past the end of a row a load takes the next row's values (past the head zeros): the tokens' are
+  // zeros there.
+  auto chunk = [&](int j) { return Q4 ? kFrags * half + j : 2 * j + half; };
+  u32x4 wa[Q4 ? SLAB / 64 : kFrags];
+  uint32_t sc[Q4 ? SLAB / 128 : 1], bi[Q4 ? SLAB / 128 : 1];
+  const __amdgpu_buffer_rsrc_t rw =
+      Q4 ? rows_rsrc(Wq + (long)v0 * (D >> 3), (long)(V - v0) * (D >> 1)) : rows_rsrc(W + (long)v0 * D, 2L * (V - v0) * D);
+  const uint32_t wo = Q4 ? (uint32_t)vr * (uint32_t)(D >> 1) + half * (SLAB / 4) : 2u * (uint32_t)vr * (uint32_t)D + 16 * half;
+  const __amdgpu_buffer_rsrc_t rs = rows_rsrc(Q4 ? Sc + (long)v0 * (D >> 6) : W, Q4 ? 2L * (V - v0) * (D >> 6) : 0);
+  const __amdgpu_buffer_rsrc_t rb = rows_rsrc(Q4 ? Bi + (long)v0 * (D >> 6) : W, Q4 ? 2L * (V - v0) * (D >> 6) : 0);
+  const uint32_t so = 2u * ((uint32_t)vr * (uint32_t)(D >> 6) + half * (SLAB / 128));
+  auto load_words = [&](int slab, int i) { wa[i] = load16(rw, wo, slab * (Q4 ? SLAB / 2 : 2 * SLAB) + (Q4 ? 16 : 32) * i); };
+  auto load_scale = [&](int slab, int i) {
+    sc[i] = __builtin_amdgcn_raw_buffer_load_b16(rs, so, slab * (SLAB / 32) + 2 * i, 0);
+    bi[i] = __builtin_amdgcn_raw_buffer_load_b16(rb, so, slab * (SLAB / 32) + 2 * i, 0);
   };
-  u32x4 ha[2 * NB];
+  u32x4 ha[kParts];
   auto load_tokens = [&](int slab) {
 #pragma unroll
-    for (int p = 0; p < 2 * NB; ++p) {
-      const int id = tid + 256 * p, row = id >> 4, k = slab * kSlab + 8 * (id & 15);
+    for (int p = 0; p < kParts; ++p) {
+      const int id = tid + 256 * p, row = id / kChunks, k = slab * SLAB + 8 * (id % kChunks);
       ha[p] = row < N && k < D ? *reinterpret_cast<const u32x4*>(H + (long)row * D + k) : zero4();
     }
   };
   auto put_tokens = [&](char* dst) {
 #pragma unroll
-    for (int p = 0; p < 2 * NB; ++p) {
-      const int id = tid + 256 * p, row = id >> 4, c = id & 15;
+    for (int p = 0; p < kParts; ++p) {
+      const int id = tid + 256 * p, row = id / kChunks, c = id % kChunks;
       lds_write16(dst + (c >> 3) * (kTok * 128), lds_off(row, c & 7), ha[p]);
     }
   };
@@ -171,32 +194,40 @@ __global__ __launch_bounds__(256) void lce_few_kernel(const bf16_t* __restrict__
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[b][r] = 0.f;
   load_tokens(0);
-  load_head(0);
+  if constexpr (Q4) {
+#pragma unroll
+    for (int i = 0; i < SLAB / 128; ++i) load_scale(0, i);
+  }
+#pragma unroll
+  for (int i = 0; i < (Q4 ? SLAB / 64 : kFrags); ++i) load_words(0, i);
   put_tokens(lds);
-  __syncthreads();
+  lds_barrier();
   for (int s = 0; s < slabs; ++s) {
     const char* cur = lds + (s & 1) * kBytes;
-    bf16x8 a[8];
+    load_tokens(s + 1);  // (past the end: zeros)
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if constexpr (Q4) a[j] = as_bf16x8(dequant8(wa[j >> 2][j & 3], bf16lo(sb), bf16hi(sb)));
-      else a[j] = as_bf16x8(wa[j]);
-    }
-    if (s + 1 < slabs) {
-      load_tokens(s + 1);
-      load_head(s + 1);
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < kFrags; ++j) {
       const int c = chunk(j);
+      bf16x8 a;
+      if constexpr (Q4) a = as_bf16x8(dequant8(wa[j >> 2][j & 3], bf16lo(sc[j >> 3]), bf16lo(bi[j >> 3])));
+      else a = as_bf16x8(wa[j]);
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         const bf16x8 t = as_bf16x8(lds_read16(cur + (c >> 3) * (kTok * 128), lds_off(32 * b + col, c & 7)));
-        acc[b] = mfma32(a[j], t, acc[b]);
+        acc[b] = mfma32(a, t, acc[b]);
+      }
+      if constexpr (Q4) {
+        if (j % 4 == 3) load_words(s + 1, j >> 2);
+        if (j % 8 == 7) load_scale(s + 1, j >> 3);
+        if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      } else {
+        load_words(s + 1, j);
+        if (j % 2 == 1) __builtin_amdgcn_sched_barrier(0);
       }
     }
-    if (s + 1 < slabs) put_tokens(lds + ((s + 1) & 1) * kBytes);
-    __syncthreads();
+    put_tokens(lds + ((s + 1) & 1) * kBytes);
+    lds_barrier();
   }
 
   // acc[b][r]: vocab row 32 w + 8 (r / 4) + 4 half + r % 4 of the group, token 32 b + col.
@@ -445,20 +476,43 @@ __device__ __forceinline__ void merge_row(const RowParts& p, long t, float& m, f
   for (int i = 1; i < kPick / 64; ++i) lse2_merge(m, s, u, x[0][i], x[1][i], x[2][i]);
 }
 
-// The K largest of a row's candidate logits, M = ngroups kGroup of them in LDS as keys, ordered, with their log
-// probabilities. The groups ascend, so positions ascend with the index. A target among them takes its logit from here.
-__device__ __forceinline__ void write_top(const uint32_t* key, const int* group, int ngroups, int K, int V, float inv_t, float lse,
-                                          long t, long long target, const LogprobsOut& out, int* at, PickScratch& s) {
-  pick_largest(key, ngroups * kGroup, K, at, s);
-  const int i = threadIdx.x;
-  if (i < K) {
-    const uint32_t mine = key[at[i]];
+// The K largest of a row's candidate logits, ngroups kGroup of them in LDS as keys, in order, with their log probabilities.
+// The groups ascend, so positions ascend with the index. `least`: the K-th largest of the groups' maxima (0 with fewer than K
+// groups), below which nothing is chosen: mostly a few more than K are left, and each one's place is its count of those before
+// it. A target among them takes its logit from here.
+constexpr int kRanked = 512;
+template <int MC>
+__device__ __forceinline__ void write_top(const uint32_t* key, const int* group, int ngroups, int K, uint32_t least, int V,
+                                          float inv_t, float lse, long t, long long target, const LogprobsOut& out, int* at,
+                                          PickScratch& s) {
+  const int tid = threadIdx.x, lane = tid & 63, M = ngroups * kGroup;
+  if (tid == 0) s.listed = 0;
+  __syncthreads();
+  for (int base = 0; base < M; base += kPick) {
+    const int i = base + tid;
+    const bool in = i < M && key[i] >= least;
+    const uint64_t who = __ballot(in);
+    int first = 0;
+    if (lane == 0 && who) first = atomicAdd(&s.listed, __popcll(who));
+    first = __builtin_amdgcn_readfirstlane(first) + __popcll(who & ((1ull << lane) - 1));
+    if (in && first < kRanked) at[first] = i;
+  }
+  __syncthreads();
+  int n = s.listed;
+  if (n > kRanked) {  // many equal ones
+    pick_largest<MC / kPick>(key, M, K, at, s);
+    n = K;
+  }
+  for (int i = tid; i < n; i += kPick) {
+    const int p = at[i];
+    const uint32_t mine = key[p];
     int rank = 0;
-    for (int j = 0; j < K; ++j) {
+    for (int j = 0; j < n; ++j) {
       const uint32_t other = key[at[j]];
-      rank += other > mine || (other == mine && j < i);
+      rank += other > mine || (other == mine && at[j] < p);
     }
-    const int id = group[at[i] / kGroup] * kGroup + at[i] % kGroup;
+    if (rank >= K) continue;
+    const int id = group[p / kGroup] * kGroup + p % kGroup;
     const float z = key_value(mine), lp = z * inv_t - lse;
     out.top_ids[t * K + rank] = id < V ? id : -1;
     out.top_logprobs[t * K + rank] = lp;
@@ -477,11 +531,12 @@ __global__ __launch_bounds__(kPick) void score_rows_kernel(RowParts parts, const
                                                            const float* __restrict__ Z, long ldz,
                                                            const int64_t* __restrict__ targets, long long ignore_index, int V,
                                                            float inv_t, int K, int take, LogprobsOut out,
-                                                           int* __restrict__ groups, int* __restrict__ counts) {
+                                                           int* __restrict__ groups, int* __restrict__ counts,
+                                                           uint32_t* __restrict__ floors) {
   __shared__ float x[3][kPick / 64];
   __shared__ PickScratch scratch;
   __shared__ uint32_t key[MG > MC ? MG : MC > 0 ? MC : 1];
-  __shared__ int group[kScoreTop], at[kScoreTop];
+  __shared__ int group[kScoreTop], at[kRanked];
   const long t = blockIdx.x;
   const int tid = threadIdx.x;
   const long long y = targets ? targets[t] : 0;
@@ -514,15 +569,17 @@ __global__ __launch_bounds__(kPick) void score_rows_kernel(RowParts parts, const
   if constexpr (MG > 0) {
     for (int i = tid; i < ngroups; i += kPick) key[i] = order_key(gmax[t * ldg + i]);
     __syncthreads();
-    pick_largest(key, ngroups, take, group, scratch);
+    uint32_t least = pick_largest<MG / kPick>(key, ngroups, take, group, scratch);
+    if (take < K) least = 0;
     if constexpr (KEPT) {
       for (int i = tid; i < take * kGroup; i += kPick)
         key[i] = order_key(Z[t * ldz + (long)group[i / kGroup] * kGroup + i % kGroup]);
       __syncthreads();
-      write_top(key, group, take, K, V, inv_t, lse, t, targets ? y : -1, out, at, scratch);
+      write_top<MC>(key, group, take, K, least, V, inv_t, lse, t, targets ? y : -1, out, at, scratch);
     } else if (tid < take) {
       groups[t * take + tid] = group[tid];
       atomicAdd(&counts[group[tid]], 1);
+      if (tid == 0) floors[t] = least;
     }
   }
 }
@@ -530,18 +587,18 @@ __global__ __launch_bounds__(kPick) void score_rows_kernel(RowParts parts, const
 // After the gather: the alternatives from the chosen groups' logits [N][take][kGroup].
 template <int MC>
 __global__ __launch_bounds__(kPick) void score_top_kernel(const float* __restrict__ rows, const int* __restrict__ groups,
-                                                          const int64_t* __restrict__ targets, int V, float inv_t, int K,
+                                                          const uint32_t* __restrict__ floors, const int64_t* __restrict__ targets, int V, float inv_t, int K,
                                                           int take, LogprobsOut out) {
   __shared__ PickScratch scratch;
   __shared__ uint32_t key[MC];
-  __shared__ int group[kScoreTop], at[kScoreTop];
+  __shared__ int group[kScoreTop], at[kRanked];
   const long t = blockIdx.x;
   const int tid = threadIdx.x;
   if (groups[t * take] < 0) return;  // an ignored token
   for (int i = tid; i < take; i += kPick) group[i] = groups[t * take + i];
   for (int i = tid; i < take * kGroup; i += kPick) key[i] = order_key(rows[t * take * kGroup + i]);
   __syncthreads();
-  write_top(key, group, take, K, V, inv_t, out.lse[t], t, targets ? targets[t] : -1, out, at, scratch);
+  write_top<MC>(key, group, take, K, floors[t], V, inv_t, out.lse[t], t, targets ? targets[t] : -1, out, at, scratch);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -819,6 +876,7 @@ struct Scratch {
   long rows, ldz, stage_rows;
   float *m, *s, *u, *gmax, *z, *gs, *gu, *cand, *picks, *row_loss;
   int *chosen, *counts, *row_counts;
+  uint32_t* floors;
   int2* entries;
   GatherTile* tiles;
   bf16_t* stage;
@@ -850,6 +908,7 @@ Scratch carve(const ScoreShape& sh, int f32, int q4, int top, int k_list, void* 
     if (top) {
       x.gmax = c.take<float>(x.rows * x.ldg);
       x.chosen = c.take<int>(x.rows * x.take);
+      x.floors = c.take<uint32_t>(x.rows);
       x.cand = c.take<float>(x.rows * x.take * kGroup);
     }
     const long entries = x.rows * (k_list ? k_list : x.take);
@@ -885,7 +944,7 @@ hipError_t few_logits(const ScoreHead& h, const ScoreShape& sh, const Scratch& x
   const int blocks = (int)ceil_div(sh.n, 32);
   auto run = [&](auto nb) {
     constexpr int NB = decltype(nb)::value;
-    auto kernel = h.h.q4 ? lce_few_kernel<1, NB> : lce_few_kernel<0, NB>;
+    auto kernel = h.h.q4 ? lce_few_kernel<1, NB, NB == 1 ? 256 : 128> : lce_few_kernel<0, NB, 128>;
     hipLaunchKernelGGL(kernel, dim3(x.groups), dim3(256), 0, st, H, h.h.w, h.h.wq, h.h.sc, h.h.bi, (int)sh.n, (int)sh.d,
                        (int)sh.v, c2, (int)x.ldz, x.z, x.gmax, x.gs, x.gu);
     return hipGetLastError();
@@ -941,11 +1000,12 @@ hipError_t launch_logprobs_fwd(const ScoreHead& h, const ScoreShape& sh, const i
     if (e != hipSuccess) return e;
     auto rows = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3((unsigned)sh.n), dim3(kPick), 0, st, row_parts(x, h, sh.n, sh.v, c2), x.gmax, x.groups, x.ldg, x.z,
-                         x.ldz, targets, ignore_index, V, sh.inv_t, top, x.take, o, nullptr, nullptr);
+                         x.ldz, targets, ignore_index, V, sh.inv_t, top, x.take, o, nullptr, nullptr, nullptr);
       return hipGetLastError();
     };
     if (!top) return rows(score_rows_kernel<true, 0, 0>);
     if (x.take <= 16 && x.groups <= 2048) return rows(score_rows_kernel<true, 2048, 2048>);
+    if (x.take <= 64 && x.groups <= 2048) return rows(score_rows_kernel<true, 2048, 64 * kGroup>);
     return rows(score_rows_kernel<true, kMaxGroups, kScoreTop * kGroup>);
   }
   for (long r0 = 0; r0 < sh.n; r0 += x.rows) {
@@ -967,7 +1027,7 @@ hipError_t launch_logprobs_fwd(const ScoreHead& h, const ScoreShape& sh, const i
     auto rows = !top ? score_rows_kernel<false, 0, 0>
                      : x.groups <= 2048 ? score_rows_kernel<false, 2048, 0> : score_rows_kernel<false, kMaxGroups, 0>;
     hipLaunchKernelGGL(rows, dim3((unsigned)n), dim3(kPick), 0, st, row_parts(x, h, n, sh.v, c2), x.gmax, x.groups, x.ldg, nullptr, 0L, y,
-                       ignore_index, V, sh.inv_t, top, x.take, out, x.chosen, x.counts);
+                       ignore_index, V, sh.inv_t, top, x.take, out, x.chosen, x.counts, x.floors);
     MTP_LAUNCHED();
     if (!top) continue;
     hipLaunchKernelGGL(gather_tiles_kernel, dim3(1), dim3(1024), 0, st, x.counts, x.groups, x.tiles, x.max_tiles);
@@ -978,7 +1038,7 @@ hipError_t launch_logprobs_fwd(const ScoreHead& h, const ScoreShape& sh, const i
     e = gather(h, sh, x, r0, st);
     if (e != hipSuccess) return e;
     auto best = x.take <= 16 ? score_top_kernel<16 * kGroup> : x.take <= 64 ? score_top_kernel<64 * kGroup> : score_top_kernel<kScoreTop * kGroup>;
-    hipLaunchKernelGGL(best, dim3((unsigned)n), dim3(kPick), 0, st, x.cand, x.chosen, y, V, sh.inv_t, top, x.take, out);
+    hipLaunchKernelGGL(best, dim3((unsigned)n), dim3(kPick), 0, st, x.cand, x.chosen, x.floors, y, V, sh.inv_t, top, x.take, out);
     MTP_LAUNCHED();
   }
   return hipSuccess;

@@ -1,6 +1,7 @@
-// The autograd nodes of flash_attention, linear_cross_entropy, preference_loss and policy_loss on plain tensors: the
-// forward and backward of attention/api.py's _KernelAttention and _ScoredAttention, core/loss.py's _KernelLCE and
-// core/preference.py's _Preference and _Policy, planned and launched from C++.
+// The autograd nodes of flash_attention, linear_cross_entropy, preference_loss, policy_loss, token_logprobs and
+// distillation_loss on plain tensors: the forward and backward of attention/api.py's _KernelAttention and _ScoredAttention,
+// core/loss.py's _KernelLCE, core/preference.py's _Preference and _Policy and core/scoring.py's _TokenLogprobs and
+// _Distillation, planned and launched from C++.
 // Autograd runs a backward on a thread of its own; a Python node there holds the interpreter lock for the
 // whole of it and pulls the interpreter's state to that thread's core, and the next forward pulls it back.
 // A node here takes the lock for a moment: once to count the backward, and in a loss also for the workspace
@@ -58,6 +59,18 @@ struct Entries {
   decltype(&mtp_policy_fwd) policy_fwd = nullptr;
   decltype(&mtp_policy_bwd) policy_bwd = nullptr;
   decltype(&mtp_policy_workspace_bytes) policy_ws = nullptr;
+  decltype(&mtp_logprobs_fwd) logprobs_fwd = nullptr;
+  decltype(&mtp_logprobs_fwd_f32) logprobs_fwd32 = nullptr;
+  decltype(&mtp_logprobs_fwd_workspace_bytes) logprobs_ws = nullptr, logprobs_ws32 = nullptr;
+  decltype(&mtp_logprobs_bwd) logprobs_bwd = nullptr;
+  decltype(&mtp_logprobs_bwd_f32) logprobs_bwd32 = nullptr;
+  decltype(&mtp_distill_fwd) distill_fwd = nullptr;
+  decltype(&mtp_distill_fwd_f32) distill_fwd32 = nullptr;
+  decltype(&mtp_distill_fwd_workspace_bytes) distill_ws = nullptr, distill_ws32 = nullptr;
+  decltype(&mtp_distill_bwd) distill_bwd = nullptr;
+  decltype(&mtp_distill_bwd_f32) distill_bwd32 = nullptr;
+  decltype(&mtp_score_bwd_workspace_bytes) score_bwd_ws = nullptr;
+  decltype(&mtp_score_bwd_f32_workspace_bytes) score_bwd_ws32 = nullptr;
 };
 Entries g_api;
 // Python: the typed error of a return code (_native.check), the call counters of the attention and the
@@ -496,6 +509,223 @@ struct KernelLoss : torch::autograd::Function<KernelLoss> {
   }
 };
 
+// The head of a scoring or distillation call, as core/scoring.py's _Inputs: owner is the weight of the cached transposed copy,
+// fwd_kind what the forward takes it as.
+struct ScoreHead {
+  at::Tensor w, w_q, scales, biases, owner;
+  int64_t kind, fwd_kind;
+  int64_t vocab() const { return w.defined() ? w.size(0) : w_q.size(0); }
+};
+
+at::Tensor bytes_like(const at::Tensor& t, size_t bytes) {
+  return at::empty({(int64_t)std::max<size_t>(bytes, 16)}, t.options().dtype(at::kByte));
+}
+
+// (dL/dhidden, dL/dw): core/scoring.py's _backward. bf16(kind, w_t, d_hidden, d_w, chunk, rows, ws, bytes) and f32(...) call
+// the entry points.
+struct ScoreBackward {
+  at::Tensor d_hidden, d_w, w_t, ws;
+  int64_t kind, chunk, rows;
+  size_t bytes;
+};
+ScoreBackward plan_score_backward(const at::Tensor& hidden, const ScoreHead& h, int64_t k, bool want_dw) {
+  ScoreBackward p;
+  const int64_t n = hidden.size(0), d = hidden.size(1), v = h.vocab();
+  p.d_hidden = at::empty_like(hidden);
+  if (want_dw) p.d_w = at::empty_like(h.w);
+  p.kind = h.kind;
+  p.rows = n;
+  if (hidden.scalar_type() == at::kFloat) {
+    p.chunk = g_api.lce_chunk32(n, d, v, budget_bytes());
+    p.bytes = g_api.score_bwd_ws32(n, d, v, p.chunk, (int)k, want_dw);
+  } else {
+    if (!want_dw || env_is("MTP_LCE_TRANSPOSED_HEAD", "1"))
+      p.w_t = python([&] {
+        const py::handle f(g_transposed_head);
+        const py::object r = f(h.owner, opt_object(h.w), opt_object(h.w_q), opt_object(h.scales), opt_object(h.biases), h.kind, v, d);
+        return r.is_none() ? at::Tensor() : r.cast<at::Tensor>();
+      });
+    const bool staged = !p.w_t.defined() && d % 64 == 0 && !env_is("MTP_LCE_STAGE_HEAD", "0");
+    const size_t budget = budget_bytes();
+    if (staged) {
+      p.kind = h.kind == MTP_HEAD_Q4 ? MTP_HEAD_Q4_STAGED : MTP_HEAD_DENSE_STAGED;
+      p.chunk = g_api.lce_stage_chunk(n, d, v, p.kind, budget);
+    } else {
+      if (!want_dw) p.rows = g_api.lce_row_block(n, d, v, budget);
+      p.chunk = p.rows < n ? (v + 255) / 256 * 256 : g_api.lce_chunk(n, d, v, budget);
+    }
+    p.bytes = g_api.score_bwd_ws(n, d, v, p.kind, p.chunk, p.rows, (int)k, want_dw);
+  }
+  p.ws = bytes_like(hidden, p.bytes);
+  return p;
+}
+
+// What a node keeps of its head: as it is, not as saved tensors (see KernelLoss).
+void keep_head(torch::autograd::AutogradContext* ctx, const ScoreHead& h, const std::optional<at::Tensor>& w) {
+  auto& sd = ctx->saved_data;
+  if (h.w.defined()) sd["w"] = h.w;
+  if (h.w_q.defined()) {
+    sd["w_q"] = h.w_q;
+    sd["scales"] = h.scales;
+    sd["biases"] = h.biases;
+  }
+  sd["owner"] = h.owner;
+  sd["kind"] = h.kind;
+  sd["d_w"] = w.has_value() && w->requires_grad();
+}
+ScoreHead kept_head(torch::autograd::AutogradContext* ctx) {
+  auto& sd = ctx->saved_data;
+  auto tensor = [&](const char* name) { return sd.count(name) ? sd[name].toTensor() : at::Tensor(); };
+  return ScoreHead{tensor("w"), tensor("w_q"), tensor("scales"), tensor("biases"), tensor("owner"), sd["kind"].toInt(), 0};
+}
+
+struct LogprobsCall {
+  ScoreHead head;
+  at::Tensor targets;  // may be missing
+  int64_t ignore_index, top;
+  double temperature;
+};
+
+struct Logprobs : torch::autograd::Function<Logprobs> {
+  // hidden, w and owner: the inputs that may ask for a gradient
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& hidden,
+                                                const std::optional<at::Tensor>& w, const at::Tensor& /*owner*/,
+                                                const LogprobsCall& c) {
+    const c10::DeviceGuard device(hidden.device());
+    const int64_t n = hidden.size(0), d = hidden.size(1), v = c.head.vocab();
+    const bool f32 = hidden.scalar_type() == at::kFloat;
+    const auto opt = hidden.options().dtype(at::kFloat);
+    const at::Tensor entropy = at::empty({n}, opt), kept = at::empty({2, n}, opt);
+    at::Tensor logprobs;
+    float *lse = ptr<float>(kept), *tgt = c.targets.defined() ? lse + n : nullptr;
+    if (c.targets.defined()) logprobs = at::empty({n}, opt);
+    const at::Tensor top = at::empty({n, c.top}, opt), ids = at::empty({n, c.top}, opt.dtype(at::kLong));
+    const size_t bytes = (f32 ? g_api.logprobs_ws32 : g_api.logprobs_ws)(n, d, v, (int)c.head.fwd_kind, (int)c.top);
+    const at::Tensor ws = bytes_like(hidden, bytes);
+    const auto* y = c.targets.defined() ? ptr<int64_t>(c.targets) : nullptr;
+    const ScoreHead& h = c.head;
+    if (f32)
+      check(g_api.logprobs_fwd32(ptr<float>(hidden), opt_ptr<float>(h.w), opt_ptr<uint32_t>(h.w_q), opt_ptr<float>(h.scales),
+                                 opt_ptr<float>(h.biases), y, n, d, v, (int)h.fwd_kind, c.ignore_index, (int)c.top, c.temperature,
+                                 opt_ptr<float>(logprobs), ptr<float>(entropy), ptr<float>(top), ptr<int64_t>(ids), lse, tgt, ptr(ws),
+                                 bytes, stream_of(hidden)),
+            "loss");
+    else
+      check(g_api.logprobs_fwd(ptr(hidden), opt_ptr(h.w), opt_ptr<uint32_t>(h.w_q), opt_ptr(h.scales), opt_ptr(h.biases), y, n, d, v,
+                               (int)h.fwd_kind, c.ignore_index, (int)c.top, c.temperature, opt_ptr<float>(logprobs), ptr<float>(entropy),
+                               ptr<float>(top), ptr<int64_t>(ids), lse, tgt, ptr(ws), bytes, stream_of(hidden)),
+            "loss");
+    ctx->save_for_backward({hidden, c.targets, kept, entropy});
+    keep_head(ctx, h, w);
+    ctx->saved_data["ignore_index"] = c.ignore_index;
+    ctx->saved_data["temperature"] = c.temperature;
+    ctx->mark_non_differentiable({top, ids});
+    ctx->set_materialize_grads(false);
+    if (!c.targets.defined()) return {entropy, top, ids};
+    return {logprobs, entropy, top, ids};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &hidden = saved[0], &targets = saved[1], &kept = saved[2], &entropy = saved[3];
+    const c10::DeviceGuard device(hidden.device());
+    const ScoreHead h = kept_head(ctx);
+    const int64_t n = hidden.size(0), d = hidden.size(1), v = h.vocab(), ignore = ctx->saved_data["ignore_index"].toInt();
+    const double temperature = ctx->saved_data["temperature"].toDouble();
+    const ScoreBackward p = plan_score_backward(hidden, h, 1, ctx->saved_data["d_w"].toBool());
+    at::Tensor d_logprobs, d_entropy;
+    const at::Tensor& g = grads[targets.defined() ? 1 : 0];
+    if (targets.defined() && grads[0].defined()) d_logprobs = grads[0].to(at::kFloat).contiguous();
+    if (g.defined()) d_entropy = g.to(at::kFloat).contiguous();
+    const auto* y = targets.defined() ? ptr<int64_t>(targets) : nullptr;
+    const float *lse = ptr<float>(kept), *tgt = y ? lse + n : nullptr;
+    if (hidden.scalar_type() == at::kFloat)
+      check(g_api.logprobs_bwd32(ptr<float>(hidden), opt_ptr<float>(h.w), opt_ptr<uint32_t>(h.w_q), opt_ptr<float>(h.scales),
+                                 opt_ptr<float>(h.biases), y, n, d, v, (int)p.kind, ignore, temperature, lse, ptr<float>(entropy), tgt,
+                                 opt_ptr<float>(d_logprobs), opt_ptr<float>(d_entropy), ptr<float>(p.d_hidden), opt_ptr<float>(p.d_w),
+                                 p.chunk, ptr(p.ws), p.bytes, stream_of(hidden)),
+            "loss");
+    else
+      check(g_api.logprobs_bwd(ptr(hidden), opt_ptr(h.w), opt_ptr(p.w_t), opt_ptr<uint32_t>(h.w_q), opt_ptr(h.scales), opt_ptr(h.biases),
+                               y, n, d, v, (int)p.kind, ignore, temperature, lse, ptr<float>(entropy), tgt, opt_ptr<float>(d_logprobs),
+                               opt_ptr<float>(d_entropy), ptr(p.d_hidden), opt_ptr(p.d_w), p.chunk, p.rows, ptr(p.ws), p.bytes,
+                               stream_of(hidden)),
+            "loss");
+    return once(grads, {p.d_hidden, p.d_w, at::Tensor(), at::Tensor()});
+  }
+};
+
+struct DistillCall {
+  ScoreHead head;
+  at::Tensor ids, teacher, mask;  // mask may be missing
+  int64_t kind, renormalize, reduction;
+  double beta, temperature;
+};
+
+struct Distillation : torch::autograd::Function<Distillation> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& hidden, const std::optional<at::Tensor>& w,
+                            const at::Tensor& /*owner*/, const DistillCall& c) {
+    const c10::DeviceGuard device(hidden.device());
+    const int64_t n = hidden.size(0), d = hidden.size(1), v = c.head.vocab(), k = c.ids.size(1);
+    const bool f32 = hidden.scalar_type() == at::kFloat;
+    const auto opt = hidden.options().dtype(at::kFloat);
+    const at::Tensor loss = c.reduction == MTP_REDUCE_NONE ? at::empty({n}, opt) : at::empty({}, opt);
+    // lse, a factor per token, a factor and a column (int32) per slot, the scale
+    const at::Tensor kept = at::empty({2 * n * (k + 1) + 1}, opt);
+    float *lse = ptr<float>(kept), *rest = lse + n, *coef = rest + n, *columns = coef + n * k, *scale = columns + n * k;
+    const size_t bytes = (f32 ? g_api.distill_ws32 : g_api.distill_ws)(n, d, v, (int)c.head.fwd_kind, (int)k);
+    const at::Tensor ws = bytes_like(hidden, bytes);
+    const ScoreHead& h = c.head;
+    const auto* ids = ptr<int64_t>(c.ids);
+    const auto* mask = static_cast<const uint8_t*>(opt_ptr(c.mask));
+    if (f32)
+      check(g_api.distill_fwd32(ptr<float>(hidden), opt_ptr<float>(h.w), opt_ptr<uint32_t>(h.w_q), opt_ptr<float>(h.scales),
+                                opt_ptr<float>(h.biases), ids, ptr<float>(c.teacher), mask, n, d, v, (int)h.fwd_kind, (int)k, (int)c.kind,
+                                c.beta, c.temperature, (int)c.renormalize, (int)c.reduction, ptr<float>(loss), scale, lse, rest, coef,
+                                reinterpret_cast<int32_t*>(columns), ptr(ws), bytes, stream_of(hidden)),
+            "loss");
+    else
+      check(g_api.distill_fwd(ptr(hidden), opt_ptr(h.w), opt_ptr<uint32_t>(h.w_q), opt_ptr(h.scales), opt_ptr(h.biases), ids,
+                              ptr<float>(c.teacher), mask, n, d, v, (int)h.fwd_kind, (int)k, (int)c.kind, c.beta, c.temperature,
+                              (int)c.renormalize, (int)c.reduction, ptr<float>(loss), scale, lse, rest, coef,
+                              reinterpret_cast<int32_t*>(columns), ptr(ws), bytes, stream_of(hidden)),
+            "loss");
+    ctx->save_for_backward({hidden, kept});
+    keep_head(ctx, h, w);
+    ctx->saved_data["k"] = k;
+    ctx->saved_data["reduction"] = c.reduction;
+    ctx->saved_data["temperature"] = c.temperature;
+    return loss;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &hidden = saved[0], &kept = saved[1];
+    const c10::DeviceGuard device(hidden.device());
+    const ScoreHead h = kept_head(ctx);
+    auto& sd = ctx->saved_data;
+    const int64_t n = hidden.size(0), d = hidden.size(1), v = h.vocab(), k = sd["k"].toInt();
+    const int reduction = (int)sd["reduction"].toInt();
+    const double temperature = sd["temperature"].toDouble();
+    const ScoreBackward p = plan_score_backward(hidden, h, k, sd["d_w"].toBool());
+    const at::Tensor ct = grads[0].to(at::kFloat).contiguous();
+    const float *lse = ptr<float>(kept), *rest = lse + n, *coef = rest + n, *columns = coef + n * k, *scale = columns + n * k;
+    if (hidden.scalar_type() == at::kFloat)
+      check(g_api.distill_bwd32(ptr<float>(hidden), opt_ptr<float>(h.w), opt_ptr<uint32_t>(h.w_q), opt_ptr<float>(h.scales),
+                                opt_ptr<float>(h.biases), n, d, v, (int)p.kind, (int)k, temperature, reduction, ptr<float>(ct), scale, lse,
+                                rest, coef, reinterpret_cast<const int32_t*>(columns), ptr<float>(p.d_hidden), opt_ptr<float>(p.d_w),
+                                p.chunk, ptr(p.ws), p.bytes, stream_of(hidden)),
+            "loss");
+    else
+      check(g_api.distill_bwd(ptr(hidden), opt_ptr(h.w), opt_ptr(p.w_t), opt_ptr<uint32_t>(h.w_q), opt_ptr(h.scales), opt_ptr(h.biases),
+                              n, d, v, (int)p.kind, (int)k, temperature, reduction, ptr<float>(ct), scale, lse, rest, coef,
+                              reinterpret_cast<const int32_t*>(columns), ptr(p.d_hidden), opt_ptr(p.d_w), p.chunk, p.rows, ptr(p.ws),
+                              p.bytes, stream_of(hidden)),
+            "loss");
+    return once(grads, {p.d_hidden, p.d_w, at::Tensor(), at::Tensor()});
+  }
+};
+
 // The node's result for a Python caller: typed errors as they are.
 template <class F>
 auto apply_node(F&& f) {
@@ -555,6 +785,27 @@ std::vector<at::Tensor> policy(const at::Tensor& nll, const at::Tensor& old, con
   return apply_node([&] { return Policy::apply(nll, call); });
 }
 
+std::vector<at::Tensor> logprobs(const at::Tensor& hidden, const std::optional<at::Tensor>& w, const std::optional<at::Tensor>& w_q,
+                                 const std::optional<at::Tensor>& scales, const std::optional<at::Tensor>& biases, int64_t kind,
+                                 const at::Tensor& owner, int64_t fwd_kind, const std::optional<at::Tensor>& targets,
+                                 int64_t ignore_index, int64_t top, double temperature) {
+  const at::Tensor none;
+  const LogprobsCall call{{w.value_or(none), w_q.value_or(none), scales.value_or(none), biases.value_or(none), owner, kind, fwd_kind},
+                          targets.value_or(none), ignore_index, top, temperature};
+  return apply_node([&] { return Logprobs::apply(hidden, w, owner, call); });
+}
+
+at::Tensor distillation(const at::Tensor& hidden, const std::optional<at::Tensor>& w, const std::optional<at::Tensor>& w_q,
+                        const std::optional<at::Tensor>& scales, const std::optional<at::Tensor>& biases, int64_t kind,
+                        const at::Tensor& owner, int64_t fwd_kind, const at::Tensor& ids, const at::Tensor& teacher,
+                        const std::optional<at::Tensor>& mask, int64_t loss_kind, double beta, double temperature,
+                        int64_t renormalize, int64_t reduction) {
+  const at::Tensor none;
+  const DistillCall call{{w.value_or(none), w_q.value_or(none), scales.value_or(none), biases.value_or(none), owner, kind, fwd_kind},
+                         ids, teacher, mask.value_or(none), loss_kind, renormalize, reduction, beta, temperature};
+  return apply_node([&] { return Distillation::apply(hidden, w, owner, call); });
+}
+
 void bind(const py::dict& entries, py::object check_fn) {
   auto set = [&](auto& f, const char* name) {
     f = reinterpret_cast<std::remove_reference_t<decltype(f)>>(entries[name].cast<uintptr_t>());
@@ -594,6 +845,20 @@ void bind(const py::dict& entries, py::object check_fn) {
   set(g_api.policy_fwd, "mtp_policy_fwd");
   set(g_api.policy_bwd, "mtp_policy_bwd");
   set(g_api.policy_ws, "mtp_policy_workspace_bytes");
+  set(g_api.logprobs_fwd, "mtp_logprobs_fwd");
+  set(g_api.logprobs_fwd32, "mtp_logprobs_fwd_f32");
+  set(g_api.logprobs_ws, "mtp_logprobs_fwd_workspace_bytes");
+  set(g_api.logprobs_ws32, "mtp_logprobs_fwd_f32_workspace_bytes");
+  set(g_api.logprobs_bwd, "mtp_logprobs_bwd");
+  set(g_api.logprobs_bwd32, "mtp_logprobs_bwd_f32");
+  set(g_api.distill_fwd, "mtp_distill_fwd");
+  set(g_api.distill_fwd32, "mtp_distill_fwd_f32");
+  set(g_api.distill_ws, "mtp_distill_fwd_workspace_bytes");
+  set(g_api.distill_ws32, "mtp_distill_fwd_f32_workspace_bytes");
+  set(g_api.distill_bwd, "mtp_distill_bwd");
+  set(g_api.distill_bwd32, "mtp_distill_bwd_f32");
+  set(g_api.score_bwd_ws, "mtp_score_bwd_workspace_bytes");
+  set(g_api.score_bwd_ws32, "mtp_score_bwd_f32_workspace_bytes");
   g_check = check_fn.release().ptr();
 }
 void bind_attention(py::object calls) { g_attn_calls = calls.release().ptr(); }
@@ -615,4 +880,6 @@ PYBIND11_MODULE(_mtp_torch, m) {
   m.def("scored_attention", &scored_attention);
   m.def("preference", &preference);
   m.def("policy", &policy);
+  m.def("logprobs", &logprobs);
+  m.def("distillation", &distillation);
 }

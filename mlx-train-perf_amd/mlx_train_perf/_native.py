@@ -204,7 +204,7 @@ def _bind_nodes(lib):
             warnings.warn(f"{path} cannot be loaded ({e}); calls take the Python autograd functions. Run "
                           "`python -c \"import __graft_entry__ as g; g.build()\"` from the repository root.", stacklevel=2)
         return False
-    if not hasattr(_mtp_torch, "preference"):   # an older build, which grows by new nodes
+    if not hasattr(_mtp_torch, "distillation"):   # an older build, which grows by new nodes
         warnings.warn(f"{_mtp_torch.__file__} is from older sources; calls take the Python autograd functions. Run "
                       "`python -c \"import __graft_entry__ as g; g.build()\"` from the repository root.", stacklevel=2)
         return False

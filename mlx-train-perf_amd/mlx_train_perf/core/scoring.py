@@ -116,6 +116,12 @@ def _inputs(hidden2: torch.Tensor, head: HeadRef) -> _Inputs:
                    _native.HEAD_Q4, head.w_q)
 
 
+def _nodes(x: _Inputs):
+    """The C++ nodes, for plain tensors; None: the Python Functions serve the call, the same bits."""
+    plain = _native.plain(*(t for t in (x.hidden, x.w, x.w_q, x.scales, x.biases, x.owner) if t is not None))
+    return _native.nodes() if plain else None
+
+
 def _forward_kind(x: _Inputs) -> int:
     """As the loss's forward: a 4-bit head dequantized into the workspace where the budget holds all of it."""
     n, d = x.hidden.shape
@@ -379,12 +385,10 @@ def token_logprobs(hidden: torch.Tensor, head: HeadRef, targets: torch.Tensor | 
         x = _inputs(hidden2, head)
         y = None if targets2 is None else targets2.to(torch.int64).contiguous()
         args = (y, int(ignore_index), top, temperature)
-        needs = x.hidden.requires_grad or (x.w is not None and x.w.requires_grad)
-        if needs and torch.is_grad_enabled():
-            parts = _TokenLogprobs.apply(*x, *args)
-        else:
-            parts = _score_forward(x, *args)[:4]
-    logprobs, entropy, top_lp, top_ids = parts
+        nodes = _nodes(x)
+        parts = _TokenLogprobs.apply(*x, *args) if nodes is None else nodes.logprobs(*x, _forward_kind(x), *args)
+    *logprobs, entropy, top_lp, top_ids = parts   # (the node has none without targets)
+    logprobs = logprobs[0] if logprobs else None
     return TokenLogprobs(None if logprobs is None else logprobs.view(leading), entropy.view(leading),
                          top_lp.view(*leading, top), top_ids.view(*leading, top))
 
@@ -441,7 +445,9 @@ def distillation_loss(hidden: torch.Tensor, head: HeadRef, teacher_ids: torch.Te
     if _resolve(hidden2, head, others, impl, ("lists", k), allow_unverified_mlx) == "reference":
         loss = _reference_distillation(hidden2, head, ids2, teacher2, mask2, kind, beta, temperature, renormalize, reduction)
     else:
-        loss = _Distillation.apply(*_inputs(hidden2, head), ids2.to(torch.int64).contiguous(), _float(teacher2),
-                                   None if mask2 is None else mask2.contiguous(), _KINDS[kind], float(beta), temperature,
-                                   int(renormalize), _REDUCTIONS[reduction])
+        x = _inputs(hidden2, head)
+        args = (ids2.to(torch.int64).contiguous(), _float(teacher2), None if mask2 is None else mask2.contiguous(), _KINDS[kind],
+                float(beta), temperature, int(renormalize), _REDUCTIONS[reduction])
+        nodes = _nodes(x)
+        loss = _Distillation.apply(*x, *args) if nodes is None else nodes.distillation(*x, _forward_kind(x), *args)
     return loss.view(leading) if reduction == "none" else loss

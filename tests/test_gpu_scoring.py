@@ -360,6 +360,52 @@ def test_runs_repeat_bit_for_bit(n):
 
 
 @pytest.mark.parametrize("n", [6, 300])
+def test_the_python_functions_give_the_same_bits(n, monkeypatch):
+    """Both autograd paths, with targets and without, each loss, each head."""
+    from mlx_train_perf import _native
+
+    def run():
+        out = []
+        for head, dtype in (("dense", "bf16"), ("trainable", "bf16"), ("q4", "bf16"), ("trainable", "fp32")):
+            hidden, hd, _ = S.make(n, 64, 500, head=head, dtype=dtype, seed=11)
+            hd = S.to(hd, "cuda")
+            h = hidden.cuda().requires_grad_(True)
+            leaves = [h] + ([hd.weight] if head == "trainable" else [])
+            ids, lp, mask = (x.cuda() for x in S.teacher_list(n, 500, 6, seed=11))
+            for y in (None, _targets(n, 500, 11).cuda()):
+                r = token_logprobs(h, hd, y, top=3, temperature=1.2)
+                out += [x.detach() for x in r if x is not None]
+                out += torch.autograd.grad(r.entropy.sum() + (0 if y is None else (r.logprobs * 0.3).sum()), leaves)
+            for kind in ("forward", "reverse", "jsd"):
+                loss = distillation_loss(h, hd, ids, lp, mask=mask, kind=kind)
+                out += [loss.detach(), *torch.autograd.grad(loss * 3, leaves)]
+        return out
+
+    assert _native.nodes() is not None
+    nodes = run()
+    monkeypatch.setattr(_native, "_nodes", False)
+    assert _native.nodes() is None
+    assert all(torch.equal(a, b) for a, b in zip(run(), nodes, strict=True))
+
+
+def test_no_second_derivative(monkeypatch):
+    """Asked for, it raises in both autograd paths and is not taken for 0."""
+    from mlx_train_perf import _native
+
+    hidden, hd, _ = S.make(5, 64, 100)
+    hd = S.to(hd, "cuda")
+    ids, lp, _ = (x.cuda() for x in S.teacher_list(5, 100, 4, holes=False))
+    for nodes in (_native.nodes(), False):
+        monkeypatch.setattr(_native, "_nodes", nodes)
+        h = hidden.cuda().requires_grad_(True)
+        for f in (lambda: token_logprobs(h, hd).entropy.sum(), lambda: distillation_loss(h, hd, ids, lp)):
+            ct = torch.ones((), device="cuda", requires_grad=True)
+            (g,) = torch.autograd.grad(f(), h, ct, create_graph=True)
+            with pytest.raises(RuntimeError, match="once_differentiable"):
+                g.float().sum().backward()
+
+
+@pytest.mark.parametrize("n", [6, 300])
 def test_on_another_stream(n):
     step, _, _ = _steps(n)
     first = step()
