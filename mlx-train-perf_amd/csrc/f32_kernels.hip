@@ -336,7 +336,8 @@ void lce32_fwd_kernel(const float* __restrict__ H, const float* __restrict__ W,
                                                         const uint32_t* __restrict__ Wq, const float* __restrict__ Sc,
                                                         const float* __restrict__ Bi, int N, int D, int V, int nsplit,
                                                         float* __restrict__ part_m, float* __restrict__ part_s, float scale2,
-                                                        float* __restrict__ part_u, float* __restrict__ gmax, int ldg) {
+                                                        float* __restrict__ part_u, float* __restrict__ gmax, int ldg,
+                                                        ScoreList list) {
   const float c2 = STAT ? scale2 : kLog2e;
   constexpr float kHidden = (STAT & kStatEntropy) ? -1e30f : kNegInf;
   __shared__ float gx[(STAT & kStatGroups) ? kT : 1];
@@ -350,6 +351,9 @@ void lce32_fwd_kernel(const float* __restrict__ H, const float* __restrict__ W,
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, wa = w & 1, wb = w >> 1, h = lane >> 5;
   RowSrc hb{H + (long)t0 * D, D, N - t0, D, aligned16(H) && D % 4 == 0};
   float m[2] = {kNegInf, kNegInf}, s[2] = {0.f, 0.f}, u[2] = {0.f, 0.f};
+  ListCursor<2> cursor;
+  const int tokens[2] = {t0 + 64 * wb + (lane & 31), t0 + 64 * wb + 32 + (lane & 31)};
+  if constexpr (STAT & kStatList) cursor.start(list, tokens, N, vt0 * kT);
   for (int vt = vt0; vt < vt1; ++vt) {
     const int v0 = vt * kT;
     f32x16 acc[2][2];
@@ -397,6 +401,7 @@ void lce32_fwd_kernel(const float* __restrict__ H, const float* __restrict__ W,
       s[j] = s[j] * f + sum;
       m[j] = mn;
     }
+    if constexpr (STAT & kStatList) cursor.tile<kT>(list, tokens, acc, v0, 64 * wa, h);
   }
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
@@ -768,19 +773,19 @@ static bool copied_tiles(long d, long ld) { return d % 4 == 0 && ld % 4 == 0 && 
 
 template <int STAT>
 static hipError_t lce32_fwd_tiles(const LceHead32& h, const float* H, int N, int D, int V, float* pm, float* ps, float scale2,
-                                  float* pu, float* gmax, int ldg, hipStream_t st) {
+                                  float* pu, float* gmax, int ldg, const ScoreList& list, hipStream_t st) {
   const int ns = lce32_fwd_nsplit(N, V);
   auto kernel = h.q4 ? lce32_fwd_kernel<kQ4, STAT> : copied_tiles(D, D) ? lce32_fwd_kernel<kCopied, STAT> : lce32_fwd_kernel<kDense, STAT>;
   hipLaunchKernelGGL(kernel, dim3((N + kT - 1) / kT, ns), dim3(256), 0, st, H, h.w, h.wq, h.sc, h.bi, N, D, V, ns, pm, ps,
-                     scale2, pu, gmax, ldg);
+                     scale2, pu, gmax, ldg, list);
   return hipGetLastError();
 }
 
 hipError_t launch_lce32_stats(const LceHead32& h, const float* H, int N, int D, int V, const ScoreStats& x, hipStream_t st) {
   if (x.gmax)
-    return lce32_fwd_tiles<kStatScaled | kStatEntropy | kStatGroups>(h, H, N, D, V, x.m, x.s, x.scale2, x.u, x.gmax, x.ldg, st);
-  if (x.u) return lce32_fwd_tiles<kStatScaled | kStatEntropy>(h, H, N, D, V, x.m, x.s, x.scale2, x.u, nullptr, 0, st);
-  return lce32_fwd_tiles<kStatScaled>(h, H, N, D, V, x.m, x.s, x.scale2, nullptr, nullptr, 0, st);
+    return lce32_fwd_tiles<kStatScaled | kStatEntropy | kStatGroups>(h, H, N, D, V, x.m, x.s, x.scale2, x.u, x.gmax, x.ldg, x.list, st);
+  if (x.u) return lce32_fwd_tiles<kStatScaled | kStatEntropy>(h, H, N, D, V, x.m, x.s, x.scale2, x.u, nullptr, 0, x.list, st);
+  return lce32_fwd_tiles<kStatScaled | kStatList>(h, H, N, D, V, x.m, x.s, x.scale2, nullptr, nullptr, 0, x.list, st);
 }
 
 hipError_t launch_lce32_target(const LceHead32& h, const float* H, const int64_t* targets, int N, int D, int V, float* tgt,
@@ -802,7 +807,7 @@ hipError_t launch_lce32_fwd(const LceHead32& h, const float* H, const int64_t* t
   const int ns = lce32_fwd_nsplit(N, V);
   float* pm = ws;
   float* ps = ws + (long)ns * N;
-  hipError_t e = lce32_fwd_tiles<0>(h, H, N, D, V, pm, ps, 0.f, nullptr, nullptr, 0, st);
+  hipError_t e = lce32_fwd_tiles<0>(h, H, N, D, V, pm, ps, 0.f, nullptr, nullptr, 0, ScoreList{}, st);
   if (e != hipSuccess) return e;
   const dim3 block(256);
   dim3 fgrid((N + 3) / 4);

@@ -21,6 +21,7 @@
 
 #include "mtp_common.hpp"
 #include "mtp_launch.hpp"
+#include "score_gather.hpp"
 
 namespace mtp {
 
@@ -887,7 +888,8 @@ __device__ __forceinline__ bool xcd_rect_tile(int mtiles, int ntiles, int& m, in
 //
 // STAT (mtp_launch.hpp, kStat...) is what token scoring wants beside it: the softmax of z / temperature (scale2 =
 // log2(e) / temperature), the sum of 2^(x - m) (x - m) that the entropy is made of (an fma per logit), and the maximum of
-// every group of kGroup logits, which the tile's own maximum holds already. 0 is the loss as it was.
+// every group of kGroup logits, which the tile's own maximum holds already; or the logits of a list of columns a row
+// (ListCursor). 0 is the loss as it was.
 // ------------------------------------------------------------------------------------------
 template <int Q4, int STAT = 0>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
@@ -895,7 +897,7 @@ void lce_fwd_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
                     const uint32_t* __restrict__ Wq, const bf16_t* __restrict__ Sc,
                     const bf16_t* __restrict__ Bi, int N, int D, int V, int nsplit, int split0, int nlocal,
                     int wrow0, float* __restrict__ part_m, float* __restrict__ part_s, float scale2,
-                    float* __restrict__ part_u, float* __restrict__ gmax, int ldg) {
+                    float* __restrict__ part_u, float* __restrict__ gmax, int ldg, ScoreList list) {
   const float c2 = STAT ? scale2 : kLog2e;
   // Hidden rows past V: beyond any logit, but finite where 0 of it has to be 0.
   constexpr float kHidden = (STAT & kStatEntropy) ? -1e30f : kNegInf;
@@ -936,6 +938,14 @@ void lce_fwd_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
     m[j] = kNegInf;
     s[j] = 0.f;
     u[j] = 0.f;
+  }
+
+  ListCursor<kNJ> cursor;
+  int tokens[kNJ];
+  if constexpr (STAT & kStatList) {
+#pragma unroll
+    for (int j = 0; j < kNJ; ++j) tokens[j] = t0 + 64 * wb + 32 * j + lcol;
+    cursor.start(list, tokens, N, vt_begin * kTile);
   }
 
   // Online (max, sum exp2) update of this lane's token columns with one 256-row vocab tile, in the
@@ -1005,6 +1015,7 @@ void lce_fwd_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
       s[j] = s[j] * f + sum;
       m[j] = mn[j];
     }
+    if constexpr (STAT & kStatList) cursor.tile<kTile>(list, tokens, acc, v0, 128 * wa, lhalf);
   };
 
   if (!Q4 && D % kBK == 0) {
@@ -2159,7 +2170,8 @@ long lce_fwd_stage_rows_used(long N, long V, long stage_rows) {
 // The forward's tiles: partials part_m, part_s (and what STAT adds, else null) [splits][N].
 template <int STAT>
 static hipError_t lce_fwd_tiles(const LceHead& h, const bf16_t* H, int N, int D, int V, float* pm, float* ps, float scale2,
-                                float* pu, float* gmax, int ldg, bf16_t* stage, long stage_rows, hipStream_t stream) {
+                                float* pu, float* gmax, int ldg, const ScoreList& list, bf16_t* stage,
+                                long stage_rows, hipStream_t stream) {
   const int ns = lce_fwd_nsplit(N, V);
   const int rtiles = (N + kTile - 1) / kTile;
   dim3 block(kThreads);
@@ -2178,17 +2190,17 @@ static hipError_t lce_fwd_tiles(const LceHead& h, const bf16_t* H, int N, int D,
       hipError_t de = hipGetLastError();
       if (de != hipSuccess) return de;
       hipLaunchKernelGGL((lce_fwd_kernel<0, STAT>), dim3(rtiles * (s1 - s0)), block, 0, stream, H, stage, h.wq, h.sc, h.bi,
-                         N, D, V, ns, s0, s1 - s0, (int)r0, pm, ps, scale2, pu, gmax, ldg);
+                         N, D, V, ns, s0, s1 - s0, (int)r0, pm, ps, scale2, pu, gmax, ldg, list);
       de = hipGetLastError();
       if (de != hipSuccess) return de;
       s0 = s1;
     }
   } else if (h.q4) {
     hipLaunchKernelGGL((lce_fwd_kernel<1, STAT>), dim3(rtiles * ns), block, 0, stream, H, h.w, h.wq, h.sc, h.bi, N, D, V,
-                       ns, 0, ns, 0, pm, ps, scale2, pu, gmax, ldg);
+                       ns, 0, ns, 0, pm, ps, scale2, pu, gmax, ldg, list);
   } else {
     hipLaunchKernelGGL((lce_fwd_kernel<0, STAT>), dim3(rtiles * ns), block, 0, stream, H, h.w, h.wq, h.sc, h.bi, N, D, V,
-                       ns, 0, ns, 0, pm, ps, scale2, pu, gmax, ldg);
+                       ns, 0, ns, 0, pm, ps, scale2, pu, gmax, ldg, list);
   }
   return hipGetLastError();
 }
@@ -2196,12 +2208,12 @@ static hipError_t lce_fwd_tiles(const LceHead& h, const bf16_t* H, int N, int D,
 hipError_t launch_lce_stats(const LceHead& h, const bf16_t* H, int N, int D, int V, const ScoreStats& st, bf16_t* stage,
                             long stage_rows, hipStream_t stream) {
   auto tiles = [&](auto stat) {
-    return lce_fwd_tiles<decltype(stat)::value>(h, H, N, D, V, st.m, st.s, st.scale2, st.u, st.gmax, st.ldg, stage, stage_rows,
-                                                stream);
+    return lce_fwd_tiles<decltype(stat)::value>(h, H, N, D, V, st.m, st.s, st.scale2, st.u, st.gmax, st.ldg, st.list, stage,
+                                                stage_rows, stream);
   };
   if (st.gmax) return tiles(std::integral_constant<int, kStatScaled | kStatEntropy | kStatGroups>{});
   if (st.u) return tiles(std::integral_constant<int, kStatScaled | kStatEntropy>{});
-  return tiles(std::integral_constant<int, kStatScaled>{});
+  return tiles(std::integral_constant<int, kStatScaled | kStatList>{});
 }
 
 hipError_t launch_lce_fwd(const LceHead& h, const bf16_t* H, const int64_t* targets, int N, int D, int V,
@@ -2210,7 +2222,7 @@ hipError_t launch_lce_fwd(const LceHead& h, const bf16_t* H, const int64_t* targ
   const int ns = lce_fwd_nsplit(N, V);
   float* pm = ws;
   float* ps = ws + (long)ns * N;
-  hipError_t e = lce_fwd_tiles<0>(h, H, N, D, V, pm, ps, 0.f, nullptr, nullptr, 0, stage, stage_rows, stream);
+  hipError_t e = lce_fwd_tiles<0>(h, H, N, D, V, pm, ps, 0.f, nullptr, nullptr, 0, ScoreList{}, stage, stage_rows, stream);
   if (e != hipSuccess) return e;
   dim3 fgrid((N + 3) / 4), fblock(256);
   if (h.q4) {

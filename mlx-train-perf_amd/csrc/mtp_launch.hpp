@@ -57,14 +57,22 @@ hipError_t launch_lce_fwd(const LceHead& h, const bf16_t* H, const int64_t* targ
                           bf16_t* stage, long stage_rows, hipStream_t stream);
 
 // Token scoring (score_kernels.hip) takes the forward's tiles with more of their statistics. A forward's STAT is a sum of:
-enum { kStatScaled = 1, kStatEntropy = 2, kStatGroups = 4 };
+enum { kStatScaled = 1, kStatEntropy = 2, kStatGroups = 4, kStatList = 8 };
 constexpr int kGroup = 128;  // consecutive logits whose maximum a forward keeps
+// Logits to keep of each row: ascending columns (kNoColumn past the last) to their places in z.
+constexpr int kNoColumn = 0x7fffffff;
+struct ScoreList {
+  const int* column;  // [N][k], or null
+  float* z;           // [N][k]
+  int k;
+};
 struct ScoreStats {
   float scale2;        // log2(e) / temperature: the partials are of x = z scale2
   float *m, *s;        // [lce_fwd_nsplit][N] maximum of x, sum of 2^(x - m)
   float* u;            // the same of 2^(x - m) (x - m), or null
   float* gmax;         // [N][ldg] the maximum z of each group of kGroup (ldg: an even number of them), or null (with u)
   int ldg;
+  ScoreList list;
 };
 hipError_t launch_lce_stats(const LceHead& h, const bf16_t* H, int N, int D, int V, const ScoreStats& st, bf16_t* stage,
                             long stage_rows, hipStream_t stream);
@@ -177,9 +185,8 @@ hipError_t launch_attn32_bwd(const AttnShape& sh, const float* q, const float* k
                              const float* lse, const float* d_o, const int32_t* seg_start, float* dq, float* dk,
                              float* dv, float* dvec, int nsplit, hipStream_t stream);
 
-// Token scoring and distillation (score_kernels.hip). Logits are recomputed for single tokens and groups of kGroup logits:
-// an entry is a token and what to keep of it, code >= 0: the whole group, to rows[code][kGroup]; code < 0: one logit,
-// column (-1 - code) % kGroup of the group, to picks[(-1 - code) / kGroup]. A tile is up to kGroup entries of one group.
+// Token scoring and distillation (score_kernels.hip). The logits of groups of kGroup that single tokens want are formed
+// again: an entry is a token (x) and the place of its group in rows (y); a tile is up to kGroup entries of one group.
 struct GatherTile {
   int group, first, count, unused;
 };
@@ -187,7 +194,7 @@ struct GatherPlan {
   const int2* entries;
   const GatherTile* tiles;  // [max_tiles], with count 0 past the last
   int max_tiles;
-  float *rows, *picks;
+  float* rows;              // [entries][kGroup]
 };
 hipError_t launch_lce_gather(const LceHead& h, const bf16_t* H, int D, int V, const GatherPlan& p, hipStream_t stream);
 hipError_t launch_lce32_gather(const LceHead32& h, const float* H, int D, int V, const GatherPlan& p, hipStream_t stream);

@@ -5,8 +5,8 @@
 
 namespace mtp {
 
-// A wave's logits acc[i][j], rows v = row0 + 32 i + (register's row) of the group, columns entries col0 + 32 j + lane % 32: to
-// rows[code] (16 bytes a lane; rows past the vocabulary as -inf), or for a single logit the register that holds it.
+// A wave's logits acc[i][j], rows v = row0 + 32 i + (register's row) of the group, columns entries col0 + 32 j + lane % 32: 16
+// bytes a lane; rows past the vocabulary as -inf.
 template <int NI, int NJ>
 __device__ __forceinline__ void store_gathered(const f32x16 (&acc)[NI][NJ], const GatherPlan& plan, const int2* entries,
                                                int count, int vleft, int row0, int col0, int lane) {
@@ -14,35 +14,78 @@ __device__ __forceinline__ void store_gathered(const f32x16 (&acc)[NI][NJ], cons
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
     const int e = col0 + 32 * j + (lane & 31);
-    const int code = e < count ? entries[e].y : 0;
     if (e >= count) continue;
-    if (code >= 0) {
-      float* dst = plan.rows + (long)code * kGroup;
+    float* dst = plan.rows + (long)entries[e].y * kGroup;
 #pragma unroll
-      for (int i = 0; i < NI; ++i)
+    for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int v = row0 + 32 * i + 8 * q + 4 * h;
-          f32x4 x;
+      for (int q = 0; q < 4; ++q) {
+        const int v = row0 + 32 * i + 8 * q + 4 * h;
+        f32x4 x;
 #pragma unroll
-          for (int u = 0; u < 4; ++u) x[u] = v + u < vleft ? acc[i][j][4 * q + u] : kNegInf;
-          *reinterpret_cast<f32x4*>(dst + v) = x;
-        }
-    } else {
-      const int want = (-1 - code) % kGroup - row0;
-      float x = 0.f;
-      bool here = false;
-#pragma unroll
-      for (int i = 0; i < NI; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (want == 32 * i + 8 * (r >> 2) + 4 * h + (r & 3)) {
-            x = acc[i][j][r];
-            here = true;
-          }
-      if (here) plan.picks[(-1 - code) / kGroup] = x;
-    }
+        for (int u = 0; u < 4; ++u) x[u] = v + u < vleft ? acc[i][j][4 * q + u] : kNegInf;
+        *reinterpret_cast<f32x4*>(dst + v) = x;
+      }
   }
 }
+
+// ------------------------------------------------------------------------------------------
+// A forward's listed logits (ScoreList). Each lane follows its token columns' lists up the vocabulary: `next` is the first
+// listed column that no tile has passed, `at` its place. A tile's lanes hold the logits of column li = 32 i + 8 (r / 4) + 4 half
+// + r % 4 of their wave's part of it, so a listed one is in one lane and one of 16 NI registers: a tree of selects by the bits
+// of li finds it (16 NI of them), a store puts it away. Most tiles have none of a wave's tokens' columns, and the rest few.
+// ------------------------------------------------------------------------------------------
+// acc[BITS' registers from `first`], the one whose index has the bits of li: register bits 0, 1 are bits 0, 1 of li, the ones
+// above are its bits 3 and on.
+template <int BITS, int NI, int NJ>
+__device__ __forceinline__ float select_logit(const f32x16 (&acc)[NI][NJ], int j, int li, int first) {
+  if constexpr (BITS == 0) {
+    return acc[first >> 4][j][first & 15];
+  } else {
+    const float lo = select_logit<BITS - 1>(acc, j, li, first), hi = select_logit<BITS - 1>(acc, j, li, first + (1 << (BITS - 1)));
+    const int bit = BITS - 1 < 2 ? BITS - 1 : BITS;
+    return (li >> bit) & 1 ? hi : lo;
+  }
+}
+
+template <int NJ>
+struct ListCursor {
+  int next[NJ], at[NJ];
+  // The first listed columns of the tokens t[j] (valid: below N) from v0 on.
+  __device__ __forceinline__ void start(const ScoreList& l, const int (&t)[NJ], int N, int v0) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      next[j] = kNoColumn;
+      at[j] = 0;
+      if (t[j] >= N) continue;
+      const int* row = l.column + (long)t[j] * l.k;
+      int lo = 0, hi = l.k;
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (row[mid] < v0) lo = mid + 1;
+        else hi = mid;
+      }
+      at[j] = lo;
+      if (lo < l.k) next[j] = row[lo];
+    }
+  }
+  // The tile [v0, v0 + SIZE): the wave holds its rows [part, part + 32 NI).
+  template <int SIZE, int NI>
+  __device__ __forceinline__ void tile(const ScoreList& l, const int (&t)[NJ], const f32x16 (&acc)[NI][NJ], int v0, int part, int half) {
+    constexpr int kBits = NI == 4 ? 6 : 5;
+    static_assert(NI == 4 || NI == 2, "16 NI registers");
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+      while (__any(next[j] < v0 + SIZE)) {
+        if (next[j] < v0 + SIZE) {
+          const int li = next[j] - v0 - part;
+          const float z = select_logit<kBits>(acc, j, li, 0);
+          if (li >= 0 && li < 32 * NI && ((li >> 2) & 1) == half) l.z[(long)t[j] * l.k + at[j]] = z;
+          ++at[j];
+          next[j] = at[j] < l.k ? l.column[(long)t[j] * l.k + at[j]] : kNoColumn;
+        }
+      }
+  }
+};
 
 }  // namespace mtp

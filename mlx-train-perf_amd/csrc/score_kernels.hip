@@ -8,9 +8,9 @@
 // alternatives, the maximum of every group of kGroup consecutive logits. The `top` largest logits of a row lie in the
 // groups with the `top` largest maxima (a logit outside them has `top` at least as large ahead of it; equal maxima go to the
 // lower group, so equal logits to the lower index). So: choose those groups, form their logits again (a product over
-// the tokens that want each group: top kGroup / V of the first one, 0.7% for 8 of 151936), choose among them. The logits of a
-// teacher's list are formed the same way, one per entry. The product's k order is the forward's, so a logit has the same bits
-// in both: what is left of 1 after a list's probabilities is exact to fp32 and not to two roundings of a large logit.
+// the tokens that want each group: top kGroup / V of the first one, 0.7% for 8 of 151936, in its k order and to its bits),
+// choose among them. The logits of a teacher's list, sorted first, the product's tiles put away as they pass (ListCursor): the
+// very ones that the sums hold, so that what a list leaves of 1 is exact to fp32 and not to two roundings of a large logit.
 //
 // Up to kFewTokens tokens the logits themselves are kept in the workspace (lce_few_kernel), which leaves two launches.
 #include <math.h>
@@ -424,17 +424,60 @@ __device__ __forceinline__ bool row_counts_by(const uint8_t* mask, long row) { r
 __device__ __forceinline__ bool listed(long long id, float lp, bool counts, long V) {
   return (id >= 0) & (id < V) & (lp != kNegInf) & counts;
 }
-// A teacher's list [N][k]: counts (COUNT) and entries of single logits.
-template <bool COUNT>
-__global__ __launch_bounds__(256) void gather_list_kernel(const int64_t* __restrict__ ids, const float* __restrict__ teacher,
-                                                          const uint8_t* __restrict__ mask, long n, int k, long V,
-                                                          int* __restrict__ cursor, int2* __restrict__ entries) {
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  const long long id = ids[i];
-  if (!listed(id, teacher[i], row_counts_by(mask, i / k), V)) return;
-  const int at = atomicAdd(&cursor[id / kGroup], 1);
-  if constexpr (!COUNT) entries[at] = int2{(int)(i / k), (int)(-1 - (i * kGroup + id % kGroup))};
+
+constexpr int kPerLane = kScoreTop / 64;
+
+// The column of slot lane + 64 i of row t's list, -1 where the slot is empty: not a token, nothing of the teacher's, or a column
+// that an earlier slot has.
+__device__ __forceinline__ void load_list(const int64_t* ids, const float* teacher, bool counts, long t, long V, int k, int lane,
+                                          int (&id)[kPerLane]) {
+  bool on[kPerLane];
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) {
+    const int s = lane + 64 * i;
+    const long long y = s < k ? ids[t * k + s] : -1;
+    on[i] = listed(y, s < k ? teacher[t * k + s] : 0.f, counts, V);
+    id[i] = on[i] ? (int)y : -1;
+  }
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i)
+    for (int j = 0; j < 64 && 64 * i + j < k; ++j) {
+      const int other = __shfl(id[i], j, 64);
+#pragma unroll
+      for (int o = 0; o < kPerLane; ++o)
+        if (64 * i + j < lane + 64 * o && other >= 0 && other == id[o]) on[o] = false;
+    }
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i)
+    if (!on[i]) id[i] = -1;
+}
+// A teacher's lists [N][k], one wave a row: its outcomes' columns, ascending and each once (kNoColumn past them), and the slot of
+// each. A place is the number of (column, slot) before one's own.
+__global__ __launch_bounds__(256) void sort_lists_kernel(const int64_t* __restrict__ ids, const float* __restrict__ teacher,
+                                                         const uint8_t* __restrict__ mask, long n, long V, int k,
+                                                         int* __restrict__ column, int* __restrict__ slot) {
+  const int lane = threadIdx.x & 63;
+  const long t = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (t >= n) return;
+  int id[kPerLane];
+  load_list(ids, teacher, row_counts_by(mask, t), t, V, k, lane, id);
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) {
+    const int s = lane + 64 * i;
+    const int key = id[i] < 0 ? kNoColumn : id[i];
+    int place = 0;
+#pragma unroll
+    for (int o = 0; o < kPerLane; ++o)
+      for (int j = 0; j < 64 && 64 * o + j < k; ++j) {
+        const int other = __shfl(id[o], j, 64);
+        const int their = other < 0 ? kNoColumn : other;
+        place += their < key || (their == key && 64 * o + j < s);
+      }
+    if (s < k) {
+      column[t * k + place] = key;
+      slot[t * k + place] = s;
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------------------
@@ -602,7 +645,7 @@ __global__ __launch_bounds__(kPick) void score_top_kernel(const float* __restric
 }
 
 // ------------------------------------------------------------------------------------------
-// Distillation, one wave a token. With q_k = p at the list's ids, R = 1 - sum q, t_k and T = 1 - sum t the teacher's, and
+// Distillation, one wave a token, its list as it came (few tokens, with their logits Z) or sorted, with the logits picks. With q_k = p at the list's ids, R = 1 - sum q, t_k and T = 1 - sum t the teacher's, and
 // f = dL/dq but for a constant (f_R for the rest),
 //   forward  sum t log(t / q) + T log(T / R):        f = -t / q,              f_R = -T / R
 //   reverse  sum q log(q / t) + R log(R / T):        f = log(q / t),          f_R = log(R / T)
@@ -625,11 +668,11 @@ __device__ __forceinline__ double log_add(double a, double b) {
   return hi + log1p(exp(fmin(a, b) - hi));
 }
 
-constexpr int kPerLane = kScoreTop / 64;
 constexpr float kLeast = 1.17549435e-38f;
 
 template <int KIND>
-__global__ __launch_bounds__(256) void distill_rows_kernel(RowParts parts, const float* __restrict__ picks,
+__global__ __launch_bounds__(256) void distill_rows_kernel(RowParts parts, const int* __restrict__ sorted,
+                                                           const int* __restrict__ slot, const float* __restrict__ picks,
                                                            const float* __restrict__ Z, long ldz,
                                                            const int64_t* __restrict__ ids, const float* __restrict__ teacher,
                                                            const uint8_t* __restrict__ mask, long n, long V, float inv_t, int k,
@@ -642,26 +685,23 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(RowParts parts, const
   if (t >= n) return;
   // Which slots hold an outcome: a column of its own that the teacher gives something to.
   int id[kPerLane];
+  if (sorted) {
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+      const int y = lane + 64 * i < k ? sorted[t * k + lane + 64 * i] : kNoColumn;
+      id[i] = y == kNoColumn ? -1 : y;
+    }
+  } else {
+    load_list(ids, teacher, row_counts_by(mask, t), t, V, k, lane, id);
+  }
   float lp[kPerLane];
   bool on[kPerLane];
-  const bool counts = row_counts_by(mask, t);
 #pragma unroll
   for (int i = 0; i < kPerLane; ++i) {
-    const int s = lane + 64 * i;
-    const long long y = s < k ? ids[t * k + s] : -1;
-    const float l = s < k ? teacher[t * k + s] : 0.f;
-    on[i] = listed(y, l, counts, V);
-    id[i] = on[i] ? (int)y : -1;
-    lp[i] = on[i] ? l : 0.f;
+    const long o = t * k + lane + 64 * i;
+    on[i] = id[i] >= 0;
+    lp[i] = on[i] ? teacher[sorted ? t * k + slot[o] : o] : 0.f;
   }
-#pragma unroll
-  for (int i = 0; i < kPerLane; ++i)
-    for (int j = 0; j < 64 && 64 * i + j < k; ++j) {  // a column that an earlier slot has is empty here
-      const int other = __shfl(id[i], j, 64);
-#pragma unroll
-      for (int o = 0; o < kPerLane; ++o)
-        if (64 * i + j < lane + 64 * o && other >= 0 && other == id[o]) on[o] = false;
-    }
   bool some = false;
 #pragma unroll
   for (int i = 0; i < kPerLane; ++i) some |= __any(on[i]);
@@ -690,7 +730,7 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(RowParts parts, const
   for (int i = 0; i < kPerLane; ++i) {
     const long o = t * k + lane + 64 * i;
     float z = 0.f;
-    if (id[i] >= 0) z = Z ? Z[t * ldz + id[i]] : picks[o];
+    if (on[i]) z = Z ? Z[t * ldz + id[i]] : picks[o];
     lq[i] = on[i] ? (double)z * (double)inv_t - lse : 0.0;
     q[i] = on[i] ? exp(lq[i]) : 0.0;
     lt[i] = (double)lp[i];
@@ -875,7 +915,7 @@ struct Scratch {
   int groups, ldg, take, max_tiles;  // ldg: floats between the rows of gmax
   long rows, ldz, stage_rows;
   float *m, *s, *u, *gmax, *z, *gs, *gu, *cand, *picks, *row_loss;
-  int *chosen, *counts, *row_counts;
+  int *chosen, *counts, *column, *slot, *row_counts;
   uint32_t* floors;
   int2* entries;
   GatherTile* tiles;
@@ -911,7 +951,7 @@ Scratch carve(const ScoreShape& sh, int f32, int q4, int top, int k_list, void* 
       x.floors = c.take<uint32_t>(x.rows);
       x.cand = c.take<float>(x.rows * x.take * kGroup);
     }
-    const long entries = x.rows * (k_list ? k_list : x.take);
+    const long entries = x.rows * x.take;
     if (entries) {
       x.counts = c.take<int>(x.groups);
       x.entries = c.take<int2>(entries);
@@ -919,7 +959,11 @@ Scratch carve(const ScoreShape& sh, int f32, int q4, int top, int k_list, void* 
       if (x.max_tiles > entries) x.max_tiles = (int)entries;
       x.tiles = c.take<GatherTile>(x.max_tiles);
     }
-    if (k_list) x.picks = c.take<float>(x.rows * k_list);
+    if (k_list) {
+      x.column = c.take<int>(x.rows * k_list);
+      x.slot = c.take<int>(x.rows * k_list);
+      x.picks = c.take<float>(x.rows * k_list);
+    }
     if (q4 && sh.stage) {
       x.stage_rows = sh.v;
       x.stage = c.take<bf16_t>(sh.v * sh.d);
@@ -961,8 +1005,8 @@ RowParts row_parts(const Scratch& x, const ScoreHead& h, long n, long v, float c
 }
 
 // The product over rows [r0, r0 + n) with its statistics.
-hipError_t tile_stats(const ScoreHead& h, const ScoreShape& sh, const Scratch& x, long r0, long n, float c2, hipStream_t st) {
-  const ScoreStats stats{c2, x.m, x.s, x.u, x.gmax, x.ldg};
+hipError_t tile_stats(const ScoreHead& h, const ScoreShape& sh, const Scratch& x, long r0, long n, float c2, int k, hipStream_t st) {
+  const ScoreStats stats{c2, x.m, x.s, x.u, x.gmax, x.ldg, ScoreList{x.column, x.picks, k}};
   if (h.f32)
     return launch_lce32_stats(h.h32, static_cast<const float*>(h.hidden) + r0 * sh.d, (int)n, (int)sh.d, (int)sh.v, stats, st);
   return launch_lce_stats(h.h, static_cast<const bf16_t*>(h.hidden) + r0 * sh.d, (int)n, (int)sh.d, (int)sh.v, stats, x.stage,
@@ -970,7 +1014,7 @@ hipError_t tile_stats(const ScoreHead& h, const ScoreShape& sh, const Scratch& x
 }
 
 hipError_t gather(const ScoreHead& h, const ScoreShape& sh, const Scratch& x, long r0, hipStream_t st) {
-  const GatherPlan plan{x.entries, x.tiles, x.max_tiles, x.cand, x.picks};
+  const GatherPlan plan{x.entries, x.tiles, x.max_tiles, x.cand};
   if (h.f32) return launch_lce32_gather(h.h32, static_cast<const float*>(h.hidden) + r0 * sh.d, (int)sh.d, (int)sh.v, plan, st);
   return launch_lce_gather(h.h, static_cast<const bf16_t*>(h.hidden) + r0 * sh.d, (int)sh.d, (int)sh.v, plan, st);
 }
@@ -1013,7 +1057,7 @@ hipError_t launch_logprobs_fwd(const ScoreHead& h, const ScoreShape& sh, const i
     const LogprobsOut out{o.logprobs ? o.logprobs + r0 : nullptr, o.entropy + r0, top ? o.top_logprobs + r0 * top : nullptr,
                           top ? o.top_ids + r0 * top : nullptr, o.lse + r0, o.tgt ? o.tgt + r0 : nullptr};
     const int64_t* y = targets ? targets + r0 : nullptr;
-    hipError_t e = tile_stats(h, sh, x, r0, n, c2, st);
+    hipError_t e = tile_stats(h, sh, x, r0, n, c2, 0, st);
     if (e != hipSuccess) return e;
     if (y) {
       e = h.f32 ? launch_lce32_target(h.h32, static_cast<const float*>(h.hidden) + r0 * sh.d, y, (int)n, (int)sh.d, V, out.tgt, st)
@@ -1067,22 +1111,14 @@ hipError_t launch_distill_fwd(const ScoreHead& h, const ScoreShape& sh, const in
       const hipError_t e = few_logits(h, sh, x, c2, st);
       if (e != hipSuccess) return e;
     } else {
-      hipError_t e = tile_stats(h, sh, x, r0, n, c2, st);
-      if (e != hipSuccess) return e;
-      const dim3 grid((unsigned)ceil_div(n * p.k, 256)), block(256);
-      hipLaunchKernelGGL(zero_counts_kernel, dim3((unsigned)ceil_div(x.groups, 256)), block, 0, st, x.counts, x.groups);
+      hipLaunchKernelGGL(sort_lists_kernel, dim3((unsigned)ceil_div(n, 4)), dim3(256), 0, st, id, lp, see, n, sh.v, p.k, x.column,
+                         x.slot);
       MTP_LAUNCHED();
-      hipLaunchKernelGGL(gather_list_kernel<true>, grid, block, 0, st, id, lp, see, n * p.k, p.k, sh.v, x.counts, x.entries);
-      MTP_LAUNCHED();
-      hipLaunchKernelGGL(gather_tiles_kernel, dim3(1), dim3(1024), 0, st, x.counts, x.groups, x.tiles, x.max_tiles);
-      MTP_LAUNCHED();
-      hipLaunchKernelGGL(gather_list_kernel<false>, grid, block, 0, st, id, lp, see, n * p.k, p.k, sh.v, x.counts, x.entries);
-      MTP_LAUNCHED();
-      e = gather(h, sh, x, r0, st);
+      const hipError_t e = tile_stats(h, sh, x, r0, n, c2, p.k, st);
       if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(n, 4)), dim3(256), 0, st, row_parts(x, h, n, sh.v, c2), x.picks,
-                       x.few ? x.z : nullptr, x.ldz, id, lp, see, n, sh.v, sh.inv_t, p.k, p.renormalize, p.beta, row_loss + r0,
+    hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(n, 4)), dim3(256), 0, st, row_parts(x, h, n, sh.v, c2), x.column,
+                       x.slot, x.picks, x.few ? x.z : nullptr, x.ldz, id, lp, see, n, sh.v, sh.inv_t, p.k, p.renormalize, p.beta, row_loss + r0,
                        x.row_counts + r0, o.lse + r0, o.rest + r0, o.coef + r0 * p.k, o.columns + r0 * p.k);
     MTP_LAUNCHED();
   }
