@@ -139,12 +139,13 @@ __device__ __forceinline__ u32x4 load16(const __amdgpu_buffer_rsrc_t r, uint32_t
 // LDS written before is seen behind it by the workgroup; loads into registers stay in flight.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-template <int Q4, int NB, int SLAB>
+template <int Q4, int NB, int ROWS, int SLAB>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NB == 1 ? 5 : NB == 2 ? 4 : 2)))
 void lce_few_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W, const uint32_t* __restrict__ Wq,
                     const bf16_t* __restrict__ Sc, const bf16_t* __restrict__ Bi, int N, int D, int V, float c2, int ldz,
                     float* __restrict__ Z, float* __restrict__ gmax, float* __restrict__ gs, float* __restrict__ gu) {
-  constexpr int kTok = 32 * NB, kBytes = kTok * 2 * SLAB;  // a slab of tokens: tiles of 64 k, 128 bytes a row
+  // A slab of tokens: tiles of 64 k, 128 bytes a row, ROWS of them (16: the products' upper 16 columns repeat the lower).
+  constexpr int kTok = ROWS, kBytes = kTok * 2 * SLAB;
   constexpr int kFrags = SLAB / 16, kParts = kBytes / 4096, kChunks = SLAB / 8;
   __shared__ __attribute__((aligned(16))) char lds[2 * kBytes];
   float(*xm)[kTok] = reinterpret_cast<float(*)[kTok]>(lds);  // after the product: 4 waves' statistics
@@ -160,17 +161,25 @@ void lce_few_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W, 
   // zeros there.
   auto chunk = [&](int j) { return Q4 ? kFrags * half + j : 2 * j + half; };
   u32x4 wa[Q4 ? SLAB / 64 : kFrags];
-  uint32_t sc[Q4 ? SLAB / 128 : 1], bi[Q4 ? SLAB / 128 : 1];
+  static_assert(!Q4 || SLAB == 256, "a lane's two groups of a slab are one word");
+  uint32_t sc = 0, bi = 0;  // scales and biases of the lane's groups of a slab
   const __amdgpu_buffer_rsrc_t rw =
       Q4 ? rows_rsrc(Wq + (long)v0 * (D >> 3), (long)(V - v0) * (D >> 1)) : rows_rsrc(W + (long)v0 * D, 2L * (V - v0) * D);
   const uint32_t wo = Q4 ? (uint32_t)vr * (uint32_t)(D >> 1) + half * (SLAB / 4) : 2u * (uint32_t)vr * (uint32_t)D + 16 * half;
   const __amdgpu_buffer_rsrc_t rs = rows_rsrc(Q4 ? Sc + (long)v0 * (D >> 6) : W, Q4 ? 2L * (V - v0) * (D >> 6) : 0);
   const __amdgpu_buffer_rsrc_t rb = rows_rsrc(Q4 ? Bi + (long)v0 * (D >> 6) : W, Q4 ? 2L * (V - v0) * (D >> 6) : 0);
   const uint32_t so = 2u * ((uint32_t)vr * (uint32_t)(D >> 6) + half * (SLAB / 128));
+  const bool pairs = (D & 127) == 0;
   auto load_words = [&](int slab, int i) { wa[i] = load16(rw, wo, slab * (Q4 ? SLAB / 2 : 2 * SLAB) + (Q4 ? 16 : 32) * i); };
-  auto load_scale = [&](int slab, int i) {
-    sc[i] = __builtin_amdgcn_raw_buffer_load_b16(rs, so, slab * (SLAB / 32) + 2 * i, 0);
-    bi[i] = __builtin_amdgcn_raw_buffer_load_b16(rb, so, slab * (SLAB / 32) + 2 * i, 0);
+  auto load_scale = [&](int slab) {
+    const int o = slab * (SLAB / 32);
+    if (pairs) {
+      sc = __builtin_amdgcn_raw_buffer_load_b32(rs, so, o, 0);
+      bi = __builtin_amdgcn_raw_buffer_load_b32(rb, so, o, 0);
+    } else {  // (a row's last group alone in its word)
+      sc = __builtin_amdgcn_raw_buffer_load_b16(rs, so, o, 0) | (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(rs, so, o + 2, 0) << 16;
+      bi = __builtin_amdgcn_raw_buffer_load_b16(rb, so, o, 0) | (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(rb, so, o + 2, 0) << 16;
+    }
   };
   u32x4 ha[kParts];
   auto load_tokens = [&](int slab) {
@@ -194,10 +203,7 @@ void lce_few_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W, 
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[b][r] = 0.f;
   load_tokens(0);
-  if constexpr (Q4) {
-#pragma unroll
-    for (int i = 0; i < SLAB / 128; ++i) load_scale(0, i);
-  }
+  if constexpr (Q4) load_scale(0);
 #pragma unroll
   for (int i = 0; i < (Q4 ? SLAB / 64 : kFrags); ++i) load_words(0, i);
   put_tokens(lds);
@@ -210,16 +216,16 @@ void lce_few_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W, 
     for (int j = 0; j < kFrags; ++j) {
       const int c = chunk(j);
       bf16x8 a;
-      if constexpr (Q4) a = as_bf16x8(dequant8(wa[j >> 2][j & 3], bf16lo(sc[j >> 3]), bf16lo(bi[j >> 3])));
+      if constexpr (Q4) a = as_bf16x8(dequant8(wa[j >> 2][j & 3], j < 8 ? bf16lo(sc) : bf16hi(sc), j < 8 ? bf16lo(bi) : bf16hi(bi)));
       else a = as_bf16x8(wa[j]);
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        const bf16x8 t = as_bf16x8(lds_read16(cur + (c >> 3) * (kTok * 128), lds_off(32 * b + col, c & 7)));
+        const bf16x8 t = as_bf16x8(lds_read16(cur + (c >> 3) * (kTok * 128), lds_off(ROWS == 16 ? col & 15 : 32 * b + col, c & 7)));
         acc[b] = mfma32(a, t, acc[b]);
       }
       if constexpr (Q4) {
         if (j % 4 == 3) load_words(s + 1, j >> 2);
-        if (j % 8 == 7) load_scale(s + 1, j >> 3);
+        if (j == kFrags - 1) load_scale(s + 1);
         if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
       } else {
         load_words(s + 1, j);
@@ -244,7 +250,7 @@ void lce_few_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W, 
         z[u] = v0 + row + u < V ? acc[b][4 * q + u] : kNegInf;
         top = fmaxf(top, z[u]);
       }
-      if (t < N) *reinterpret_cast<f32x4*>(Z + (long)t * ldz + v0 + row) = z;
+      if (t < N && t < kTok) *reinterpret_cast<f32x4*>(Z + (long)t * ldz + v0 + row) = z;
     }
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     const float base = top == kNegInf ? 0.f : top * c2;
@@ -258,7 +264,7 @@ void lce_few_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W, 
       }
     s += __shfl_xor(s, 32, 64);
     u += __shfl_xor(u, 32, 64);
-    if (half == 0) {
+    if (half == 0 && t < kTok) {
       xm[w][t] = top;
       xs[w][t] = s;
       xu[w][t] = u;
@@ -986,16 +992,17 @@ Scratch carve(const ScoreShape& sh, int f32, int q4, int top, int k_list, void* 
 hipError_t few_logits(const ScoreHead& h, const ScoreShape& sh, const Scratch& x, float c2, hipStream_t st) {
   const bf16_t* H = static_cast<const bf16_t*>(h.hidden);
   const int blocks = (int)ceil_div(sh.n, 32);
-  auto run = [&](auto nb) {
-    constexpr int NB = decltype(nb)::value;
-    auto kernel = h.h.q4 ? lce_few_kernel<1, NB, NB == 1 ? 256 : 128> : lce_few_kernel<0, NB, 128>;
+  auto run = [&](auto nb, auto rows) {
+    constexpr int NB = decltype(nb)::value, ROWS = decltype(rows)::value;
+    auto kernel = h.h.q4 ? lce_few_kernel<1, NB, ROWS, 256> : lce_few_kernel<0, NB, ROWS, 128>;
     hipLaunchKernelGGL(kernel, dim3(x.groups), dim3(256), 0, st, H, h.h.w, h.h.wq, h.h.sc, h.h.bi, (int)sh.n, (int)sh.d,
                        (int)sh.v, c2, (int)x.ldz, x.z, x.gmax, x.gs, x.gu);
     return hipGetLastError();
   };
-  if (blocks == 1) return run(std::integral_constant<int, 1>{});
-  if (blocks == 2) return run(std::integral_constant<int, 2>{});
-  return run(std::integral_constant<int, 4>{});
+  if (sh.n <= 16) return run(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
+  if (blocks == 1) return run(std::integral_constant<int, 1>{}, std::integral_constant<int, 32>{});
+  if (blocks == 2) return run(std::integral_constant<int, 2>{}, std::integral_constant<int, 64>{});
+  return run(std::integral_constant<int, 4>{}, std::integral_constant<int, 128>{});
 }
 
 RowParts row_parts(const Scratch& x, const ScoreHead& h, long n, long v, float c2) {
