@@ -392,8 +392,8 @@ int mtp_policy_bwd(const float* d_loss, const float* nll, const float* old_nll, 
  *
  * hidden, head, n, d, v, head_kind: as (A), v <= 2^21. With x = hidden . w / temperature, lse = logsumexp x,
  * p = exp(x - lse). temperature in [1e-3, 1e3]. The _f32 forms take fp32 hidden states and heads.
- * A forward's head_kind MTP_HEAD_Q4_STAGED dequantizes the whole head into the workspace; a backward's kinds, chunk,
- * row_block and w_t are mtp_lce_bwd's (mtp_lce_bwd_f32's).
+ * A forward's head_kind MTP_HEAD_Q4_STAGED dequantizes the whole head into the workspace (few tokens: none of it), an fp32
+ * backward's too; a bf16 backward's kinds, and chunk, row_block and w_t, are mtp_lce_bwd's (mtp_lce_bwd_f32's).
  * Rows that are left out (an ignored target; a mask of 0; an empty list) may hold anything, NaN too, and get gradients of 0.
  * ------------------------------------------------------------------------------------------- */
 #define MTP_SCORE_MAX 128 /* most alternatives, and longest teacher's list */
@@ -420,7 +420,8 @@ int mtp_logprobs_fwd_f32(const float* hidden, const float* w, const uint32_t* w_
  * length for distillation) and, for a trainable head, a copy of the hidden states. */
 size_t mtp_score_bwd_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int64_t chunk, int64_t row_block,
                                      int32_t k, int32_t trainable);
-size_t mtp_score_bwd_f32_workspace_bytes(int64_t n, int64_t d, int64_t v, int64_t chunk, int32_t k, int32_t trainable);
+size_t mtp_score_bwd_f32_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int64_t chunk, int32_t k,
+                                         int32_t trainable);
 
 /* dL/dx = d_logprobs ([v = y] - p) - d_entropy p (x - lse + entropy); either gradient may be NULL (0). */
 int mtp_logprobs_bwd(const void* hidden, const void* w, const void* w_t, const uint32_t* w_q, const void* scales,

@@ -821,13 +821,16 @@ static int check_list(int32_t k) {
   return MTP_OK;
 }
 
+static bool q4_kind(int32_t head_kind) { return head_kind == MTP_HEAD_Q4 || head_kind == MTP_HEAD_Q4_STAGED; }
+
 static mtp::ScoreHead score_head(int f32, const void* hidden, const void* w, const uint32_t* w_q, const void* scales,
                                  const void* biases, int32_t head_kind) {
   mtp::ScoreHead h{};
   h.f32 = f32;
   h.hidden = hidden;
   if (f32)
-    h.h32 = make_head32(static_cast<const float*>(w), w_q, static_cast<const float*>(scales), static_cast<const float*>(biases), head_kind);
+    h.h32 = make_head32(static_cast<const float*>(w), w_q, static_cast<const float*>(scales), static_cast<const float*>(biases),
+                        q4_kind(head_kind) ? MTP_HEAD_Q4 : head_kind);
   else
     h.h = make_head(w, w_q, scales, biases, head_kind);
   return h;
@@ -837,9 +840,9 @@ static mtp::ScoreHead score_head(int f32, const void* hidden, const void* w, con
 static int check_score_head(int f32, const void* hidden, const void* w, const uint32_t* w_q, const void* scales,
                             const void* biases, int64_t n, int64_t d, int64_t v, int32_t head_kind) {
   static const int64_t any = 0;
-  if (f32)
+  if (f32)  // (staged: this section's alone)
     return check_lce32(static_cast<const float*>(hidden), static_cast<const float*>(w), w_q, static_cast<const float*>(scales),
-                       static_cast<const float*>(biases), &any, n, d, v, head_kind);
+                       static_cast<const float*>(biases), &any, n, d, v, head_kind == MTP_HEAD_Q4_STAGED ? MTP_HEAD_Q4 : head_kind);
   return check_lce_common(hidden, w, w_q, scales, biases, &any, n, d, v, head_kind);
 }
 
@@ -847,7 +850,6 @@ static mtp::ScoreShape score_shape(int64_t n, int64_t d, int64_t v, double tempe
   return mtp::ScoreShape{(long)n, (long)d, (long)v, (float)(1.0 / temperature), head_kind == MTP_HEAD_Q4_STAGED};
 }
 
-static bool q4_kind(int32_t head_kind) { return head_kind == MTP_HEAD_Q4 || head_kind == MTP_HEAD_Q4_STAGED; }
 static bool score_sizes(int64_t n, int64_t d, int64_t v) {
   return n >= 1 && d >= 1 && v >= 1 && n <= kMaxDim && d <= kMaxDim && v <= mtp::kScoreVocab;
 }
@@ -901,11 +903,12 @@ int mtp_logprobs_fwd_f32(const float* hidden, const float* w, const uint32_t* w_
                       mtp::LogprobsOut{logprobs, entropy, top_logprobs, top_ids, lse, tgt}, workspace, workspace_bytes, stream);
 }
 
-// After the loss's workspace: alpha [n], beta [n], the columns [n] of scoring, the values [n][k], the cleared hidden states.
+// After the loss's workspace: alpha [n], beta [n], the columns [n] of scoring, the values [n][k], the cleared hidden states, or
+// an fp32 4-bit head's rows (staged bytes).
 struct ScoreBwd {
   size_t alpha, beta, columns, value, clean, bytes;
 };
-static ScoreBwd score_bwd_parts(size_t lce, int64_t n, int64_t d, int32_t k, int32_t trainable, size_t elem) {
+static ScoreBwd score_bwd_parts(size_t lce, int64_t n, int64_t d, int32_t k, int32_t trainable, size_t elem, size_t staged) {
   auto pad = [](size_t x) { return (x + 255) / 256 * 256; };
   ScoreBwd p;
   p.alpha = pad(lce);
@@ -913,17 +916,18 @@ static ScoreBwd score_bwd_parts(size_t lce, int64_t n, int64_t d, int32_t k, int
   p.columns = p.beta + pad((size_t)n * 4);
   p.value = p.columns + pad((size_t)n * 4);
   p.clean = p.value + pad((size_t)n * k * 4);
-  p.bytes = p.clean + (trainable ? (size_t)n * d * elem : 0);
+  p.bytes = p.clean + (trainable ? (size_t)n * d * elem : staged);
   return p;
 }
 size_t mtp_score_bwd_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int64_t chunk, int64_t row_block,
                                      int32_t k, int32_t trainable) {
   const size_t lce = mtp_lce_bwd_workspace_bytes(n, d, v, head_kind, chunk, row_block);
-  return !lce || k < 1 || k > MTP_SCORE_MAX ? 0 : score_bwd_parts(lce, n, d, k, trainable, 2).bytes;
+  return !lce || k < 1 || k > MTP_SCORE_MAX ? 0 : score_bwd_parts(lce, n, d, k, trainable, 2, 0).bytes;
 }
-size_t mtp_score_bwd_f32_workspace_bytes(int64_t n, int64_t d, int64_t v, int64_t chunk, int32_t k, int32_t trainable) {
+static size_t staged32_bytes(int64_t d, int64_t v, int32_t head_kind) { return head_kind == MTP_HEAD_Q4_STAGED ? (size_t)v * d * 4 : 0; }
+size_t mtp_score_bwd_f32_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int64_t chunk, int32_t k, int32_t trainable) {
   const size_t lce = mtp_lce_bwd_f32_workspace_bytes(n, d, v, chunk);
-  return !lce || k < 1 || k > MTP_SCORE_MAX ? 0 : score_bwd_parts(lce, n, d, k, trainable, 4).bytes;
+  return !lce || k < 1 || k > MTP_SCORE_MAX ? 0 : score_bwd_parts(lce, n, d, k, trainable, 4, staged32_bytes(d, v, head_kind)).bytes;
 }
 
 }  // extern "C"
@@ -951,7 +955,7 @@ static int score_bwd(int f32, const void* hidden, const void* w, const void* w_t
     return fail(MTP_ERR_INPUT, "row_block must be 0, >= n, or (bf16) a positive multiple of 256 (got %lld)", (long long)row_block);
   if (d_w && row_block < n) return fail(MTP_ERR_INPUT, "a trainable head (d_w) sums over every row: row_block must cover all n=%lld rows", (long long)n);
   const size_t lce = f32 ? mtp_lce_bwd_f32_workspace_bytes(n, d, v, chunk) : mtp_lce_bwd_workspace_bytes(n, d, v, head_kind, chunk, row_block);
-  const ScoreBwd parts = score_bwd_parts(lce, n, d, k, d_w != nullptr, f32 ? 4 : 2);
+  const ScoreBwd parts = score_bwd_parts(lce, n, d, k, d_w != nullptr, f32 ? 4 : 2, f32 ? staged32_bytes(d, v, head_kind) : 0);
   if (!workspace || workspace_bytes < parts.bytes)
     return fail(MTP_ERR_WORKSPACE, "the backward needs a workspace of %zu bytes at chunk=%lld, row_block=%lld (got %zu)", parts.bytes, (long long)chunk, (long long)row_block, workspace ? workspace_bytes : (size_t)0);
   if (!aligned16(workspace)) return fail(MTP_ERR_UNSUPPORTED, "workspace must be 16-byte aligned");
@@ -968,8 +972,14 @@ static int score_bwd(int f32, const void* hidden, const void* w, const void* w_t
     const float inv_t = (float)(1.0 / temperature);
     const mtp::AffineGrad grad{{alpha, has_beta ? beta : nullptr, 1.4426950408889634f * inv_t}, columns ? columns : own_columns, value, (int)k, ws + parts.clean};
     if (f32) {
-      e = mtp::launch_lce32_bwd(score_head(1, hidden, w, w_q, scales, biases, head_kind).h32, static_cast<const float*>(hidden), nullptr,
-                                lse, nullptr, (int)n, (int)d, (int)v, 0, (int)chunk, static_cast<float*>(d_hidden),
+      mtp::LceHead32 head = score_head(1, hidden, w, w_q, scales, biases, head_kind).h32;
+      if (head_kind == MTP_HEAD_Q4_STAGED) {
+        float* rows = reinterpret_cast<float*>(ws + parts.clean);
+        e = mtp::launch_dequant32(head, (long)v, (long)d, rows, stream);
+        if (e != hipSuccess) return fail(MTP_ERR_RUNTIME, "backward launch failed: %s", hipGetErrorString(e));
+        head = mtp::LceHead32{0, rows, nullptr, nullptr, nullptr};
+      }
+      e = mtp::launch_lce32_bwd(head, static_cast<const float*>(hidden), nullptr, lse, nullptr, (int)n, (int)d, (int)v, 0, (int)chunk, static_cast<float*>(d_hidden),
                                 static_cast<float*>(d_w), static_cast<float*>(workspace), stream, &grad);
     } else {
       mtp::LceHead head = make_head(w, w_q, scales, biases, head_kind);

@@ -196,6 +196,7 @@ struct GatherPlan {
   int max_tiles;
   float* rows;              // [entries][kGroup]
 };
+hipError_t launch_dequant32(const LceHead32& h, long V, long D, float* out, hipStream_t stream);  // [V][D]
 hipError_t launch_lce_gather(const LceHead& h, const bf16_t* H, int D, int V, const GatherPlan& p, hipStream_t stream);
 hipError_t launch_lce32_gather(const LceHead32& h, const float* H, int D, int V, const GatherPlan& p, hipStream_t stream);
 
@@ -203,6 +204,7 @@ constexpr long kScoreRows = 16384;   // tokens of one pass of a forward: more ar
 constexpr int kScoreTop = 128;       // most alternatives, and longest teacher's list
 constexpr long kScoreVocab = 1 << 21;
 constexpr long kFewTokens = 128;     // tokens up to which a bf16 forward keeps its logits
+constexpr long kFewTokens32 = 64;    // an fp32 one (hidden dims that are multiples of 4)
 constexpr double kTailFloor = 1e-6;  // least mass that the outcomes outside a list count as
 
 // One head of either type; w32 where the hidden states are fp32.
@@ -215,7 +217,7 @@ struct ScoreHead {
 struct ScoreShape {
   long n, d, v;
   float inv_t;       // 1 / temperature
-  int stage;         // bf16, 4-bit: dequantize the whole head into the workspace first
+  int stage;         // 4-bit: dequantize the whole head into the workspace first
 };
 struct LogprobsOut {
   float *logprobs, *entropy, *top_logprobs;

@@ -12,7 +12,7 @@
 // choose among them. The logits of a teacher's list, sorted first, the product's tiles put away as they pass (ListCursor): the
 // very ones that the sums hold, so that what a list leaves of 1 is exact to fp32 and not to two roundings of a large logit.
 //
-// Up to kFewTokens tokens the logits themselves are kept in the workspace (lce_few_kernel), which leaves two launches.
+// Up to kFewTokens tokens (kFewTokens32) the logits themselves are kept in the workspace (lce_few_kernel), which leaves two launches.
 #include <math.h>
 
 #include <type_traits>
@@ -123,7 +123,7 @@ __device__ __forceinline__ uint32_t pick_largest(const uint32_t* key, int M, int
 }
 
 // ------------------------------------------------------------------------------------------
-// Few tokens (bf16 hidden states): the logits [N][ldz] in fp32, and per group of kGroup of them their maximum and, relative to
+// Few tokens: the logits [N][ldz] in fp32, and per group of kGroup of them their maximum and, relative to
 // it, the two sums. The head is read once and bounds it; a workgroup takes one group: 4 waves of 32 vocab rows, the rows'
 // fragments straight from memory to registers, each loaded for the next slab as soon as its product has gone out (a whole slab in
 // flight a wave, 8 KiB of a dense head, 4 or 2 of a 4-bit one), the tokens' slab (NB blocks of 32) through LDS, one barrier a
@@ -139,53 +139,61 @@ __device__ __forceinline__ u32x4 load16(const __amdgpu_buffer_rsrc_t r, uint32_t
 // LDS written before is seen behind it by the workgroup; loads into registers stay in flight.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-template <int Q4, int NB, int ROWS, int SLAB>
+// T: the hidden states' type, and a dense head's and the scales' too (fp32: v_mfma_f32_32x32x2_f32, a lane's 4 values a step
+// of 8 k). ROWS: of the tokens' slab (16: the products' upper 16 columns repeat the lower).
+template <class T, int Q4, int NB, int ROWS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NB == 1 ? 5 : NB == 2 ? 4 : 2)))
-void lce_few_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W, const uint32_t* __restrict__ Wq,
-                    const bf16_t* __restrict__ Sc, const bf16_t* __restrict__ Bi, int N, int D, int V, float c2, int ldz,
-                    float* __restrict__ Z, float* __restrict__ gmax, float* __restrict__ gs, float* __restrict__ gu) {
-  // A slab of tokens: tiles of 64 k, 128 bytes a row, ROWS of them (16: the products' upper 16 columns repeat the lower).
-  constexpr int kTok = ROWS, kBytes = kTok * 2 * SLAB;
-  constexpr int kFrags = SLAB / 16, kParts = kBytes / 4096, kChunks = SLAB / 8;
+void lce_few_kernel(const T* __restrict__ H, const T* __restrict__ W, const uint32_t* __restrict__ Wq, const T* __restrict__ Sc,
+                    const T* __restrict__ Bi, int N, int D, int V, float c2, int ldz, float* __restrict__ Z,
+                    float* __restrict__ gmax, float* __restrict__ gs, float* __restrict__ gu) {
+  constexpr bool F32 = sizeof(T) == 4;
+  constexpr int kSlab = F32 ? 64 : Q4 ? 256 : 128;               // k
+  constexpr int kRow = kSlab * (int)sizeof(T), kBytes = ROWS * kRow;  // a token's, and all of them: tiles of 128 bytes a row
+  constexpr int kParts = kBytes / 4096, kChunks = kRow / 16;     // 16-byte chunks: a thread's, and a row's
+  constexpr int kWords = Q4 ? kSlab / 16 : 0;                    // a lane's packed words
+  constexpr int kLoads = Q4 ? kWords / 4 : kChunks / 2;          // a lane's 16-byte loads of the head
+  constexpr int kFrags = Q4 ? kWords : kLoads;                   // products' operands (8 values of a row's k: bf16, or 2 x 4)
   __shared__ __attribute__((aligned(16))) char lds[2 * kBytes];
-  float(*xm)[kTok] = reinterpret_cast<float(*)[kTok]>(lds);  // after the product: 4 waves' statistics
-  float(*xs)[kTok] = xm + 4;
-  float(*xu)[kTok] = xm + 8;
+  float(*xm)[ROWS] = reinterpret_cast<float(*)[ROWS]>(lds);  // after the product: 4 waves' statistics
+  float(*xs)[ROWS] = xm + 4;
+  float(*xu)[ROWS] = xm + 8;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, half = lane >> 5, col = lane & 31;
   const int v0 = blockIdx.x * kGroup;
   const int vr = 32 * w + col < V - v0 ? 32 * w + col : V - 1 - v0;  // rows past the end: their logits are replaced
-  const int slabs = (D + SLAB - 1) / SLAB;
+  const int slabs = (D + kSlab - 1) / kSlab;
 
-  // Fragment j of a slab contracts k chunk (8 values) `2 j + half` of it; with packed words kFrags half + j, so that a lane's
-  // words lie together. Past the end of a row a load takes the next row's values (past the head zeros): the tokens' are
-  // zeros there.
-  auto chunk = [&](int j) { return Q4 ? kFrags * half + j : 2 * j + half; };
-  u32x4 wa[Q4 ? SLAB / 64 : kFrags];
-  static_assert(!Q4 || SLAB == 256, "a lane's two groups of a slab are one word");
-  uint32_t sc = 0, bi = 0;  // scales and biases of the lane's groups of a slab
-  const __amdgpu_buffer_rsrc_t rw =
-      Q4 ? rows_rsrc(Wq + (long)v0 * (D >> 3), (long)(V - v0) * (D >> 1)) : rows_rsrc(W + (long)v0 * D, 2L * (V - v0) * D);
-  const uint32_t wo = Q4 ? (uint32_t)vr * (uint32_t)(D >> 1) + half * (SLAB / 4) : 2u * (uint32_t)vr * (uint32_t)D + 16 * half;
-  const __amdgpu_buffer_rsrc_t rs = rows_rsrc(Q4 ? Sc + (long)v0 * (D >> 6) : W, Q4 ? 2L * (V - v0) * (D >> 6) : 0);
-  const __amdgpu_buffer_rsrc_t rb = rows_rsrc(Q4 ? Bi + (long)v0 * (D >> 6) : W, Q4 ? 2L * (V - v0) * (D >> 6) : 0);
-  const uint32_t so = 2u * ((uint32_t)vr * (uint32_t)(D >> 6) + half * (SLAB / 128));
-  const bool pairs = (D & 127) == 0;
-  auto load_words = [&](int slab, int i) { wa[i] = load16(rw, wo, slab * (Q4 ? SLAB / 2 : 2 * SLAB) + (Q4 ? 16 : 32) * i); };
-  auto load_scale = [&](int slab) {
-    const int o = slab * (SLAB / 32);
+  // Operand j of a slab is the 16-byte chunk `2 j + half` of a dense row's; of packed words, word kFrags half + j, so that a
+  // lane's words lie together. Past the end of a row a load takes the next row's values (past the head zeros): the tokens'
+  // are zeros there.
+  u32x4 wa[kLoads];
+  const long left = V - v0;
+  const __amdgpu_buffer_rsrc_t rw = Q4 ? rows_rsrc(Wq + (long)v0 * (D >> 3), left * (D >> 1))
+                                       : rows_rsrc(W + (long)v0 * D, left * D * (long)sizeof(T));
+  uint32_t wo = Q4 ? (uint32_t)vr * (uint32_t)(D >> 1) + half * (kSlab / 4) : (uint32_t)vr * (uint32_t)D * (uint32_t)sizeof(T) + 16 * half;
+  // Scales and biases of the lane's groups of a slab: two in a word (bf16), or one.
+  uint32_t sc = 0, bi = 0;
+  const __amdgpu_buffer_rsrc_t rs = rows_rsrc(Q4 ? Sc + (long)v0 * (D >> 6) : W, Q4 ? left * (D >> 6) * (long)sizeof(T) : 0);
+  const __amdgpu_buffer_rsrc_t rb = rows_rsrc(Q4 ? Bi + (long)v0 * (D >> 6) : W, Q4 ? left * (D >> 6) * (long)sizeof(T) : 0);
+  uint32_t so = (uint32_t)vr * (uint32_t)(D >> 6) * (uint32_t)sizeof(T) + (F32 ? 0 : 4 * half);
+  const bool pairs = F32 || (D & 127) == 0;
+  // The loads' offsets are in the vector operand, which the range is checked for.
+  auto load_head = [&](int i) { wa[i] = load16(rw, wo + (Q4 ? 16 : 32) * i, 0); };
+  auto next_head = [&] { wo += Q4 ? kSlab / 2 : kRow; };
+  auto load_scales = [&] {
     if (pairs) {
-      sc = __builtin_amdgcn_raw_buffer_load_b32(rs, so, o, 0);
-      bi = __builtin_amdgcn_raw_buffer_load_b32(rb, so, o, 0);
+      sc = __builtin_amdgcn_raw_buffer_load_b32(rs, so, 0, 0);
+      bi = __builtin_amdgcn_raw_buffer_load_b32(rb, so, 0, 0);
     } else {  // (a row's last group alone in its word)
-      sc = __builtin_amdgcn_raw_buffer_load_b16(rs, so, o, 0) | (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(rs, so, o + 2, 0) << 16;
-      bi = __builtin_amdgcn_raw_buffer_load_b16(rb, so, o, 0) | (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(rb, so, o + 2, 0) << 16;
+      sc = __builtin_amdgcn_raw_buffer_load_b16(rs, so, 0, 0) | (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(rs, so + 2, 0, 0) << 16;
+      bi = __builtin_amdgcn_raw_buffer_load_b16(rb, so, 0, 0) | (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(rb, so + 2, 0, 0) << 16;
     }
+    so += kSlab / 64 * (uint32_t)sizeof(T);
   };
   u32x4 ha[kParts];
   auto load_tokens = [&](int slab) {
 #pragma unroll
     for (int p = 0; p < kParts; ++p) {
-      const int id = tid + 256 * p, row = id / kChunks, k = slab * SLAB + 8 * (id % kChunks);
+      const int id = tid + 256 * p, row = id / kChunks, k = slab * kSlab + (16 / (int)sizeof(T)) * (id % kChunks);
       ha[p] = row < N && k < D ? *reinterpret_cast<const u32x4*>(H + (long)row * D + k) : zero4();
     }
   };
@@ -193,8 +201,11 @@ void lce_few_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W, 
 #pragma unroll
     for (int p = 0; p < kParts; ++p) {
       const int id = tid + 256 * p, row = id / kChunks, c = id % kChunks;
-      lds_write16(dst + (c >> 3) * (kTok * 128), lds_off(row, c & 7), ha[p]);
+      lds_write16(dst + (c >> 3) * (ROWS * 128), lds_off(row, c & 7), ha[p]);
     }
+  };
+  auto token = [&](const char* cur, int c, int b) {
+    return lds_read16(cur + (c >> 3) * (ROWS * 128), lds_off(ROWS == 16 ? col & 15 : 32 * b + col, c & 7));
   };
 
   f32x16 acc[NB];
@@ -202,10 +213,16 @@ void lce_few_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W, 
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[b][r] = 0.f;
-  load_tokens(0);
-  if constexpr (Q4) load_scale(0);
+  auto product4 = [&](const f32x4& a, const u32x4& t, int b) {
+    const f32x4 y = __builtin_bit_cast(f32x4, t);
 #pragma unroll
-  for (int i = 0; i < (Q4 ? SLAB / 64 : kFrags); ++i) load_words(0, i);
+    for (int e = 0; e < 4; ++e) acc[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], y[e], acc[b], 0, 0, 0);
+  };
+  load_tokens(0);
+  if constexpr (Q4) load_scales();
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) load_head(i);
+  next_head();
   put_tokens(lds);
   lds_barrier();
   for (int s = 0; s < slabs; ++s) {
@@ -214,24 +231,40 @@ void lce_few_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W, 
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int j = 0; j < kFrags; ++j) {
-      const int c = chunk(j);
-      bf16x8 a;
-      if constexpr (Q4) a = as_bf16x8(dequant8(wa[j >> 2][j & 3], j < 8 ? bf16lo(sc) : bf16hi(sc), j < 8 ? bf16lo(bi) : bf16hi(bi)));
-      else a = as_bf16x8(wa[j]);
+      if constexpr (F32 && Q4) {
+        const uint32_t q = wa[j >> 2][j & 3];
+        const float sf = __uint_as_float(sc), bf = __uint_as_float(bi);
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        const bf16x8 t = as_bf16x8(lds_read16(cur + (c >> 3) * (kTok * 128), lds_off(ROWS == 16 ? col & 15 : 32 * b + col, c & 7)));
-        acc[b] = mfma32(a, t, acc[b]);
+        for (int h = 0; h < 2; ++h) {
+          f32x4 a;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) a[e] = __builtin_fmaf(sf, (float)((q >> (16 * h + 4 * e)) & 15u), bf);
+#pragma unroll
+          for (int b = 0; b < NB; ++b) product4(a, token(cur, 8 * half + 2 * j + h, b), b);
+        }
+      } else if constexpr (F32) {
+        const f32x4 a = __builtin_bit_cast(f32x4, wa[j]);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) product4(a, token(cur, 2 * j + half, b), b);
+      } else {
+        bf16x8 a;
+        if constexpr (Q4) a = as_bf16x8(dequant8(wa[j >> 2][j & 3], j < 8 ? bf16lo(sc) : bf16hi(sc), j < 8 ? bf16lo(bi) : bf16hi(bi)));
+        else a = as_bf16x8(wa[j]);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) acc[b] = mfma32(a, as_bf16x8(token(cur, Q4 ? kFrags * half + j : 2 * j + half, b)), acc[b]);
       }
       if constexpr (Q4) {
-        if (j % 4 == 3) load_words(s + 1, j >> 2);
-        if (j == kFrags - 1) load_scale(s + 1);
-        if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        if (j == kFrags - 1) load_scales();
+        if (j % 4 == 3) {
+          load_head(j >> 2);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       } else {
-        load_words(s + 1, j);
+        load_head(j);
         if (j % 2 == 1) __builtin_amdgcn_sched_barrier(0);
       }
     }
+    next_head();
     put_tokens(lds + ((s + 1) & 1) * kBytes);
     lds_barrier();
   }
@@ -250,7 +283,7 @@ void lce_few_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W, 
         z[u] = v0 + row + u < V ? acc[b][4 * q + u] : kNegInf;
         top = fmaxf(top, z[u]);
       }
-      if (t < N && t < kTok) *reinterpret_cast<f32x4*>(Z + (long)t * ldz + v0 + row) = z;
+      if (t < N && t < ROWS) *reinterpret_cast<f32x4*>(Z + (long)t * ldz + v0 + row) = z;
     }
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     const float base = top == kNegInf ? 0.f : top * c2;
@@ -264,7 +297,7 @@ void lce_few_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W, 
       }
     s += __shfl_xor(s, 32, 64);
     u += __shfl_xor(u, 32, 64);
-    if (half == 0 && t < kTok) {
+    if (half == 0 && t < ROWS) {
       xm[w][t] = top;
       xs[w][t] = s;
       xu[w][t] = u;
@@ -926,13 +959,14 @@ struct Scratch {
   int2* entries;
   GatherTile* tiles;
   bf16_t* stage;
+  float* stage32;
 };
 
 // k_list: length of a teacher's list (0: scoring, with `top` alternatives).
 Scratch carve(const ScoreShape& sh, int f32, int q4, int top, int k_list, void* ws, size_t* bytes) {
   Scratch x{};
   Carver c{static_cast<char*>(ws)};
-  x.few = !f32 && sh.n <= kFewTokens;
+  x.few = f32 ? sh.n <= kFewTokens32 && sh.d % 4 == 0 : sh.n <= kFewTokens;
   x.rows = sh.n < kScoreRows ? sh.n : kScoreRows;
   x.groups = groups_of(sh.v);
   x.ldg = x.few ? x.groups : (x.groups + 1) / 2 * 2;  // a tile of 256 logits writes both its groups, the last one too
@@ -972,7 +1006,8 @@ Scratch carve(const ScoreShape& sh, int f32, int q4, int top, int k_list, void* 
     }
     if (q4 && sh.stage) {
       x.stage_rows = sh.v;
-      x.stage = c.take<bf16_t>(sh.v * sh.d);
+      if (f32) x.stage32 = c.take<float>(sh.v * sh.d);
+      else x.stage = c.take<bf16_t>(sh.v * sh.d);
     }
   }
   if (k_list) {
@@ -989,20 +1024,46 @@ Scratch carve(const ScoreShape& sh, int f32, int q4, int top, int k_list, void* 
     if (e != hipSuccess) return e;            \
   } while (0)
 
-hipError_t few_logits(const ScoreHead& h, const ScoreShape& sh, const Scratch& x, float c2, hipStream_t st) {
-  const bf16_t* H = static_cast<const bf16_t*>(h.hidden);
-  const int blocks = (int)ceil_div(sh.n, 32);
+template <class T>
+hipError_t run_few(const T* H, int q4, const T* w, const uint32_t* wq, const T* sc, const T* bi, const ScoreShape& sh, const Scratch& x,
+                   float c2, hipStream_t st) {
   auto run = [&](auto nb, auto rows) {
     constexpr int NB = decltype(nb)::value, ROWS = decltype(rows)::value;
-    auto kernel = h.h.q4 ? lce_few_kernel<1, NB, ROWS, 256> : lce_few_kernel<0, NB, ROWS, 128>;
-    hipLaunchKernelGGL(kernel, dim3(x.groups), dim3(256), 0, st, H, h.h.w, h.h.wq, h.h.sc, h.h.bi, (int)sh.n, (int)sh.d,
-                       (int)sh.v, c2, (int)x.ldz, x.z, x.gmax, x.gs, x.gu);
+    auto kernel = q4 ? lce_few_kernel<T, 1, NB, ROWS> : lce_few_kernel<T, 0, NB, ROWS>;
+    hipLaunchKernelGGL(kernel, dim3(x.groups), dim3(256), 0, st, H, w, wq, sc, bi, (int)sh.n, (int)sh.d, (int)sh.v, c2, (int)x.ldz,
+                       x.z, x.gmax, x.gs, x.gu);
     return hipGetLastError();
   };
   if (sh.n <= 16) return run(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
-  if (blocks == 1) return run(std::integral_constant<int, 1>{}, std::integral_constant<int, 32>{});
-  if (blocks == 2) return run(std::integral_constant<int, 2>{}, std::integral_constant<int, 64>{});
-  return run(std::integral_constant<int, 4>{}, std::integral_constant<int, 128>{});
+  if (sh.n <= 32) return run(std::integral_constant<int, 1>{}, std::integral_constant<int, 32>{});
+  if (sizeof(T) == 4 || sh.n <= 64) return run(std::integral_constant<int, 2>{}, std::integral_constant<int, 64>{});
+  return run(std::integral_constant<int, sizeof(T) == 4 ? 2 : 4>{}, std::integral_constant<int, sizeof(T) == 4 ? 64 : 128>{});
+}
+hipError_t few_logits(const ScoreHead& h, const ScoreShape& sh, const Scratch& x, float c2, hipStream_t st) {
+  if (h.f32) return run_few(static_cast<const float*>(h.hidden), h.h32.q4, h.h32.w, h.h32.wq, h.h32.sc, h.h32.bi, sh, x, c2, st);
+  return run_few(static_cast<const bf16_t*>(h.hidden), h.h.q4, h.h.w, h.h.wq, h.h.sc, h.h.bi, sh, x, c2, st);
+}
+
+// A 4-bit head's rows in fp32 (its group size divides the words of a thread's row).
+__global__ __launch_bounds__(256) void dequant32_kernel(const uint32_t* __restrict__ Wq, const float* __restrict__ Sc,
+                                                        const float* __restrict__ Bi, long words, float* __restrict__ out) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= words) return;
+  const uint32_t q = Wq[i];
+  const float s = Sc[i >> 3], b = Bi[i >> 3];
+  f32x4 x[2];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e >> 2][e & 3] = __builtin_fmaf(s, (float)((q >> (4 * e)) & 15u), b);
+  reinterpret_cast<f32x4*>(out)[2 * i] = x[0];
+  reinterpret_cast<f32x4*>(out)[2 * i + 1] = x[1];
+}
+
+// The head that the product takes: an fp32 4-bit one with a stage is dequantized into it first.
+hipError_t staged_head(ScoreHead& h, const ScoreShape& sh, const Scratch& x, hipStream_t st) {
+  if (x.stage32 == nullptr) return hipSuccess;
+  const hipError_t e = launch_dequant32(h.h32, sh.v, sh.d, x.stage32, st);
+  h.h32 = LceHead32{0, x.stage32, nullptr, nullptr, nullptr};
+  return e;
 }
 
 RowParts row_parts(const Scratch& x, const ScoreHead& h, long n, long v, float c2) {
@@ -1040,12 +1101,21 @@ size_t logprobs_fwd_workspace(const ScoreShape& sh, int f32, int q4, int top) {
   return bytes;
 }
 
-hipError_t launch_logprobs_fwd(const ScoreHead& h, const ScoreShape& sh, const int64_t* targets, long long ignore_index,
+hipError_t launch_dequant32(const LceHead32& h, long V, long D, float* out, hipStream_t st) {
+  const long words = V * D / 8;
+  hipLaunchKernelGGL(dequant32_kernel, dim3((unsigned)ceil_div(words, 256)), dim3(256), 0, st, h.wq, h.sc, h.bi, words, out);
+  return hipGetLastError();
+}
+
+hipError_t launch_logprobs_fwd(const ScoreHead& head, const ScoreShape& sh, const int64_t* targets, long long ignore_index,
                                int top, const LogprobsOut& o, void* ws, hipStream_t st) {
   size_t bytes;
+  ScoreHead h = head;
   const Scratch x = carve(sh, h.f32, h.f32 ? h.h32.q4 : h.h.q4, top, 0, ws, &bytes);
   const float c2 = kLog2e * sh.inv_t;
   const int V = (int)sh.v;
+  const hipError_t staged = staged_head(h, sh, x, st);
+  if (staged != hipSuccess) return staged;
   if (x.few) {
     const hipError_t e = few_logits(h, sh, x, c2, st);
     if (e != hipSuccess) return e;
@@ -1101,11 +1171,14 @@ size_t distill_fwd_workspace(const ScoreShape& sh, int f32, int q4, int k) {
   return bytes;
 }
 
-hipError_t launch_distill_fwd(const ScoreHead& h, const ScoreShape& sh, const int64_t* ids, const float* teacher,
+hipError_t launch_distill_fwd(const ScoreHead& head, const ScoreShape& sh, const int64_t* ids, const float* teacher,
                               const uint8_t* mask, const DistillLoss& p, const DistillOut& o, void* ws, hipStream_t st) {
   size_t bytes;
+  ScoreHead h = head;
   const Scratch x = carve(sh, h.f32, h.f32 ? h.h32.q4 : h.h.q4, 0, p.k, ws, &bytes);
   const float c2 = kLog2e * sh.inv_t;
+  const hipError_t staged = staged_head(h, sh, x, st);
+  if (staged != hipSuccess) return staged;
   float* row_loss = p.reduction == kReduceNone ? o.loss : x.row_loss;
   auto kernel = p.kind == kDistillForward ? distill_rows_kernel<kDistillForward>
                 : p.kind == kDistillReverse ? distill_rows_kernel<kDistillReverse> : distill_rows_kernel<kDistillJsd>;

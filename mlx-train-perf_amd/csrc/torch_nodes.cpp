@@ -536,8 +536,10 @@ ScoreBackward plan_score_backward(const at::Tensor& hidden, const ScoreHead& h, 
   p.kind = h.kind;
   p.rows = n;
   if (hidden.scalar_type() == at::kFloat) {
-    p.chunk = g_api.lce_chunk32(n, d, v, budget_bytes());
-    p.bytes = g_api.score_bwd_ws32(n, d, v, p.chunk, (int)k, want_dw);
+    const size_t budget = budget_bytes();
+    if (h.kind == MTP_HEAD_Q4 && (size_t)v * d * 4 <= budget && !env_is("MTP_LCE_STAGE_HEAD", "0")) p.kind = MTP_HEAD_Q4_STAGED;
+    p.chunk = g_api.lce_chunk32(n, d, v, budget);
+    p.bytes = g_api.score_bwd_ws32(n, d, v, (int)p.kind, p.chunk, (int)k, want_dw);
   } else {
     if (!want_dw || env_is("MTP_LCE_TRANSPOSED_HEAD", "1"))
       p.w_t = python([&] {

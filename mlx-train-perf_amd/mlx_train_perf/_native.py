@@ -131,7 +131,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
        for name in ("mtp_logprobs_fwd_workspace_bytes", "mtp_logprobs_fwd_f32_workspace_bytes",
                     "mtp_distill_fwd_workspace_bytes", "mtp_distill_fwd_f32_workspace_bytes")},
     "mtp_score_bwd_workspace_bytes": (_size, [_i64, _i64, _i64, _i32, _i64, _i64, _i32, _i32]),
-    "mtp_score_bwd_f32_workspace_bytes": (_size, [_i64, _i64, _i64, _i64, _i32, _i32]),
+    "mtp_score_bwd_f32_workspace_bytes": (_size, [_i64, _i64, _i64, _i32, _i64, _i32, _i32]),
     **{name: (ctypes.c_int, [*[_c_void_p] * 6, _i64, _i64, _i64, _i32, _i64, _i32, _f64, *[_c_void_p] * 7, _size, _c_void_p])
        for name in ("mtp_logprobs_fwd", "mtp_logprobs_fwd_f32")},
     **{name: (ctypes.c_int, [*[_c_void_p] * 8, _i64, _i64, _i64, _i32, _i32, _i32, _f64, _f64, _i32, _i32, *[_c_void_p] * 7,

@@ -123,10 +123,19 @@ def _nodes(x: _Inputs):
 
 
 def _forward_kind(x: _Inputs) -> int:
-    """As the loss's forward: a 4-bit head dequantized into the workspace where the budget holds all of it."""
+    """As the loss's forward: a 4-bit head dequantized into the workspace where the budget holds all of it, also in fp32."""
     n, d = x.hidden.shape
-    staged = _loss._forward_stage_bytes(_native.load(), n, d, x.v, x.kind, x.hidden.dtype == torch.float32)
+    f32 = x.hidden.dtype == torch.float32
+    if f32:
+        return _staged32(x)
+    staged = _loss._forward_stage_bytes(_native.load(), n, d, x.v, x.kind, f32)
     return _native.HEAD_Q4_STAGED if staged else x.kind
+
+
+def _staged32(x: _Inputs) -> int:
+    """The kind of an fp32 call: with its weights in registers a 4-bit head's products take some four times as long."""
+    fits = x.kind == _native.HEAD_Q4 and x.v * x.hidden.shape[1] * 4 <= _plan.lce_bwd_budget_bytes()
+    return _native.HEAD_Q4_STAGED if fits and _loss.os.environ.get("MTP_LCE_STAGE_HEAD", "1") != "0" else x.kind
 
 
 def _head_ptrs(x: _Inputs) -> tuple:
@@ -147,8 +156,9 @@ def _backward(x: _Inputs, k: int, want_dw: bool, call) -> tuple[torch.Tensor, to
     d_w = torch.empty_like(x.w) if want_dw else None
     w, w_q, scales, biases = _head_ptrs(x)
     if x.hidden.dtype == torch.float32:
+        kind = _staged32(x)
         chunk = lib.mtp_lce_bwd_f32_chunk(n, d, v, budget)
-        ws_bytes = lib.mtp_score_bwd_f32_workspace_bytes(n, d, v, chunk, k, int(want_dw))
+        ws_bytes = lib.mtp_score_bwd_f32_workspace_bytes(n, d, v, kind, chunk, k, int(want_dw))
         head, after = (w, w_q, scales, biases), (chunk,)
     else:
         mode = _loss.os.environ.get("MTP_LCE_TRANSPOSED_HEAD", "auto")

@@ -117,14 +117,24 @@ def test_hidden_dims_that_no_tile_divides(n, d, v, top):
 
 
 @pytest.mark.parametrize("head", ["dense", "trainable", "q4"])
-@pytest.mark.parametrize(("n", "d", "v", "top"), [(1, 64, 97, 5), (129, 64, 700, 20), (300, 192, 1501, 128)])
+@pytest.mark.parametrize(("n", "d", "v", "top"), [(1, 64, 97, 5), (17, 192, 700, 20), (40, 64, 129, 1), (64, 128, 1000, 64), (65, 64, 300, 4),
+                                                  (129, 64, 700, 20), (300, 192, 1501, 128)])
 def test_fp32(n, d, v, top, head):
     _check_score(n, d, v, top=top, head=head, dtype="fp32", seed=n, temperature=0.8)
 
 
-@pytest.mark.parametrize(("n", "d", "v"), [(7, 33, 301), (131, 33, 301), (150, 70, 500)])
+@pytest.mark.parametrize(("n", "d", "v"), [(7, 33, 301), (9, 36, 500), (131, 33, 301), (150, 70, 500)])
 def test_fp32_odd_hidden_dims(n, d, v):
     _check_score(n, d, v, top=6, head="trainable", dtype="fp32", seed=n)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("n", [3, 90, 140])
+def test_a_4bit_head_in_registers(n, dtype, monkeypatch):
+    """MTP_LCE_STAGE_HEAD=0: no copy of the head's rows, forward or backward."""
+    monkeypatch.setenv("MTP_LCE_STAGE_HEAD", "0")
+    _check_score(n, 192, 700, top=5, head="q4", dtype=dtype, seed=n)
+    _check_distill(n, 192, 700, 6, head="q4", dtype=dtype, seed=n)
 
 
 @pytest.mark.parametrize("n", [4, 140])
