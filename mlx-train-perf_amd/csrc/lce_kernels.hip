@@ -1882,7 +1882,9 @@ void lce_bwd_dw_kernel(const bf16_t* __restrict__ G, int ldg, const bf16_t* __re
   __shared__ __attribute__((aligned(16))) char lds[kLdsBytes];
   const int dtiles = (D + kTile - 1) / kTile;
   int vt, dt;
-  if (!xcd_tile(ctiles, dtiles, vt, dt)) return;
+  // xcd_tile deals its second axis out to the XCDs: the dims where they are whole rounds of 8 tiles, else the vocabulary (4 dim
+  // tiles gave half the XCDs nothing: 2048 x 896 x 151936 1161 us, now DWORDER).
+  if (!(dtiles % 8 == 0 ? xcd_tile(ctiles, dtiles, vt, dt) : xcd_tile(dtiles, ctiles, dt, vt))) return;
   const int tid = threadIdx.x;
   const int lane = tid & 63, w = tid >> 6;
   const int wa = w & 1, wb = w >> 1;
@@ -2402,7 +2404,7 @@ static hipError_t lce_bwd_rows(const LceHead& h, const bf16_t* H, const int64_t*
       }
     }
     if (dW != nullptr && !h.q4) {
-      dim3 wgrid(8 * ctiles * ((dtiles + 7) / 8));
+      dim3 wgrid(dtiles % 8 == 0 ? ctiles * dtiles : 8 * dtiles * ((ctiles + 7) / 8));
       const bf16_t* rows = affine ? static_cast<const bf16_t*>(affine->clean) : H;
       hipLaunchKernelGGL(lce_bwd_dw_kernel, wgrid, block, 0, stream, Gbuf, ldg, rows, N, D, V, vb, ve, ctiles, dW);
       e = hipGetLastError();
