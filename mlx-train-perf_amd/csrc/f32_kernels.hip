@@ -337,7 +337,7 @@ void lce32_fwd_kernel(const float* __restrict__ H, const float* __restrict__ W,
                                                         const float* __restrict__ Bi, int N, int D, int V, int nsplit,
                                                         float* __restrict__ part_m, float* __restrict__ part_s, float scale2,
                                                         float* __restrict__ part_u, float* __restrict__ gmax, int ldg,
-                                                        ScoreList list) {
+                                                        float* __restrict__ Z, long ldz, ScoreList list) {
   const float c2 = STAT ? scale2 : kLog2e;
   constexpr float kHidden = (STAT & kStatEntropy) ? -1e30f : kNegInf;
   __shared__ float gx[(STAT & kStatGroups) ? kT : 1];
@@ -377,6 +377,18 @@ void lce32_fwd_kernel(const float* __restrict__ H, const float* __restrict__ W,
           if (v >= V) acc[i][j][r] = kHidden;
           mz = fmaxf(mz, acc[i][j][r]);
         }
+      if constexpr (STAT & kStatKeep) {
+        const int t = t0 + 64 * wb + 32 * j + (lane & 31);
+        if (t < N) {
+          float* row = Z + t * ldz + v0 + 64 * wa + 4 * h;
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              *reinterpret_cast<f32x4*>(row + 32 * i + 8 * q) =
+                  f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        }
+      }
       if constexpr (STAT & kStatGroups) {  // the tile's maximum of each token: of both halves of both waves
         const float both = fmaxf(mz, __shfl_xor(mz, 32, 64));
         const int tl = 64 * wb + 32 * j + (lane & 31);
@@ -772,20 +784,20 @@ int lce32_fwd_nsplit(long N, long V) {
 static bool copied_tiles(long d, long ld) { return d % 4 == 0 && ld % 4 == 0 && d < (1L << 21) && ld < (1L << 21); }
 
 template <int STAT>
-static hipError_t lce32_fwd_tiles(const LceHead32& h, const float* H, int N, int D, int V, float* pm, float* ps, float scale2,
-                                  float* pu, float* gmax, int ldg, const ScoreList& list, hipStream_t st) {
+static hipError_t lce32_fwd_tiles(const LceHead32& h, const float* H, int N, int D, int V, const ScoreStats& x, hipStream_t st) {
   const int ns = lce32_fwd_nsplit(N, V);
   auto kernel = h.q4 ? lce32_fwd_kernel<kQ4, STAT> : copied_tiles(D, D) ? lce32_fwd_kernel<kCopied, STAT> : lce32_fwd_kernel<kDense, STAT>;
-  hipLaunchKernelGGL(kernel, dim3((N + kT - 1) / kT, ns), dim3(256), 0, st, H, h.w, h.wq, h.sc, h.bi, N, D, V, ns, pm, ps,
-                     scale2, pu, gmax, ldg, list);
+  hipLaunchKernelGGL(kernel, dim3((N + kT - 1) / kT, ns), dim3(256), 0, st, H, h.w, h.wq, h.sc, h.bi, N, D, V, ns, x.m, x.s,
+                     x.scale2, x.u, x.gmax, x.ldg, x.z, x.ldz, x.list);
   return hipGetLastError();
 }
 
 hipError_t launch_lce32_stats(const LceHead32& h, const float* H, int N, int D, int V, const ScoreStats& x, hipStream_t st) {
-  if (x.gmax)
-    return lce32_fwd_tiles<kStatScaled | kStatEntropy | kStatGroups>(h, H, N, D, V, x.m, x.s, x.scale2, x.u, x.gmax, x.ldg, x.list, st);
-  if (x.u) return lce32_fwd_tiles<kStatScaled | kStatEntropy>(h, H, N, D, V, x.m, x.s, x.scale2, x.u, nullptr, 0, x.list, st);
-  return lce32_fwd_tiles<kStatScaled | kStatList>(h, H, N, D, V, x.m, x.s, x.scale2, nullptr, nullptr, 0, x.list, st);
+  constexpr int kEntropy = kStatScaled | kStatEntropy, kGroups = kEntropy | kStatGroups;
+  if (x.z) return lce32_fwd_tiles<kGroups | kStatKeep>(h, H, N, D, V, x, st);
+  if (x.gmax) return lce32_fwd_tiles<kGroups>(h, H, N, D, V, x, st);
+  if (x.u) return lce32_fwd_tiles<kEntropy>(h, H, N, D, V, x, st);
+  return lce32_fwd_tiles<kStatScaled | kStatList>(h, H, N, D, V, x, st);
 }
 
 hipError_t launch_lce32_target(const LceHead32& h, const float* H, const int64_t* targets, int N, int D, int V, float* tgt,
@@ -807,7 +819,10 @@ hipError_t launch_lce32_fwd(const LceHead32& h, const float* H, const int64_t* t
   const int ns = lce32_fwd_nsplit(N, V);
   float* pm = ws;
   float* ps = ws + (long)ns * N;
-  hipError_t e = lce32_fwd_tiles<0>(h, H, N, D, V, pm, ps, 0.f, nullptr, nullptr, 0, ScoreList{}, st);
+  ScoreStats stats{};
+  stats.m = pm;
+  stats.s = ps;
+  hipError_t e = lce32_fwd_tiles<0>(h, H, N, D, V, stats, st);
   if (e != hipSuccess) return e;
   const dim3 block(256);
   dim3 fgrid((N + 3) / 4);

@@ -888,8 +888,8 @@ __device__ __forceinline__ bool xcd_rect_tile(int mtiles, int ntiles, int& m, in
 //
 // STAT (mtp_launch.hpp, kStat...) is what token scoring wants beside it: the softmax of z / temperature (scale2 =
 // log2(e) / temperature), the sum of 2^(x - m) (x - m) that the entropy is made of (an fma per logit), and the maximum of
-// every group of kGroup logits, which the tile's own maximum holds already; or the logits of a list of columns a row
-// (ListCursor). 0 is the loss as it was.
+// every group of kGroup logits, which the tile's own maximum holds already, with the logits themselves or without; or the
+// logits of a list of columns a row (ListCursor). 0 is the loss as it was.
 // ------------------------------------------------------------------------------------------
 template <int Q4, int STAT = 0>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
@@ -897,7 +897,8 @@ void lce_fwd_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
                     const uint32_t* __restrict__ Wq, const bf16_t* __restrict__ Sc,
                     const bf16_t* __restrict__ Bi, int N, int D, int V, int nsplit, int split0, int nlocal,
                     int wrow0, float* __restrict__ part_m, float* __restrict__ part_s, float scale2,
-                    float* __restrict__ part_u, float* __restrict__ gmax, int ldg, ScoreList list) {
+                    float* __restrict__ part_u, float* __restrict__ gmax, int ldg, float* __restrict__ Z, long ldz,
+                    ScoreList list) {
   const float c2 = STAT ? scale2 : kLog2e;
   // Hidden rows past V: beyond any logit, but finite where 0 of it has to be 0.
   constexpr float kHidden = (STAT & kStatEntropy) ? -1e30f : kNegInf;
@@ -964,6 +965,21 @@ void lce_fwd_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
             const int v = v0 + 128 * wa + 32 * i + 8 * (r >> 2) + 4 * lhalf + (r & 3);
             if (v >= V) acc[i][j][r] = kHidden;
           }
+    }
+    if constexpr (STAT & kStatKeep) {
+      const int v = v0 + 128 * wa + 4 * lhalf;
+#pragma unroll
+      for (int j = 0; j < kNJ; ++j) {
+        const int t = t0 + 64 * wb + 32 * j + lcol;
+        if (t >= N || v0 + 128 * wa >= ldz) continue;
+        float* row = Z + t * ldz + v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<f32x4*>(row + 32 * i + 8 * q) =
+                f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+      }
     }
     // Four partial maxima and sums per token column, combined in a fixed order: four short
     // dependency chains instead of one 64 long (forward -1%).
@@ -1883,7 +1899,7 @@ void lce_bwd_dw_kernel(const bf16_t* __restrict__ G, int ldg, const bf16_t* __re
   const int dtiles = (D + kTile - 1) / kTile;
   int vt, dt;
   // xcd_tile deals its second axis out to the XCDs: the dims where they are whole rounds of 8 tiles, else the vocabulary (4 dim
-  // tiles gave half the XCDs nothing: 2048 x 896 x 151936 1161 us, now DWORDER).
+  // tiles gave half the XCDs nothing: 2048 x 896 x 151936 1161 us, now 668).
   if (!(dtiles % 8 == 0 ? xcd_tile(ctiles, dtiles, vt, dt) : xcd_tile(dtiles, ctiles, dt, vt))) return;
   const int tid = threadIdx.x;
   const int lane = tid & 63, w = tid >> 6;
@@ -2169,14 +2185,18 @@ long lce_fwd_stage_rows_used(long N, long V, long stage_rows) {
   return most;
 }
 
-// The forward's tiles: partials part_m, part_s (and what STAT adds, else null) [splits][N].
+// The forward's tiles with the statistics of STAT.
 template <int STAT>
-static hipError_t lce_fwd_tiles(const LceHead& h, const bf16_t* H, int N, int D, int V, float* pm, float* ps, float scale2,
-                                float* pu, float* gmax, int ldg, const ScoreList& list, bf16_t* stage,
+static hipError_t lce_fwd_tiles(const LceHead& h, const bf16_t* H, int N, int D, int V, const ScoreStats& x, bf16_t* stage,
                                 long stage_rows, hipStream_t stream) {
   const int ns = lce_fwd_nsplit(N, V);
   const int rtiles = (N + kTile - 1) / kTile;
-  dim3 block(kThreads);
+  // Splits [s0, s1) over rows w of the head from row r0 on.
+  auto run = [&](auto q4, const bf16_t* w, int s0, int s1, long r0) {
+    hipLaunchKernelGGL((lce_fwd_kernel<decltype(q4)::value, STAT>), dim3(rtiles * (s1 - s0)), dim3(kThreads), 0, stream, H, w, h.wq,
+                       h.sc, h.bi, N, D, V, ns, s0, s1 - s0, (int)r0, x.m, x.s, x.scale2, x.u, x.gmax, x.ldg, x.z, x.ldz, x.list);
+    return hipGetLastError();
+  };
   if (h.q4 && stage != nullptr && D % kBK == 0) {
     // Runs of whole vocab splits whose rows fit the staging buffer: each run's rows dequantized
     // into it, then the dense product over them. The splits and their tiles are those of the
@@ -2189,33 +2209,23 @@ static hipError_t lce_fwd_tiles(const LceHead& h, const bf16_t* H, int N, int D,
       const long nw = rows * D / 8;
       hipLaunchKernelGGL(lce_head_dequant_kernel, dim3((unsigned)((nw + 1023) / 1024)), dim3(256), 0, stream,
                          h.wq + r0 * (D >> 3), h.sc + r0 * (D >> 6), h.bi + r0 * (D >> 6), nw, stage);
-      hipError_t de = hipGetLastError();
-      if (de != hipSuccess) return de;
-      hipLaunchKernelGGL((lce_fwd_kernel<0, STAT>), dim3(rtiles * (s1 - s0)), block, 0, stream, H, stage, h.wq, h.sc, h.bi,
-                         N, D, V, ns, s0, s1 - s0, (int)r0, pm, ps, scale2, pu, gmax, ldg, list);
-      de = hipGetLastError();
-      if (de != hipSuccess) return de;
+      hipError_t e = hipGetLastError();
+      if (e == hipSuccess) e = run(std::integral_constant<int, 0>{}, stage, s0, s1, r0);
+      if (e != hipSuccess) return e;
       s0 = s1;
     }
-  } else if (h.q4) {
-    hipLaunchKernelGGL((lce_fwd_kernel<1, STAT>), dim3(rtiles * ns), block, 0, stream, H, h.w, h.wq, h.sc, h.bi, N, D, V,
-                       ns, 0, ns, 0, pm, ps, scale2, pu, gmax, ldg, list);
-  } else {
-    hipLaunchKernelGGL((lce_fwd_kernel<0, STAT>), dim3(rtiles * ns), block, 0, stream, H, h.w, h.wq, h.sc, h.bi, N, D, V,
-                       ns, 0, ns, 0, pm, ps, scale2, pu, gmax, ldg, list);
+    return hipSuccess;
   }
-  return hipGetLastError();
+  return h.q4 ? run(std::integral_constant<int, 1>{}, h.w, 0, ns, 0) : run(std::integral_constant<int, 0>{}, h.w, 0, ns, 0);
 }
 
-hipError_t launch_lce_stats(const LceHead& h, const bf16_t* H, int N, int D, int V, const ScoreStats& st, bf16_t* stage,
+hipError_t launch_lce_stats(const LceHead& h, const bf16_t* H, int N, int D, int V, const ScoreStats& x, bf16_t* stage,
                             long stage_rows, hipStream_t stream) {
-  auto tiles = [&](auto stat) {
-    return lce_fwd_tiles<decltype(stat)::value>(h, H, N, D, V, st.m, st.s, st.scale2, st.u, st.gmax, st.ldg, st.list, stage,
-                                                stage_rows, stream);
-  };
-  if (st.gmax) return tiles(std::integral_constant<int, kStatScaled | kStatEntropy | kStatGroups>{});
-  if (st.u) return tiles(std::integral_constant<int, kStatScaled | kStatEntropy>{});
-  return tiles(std::integral_constant<int, kStatScaled | kStatList>{});
+  constexpr int kEntropy = kStatScaled | kStatEntropy, kGroups = kEntropy | kStatGroups;
+  if (x.z) return lce_fwd_tiles<kGroups | kStatKeep>(h, H, N, D, V, x, stage, stage_rows, stream);
+  if (x.gmax) return lce_fwd_tiles<kGroups>(h, H, N, D, V, x, stage, stage_rows, stream);
+  if (x.u) return lce_fwd_tiles<kEntropy>(h, H, N, D, V, x, stage, stage_rows, stream);
+  return lce_fwd_tiles<kStatScaled | kStatList>(h, H, N, D, V, x, stage, stage_rows, stream);
 }
 
 hipError_t launch_lce_fwd(const LceHead& h, const bf16_t* H, const int64_t* targets, int N, int D, int V,
@@ -2224,7 +2234,10 @@ hipError_t launch_lce_fwd(const LceHead& h, const bf16_t* H, const int64_t* targ
   const int ns = lce_fwd_nsplit(N, V);
   float* pm = ws;
   float* ps = ws + (long)ns * N;
-  hipError_t e = lce_fwd_tiles<0>(h, H, N, D, V, pm, ps, 0.f, nullptr, nullptr, 0, ScoreList{}, stage, stage_rows, stream);
+  ScoreStats stats{};
+  stats.m = pm;
+  stats.s = ps;
+  hipError_t e = lce_fwd_tiles<0>(h, H, N, D, V, stats, stage, stage_rows, stream);
   if (e != hipSuccess) return e;
   dim3 fgrid((N + 3) / 4), fblock(256);
   if (h.q4) {

@@ -57,7 +57,7 @@ hipError_t launch_lce_fwd(const LceHead& h, const bf16_t* H, const int64_t* targ
                           bf16_t* stage, long stage_rows, hipStream_t stream);
 
 // Token scoring (score_kernels.hip) takes the forward's tiles with more of their statistics. A forward's STAT is a sum of:
-enum { kStatScaled = 1, kStatEntropy = 2, kStatGroups = 4, kStatList = 8 };
+enum { kStatScaled = 1, kStatEntropy = 2, kStatGroups = 4, kStatList = 8, kStatKeep = 16 };
 constexpr int kGroup = 128;  // consecutive logits whose maximum a forward keeps
 // Logits to keep of each row: ascending columns (kNoColumn past the last) to their places in z.
 constexpr int kNoColumn = 0x7fffffff;
@@ -72,6 +72,8 @@ struct ScoreStats {
   float* u;            // the same of 2^(x - m) (x - m), or null
   float* gmax;         // [N][ldg] the maximum z of each group of kGroup (ldg: an even number of them), or null (with u)
   int ldg;
+  float* z;            // [N][ldz] the logits, or null (with gmax); ldz a multiple of kGroup
+  long ldz;
   ScoreList list;
 };
 hipError_t launch_lce_stats(const LceHead& h, const bf16_t* H, int N, int D, int V, const ScoreStats& st, bf16_t* stage,
@@ -205,6 +207,7 @@ constexpr int kScoreTop = 128;       // most alternatives, and longest teacher's
 constexpr long kScoreVocab = 1 << 21;
 constexpr long kFewTokens = 128;     // tokens up to which a bf16 forward keeps its logits
 constexpr long kFewTokens32 = 64;    // an fp32 one (hidden dims that are multiples of 4)
+constexpr long kKeptBytes = 256L << 20;  // of logits that a forward with alternatives may keep
 constexpr double kTailFloor = 1e-6;  // least mass that the outcomes outside a list count as
 
 // One head of either type; w32 where the hidden states are fp32.

@@ -12,7 +12,8 @@
 // choose among them. The logits of a teacher's list, sorted first, the product's tiles put away as they pass (ListCursor): the
 // very ones that the sums hold, so that what a list leaves of 1 is exact to fp32 and not to two roundings of a large logit.
 //
-// Up to kFewTokens tokens (kFewTokens32) the logits themselves are kept in the workspace (lce_few_kernel), which leaves two launches.
+// Up to kFewTokens tokens (kFewTokens32) the logits themselves are kept in the workspace (lce_few_kernel), which leaves two launches;
+// where there are not many of them (keep_logits), the product's tiles keep them too.
 #include <math.h>
 
 #include <type_traits>
@@ -34,9 +35,12 @@ __device__ __forceinline__ uint32_t order_key(float x) {
 }
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 
+constexpr int kRanked = 512;  // keys that are ordered by counting
 struct PickScratch {
   int4 count[2][kPick / 64];
   int sum[kPick / 64], listed;
+  uint32_t least, top[kPick];
+  int list[kRanked], rank[kRanked];
 };
 
 // Sum over the threads before this one.
@@ -122,13 +126,80 @@ __device__ __forceinline__ uint32_t pick_largest(const uint32_t* key, int M, int
   return least;
 }
 
+// The positions of the keys that are at least `least` to s.list, in no order; how many of them (beyond kRanked: not all listed).
+__device__ __forceinline__ int list_from(const uint32_t* key, int M, uint32_t least, PickScratch& s) {
+  const int lane = threadIdx.x & 63;
+  if (threadIdx.x == 0) s.listed = 0;
+  __syncthreads();
+  for (int base = 0; base < M; base += kPick) {
+    const int i = base + threadIdx.x;
+    const bool in = i < M && key[i] >= least;
+    const uint64_t who = __ballot(in);
+    int first = 0;
+    if (lane == 0 && who) first = atomicAdd(&s.listed, __popcll(who));
+    first = __builtin_amdgcn_readfirstlane(first) + __popcll(who & ((1ull << lane) - 1));
+    if (in && first < kRanked) s.list[first] = i;
+  }
+  __syncthreads();
+  return s.listed;
+}
+// How many of the n listed keys come before the i-th listed: larger ones, and equal ones of a lower position.
+__device__ __forceinline__ int rank_of(const uint32_t* key, int i, int n, const PickScratch& s) {
+  const int p = s.list[i];
+  const uint32_t mine = key[p];
+  int rank = 0;
+  for (int j = 0; j < n; ++j) {
+    const int o = s.list[j];
+    const uint32_t other = key[o];
+    rank += other > mine || (other == mine && o < p);
+  }
+  return rank;
+}
+
+// pick_largest for keys that mostly differ. The K-th largest of the 256 threads' own maxima is at most the K-th largest key, and
+// mostly few more than K keys reach it (every wave finds it by itself, from four of them a lane: no barriers); those are put in
+// order by counting. 1187 keys, 8 of them: 8192 rows 95 us with 16 counts over all keys, now 61.
+template <int R>
+__device__ __forceinline__ uint32_t pick_few(const uint32_t* key, int M, int K, int* at, PickScratch& s) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  uint32_t mine = 0;
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    if (r * kPick + tid < M) mine = key[r * kPick + tid] > mine ? key[r * kPick + tid] : mine;
+  s.top[tid] = mine;
+  __syncthreads();
+  uint32_t v[kPick / 64], least = 0;
+#pragma unroll
+  for (int i = 0; i < kPick / 64; ++i) v[i] = s.top[lane + 64 * i];
+  for (int b = 31; b >= 0; --b) {
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < kPick / 64; ++i) n += __popcll(__ballot(v[i] >= (least | 1u << b)));
+    if (n >= K) least |= 1u << b;
+  }
+  const int n = list_from(key, M, least, s);
+  if (n > kRanked) return pick_largest<R>(key, M, K, at, s);
+  for (int i = tid; i < n; i += kPick) s.rank[i] = rank_of(key, i, n, s);
+  __syncthreads();
+  for (int i = tid; i < n; i += kPick) {
+    if (s.rank[i] >= K) continue;
+    if (s.rank[i] == K - 1) s.least = key[s.list[i]];
+    int place = 0;
+    for (int j = 0; j < n; ++j) place += s.rank[j] < K && s.list[j] < s.list[i];
+    at[place] = s.list[i];
+  }
+  __syncthreads();
+  return s.least;
+}
+
 // ------------------------------------------------------------------------------------------
 // Few tokens: the logits [N][ldz] in fp32, and per group of kGroup of them their maximum and, relative to
 // it, the two sums. The head is read once and bounds it; a workgroup takes one group: 4 waves of 32 vocab rows, the rows'
 // fragments straight from memory to registers, each loaded for the next slab as soon as its product has gone out (a whole slab in
-// flight a wave, 8 KiB of a dense head, 4 or 2 of a 4-bit one), the tokens' slab (NB blocks of 32) through LDS, one barrier a
-// slab. The registers leave room for 5 workgroups a CU: all 1187 groups of 151936 run at once (with 4 the rest ran alone
-// after them: 262 us a token at 4096 x 151936, now FEWDENSE).
+// flight a wave, 8 KiB of a dense head, 4 of a 4-bit one), the tokens' slab (NB blocks of 32) through LDS, one barrier a
+// slab. The registers and, up to 16 tokens, the LDS leave room for 5 workgroups a CU: all 1187 groups of 151936 run at once
+// (16 tokens over a 4-bit head, 4 workgroups and 5: 157 and 130 us). 4096 x 151936: a dense head's 1.24 GB in 245 us (5.1 TB/s, as
+// a library product of one row), a 4-bit head's 0.39 GB in 104, where the vector units are busy for some 60.
 // ------------------------------------------------------------------------------------------
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base, long bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, bytes > 0x7fffffffL ? 0x7fffffff : (int)bytes, 0x00020000);
@@ -153,7 +224,11 @@ void lce_few_kernel(const T* __restrict__ H, const T* __restrict__ W, const uint
   constexpr int kWords = Q4 ? kSlab / 16 : 0;                    // a lane's packed words
   constexpr int kLoads = Q4 ? kWords / 4 : kChunks / 2;          // a lane's 16-byte loads of the head
   constexpr int kFrags = Q4 ? kWords : kLoads;                   // products' operands (8 values of a row's k: bf16, or 2 x 4)
-  __shared__ __attribute__((aligned(16))) char lds[2 * kBytes];
+  // bf16 4-bit: scales and biases of four slabs, [128 rows][16 groups] each, through LDS: a row's line of them holds 64 groups,
+  // and loaded for one slab at a time it did not last in L1 (16 x 4096 x 151936: 138 us against 104).
+  constexpr bool kStage = Q4 && !F32;
+  constexpr int kScales = kStage ? 2 * 128 * 32 : 0;
+  __shared__ __attribute__((aligned(16))) char lds[2 * kBytes + kScales];
   float(*xm)[ROWS] = reinterpret_cast<float(*)[ROWS]>(lds);  // after the product: 4 waves' statistics
   float(*xs)[ROWS] = xm + 4;
   float(*xu)[ROWS] = xm + 8;
@@ -172,22 +247,37 @@ void lce_few_kernel(const T* __restrict__ H, const T* __restrict__ W, const uint
   uint32_t wo = Q4 ? (uint32_t)vr * (uint32_t)(D >> 1) + half * (kSlab / 4) : (uint32_t)vr * (uint32_t)D * (uint32_t)sizeof(T) + 16 * half;
   // Scales and biases of the lane's groups of a slab: two in a word (bf16), or one.
   uint32_t sc = 0, bi = 0;
-  const __amdgpu_buffer_rsrc_t rs = rows_rsrc(Q4 ? Sc + (long)v0 * (D >> 6) : W, Q4 ? left * (D >> 6) * (long)sizeof(T) : 0);
-  const __amdgpu_buffer_rsrc_t rb = rows_rsrc(Q4 ? Bi + (long)v0 * (D >> 6) : W, Q4 ? left * (D >> 6) * (long)sizeof(T) : 0);
-  uint32_t so = (uint32_t)vr * (uint32_t)(D >> 6) * (uint32_t)sizeof(T) + (F32 ? 0 : 4 * half);
-  const bool pairs = F32 || (D & 127) == 0;
+  u32x4 stage[2];
+  auto load_stage = [&](int slab) {  // thread: 8 groups of row tid / 2
+    const int row = tid >> 1, g0 = 4 * slab + 8 * (tid & 1), groups = D >> 6;
+    const long at = (long)(v0 + row < V ? v0 + row : V - 1) * groups + g0;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const bf16_t* p = reinterpret_cast<const bf16_t*>(x ? Bi : Sc) + at;
+      stage[x] = zero4();
+      if (groups % 8 == 0) {
+        if (g0 < groups) stage[x] = *reinterpret_cast<const u32x4*>(p);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (g0 + i < groups) stage[x][i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
+      }
+    }
+  };
+  auto put_stage = [&] {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) lds_write16(lds + 2 * kBytes + 4096 * x, 16 * tid, stage[x]);
+  };
+  const __amdgpu_buffer_rsrc_t rs = rows_rsrc(Q4 ? Sc + (long)v0 * (D >> 6) : W, Q4 ? left * (D >> 6) * 4 : 0);
+  const __amdgpu_buffer_rsrc_t rb = rows_rsrc(Q4 ? Bi + (long)v0 * (D >> 6) : W, Q4 ? left * (D >> 6) * 4 : 0);
+  uint32_t so = (uint32_t)vr * (uint32_t)(D >> 6) * 4;
   // The loads' offsets are in the vector operand, which the range is checked for.
   auto load_head = [&](int i) { wa[i] = load16(rw, wo + (Q4 ? 16 : 32) * i, 0); };
   auto next_head = [&] { wo += Q4 ? kSlab / 2 : kRow; };
-  auto load_scales = [&] {
-    if (pairs) {
-      sc = __builtin_amdgcn_raw_buffer_load_b32(rs, so, 0, 0);
-      bi = __builtin_amdgcn_raw_buffer_load_b32(rb, so, 0, 0);
-    } else {  // (a row's last group alone in its word)
-      sc = __builtin_amdgcn_raw_buffer_load_b16(rs, so, 0, 0) | (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(rs, so + 2, 0, 0) << 16;
-      bi = __builtin_amdgcn_raw_buffer_load_b16(rb, so, 0, 0) | (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(rb, so + 2, 0, 0) << 16;
-    }
-    so += kSlab / 64 * (uint32_t)sizeof(T);
+  auto load_scales = [&] {  // fp32
+    sc = __builtin_amdgcn_raw_buffer_load_b32(rs, so, 0, 0);
+    bi = __builtin_amdgcn_raw_buffer_load_b32(rb, so, 0, 0);
+    so += 4;
   };
   u32x4 ha[kParts];
   auto load_tokens = [&](int slab) {
@@ -219,15 +309,23 @@ void lce_few_kernel(const T* __restrict__ H, const T* __restrict__ W, const uint
     for (int e = 0; e < 4; ++e) acc[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], y[e], acc[b], 0, 0, 0);
   };
   load_tokens(0);
-  if constexpr (Q4) load_scales();
+  if constexpr (kStage) load_stage(0);
+  else if constexpr (Q4) load_scales();
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) load_head(i);
   next_head();
   put_tokens(lds);
+  if constexpr (kStage) put_stage();
   lds_barrier();
   for (int s = 0; s < slabs; ++s) {
     const char* cur = lds + (s & 1) * kBytes;
     load_tokens(s + 1);  // (past the end: zeros)
+    if constexpr (kStage) {
+      const char* p = lds + 2 * kBytes + 32 * (32 * w + col) + 8 * (s & 3) + 4 * half;
+      sc = *reinterpret_cast<const uint32_t*>(p);
+      bi = *reinterpret_cast<const uint32_t*>(p + 4096);
+      if ((s & 3) == 3) load_stage(s + 1);  // (past the end: zeros)
+    }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int j = 0; j < kFrags; ++j) {
@@ -254,7 +352,7 @@ void lce_few_kernel(const T* __restrict__ H, const T* __restrict__ W, const uint
         for (int b = 0; b < NB; ++b) acc[b] = mfma32(a, as_bf16x8(token(cur, Q4 ? kFrags * half + j : 2 * j + half, b)), acc[b]);
       }
       if constexpr (Q4) {
-        if (j == kFrags - 1) load_scales();
+        if (F32 && j == kFrags - 1) load_scales();
         if (j % 4 == 3) {
           load_head(j >> 2);
           __builtin_amdgcn_sched_barrier(0);
@@ -267,6 +365,12 @@ void lce_few_kernel(const T* __restrict__ H, const T* __restrict__ W, const uint
     next_head();
     put_tokens(lds + ((s + 1) & 1) * kBytes);
     lds_barrier();
+    if constexpr (kStage) {
+      if ((s & 3) == 3) {  // every wave has read its last of the four
+        put_stage();
+        lds_barrier();
+      }
+    }
   }
 
   // acc[b][r]: vocab row 32 w + 8 (r / 4) + 4 half + r % 4 of the group, token 32 b + col.
@@ -562,40 +666,20 @@ __device__ __forceinline__ void merge_row(const RowParts& p, long t, float& m, f
 // The groups ascend, so positions ascend with the index. `least`: the K-th largest of the groups' maxima (0 with fewer than K
 // groups), below which nothing is chosen: mostly a few more than K are left, and each one's place is its count of those before
 // it. A target among them takes its logit from here.
-constexpr int kRanked = 512;
 template <int MC>
 __device__ __forceinline__ void write_top(const uint32_t* key, const int* group, int ngroups, int K, uint32_t least, int V,
-                                          float inv_t, float lse, long t, long long target, const LogprobsOut& out, int* at,
-                                          PickScratch& s) {
-  const int tid = threadIdx.x, lane = tid & 63, M = ngroups * kGroup;
-  if (tid == 0) s.listed = 0;
-  __syncthreads();
-  for (int base = 0; base < M; base += kPick) {
-    const int i = base + tid;
-    const bool in = i < M && key[i] >= least;
-    const uint64_t who = __ballot(in);
-    int first = 0;
-    if (lane == 0 && who) first = atomicAdd(&s.listed, __popcll(who));
-    first = __builtin_amdgcn_readfirstlane(first) + __popcll(who & ((1ull << lane) - 1));
-    if (in && first < kRanked) at[first] = i;
-  }
-  __syncthreads();
-  int n = s.listed;
-  if (n > kRanked) {  // many equal ones
-    pick_largest<MC / kPick>(key, M, K, at, s);
+                                          float inv_t, float lse, long t, long long target, const LogprobsOut& out, PickScratch& s) {
+  const int M = ngroups * kGroup;
+  int n = list_from(key, M, least, s);
+  if (n > kRanked || n < K) {  // many equal ones; or logits that are no numbers
+    pick_largest<MC / kPick>(key, M, K, s.list, s);
     n = K;
   }
-  for (int i = tid; i < n; i += kPick) {
-    const int p = at[i];
-    const uint32_t mine = key[p];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) {
-      const uint32_t other = key[at[j]];
-      rank += other > mine || (other == mine && at[j] < p);
-    }
+  for (int i = threadIdx.x; i < n; i += kPick) {
+    const int rank = rank_of(key, i, n, s);
     if (rank >= K) continue;
-    const int id = group[p / kGroup] * kGroup + p % kGroup;
-    const float z = key_value(mine), lp = z * inv_t - lse;
+    const int p = s.list[i], id = group[p / kGroup] * kGroup + p % kGroup;
+    const float z = key_value(key[p]), lp = z * inv_t - lse;
     out.top_ids[t * K + rank] = id < V ? id : -1;
     out.top_logprobs[t * K + rank] = lp;
     if (id == target) {
@@ -618,7 +702,7 @@ __global__ __launch_bounds__(kPick) void score_rows_kernel(RowParts parts, const
   __shared__ float x[3][kPick / 64];
   __shared__ PickScratch scratch;
   __shared__ uint32_t key[MG > MC ? MG : MC > 0 ? MC : 1];
-  __shared__ int group[kScoreTop], at[kRanked];
+  __shared__ int group[kScoreTop];
   const long t = blockIdx.x;
   const int tid = threadIdx.x;
   const long long y = targets ? targets[t] : 0;
@@ -651,13 +735,13 @@ __global__ __launch_bounds__(kPick) void score_rows_kernel(RowParts parts, const
   if constexpr (MG > 0) {
     for (int i = tid; i < ngroups; i += kPick) key[i] = order_key(gmax[t * ldg + i]);
     __syncthreads();
-    uint32_t least = pick_largest<MG / kPick>(key, ngroups, take, group, scratch);
+    uint32_t least = pick_few<MG / kPick>(key, ngroups, take, group, scratch);
     if (take < K) least = 0;
     if constexpr (KEPT) {
       for (int i = tid; i < take * kGroup; i += kPick)
         key[i] = order_key(Z[t * ldz + (long)group[i / kGroup] * kGroup + i % kGroup]);
       __syncthreads();
-      write_top<MC>(key, group, take, K, least, V, inv_t, lse, t, targets ? y : -1, out, at, scratch);
+      write_top<MC>(key, group, take, K, least, V, inv_t, lse, t, targets ? y : -1, out, scratch);
     } else if (tid < take) {
       groups[t * take + tid] = group[tid];
       atomicAdd(&counts[group[tid]], 1);
@@ -673,14 +757,14 @@ __global__ __launch_bounds__(kPick) void score_top_kernel(const float* __restric
                                                           int take, LogprobsOut out) {
   __shared__ PickScratch scratch;
   __shared__ uint32_t key[MC];
-  __shared__ int group[kScoreTop], at[kRanked];
+  __shared__ int group[kScoreTop];
   const long t = blockIdx.x;
   const int tid = threadIdx.x;
   if (groups[t * take] < 0) return;  // an ignored token
   for (int i = tid; i < take; i += kPick) group[i] = groups[t * take + i];
   for (int i = tid; i < take * kGroup; i += kPick) key[i] = order_key(rows[t * take * kGroup + i]);
   __syncthreads();
-  write_top<MC>(key, group, take, K, floors[t], V, inv_t, out.lse[t], t, targets ? targets[t] : -1, out, at, scratch);
+  write_top<MC>(key, group, take, K, floors[t], V, inv_t, out.lse[t], t, targets ? targets[t] : -1, out, scratch);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -950,7 +1034,7 @@ struct Carver {
 };
 
 struct Scratch {
-  bool few;
+  bool few, kept;  // kept: the logits are, by the few tokens' kernel or the tiles'
   int groups, ldg, take, max_tiles;  // ldg: floats between the rows of gmax
   long rows, ldz, stage_rows;
   float *m, *s, *u, *gmax, *z, *gs, *gu, *cand, *picks, *row_loss;
@@ -962,17 +1046,23 @@ struct Scratch {
   float* stage32;
 };
 
+// Whether a forward with alternatives writes its logits rather than forming some again: 4 bytes a logit, against the head read
+// once more and five small launches. N x D x V, alternatives; formed again / kept: 333 x 2048 x 32003, 8: 120 / 84 us; 440 x 4096 x
+// 151936, 8: 834 / 617; 2000 x 2048 x 32003, 8: 296 / 292; 8000 x 256 x 8000, 8: 341 / 173; 1000 x 512 x 50000, 8: 110 / 116.
+bool keep_logits(const ScoreShape& sh) { return 4 * sh.n * sh.v <= kKeptBytes; }
+
 // k_list: length of a teacher's list (0: scoring, with `top` alternatives).
 Scratch carve(const ScoreShape& sh, int f32, int q4, int top, int k_list, void* ws, size_t* bytes) {
   Scratch x{};
   Carver c{static_cast<char*>(ws)};
   x.few = f32 ? sh.n <= kFewTokens32 && sh.d % 4 == 0 : sh.n <= kFewTokens;
-  x.rows = sh.n < kScoreRows ? sh.n : kScoreRows;
   x.groups = groups_of(sh.v);
   x.ldg = x.few ? x.groups : (x.groups + 1) / 2 * 2;  // a tile of 256 logits writes both its groups, the last one too
   x.take = top < x.groups ? top : x.groups;
+  x.ldz = (long)x.groups * kGroup;
+  x.kept = x.few || (top && keep_logits(sh));
+  x.rows = x.kept || sh.n < kScoreRows ? sh.n : kScoreRows;
   if (x.few) {
-    x.ldz = (long)x.groups * kGroup;
     x.z = c.take<float>(x.rows * x.ldz);
     x.gmax = c.take<float>(x.rows * x.groups);
     x.gs = c.take<float>(x.rows * x.groups);
@@ -987,12 +1077,13 @@ Scratch carve(const ScoreShape& sh, int f32, int q4, int top, int k_list, void* 
     if (!k_list) x.u = c.take<float>(parts);
     if (top) {
       x.gmax = c.take<float>(x.rows * x.ldg);
-      x.chosen = c.take<int>(x.rows * x.take);
-      x.floors = c.take<uint32_t>(x.rows);
-      x.cand = c.take<float>(x.rows * x.take * kGroup);
     }
-    const long entries = x.rows * x.take;
+    if (x.kept) x.z = c.take<float>(x.rows * x.ldz);
+    const long entries = x.kept ? 0 : x.rows * x.take;
     if (entries) {
+      x.chosen = c.take<int>(entries);
+      x.floors = c.take<uint32_t>(x.rows);
+      x.cand = c.take<float>(entries * kGroup);
       x.counts = c.take<int>(x.groups);
       x.entries = c.take<int2>(entries);
       x.max_tiles = (int)(x.groups + entries / kGroup);  // each group's last tile may be part of one
@@ -1074,7 +1165,7 @@ RowParts row_parts(const Scratch& x, const ScoreHead& h, long n, long v, float c
 
 // The product over rows [r0, r0 + n) with its statistics.
 hipError_t tile_stats(const ScoreHead& h, const ScoreShape& sh, const Scratch& x, long r0, long n, float c2, int k, hipStream_t st) {
-  const ScoreStats stats{c2, x.m, x.s, x.u, x.gmax, x.ldg, ScoreList{x.column, x.picks, k}};
+  const ScoreStats stats{c2, x.m, x.s, x.u, x.gmax, x.ldg, x.kept ? x.z : nullptr, x.ldz, ScoreList{x.column, x.picks, k}};
   if (h.f32)
     return launch_lce32_stats(h.h32, static_cast<const float*>(h.hidden) + r0 * sh.d, (int)n, (int)sh.d, (int)sh.v, stats, st);
   return launch_lce_stats(h.h, static_cast<const bf16_t*>(h.hidden) + r0 * sh.d, (int)n, (int)sh.d, (int)sh.v, stats, x.stage,
@@ -1116,8 +1207,8 @@ hipError_t launch_logprobs_fwd(const ScoreHead& head, const ScoreShape& sh, cons
   const int V = (int)sh.v;
   const hipError_t staged = staged_head(h, sh, x, st);
   if (staged != hipSuccess) return staged;
-  if (x.few) {
-    const hipError_t e = few_logits(h, sh, x, c2, st);
+  if (x.kept) {  // (one pass: as many rows as that keeps are fewer than a pass takes)
+    const hipError_t e = x.few ? few_logits(h, sh, x, c2, st) : tile_stats(h, sh, x, 0, sh.n, c2, 0, st);
     if (e != hipSuccess) return e;
     auto rows = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, dim3((unsigned)sh.n), dim3(kPick), 0, st, row_parts(x, h, sh.n, sh.v, c2), x.gmax, x.groups, x.ldg, x.z,

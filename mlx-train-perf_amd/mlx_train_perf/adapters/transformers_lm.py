@@ -1,6 +1,7 @@
 """Trainer adapter for torch causal LMs: `split_model`, `make_loss_fn`, `make_packed_loss_fn`
 (the torch counterpart of src/mlx_train_perf/adapters/mlx_lm.py:140-297), and beyond the reference
-`make_token_nll_fn`, `make_preference_loss_fn` and `make_policy_loss_fn` for steps on preferences and rewards.
+`make_token_nll_fn`, `make_preference_loss_fn` and `make_policy_loss_fn` for steps on preferences and rewards,
+`make_token_logprobs_fn` and `make_distillation_loss_fn` for scoring tokens and for learning from a teacher's scores.
 
 Loss contract (the mlx-lm trainer's `default_loss`, quoted at adapters/mlx_lm.py:5-20):
 inputs = batch[:, :-1], targets = batch[:, 1:], steps = 1..T, mask = (steps >= lengths[:, 0]) &
@@ -26,6 +27,7 @@ from torch import nn
 from mlx_train_perf.attention.segments import PackedMask, SpanMask
 from mlx_train_perf.core.loss import DenseHead, HeadRef, linear_cross_entropy, resolve_impl, tied_head
 from mlx_train_perf.core.preference import PolicyLoss, PreferenceLoss, policy_loss, preference_loss
+from mlx_train_perf.core.scoring import TokenLogprobs, distillation_loss, token_logprobs
 from mlx_train_perf.errors import AdapterError
 
 _Impl = Literal["auto", "kernel", "chunked", "naive"]
@@ -115,23 +117,32 @@ def make_packed_loss_fn(model: Any, *, impl: _Impl = "auto", allow_unverified_ml
     return loss_fn
 
 
+def _refuse_capped_logits(model: Any) -> None:
+    cfg = getattr(model, "config", None)
+    if getattr(cfg, "final_logit_softcapping", None):   # (0, like None: no cap)
+        raise AdapterError("the fused loss does not cap logits (config.final_logit_softcapping is set)")
+
+
+def _hidden_and_head(model: Any, batch: torch.Tensor, spans: SpanMask | None) -> tuple[torch.Tensor, HeadRef]:
+    """The hidden states of the inputs batch[:, :-1] and the head."""
+    from mlx_train_perf.attention.wrapper import is_enabled  # noqa: PLC0415
+
+    trunk, head = split_model(model)
+    if spans is not None and not is_enabled(model):
+        raise AdapterError("spans require enable_flash_attention(model) first")
+    return trunk(batch[:, :-1], **({} if spans is None else {"mtp_spans": spans})), head
+
+
 def make_token_nll_fn(model: Any, *, impl: _Impl = "auto",
                       allow_unverified_mlx: bool = False) -> Callable[..., torch.Tensor]:
     """`nll(model, batch, spans=None) -> (B, T)`, the per-token losses of the targets batch[:, 1:]: what the losses
     below take from frozen models (call it under `torch.no_grad()` for those). `spans`: a `SpanMask` over the inputs
     batch[:, :-1], handed to every attention call; requires `enable_flash_attention(model)`."""
-    from mlx_train_perf.attention.wrapper import is_enabled  # noqa: PLC0415
-
     split_model(model)
-    cfg = getattr(model, "config", None)
-    if getattr(cfg, "final_logit_softcapping", None):   # (0, like None: no cap)
-        raise AdapterError("the fused loss does not cap logits (config.final_logit_softcapping is set)")
+    _refuse_capped_logits(model)
 
     def nll_fn(model_arg: Any, batch: torch.Tensor, spans: SpanMask | None = None) -> torch.Tensor:
-        trunk, head = split_model(model_arg)
-        if spans is not None and not is_enabled(model_arg):
-            raise AdapterError("spans require enable_flash_attention(model) first")
-        hidden = trunk(batch[:, :-1], **({} if spans is None else {"mtp_spans": spans}))
+        hidden, head = _hidden_and_head(model_arg, batch, spans)
         return linear_cross_entropy(hidden, head, batch[:, 1:], impl=impl, reduction="none", validate_targets=False,
                                     allow_unverified_mlx=allow_unverified_mlx).to(torch.float32)
 
@@ -179,5 +190,44 @@ def make_policy_loss_fn(model: Any, *, clip_low: float = 0.2, clip_high: float =
         return policy_loss(nll, old_nll, advantages, ref_nll=ref_nll, mask=_target_mask(lengths, nll.shape[1]),
                            clip_low=clip_low, clip_high=clip_high, kl_coef=kl_coef, reduction=reduction,
                            impl=_row_loss_impl(impl))
+
+    return loss_fn
+
+
+def make_token_logprobs_fn(model: Any, *, top: int = 0, temperature: float = 1.0, impl: _Impl = "auto",
+                           allow_unverified_mlx: bool = False) -> Callable[..., TokenLogprobs]:
+    """`score(model, batch, lengths=None, spans=None) -> TokenLogprobs` of the targets batch[:, 1:], (B, T) each, with the `top`
+    alternatives of every position (a teacher's lists for `make_distillation_loss_fn`: call it under `torch.no_grad()`).
+    `lengths` (B, 2) as in `make_loss_fn` leaves the positions outside out. `spans` as in `make_token_nll_fn`."""
+    split_model(model)
+    _refuse_capped_logits(model)
+
+    def score_fn(model_arg: Any, batch: torch.Tensor, lengths: torch.Tensor | None = None,
+                 spans: SpanMask | None = None) -> TokenLogprobs:
+        hidden, head = _hidden_and_head(model_arg, batch, spans)
+        targets = batch[:, 1:]
+        if lengths is not None:
+            targets = targets.masked_fill(~_target_mask(lengths, targets.shape[1]), -100)
+        return token_logprobs(hidden, head, targets, top=top, temperature=temperature, impl=_row_loss_impl(impl),
+                              allow_unverified_mlx=allow_unverified_mlx, validate_targets=False)
+
+    return score_fn
+
+
+def make_distillation_loss_fn(model: Any, *, kind: Literal["forward", "reverse", "jsd"] = "forward", beta: float = 0.5,
+                              temperature: float = 1.0, renormalize: bool = False, impl: _Impl = "auto",
+                              allow_unverified_mlx: bool = False) -> Callable[..., torch.Tensor]:
+    """`loss(model, batch, lengths, teacher_ids, teacher_logprobs, spans=None) -> loss`: `distillation_loss` over the positions
+    of the targets batch[:, 1:] that `lengths` (as in `make_loss_fn`) takes in; the teacher's lists (B, T, K) are its
+    `make_token_logprobs_fn(..., top=K)` of the same batch."""
+    split_model(model)
+    _refuse_capped_logits(model)
+
+    def loss_fn(model_arg: Any, batch: torch.Tensor, lengths: torch.Tensor, teacher_ids: torch.Tensor,
+                teacher_logprobs: torch.Tensor, spans: SpanMask | None = None) -> torch.Tensor:
+        hidden, head = _hidden_and_head(model_arg, batch, spans)
+        return distillation_loss(hidden, head, teacher_ids, teacher_logprobs, mask=_target_mask(lengths, batch.shape[1] - 1),
+                                 kind=kind, beta=beta, temperature=temperature, renormalize=renormalize,
+                                 impl=_row_loss_impl(impl), allow_unverified_mlx=allow_unverified_mlx, validate_ids=False)
 
     return loss_fn

@@ -100,7 +100,8 @@ def _check_distill(n, d, v, k, *, head="dense", dtype="bf16", kind="forward", re
 # ---- scoring ------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("head", ["dense", "trainable", "q4"])
-@pytest.mark.parametrize(("n", "d", "v", "top"), [(1, 64, 97, 5), (3, 128, 1000, 20), (33, 64, 129, 1), (65, 192, 700, 128), (128, 256, 3001, 8)])
+@pytest.mark.parametrize(("n", "d", "v", "top"), [(1, 64, 97, 5), (3, 128, 1000, 20), (33, 64, 129, 1), (65, 192, 700, 128), (128, 256, 3001, 8),
+                                                  (9, 1024, 300, 4), (20, 1536, 260, 6), (40, 640, 200, 3)])
 def test_few_tokens(n, d, v, top, head):
     _check_score(n, d, v, top=top, head=head, seed=n)
 
@@ -185,9 +186,96 @@ def test_a_vocabulary_of_many_groups(n):
     S.within(r.top_logprobs, want, S.stat(v) + 256 * S.U, "top_logprobs")
 
 
+@pytest.mark.parametrize(("n", "d", "v", "top", "head", "dtype"), [
+    (1400, 64, 50001, 20, "dense", "bf16"), (1400, 72, 50001, 3, "dense", "bf16"), (800, 64, 100003, 128, "q4", "bf16"),
+    (17000, 64, 4100, 5, "dense", "bf16"), (1400, 64, 50001, 8, "dense", "fp32"), (1400, 33, 50001, 2, "dense", "fp32"),
+    (800, 64, 100003, 16, "q4", "fp32"), (300, 64, 2048 * 128 + 77, 4, "dense", "bf16")])
+def test_logits_that_are_not_kept(n, d, v, top, head, dtype):
+    """More logits than a forward writes down: the alternatives' groups are formed again."""
+    hidden, hd, w = S.make(n, d, v, head=head, dtype=dtype, seed=3)
+    y = _targets(n, v, 3)
+    h = hidden.clone()
+    h[y == -100] = math.nan
+    got = token_logprobs(h.cuda(), S.to(hd, "cuda"), y.cuda(), top=top, temperature=0.9)
+    live = (y != -100).cuda()
+    at = 0
+    for rows in live.nonzero()[:, 0].split(400):
+        z = hidden[rows.cpu()].double().cuda() @ w.T.cuda()
+        value, ids = torch.sort(z, dim=1, descending=True, stable=True)
+        assert torch.equal(got.top_ids[rows], ids[:, :top])
+        logp = torch.log_softmax(z / 0.9, 1)
+        off = S.stat(v) + 256 * S.U
+        S.within(got.top_logprobs[rows], logp.gather(1, ids[:, :top]).cpu(), off, "top_logprobs")
+        S.within(got.logprobs[rows], logp.gather(1, y.cuda()[rows][:, None])[:, 0].cpu(), off, "logprobs")
+        S.within(got.entropy[rows], -(logp.exp() * logp).sum(1).cpu(), off + 128 * S.stat(v), "entropy")
+        at += rows.numel()
+    assert at == int(live.sum()) and bool((got.top_ids[~live] == -1).all()) and bool((got.top_logprobs[~live] == -math.inf).all())
+
+
+def test_equal_logits_that_are_not_kept():
+    _, hd, _ = S.make(1, 64, 50000)
+    r = token_logprobs(torch.zeros(1400, 64, dtype=torch.bfloat16, device="cuda"), S.to(hd, "cuda"), top=70)
+    assert torch.equal(r.top_ids.cpu(), torch.arange(70).expand(1400, 70))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("n", [1, 3, 140])
+def test_the_smallest_head(n, dtype):
+    """One word: certain, no entropy, nothing to learn."""
+    hidden, hd, _ = S.make(n, 8, 1, head="trainable", dtype=dtype)
+    hd = S.to(hd, "cuda")
+    h = hidden.cuda().requires_grad_(True)
+    r = token_logprobs(h, hd, torch.zeros(n, dtype=torch.int64, device="cuda"), top=1)
+    assert bool((r.top_ids == 0).all()) and float(r.logprobs.detach().abs().max()) <= 64 * S.U and float(r.entropy.detach().abs().max()) <= 64 * S.U
+    loss = distillation_loss(h, hd, torch.zeros(n, 1, dtype=torch.int64, device="cuda"), torch.zeros(n, 1, device="cuda"), renormalize=True)
+    for g in torch.autograd.grad(r.logprobs.sum() + r.entropy.sum() + loss, (h, hd.weight)):
+        assert float(g.abs().max()) <= 1e-4
+
+
+@pytest.mark.parametrize("n", [2, 140])
+def test_logits_that_are_no_numbers(n):
+    """Rows of NaN and of infinities among others: theirs is what comes of them, the others' is as without."""
+    hidden, hd, _ = S.make(n, 64, 1000, seed=5)
+    hd = S.to(hd, "cuda")
+    h = hidden.cuda()
+    want = token_logprobs(h, hd, top=7)
+    bad = h.clone()
+    bad[0] = math.nan
+    bad[-1, 0] = math.inf
+    got = token_logprobs(bad, hd, top=7)
+    assert bool(torch.isnan(got.entropy[0]))
+    for a, b in zip(got[1:], want[1:]):
+        assert torch.equal(a[1:-1], b[1:-1])
+
+
+@pytest.mark.parametrize("n", [3, 140])
+@pytest.mark.parametrize("temperature", [1e-3, 1e3])
+def test_extreme_temperatures(n, temperature):
+    """All on the likeliest, or near to evenly spread."""
+    hidden, hd, w = S.make(n, 64, 500, seed=5)
+    r = token_logprobs(hidden.cuda(), S.to(hd, "cuda"), top=1, temperature=temperature)
+    z = S.logits(hidden, w, torch.ones(n, dtype=torch.bool)).detach() / temperature
+    p = torch.softmax(z, 1)
+    want = -torch.special.xlogy(p, p).sum(1)
+    size = 2 * float(z.abs().max()) + 1   # x is rounded at its own size, not below 64
+    assert float((r.entropy.double().cpu() - want).abs().max()) <= (S.stat(500) + 256 * S.U) * size * 8
+
+
+def test_in_inference_mode():
+    hidden, hd, _ = S.make(9, 64, 300)
+    h, hd = hidden.cuda(), S.to(hd, "cuda")
+    want = token_logprobs(h, hd, top=3)
+    ids, lp, _ = (x.cuda() for x in S.teacher_list(9, 300, 4, holes=False))
+    loss = distillation_loss(h, hd, ids, lp)
+    with torch.inference_mode():
+        got = token_logprobs(h, hd, top=3)
+        again = distillation_loss(h, hd, ids, lp)
+    assert all(torch.equal(a, b) for a, b in zip(got[1:], want[1:])) and torch.equal(again, loss)
+
+
 def test_more_tokens_than_a_pass_takes():
     """Blocks of 16384 tokens: every one as if it were alone."""
-    n, d, v = 16384 + 300, 64, 300
+    n, d, v = 16384 + 300, 64, 4100
     hidden, hd, _ = S.make(n, d, v, seed=4)
     hd = S.to(hd, "cuda")
     y = _targets(n, v, 4).cuda()

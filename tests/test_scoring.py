@@ -194,11 +194,15 @@ def test_workspaces():
     from mlx_train_perf import _native as N
 
     lib = N.load()
-    for n in (1, 128, 129, 4096, 16384, 16385, 100000):
+    for n in (1, 128, 129, 2048, 4096, 16384, 16385, 100000):
         for top in (0, 1, 128):
             ws = lib.mtp_logprobs_fwd_workspace_bytes(n, 512, 32000, 0, top)
-            rows = min(n, 16384)
-            assert 0 < ws <= rows * (32128 * 4 + 3 * 251 * 4 if n <= 128 else top * 128 * 4 + 251 * 4 + 16 * top) + (8 << 20)
+            rows, partials = min(n, 16384), 8 << 20
+            if n <= 128 or (top and n * 32000 * 4 <= 256 << 20):   # the logits, and each group's maximum (and sums)
+                most = n * (32128 * 4 + 3 * 252 * 4)
+            else:   # the groups that a row's alternatives are looked for in
+                most = rows * top * (128 * 4 + 16) + rows * (252 + 1) * 4
+            assert 0 < ws <= most + partials
     assert lib.mtp_logprobs_fwd_workspace_bytes(0, 64, 100, 0, 1) == 0
     assert lib.mtp_logprobs_fwd_workspace_bytes(8, 64, 2 ** 21 + 1, 0, 1) == 0
     # a staged 4-bit head adds its rows, a few tokens none
