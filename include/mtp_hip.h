@@ -398,8 +398,11 @@ int mtp_policy_bwd(const float* d_loss, const float* nll, const float* old_nll, 
  * ------------------------------------------------------------------------------------------- */
 #define MTP_SCORE_MAX 128 /* most alternatives, and longest teacher's list */
 
-size_t mtp_logprobs_fwd_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t top);
-size_t mtp_logprobs_fwd_f32_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t top);
+/* keep, in the forwards' sizes: whether the forward gets `logits`, fp32 [n][mtp_score_logits_ld(v)], in which it keeps them for
+ * its backward, which then forms none again (NULL in both: it does). */
+int64_t mtp_score_logits_ld(int64_t v);
+size_t mtp_logprobs_fwd_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t top, int32_t keep);
+size_t mtp_logprobs_fwd_f32_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t top, int32_t keep);
 
 /* Per token: logprobs = x_y - lse of the target y (targets NULL: no targets, and logprobs and tgt may be NULL; a target outside
  * [0, v) counts as a logit of 0, as in mtp_lce_fwd), entropy = lse - sum p x, and the `top` largest logits (0 to
@@ -409,11 +412,12 @@ size_t mtp_logprobs_fwd_f32_workspace_bytes(int64_t n, int64_t d, int64_t v, int
 int mtp_logprobs_fwd(const void* hidden, const void* w, const uint32_t* w_q, const void* scales, const void* biases,
                      const int64_t* targets, int64_t n, int64_t d, int64_t v, int32_t head_kind, int64_t ignore_index,
                      int32_t top, double temperature, float* logprobs, float* entropy, float* top_logprobs,
-                     int64_t* top_ids, float* lse, float* tgt, void* workspace, size_t workspace_bytes, void* stream);
+                     int64_t* top_ids, float* lse, float* tgt, float* logits, void* workspace, size_t workspace_bytes,
+                     void* stream);
 int mtp_logprobs_fwd_f32(const float* hidden, const float* w, const uint32_t* w_q, const float* scales, const float* biases,
                          const int64_t* targets, int64_t n, int64_t d, int64_t v, int32_t head_kind,
                          int64_t ignore_index, int32_t top, double temperature, float* logprobs, float* entropy,
-                         float* top_logprobs, int64_t* top_ids, float* lse, float* tgt, void* workspace,
+                         float* top_logprobs, int64_t* top_ids, float* lse, float* tgt, float* logits, void* workspace,
                          size_t workspace_bytes, void* stream);
 
 /* Workspace of the backwards below: mtp_lce_bwd's, then the factors of the gradient (k columns a row: 1 for scoring, the list's
@@ -427,12 +431,14 @@ size_t mtp_score_bwd_f32_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_
 int mtp_logprobs_bwd(const void* hidden, const void* w, const void* w_t, const uint32_t* w_q, const void* scales,
                      const void* biases, const int64_t* targets, int64_t n, int64_t d, int64_t v, int32_t head_kind,
                      int64_t ignore_index, double temperature, const float* lse, const float* entropy,
-                     const float* tgt, const float* d_logprobs, const float* d_entropy, void* d_hidden, void* d_w,
+                     const float* tgt, const float* logits, const float* d_logprobs, const float* d_entropy,
+                     void* d_hidden, void* d_w,
                      int64_t chunk, int64_t row_block, void* workspace, size_t workspace_bytes, void* stream);
 int mtp_logprobs_bwd_f32(const float* hidden, const float* w, const uint32_t* w_q, const float* scales, const float* biases,
                          const int64_t* targets, int64_t n, int64_t d, int64_t v, int32_t head_kind,
                          int64_t ignore_index, double temperature, const float* lse, const float* entropy,
-                         const float* tgt, const float* d_logprobs, const float* d_entropy, float* d_hidden, float* d_w,
+                         const float* tgt, const float* logits, const float* d_logprobs, const float* d_entropy,
+                         float* d_hidden, float* d_w,
                          int64_t chunk, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Divergence of a teacher's list from p, per token: ids int64 [n][k], 1 <= k <= MTP_SCORE_MAX, and the log probabilities
@@ -446,28 +452,30 @@ int mtp_logprobs_bwd_f32(const float* hidden, const float* w, const uint32_t* w_
 #define MTP_DISTILL_REVERSE 1
 #define MTP_DISTILL_JSD 2
 
-size_t mtp_distill_fwd_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t k);
-size_t mtp_distill_fwd_f32_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t k);
+size_t mtp_distill_fwd_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t k, int32_t keep);
+size_t mtp_distill_fwd_f32_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t k, int32_t keep);
 int mtp_distill_fwd(const void* hidden, const void* w, const uint32_t* w_q, const void* scales, const void* biases,
                     const int64_t* ids, const float* teacher, const uint8_t* mask, int64_t n, int64_t d, int64_t v,
                     int32_t head_kind, int32_t k, int32_t kind, double beta, double temperature, int32_t renormalize,
                     int32_t reduction, float* loss, float* scale, float* lse, float* rest, float* coef,
-                    int32_t* columns, void* workspace, size_t workspace_bytes, void* stream);
+                    int32_t* columns, float* logits, void* workspace, size_t workspace_bytes, void* stream);
 int mtp_distill_fwd_f32(const float* hidden, const float* w, const uint32_t* w_q, const float* scales, const float* biases,
                         const int64_t* ids, const float* teacher, const uint8_t* mask, int64_t n, int64_t d, int64_t v,
                         int32_t head_kind, int32_t k, int32_t kind, double beta, double temperature,
                         int32_t renormalize, int32_t reduction, float* loss, float* scale, float* lse, float* rest,
-                        float* coef, int32_t* columns, void* workspace, size_t workspace_bytes, void* stream);
+                        float* coef, int32_t* columns, float* logits, void* workspace, size_t workspace_bytes,
+                        void* stream);
 /* From d_loss [n] (none) or [1] and what the forward left. */
 int mtp_distill_bwd(const void* hidden, const void* w, const void* w_t, const uint32_t* w_q, const void* scales,
                     const void* biases, int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t k, double temperature,
                     int32_t reduction, const float* d_loss, const float* scale, const float* lse, const float* rest,
-                    const float* coef, const int32_t* columns, void* d_hidden, void* d_w, int64_t chunk,
-                    int64_t row_block, void* workspace, size_t workspace_bytes, void* stream);
+                    const float* coef, const int32_t* columns, const float* logits, void* d_hidden, void* d_w,
+                    int64_t chunk, int64_t row_block, void* workspace, size_t workspace_bytes, void* stream);
 int mtp_distill_bwd_f32(const float* hidden, const float* w, const uint32_t* w_q, const float* scales, const float* biases,
                         int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t k, double temperature,
                         int32_t reduction, const float* d_loss, const float* scale, const float* lse, const float* rest,
-                        const float* coef, const int32_t* columns, float* d_hidden, float* d_w, int64_t chunk,
+                        const float* coef, const int32_t* columns, const float* logits, float* d_hidden, float* d_w,
+                        int64_t chunk,
                         void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

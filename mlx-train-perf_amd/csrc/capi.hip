@@ -854,15 +854,17 @@ static bool score_sizes(int64_t n, int64_t d, int64_t v) {
   return n >= 1 && d >= 1 && v >= 1 && n <= kMaxDim && d <= kMaxDim && v <= mtp::kScoreVocab;
 }
 
-static size_t logprobs_fwd_ws(int f32, int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t top) {
+int64_t mtp_score_logits_ld(int64_t v) { return v < 1 ? 0 : (int64_t)mtp::logits_ld((long)v); }
+
+static size_t logprobs_fwd_ws(int f32, int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t top, int keep) {
   if (!score_sizes(n, d, v) || top < 0 || top > MTP_SCORE_MAX) return 0;
-  return mtp::logprobs_fwd_workspace(score_shape(n, d, v, 1.0, head_kind), f32, q4_kind(head_kind), top);
+  return mtp::logprobs_fwd_workspace(score_shape(n, d, v, 1.0, head_kind), f32, q4_kind(head_kind), top, keep != 0);
 }
-size_t mtp_logprobs_fwd_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t top) {
-  return logprobs_fwd_ws(0, n, d, v, head_kind, top);
+size_t mtp_logprobs_fwd_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t top, int32_t keep) {
+  return logprobs_fwd_ws(0, n, d, v, head_kind, top, keep);
 }
-size_t mtp_logprobs_fwd_f32_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t top) {
-  return logprobs_fwd_ws(1, n, d, v, head_kind, top);
+size_t mtp_logprobs_fwd_f32_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t top, int32_t keep) {
+  return logprobs_fwd_ws(1, n, d, v, head_kind, top, keep);
 }
 
 static int logprobs_fwd(int f32, const void* hidden, const void* w, const uint32_t* w_q, const void* scales, const void* biases,
@@ -877,7 +879,8 @@ static int logprobs_fwd(int f32, const void* hidden, const void* w, const uint32
   if (top > MTP_SCORE_MAX) return fail(MTP_ERR_UNSUPPORTED, "at most %d alternatives (got top=%d); use impl='reference'", MTP_SCORE_MAX, (int)top);
   if (!out.entropy || !out.lse || (targets && (!out.logprobs || !out.tgt)) || (top && (!out.top_logprobs || !out.top_ids)))
     return fail(MTP_ERR_INPUT, "entropy and lse, with targets logprobs and tgt, with top top_logprobs and top_ids must be non-null");
-  const size_t need = logprobs_fwd_ws(f32, n, d, v, head_kind, top);
+  if (!aligned16(out.logits)) return fail(MTP_ERR_UNSUPPORTED, "logits must be 16-byte aligned");
+  const size_t need = logprobs_fwd_ws(f32, n, d, v, head_kind, top, out.logits != nullptr);
   if (!workspace || workspace_bytes < need)
     return fail(MTP_ERR_WORKSPACE, "token scoring needs a workspace of %zu bytes (got %zu)", need, workspace ? workspace_bytes : (size_t)0);
   if (!aligned16(workspace)) return fail(MTP_ERR_UNSUPPORTED, "workspace must be 16-byte aligned");
@@ -891,16 +894,18 @@ static int logprobs_fwd(int f32, const void* hidden, const void* w, const uint32
 int mtp_logprobs_fwd(const void* hidden, const void* w, const uint32_t* w_q, const void* scales, const void* biases,
                      const int64_t* targets, int64_t n, int64_t d, int64_t v, int32_t head_kind, int64_t ignore_index,
                      int32_t top, double temperature, float* logprobs, float* entropy, float* top_logprobs,
-                     int64_t* top_ids, float* lse, float* tgt, void* workspace, size_t workspace_bytes, void* stream) {
+                     int64_t* top_ids, float* lse, float* tgt, float* logits, void* workspace, size_t workspace_bytes,
+                     void* stream) {
   return logprobs_fwd(0, hidden, w, w_q, scales, biases, targets, n, d, v, head_kind, ignore_index, top, temperature,
-                      mtp::LogprobsOut{logprobs, entropy, top_logprobs, top_ids, lse, tgt}, workspace, workspace_bytes, stream);
+                      mtp::LogprobsOut{logprobs, entropy, top_logprobs, top_ids, lse, tgt, logits}, workspace, workspace_bytes, stream);
 }
 int mtp_logprobs_fwd_f32(const float* hidden, const float* w, const uint32_t* w_q, const float* scales, const float* biases,
                          const int64_t* targets, int64_t n, int64_t d, int64_t v, int32_t head_kind, int64_t ignore_index,
                          int32_t top, double temperature, float* logprobs, float* entropy, float* top_logprobs,
-                         int64_t* top_ids, float* lse, float* tgt, void* workspace, size_t workspace_bytes, void* stream) {
+                         int64_t* top_ids, float* lse, float* tgt, float* logits, void* workspace, size_t workspace_bytes,
+                     void* stream) {
   return logprobs_fwd(1, hidden, w, w_q, scales, biases, targets, n, d, v, head_kind, ignore_index, top, temperature,
-                      mtp::LogprobsOut{logprobs, entropy, top_logprobs, top_ids, lse, tgt}, workspace, workspace_bytes, stream);
+                      mtp::LogprobsOut{logprobs, entropy, top_logprobs, top_ids, lse, tgt, logits}, workspace, workspace_bytes, stream);
 }
 
 // After the loss's workspace: alpha [n], beta [n], the columns [n] of scoring, the values [n][k], the cleared hidden states, or
@@ -936,15 +941,15 @@ size_t mtp_score_bwd_f32_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_
 template <class FACTORS>
 static int score_bwd(int f32, const void* hidden, const void* w, const void* w_t, const uint32_t* w_q, const void* scales,
                      const void* biases, int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t k, double temperature,
-                     const float* lse, const int32_t* columns, void* d_hidden, void* d_w, int64_t chunk, int64_t row_block,
-                     void* workspace, size_t workspace_bytes, hipStream_t stream, const FACTORS& factors) {
+                     const float* lse, const int32_t* columns, const float* logits, void* d_hidden, void* d_w, int64_t chunk,
+                     int64_t row_block, void* workspace, size_t workspace_bytes, hipStream_t stream, const FACTORS& factors) {
   int rc = check_score_head(f32, hidden, w, w_q, scales, biases, n, d, v, head_kind);
   if (rc) return rc;
   rc = check_score(n, d, v, temperature);
   if (rc) return rc;
   if (!lse || !d_hidden) return fail(MTP_ERR_INPUT, "lse and d_hidden must be non-null");
-  if (!aligned16(d_hidden) || (d_w && !aligned16(d_w)) || (w_t && !aligned16(w_t)))
-    return fail(MTP_ERR_UNSUPPORTED, "d_hidden, d_w and w_t must be 16-byte aligned");
+  if (!aligned16(d_hidden) || !aligned16(d_w) || !aligned16(w_t) || !aligned16(logits))
+    return fail(MTP_ERR_UNSUPPORTED, "d_hidden, d_w, w_t and logits must be 16-byte aligned");
   if (d_w && q4_kind(head_kind)) return fail(MTP_ERR_UNSUPPORTED, "a quantized head is frozen: d_w must be null");
   if (w_t && (f32 || staged_kind(head_kind))) return fail(MTP_ERR_INPUT, "fp32 and the staged head kinds take no w_t");
   const int64_t tile = f32 ? 128 : kTile;
@@ -970,7 +975,7 @@ static int score_bwd(int f32, const void* hidden, const void* w, const void* w_t
     e = mtp::launch_clean_rows(hidden, alpha, has_beta ? beta : nullptr, (long)n, (long)d * (f32 ? 4 : 2), ws + parts.clean, stream);
   if (e == hipSuccess) {
     const float inv_t = (float)(1.0 / temperature);
-    const mtp::AffineGrad grad{{alpha, has_beta ? beta : nullptr, 1.4426950408889634f * inv_t}, columns ? columns : own_columns, value, (int)k, ws + parts.clean};
+    const mtp::AffineGrad grad{{alpha, has_beta ? beta : nullptr, 1.4426950408889634f * inv_t}, columns ? columns : own_columns, value, (int)k, logits, mtp::logits_ld((long)v), ws + parts.clean};
     if (f32) {
       mtp::LceHead32 head = score_head(1, hidden, w, w_q, scales, biases, head_kind).h32;
       if (head_kind == MTP_HEAD_Q4_STAGED) {
@@ -1001,12 +1006,12 @@ extern "C" {
 static int logprobs_bwd(int f32, const void* hidden, const void* w, const void* w_t, const uint32_t* w_q, const void* scales,
                         const void* biases, const int64_t* targets, int64_t n, int64_t d, int64_t v, int32_t head_kind,
                         int64_t ignore_index, double temperature, const float* lse, const float* entropy, const float* tgt,
-                        const float* d_logprobs, const float* d_entropy, void* d_hidden, void* d_w, int64_t chunk,
+                        const float* logits, const float* d_logprobs, const float* d_entropy, void* d_hidden, void* d_w, int64_t chunk,
                         int64_t row_block, void* workspace, size_t workspace_bytes, void* stream) {
   if (!entropy || (targets && !tgt)) return fail(MTP_ERR_INPUT, "entropy, and with targets tgt, must be non-null");
   if (d_logprobs && !targets) return fail(MTP_ERR_INPUT, "d_logprobs needs targets");
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  return score_bwd(f32, hidden, w, w_t, w_q, scales, biases, n, d, v, head_kind, 1, temperature, lse, nullptr, d_hidden, d_w, chunk,
+  return score_bwd(f32, hidden, w, w_t, w_q, scales, biases, n, d, v, head_kind, 1, temperature, lse, nullptr, logits, d_hidden, d_w, chunk,
                    row_block, workspace, workspace_bytes, st, [&](float* alpha, float* beta, int* columns, float* value, bool* has_beta) {
                      *has_beta = d_entropy != nullptr;
                      return mtp::launch_logprobs_coef(d_logprobs, d_entropy, targets, (long long)ignore_index, lse, entropy, tgt,
@@ -1016,29 +1021,29 @@ static int logprobs_bwd(int f32, const void* hidden, const void* w, const void* 
 int mtp_logprobs_bwd(const void* hidden, const void* w, const void* w_t, const uint32_t* w_q, const void* scales,
                      const void* biases, const int64_t* targets, int64_t n, int64_t d, int64_t v, int32_t head_kind,
                      int64_t ignore_index, double temperature, const float* lse, const float* entropy, const float* tgt,
-                     const float* d_logprobs, const float* d_entropy, void* d_hidden, void* d_w, int64_t chunk,
+                     const float* logits, const float* d_logprobs, const float* d_entropy, void* d_hidden, void* d_w, int64_t chunk,
                      int64_t row_block, void* workspace, size_t workspace_bytes, void* stream) {
   return logprobs_bwd(0, hidden, w, w_t, w_q, scales, biases, targets, n, d, v, head_kind, ignore_index, temperature, lse, entropy,
-                      tgt, d_logprobs, d_entropy, d_hidden, d_w, chunk, row_block, workspace, workspace_bytes, stream);
+                      tgt, logits, d_logprobs, d_entropy, d_hidden, d_w, chunk, row_block, workspace, workspace_bytes, stream);
 }
 int mtp_logprobs_bwd_f32(const float* hidden, const float* w, const uint32_t* w_q, const float* scales, const float* biases,
                          const int64_t* targets, int64_t n, int64_t d, int64_t v, int32_t head_kind, int64_t ignore_index,
-                         double temperature, const float* lse, const float* entropy, const float* tgt, const float* d_logprobs,
-                         const float* d_entropy, float* d_hidden, float* d_w, int64_t chunk, void* workspace,
+                         double temperature, const float* lse, const float* entropy, const float* tgt, const float* logits,
+                         const float* d_logprobs, const float* d_entropy, float* d_hidden, float* d_w, int64_t chunk, void* workspace,
                          size_t workspace_bytes, void* stream) {
   return logprobs_bwd(1, hidden, w, nullptr, w_q, scales, biases, targets, n, d, v, head_kind, ignore_index, temperature, lse, entropy,
-                      tgt, d_logprobs, d_entropy, d_hidden, d_w, chunk, 0, workspace, workspace_bytes, stream);
+                      tgt, logits, d_logprobs, d_entropy, d_hidden, d_w, chunk, 0, workspace, workspace_bytes, stream);
 }
 
-static size_t distill_fwd_ws(int f32, int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t k) {
+static size_t distill_fwd_ws(int f32, int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t k, int keep) {
   if (!score_sizes(n, d, v) || k < 1 || k > MTP_SCORE_MAX) return 0;
-  return mtp::distill_fwd_workspace(score_shape(n, d, v, 1.0, head_kind), f32, q4_kind(head_kind), k);
+  return mtp::distill_fwd_workspace(score_shape(n, d, v, 1.0, head_kind), f32, q4_kind(head_kind), k, keep != 0);
 }
-size_t mtp_distill_fwd_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t k) {
-  return distill_fwd_ws(0, n, d, v, head_kind, k);
+size_t mtp_distill_fwd_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t k, int32_t keep) {
+  return distill_fwd_ws(0, n, d, v, head_kind, k, keep);
 }
-size_t mtp_distill_fwd_f32_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t k) {
-  return distill_fwd_ws(1, n, d, v, head_kind, k);
+size_t mtp_distill_fwd_f32_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t k, int32_t keep) {
+  return distill_fwd_ws(1, n, d, v, head_kind, k, keep);
 }
 
 static int check_reduction(int32_t reduction) {
@@ -1060,7 +1065,8 @@ static int distill_fwd(int f32, const void* hidden, const void* w, const uint32_
   if (!ids || !teacher) return fail(MTP_ERR_INPUT, "ids and teacher must be non-null");
   if (!out.loss || !out.lse || !out.rest || !out.coef || !out.columns || (reduction != MTP_REDUCE_NONE && !out.scale))
     return fail(MTP_ERR_INPUT, "loss, scale, lse, rest, coef and columns must be non-null");
-  const size_t need = distill_fwd_ws(f32, n, d, v, head_kind, k);
+  if (!aligned16(out.logits)) return fail(MTP_ERR_UNSUPPORTED, "logits must be 16-byte aligned");
+  const size_t need = distill_fwd_ws(f32, n, d, v, head_kind, k, out.logits != nullptr);
   if (!workspace || workspace_bytes < need)
     return fail(MTP_ERR_WORKSPACE, "distillation needs a workspace of %zu bytes (got %zu)", need, workspace ? workspace_bytes : (size_t)0);
   if (!aligned16(workspace)) return fail(MTP_ERR_UNSUPPORTED, "workspace must be 16-byte aligned");
@@ -1075,30 +1081,30 @@ int mtp_distill_fwd(const void* hidden, const void* w, const uint32_t* w_q, cons
                     const int64_t* ids, const float* teacher, const uint8_t* mask, int64_t n, int64_t d, int64_t v,
                     int32_t head_kind, int32_t k, int32_t kind, double beta, double temperature, int32_t renormalize,
                     int32_t reduction, float* loss, float* scale, float* lse, float* rest, float* coef, int32_t* columns,
-                    void* workspace, size_t workspace_bytes, void* stream) {
+                    float* logits, void* workspace, size_t workspace_bytes, void* stream) {
   return distill_fwd(0, hidden, w, w_q, scales, biases, ids, teacher, mask, n, d, v, head_kind, k, kind, beta, temperature, renormalize,
-                     reduction, mtp::DistillOut{loss, scale, lse, rest, coef, columns}, workspace, workspace_bytes, stream);
+                     reduction, mtp::DistillOut{loss, scale, lse, rest, coef, columns, logits}, workspace, workspace_bytes, stream);
 }
 int mtp_distill_fwd_f32(const float* hidden, const float* w, const uint32_t* w_q, const float* scales, const float* biases,
                         const int64_t* ids, const float* teacher, const uint8_t* mask, int64_t n, int64_t d, int64_t v,
                         int32_t head_kind, int32_t k, int32_t kind, double beta, double temperature, int32_t renormalize,
                         int32_t reduction, float* loss, float* scale, float* lse, float* rest, float* coef, int32_t* columns,
-                        void* workspace, size_t workspace_bytes, void* stream) {
+                        float* logits, void* workspace, size_t workspace_bytes, void* stream) {
   return distill_fwd(1, hidden, w, w_q, scales, biases, ids, teacher, mask, n, d, v, head_kind, k, kind, beta, temperature, renormalize,
-                     reduction, mtp::DistillOut{loss, scale, lse, rest, coef, columns}, workspace, workspace_bytes, stream);
+                     reduction, mtp::DistillOut{loss, scale, lse, rest, coef, columns, logits}, workspace, workspace_bytes, stream);
 }
 
 static int distill_bwd(int f32, const void* hidden, const void* w, const void* w_t, const uint32_t* w_q, const void* scales,
                        const void* biases, int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t k, double temperature,
                        int32_t reduction, const float* d_loss, const float* scale, const float* lse, const float* rest,
-                       const float* coef, const int32_t* columns, void* d_hidden, void* d_w, int64_t chunk, int64_t row_block,
-                       void* workspace, size_t workspace_bytes, void* stream) {
+                       const float* coef, const int32_t* columns, const float* logits, void* d_hidden, void* d_w, int64_t chunk,
+                       int64_t row_block, void* workspace, size_t workspace_bytes, void* stream) {
   int rc;
   if ((rc = check_list(k)) || (rc = check_reduction(reduction))) return rc;
   if (!d_loss || !rest || !coef || !columns || (reduction != MTP_REDUCE_NONE && !scale))
     return fail(MTP_ERR_INPUT, "d_loss, scale, rest, coef and columns must be non-null");
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  return score_bwd(f32, hidden, w, w_t, w_q, scales, biases, n, d, v, head_kind, k, temperature, lse, columns, d_hidden, d_w, chunk,
+  return score_bwd(f32, hidden, w, w_t, w_q, scales, biases, n, d, v, head_kind, k, temperature, lse, columns, logits, d_hidden, d_w, chunk,
                    row_block, workspace, workspace_bytes, st, [&](float* alpha, float*, int*, float* value, bool*) {
                      return mtp::launch_distill_coef(d_loss, reduction == MTP_REDUCE_NONE, scale, rest, coef, (long)n, (int)k, alpha, value, st);
                    });
@@ -1106,18 +1112,18 @@ static int distill_bwd(int f32, const void* hidden, const void* w, const void* w
 int mtp_distill_bwd(const void* hidden, const void* w, const void* w_t, const uint32_t* w_q, const void* scales,
                     const void* biases, int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t k, double temperature,
                     int32_t reduction, const float* d_loss, const float* scale, const float* lse, const float* rest,
-                    const float* coef, const int32_t* columns, void* d_hidden, void* d_w, int64_t chunk, int64_t row_block,
-                    void* workspace, size_t workspace_bytes, void* stream) {
+                    const float* coef, const int32_t* columns, const float* logits, void* d_hidden, void* d_w, int64_t chunk,
+                    int64_t row_block, void* workspace, size_t workspace_bytes, void* stream) {
   return distill_bwd(0, hidden, w, w_t, w_q, scales, biases, n, d, v, head_kind, k, temperature, reduction, d_loss, scale, lse, rest, coef,
-                     columns, d_hidden, d_w, chunk, row_block, workspace, workspace_bytes, stream);
+                     columns, logits, d_hidden, d_w, chunk, row_block, workspace, workspace_bytes, stream);
 }
 int mtp_distill_bwd_f32(const float* hidden, const float* w, const uint32_t* w_q, const float* scales, const float* biases,
                         int64_t n, int64_t d, int64_t v, int32_t head_kind, int32_t k, double temperature, int32_t reduction,
                         const float* d_loss, const float* scale, const float* lse, const float* rest, const float* coef,
-                        const int32_t* columns, float* d_hidden, float* d_w, int64_t chunk, void* workspace,
+                        const int32_t* columns, const float* logits, float* d_hidden, float* d_w, int64_t chunk, void* workspace,
                         size_t workspace_bytes, void* stream) {
   return distill_bwd(1, hidden, w, nullptr, w_q, scales, biases, n, d, v, head_kind, k, temperature, reduction, d_loss, scale, lse, rest,
-                     coef, columns, d_hidden, d_w, chunk, 0, workspace, workspace_bytes, stream);
+                     coef, columns, logits, d_hidden, d_w, chunk, 0, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -794,7 +794,8 @@ static hipError_t lce32_fwd_tiles(const LceHead32& h, const float* H, int N, int
 
 hipError_t launch_lce32_stats(const LceHead32& h, const float* H, int N, int D, int V, const ScoreStats& x, hipStream_t st) {
   constexpr int kEntropy = kStatScaled | kStatEntropy, kGroups = kEntropy | kStatGroups;
-  if (x.z) return lce32_fwd_tiles<kGroups | kStatKeep>(h, H, N, D, V, x, st);
+  if (x.z && x.gmax) return lce32_fwd_tiles<kGroups | kStatKeep>(h, H, N, D, V, x, st);
+  if (x.z) return lce32_fwd_tiles<kEntropy | kStatKeep>(h, H, N, D, V, x, st);
   if (x.gmax) return lce32_fwd_tiles<kGroups>(h, H, N, D, V, x, st);
   if (x.u) return lce32_fwd_tiles<kEntropy>(h, H, N, D, V, x, st);
   return lce32_fwd_tiles<kStatScaled | kStatList>(h, H, N, D, V, x, st);
@@ -859,8 +860,13 @@ hipError_t launch_lce32_bwd(const LceHead32& h, const float* H, const int64_t* t
     dim3 ggrid((N + kT - 1) / kT, (kc + kT - 1) / kT);
     auto gradient = affine ? (h.q4 ? lce32_bwd_g_kernel<kQ4, 1> : copied ? lce32_bwd_g_kernel<kCopied, 1> : lce32_bwd_g_kernel<kDense, 1>)
                            : (h.q4 ? lce32_bwd_g_kernel<kQ4> : copied ? lce32_bwd_g_kernel<kCopied> : lce32_bwd_g_kernel<kDense>);
-    hipLaunchKernelGGL(gradient, ggrid, block, 0, st, H, h.w, h.wq, h.sc, h.bi, targets, lse, dnll, D, V, ignore_index, 0, N,
-                       c0, kc, Gbuf, ldg, affine ? affine->rows : AffineRows{});
+    if (affine && affine->z) {
+      const hipError_t ke = launch_affine_tiles(*affine, lse, N, c0, c0 + kc, (kc + 3) & ~3, ldg, Gbuf, st);
+      if (ke != hipSuccess) return ke;
+    } else {
+      hipLaunchKernelGGL(gradient, ggrid, block, 0, st, H, h.w, h.wq, h.sc, h.bi, targets, lse, dnll, D, V, ignore_index, 0, N,
+                         c0, kc, Gbuf, ldg, affine ? affine->rows : AffineRows{});
+    }
     if (affine)
       hipLaunchKernelGGL(lce32_bwd_g_columns_kernel, dim3((N + 3) / 4), block, 0, st, affine->columns, affine->value, affine->k,
                          N, c0, kc, Gbuf, ldg);

@@ -2222,7 +2222,8 @@ static hipError_t lce_fwd_tiles(const LceHead& h, const bf16_t* H, int N, int D,
 hipError_t launch_lce_stats(const LceHead& h, const bf16_t* H, int N, int D, int V, const ScoreStats& x, bf16_t* stage,
                             long stage_rows, hipStream_t stream) {
   constexpr int kEntropy = kStatScaled | kStatEntropy, kGroups = kEntropy | kStatGroups;
-  if (x.z) return lce_fwd_tiles<kGroups | kStatKeep>(h, H, N, D, V, x, stage, stage_rows, stream);
+  if (x.z && x.gmax) return lce_fwd_tiles<kGroups | kStatKeep>(h, H, N, D, V, x, stage, stage_rows, stream);
+  if (x.z) return lce_fwd_tiles<kEntropy | kStatKeep>(h, H, N, D, V, x, stage, stage_rows, stream);
   if (x.gmax) return lce_fwd_tiles<kGroups>(h, H, N, D, V, x, stage, stage_rows, stream);
   if (x.u) return lce_fwd_tiles<kEntropy>(h, H, N, D, V, x, stage, stage_rows, stream);
   return lce_fwd_tiles<kStatScaled | kStatList>(h, H, N, D, V, x, stage, stage_rows, stream);
@@ -2316,6 +2317,7 @@ static hipError_t lce_bwd_rows(const LceHead& h, const bf16_t* H, const int64_t*
   const int ldg = chunk + kGPitchPad;
   const int ldt = (int)lce_head_t_ld(V);
   dim3 block(kThreads);
+  const bool kept = affine && affine->z;  // the forward's logits: no product for the gradient tiles
   for (int c = 0; c < nchunks; ++c) {
     const int vb = c * chunk;
     const int ve = (vb + chunk < V) ? vb + chunk : V;
@@ -2337,7 +2339,7 @@ static hipError_t lce_bwd_rows(const LceHead& h, const bf16_t* H, const int64_t*
       } else {
         hc.w = h.w + (long)vb * D;
       }
-      bf16_t* rows = h.q4 && kQ4StageRows ? stage + lce_stage_rows_offset(D, chunk) : nullptr;
+      bf16_t* rows = h.q4 && kQ4StageRows && !kept ? stage + lce_stage_rows_offset(D, chunk) : nullptr;
       hipError_t se = launch_lce_head_transpose(hc, ve - vb, D, stage, stream, rows);
       if (se != hipSuccess) return se;
       wt = stage;
@@ -2349,7 +2351,10 @@ static hipError_t lce_bwd_rows(const LceHead& h, const bf16_t* H, const int64_t*
         wrow0 = vb;
       }
     }
-    if (D % kBK == 0) {
+    if (kept) {
+      hipError_t ke = launch_affine_tiles(*affine, lse, N, vb, ve, ctiles * kTile, ldg, Gbuf, stream);
+      if (ke != hipSuccess) return ke;
+    } else if (D % kBK == 0) {
       // One resident workgroup per CU (160 KiB of LDS, all of it, with a dense head; 130 KiB with a 4-bit one).
       const int ns = lce_nsplit(N, (long)ctiles * kTile, 1);
       dim3 pgrid(rtiles * ns);
@@ -2446,6 +2451,7 @@ hipError_t launch_lce_bwd(const LceHead& h, const bf16_t* H, const int64_t* targ
       if (a.rows.beta) a.rows.beta += r0;
       a.columns += (long)r0 * a.k;
       a.value += (long)r0 * a.k;
+      if (a.z) a.z += r0 * a.ldz;
       e = lce_bwd_rows(h, H + (long)r0 * D, nullptr, lse + r0, nullptr, rows, D, V, ignore_index, chunk, dH + (long)r0 * D,
                        nullptr, Gbuf, acc32, parts, stage, &a, stream);
     } else {

@@ -72,7 +72,7 @@ struct ScoreStats {
   float* u;            // the same of 2^(x - m) (x - m), or null
   float* gmax;         // [N][ldg] the maximum z of each group of kGroup (ldg: an even number of them), or null (with u)
   int ldg;
-  float* z;            // [N][ldz] the logits, or null (with gmax); ldz a multiple of kGroup
+  float* z;            // [N][ldz] the logits, or null (with u); ldz a multiple of kGroup
   long ldz;
   ScoreList list;
 };
@@ -92,6 +92,8 @@ struct AffineGrad {
   const int* columns;    // [N][k], no column twice in a row; < 0: none
   const float* value;    // [N][k] the gradient there
   int k;
+  const float* z;        // [N][ldz] the logits that a forward kept, or null: they are formed again
+  long ldz;
   const void* clean;     // for dW: the hidden states with the rows that get zeros cleared (bf16; fp32 in the fp32 backward)
 };
 
@@ -222,12 +224,14 @@ struct ScoreShape {
   float inv_t;       // 1 / temperature
   int stage;         // 4-bit: dequantize the whole head into the workspace first
 };
+// logits, in a forward's outputs: [n][logits_ld(v)], which then keeps them there for its backward, or null.
+inline long logits_ld(long v) { return (v + kGroup - 1) / kGroup * kGroup; }
 struct LogprobsOut {
   float *logprobs, *entropy, *top_logprobs;
   int64_t* top_ids;
-  float *lse, *tgt;
+  float *lse, *tgt, *logits;
 };
-size_t logprobs_fwd_workspace(const ScoreShape& sh, int f32, int q4, int top);
+size_t logprobs_fwd_workspace(const ScoreShape& sh, int f32, int q4, int top, int keep);
 hipError_t launch_logprobs_fwd(const ScoreHead& h, const ScoreShape& sh, const int64_t* targets, long long ignore_index,
                                int top, const LogprobsOut& out, void* ws, hipStream_t stream);
 enum { kDistillForward = 0, kDistillReverse = 1, kDistillJsd = 2 };
@@ -239,14 +243,20 @@ struct DistillOut {
   float *loss, *scale;        // scale [1]: what a row's gradient is multiplied with, 1 / rows that count for a mean
   float *lse, *rest, *coef;   // [n], [n], [n][k]
   int* columns;               // [n][k]
+  float* logits;
 };
-size_t distill_fwd_workspace(const ScoreShape& sh, int f32, int q4, int k);
+size_t distill_fwd_workspace(const ScoreShape& sh, int f32, int q4, int k, int keep);
 hipError_t launch_distill_fwd(const ScoreHead& h, const ScoreShape& sh, const int64_t* ids, const float* teacher,
                               const uint8_t* mask, const DistillLoss& p, const DistillOut& out, void* ws, hipStream_t stream);
 // What the backwards hand to launch_lce_bwd / launch_lce32_bwd: alpha, beta, columns, value (k = 1).
 hipError_t launch_logprobs_coef(const float* d_logprobs, const float* d_entropy, const int64_t* targets, long long ignore_index,
                                 const float* lse, const float* entropy, const float* tgt, long n, long v, float inv_t,
                                 float* alpha, float* beta, int* columns, float* value, hipStream_t stream);
+// Gradient tiles from kept logits, columns [v_begin, v_begin + cols) (zeros from vlim on; cols a multiple of 8, fp32: of 4).
+hipError_t launch_affine_tiles(const AffineGrad& a, const float* lse, long n, int v_begin, int vlim, int cols, long ldg, bf16_t* g,
+                               hipStream_t stream);
+hipError_t launch_affine_tiles(const AffineGrad& a, const float* lse, long n, int v_begin, int vlim, int cols, long ldg, float* g,
+                               hipStream_t stream);
 hipError_t launch_distill_coef(const float* d_loss, int per_row, const float* scale, const float* rest, const float* coef,
                                long n, int k, float* alpha, float* value, hipStream_t stream);
 // Hidden states with the rows whose factors are both 0 cleared; row_bytes a multiple of 4.

@@ -1006,6 +1006,34 @@ __global__ __launch_bounds__(256) void distill_coef_kernel(const float* __restri
   }
 }
 
+// G = p (alpha + beta z) from kept logits, a row a blockIdx.y, 16 bytes a thread; bound by reading z and writing G (AffineGrad's
+// listed columns follow).
+template <class G>
+__global__ __launch_bounds__(256) void affine_tiles_kernel(const float* __restrict__ Z, long ldz, const float* __restrict__ lse,
+                                                           AffineRows rows, int v_begin, int vlim, int cols, long ldg,
+                                                           G* __restrict__ out) {
+  constexpr int kEach = 16 / (int)sizeof(G);
+  const long t = blockIdx.y;
+  const int c = (blockIdx.x * 256 + threadIdx.x) * kEach, v = v_begin + c;
+  if (c >= cols) return;
+  const float alpha = rows.alpha[t], beta = rows.beta ? rows.beta[t] : 0.f, l2 = lse[t] * kLog2e;
+  const bool live = alpha != 0.f || beta != 0.f;
+  float g[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; i += 4) {
+    const f32x4 z = live && v + i < vlim ? *reinterpret_cast<const f32x4*>(Z + t * ldz + v + i) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      g[i + u] = live && v + i + u < vlim ? fast_exp2(__builtin_fmaf(z[u], rows.scale2, -l2)) * __builtin_fmaf(beta, z[u], alpha) : 0.f;
+  }
+  if constexpr (sizeof(G) == 2) {
+    *reinterpret_cast<u32x4*>(out + t * ldg + c) =
+        u32x4{pack_bf16x2(g[0], g[1]), pack_bf16x2(g[2], g[3]), pack_bf16x2(g[4], g[5]), pack_bf16x2(g[6], g[7])};
+  } else {
+    *reinterpret_cast<f32x4*>(out + t * ldg + c) = f32x4{g[0], g[1], g[2], g[3]};
+  }
+}
+
 // A row whose factors are both 0 gets no gradient and may hold anything, NaN too: in dW = G^T H its zeros would meet that.
 __global__ __launch_bounds__(256) void clean_rows_kernel(const uint32_t* __restrict__ h, const float* __restrict__ alpha,
                                                          const float* __restrict__ beta, long row_words,
@@ -1052,7 +1080,8 @@ struct Scratch {
 bool keep_logits(const ScoreShape& sh) { return 4 * sh.n * sh.v <= kKeptBytes; }
 
 // k_list: length of a teacher's list (0: scoring, with `top` alternatives).
-Scratch carve(const ScoreShape& sh, int f32, int q4, int top, int k_list, void* ws, size_t* bytes) {
+// logits: the caller's, which keeps them (or, for its size alone, any address).
+Scratch carve(const ScoreShape& sh, int f32, int q4, int top, int k_list, float* logits, void* ws, size_t* bytes) {
   Scratch x{};
   Carver c{static_cast<char*>(ws)};
   x.few = f32 ? sh.n <= kFewTokens32 && sh.d % 4 == 0 : sh.n <= kFewTokens;
@@ -1060,10 +1089,10 @@ Scratch carve(const ScoreShape& sh, int f32, int q4, int top, int k_list, void* 
   x.ldg = x.few ? x.groups : (x.groups + 1) / 2 * 2;  // a tile of 256 logits writes both its groups, the last one too
   x.take = top < x.groups ? top : x.groups;
   x.ldz = (long)x.groups * kGroup;
-  x.kept = x.few || (top && keep_logits(sh));
+  x.kept = x.few || logits || (top && keep_logits(sh));
   x.rows = x.kept || sh.n < kScoreRows ? sh.n : kScoreRows;
   if (x.few) {
-    x.z = c.take<float>(x.rows * x.ldz);
+    x.z = logits ? logits : c.take<float>(x.rows * x.ldz);
     x.gmax = c.take<float>(x.rows * x.groups);
     x.gs = c.take<float>(x.rows * x.groups);
     x.gu = c.take<float>(x.rows * x.groups);
@@ -1074,11 +1103,11 @@ Scratch carve(const ScoreShape& sh, int f32, int q4, int top, int k_list, void* 
     const long parts = splits(x.rows) * x.rows > splits(last) * last ? splits(x.rows) * x.rows : splits(last) * last;
     x.m = c.take<float>(parts);
     x.s = c.take<float>(parts);
-    if (!k_list) x.u = c.take<float>(parts);
+    if (!k_list || x.kept) x.u = c.take<float>(parts);
     if (top) {
       x.gmax = c.take<float>(x.rows * x.ldg);
     }
-    if (x.kept) x.z = c.take<float>(x.rows * x.ldz);
+    if (x.kept) x.z = logits ? logits : c.take<float>(x.rows * x.ldz);
     const long entries = x.kept ? 0 : x.rows * x.take;
     if (entries) {
       x.chosen = c.take<int>(entries);
@@ -1090,7 +1119,7 @@ Scratch carve(const ScoreShape& sh, int f32, int q4, int top, int k_list, void* 
       if (x.max_tiles > entries) x.max_tiles = (int)entries;
       x.tiles = c.take<GatherTile>(x.max_tiles);
     }
-    if (k_list) {
+    if (k_list && !x.kept) {
       x.column = c.take<int>(x.rows * k_list);
       x.slot = c.take<int>(x.rows * k_list);
       x.picks = c.take<float>(x.rows * k_list);
@@ -1186,9 +1215,11 @@ hipError_t launch_lce_gather(const LceHead& h, const bf16_t* H, int D, int V, co
   return hipGetLastError();
 }
 
-size_t logprobs_fwd_workspace(const ScoreShape& sh, int f32, int q4, int top) {
+// Any address of a caller's logits: whether there are some is all that the sizes depend on.
+float* some_logits(int keep) { return keep ? reinterpret_cast<float*>(16) : nullptr; }
+size_t logprobs_fwd_workspace(const ScoreShape& sh, int f32, int q4, int top, int keep) {
   size_t bytes;
-  carve(sh, f32, q4, top, 0, nullptr, &bytes);
+  carve(sh, f32, q4, top, 0, some_logits(keep), nullptr, &bytes);
   return bytes;
 }
 
@@ -1202,12 +1233,12 @@ hipError_t launch_logprobs_fwd(const ScoreHead& head, const ScoreShape& sh, cons
                                int top, const LogprobsOut& o, void* ws, hipStream_t st) {
   size_t bytes;
   ScoreHead h = head;
-  const Scratch x = carve(sh, h.f32, h.f32 ? h.h32.q4 : h.h.q4, top, 0, ws, &bytes);
+  const Scratch x = carve(sh, h.f32, h.f32 ? h.h32.q4 : h.h.q4, top, 0, o.logits, ws, &bytes);
   const float c2 = kLog2e * sh.inv_t;
   const int V = (int)sh.v;
   const hipError_t staged = staged_head(h, sh, x, st);
   if (staged != hipSuccess) return staged;
-  if (x.kept) {  // (one pass: as many rows as that keeps are fewer than a pass takes)
+  if (x.kept) {  // (one pass)
     const hipError_t e = x.few ? few_logits(h, sh, x, c2, st) : tile_stats(h, sh, x, 0, sh.n, c2, 0, st);
     if (e != hipSuccess) return e;
     auto rows = [&](auto kernel) {
@@ -1256,9 +1287,9 @@ hipError_t launch_logprobs_fwd(const ScoreHead& head, const ScoreShape& sh, cons
   return hipSuccess;
 }
 
-size_t distill_fwd_workspace(const ScoreShape& sh, int f32, int q4, int k) {
+size_t distill_fwd_workspace(const ScoreShape& sh, int f32, int q4, int k, int keep) {
   size_t bytes;
-  carve(sh, f32, q4, 0, k, nullptr, &bytes);
+  carve(sh, f32, q4, 0, k, some_logits(keep), nullptr, &bytes);
   return bytes;
 }
 
@@ -1266,7 +1297,7 @@ hipError_t launch_distill_fwd(const ScoreHead& head, const ScoreShape& sh, const
                               const uint8_t* mask, const DistillLoss& p, const DistillOut& o, void* ws, hipStream_t st) {
   size_t bytes;
   ScoreHead h = head;
-  const Scratch x = carve(sh, h.f32, h.f32 ? h.h32.q4 : h.h.q4, 0, p.k, ws, &bytes);
+  const Scratch x = carve(sh, h.f32, h.f32 ? h.h32.q4 : h.h.q4, 0, p.k, o.logits, ws, &bytes);
   const float c2 = kLog2e * sh.inv_t;
   const hipError_t staged = staged_head(h, sh, x, st);
   if (staged != hipSuccess) return staged;
@@ -1278,8 +1309,8 @@ hipError_t launch_distill_fwd(const ScoreHead& head, const ScoreShape& sh, const
     const int64_t* id = ids + r0 * p.k;
     const float* lp = teacher + r0 * p.k;
     const uint8_t* see = mask ? mask + r0 : nullptr;
-    if (x.few) {
-      const hipError_t e = few_logits(h, sh, x, c2, st);
+    if (x.kept) {
+      const hipError_t e = x.few ? few_logits(h, sh, x, c2, st) : tile_stats(h, sh, x, 0, n, c2, 0, st);
       if (e != hipSuccess) return e;
     } else {
       hipLaunchKernelGGL(sort_lists_kernel, dim3((unsigned)ceil_div(n, 4)), dim3(256), 0, st, id, lp, see, n, sh.v, p.k, x.column,
@@ -1289,7 +1320,7 @@ hipError_t launch_distill_fwd(const ScoreHead& head, const ScoreShape& sh, const
       if (e != hipSuccess) return e;
     }
     hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(n, 4)), dim3(256), 0, st, row_parts(x, h, n, sh.v, c2), x.column,
-                       x.slot, x.picks, x.few ? x.z : nullptr, x.ldz, id, lp, see, n, sh.v, sh.inv_t, p.k, p.renormalize, p.beta, row_loss + r0,
+                       x.slot, x.picks, x.kept ? x.z : nullptr, x.ldz, id, lp, see, n, sh.v, sh.inv_t, p.k, p.renormalize, p.beta, row_loss + r0,
                        x.row_counts + r0, o.lse + r0, o.rest + r0, o.coef + r0 * p.k, o.columns + r0 * p.k);
     MTP_LAUNCHED();
   }
@@ -1305,6 +1336,29 @@ hipError_t launch_logprobs_coef(const float* d_logprobs, const float* d_entropy,
   hipLaunchKernelGGL(logprobs_coef_kernel, dim3((unsigned)ceil_div(n, 256)), dim3(256), 0, st, d_logprobs, d_entropy, targets,
                      ignore_index, lse, entropy, tgt, n, v, inv_t, alpha, beta, columns, value);
   return hipGetLastError();
+}
+
+template <class G>
+hipError_t affine_tiles(const AffineGrad& a, const float* lse, long n, int v_begin, int vlim, int cols, long ldg, G* g, hipStream_t st) {
+  const int each = 16 / (int)sizeof(G);
+  for (long r0 = 0; r0 < n; r0 += 32768) {  // blockIdx.y
+    const long rows = n - r0 < 32768 ? n - r0 : 32768;
+    AffineRows r = a.rows;
+    r.alpha += r0;
+    if (r.beta) r.beta += r0;
+    hipLaunchKernelGGL(affine_tiles_kernel<G>, dim3((unsigned)ceil_div(cols, 256 * each), (unsigned)rows), dim3(256), 0, st, a.z + r0 * a.ldz,
+                       a.ldz, lse + r0, r, v_begin, vlim, cols, ldg, g + r0 * ldg);
+    MTP_LAUNCHED();
+  }
+  return hipSuccess;
+}
+hipError_t launch_affine_tiles(const AffineGrad& a, const float* lse, long n, int v_begin, int vlim, int cols, long ldg, bf16_t* g,
+                               hipStream_t st) {
+  return affine_tiles(a, lse, n, v_begin, vlim, cols, ldg, g, st);
+}
+hipError_t launch_affine_tiles(const AffineGrad& a, const float* lse, long n, int v_begin, int vlim, int cols, long ldg, float* g,
+                               hipStream_t st) {
+  return affine_tiles(a, lse, n, v_begin, vlim, cols, ldg, g, st);
 }
 
 hipError_t launch_distill_coef(const float* d_loss, int per_row, const float* scale, const float* rest, const float* coef, long n,

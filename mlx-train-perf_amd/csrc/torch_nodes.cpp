@@ -510,10 +510,11 @@ struct KernelLoss : torch::autograd::Function<KernelLoss> {
 };
 
 // The head of a scoring or distillation call, as core/scoring.py's _Inputs: owner is the weight of the cached transposed copy,
-// fwd_kind what the forward takes it as.
+// fwd_kind what the forward takes it as; kept: bytes of the logits that it keeps for a backward.
 struct ScoreHead {
   at::Tensor w, w_q, scales, biases, owner;
-  int64_t kind, fwd_kind;
+  int64_t kind, fwd_kind, kept;
+  bool recorded = false;  // a graph is
   int64_t vocab() const { return w.defined() ? w.size(0) : w_q.size(0); }
 };
 
@@ -578,7 +579,13 @@ void keep_head(torch::autograd::AutogradContext* ctx, const ScoreHead& h, const 
 ScoreHead kept_head(torch::autograd::AutogradContext* ctx) {
   auto& sd = ctx->saved_data;
   auto tensor = [&](const char* name) { return sd.count(name) ? sd[name].toTensor() : at::Tensor(); };
-  return ScoreHead{tensor("w"), tensor("w_q"), tensor("scales"), tensor("biases"), tensor("owner"), sd["kind"].toInt(), 0};
+  return ScoreHead{tensor("w"), tensor("w_q"), tensor("scales"), tensor("biases"), tensor("owner"), sd["kind"].toInt(), 0, 0};
+}
+// Room for the logits of a call that has a backward to come, or none.
+at::Tensor kept_logits(const at::Tensor& hidden, const ScoreHead& h, const std::optional<at::Tensor>& w, const at::Tensor& owner) {
+  // (inside a node's forward: whether its inputs ask for a gradient, and whether one is recorded)
+  const bool asked = hidden.requires_grad() || (w.has_value() && w->requires_grad()) || owner.requires_grad();
+  return h.kept && asked && h.recorded ? at::empty({h.kept / 4}, hidden.options().dtype(at::kFloat)) : at::Tensor();
 }
 
 struct LogprobsCall {
@@ -591,7 +598,7 @@ struct LogprobsCall {
 struct Logprobs : torch::autograd::Function<Logprobs> {
   // hidden, w and owner: the inputs that may ask for a gradient
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& hidden,
-                                                const std::optional<at::Tensor>& w, const at::Tensor& /*owner*/,
+                                                const std::optional<at::Tensor>& w, const at::Tensor& owner,
                                                 const LogprobsCall& c) {
     const c10::DeviceGuard device(hidden.device());
     const int64_t n = hidden.size(0), d = hidden.size(1), v = c.head.vocab();
@@ -602,22 +609,23 @@ struct Logprobs : torch::autograd::Function<Logprobs> {
     float *lse = ptr<float>(kept), *tgt = c.targets.defined() ? lse + n : nullptr;
     if (c.targets.defined()) logprobs = at::empty({n}, opt);
     const at::Tensor top = at::empty({n, c.top}, opt), ids = at::empty({n, c.top}, opt.dtype(at::kLong));
-    const size_t bytes = (f32 ? g_api.logprobs_ws32 : g_api.logprobs_ws)(n, d, v, (int)c.head.fwd_kind, (int)c.top);
+    const at::Tensor logits = kept_logits(hidden, c.head, w, owner);
+    const size_t bytes = (f32 ? g_api.logprobs_ws32 : g_api.logprobs_ws)(n, d, v, (int)c.head.fwd_kind, (int)c.top, logits.defined());
     const at::Tensor ws = bytes_like(hidden, bytes);
     const auto* y = c.targets.defined() ? ptr<int64_t>(c.targets) : nullptr;
     const ScoreHead& h = c.head;
     if (f32)
       check(g_api.logprobs_fwd32(ptr<float>(hidden), opt_ptr<float>(h.w), opt_ptr<uint32_t>(h.w_q), opt_ptr<float>(h.scales),
                                  opt_ptr<float>(h.biases), y, n, d, v, (int)h.fwd_kind, c.ignore_index, (int)c.top, c.temperature,
-                                 opt_ptr<float>(logprobs), ptr<float>(entropy), ptr<float>(top), ptr<int64_t>(ids), lse, tgt, ptr(ws),
-                                 bytes, stream_of(hidden)),
+                                 opt_ptr<float>(logprobs), ptr<float>(entropy), ptr<float>(top), ptr<int64_t>(ids), lse, tgt, opt_ptr<float>(logits),
+                                 ptr(ws), bytes, stream_of(hidden)),
             "loss");
     else
       check(g_api.logprobs_fwd(ptr(hidden), opt_ptr(h.w), opt_ptr<uint32_t>(h.w_q), opt_ptr(h.scales), opt_ptr(h.biases), y, n, d, v,
                                (int)h.fwd_kind, c.ignore_index, (int)c.top, c.temperature, opt_ptr<float>(logprobs), ptr<float>(entropy),
-                               ptr<float>(top), ptr<int64_t>(ids), lse, tgt, ptr(ws), bytes, stream_of(hidden)),
+                               ptr<float>(top), ptr<int64_t>(ids), lse, tgt, opt_ptr<float>(logits), ptr(ws), bytes, stream_of(hidden)),
             "loss");
-    ctx->save_for_backward({hidden, c.targets, kept, entropy});
+    ctx->save_for_backward({hidden, c.targets, kept, entropy, logits});
     keep_head(ctx, h, w);
     ctx->saved_data["ignore_index"] = c.ignore_index;
     ctx->saved_data["temperature"] = c.temperature;
@@ -629,7 +637,7 @@ struct Logprobs : torch::autograd::Function<Logprobs> {
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const at::Tensor &hidden = saved[0], &targets = saved[1], &kept = saved[2], &entropy = saved[3];
+    const at::Tensor &hidden = saved[0], &targets = saved[1], &kept = saved[2], &entropy = saved[3], &logits = saved[4];
     const c10::DeviceGuard device(hidden.device());
     const ScoreHead h = kept_head(ctx);
     const int64_t n = hidden.size(0), d = hidden.size(1), v = h.vocab(), ignore = ctx->saved_data["ignore_index"].toInt();
@@ -644,12 +652,12 @@ struct Logprobs : torch::autograd::Function<Logprobs> {
     if (hidden.scalar_type() == at::kFloat)
       check(g_api.logprobs_bwd32(ptr<float>(hidden), opt_ptr<float>(h.w), opt_ptr<uint32_t>(h.w_q), opt_ptr<float>(h.scales),
                                  opt_ptr<float>(h.biases), y, n, d, v, (int)p.kind, ignore, temperature, lse, ptr<float>(entropy), tgt,
-                                 opt_ptr<float>(d_logprobs), opt_ptr<float>(d_entropy), ptr<float>(p.d_hidden), opt_ptr<float>(p.d_w),
+                                 opt_ptr<float>(logits), opt_ptr<float>(d_logprobs), opt_ptr<float>(d_entropy), ptr<float>(p.d_hidden), opt_ptr<float>(p.d_w),
                                  p.chunk, ptr(p.ws), p.bytes, stream_of(hidden)),
             "loss");
     else
       check(g_api.logprobs_bwd(ptr(hidden), opt_ptr(h.w), opt_ptr(p.w_t), opt_ptr<uint32_t>(h.w_q), opt_ptr(h.scales), opt_ptr(h.biases),
-                               y, n, d, v, (int)p.kind, ignore, temperature, lse, ptr<float>(entropy), tgt, opt_ptr<float>(d_logprobs),
+                               y, n, d, v, (int)p.kind, ignore, temperature, lse, ptr<float>(entropy), tgt, opt_ptr<float>(logits), opt_ptr<float>(d_logprobs),
                                opt_ptr<float>(d_entropy), ptr(p.d_hidden), opt_ptr(p.d_w), p.chunk, p.rows, ptr(p.ws), p.bytes,
                                stream_of(hidden)),
             "loss");
@@ -666,7 +674,7 @@ struct DistillCall {
 
 struct Distillation : torch::autograd::Function<Distillation> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& hidden, const std::optional<at::Tensor>& w,
-                            const at::Tensor& /*owner*/, const DistillCall& c) {
+                            const at::Tensor& owner, const DistillCall& c) {
     const c10::DeviceGuard device(hidden.device());
     const int64_t n = hidden.size(0), d = hidden.size(1), v = c.head.vocab(), k = c.ids.size(1);
     const bool f32 = hidden.scalar_type() == at::kFloat;
@@ -675,7 +683,8 @@ struct Distillation : torch::autograd::Function<Distillation> {
     // lse, a factor per token, a factor and a column (int32) per slot, the scale
     const at::Tensor kept = at::empty({2 * n * (k + 1) + 1}, opt);
     float *lse = ptr<float>(kept), *rest = lse + n, *coef = rest + n, *columns = coef + n * k, *scale = columns + n * k;
-    const size_t bytes = (f32 ? g_api.distill_ws32 : g_api.distill_ws)(n, d, v, (int)c.head.fwd_kind, (int)k);
+    const at::Tensor logits = kept_logits(hidden, c.head, w, owner);
+    const size_t bytes = (f32 ? g_api.distill_ws32 : g_api.distill_ws)(n, d, v, (int)c.head.fwd_kind, (int)k, logits.defined());
     const at::Tensor ws = bytes_like(hidden, bytes);
     const ScoreHead& h = c.head;
     const auto* ids = ptr<int64_t>(c.ids);
@@ -684,15 +693,15 @@ struct Distillation : torch::autograd::Function<Distillation> {
       check(g_api.distill_fwd32(ptr<float>(hidden), opt_ptr<float>(h.w), opt_ptr<uint32_t>(h.w_q), opt_ptr<float>(h.scales),
                                 opt_ptr<float>(h.biases), ids, ptr<float>(c.teacher), mask, n, d, v, (int)h.fwd_kind, (int)k, (int)c.kind,
                                 c.beta, c.temperature, (int)c.renormalize, (int)c.reduction, ptr<float>(loss), scale, lse, rest, coef,
-                                reinterpret_cast<int32_t*>(columns), ptr(ws), bytes, stream_of(hidden)),
+                                reinterpret_cast<int32_t*>(columns), opt_ptr<float>(logits), ptr(ws), bytes, stream_of(hidden)),
             "loss");
     else
       check(g_api.distill_fwd(ptr(hidden), opt_ptr(h.w), opt_ptr<uint32_t>(h.w_q), opt_ptr(h.scales), opt_ptr(h.biases), ids,
                               ptr<float>(c.teacher), mask, n, d, v, (int)h.fwd_kind, (int)k, (int)c.kind, c.beta, c.temperature,
                               (int)c.renormalize, (int)c.reduction, ptr<float>(loss), scale, lse, rest, coef,
-                              reinterpret_cast<int32_t*>(columns), ptr(ws), bytes, stream_of(hidden)),
+                              reinterpret_cast<int32_t*>(columns), opt_ptr<float>(logits), ptr(ws), bytes, stream_of(hidden)),
             "loss");
-    ctx->save_for_backward({hidden, kept});
+    ctx->save_for_backward({hidden, kept, logits});
     keep_head(ctx, h, w);
     ctx->saved_data["k"] = k;
     ctx->saved_data["reduction"] = c.reduction;
@@ -702,7 +711,7 @@ struct Distillation : torch::autograd::Function<Distillation> {
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const at::Tensor &hidden = saved[0], &kept = saved[1];
+    const at::Tensor &hidden = saved[0], &kept = saved[1], &logits = saved[2];
     const c10::DeviceGuard device(hidden.device());
     const ScoreHead h = kept_head(ctx);
     auto& sd = ctx->saved_data;
@@ -715,13 +724,13 @@ struct Distillation : torch::autograd::Function<Distillation> {
     if (hidden.scalar_type() == at::kFloat)
       check(g_api.distill_bwd32(ptr<float>(hidden), opt_ptr<float>(h.w), opt_ptr<uint32_t>(h.w_q), opt_ptr<float>(h.scales),
                                 opt_ptr<float>(h.biases), n, d, v, (int)p.kind, (int)k, temperature, reduction, ptr<float>(ct), scale, lse,
-                                rest, coef, reinterpret_cast<const int32_t*>(columns), ptr<float>(p.d_hidden), opt_ptr<float>(p.d_w),
+                                rest, coef, reinterpret_cast<const int32_t*>(columns), opt_ptr<float>(logits), ptr<float>(p.d_hidden), opt_ptr<float>(p.d_w),
                                 p.chunk, ptr(p.ws), p.bytes, stream_of(hidden)),
             "loss");
     else
       check(g_api.distill_bwd(ptr(hidden), opt_ptr(h.w), opt_ptr(p.w_t), opt_ptr<uint32_t>(h.w_q), opt_ptr(h.scales), opt_ptr(h.biases),
                               n, d, v, (int)p.kind, (int)k, temperature, reduction, ptr<float>(ct), scale, lse, rest, coef,
-                              reinterpret_cast<const int32_t*>(columns), ptr(p.d_hidden), opt_ptr(p.d_w), p.chunk, p.rows, ptr(p.ws),
+                              reinterpret_cast<const int32_t*>(columns), opt_ptr<float>(logits), ptr(p.d_hidden), opt_ptr(p.d_w), p.chunk, p.rows, ptr(p.ws),
                               p.bytes, stream_of(hidden)),
             "loss");
     return once(grads, {p.d_hidden, p.d_w, at::Tensor(), at::Tensor()});
@@ -789,21 +798,23 @@ std::vector<at::Tensor> policy(const at::Tensor& nll, const at::Tensor& old, con
 
 std::vector<at::Tensor> logprobs(const at::Tensor& hidden, const std::optional<at::Tensor>& w, const std::optional<at::Tensor>& w_q,
                                  const std::optional<at::Tensor>& scales, const std::optional<at::Tensor>& biases, int64_t kind,
-                                 const at::Tensor& owner, int64_t fwd_kind, const std::optional<at::Tensor>& targets,
+                                 const at::Tensor& owner, int64_t fwd_kind, int64_t kept, const std::optional<at::Tensor>& targets,
                                  int64_t ignore_index, int64_t top, double temperature) {
   const at::Tensor none;
-  const LogprobsCall call{{w.value_or(none), w_q.value_or(none), scales.value_or(none), biases.value_or(none), owner, kind, fwd_kind},
+  const LogprobsCall call{{w.value_or(none), w_q.value_or(none), scales.value_or(none), biases.value_or(none), owner, kind, fwd_kind, kept,
+                           at::GradMode::is_enabled()},
                           targets.value_or(none), ignore_index, top, temperature};
   return apply_node([&] { return Logprobs::apply(hidden, w, owner, call); });
 }
 
 at::Tensor distillation(const at::Tensor& hidden, const std::optional<at::Tensor>& w, const std::optional<at::Tensor>& w_q,
                         const std::optional<at::Tensor>& scales, const std::optional<at::Tensor>& biases, int64_t kind,
-                        const at::Tensor& owner, int64_t fwd_kind, const at::Tensor& ids, const at::Tensor& teacher,
+                        const at::Tensor& owner, int64_t fwd_kind, int64_t kept, const at::Tensor& ids, const at::Tensor& teacher,
                         const std::optional<at::Tensor>& mask, int64_t loss_kind, double beta, double temperature,
                         int64_t renormalize, int64_t reduction) {
   const at::Tensor none;
-  const DistillCall call{{w.value_or(none), w_q.value_or(none), scales.value_or(none), biases.value_or(none), owner, kind, fwd_kind},
+  const DistillCall call{{w.value_or(none), w_q.value_or(none), scales.value_or(none), biases.value_or(none), owner, kind, fwd_kind, kept,
+                           at::GradMode::is_enabled()},
                          ids, teacher, mask.value_or(none), loss_kind, renormalize, reduction, beta, temperature};
   return apply_node([&] { return Distillation::apply(hidden, w, owner, call); });
 }

@@ -127,21 +127,22 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "mtp_policy_bwd": (ctypes.c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _c_void_p, _c_void_p,
                                       _i64, _i64, _f64, _f64, _f64, _i32, _c_void_p, _c_void_p, _c_void_p]),
     # token scoring and distillation
-    **{name: (_size, [_i64, _i64, _i64, _i32, _i32])
+    "mtp_score_logits_ld": (_i64, [_i64]),
+    **{name: (_size, [_i64, _i64, _i64, _i32, _i32, _i32])
        for name in ("mtp_logprobs_fwd_workspace_bytes", "mtp_logprobs_fwd_f32_workspace_bytes",
                     "mtp_distill_fwd_workspace_bytes", "mtp_distill_fwd_f32_workspace_bytes")},
     "mtp_score_bwd_workspace_bytes": (_size, [_i64, _i64, _i64, _i32, _i64, _i64, _i32, _i32]),
     "mtp_score_bwd_f32_workspace_bytes": (_size, [_i64, _i64, _i64, _i32, _i64, _i32, _i32]),
-    **{name: (ctypes.c_int, [*[_c_void_p] * 6, _i64, _i64, _i64, _i32, _i64, _i32, _f64, *[_c_void_p] * 7, _size, _c_void_p])
+    **{name: (ctypes.c_int, [*[_c_void_p] * 6, _i64, _i64, _i64, _i32, _i64, _i32, _f64, *[_c_void_p] * 8, _size, _c_void_p])
        for name in ("mtp_logprobs_fwd", "mtp_logprobs_fwd_f32")},
-    **{name: (ctypes.c_int, [*[_c_void_p] * 8, _i64, _i64, _i64, _i32, _i32, _i32, _f64, _f64, _i32, _i32, *[_c_void_p] * 7,
+    **{name: (ctypes.c_int, [*[_c_void_p] * 8, _i64, _i64, _i64, _i32, _i32, _i32, _f64, _f64, _i32, _i32, *[_c_void_p] * 8,
                              _size, _c_void_p])
        for name in ("mtp_distill_fwd", "mtp_distill_fwd_f32")},
     # bf16: w_t after w, row_block after chunk
-    **{name: (ctypes.c_int, [*[_c_void_p] * (7 - f32), _i64, _i64, _i64, _i32, _i64, _f64, *[_c_void_p] * 7, *[_i64] * (2 - f32),
+    **{name: (ctypes.c_int, [*[_c_void_p] * (7 - f32), _i64, _i64, _i64, _i32, _i64, _f64, *[_c_void_p] * 8, *[_i64] * (2 - f32),
                              _c_void_p, _size, _c_void_p])
        for name, f32 in (("mtp_logprobs_bwd", 0), ("mtp_logprobs_bwd_f32", 1))},
-    **{name: (ctypes.c_int, [*[_c_void_p] * (6 - f32), _i64, _i64, _i64, _i32, _i32, _f64, _i32, *[_c_void_p] * 8,
+    **{name: (ctypes.c_int, [*[_c_void_p] * (6 - f32), _i64, _i64, _i64, _i32, _i32, _f64, _i32, *[_c_void_p] * 9,
                              *[_i64] * (2 - f32), _c_void_p, _size, _c_void_p])
        for name, f32 in (("mtp_distill_bwd", 0), ("mtp_distill_bwd_f32", 1))},
 }

@@ -138,6 +138,19 @@ def _staged32(x: _Inputs) -> int:
     return _native.HEAD_Q4_STAGED if fits and _loss.os.environ.get("MTP_LCE_STAGE_HEAD", "1") != "0" else x.kind
 
 
+def _kept_bytes(x: _Inputs) -> int:
+    """Bytes of the logits that a forward with a backward to come keeps for it, which then forms none again: a sixth of the
+    backward's workspace budget holds them (256 MiB of 1.5 GiB), or 0. A product less: fp32 training at 1588 x 4096 x 10500
+    5250 -> 4030 us, a 4-bit student's 488 -> 407 us."""
+    nbytes = x.hidden.shape[0] * ((x.v + 127) // 128 * 128) * 4
+    return nbytes if nbytes <= _plan.lce_bwd_budget_bytes() // 6 else 0
+
+
+def _kept_logits(x: _Inputs) -> torch.Tensor | None:
+    nbytes = _kept_bytes(x)
+    return torch.empty(nbytes // 4, dtype=torch.float32, device=x.hidden.device) if nbytes else None
+
+
 def _head_ptrs(x: _Inputs) -> tuple:
     return _native.ptr(x.w), _native.ptr(x.w_q), _native.ptr(x.scales), _native.ptr(x.biases)
 
@@ -189,7 +202,7 @@ def _entry(lib, name: str, x: _Inputs):
     return getattr(lib, name + ("_f32" if x.hidden.dtype == torch.float32 else ""))
 
 
-def _score_forward(x: _Inputs, targets, ignore_index: int, top: int, temperature: float):
+def _score_forward(x: _Inputs, targets, ignore_index: int, top: int, temperature: float, logits: torch.Tensor | None):
     """(logprobs, entropy, top_logprobs, top_ids, lse, tgt) of mtp_logprobs_fwd."""
     lib = _native.load()
     n, d = x.hidden.shape
@@ -202,25 +215,26 @@ def _score_forward(x: _Inputs, targets, ignore_index: int, top: int, temperature
     top_lp = torch.empty((n, top), dtype=torch.float32, device=dev)
     top_ids = torch.empty((n, top), dtype=torch.int64, device=dev)
     size = lib.mtp_logprobs_fwd_f32_workspace_bytes if f32 else lib.mtp_logprobs_fwd_workspace_bytes
-    ws_bytes = size(n, d, x.v, kind, top)
+    ws_bytes = size(n, d, x.v, kind, top, int(logits is not None))
     ws = _workspace(ws_bytes, x.hidden)
     with _native.on_device(x.hidden):
         rc = _entry(lib, "mtp_logprobs_fwd", x)(
             x.hidden.data_ptr(), *_head_ptrs(x), _native.ptr(targets), n, d, x.v, kind, ignore_index, top, temperature,
             _native.ptr(logprobs), entropy.data_ptr(), top_lp.data_ptr(), top_ids.data_ptr(), lse.data_ptr(), _native.ptr(tgt),
-            ws.data_ptr(), ws_bytes, _native.stream_of(x.hidden))
+            _native.ptr(logits), ws.data_ptr(), ws_bytes, _native.stream_of(x.hidden))
     _native.check(rc, domain="loss")
     return logprobs, entropy, top_lp, top_ids, lse, tgt
 
 
 class _TokenLogprobs(torch.autograd.Function):
-    """Saves each token's log-sum-exp, entropy and target logit; the backward forms the logits again."""
+    """Saves each token's log-sum-exp, entropy and target logit, and few enough logits; more of them the backward forms again."""
 
     @staticmethod
     def forward(ctx, hidden, w, w_q, scales, biases, kind, owner, targets, ignore_index, top, temperature):
         x = _Inputs(hidden, w, w_q, scales, biases, kind, owner)
-        logprobs, entropy, top_lp, top_ids, lse, tgt = _score_forward(x, targets, ignore_index, top, temperature)
-        ctx.save_for_backward(hidden, targets, lse, entropy, tgt)
+        logits = _kept_logits(x) if any(ctx.needs_input_grad) else None
+        logprobs, entropy, top_lp, top_ids, lse, tgt = _score_forward(x, targets, ignore_index, top, temperature, logits)
+        ctx.save_for_backward(hidden, targets, lse, entropy, tgt, logits)
         ctx.inputs, ctx.args = x._replace(hidden=None), (ignore_index, temperature)
         ctx.mark_non_differentiable(top_lp, top_ids)
         ctx.set_materialize_grads(False)
@@ -229,7 +243,7 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, d_logprobs, d_entropy, _d_top, _d_ids):
-        hidden, targets, lse, entropy, tgt = ctx.saved_tensors
+        hidden, targets, lse, entropy, tgt, logits = ctx.saved_tensors
         ignore_index, temperature = ctx.args
         x = ctx.inputs._replace(hidden=hidden)
         d_logprobs, d_entropy = _float(d_logprobs), _float(d_entropy)
@@ -237,14 +251,14 @@ class _TokenLogprobs(torch.autograd.Function):
         def call(lib, head, shape, rest):
             return _entry(lib, "mtp_logprobs_bwd", x)(
                 *head, _native.ptr(targets), *shape, ignore_index, temperature, lse.data_ptr(), entropy.data_ptr(),
-                _native.ptr(tgt), _native.ptr(d_logprobs), _native.ptr(d_entropy), *rest)
+                _native.ptr(tgt), _native.ptr(logits), _native.ptr(d_logprobs), _native.ptr(d_entropy), *rest)
 
         d_hidden, d_w = _backward(x, 1, x.w is not None and ctx.needs_input_grad[1], call)
         return (d_hidden, d_w, *[None] * 9)
 
 
 class _Distillation(torch.autograd.Function):
-    """Saves the gradient's factors: one per token, and one per slot of its list."""
+    """Saves the gradient's factors, one per token and one per slot of its list, and few enough logits."""
 
     @staticmethod
     def forward(ctx, hidden, w, w_q, scales, biases, kind, owner, ids, teacher, mask, loss_kind, beta, temperature,
@@ -261,22 +275,24 @@ class _Distillation(torch.autograd.Function):
         coef = torch.empty((n, k), dtype=torch.float32, device=dev)
         columns = torch.empty((n, k), dtype=torch.int32, device=dev)
         size = lib.mtp_distill_fwd_f32_workspace_bytes if f32 else lib.mtp_distill_fwd_workspace_bytes
-        ws_bytes = size(n, d, x.v, fwd_kind, k)
+        logits = _kept_logits(x) if any(ctx.needs_input_grad) else None
+        ws_bytes = size(n, d, x.v, fwd_kind, k, int(logits is not None))
         ws = _workspace(ws_bytes, hidden)
         with _native.on_device(hidden):
             rc = _entry(lib, "mtp_distill_fwd", x)(
                 hidden.data_ptr(), *_head_ptrs(x), ids.data_ptr(), teacher.data_ptr(), _native.ptr(mask), n, d, x.v, fwd_kind, k,
                 loss_kind, beta, temperature, renormalize, reduction, loss.data_ptr(), scale.data_ptr(), lse.data_ptr(),
-                rest.data_ptr(), coef.data_ptr(), columns.data_ptr(), ws.data_ptr(), ws_bytes, _native.stream_of(hidden))
+                rest.data_ptr(), coef.data_ptr(), columns.data_ptr(), _native.ptr(logits), ws.data_ptr(), ws_bytes,
+                _native.stream_of(hidden))
         _native.check(rc, domain="loss")
-        ctx.save_for_backward(hidden, scale, lse, rest, coef, columns)
+        ctx.save_for_backward(hidden, scale, lse, rest, coef, columns, logits)
         ctx.inputs, ctx.args = x._replace(hidden=None), (temperature, reduction)
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_loss):
-        hidden, scale, lse, rest, coef, columns = ctx.saved_tensors
+        hidden, scale, lse, rest, coef, columns, logits = ctx.saved_tensors
         temperature, reduction = ctx.args
         x = ctx.inputs._replace(hidden=hidden)
         ct, k = _float(d_loss), coef.shape[1]
@@ -284,7 +300,7 @@ class _Distillation(torch.autograd.Function):
         def call(lib, head, shape, after):
             return _entry(lib, "mtp_distill_bwd", x)(
                 *head, *shape, k, temperature, reduction, ct.data_ptr(), scale.data_ptr(), lse.data_ptr(), rest.data_ptr(),
-                coef.data_ptr(), columns.data_ptr(), *after)
+                coef.data_ptr(), columns.data_ptr(), _native.ptr(logits), *after)
 
         d_hidden, d_w = _backward(x, k, x.w is not None and ctx.needs_input_grad[1], call)
         return (d_hidden, d_w, *[None] * 13)
@@ -396,7 +412,7 @@ def token_logprobs(hidden: torch.Tensor, head: HeadRef, targets: torch.Tensor | 
         y = None if targets2 is None else targets2.to(torch.int64).contiguous()
         args = (y, int(ignore_index), top, temperature)
         nodes = _nodes(x)
-        parts = _TokenLogprobs.apply(*x, *args) if nodes is None else nodes.logprobs(*x, _forward_kind(x), *args)
+        parts = _TokenLogprobs.apply(*x, *args) if nodes is None else nodes.logprobs(*x, _forward_kind(x), _kept_bytes(x), *args)
     *logprobs, entropy, top_lp, top_ids = parts   # (the node has none without targets)
     logprobs = logprobs[0] if logprobs else None
     return TokenLogprobs(None if logprobs is None else logprobs.view(leading), entropy.view(leading),
@@ -459,5 +475,5 @@ def distillation_loss(hidden: torch.Tensor, head: HeadRef, teacher_ids: torch.Te
         args = (ids2.to(torch.int64).contiguous(), _float(teacher2), None if mask2 is None else mask2.contiguous(), _KINDS[kind],
                 float(beta), temperature, int(renormalize), _REDUCTIONS[reduction])
         nodes = _nodes(x)
-        loss = _Distillation.apply(*x, *args) if nodes is None else nodes.distillation(*x, _forward_kind(x), *args)
+        loss = _Distillation.apply(*x, *args) if nodes is None else nodes.distillation(*x, _forward_kind(x), _kept_bytes(x), *args)
     return loss.view(leading) if reduction == "none" else loss

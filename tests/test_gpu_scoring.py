@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from mlx_train_perf import DenseHead, distillation_loss, linear_cross_entropy, policy_loss, token_logprobs
+from mlx_train_perf.core import scoring
 from mlx_train_perf.errors import LossInputError
 
 pytestmark = pytest.mark.gpu
@@ -377,6 +378,39 @@ def test_unchecked_ids_out_of_range_are_empty(n):
 
 
 # ---- as they are used ---------------------------------------------------------------------------------------------
+
+# A backward without its forward's logits forms them again; sizes as small as these keep them by themselves.
+_FORMED_AGAIN = [(5, 64, 97, 4, "dense", "bf16"), (300, 128, 1000, 20, "trainable", "bf16"), (300, 200, 1500, 64, "dense", "bf16"),
+                 (257, 192, 3001, 20, "q4", "bf16"), (150, 128, 1000, 20, "trainable", "fp32"), (150, 64, 700, 8, "q4", "fp32"),
+                 (70, 33, 301, 5, "dense", "fp32")]
+
+
+@pytest.mark.parametrize(("n", "d", "v", "k", "head", "dtype"), _FORMED_AGAIN)
+def test_gradients_of_logits_formed_again(n, d, v, k, head, dtype, monkeypatch):
+    monkeypatch.setattr(scoring, "_kept_bytes", lambda x: 0)
+    _check_score(n, d, v, top=k, head=head, dtype=dtype)
+    _check_distill(n, d, v, k, head=head, dtype=dtype)
+
+
+def test_which_logits_a_forward_keeps(monkeypatch):
+    hidden, hd, _ = S.make(40, 64, 300, head="dense", dtype="bf16")
+    hidden, hd = hidden.cuda().requires_grad_(), S.to(hd, "cuda")
+    kept = 40 * 384 * 4
+    y = torch.zeros(40, dtype=torch.long, device="cuda")
+    token_logprobs(hidden, hd, y)  # the library's own first uses
+
+    def held(grad, budget):
+        monkeypatch.setenv("MTP_LCE_BWD_BUDGET", str(budget))
+        before = torch.cuda.memory_allocated()
+        with torch.set_grad_enabled(grad):
+            out = token_logprobs(hidden, hd, y)
+        now = torch.cuda.memory_allocated() - before
+        del out
+        return now
+
+    assert held(True, 6 * kept) >= kept > held(True, 6 * kept - 6)
+    assert held(False, 6 * kept) < kept
+
 
 @pytest.mark.parametrize("n", [20, 300])
 def test_a_teacher_scores_a_student_learns(n):

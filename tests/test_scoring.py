@@ -166,9 +166,9 @@ def _call(name, **kw):
     lib = N.load()
     p = 1 << 20   # a pointer that nothing reads: every call here is refused before a launch
     base = {"logprobs": {"head": (p, p, None, None, None), "targets": p, "n": 4, "d": 64, "v": 100, "kind": 0, "top": 3, "t": 1.0,
-                         "out": (p, p, p, p, p, p), "ws": p, "bytes": 1 << 40},
+                         "out": (p, p, p, p, p, p, None), "ws": p, "bytes": 1 << 40},
             "distill": {"head": (p, p, None, None, None), "lists": (p, p, None), "n": 4, "d": 64, "v": 100, "kind": 0, "k": 3,
-                        "loss": 0, "beta": 0.5, "t": 1.0, "renorm": 0, "red": 1, "out": (p, p, p, p, p, p), "ws": p,
+                        "loss": 0, "beta": 0.5, "t": 1.0, "renorm": 0, "red": 1, "out": (p, p, p, p, p, p, None), "ws": p,
                         "bytes": 1 << 40}}[name]
     a = {**base, **kw}
     if name == "logprobs":
@@ -181,8 +181,8 @@ def _call(name, **kw):
 @pytest.mark.parametrize(("name", "kw", "code"), [
     ("logprobs", {"n": 0}, -1), ("logprobs", {"v": 2 ** 21 + 1}, -2), ("logprobs", {"d": 63}, -2), ("logprobs", {"top": -1}, -1),
     ("logprobs", {"top": 101}, -1), ("logprobs", {"top": 129, "v": 1000}, -2), ("logprobs", {"t": 0.0}, -1),
-    ("logprobs", {"t": math.nan}, -1), ("logprobs", {"bytes": 16}, -3), ("logprobs", {"ws": None}, -3), ("logprobs", {"ws": 8}, -2),
-    ("logprobs", {"out": (None,) * 6}, -1), ("logprobs", {"head": (8, 16, None, None, None)}, -2), ("logprobs", {"kind": 1}, -1),
+    ("logprobs", {"t": math.nan}, -1), ("logprobs", {"bytes": 16}, -3), ("logprobs", {"ws": None}, -3), ("logprobs", {"ws": 8}, -2), ("logprobs", {"out": (1 << 20,) * 6 + (8,)}, -2),
+    ("logprobs", {"out": (None,) * 7}, -1), ("logprobs", {"head": (8, 16, None, None, None)}, -2), ("logprobs", {"kind": 1}, -1),
     ("distill", {"k": 0}, -2), ("distill", {"k": 129}, -2), ("distill", {"loss": 3}, -1), ("distill", {"loss": 2, "beta": 1.0}, -1),
     ("distill", {"loss": 1, "renorm": 1}, -1), ("distill", {"red": 3}, -1), ("distill", {"lists": (None, None, None)}, -1),
     ("distill", {"bytes": 16}, -3), ("distill", {"t": 2e3}, -1)])
@@ -196,18 +196,18 @@ def test_workspaces():
     lib = N.load()
     for n in (1, 128, 129, 2048, 4096, 16384, 16385, 100000):
         for top in (0, 1, 128):
-            ws = lib.mtp_logprobs_fwd_workspace_bytes(n, 512, 32000, 0, top)
+            ws = lib.mtp_logprobs_fwd_workspace_bytes(n, 512, 32000, 0, top, 0)
             rows, partials = min(n, 16384), 8 << 20
             if n <= 128 or (top and n * 32000 * 4 <= 256 << 20):   # the logits, and each group's maximum (and sums)
                 most = n * (32128 * 4 + 3 * 252 * 4)
             else:   # the groups that a row's alternatives are looked for in
                 most = rows * top * (128 * 4 + 16) + rows * (252 + 1) * 4
             assert 0 < ws <= most + partials
-    assert lib.mtp_logprobs_fwd_workspace_bytes(0, 64, 100, 0, 1) == 0
-    assert lib.mtp_logprobs_fwd_workspace_bytes(8, 64, 2 ** 21 + 1, 0, 1) == 0
+    assert lib.mtp_logprobs_fwd_workspace_bytes(0, 64, 100, 0, 1, 0) == 0
+    assert lib.mtp_logprobs_fwd_workspace_bytes(8, 64, 2 ** 21 + 1, 0, 1, 0) == 0
     # a staged 4-bit head adds its rows, a few tokens none
-    staged, plain = (lib.mtp_logprobs_fwd_workspace_bytes(1000, 512, 32000, k, 4) for k in (N.HEAD_Q4_STAGED, N.HEAD_Q4))
+    staged, plain = (lib.mtp_logprobs_fwd_workspace_bytes(1000, 512, 32000, k, 4, 0) for k in (N.HEAD_Q4_STAGED, N.HEAD_Q4))
     assert staged == plain + 32000 * 512 * 2
-    assert lib.mtp_logprobs_fwd_workspace_bytes(8, 512, 32000, N.HEAD_Q4_STAGED, 4) == lib.mtp_logprobs_fwd_workspace_bytes(8, 512, 32000, N.HEAD_Q4, 4)
+    assert lib.mtp_logprobs_fwd_workspace_bytes(8, 512, 32000, N.HEAD_Q4_STAGED, 4, 0) == lib.mtp_logprobs_fwd_workspace_bytes(8, 512, 32000, N.HEAD_Q4, 4, 0)
     lce = lib.mtp_lce_bwd_workspace_bytes(300, 64, 1000, 0, 1024, 300)
     assert lib.mtp_score_bwd_workspace_bytes(300, 64, 1000, 0, 1024, 300, 5, 1) >= lce + 300 * (12 + 20) + 300 * 64 * 2
