@@ -238,8 +238,8 @@ void lce_few_kernel(const T* __restrict__ H, const T* __restrict__ W, const uint
   const int slabs = (D + kSlab - 1) / kSlab;
 
   // Operand j of a slab is the 16-byte chunk `2 j + half` of a dense row's; of packed words, word kFrags half + j, so that a
-  // lane's words lie together. Past the end of a row a load takes the next row's values (past the head zeros): the tokens'
-  // are zeros there.
+  // lane's words lie together. Past the end of a row a load takes the next row's values (past the head zeros),
+  // which in_row makes zeros, as the tokens' are (a 4-bit head's scales are): theirs may be infinite.
   u32x4 wa[kLoads];
   const long left = V - v0;
   const __amdgpu_buffer_rsrc_t rw = Q4 ? rows_rsrc(Wq + (long)v0 * (D >> 3), left * (D >> 1))
@@ -317,7 +317,9 @@ void lce_few_kernel(const T* __restrict__ H, const T* __restrict__ W, const uint
   put_tokens(lds);
   if constexpr (kStage) put_stage();
   lds_barrier();
-  for (int s = 0; s < slabs; ++s) {
+  int row_left = D * (int)sizeof(T) - 16 * half;  // bytes
+  auto in_row = [&](int j) { return 32 * j < row_left ? wa[j] : zero4(); };
+  for (int s = 0; s < slabs; ++s, row_left -= kRow) {
     const char* cur = lds + (s & 1) * kBytes;
     load_tokens(s + 1);  // (past the end: zeros)
     if constexpr (kStage) {
@@ -341,13 +343,13 @@ void lce_few_kernel(const T* __restrict__ H, const T* __restrict__ W, const uint
           for (int b = 0; b < NB; ++b) product4(a, token(cur, 8 * half + 2 * j + h, b), b);
         }
       } else if constexpr (F32) {
-        const f32x4 a = __builtin_bit_cast(f32x4, wa[j]);
+        const f32x4 a = __builtin_bit_cast(f32x4, in_row(j));
 #pragma unroll
         for (int b = 0; b < NB; ++b) product4(a, token(cur, 2 * j + half, b), b);
       } else {
         bf16x8 a;
         if constexpr (Q4) a = as_bf16x8(dequant8(wa[j >> 2][j & 3], j < 8 ? bf16lo(sc) : bf16hi(sc), j < 8 ? bf16lo(bi) : bf16hi(bi)));
-        else a = as_bf16x8(wa[j]);
+        else a = as_bf16x8(in_row(j));
 #pragma unroll
         for (int b = 0; b < NB; ++b) acc[b] = mfma32(a, as_bf16x8(token(cur, Q4 ? kFrags * half + j : 2 * j + half, b)), acc[b]);
       }
@@ -739,7 +741,7 @@ __global__ __launch_bounds__(kPick) void score_rows_kernel(RowParts parts, const
     if (take < K) least = 0;
     if constexpr (KEPT) {
       for (int i = tid; i < take * kGroup; i += kPick)
-        key[i] = order_key(Z[t * ldz + (long)group[i / kGroup] * kGroup + i % kGroup]);
+        key[i] = group[i / kGroup] * kGroup + i % kGroup < V ? order_key(Z[t * ldz + (long)group[i / kGroup] * kGroup + i % kGroup]) : 0u;
       __syncthreads();
       write_top<MC>(key, group, take, K, least, V, inv_t, lse, t, targets ? y : -1, out, scratch);
     } else if (tid < take) {

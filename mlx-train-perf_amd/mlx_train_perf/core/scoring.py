@@ -12,6 +12,7 @@ and give none.
 from __future__ import annotations
 
 import math
+import operator
 from typing import Literal, NamedTuple
 
 import torch
@@ -28,6 +29,7 @@ MAX_LIST = 128          # alternatives, and slots of a teacher's list, that the 
 MAX_VOCAB = 1 << 21     # vocabulary that the kernels serve
 TAIL_FLOOR = 1e-6       # least mass that the outcomes outside a list count as
 _KINDS = {"forward": 0, "reverse": 1, "jsd": 2}
+_ID_TYPES = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
 _REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
@@ -398,7 +400,10 @@ def token_logprobs(hidden: torch.Tensor, head: HeadRef, targets: torch.Tensor | 
         _loss._validate_inputs(hidden=hidden, head=head, targets=targets, validate_targets=validate_targets,
                                ignore_index=ignore_index)
     temperature = _temperature(temperature)
-    top = int(top)
+    try:
+        top = operator.index(top)
+    except TypeError:
+        raise LossInputError(f"top must be a whole number; got {top!r}") from None
     if not 0 <= top <= _head_v(head):
         raise LossInputError(f"top must be in [0, V={_head_v(head)}]; got {top}")
     if not _loss._int64(ignore_index):
@@ -451,8 +456,8 @@ def distillation_loss(hidden: torch.Tensor, head: HeadRef, teacher_ids: torch.Te
     if teacher_ids.dim() != hidden.dim() or tuple(teacher_ids.shape[:-1]) != leading or teacher_ids.shape[-1] < 1:
         raise LossInputError(f"teacher_ids must be hidden's leading dims {leading} and at least one slot; got shape "
                              f"{tuple(teacher_ids.shape)}")
-    if teacher_ids.dtype.is_floating_point or teacher_ids.dtype.is_complex or teacher_ids.dtype == torch.bool:
-        raise LossInputError(f"teacher_ids must be an integer dtype, got {teacher_ids.dtype}")
+    if teacher_ids.dtype not in _ID_TYPES:
+        raise LossInputError(f"teacher_ids must be int8 to int64 or uint8, got {teacher_ids.dtype}")
     if teacher_logprobs.shape != teacher_ids.shape or not teacher_logprobs.dtype.is_floating_point:
         raise LossInputError(f"teacher_logprobs must be floating-point of teacher_ids' shape {tuple(teacher_ids.shape)}; got "
                              f"{teacher_logprobs.dtype} {tuple(teacher_logprobs.shape)}")

@@ -249,6 +249,25 @@ def test_logits_that_are_no_numbers(n):
         assert torch.equal(a[1:-1], b[1:-1])
 
 
+@pytest.mark.parametrize(("n", "d", "dtype"), [(3, 72, "bf16"), (40, 72, "bf16"), (140, 72, "bf16"), (3, 36, "fp32"), (140, 36, "fp32")])
+def test_a_token_that_is_ruled_out_by_its_weight(n, d, dtype):
+    """-inf at a place where every hidden state is positive: a logit of -inf, and the row before it as without."""
+    hidden, hd, w = S.make(n, d, 100, dtype=dtype, seed=5)
+    hidden[:, 5] = 1.0
+    w[8, 5] = -math.inf
+    hd = DenseHead(weight=w.to(hidden.dtype).cuda(), trainable=False)
+    y = torch.arange(n) % 8
+    got = token_logprobs(hidden.cuda(), hd, y.cuda(), top=100)
+    z = hidden.double() @ w.T
+    logp = torch.log_softmax(z, 1)
+    off = S.stat(100) + 256 * S.U
+    S.within(got.logprobs, logp.gather(1, y[:, None])[:, 0], off, "logprobs")
+    value, ids = torch.sort(logp, dim=1, descending=True, stable=True)
+    assert torch.equal(got.top_ids.cpu(), ids)
+    S.within(got.top_logprobs[:, :-1], value[:, :-1], off, "top_logprobs")
+    assert bool((got.top_logprobs[:, -1] == -math.inf).all())
+
+
 @pytest.mark.parametrize("n", [3, 140])
 @pytest.mark.parametrize("temperature", [1e-3, 1e3])
 def test_extreme_temperatures(n, temperature):

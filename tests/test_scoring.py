@@ -118,7 +118,7 @@ def _score(**kw):
 
 
 @pytest.mark.parametrize("kw", [{"hidden": torch.zeros(4)}, {"targets": torch.zeros(3, dtype=torch.int64)}, {"targets": torch.zeros(4)},
-                                {"targets": torch.full((4,), 30)}, {"targets": torch.full((4,), -1)}, {"top": -1}, {"top": 31},
+                                {"targets": torch.full((4,), 30)}, {"targets": torch.full((4,), -1)}, {"top": -1}, {"top": 31}, {"top": 2.5},
                                 {"temperature": 0.0}, {"temperature": math.nan}, {"temperature": 1e4}, {"impl": "other"},
                                 {"ignore_index": 0.5}, {"hidden": torch.zeros(4, 32)}, {"hidden": torch.zeros(4, 64, dtype=torch.bfloat16)}])
 def test_scoring_refuses(kw):
@@ -133,7 +133,8 @@ def _distill(**kw):
     return distillation_loss(args.pop("hidden"), args.pop("head"), args.pop("ids"), args.pop("lp"), **args)
 
 
-@pytest.mark.parametrize("kw", [{"ids": torch.zeros(4, dtype=torch.int64)}, {"ids": torch.zeros(4, 3)}, {"ids": torch.full((4, 3), 30)},
+@pytest.mark.parametrize("kw", [{"ids": torch.zeros(4, dtype=torch.int64)}, {"ids": torch.zeros(4, 3)}, {"ids": torch.zeros(4, 3, dtype=torch.bool)}, {"ids": torch.zeros(4, 3, dtype=torch.int32).view(torch.uint32)},
+                                {"ids": torch.full((4, 3), 30)},
                                 {"ids": torch.zeros(4, 0, dtype=torch.int64), "lp": torch.zeros(4, 0)}, {"lp": torch.zeros(4, 2)},
                                 {"lp": torch.zeros(4, 3, dtype=torch.int64)}, {"lp": torch.zeros(4, 3, requires_grad=True)},
                                 {"mask": torch.ones(3, dtype=torch.bool)}, {"mask": torch.ones(4)}, {"kind": "other"},
