@@ -908,31 +908,35 @@ int mtp_logprobs_fwd_f32(const float* hidden, const float* w, const uint32_t* w_
                       mtp::LogprobsOut{logprobs, entropy, top_logprobs, top_ids, lse, tgt, logits}, workspace, workspace_bytes, stream);
 }
 
-// After the loss's workspace: alpha [n], beta [n], the columns [n] of scoring, the values [n][k], the cleared hidden states, or
-// an fp32 4-bit head's rows (staged bytes).
+// Rows of G in the bf16 backward: two a token where that fills a row tile at most (AffineGrad's halves).
+static int64_t score_g_rows(int64_t n) { return 2 * n <= kTile ? 2 * n : n; }
+// After the loss's workspace (of score_g_rows rows): alpha [n], beta [n], the columns [n] of scoring, the values [n][k], the halves, the
+// cleared hidden states, or an fp32 4-bit head's rows (staged bytes). g_rows: of G.
 struct ScoreBwd {
-  size_t alpha, beta, columns, value, clean, bytes;
+  size_t alpha, beta, columns, value, halves, clean, bytes;
 };
-static ScoreBwd score_bwd_parts(size_t lce, int64_t n, int64_t d, int32_t k, int32_t trainable, size_t elem, size_t staged) {
+static ScoreBwd score_bwd_parts(size_t lce, int64_t n, int64_t g_rows, int64_t d, int32_t k, int32_t trainable, size_t elem, size_t staged) {
   auto pad = [](size_t x) { return (x + 255) / 256 * 256; };
   ScoreBwd p;
   p.alpha = pad(lce);
   p.beta = p.alpha + pad((size_t)n * 4);
   p.columns = p.beta + pad((size_t)n * 4);
   p.value = p.columns + pad((size_t)n * 4);
-  p.clean = p.value + pad((size_t)n * k * 4);
-  p.bytes = p.clean + (trainable ? (size_t)n * d * elem : staged);
+  p.halves = p.value + pad((size_t)n * k * 4);
+  p.clean = p.halves + (g_rows > n ? pad((size_t)g_rows * d * 4) : 0);
+  p.bytes = p.clean + (trainable ? (size_t)g_rows * d * elem : staged);
   return p;
 }
 size_t mtp_score_bwd_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int64_t chunk, int64_t row_block,
                                      int32_t k, int32_t trainable) {
-  const size_t lce = mtp_lce_bwd_workspace_bytes(n, d, v, head_kind, chunk, row_block);
-  return !lce || k < 1 || k > MTP_SCORE_MAX ? 0 : score_bwd_parts(lce, n, d, k, trainable, 2, 0).bytes;
+  const int64_t rows = score_g_rows(n);
+  const size_t lce = mtp_lce_bwd_workspace_bytes(rows, d, v, head_kind, chunk, rows > n ? rows : row_block);
+  return !lce || k < 1 || k > MTP_SCORE_MAX ? 0 : score_bwd_parts(lce, n, rows, d, k, trainable, 2, 0).bytes;
 }
 static size_t staged32_bytes(int64_t d, int64_t v, int32_t head_kind) { return head_kind == MTP_HEAD_Q4_STAGED ? (size_t)v * d * 4 : 0; }
 size_t mtp_score_bwd_f32_workspace_bytes(int64_t n, int64_t d, int64_t v, int32_t head_kind, int64_t chunk, int32_t k, int32_t trainable) {
   const size_t lce = mtp_lce_bwd_f32_workspace_bytes(n, d, v, chunk);
-  return !lce || k < 1 || k > MTP_SCORE_MAX ? 0 : score_bwd_parts(lce, n, d, k, trainable, 4, staged32_bytes(d, v, head_kind)).bytes;
+  return !lce || k < 1 || k > MTP_SCORE_MAX ? 0 : score_bwd_parts(lce, n, n, d, k, trainable, 4, staged32_bytes(d, v, head_kind)).bytes;
 }
 
 }  // extern "C"
@@ -959,8 +963,10 @@ static int score_bwd(int f32, const void* hidden, const void* w, const void* w_t
   if (row_block < n && (f32 || row_block < 0 || row_block % kTile))
     return fail(MTP_ERR_INPUT, "row_block must be 0, >= n, or (bf16) a positive multiple of 256 (got %lld)", (long long)row_block);
   if (d_w && row_block < n) return fail(MTP_ERR_INPUT, "a trainable head (d_w) sums over every row: row_block must cover all n=%lld rows", (long long)n);
-  const size_t lce = f32 ? mtp_lce_bwd_f32_workspace_bytes(n, d, v, chunk) : mtp_lce_bwd_workspace_bytes(n, d, v, head_kind, chunk, row_block);
-  const ScoreBwd parts = score_bwd_parts(lce, n, d, k, d_w != nullptr, f32 ? 4 : 2, f32 ? staged32_bytes(d, v, head_kind) : 0);
+  const int64_t g_rows = f32 ? n : score_g_rows(n);
+  if (g_rows > n) row_block = g_rows;  // (all rows in one block)
+  const size_t lce = f32 ? mtp_lce_bwd_f32_workspace_bytes(n, d, v, chunk) : mtp_lce_bwd_workspace_bytes(g_rows, d, v, head_kind, chunk, row_block);
+  const ScoreBwd parts = score_bwd_parts(lce, n, g_rows, d, k, d_w != nullptr, f32 ? 4 : 2, f32 ? staged32_bytes(d, v, head_kind) : 0);
   if (!workspace || workspace_bytes < parts.bytes)
     return fail(MTP_ERR_WORKSPACE, "the backward needs a workspace of %zu bytes at chunk=%lld, row_block=%lld (got %zu)", parts.bytes, (long long)chunk, (long long)row_block, workspace ? workspace_bytes : (size_t)0);
   if (!aligned16(workspace)) return fail(MTP_ERR_UNSUPPORTED, "workspace must be 16-byte aligned");
@@ -969,13 +975,14 @@ static int score_bwd(int f32, const void* hidden, const void* w, const void* w_t
   float* beta = reinterpret_cast<float*>(ws + parts.beta);
   int* own_columns = reinterpret_cast<int*>(ws + parts.columns);
   float* value = reinterpret_cast<float*>(ws + parts.value);
+  float* halves = logits && g_rows > n ? reinterpret_cast<float*>(ws + parts.halves) : nullptr;
   bool has_beta = false;
   hipError_t e = factors(alpha, beta, own_columns, value, &has_beta);
   if (e == hipSuccess && d_w)
-    e = mtp::launch_clean_rows(hidden, alpha, has_beta ? beta : nullptr, (long)n, (long)d * (f32 ? 4 : 2), ws + parts.clean, stream);
+    e = mtp::launch_clean_rows(hidden, alpha, has_beta ? beta : nullptr, (long)n, (long)d * (f32 ? 4 : 2), halves ? 2 : 1, ws + parts.clean, stream);
   if (e == hipSuccess) {
     const float inv_t = (float)(1.0 / temperature);
-    const mtp::AffineGrad grad{{alpha, has_beta ? beta : nullptr, 1.4426950408889634f * inv_t}, columns ? columns : own_columns, value, (int)k, logits, mtp::logits_ld((long)v), ws + parts.clean};
+    const mtp::AffineGrad grad{{alpha, has_beta ? beta : nullptr, 1.4426950408889634f * inv_t}, columns ? columns : own_columns, value, (int)k, logits, mtp::logits_ld((long)v), ws + parts.clean, halves};
     if (f32) {
       mtp::LceHead32 head = score_head(1, hidden, w, w_q, scales, biases, head_kind).h32;
       if (head_kind == MTP_HEAD_Q4_STAGED) {
@@ -989,7 +996,7 @@ static int score_bwd(int f32, const void* hidden, const void* w, const void* w_t
     } else {
       mtp::LceHead head = make_head(w, w_q, scales, biases, head_kind);
       head.wt = static_cast<const mtp::bf16_t*>(w_t);
-      mtp::bf16_t* stage = staged_kind(head_kind) ? reinterpret_cast<mtp::bf16_t*>(ws + lce_bwd_stage_offset(n, d, v, chunk, row_block)) : nullptr;
+      mtp::bf16_t* stage = staged_kind(head_kind) ? reinterpret_cast<mtp::bf16_t*>(ws + lce_bwd_stage_offset(g_rows, d, v, chunk, row_block)) : nullptr;
       e = mtp::launch_lce_bwd(head, static_cast<const mtp::bf16_t*>(hidden), nullptr, lse, nullptr, (int)n, (int)d, (int)v, 0,
                               (int)chunk, (int)row_block, static_cast<mtp::bf16_t*>(d_hidden), static_cast<mtp::bf16_t*>(d_w),
                               static_cast<mtp::bf16_t*>(workspace),

@@ -1604,18 +1604,22 @@ __global__ __launch_bounds__(256) void lce_bwd_g_fix_kernel(
 
 // Backward step 1b of an affine gradient, one wave per row of the chunk's G: the columns past the chunk's last vocab row
 // are set to zero, and the row's listed columns (column < 0: none) to their whole gradient, rounded once. No column is listed
-// twice in a row.
+// twice in a row. rest_rows: rows behind it that what rounding leaves goes to (AffineGrad's halves), or 0.
 __global__ __launch_bounds__(256) void lce_bwd_g_columns_kernel(const int* __restrict__ columns,
                                                                 const float* __restrict__ value, int k, int N, int vlim,
-                                                                int v_begin, int kc, int ldg, bf16_t* __restrict__ G) {
+                                                                int v_begin, int kc, int ldg, int rest_rows, bf16_t* __restrict__ G) {
   const int lane = threadIdx.x & 63;
   const int t = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (t >= N) return;
   bf16_t* row = G + (long)t * ldg;
-  for (int c = vlim - v_begin + lane; c < kc; c += 64) row[c] = 0;
+  bf16_t* rest = row + (long)rest_rows * ldg;
+  for (int c = vlim - v_begin + lane; c < kc; c += 64) row[c] = 0;  // (rest has them)
   for (int i = lane; i < k; i += 64) {
     const int y = columns[(long)t * k + i];
-    if (y >= v_begin && y < vlim) row[y - v_begin] = __builtin_bit_cast(bf16_t, (__bf16)value[(long)t * k + i]);
+    if (y < v_begin || y >= vlim) continue;
+    const float g = value[(long)t * k + i];
+    row[y - v_begin] = __builtin_bit_cast(bf16_t, (__bf16)g);
+    if (rest_rows) rest[y - v_begin] = __builtin_bit_cast(bf16_t, (__bf16)bf16_rest(g));
   }
 }
 
@@ -2318,6 +2322,9 @@ static hipError_t lce_bwd_rows(const LceHead& h, const bf16_t* H, const int64_t*
   const int ldt = (int)lce_head_t_ld(V);
   dim3 block(kThreads);
   const bool kept = affine && affine->z;  // the forward's logits: no product for the gradient tiles
+  float* halves = kept ? affine->halves : nullptr;
+  float* acc = halves ? halves : acc32;
+  const int GN = halves ? 2 * N : N, gtiles = (GN + kTile - 1) / kTile;  // rows of G, and their tiles
   for (int c = 0; c < nchunks; ++c) {
     const int vb = c * chunk;
     const int ve = (vb + chunk < V) ? vb + chunk : V;
@@ -2382,41 +2389,42 @@ static hipError_t lce_bwd_rows(const LceHead& h, const bf16_t* H, const int64_t*
     if (e != hipSuccess) return e;
     if (affine) {
       hipLaunchKernelGGL(lce_bwd_g_columns_kernel, dim3((N + 3) / 4), dim3(256), 0, stream, affine->columns, affine->value,
-                         affine->k, N, ve, vb, ctiles * kTile, ldg, Gbuf);
+                         affine->k, N, ve, vb, ctiles * kTile, ldg, halves ? N : 0, Gbuf);
       e = hipGetLastError();
       if (e != hipSuccess) return e;
     }
     int mode;
-    if (nchunks == 1) mode = 3;
+    if (halves) mode = c == 0 ? 0 : 1;
+    else if (nchunks == 1) mode = 3;
     else if (c == 0) mode = 0;
     else if (c == nchunks - 1) mode = 2;
     else mode = 1;
-    const int ks = lce_dh_ksplit(N, D, ctiles);
-    if (wt != nullptr && D % kBK == 0 && lce_dh_small(N, D, ctiles, ks)) {
-      const int wgs = (N + kSmallTile - 1) / kSmallTile * (D / kSmallTile);
-      hipLaunchKernelGGL(lce_bwd_dh_small_kernel, dim3(wgs), block, 0, stream, Gbuf, ldg, ctiles * kTile, wt, ldw, tcol0, N, D,
-                         acc32, dH, mode);
+    const int ks = lce_dh_ksplit(GN, D, ctiles);
+    if (wt != nullptr && D % kBK == 0 && lce_dh_small(GN, D, ctiles, ks)) {
+      const int wgs = (GN + kSmallTile - 1) / kSmallTile * (D / kSmallTile);
+      hipLaunchKernelGGL(lce_bwd_dh_small_kernel, dim3(wgs), block, 0, stream, Gbuf, ldg, ctiles * kTile, wt, ldw, tcol0, GN, D,
+                         acc, dH, mode);
       e = hipGetLastError();
       if (e != hipSuccess) return e;
     } else {
-      const int sa = ks > 1 ? lce_dh_split_a(rtiles, dtiles) : 0;
-      dim3 hgrid(8 * rtiles * ((dtiles + 7) / 8));
+      const int sa = ks > 1 ? lce_dh_split_a(gtiles, dtiles) : 0;
+      dim3 hgrid(8 * gtiles * ((dtiles + 7) / 8));
       if (ks > 1) {
-        const int blocks = sa ? (rtiles / sa) * (dtiles / (32 / sa)) * ks : 0;
-        hgrid = dim3(sa ? (blocks + 7) / 8 * 256 : rtiles * dtiles * ks);
+        const int blocks = sa ? (gtiles / sa) * (dtiles / (32 / sa)) * ks : 0;
+        hgrid = dim3(sa ? (blocks + 7) / 8 * 256 : gtiles * dtiles * ks);
       }
       if (h.q4) {
         hipLaunchKernelGGL(lce_bwd_dh_kernel<1>, hgrid, block, 0, stream, Gbuf, ldg, ctiles * kTile, h.w, wt, ldw,
-                           tcol0, h.wq, h.sc, h.bi, N, D, V, vb, ve, acc32, dH, mode, ks, sa, parts);
+                           tcol0, h.wq, h.sc, h.bi, GN, D, V, vb, ve, acc, dH, mode, ks, sa, parts);
       } else {
         hipLaunchKernelGGL(lce_bwd_dh_kernel<0>, hgrid, block, 0, stream, Gbuf, ldg, ctiles * kTile, h.w, wt, ldw,
-                           tcol0, h.wq, h.sc, h.bi, N, D, V, vb, ve, acc32, dH, mode, ks, sa, parts);
+                           tcol0, h.wq, h.sc, h.bi, GN, D, V, vb, ve, acc, dH, mode, ks, sa, parts);
       }
       e = hipGetLastError();
       if (e != hipSuccess) return e;
       if (ks > 1) {
-        hipLaunchKernelGGL(lce_bwd_dh_reduce_kernel, dim3(rtiles * dtiles * 64), dim3(256), 0, stream, parts, ks, N, D,
-                           acc32, dH, mode);
+        hipLaunchKernelGGL(lce_bwd_dh_reduce_kernel, dim3(gtiles * dtiles * 64), dim3(256), 0, stream, parts, ks, GN, D,
+                           acc, dH, mode);
         e = hipGetLastError();
         if (e != hipSuccess) return e;
       }
@@ -2424,12 +2432,12 @@ static hipError_t lce_bwd_rows(const LceHead& h, const bf16_t* H, const int64_t*
     if (dW != nullptr && !h.q4) {
       dim3 wgrid(dtiles % 8 == 0 ? ctiles * dtiles : 8 * dtiles * ((ctiles + 7) / 8));
       const bf16_t* rows = affine ? static_cast<const bf16_t*>(affine->clean) : H;
-      hipLaunchKernelGGL(lce_bwd_dw_kernel, wgrid, block, 0, stream, Gbuf, ldg, rows, N, D, V, vb, ve, ctiles, dW);
+      hipLaunchKernelGGL(lce_bwd_dw_kernel, wgrid, block, 0, stream, Gbuf, ldg, rows, GN, D, V, vb, ve, ctiles, dW);
       e = hipGetLastError();
       if (e != hipSuccess) return e;
     }
   }
-  return hipSuccess;
+  return halves ? launch_join_halves(halves, (long)N * D, dH, stream) : hipSuccess;
 }
 
 // The backward in blocks of row_block rows (a multiple of 256): each block's gradient tiles reuse

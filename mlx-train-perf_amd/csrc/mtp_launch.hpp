@@ -95,6 +95,10 @@ struct AffineGrad {
   const float* z;        // [N][ldz] the logits that a forward kept, or null: they are formed again
   long ldz;
   const void* clean;     // for dW: the hidden states with the rows that get zeros cleared (bf16; fp32 in the fp32 backward)
+  // With z, bf16: fp32 [2 N][D], or null. A gradient then is two bf16 numbers, its rounding and what that leaves, in rows t and N + t of
+  // G (and clean holds the hidden states twice): the products' rows up to a tile cost nothing (steps of 5 to 75 tokens take the same time),
+  // and dH is off by its own rounding alone: 5 x 64 x 997, lists of 4: 1.7e-3 of the norm, with one number 2.6e-3.
+  float* halves;
 };
 
 // affine: that gradient in the place of the loss's (targets, dnll unused).
@@ -255,12 +259,14 @@ hipError_t launch_logprobs_coef(const float* d_logprobs, const float* d_entropy,
 // Gradient tiles from kept logits, columns [v_begin, v_begin + cols) (zeros from vlim on; cols a multiple of 8, fp32: of 4).
 hipError_t launch_affine_tiles(const AffineGrad& a, const float* lse, long n, int v_begin, int vlim, int cols, long ldg, bf16_t* g,
                                hipStream_t stream);
+// dH = the sum of its halves.
+hipError_t launch_join_halves(const float* halves, long count, bf16_t* dH, hipStream_t stream);
 hipError_t launch_affine_tiles(const AffineGrad& a, const float* lse, long n, int v_begin, int vlim, int cols, long ldg, float* g,
                                hipStream_t stream);
 hipError_t launch_distill_coef(const float* d_loss, int per_row, const float* scale, const float* rest, const float* coef,
                                long n, int k, float* alpha, float* value, hipStream_t stream);
 // Hidden states with the rows whose factors are both 0 cleared; row_bytes a multiple of 4.
-hipError_t launch_clean_rows(const void* hidden, const float* alpha, const float* beta, long n, long row_bytes, void* out,
+hipError_t launch_clean_rows(const void* hidden, const float* alpha, const float* beta, long n, long row_bytes, int copies, void* out,
                              hipStream_t stream);
 
 // Preference and policy losses (preference_kernels.hip).

@@ -199,7 +199,7 @@ __device__ __forceinline__ uint32_t pick_few(const uint32_t* key, int M, int K, 
 // flight a wave, 8 KiB of a dense head, 4 of a 4-bit one), the tokens' slab (NB blocks of 32) through LDS, one barrier a
 // slab. The registers and, up to 16 tokens, the LDS leave room for 5 workgroups a CU: all 1187 groups of 151936 run at once
 // (16 tokens over a 4-bit head, 4 workgroups and 5: 157 and 130 us). 4096 x 151936: a dense head's 1.24 GB in 245 us (5.1 TB/s, as
-// a library product of one row), a 4-bit head's 0.39 GB in 104, where the vector units are busy for some 60.
+// a library product of one row), a 4-bit head's 0.35 GB in 104, where the vector units are busy for some 60.
 // ------------------------------------------------------------------------------------------
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base, long bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, bytes > 0x7fffffffL ? 0x7fffffff : (int)bytes, 0x00020000);
@@ -426,8 +426,8 @@ void lce_few_kernel(const T* __restrict__ H, const T* __restrict__ W, const uint
 
 // ------------------------------------------------------------------------------------------
 // The logits of a gather (GatherPlan): C[v][entry] = W_v . H_token, 128 x 128 a workgroup (4 waves of 64 x 64), 64-deep stages
-// through registers, a stage ahead. Bound by the hidden rows it fetches again for every entry (2 D bytes each, out of L2 and
-// the last-level cache).
+// through registers, a stage ahead. Bound by what it fetches again: the head once (nearly every group is wanted by some token) and
+// the hidden rows for every entry (2 D bytes each). 8 of 8192 x 4096 x 151936: 346 us, 250 of them the head's bytes.
 // ------------------------------------------------------------------------------------------
 template <int Q4>
 __global__ __launch_bounds__(256) void lce_gather_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
@@ -627,7 +627,8 @@ __global__ __launch_bounds__(256) void sort_lists_kernel(const int64_t* __restri
 
 // ------------------------------------------------------------------------------------------
 // Scoring, per token: the statistics of its row, the target's log probability, the groups to look into (and, where the logits
-// were kept, the alternatives themselves). One workgroup a token.
+// were kept, the alternatives themselves). One workgroup a token: bound by the barriers of the choice where there are few tokens (13 us
+// for 16 x 151936, 19 for 20 alternatives of one), by its vector instructions where there are many (8192: 60).
 // ------------------------------------------------------------------------------------------
 // Partials of one row: value i at base[i * stride]. m: of x in the log2 domain, or (few tokens) of z, times c2.
 struct RowParts {
@@ -776,7 +777,8 @@ __global__ __launch_bounds__(kPick) void score_top_kernel(const float* __restric
 //   reverse  sum q log(q / t) + R log(R / T):        f = log(q / t),          f_R = log(R / T)
 //   jsd      b KL(t | m) + (1 - b) KL(q | m), m = b t + (1 - b) q:  f = (1 - b) log(q / m), f_R = (1 - b) log(R / m_R)
 // the gradient by a logit is p (f_R - F) off the list and q (f - F) on it, F = sum q f + R f_R. R and T (but in F) are at least
-// kTailFloor. All of it in 64 bits: what the list leaves of 1 is a difference, and the products above are what take the time.
+// kTailFloor. All of it in 64 bits: what the list leaves of 1 is a difference, and the products above are what take the time
+// (8192 lists of 64: 14 us, their sorting 38, the products 21.6 ms).
 // ------------------------------------------------------------------------------------------
 __device__ __forceinline__ double wave_sum64(double v) {
 #pragma unroll
@@ -1009,11 +1011,12 @@ __global__ __launch_bounds__(256) void distill_coef_kernel(const float* __restri
 }
 
 // G = p (alpha + beta z) from kept logits, a row a blockIdx.y, 16 bytes a thread; bound by reading z and writing G (AffineGrad's
-// listed columns follow).
+// listed columns follow). rest: what rounding leaves (AffineGrad's halves), or null. 1023 x 32000, bf16: 36 us, and with it the step of a
+// 4-bit head at 2048 dims 488 -> 407.
 template <class G>
 __global__ __launch_bounds__(256) void affine_tiles_kernel(const float* __restrict__ Z, long ldz, const float* __restrict__ lse,
                                                            AffineRows rows, int v_begin, int vlim, int cols, long ldg,
-                                                           G* __restrict__ out) {
+                                                           G* __restrict__ out, G* __restrict__ rest) {
   constexpr int kEach = 16 / (int)sizeof(G);
   const long t = blockIdx.y;
   const int c = (blockIdx.x * 256 + threadIdx.x) * kEach, v = v_begin + c;
@@ -1031,6 +1034,11 @@ __global__ __launch_bounds__(256) void affine_tiles_kernel(const float* __restri
   if constexpr (sizeof(G) == 2) {
     *reinterpret_cast<u32x4*>(out + t * ldg + c) =
         u32x4{pack_bf16x2(g[0], g[1]), pack_bf16x2(g[2], g[3]), pack_bf16x2(g[4], g[5]), pack_bf16x2(g[6], g[7])};
+    if (!rest) return;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) g[i] = bf16_rest(g[i]);
+    *reinterpret_cast<u32x4*>(rest + t * ldg + c) =
+        u32x4{pack_bf16x2(g[0], g[1]), pack_bf16x2(g[2], g[3]), pack_bf16x2(g[4], g[5]), pack_bf16x2(g[6], g[7])};
   } else {
     *reinterpret_cast<f32x4*>(out + t * ldg + c) = f32x4{g[0], g[1], g[2], g[3]};
   }
@@ -1038,11 +1046,19 @@ __global__ __launch_bounds__(256) void affine_tiles_kernel(const float* __restri
 
 // A row whose factors are both 0 gets no gradient and may hold anything, NaN too: in dW = G^T H its zeros would meet that.
 __global__ __launch_bounds__(256) void clean_rows_kernel(const uint32_t* __restrict__ h, const float* __restrict__ alpha,
-                                                         const float* __restrict__ beta, long row_words,
+                                                         const float* __restrict__ beta, long row_words, int copies,
                                                          uint32_t* __restrict__ out) {
-  const long t = blockIdx.x;
+  const long t = blockIdx.x, all = gridDim.x * row_words;
   const bool live = alpha[t] != 0.f || (beta && beta[t] != 0.f);
-  for (long i = threadIdx.x; i < row_words; i += 256) out[t * row_words + i] = live ? h[t * row_words + i] : 0u;
+  for (long i = threadIdx.x; i < row_words; i += 256) {
+    const uint32_t x = live ? h[t * row_words + i] : 0u;
+    for (int c = 0; c < copies; ++c) out[c * all + t * row_words + i] = x;
+  }
+}
+
+__global__ __launch_bounds__(256) void join_halves_kernel(const float* __restrict__ halves, long count, bf16_t* __restrict__ dH) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i < count) dH[i] = __builtin_bit_cast(bf16_t, (__bf16)(halves[i] + halves[count + i]));
 }
 
 // ------------------------------------------------------------------------------------------
@@ -1349,7 +1365,7 @@ hipError_t affine_tiles(const AffineGrad& a, const float* lse, long n, int v_beg
     r.alpha += r0;
     if (r.beta) r.beta += r0;
     hipLaunchKernelGGL(affine_tiles_kernel<G>, dim3((unsigned)ceil_div(cols, 256 * each), (unsigned)rows), dim3(256), 0, st, a.z + r0 * a.ldz,
-                       a.ldz, lse + r0, r, v_begin, vlim, cols, ldg, g + r0 * ldg);
+                       a.ldz, lse + r0, r, v_begin, vlim, cols, ldg, g + r0 * ldg, a.halves ? g + (n + r0) * ldg : nullptr);
     MTP_LAUNCHED();
   }
   return hipSuccess;
@@ -1370,10 +1386,15 @@ hipError_t launch_distill_coef(const float* d_loss, int per_row, const float* sc
   return hipGetLastError();
 }
 
-hipError_t launch_clean_rows(const void* hidden, const float* alpha, const float* beta, long n, long row_bytes, void* out,
+hipError_t launch_join_halves(const float* halves, long count, bf16_t* dH, hipStream_t st) {
+  hipLaunchKernelGGL(join_halves_kernel, dim3((unsigned)ceil_div(count, 256)), dim3(256), 0, st, halves, count, dH);
+  return hipGetLastError();
+}
+
+hipError_t launch_clean_rows(const void* hidden, const float* alpha, const float* beta, long n, long row_bytes, int copies, void* out,
                              hipStream_t st) {
   hipLaunchKernelGGL(clean_rows_kernel, dim3((unsigned)n), dim3(256), 0, st, static_cast<const uint32_t*>(hidden), alpha, beta,
-                     row_bytes / 4, static_cast<uint32_t*>(out));
+                     row_bytes / 4, copies, static_cast<uint32_t*>(out));
   return hipGetLastError();
 }
 

@@ -154,17 +154,19 @@ def jsd(t, q, beta):
     return beta * kl(t, m) + (1 - beta) * kl(q, m)
 
 
-def gradient_bounds(g, p, extra, hidden, w, want_dw, dtype):
+def gradient_bounds(g, p, extra, hidden, w, want_dw, dtype, halves):
     """(dL/dhidden, its bound, dL/dw, its bound) of a gradient g by the logits with the probabilities p; extra: the size of what
-    its factors are made of, per row."""
+    its factors are made of, per row. halves: g goes into the products as two bf16 numbers, so half a step of the second, which is at
+    most half a step of the first, is lost."""
     n, v = g.shape
-    off = (stat(v) + 512 * U) * (p * extra[:, None]) + (stat(v) + 512 * U) * g.abs() + (R if dtype == "bf16" else U) * g.abs()
+    off = (stat(v) + 512 * U) * (p * extra[:, None]) + (stat(v) + 512 * U) * g.abs()
+    off = off + ((R * R if halves else R) if dtype == "bf16" else U) * g.abs()
     half = R if dtype == "bf16" else U
     dh, dh_sum = g @ w, g.abs() @ w.abs()
     out = [dh, off @ w.abs() + v * U * dh_sum + half * dh.abs() + 1e-12]
     if want_dw:
         dw, dw_sum = g.T @ hidden, g.abs().T @ hidden.abs()
-        out += [dw, off.T @ hidden.abs() + n * U * dw_sum + half * dw.abs() + 1e-12]
+        out += [dw, off.T @ hidden.abs() + (2 * n if halves else n) * U * dw_sum + half * dw.abs() + 1e-12]
     else:
         out += [None, None]
     return out

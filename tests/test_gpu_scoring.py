@@ -23,7 +23,7 @@ def _targets(n, v, seed, ignored=True):
     return y
 
 
-def _check_score(n, d, v, *, top=0, head="dense", dtype="bf16", temperature=1.0, targets=True, seed=0, grads=True):
+def _check_score(n, d, v, *, top=0, head="dense", dtype="bf16", temperature=1.0, targets=True, seed=0, grads=True, halves=None):
     hidden, hd, w = S.make(n, d, v, head=head, dtype=dtype, seed=seed)
     y = _targets(n, v, seed) if targets else None
     live = torch.ones(n, dtype=torch.bool) if y is None else y != -100
@@ -55,14 +55,14 @@ def _check_score(n, d, v, *, top=0, head="dense", dtype="bf16", temperature=1.0,
     p = torch.softmax(z.detach() / temperature, 1)
     extra = (a.abs() + 64 * b.abs()).double() / temperature
     clean = torch.where(live[:, None], hidden.double(), 0.0)
-    dh, dh_off, dw, dw_off = S.gradient_bounds(gz, p, extra, clean, w, want_dw, dtype)
+    dh, dh_off, dw, dw_off = S.gradient_bounds(gz, p, extra, clean, w, want_dw, dtype, n <= 128 if halves is None else halves)
     S.within(grad[0], dh, dh_off, "d_hidden")
     if want_dw:
         S.within(grad[1], dw, dw_off, "d_weight")
 
 
 def _check_distill(n, d, v, k, *, head="dense", dtype="bf16", kind="forward", renormalize=False, reduction="mean", temperature=1.0,
-                   beta=0.4, seed=0, holes=True):
+                   beta=0.4, seed=0, holes=True, halves=None):
     hidden, hd, w = S.make(n, d, v, head=head, dtype=dtype, seed=seed)
     ids, lp, mask = S.teacher_list(n, v, k, seed=seed, renormalize=renormalize, holes=holes)
     args = {"kind": kind, "beta": beta, "temperature": temperature, "renormalize": renormalize, "reduction": reduction}
@@ -91,7 +91,7 @@ def _check_distill(n, d, v, k, *, head="dense", dtype="bf16", kind="forward", re
     scale = ct.abs() if reduction == "none" else ct.abs() / (max(1, int(live.sum())) if reduction == "mean" else 1)
     extra = (scale * torch.ones(n, dtype=torch.float64)) * (64 + 2 / left) / temperature
     clean = torch.where(live[:, None], hidden.double(), 0.0)
-    dh, dh_off, dw, dw_off = S.gradient_bounds(gz, q, extra, clean, w, want_dw, dtype)
+    dh, dh_off, dw, dw_off = S.gradient_bounds(gz, q, extra, clean, w, want_dw, dtype, n <= 128 if halves is None else halves)
     S.within(grad[0], dh, dh_off, "d_hidden")
     assert bool((grad[0].cpu()[~live] == 0).all())
     if want_dw:
@@ -407,8 +407,20 @@ _FORMED_AGAIN = [(5, 64, 97, 4, "dense", "bf16"), (300, 128, 1000, 20, "trainabl
 @pytest.mark.parametrize(("n", "d", "v", "k", "head", "dtype"), _FORMED_AGAIN)
 def test_gradients_of_logits_formed_again(n, d, v, k, head, dtype, monkeypatch):
     monkeypatch.setattr(scoring, "_kept_bytes", lambda x: 0)
-    _check_score(n, d, v, top=k, head=head, dtype=dtype)
-    _check_distill(n, d, v, k, head=head, dtype=dtype)
+    _check_score(n, d, v, top=k, head=head, dtype=dtype, halves=False)
+    _check_distill(n, d, v, k, head=head, dtype=dtype, halves=False)
+
+
+@pytest.mark.parametrize(("n", "d", "head"), [(5, 512, "dense"), (5, 512, "trainable"), (32, 512, "q4"), (129, 1536, "trainable")])
+def test_gradients_of_kept_logits_by_vocabulary_chunks(n, d, head, monkeypatch):
+    """A budget of six times the kept logits, which the staged head's chunks and the gradient tiles overrun: several chunks."""
+    v = 6000
+    budget = 6 * n * 6016 * 4
+    assert 2 * (n + d) * v > budget
+    monkeypatch.setenv("MTP_LCE_BWD_BUDGET", str(budget))
+    monkeypatch.setenv("MTP_LCE_TRANSPOSED_HEAD", "0")
+    _check_score(n, d, v, top=4, head=head)
+    _check_distill(n, d, v, 20, head=head)
 
 
 def test_which_logits_a_forward_keeps(monkeypatch):
@@ -464,7 +476,7 @@ def test_a_policy_step_with_an_entropy_bonus():
     want = policy_loss(-lp.view(4, -1), old.double().cpu(), adv.double().cpu(), impl="reference").loss - 0.01 * ent.mean()
     (gz,) = torch.autograd.grad(want, z)
     p = torch.softmax(z.detach(), 1)
-    dh, off, _, _ = S.gradient_bounds(gz, p, torch.full((n,), 64.0 / n, dtype=torch.float64), hidden.double(), w, False, "bf16")
+    dh, off, _, _ = S.gradient_bounds(gz, p, torch.full((n,), 64.0 / n, dtype=torch.float64), hidden.double(), w, False, "bf16", n <= 128)
     S.within(got, dh, off, "d_hidden")
 
 
