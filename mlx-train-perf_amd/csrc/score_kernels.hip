@@ -40,8 +40,12 @@ struct PickScratch {
   int4 count[2][kPick / 64];
   int sum[kPick / 64], listed;
   uint32_t least, top[kPick];
-  int list[kRanked], rank[kRanked];
+  uint64_t list[kRanked];  // keys and their positions, as one number that falls in the order of choice
+  int rank[kRanked];
 };
+__device__ __forceinline__ uint64_t entry_of(uint32_t key, int at) { return (uint64_t)key << 32 | (uint32_t)~at; }
+__device__ __forceinline__ uint32_t entry_key(uint64_t e) { return (uint32_t)(e >> 32); }
+__device__ __forceinline__ int entry_at(uint64_t e) { return (int)~(uint32_t)e; }
 
 // Sum over the threads before this one.
 __device__ __forceinline__ int block_before(int mine, PickScratch& s) {
@@ -99,10 +103,10 @@ __device__ __forceinline__ uint32_t kth_largest(const uint32_t (&key)[R], int K,
   return least;
 }
 
-// The positions, ascending, of the K largest of M >= K keys in LDS; equal keys go to the lower position. Ends with a barrier.
-// R: at least M / kPick. Returns the K-th largest.
-template <int R>
-__device__ __forceinline__ uint32_t pick_largest(const uint32_t* key, int M, int K, int* at, PickScratch& s) {
+// The K largest of M >= K keys in LDS, their positions ascending: put(place, position). Equal keys go to the lower position. Ends with
+// a barrier. R: at least M / kPick. Returns the K-th largest.
+template <int R, class PUT>
+__device__ __forceinline__ uint32_t pick_largest(const uint32_t* key, int M, int K, const PUT& put, PickScratch& s) {
   const int tid = threadIdx.x;
   uint32_t mine_keys[R];
 #pragma unroll
@@ -121,7 +125,7 @@ __device__ __forceinline__ uint32_t pick_largest(const uint32_t* key, int M, int
   }
   int to = block_before(taken, s);
   for (int i = lo; i < hi; ++i)
-    if (key[i] > least || (key[i] == least && seen++ < equal)) at[to++] = i;
+    if (key[i] > least || (key[i] == least && seen++ < equal)) put(to++, i);
   __syncthreads();
   return least;
 }
@@ -138,27 +142,23 @@ __device__ __forceinline__ int list_from(const uint32_t* key, int M, uint32_t le
     int first = 0;
     if (lane == 0 && who) first = atomicAdd(&s.listed, __popcll(who));
     first = __builtin_amdgcn_readfirstlane(first) + __popcll(who & ((1ull << lane) - 1));
-    if (in && first < kRanked) s.list[first] = i;
+    if (in && first < kRanked) s.list[first] = entry_of(key[i], i);
   }
   __syncthreads();
   return s.listed;
 }
-// How many of the n listed keys come before the i-th listed: larger ones, and equal ones of a lower position.
-__device__ __forceinline__ int rank_of(const uint32_t* key, int i, int n, const PickScratch& s) {
-  const int p = s.list[i];
-  const uint32_t mine = key[p];
+// How many of the n listed come before `mine`.
+__device__ __forceinline__ int rank_of(uint64_t mine, int n, const PickScratch& s) {
   int rank = 0;
-  for (int j = 0; j < n; ++j) {
-    const int o = s.list[j];
-    const uint32_t other = key[o];
-    rank += other > mine || (other == mine && o < p);
-  }
+#pragma unroll 8
+  for (int j = 0; j < n; ++j) rank += s.list[j] > mine;
   return rank;
 }
 
 // pick_largest for keys that mostly differ. The K-th largest of the 256 threads' own maxima is at most the K-th largest key, and
 // mostly few more than K keys reach it (every wave finds it by itself, from four of them a lane: no barriers); those are put in
-// order by counting. 1187 keys, 8 of them: 8192 rows 95 us with 16 counts over all keys, now 61.
+// order by counting. 1187 keys, 8 of them: 8192 rows 95 us with 16 counts over all keys, then 61, and 51 with
+// a key and its position as one number to compare.
 template <int R>
 __device__ __forceinline__ uint32_t pick_few(const uint32_t* key, int M, int K, int* at, PickScratch& s) {
   const int tid = threadIdx.x, lane = tid & 63;
@@ -178,15 +178,17 @@ __device__ __forceinline__ uint32_t pick_few(const uint32_t* key, int M, int K, 
     if (n >= K) least |= 1u << b;
   }
   const int n = list_from(key, M, least, s);
-  if (n > kRanked) return pick_largest<R>(key, M, K, at, s);
-  for (int i = tid; i < n; i += kPick) s.rank[i] = rank_of(key, i, n, s);
+  if (n > kRanked) return pick_largest<R>(key, M, K, [&](int place, int i) { at[place] = i; }, s);
+  for (int i = tid; i < n; i += kPick) s.rank[i] = rank_of(s.list[i], n, s);
   __syncthreads();
   for (int i = tid; i < n; i += kPick) {
     if (s.rank[i] >= K) continue;
-    if (s.rank[i] == K - 1) s.least = key[s.list[i]];
+    const int p = entry_at(s.list[i]);
+    if (s.rank[i] == K - 1) s.least = entry_key(s.list[i]);
     int place = 0;
-    for (int j = 0; j < n; ++j) place += s.rank[j] < K && s.list[j] < s.list[i];
-    at[place] = s.list[i];
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) place += s.rank[j] < K && entry_at(s.list[j]) < p;
+    at[place] = p;
   }
   __syncthreads();
   return s.least;
@@ -627,8 +629,8 @@ __global__ __launch_bounds__(256) void sort_lists_kernel(const int64_t* __restri
 
 // ------------------------------------------------------------------------------------------
 // Scoring, per token: the statistics of its row, the target's log probability, the groups to look into (and, where the logits
-// were kept, the alternatives themselves). One workgroup a token: bound by the barriers of the choice where there are few tokens (13 us
-// for 16 x 151936, 19 for 20 alternatives of one), by its vector instructions where there are many (8192: 60).
+// were kept, the alternatives themselves). One workgroup a token: bound by the chain of loads, barriers and counts where there are few tokens (12 us
+// for 16 x 151936, 17 for 20 alternatives of one), by its vector instructions where there are many (8192: 51).
 // ------------------------------------------------------------------------------------------
 // Partials of one row: value i at base[i * stride]. m: of x in the log2 domain, or (few tokens) of z, times c2.
 struct RowParts {
@@ -638,15 +640,27 @@ struct RowParts {
   float m_scale;
 };
 
+// put(i, load(i)) for i < n, one i a thread and step, the loads of B steps in flight at once.
+template <int B, class LOAD, class PUT>
+__device__ __forceinline__ void each(int n, const LOAD& load, const PUT& put) {
+  for (int base = threadIdx.x; base < n; base += B * kPick) {
+    decltype(load(0)) x[B];
+#pragma unroll
+    for (int b = 0; b < B; ++b) x[b] = load(base + b * kPick < n ? base + b * kPick : n - 1);
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+      if (base + b * kPick < n) put(base + b * kPick, x[b]);
+  }
+}
+
 // (m, s, u) of a row, in every thread of the workgroup.
 __device__ __forceinline__ void merge_row(const RowParts& p, long t, float& m, float& s, float& u, float (&x)[3][kPick / 64]) {
   m = kNegInf;
   s = u = 0.f;
   const float *pm = p.m + t * p.row, *ps = p.s + t * p.row, *pu = p.u + t * p.row;
-  for (int i = threadIdx.x; i < p.count; i += kPick) {
-    const float mi = pm[i * p.stride];
-    lse2_merge(m, s, u, mi == kNegInf ? kNegInf : mi * p.m_scale, ps[i * p.stride], pu[i * p.stride]);
-  }
+  struct Part { float m, s, u; };
+  each<5>(p.count, [&](int i) { return Part{pm[i * p.stride], ps[i * p.stride], pu[i * p.stride]}; },
+          [&](int, const Part& x) { lse2_merge(m, s, u, x.m == kNegInf ? kNegInf : x.m * p.m_scale, x.s, x.u); });
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) {
     const float mo = __shfl_xor(m, o, 64), so = __shfl_xor(s, o, 64), uo = __shfl_xor(u, o, 64);
@@ -675,14 +689,14 @@ __device__ __forceinline__ void write_top(const uint32_t* key, const int* group,
   const int M = ngroups * kGroup;
   int n = list_from(key, M, least, s);
   if (n > kRanked || n < K) {  // many equal ones; or logits that are no numbers
-    pick_largest<MC / kPick>(key, M, K, s.list, s);
+    pick_largest<MC / kPick>(key, M, K, [&](int place, int i) { s.list[place] = entry_of(key[i], i); }, s);
     n = K;
   }
   for (int i = threadIdx.x; i < n; i += kPick) {
-    const int rank = rank_of(key, i, n, s);
+    const int rank = rank_of(s.list[i], n, s);
     if (rank >= K) continue;
-    const int p = s.list[i], id = group[p / kGroup] * kGroup + p % kGroup;
-    const float z = key_value(key[p]), lp = z * inv_t - lse;
+    const int p = entry_at(s.list[i]), id = group[p / kGroup] * kGroup + p % kGroup;
+    const float z = key_value(entry_key(s.list[i])), lp = z * inv_t - lse;
     out.top_ids[t * K + rank] = id < V ? id : -1;
     out.top_logprobs[t * K + rank] = lp;
     if (id == target) {
@@ -736,13 +750,13 @@ __global__ __launch_bounds__(kPick) void score_rows_kernel(RowParts parts, const
     }
   }
   if constexpr (MG > 0) {
-    for (int i = tid; i < ngroups; i += kPick) key[i] = order_key(gmax[t * ldg + i]);
+    each<5>(ngroups, [&](int i) { return gmax[t * ldg + i]; }, [&](int i, float x) { key[i] = order_key(x); });
     __syncthreads();
     uint32_t least = pick_few<MG / kPick>(key, ngroups, take, group, scratch);
     if (take < K) least = 0;
     if constexpr (KEPT) {
-      for (int i = tid; i < take * kGroup; i += kPick)
-        key[i] = group[i / kGroup] * kGroup + i % kGroup < V ? order_key(Z[t * ldz + (long)group[i / kGroup] * kGroup + i % kGroup]) : 0u;
+      each<5>(take * kGroup, [&](int i) { return Z[t * ldz + (long)group[i / kGroup] * kGroup + i % kGroup]; },
+              [&](int i, float x) { key[i] = group[i / kGroup] * kGroup + i % kGroup < V ? order_key(x) : 0u; });
       __syncthreads();
       write_top<MC>(key, group, take, K, least, V, inv_t, lse, t, targets ? y : -1, out, scratch);
     } else if (tid < take) {
@@ -765,7 +779,7 @@ __global__ __launch_bounds__(kPick) void score_top_kernel(const float* __restric
   const int tid = threadIdx.x;
   if (groups[t * take] < 0) return;  // an ignored token
   for (int i = tid; i < take; i += kPick) group[i] = groups[t * take + i];
-  for (int i = tid; i < take * kGroup; i += kPick) key[i] = order_key(rows[t * take * kGroup + i]);
+  each<4>(take * kGroup, [&](int i) { return rows[t * take * kGroup + i]; }, [&](int i, float x) { key[i] = order_key(x); });
   __syncthreads();
   write_top<MC>(key, group, take, K, floors[t], V, inv_t, out.lse[t], t, targets ? targets[t] : -1, out, scratch);
 }
