@@ -423,6 +423,30 @@ def test_gradients_of_kept_logits_by_vocabulary_chunks(n, d, head, monkeypatch):
     _check_distill(n, d, v, 20, head=head)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_kept_logits_of_more_rows_than_a_grid_has(dtype):
+    """A small vocabulary: 40000 tokens' logits are kept whole, and the gradient tiles take their rows in blocks."""
+    n, d, v = 40000, 64, 500
+    hidden, hd, w = S.make(n, d, v, head="trainable", dtype=dtype, seed=6)
+    hd = S.to(hd, "cuda")
+    h = hidden.cuda().requires_grad_()
+    y = torch.arange(n) % v
+    got = token_logprobs(h, hd, y.cuda())
+    z = S.logits(hidden, w, torch.ones(n, dtype=torch.bool))
+    logp = torch.log_softmax(z, 1)
+    logprobs, entropy = logp.gather(1, y[:, None])[:, 0], -(logp.exp() * logp).sum(1)
+    off = S.stat(v) + 256 * S.U
+    S.within(got.logprobs, logprobs, off, "logprobs")
+    S.within(got.entropy, entropy, off + 128 * S.stat(v), "entropy")
+    a, b = torch.randn(2, n, generator=torch.Generator().manual_seed(7))
+    (gz,) = torch.autograd.grad((logprobs * a.double() + entropy * b.double()).sum(), z)
+    grad = torch.autograd.grad((got.logprobs, got.entropy), (h, hd.weight), (a.cuda(), b.cuda()))
+    extra = (a.abs() + 64 * b.abs()).double()
+    dh, dh_off, dw, dw_off = S.gradient_bounds(gz, torch.softmax(z.detach(), 1), extra, hidden.double(), w, True, dtype, False)
+    S.within(grad[0], dh, dh_off, "d_hidden")
+    S.within(grad[1], dw, dw_off, "d_weight")
+
+
 def test_which_logits_a_forward_keeps(monkeypatch):
     hidden, hd, _ = S.make(40, 64, 300, head="dense", dtype="bf16")
     hidden, hd = hidden.cuda().requires_grad_(), S.to(hd, "cuda")
