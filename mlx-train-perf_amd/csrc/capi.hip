@@ -846,8 +846,9 @@ static int check_score_head(int f32, const void* hidden, const void* w, const ui
   return check_lce_common(hidden, w, w_q, scales, biases, &any, n, d, v, head_kind);
 }
 
+static float log2e_over(double temperature) { return (float)(1.4426950408889634 / temperature); }
 static mtp::ScoreShape score_shape(int64_t n, int64_t d, int64_t v, double temperature, int32_t head_kind) {
-  return mtp::ScoreShape{(long)n, (long)d, (long)v, (float)(1.0 / temperature), head_kind == MTP_HEAD_Q4_STAGED};
+  return mtp::ScoreShape{(long)n, (long)d, (long)v, (float)(1.0 / temperature), log2e_over(temperature), head_kind == MTP_HEAD_Q4_STAGED};
 }
 
 static bool score_sizes(int64_t n, int64_t d, int64_t v) {
@@ -981,8 +982,7 @@ static int score_bwd(int f32, const void* hidden, const void* w, const void* w_t
   if (e == hipSuccess && d_w)
     e = mtp::launch_clean_rows(hidden, alpha, has_beta ? beta : nullptr, (long)n, (long)d * (f32 ? 4 : 2), halves ? 2 : 1, ws + parts.clean, stream);
   if (e == hipSuccess) {
-    const float inv_t = (float)(1.0 / temperature);
-    const mtp::AffineGrad grad{{alpha, has_beta ? beta : nullptr, 1.4426950408889634f * inv_t}, columns ? columns : own_columns, value, (int)k, logits, mtp::logits_ld((long)v), ws + parts.clean, halves};
+    const mtp::AffineGrad grad{{alpha, has_beta ? beta : nullptr, log2e_over(temperature)}, columns ? columns : own_columns, value, (int)k, logits, mtp::logits_ld((long)v), ws + parts.clean, halves};
     if (f32) {
       mtp::LceHead32 head = score_head(1, hidden, w, w_q, scales, biases, head_kind).h32;
       if (head_kind == MTP_HEAD_Q4_STAGED) {
@@ -1079,7 +1079,7 @@ static int distill_fwd(int f32, const void* hidden, const void* w, const uint32_
   if (!aligned16(workspace)) return fail(MTP_ERR_UNSUPPORTED, "workspace must be 16-byte aligned");
   const hipError_t e = mtp::launch_distill_fwd(score_head(f32, hidden, w, w_q, scales, biases, head_kind),
                                                score_shape(n, d, v, temperature, head_kind), ids, teacher, mask,
-                                               mtp::DistillLoss{(int)k, kind, renormalize != 0, reduction, beta}, out, workspace,
+                                               mtp::DistillLoss{(int)k, kind, renormalize != 0, reduction, beta, 1.0 / temperature}, out, workspace,
                                                static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return fail(MTP_ERR_RUNTIME, "distillation launch failed: %s", hipGetErrorString(e));
   return ok();

@@ -368,15 +368,11 @@ void lce32_fwd_kernel(const float* __restrict__ H, const float* __restrict__ W,
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      float mz = kNegInf;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int v = v0 + 64 * wa + 32 * i + rrow(r, h);
-          if (v >= V) acc[i][j][r] = kHidden;
-          mz = fmaxf(mz, acc[i][j][r]);
-        }
+        for (int r = 0; r < 16; ++r)
+          if (v0 + 64 * wa + 32 * i + rrow(r, h) >= V) acc[i][j][r] = kHidden;
       if constexpr (STAT & kStatKeep) {
         const int t = t0 + 64 * wb + 32 * j + (lane & 31);
         if (t < N) {
@@ -389,6 +385,15 @@ void lce32_fwd_kernel(const float* __restrict__ H, const float* __restrict__ W,
                   f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
         }
       }
+    }
+    if constexpr (STAT & kStatList) cursor.take<kT>(list, tokens, acc, v0, 64 * wa, h);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float mz = kNegInf;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mz = fmaxf(mz, acc[i][j][r]);
       if constexpr (STAT & kStatGroups) {  // the tile's maximum of each token: of both halves of both waves
         const float both = fmaxf(mz, __shfl_xor(mz, 32, 64));
         const int tl = 64 * wb + 32 * j + (lane & 31);
@@ -413,7 +418,6 @@ void lce32_fwd_kernel(const float* __restrict__ H, const float* __restrict__ W,
       s[j] = s[j] * f + sum;
       m[j] = mn;
     }
-    if constexpr (STAT & kStatList) cursor.tile<kT>(list, tokens, acc, v0, 64 * wa, h);
   }
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
@@ -795,6 +799,7 @@ static hipError_t lce32_fwd_tiles(const LceHead32& h, const float* H, int N, int
 hipError_t launch_lce32_stats(const LceHead32& h, const float* H, int N, int D, int V, const ScoreStats& x, hipStream_t st) {
   constexpr int kEntropy = kStatScaled | kStatEntropy, kGroups = kEntropy | kStatGroups;
   if (x.z && x.gmax) return lce32_fwd_tiles<kGroups | kStatKeep>(h, H, N, D, V, x, st);
+  if (x.z && x.list.column) return lce32_fwd_tiles<kStatScaled | kStatList | kStatKeep>(h, H, N, D, V, x, st);
   if (x.z) return lce32_fwd_tiles<kEntropy | kStatKeep>(h, H, N, D, V, x, st);
   if (x.gmax) return lce32_fwd_tiles<kGroups>(h, H, N, D, V, x, st);
   if (x.u) return lce32_fwd_tiles<kEntropy>(h, H, N, D, V, x, st);

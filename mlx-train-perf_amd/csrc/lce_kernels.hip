@@ -888,8 +888,8 @@ __device__ __forceinline__ bool xcd_rect_tile(int mtiles, int ntiles, int& m, in
 //
 // STAT (mtp_launch.hpp, kStat...) is what token scoring wants beside it: the softmax of z / temperature (scale2 =
 // log2(e) / temperature), the sum of 2^(x - m) (x - m) that the entropy is made of (an fma per logit), and the maximum of
-// every group of kGroup logits, which the tile's own maximum holds already, with the logits themselves or without; or the
-// logits of a list of columns a row (ListCursor). 0 is the loss as it was.
+// every group of kGroup logits, which the tile's own maximum holds already; or the logits of a list of columns a row, which
+// then are in no statistic (ListCursor); with all logits themselves or without. 0 is the loss as it was.
 // ------------------------------------------------------------------------------------------
 template <int Q4, int STAT = 0>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
@@ -981,6 +981,7 @@ void lce_fwd_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
                 f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
       }
     }
+    if constexpr (STAT & kStatList) cursor.take<kTile>(list, tokens, acc, v0, 128 * wa, lhalf);
     // Four partial maxima and sums per token column, combined in a fixed order: four short
     // dependency chains instead of one 64 long (forward -1%).
     float pm[kNJ][4], ps[kNJ][4], pu[kNJ][4];
@@ -1031,7 +1032,6 @@ void lce_fwd_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
       s[j] = s[j] * f + sum;
       m[j] = mn[j];
     }
-    if constexpr (STAT & kStatList) cursor.tile<kTile>(list, tokens, acc, v0, 128 * wa, lhalf);
   };
 
   if (!Q4 && D % kBK == 0) {
@@ -2227,6 +2227,7 @@ hipError_t launch_lce_stats(const LceHead& h, const bf16_t* H, int N, int D, int
                             long stage_rows, hipStream_t stream) {
   constexpr int kEntropy = kStatScaled | kStatEntropy, kGroups = kEntropy | kStatGroups;
   if (x.z && x.gmax) return lce_fwd_tiles<kGroups | kStatKeep>(h, H, N, D, V, x, stage, stage_rows, stream);
+  if (x.z && x.list.column) return lce_fwd_tiles<kStatScaled | kStatList | kStatKeep>(h, H, N, D, V, x, stage, stage_rows, stream);
   if (x.z) return lce_fwd_tiles<kEntropy | kStatKeep>(h, H, N, D, V, x, stage, stage_rows, stream);
   if (x.gmax) return lce_fwd_tiles<kGroups>(h, H, N, D, V, x, stage, stage_rows, stream);
   if (x.u) return lce_fwd_tiles<kEntropy>(h, H, N, D, V, x, stage, stage_rows, stream);

@@ -59,7 +59,7 @@ hipError_t launch_lce_fwd(const LceHead& h, const bf16_t* H, const int64_t* targ
 // Token scoring (score_kernels.hip) takes the forward's tiles with more of their statistics. A forward's STAT is a sum of:
 enum { kStatScaled = 1, kStatEntropy = 2, kStatGroups = 4, kStatList = 8, kStatKeep = 16 };
 constexpr int kGroup = 128;  // consecutive logits whose maximum a forward keeps
-// Logits to keep of each row: ascending columns (kNoColumn past the last) to their places in z.
+// Logits to put away of each row: ascending columns (kNoColumn past the last) to their places in z. The statistics leave them out.
 constexpr int kNoColumn = 0x7fffffff;
 struct ScoreList {
   const int* column;  // [N][k], or null
@@ -225,7 +225,7 @@ struct ScoreHead {
 };
 struct ScoreShape {
   long n, d, v;
-  float inv_t;       // 1 / temperature
+  float inv_t, c2;   // 1 / temperature; log2(e) / temperature, rounded once: softmax(z / temperature) is that of 2^(z c2) everywhere
   int stage;         // 4-bit: dequantize the whole head into the workspace first
 };
 // logits, in a forward's outputs: [n][logits_ld(v)], which then keeps them there for its backward, or null.
@@ -241,7 +241,7 @@ hipError_t launch_logprobs_fwd(const ScoreHead& h, const ScoreShape& sh, const i
 enum { kDistillForward = 0, kDistillReverse = 1, kDistillJsd = 2 };
 struct DistillLoss {
   int k, kind, renormalize, reduction;
-  double beta;
+  double beta, inv_t;
 };
 struct DistillOut {
   float *loss, *scale;        // scale [1]: what a row's gradient is multiplied with, 1 / rows that count for a mean

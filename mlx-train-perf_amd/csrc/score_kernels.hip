@@ -9,8 +9,9 @@
 // groups with the `top` largest maxima (a logit outside them has `top` at least as large ahead of it; equal maxima go to the
 // lower group, so equal logits to the lower index). So: choose those groups, form their logits again (a product over
 // the tokens that want each group: top kGroup / V of the first one, 0.7% for 8 of 151936, in its k order and to its bits),
-// choose among them. The logits of a teacher's list, sorted first, the product's tiles put away as they pass (ListCursor): the
-// very ones that the sums hold, so that what a list leaves of 1 is exact to fp32 and not to two roundings of a large logit.
+// choose among them. The logits of a teacher's list, sorted first, the product's tiles put away as they pass (ListCursor) and
+// leave out of their sums, so that what a list leaves of 1 is a sum of its own. As a difference of 1 and the list's own
+// probabilities it was off by their last digits: 5% of 1.5e-5 at logits of 44.
 //
 // Up to kFewTokens tokens (kFewTokens32) the logits themselves are kept in the workspace (lce_few_kernel), which leaves two launches;
 // where there are not many of them (keep_logits), the product's tiles keep them too.
@@ -785,13 +786,14 @@ __global__ __launch_bounds__(kPick) void score_top_kernel(const float* __restric
 }
 
 // ------------------------------------------------------------------------------------------
-// Distillation, one wave a token, its list as it came (few tokens, with their logits Z) or sorted, with the logits picks. With q_k = p at the list's ids, R = 1 - sum q, t_k and T = 1 - sum t the teacher's, and
-// f = dL/dq but for a constant (f_R for the rest),
+// Distillation, one wave a token, its list as it came (FEW: few tokens, with their logits Z and every group's maximum and sum)
+// or sorted, with the logits picks and the partials of all others. With q_k = p at the list's ids, R the others' sum of p, t_k
+// and T = 1 - sum t the teacher's, and f = dL/dq but for a constant (f_R for the rest),
 //   forward  sum t log(t / q) + T log(T / R):        f = -t / q,              f_R = -T / R
 //   reverse  sum q log(q / t) + R log(R / T):        f = log(q / t),          f_R = log(R / T)
 //   jsd      b KL(t | m) + (1 - b) KL(q | m), m = b t + (1 - b) q:  f = (1 - b) log(q / m), f_R = (1 - b) log(R / m_R)
 // the gradient by a logit is p (f_R - F) off the list and q (f - F) on it, F = sum q f + R f_R. R and T (but in F) are at least
-// kTailFloor. All of it in 64 bits: what the list leaves of 1 is a difference, and the products above are what take the time
+// kTailFloor. From the partials on in 64 bits: T is a difference, and the products above are what take the time
 // (8192 lists of 64: 14 us, their sorting 38, the products 21.6 ms).
 // ------------------------------------------------------------------------------------------
 __device__ __forceinline__ double wave_sum64(double v) {
@@ -811,29 +813,101 @@ __device__ __forceinline__ double log_add(double a, double b) {
 
 constexpr float kLeast = 1.17549435e-38f;
 
-template <int KIND>
+// Few tokens: (base, the sum of 2^(z c2 - base)) over the columns that the wave's list `id` leaves. Groups without a listed
+// column give their sums; the others are summed again without it, two columns a lane, eight groups' loads in flight.
+struct OffList {
+  float base;
+  double sum;
+};
+struct GroupScratch {
+  uint32_t listed[kScoreVocab / kGroup / 32];  // bit g: group g has a listed column
+  uint32_t columns[kScoreTop][kGroup / 32];    // the listed columns of a group, at the slot of its first one
+  int group[kScoreTop], slot[kScoreTop];       // the groups that have some, and that slot
+};
+__device__ __forceinline__ OffList few_off_list(const RowParts& p, long t, const float* __restrict__ z, const int (&id)[kPerLane], int k,
+                                                int lane, GroupScratch& x) {
+  static_assert(kGroup == 128, "two columns a lane");
+  for (int i = lane; i < (p.count + 31) / 32; i += 64) x.listed[i] = 0u;
+  for (int i = lane; i < kScoreTop * (kGroup / 32); i += 64) x.columns[i / (kGroup / 32)][i % (kGroup / 32)] = 0u;
+  int first[kPerLane];
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) first[i] = -1;
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i)
+    for (int j = 0; j < 64 && 64 * i + j < k; ++j) {
+      const int other = __builtin_amdgcn_readlane(id[i], j);
+#pragma unroll
+      for (int o = 0; o < kPerLane; ++o)
+        if (first[o] < 0 && other >= 0 && id[o] >= 0 && other / kGroup == id[o] / kGroup) first[o] = 64 * i + j;
+    }
+  __threadfence_block();  // (the wave's own LDS)
+  int groups = 0;
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) {
+    const int g = id[i] / kGroup, c = id[i] % kGroup;
+    if (id[i] >= 0) {
+      atomicOr(&x.listed[g >> 5], 1u << (g & 31));
+      atomicOr(&x.columns[first[i]][c >> 5], 1u << (c & 31));
+    }
+    const uint64_t firsts = __ballot(first[i] == lane + 64 * i);
+    if (first[i] == lane + 64 * i) {
+      const int at = groups + __popcll(firsts & ((1ull << lane) - 1));
+      x.group[at] = g;
+      x.slot[at] = first[i];
+    }
+    groups += __popcll(firsts);
+  }
+  __threadfence_block();
+  float top = kNegInf, m = kNegInf, s = 0.f;
+  for (int i = lane; i < p.count; i += 64) {
+    const float mi = p.m[t * p.row + i * p.stride];
+    top = fmaxf(top, mi);
+    if (!(x.listed[i >> 5] >> (i & 31) & 1)) lse2_merge(m, s, mi == kNegInf ? kNegInf : mi * p.m_scale, p.s[t * p.row + i * p.stride]);
+  }
+  top = wave_max(top) * p.m_scale;
+  const float base = top == kNegInf ? 0.f : top;
+  double sum = (double)s * (double)fast_exp2(m - base);
+  constexpr int kFlight = 8;
+  for (int b = 0; b < groups; b += kFlight) {
+    f32x2 v[kFlight];
+#pragma unroll
+    for (int e = 0; e < kFlight; ++e)
+      v[e] = *reinterpret_cast<const f32x2*>(z + (long)x.group[b + e < groups ? b + e : b] * kGroup + 2 * lane);
+#pragma unroll
+    for (int e = 0; e < kFlight; ++e) {
+      if (b + e >= groups) continue;
+      const uint32_t listed = x.columns[x.slot[b + e]][lane >> 4] >> (2 * lane & 31);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) sum += listed >> c & 1 ? 0.0 : (double)fast_exp2(__builtin_fmaf(v[e][c], p.m_scale, -base));
+    }
+  }
+  return {base, wave_sum64(sum)};
+}
+
+template <int KIND, bool FEW>
 __global__ __launch_bounds__(256) void distill_rows_kernel(RowParts parts, const int* __restrict__ sorted,
                                                            const int* __restrict__ slot, const float* __restrict__ picks,
                                                            const float* __restrict__ Z, long ldz,
                                                            const int64_t* __restrict__ ids, const float* __restrict__ teacher,
-                                                           const uint8_t* __restrict__ mask, long n, long V, float inv_t, int k,
-                                                           int renormalize, double beta, float* __restrict__ row_loss,
+                                                           const uint8_t* __restrict__ mask, long n, long V, float c2, double inv_t,
+                                                           int k, int renormalize, double beta, float* __restrict__ row_loss,
                                                            int* __restrict__ row_counts, float* __restrict__ lse_out,
                                                            float* __restrict__ rest_out, float* __restrict__ coef,
                                                            int* __restrict__ columns) {
+  __shared__ GroupScratch scratch[FEW ? 4 : 1];
   const int lane = threadIdx.x & 63;
   const long t = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (t >= n) return;
   // Which slots hold an outcome: a column of its own that the teacher gives something to.
   int id[kPerLane];
-  if (sorted) {
+  if constexpr (FEW) {
+    load_list(ids, teacher, row_counts_by(mask, t), t, V, k, lane, id);
+  } else {
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
       const int y = lane + 64 * i < k ? sorted[t * k + lane + 64 * i] : kNoColumn;
       id[i] = y == kNoColumn ? -1 : y;
     }
-  } else {
-    load_list(ids, teacher, row_counts_by(mask, t), t, V, k, lane, id);
   }
   float lp[kPerLane];
   bool on[kPerLane];
@@ -841,7 +915,7 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(RowParts parts, const
   for (int i = 0; i < kPerLane; ++i) {
     const long o = t * k + lane + 64 * i;
     on[i] = id[i] >= 0;
-    lp[i] = on[i] ? teacher[sorted ? t * k + slot[o] : o] : 0.f;
+    lp[i] = on[i] ? teacher[FEW ? o : t * k + slot[o]] : 0.f;
   }
   bool some = false;
 #pragma unroll
@@ -857,30 +931,47 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(RowParts parts, const
     }
     return;
   }
-  float m = kNegInf, s = 0.f;
-  for (int i = lane; i < parts.count; i += 64) {
-    const float mi = parts.m[t * parts.row + i * parts.stride];
-    lse2_merge(m, s, mi == kNegInf ? kNegInf : mi * parts.m_scale, parts.s[t * parts.row + i * parts.stride]);
+  OffList off;
+  if constexpr (FEW) {
+    off = few_off_list(parts, t, Z + t * ldz, id, k, lane, scratch[threadIdx.x >> 6]);
+  } else {
+    float m = kNegInf, s = 0.f;
+    for (int i = lane; i < parts.count; i += 64)
+      lse2_merge(m, s, parts.m[t * parts.row + i * parts.stride], parts.s[t * parts.row + i * parts.stride]);
+    off.base = wave_max(m);
+    off.sum = wave_sum64((double)s * (double)fast_exp2(off.base == kNegInf ? m : m - off.base));  // (-inf: all is listed)
   }
-  const float top = wave_max(m);
-  const double total = wave_sum64((double)s * (double)fast_exp2(m - top));
-  const double lse = ((double)top + log2(total)) * 0.6931471805599453;
 
-  double lq[kPerLane], lt[kPerLane], q[kPerLane], p[kPerLane];
+  // x = z c2 is exact in 64 bits, and the partials' are of the same c2.
+  double x[kPerLane], lq[kPerLane], lt[kPerLane], q[kPerLane], p[kPerLane], top = -HUGE_VAL, total = 0.0;
 #pragma unroll
   for (int i = 0; i < kPerLane; ++i) {
-    const long o = t * k + lane + 64 * i;
     float z = 0.f;
-    if (on[i]) z = Z ? Z[t * ldz + id[i]] : picks[o];
-    lq[i] = on[i] ? (double)z * (double)inv_t - lse : 0.0;
-    q[i] = on[i] ? exp(lq[i]) : 0.0;
+    if (on[i]) z = FEW ? Z[t * ldz + id[i]] : picks[t * k + lane + 64 * i];
+    x[i] = (double)z * (double)c2;
+    if (on[i]) top = fmax(top, x[i]);
     lt[i] = (double)lp[i];
+  }
+  top = fmax(wave_max64(top), (double)off.base);
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) {
+    q[i] = on[i] ? exp2(x[i] - top) : 0.0;
+    total += q[i];
+  }
+  const double rest = off.sum * exp2((double)off.base - top);
+  total = wave_sum64(total) + rest;
+  const double lse2 = top + log2(total), left = rest / total;
+  constexpr double kLog2 = 0.6931471805599453;
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) {
+    lq[i] = on[i] ? (x[i] - lse2) * kLog2 : 0.0;
+    q[i] /= total;
   }
   if (renormalize) {
     double hi = -HUGE_VAL, sum = 0.0;
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
-      lt[i] *= (double)inv_t;
+      lt[i] *= inv_t;
       if (on[i]) hi = fmax(hi, lt[i]);
     }
     hi = wave_max64(hi);
@@ -891,14 +982,12 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(RowParts parts, const
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) lt[i] -= hi;
   }
-  double sq = 0.0, st = 0.0;
+  double st = 0.0;
 #pragma unroll
   for (int i = 0; i < kPerLane; ++i) {
     p[i] = on[i] ? exp(lt[i]) : 0.0;
-    sq += q[i];
     st += p[i];
   }
-  const double left = 1.0 - wave_sum64(sq);
   const double rq = fmax(left, kTailFloor), rt = renormalize ? 0.0 : fmax(1.0 - wave_sum64(st), kTailFloor);
   double loss = 0.0, qf[kPerLane], sqf = 0.0, frest;
   if constexpr (KIND == kDistillForward) {
@@ -938,16 +1027,16 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(RowParts parts, const
   for (int i = 0; i < kPerLane; ++i) {
     const int slot = lane + 64 * i;
     if (slot < k) {
-      coef[t * k + slot] = on[i] ? (float)((qf[i] - q[i] * mean) * (double)inv_t) : 0.f;
+      coef[t * k + slot] = on[i] ? (float)((qf[i] - q[i] * mean) * inv_t) : 0.f;
       columns[t * k + slot] = on[i] ? id[i] : -1;
     }
   }
   if (lane == 0) {
     row_loss[t] = (float)loss;
     row_counts[t] = 1;
-    lse_out[t] = (float)lse;
-    const float rest = (float)((frest - mean) * (double)inv_t);
-    rest_out[t] = rest == 0.f ? kLeast : rest;  // 0 is a row that gets no gradient
+    lse_out[t] = (float)(lse2 * kLog2);
+    const float factor = (float)((frest - mean) * inv_t);
+    rest_out[t] = factor == 0.f ? kLeast : factor;  // 0 is a row that gets no gradient
   }
 }
 
@@ -1135,7 +1224,7 @@ Scratch carve(const ScoreShape& sh, int f32, int q4, int top, int k_list, float*
     const long parts = splits(x.rows) * x.rows > splits(last) * last ? splits(x.rows) * x.rows : splits(last) * last;
     x.m = c.take<float>(parts);
     x.s = c.take<float>(parts);
-    if (!k_list || x.kept) x.u = c.take<float>(parts);
+    if (!k_list) x.u = c.take<float>(parts);
     if (top) {
       x.gmax = c.take<float>(x.rows * x.ldg);
     }
@@ -1151,7 +1240,7 @@ Scratch carve(const ScoreShape& sh, int f32, int q4, int top, int k_list, float*
       if (x.max_tiles > entries) x.max_tiles = (int)entries;
       x.tiles = c.take<GatherTile>(x.max_tiles);
     }
-    if (k_list && !x.kept) {
+    if (k_list) {
       x.column = c.take<int>(x.rows * k_list);
       x.slot = c.take<int>(x.rows * k_list);
       x.picks = c.take<float>(x.rows * k_list);
@@ -1266,7 +1355,7 @@ hipError_t launch_logprobs_fwd(const ScoreHead& head, const ScoreShape& sh, cons
   size_t bytes;
   ScoreHead h = head;
   const Scratch x = carve(sh, h.f32, h.f32 ? h.h32.q4 : h.h.q4, top, 0, o.logits, ws, &bytes);
-  const float c2 = kLog2e * sh.inv_t;
+  const float c2 = sh.c2;
   const int V = (int)sh.v;
   const hipError_t staged = staged_head(h, sh, x, st);
   if (staged != hipSuccess) return staged;
@@ -1330,29 +1419,30 @@ hipError_t launch_distill_fwd(const ScoreHead& head, const ScoreShape& sh, const
   size_t bytes;
   ScoreHead h = head;
   const Scratch x = carve(sh, h.f32, h.f32 ? h.h32.q4 : h.h.q4, 0, p.k, o.logits, ws, &bytes);
-  const float c2 = kLog2e * sh.inv_t;
+  const float c2 = sh.c2;
   const hipError_t staged = staged_head(h, sh, x, st);
   if (staged != hipSuccess) return staged;
   float* row_loss = p.reduction == kReduceNone ? o.loss : x.row_loss;
-  auto kernel = p.kind == kDistillForward ? distill_rows_kernel<kDistillForward>
-                : p.kind == kDistillReverse ? distill_rows_kernel<kDistillReverse> : distill_rows_kernel<kDistillJsd>;
-  for (long r0 = 0; r0 < sh.n; r0 += x.rows) {
+  auto rows = [&](auto few) {
+    constexpr bool FEW = decltype(few)::value;
+    return p.kind == kDistillForward ? distill_rows_kernel<kDistillForward, FEW>
+           : p.kind == kDistillReverse ? distill_rows_kernel<kDistillReverse, FEW> : distill_rows_kernel<kDistillJsd, FEW>;
+  };
+  auto kernel = x.few ? rows(std::true_type{}) : rows(std::false_type{});
+  for (long r0 = 0; r0 < sh.n; r0 += x.rows) {  // (kept: one pass)
     const long n = sh.n - r0 < x.rows ? sh.n - r0 : x.rows;
     const int64_t* id = ids + r0 * p.k;
     const float* lp = teacher + r0 * p.k;
     const uint8_t* see = mask ? mask + r0 : nullptr;
-    if (x.kept) {
-      const hipError_t e = x.few ? few_logits(h, sh, x, c2, st) : tile_stats(h, sh, x, 0, n, c2, 0, st);
-      if (e != hipSuccess) return e;
-    } else {
+    if (!x.few) {
       hipLaunchKernelGGL(sort_lists_kernel, dim3((unsigned)ceil_div(n, 4)), dim3(256), 0, st, id, lp, see, n, sh.v, p.k, x.column,
                          x.slot);
       MTP_LAUNCHED();
-      const hipError_t e = tile_stats(h, sh, x, r0, n, c2, p.k, st);
-      if (e != hipSuccess) return e;
     }
+    const hipError_t e = x.few ? few_logits(h, sh, x, c2, st) : tile_stats(h, sh, x, r0, n, c2, p.k, st);
+    if (e != hipSuccess) return e;
     hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(n, 4)), dim3(256), 0, st, row_parts(x, h, n, sh.v, c2), x.column,
-                       x.slot, x.picks, x.kept ? x.z : nullptr, x.ldz, id, lp, see, n, sh.v, sh.inv_t, p.k, p.renormalize, p.beta, row_loss + r0,
+                       x.slot, x.picks, x.z, x.ldz, id, lp, see, n, sh.v, c2, p.inv_t, p.k, p.renormalize, p.beta, row_loss + r0,
                        x.row_counts + r0, o.lse + r0, o.rest + r0, o.coef + r0 * p.k, o.columns + r0 * p.k);
     MTP_LAUNCHED();
   }
