@@ -339,7 +339,6 @@ void lce32_fwd_kernel(const float* __restrict__ H, const float* __restrict__ W,
                                                         float* __restrict__ part_u, float* __restrict__ gmax, int ldg,
                                                         float* __restrict__ Z, long ldz, ScoreList list) {
   const float c2 = STAT ? scale2 : kLog2e;
-  constexpr float kHidden = (STAT & kStatEntropy) ? -1e30f : kNegInf;
   __shared__ float gx[(STAT & kStatGroups) ? kT : 1];
   __shared__ __attribute__((aligned(1024))) char s0[kStage0<KIND>];
   __shared__ __attribute__((aligned(1024))) char s1[kStage1<KIND>];
@@ -372,7 +371,7 @@ void lce32_fwd_kernel(const float* __restrict__ H, const float* __restrict__ W,
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (v0 + 64 * wa + 32 * i + rrow(r, h) >= V) acc[i][j][r] = kHidden;
+          if (v0 + 64 * wa + 32 * i + rrow(r, h) >= V) acc[i][j][r] = kNegInf;
       if constexpr (STAT & kStatKeep) {
         const int t = t0 + 64 * wb + 32 * j + (lane & 31);
         if (t < N) {
@@ -402,7 +401,7 @@ void lce32_fwd_kernel(const float* __restrict__ H, const float* __restrict__ W,
         if (wa == 0 && h == 0 && t0 + tl < N) gmax[(long)(t0 + tl) * ldg + vt] = fmaxf(both, gx[tl]);
       }
       const float mn = fmaxf(m[j], mz * c2);
-      const float base = (STAT & kStatEntropy) ? fmaxf(mn, -1e28f) : (mn == kNegInf) ? 0.f : mn;
+      const float base = (mn == kNegInf) ? 0.f : mn;
       float sum = 0.f, sumu = 0.f;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -411,7 +410,7 @@ void lce32_fwd_kernel(const float* __restrict__ H, const float* __restrict__ W,
           const float x = __builtin_fmaf(acc[i][j][r], c2, -base);
           const float e = fast_exp2(x);
           sum += e;
-          if constexpr (STAT & kStatEntropy) sumu = __builtin_fmaf(e, x, sumu);
+          if constexpr (STAT & kStatEntropy) sumu = __builtin_fmaf(e, finite_exponent(x), sumu);
         }
       const float f = fast_exp2(m[j] - base);
       if constexpr (STAT & kStatEntropy) u[j] = __builtin_fmaf(s[j], m[j] == kNegInf ? 0.f : m[j] - base, u[j]) * f + sumu;

@@ -900,8 +900,6 @@ void lce_fwd_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
                     float* __restrict__ part_u, float* __restrict__ gmax, int ldg, float* __restrict__ Z, long ldz,
                     ScoreList list) {
   const float c2 = STAT ? scale2 : kLog2e;
-  // Hidden rows past V: beyond any logit, but finite where 0 of it has to be 0.
-  constexpr float kHidden = (STAT & kStatEntropy) ? -1e30f : kNegInf;
   __shared__ __attribute__((aligned(16))) char lds[Q4 ? kLdsBytes + kQ4SbBytes : kLdsBytes];
   // Workgroup g runs on XCD g % 8. When the row tiles divide into 8 groups, XCD x owns row tiles
   // [x R/8, (x+1) R/8) for every split, walked split-major: the ~32 workgroups resident on one XCD
@@ -963,7 +961,7 @@ void lce_fwd_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int v = v0 + 128 * wa + 32 * i + 8 * (r >> 2) + 4 * lhalf + (r & 3);
-            if (v >= V) acc[i][j][r] = kHidden;
+            if (v >= V) acc[i][j][r] = kNegInf;
           }
     }
     if constexpr (STAT & kStatKeep) {
@@ -1000,8 +998,7 @@ void lce_fwd_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
     for (int j = 0; j < kNJ; ++j) {
       const float a0 = fmaxf(fmaxf(pm[j][0], pm[j][1]), fmaxf(pm[j][2], pm[j][3]));
       mn[j] = fmaxf(m[j], a0 * c2);
-      // (a lane may have met nothing but hidden rows: they stay far below the base)
-      base[j] = (STAT & kStatEntropy) ? fmaxf(mn[j], -1e28f) : (mn[j] == kNegInf) ? 0.f : mn[j];
+      base[j] = (mn[j] == kNegInf) ? 0.f : mn[j];
       if constexpr (STAT & kStatGroups) {
         const float both = fmaxf(a0, __shfl_xor(a0, 32, 64));
         const int t = t0 + 64 * wb + 32 * j + lcol;
@@ -1019,7 +1016,7 @@ void lce_fwd_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
           const float x = __builtin_fmaf(acc[i][j][r], c2, -base[j]);
           const float e = fast_exp2(x);
           ps[j][r & 3] += e;
-          if constexpr (STAT & kStatEntropy) pu[j][r & 3] = __builtin_fmaf(e, x, pu[j][r & 3]);
+          if constexpr (STAT & kStatEntropy) pu[j][r & 3] = __builtin_fmaf(e, finite_exponent(x), pu[j][r & 3]);
         }
 #pragma unroll
     for (int j = 0; j < kNJ; ++j) {

@@ -118,6 +118,9 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v;
 }
 
+// x where 2^x x is wanted: what is ruled out (x = -inf, a row past the head's end or a logit) adds 0 and no NaN.
+__device__ __forceinline__ float finite_exponent(float x) { return fmaxf(x, -1e30f); }
+
 // Merge two (max, sum-of-exp2) partials in the log2 domain; -inf maxima are handled so that an
 // empty partial contributes nothing and two empty partials stay empty (no NaN).
 __device__ __forceinline__ void lse2_merge(float& m, float& s, float mo, float so) {
