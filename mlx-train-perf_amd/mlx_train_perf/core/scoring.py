@@ -89,6 +89,12 @@ def _check_hidden(hidden: torch.Tensor, head: HeadRef) -> tuple[int, ...]:
     return leading
 
 
+def _as_int64(ids: torch.Tensor) -> torch.Tensor:
+    """Whole numbers in 64 bits, before anything is compared with them: a narrower type takes V and ignore_index into its own
+    range first (300 is 44 in uint8). Others as they are, for their refusal."""
+    return ids if ids.dtype.is_floating_point or ids.dtype.is_complex or ids.dtype == torch.bool else ids.to(torch.int64)
+
+
 class _Inputs(NamedTuple):
     """hidden and head as the kernels read them."""
     hidden: torch.Tensor | None
@@ -330,7 +336,7 @@ def _reference_score(hidden2, head, targets2, ignore_index, top, temperature):
     entropy = torch.where(live, -(logp.exp() * logp).sum(1), 0.0)
     logprobs = None
     if targets2 is not None:
-        y = torch.where(live, targets2, 0).long()
+        y = torch.where(live, targets2, 0)
         logprobs = torch.where(live, logp.gather(1, y[:, None])[:, 0], 0.0)
         logprobs = _out(logprobs, hidden2)
     with torch.no_grad():
@@ -351,7 +357,7 @@ def _reference_distillation(hidden2, head, ids, teacher, mask, kind, beta, tempe
     on = on & first
     live = on.any(1)
     logp = torch.log_softmax(_reference_logits(hidden2, head, live, temperature), dim=1)
-    lq = logp.gather(1, torch.where(on, ids, 0).long())
+    lq = logp.gather(1, torch.where(on, ids, 0))
     lt = torch.where(on, teacher.double(), 0.0)
     if renormalize:
         lt = torch.where(on, lt / temperature, -math.inf)
@@ -397,6 +403,7 @@ def token_logprobs(hidden: torch.Tensor, head: HeadRef, targets: torch.Tensor | 
     `linear_cross_entropy`: unchecked targets outside the vocabulary count as a logit of 0."""
     leading = _check_hidden(hidden, head)
     if targets is not None:
+        targets = _as_int64(targets)
         _loss._validate_inputs(hidden=hidden, head=head, targets=targets, validate_targets=validate_targets,
                                ignore_index=ignore_index)
     temperature = _temperature(temperature)
@@ -414,7 +421,7 @@ def token_logprobs(hidden: torch.Tensor, head: HeadRef, targets: torch.Tensor | 
         parts = _reference_score(hidden2, head, targets2, ignore_index, top, temperature)
     else:
         x = _inputs(hidden2, head)
-        y = None if targets2 is None else targets2.to(torch.int64).contiguous()
+        y = None if targets2 is None else targets2.contiguous()
         args = (y, int(ignore_index), top, temperature)
         nodes = _nodes(x)
         parts = _TokenLogprobs.apply(*x, *args) if nodes is None else nodes.logprobs(*x, _forward_kind(x), _kept_bytes(x), *args)
@@ -465,6 +472,7 @@ def distillation_loss(hidden: torch.Tensor, head: HeadRef, teacher_ids: torch.Te
         raise LossInputError("teacher_logprobs belong to a frozen model and get no gradient: detach them")
     if mask is not None and (tuple(mask.shape) != leading or mask.dtype not in (torch.bool, torch.uint8)):
         raise LossInputError(f"mask must be bool or uint8 of hidden's leading dims {leading}; got {mask.dtype} {tuple(mask.shape)}")
+    teacher_ids = _as_int64(teacher_ids)
     v = _head_v(head)
     if validate_ids and bool((teacher_ids >= v).any()):   # a host sync
         raise LossInputError(f"teacher_ids must be below V={v} (negative ones are empty slots)")
@@ -477,7 +485,7 @@ def distillation_loss(hidden: torch.Tensor, head: HeadRef, teacher_ids: torch.Te
         loss = _reference_distillation(hidden2, head, ids2, teacher2, mask2, kind, beta, temperature, renormalize, reduction)
     else:
         x = _inputs(hidden2, head)
-        args = (ids2.to(torch.int64).contiguous(), _float(teacher2), None if mask2 is None else mask2.contiguous(), _KINDS[kind],
+        args = (ids2.contiguous(), _float(teacher2), None if mask2 is None else mask2.contiguous(), _KINDS[kind],
                 float(beta), temperature, int(renormalize), _REDUCTIONS[reduction])
         nodes = _nodes(x)
         loss = _Distillation.apply(*x, *args) if nodes is None else nodes.distillation(*x, _forward_kind(x), _kept_bytes(x), *args)
