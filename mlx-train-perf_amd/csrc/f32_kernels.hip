@@ -578,7 +578,7 @@ void lce32_bwd_g_kernel(const float* __restrict__ H, const float* __restrict__ W
         if constexpr (AFFINE) {
           const float slope = __builtin_bit_cast(float, y);
           const float p = fast_exp2(__builtin_fmaf(acc[i][j][r], rows.scale2, -l2));
-          if (c0 + vl < V && (coef != 0.f || slope != 0.f)) g = p * __builtin_fmaf(slope, acc[i][j][r], coef);
+          if (c0 + vl < V && (coef != 0.f || slope != 0.f)) g = p * __builtin_fmaf(slope, finite_exponent(acc[i][j][r]), coef);
         } else if (c0 + vl < V) {
           const float p = fast_exp2(__builtin_fmaf(acc[i][j][r], kLog2e, -l2));
           g = (p - (vl == y ? 1.f : 0.f)) * coef;

@@ -1335,7 +1335,7 @@ void lce_bwd_g_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W
           const int v = v0 + 128 * wa + 32 * i + 8 * q + 4 * lhalf + u;
           if constexpr (AFFINE) {
             const float p = fast_exp2(acc[i][j][r] * rows.scale2 - l2);
-            gv[u] = (v < vlim && live) ? p * __builtin_fmaf(slope, acc[i][j][r], coef) : 0.f;
+            gv[u] = (v < vlim && live) ? p * __builtin_fmaf(slope, finite_exponent(acc[i][j][r]), coef) : 0.f;
           } else {
             float p = fast_exp2(acc[i][j][r] * kLog2e - l2);
             if (v == y) p -= 1.f;
@@ -1558,7 +1558,7 @@ void lce_bwd_g_persist_kernel(const bf16_t* __restrict__ H, const bf16_t* __rest
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const float z = acc[i][j][4 * q + u];
-          gv[u] = fast_exp2(z * rows.scale2 - l2[j]) * __builtin_fmaf(slope[j], z, coef[j]);
+          gv[u] = fast_exp2(z * rows.scale2 - l2[j]) * __builtin_fmaf(slope[j], finite_exponent(z), coef[j]);
         }
         return u32x2{pack_bf16x2(gv[0], gv[1]) & keep, pack_bf16x2(gv[2], gv[3]) & keep};
       }

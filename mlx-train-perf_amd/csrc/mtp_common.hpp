@@ -118,7 +118,7 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v;
 }
 
-// x where 2^x x is wanted: what is ruled out (x = -inf, a row past the head's end or a logit) adds 0 and no NaN.
+// A factor x of 2^x: what is ruled out (x = -inf, a row past the head's end or a logit) adds 0 and no NaN.
 __device__ __forceinline__ float finite_exponent(float x) { return fmaxf(x, -1e30f); }
 
 // Merge two (max, sum-of-exp2) partials in the log2 domain; -inf maxima are handled so that an

@@ -402,7 +402,7 @@ void lce_few_kernel(const T* __restrict__ H, const T* __restrict__ W, const uint
       if (v0 + 32 * w + 8 * (r >> 2) + 4 * half + (r & 3) < V) {
         const float x = __builtin_fmaf(acc[b][r], c2, -base), e = fast_exp2(x);
         s += e;
-        u = __builtin_fmaf(e, x, u);
+        u = __builtin_fmaf(e, finite_exponent(x), u);
       }
     s += __shfl_xor(s, 32, 64);
     u += __shfl_xor(u, 32, 64);
@@ -1003,7 +1003,7 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(RowParts parts, const
     frest = log(rq / rt);
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
-      qf[i] = on[i] ? q[i] * (lq[i] - lt[i]) : 0.0;
+      qf[i] = on[i] && q[i] != 0.0 ? q[i] * (lq[i] - lt[i]) : 0.0;
       sqf += qf[i];
     }
     loss = wave_sum64(sqf) + rq * frest;
@@ -1015,7 +1015,7 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(RowParts parts, const
       qf[i] = 0.0;
       if (on[i]) {
         const double lm = log_add(a + lt[i], b + lq[i]);
-        qf[i] = (1.0 - beta) * q[i] * (lq[i] - lm);
+        if (q[i] != 0.0) qf[i] = (1.0 - beta) * q[i] * (lq[i] - lm);
         loss += beta * p[i] * (lt[i] - lm);
       }
       sqf += qf[i];
@@ -1090,7 +1090,7 @@ __global__ __launch_bounds__(256) void logprobs_coef_kernel(const float* __restr
   const long long y = targets ? targets[t] : -1;
   const bool dead = targets && y == ignore_index, in = !dead && targets && y >= 0 && y < V;
   const float a = !dead && d_logprobs ? d_logprobs[t] : 0.f, b = !dead && d_entropy ? d_entropy[t] : 0.f;
-  const float up = lse[t] - entropy[t], l = in ? tgt[t] * inv_t - lse[t] : 0.f;
+  const float up = lse[t] - entropy[t], l = in ? finite_exponent(tgt[t] * inv_t - lse[t]) : 0.f;
   alpha[t] = (b * up - a) * inv_t;
   beta[t] = -b * inv_t * inv_t;
   columns[t] = in ? (int)y : -1;
@@ -1132,7 +1132,7 @@ __global__ __launch_bounds__(256) void affine_tiles_kernel(const float* __restri
     const f32x4 z = live && v + i < vlim ? *reinterpret_cast<const f32x4*>(Z + t * ldz + v + i) : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      g[i + u] = live && v + i + u < vlim ? fast_exp2(__builtin_fmaf(z[u], rows.scale2, -l2)) * __builtin_fmaf(beta, z[u], alpha) : 0.f;
+      g[i + u] = live && v + i + u < vlim ? fast_exp2(__builtin_fmaf(z[u], rows.scale2, -l2)) * __builtin_fmaf(beta, finite_exponent(z[u]), alpha) : 0.f;
   }
   if constexpr (sizeof(G) == 2) {
     *reinterpret_cast<u32x4*>(out + t * ldg + c) =

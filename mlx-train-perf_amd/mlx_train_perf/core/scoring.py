@@ -329,11 +329,16 @@ def _out(x: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
     return x if like.dtype == torch.float64 else x.to(torch.float32)
 
 
+def _finite(logp: torch.Tensor) -> torch.Tensor:
+    """A factor of exp(logp): what is ruled out (-inf) adds 0 and no NaN, to the value and to its gradient."""
+    return logp.masked_fill(logp == -math.inf, 0.0)
+
+
 def _reference_score(hidden2, head, targets2, ignore_index, top, temperature):
     n = hidden2.shape[0]
     live = torch.ones(n, dtype=torch.bool, device=hidden2.device) if targets2 is None else targets2 != ignore_index
     logp = torch.log_softmax(_reference_logits(hidden2, head, live, temperature), dim=1)
-    entropy = torch.where(live, -(logp.exp() * logp).sum(1), 0.0)
+    entropy = torch.where(live, -(logp.exp() * _finite(logp)).sum(1), 0.0)
     logprobs = None
     if targets2 is not None:
         y = torch.where(live, targets2, 0)
@@ -374,11 +379,11 @@ def _reference_distillation(hidden2, head, ids, teacher, mask, kind, beta, tempe
     if kind == "forward":
         loss = torch.where(on, t * (lt - lq), 0.0).sum(1) + rt * (safe / rq).log()
     elif kind == "reverse":
-        loss = torch.where(on, q * (lq - lt), 0.0).sum(1) + rq * (rq / rt).log()
+        loss = torch.where(on, q * (_finite(lq) - lt), 0.0).sum(1) + rq * (rq / rt).log()
     else:
         lm = torch.logaddexp(math.log(beta) + lt, math.log1p(-beta) + lq)
         rm = beta * rt + (1 - beta) * rq
-        loss = torch.where(on, beta * t * (lt - lm) + (1 - beta) * q * (lq - lm), 0.0).sum(1)
+        loss = torch.where(on, beta * t * (lt - lm) + (1 - beta) * q * (_finite(lq) - lm), 0.0).sum(1)
         loss = loss + beta * rt * (safe / rm).log() + (1 - beta) * rq * (rq / rm).log()
     loss = torch.where(live, loss, 0.0)
     if reduction == "mean":
