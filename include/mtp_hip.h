@@ -390,7 +390,7 @@ int mtp_policy_bwd(const float* d_loss, const float* nll, const float* old_nll, 
 /* ---------------------------------------------------------------------------------------------
  * (E) Token scoring and distillation over a head (no counterpart in the reference)
  *
- * hidden, head, n, d, v, head_kind: as (A), v <= 2^21. With x = hidden . w / temperature, lse = logsumexp x,
+ * hidden, head, n, d, v, head_kind: as (A), v <= 2^21, bf16 d < 2^22. With x = hidden . w / temperature, lse = logsumexp x,
  * p = exp(x - lse). temperature in [1e-3, 1e3]. The _f32 forms take fp32 hidden states and heads.
  * A forward's head_kind MTP_HEAD_Q4_STAGED dequantizes the whole head into the workspace (few tokens: none of it), an fp32
  * backward's too; a bf16 backward's kinds, and chunk, row_block and w_t, are mtp_lce_bwd's (mtp_lce_bwd_f32's).

@@ -810,7 +810,8 @@ int mtp_policy_bwd(const float* d_loss, const float* nll, const float* old_nll, 
 // Token scoring and distillation
 // ---------------------------------------------------------------------------------------------
 
-static int check_score(int64_t n, int64_t d, int64_t v, double temperature) {
+static int check_score(int f32, int64_t d, int64_t v, double temperature) {
+  if (!f32 && d >= mtp::kScoreDims) return fail(MTP_ERR_UNSUPPORTED, "token scoring and distillation serve fewer than 2^22 bf16 hidden dims (got d=%lld); use impl='reference'", (long long)d);
   if (v > mtp::kScoreVocab) return fail(MTP_ERR_UNSUPPORTED, "token scoring and distillation serve a vocabulary of at most 2^21 (got v=%lld); use impl='reference'", (long long)v);
   if (!(temperature >= 1e-3 && temperature <= 1e3)) return fail(MTP_ERR_INPUT, "temperature must be in [1e-3, 1e3] (got %g)", temperature);
   return MTP_OK;
@@ -874,7 +875,7 @@ static int logprobs_fwd(int f32, const void* hidden, const void* w, const uint32
                         size_t workspace_bytes, void* stream) {
   int rc = check_score_head(f32, hidden, w, w_q, scales, biases, n, d, v, head_kind);
   if (rc) return rc;
-  rc = check_score(n, d, v, temperature);
+  rc = check_score(f32, d, v, temperature);
   if (rc) return rc;
   if (top < 0 || top > v) return fail(MTP_ERR_INPUT, "top must be in [0, v=%lld] (got %d)", (long long)v, (int)top);
   if (top > MTP_SCORE_MAX) return fail(MTP_ERR_UNSUPPORTED, "at most %d alternatives (got top=%d); use impl='reference'", MTP_SCORE_MAX, (int)top);
@@ -950,7 +951,7 @@ static int score_bwd(int f32, const void* hidden, const void* w, const void* w_t
                      int64_t row_block, void* workspace, size_t workspace_bytes, hipStream_t stream, const FACTORS& factors) {
   int rc = check_score_head(f32, hidden, w, w_q, scales, biases, n, d, v, head_kind);
   if (rc) return rc;
-  rc = check_score(n, d, v, temperature);
+  rc = check_score(f32, d, v, temperature);
   if (rc) return rc;
   if (!lse || !d_hidden) return fail(MTP_ERR_INPUT, "lse and d_hidden must be non-null");
   if (!aligned16(d_hidden) || !aligned16(d_w) || !aligned16(w_t) || !aligned16(logits))
@@ -1065,7 +1066,7 @@ static int distill_fwd(int f32, const void* hidden, const void* w, const uint32_
                        int32_t reduction, const mtp::DistillOut& out, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_score_head(f32, hidden, w, w_q, scales, biases, n, d, v, head_kind);
   if (rc) return rc;
-  if ((rc = check_score(n, d, v, temperature)) || (rc = check_list(k)) || (rc = check_reduction(reduction))) return rc;
+  if ((rc = check_score(f32, d, v, temperature)) || (rc = check_list(k)) || (rc = check_reduction(reduction))) return rc;
   if (kind < MTP_DISTILL_FORWARD || kind > MTP_DISTILL_JSD) return fail(MTP_ERR_INPUT, "unknown kind %d of a distillation loss", (int)kind);
   if (kind == MTP_DISTILL_JSD && !(beta > 0.0 && beta < 1.0)) return fail(MTP_ERR_INPUT, "beta must be in (0, 1) (got %g)", beta);
   if (kind == MTP_DISTILL_REVERSE && renormalize) return fail(MTP_ERR_INPUT, "a renormalized teacher gives nothing to what its list leaves out: the reverse divergence is infinite");

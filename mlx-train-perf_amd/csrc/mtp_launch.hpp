@@ -211,6 +211,8 @@ hipError_t launch_lce32_gather(const LceHead32& h, const float* H, int D, int V,
 constexpr long kScoreRows = 16384;   // tokens of one pass of a forward: more are taken in blocks
 constexpr int kScoreTop = 128;       // most alternatives, and longest teacher's list
 constexpr long kScoreVocab = 1 << 21;
+constexpr long kScoreDims = 1 << 22; // hidden dims from which a tile's rows (256 of bf16, 128 of fp32) pass its 31-bit offsets: bf16 is
+                                     // refused there, fp32 takes the core that has none
 constexpr long kFewTokens = 128;     // tokens up to which a bf16 forward keeps its logits
 constexpr long kFewTokens32 = 64;    // an fp32 one (hidden dims that are multiples of 4)
 constexpr long kKeptBytes = 256L << 20;  // of logits that a forward with alternatives may keep

@@ -1205,7 +1205,7 @@ bool keep_logits(const ScoreShape& sh) { return 4 * sh.n * sh.v <= kKeptBytes; }
 Scratch carve(const ScoreShape& sh, int f32, int q4, int top, int k_list, float* logits, void* ws, size_t* bytes) {
   Scratch x{};
   Carver c{static_cast<char*>(ws)};
-  x.few = f32 ? sh.n <= kFewTokens32 && sh.d % 4 == 0 : sh.n <= kFewTokens;
+  x.few = f32 ? sh.n <= kFewTokens32 && sh.d % 4 == 0 && sh.d < kScoreDims : sh.n <= kFewTokens;
   x.groups = groups_of(sh.v);
   x.ldg = x.few ? x.groups : (x.groups + 1) / 2 * 2;  // a tile of 256 logits writes both its groups, the last one too
   x.take = top < x.groups ? top : x.groups;
