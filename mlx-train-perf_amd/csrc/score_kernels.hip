@@ -1199,6 +1199,11 @@ struct Scratch {
 // once more and five small launches. N x D x V, alternatives; formed again / kept: 333 x 2048 x 32003, 8: 120 / 84 us; 440 x 4096 x
 // 151936, 8: 834 / 617; 2000 x 2048 x 32003, 8: 296 / 292; 8000 x 256 x 8000, 8: 341 / 173; 1000 x 512 x 50000, 8: 110 / 116.
 bool keep_logits(const ScoreShape& sh) { return 4 * sh.n * sh.v <= kKeptBytes; }
+// Tokens of one pass that does: a row is a whole number of groups, which a small vocabulary is far from.
+long kept_rows(long n, long ldz) {
+  const long most = kKeptBytes / (4 * ldz) / 256 * 256;
+  return n < most ? n : most > 256 ? most : 256;
+}
 
 // k_list: length of a teacher's list (0: scoring, with `top` alternatives).
 // logits: the caller's, which keeps them (or, for its size alone, any address).
@@ -1211,7 +1216,7 @@ Scratch carve(const ScoreShape& sh, int f32, int q4, int top, int k_list, float*
   x.take = top < x.groups ? top : x.groups;
   x.ldz = (long)x.groups * kGroup;
   x.kept = x.few || logits || (top && keep_logits(sh));
-  x.rows = x.kept || sh.n < kScoreRows ? sh.n : kScoreRows;
+  x.rows = x.few || logits ? sh.n : x.kept ? kept_rows(sh.n, x.ldz) : sh.n < kScoreRows ? sh.n : kScoreRows;
   if (x.few) {
     x.z = logits ? logits : c.take<float>(x.rows * x.ldz);
     x.gmax = c.take<float>(x.rows * x.groups);
@@ -1359,24 +1364,23 @@ hipError_t launch_logprobs_fwd(const ScoreHead& head, const ScoreShape& sh, cons
   const int V = (int)sh.v;
   const hipError_t staged = staged_head(h, sh, x, st);
   if (staged != hipSuccess) return staged;
-  if (x.kept) {  // (one pass)
-    const hipError_t e = x.few ? few_logits(h, sh, x, c2, st) : tile_stats(h, sh, x, 0, sh.n, c2, 0, st);
-    if (e != hipSuccess) return e;
-    auto rows = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3((unsigned)sh.n), dim3(kPick), 0, st, row_parts(x, h, sh.n, sh.v, c2), x.gmax, x.groups, x.ldg, x.z,
-                         x.ldz, targets, ignore_index, V, sh.inv_t, top, x.take, o, nullptr, nullptr, nullptr);
-      return hipGetLastError();
-    };
-    if (!top) return rows(score_rows_kernel<true, 0, 0>);
-    if (x.take <= 16 && x.groups <= 2048) return rows(score_rows_kernel<true, 2048, 2048>);
-    if (x.take <= 64 && x.groups <= 2048) return rows(score_rows_kernel<true, 2048, 64 * kGroup>);
-    return rows(score_rows_kernel<true, kMaxGroups, kScoreTop * kGroup>);
-  }
-  for (long r0 = 0; r0 < sh.n; r0 += x.rows) {
+  for (long r0 = 0; r0 < sh.n; r0 += x.rows) {  // (few tokens, or a caller's logits: one pass)
     const long n = sh.n - r0 < x.rows ? sh.n - r0 : x.rows;
     const LogprobsOut out{o.logprobs ? o.logprobs + r0 : nullptr, o.entropy + r0, top ? o.top_logprobs + r0 * top : nullptr,
                           top ? o.top_ids + r0 * top : nullptr, o.lse + r0, o.tgt ? o.tgt + r0 : nullptr};
     const int64_t* y = targets ? targets + r0 : nullptr;
+    if (x.kept) {
+      const hipError_t e = x.few ? few_logits(h, sh, x, c2, st) : tile_stats(h, sh, x, r0, n, c2, 0, st);
+      if (e != hipSuccess) return e;
+      auto kernel = !top ? score_rows_kernel<true, 0, 0>
+                    : x.take <= 16 && x.groups <= 2048 ? score_rows_kernel<true, 2048, 2048>
+                    : x.take <= 64 && x.groups <= 2048 ? score_rows_kernel<true, 2048, 64 * kGroup>
+                                                       : score_rows_kernel<true, kMaxGroups, kScoreTop * kGroup>;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(kPick), 0, st, row_parts(x, h, n, sh.v, c2), x.gmax, x.groups, x.ldg, x.z,
+                         x.ldz, y, ignore_index, V, sh.inv_t, top, x.take, out, nullptr, nullptr, nullptr);
+      MTP_LAUNCHED();
+      continue;
+    }
     hipError_t e = tile_stats(h, sh, x, r0, n, c2, 0, st);
     if (e != hipSuccess) return e;
     if (y) {
