@@ -235,12 +235,13 @@ def _score_forward(x: _Inputs, targets, ignore_index: int, top: int, temperature
 
 
 class _TokenLogprobs(torch.autograd.Function):
-    """Saves each token's log-sum-exp, entropy and target logit, and few enough logits; more of them the backward forms again."""
+    """Saves each token's log-sum-exp, entropy and target logit, and few enough logits; more of them the backward forms again.
+    record: whether autograd is (inside a forward it is off, and what asks for a gradient asks under no_grad too)."""
 
     @staticmethod
-    def forward(ctx, hidden, w, w_q, scales, biases, kind, owner, targets, ignore_index, top, temperature):
+    def forward(ctx, hidden, w, w_q, scales, biases, kind, owner, targets, ignore_index, top, temperature, record=True):
         x = _Inputs(hidden, w, w_q, scales, biases, kind, owner)
-        logits = _kept_logits(x) if any(ctx.needs_input_grad) else None
+        logits = _kept_logits(x) if record and any(ctx.needs_input_grad) else None
         logprobs, entropy, top_lp, top_ids, lse, tgt = _score_forward(x, targets, ignore_index, top, temperature, logits)
         ctx.save_for_backward(hidden, targets, lse, entropy, tgt, logits)
         ctx.inputs, ctx.args = x._replace(hidden=None), (ignore_index, temperature)
@@ -262,7 +263,7 @@ class _TokenLogprobs(torch.autograd.Function):
                 _native.ptr(tgt), _native.ptr(logits), _native.ptr(d_logprobs), _native.ptr(d_entropy), *rest)
 
         d_hidden, d_w = _backward(x, 1, x.w is not None and ctx.needs_input_grad[1], call)
-        return (d_hidden, d_w, *[None] * 9)
+        return (d_hidden, d_w, *[None] * 10)
 
 
 class _Distillation(torch.autograd.Function):
@@ -270,7 +271,7 @@ class _Distillation(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, hidden, w, w_q, scales, biases, kind, owner, ids, teacher, mask, loss_kind, beta, temperature,
-                renormalize, reduction):
+                renormalize, reduction, record=True):
         lib = _native.load()
         x = _Inputs(hidden, w, w_q, scales, biases, kind, owner)
         n, d = hidden.shape
@@ -283,7 +284,7 @@ class _Distillation(torch.autograd.Function):
         coef = torch.empty((n, k), dtype=torch.float32, device=dev)
         columns = torch.empty((n, k), dtype=torch.int32, device=dev)
         size = lib.mtp_distill_fwd_f32_workspace_bytes if f32 else lib.mtp_distill_fwd_workspace_bytes
-        logits = _kept_logits(x) if any(ctx.needs_input_grad) else None
+        logits = _kept_logits(x) if record and any(ctx.needs_input_grad) else None
         ws_bytes = size(n, d, x.v, fwd_kind, k, int(logits is not None))
         ws = _workspace(ws_bytes, hidden)
         with _native.on_device(hidden):
@@ -311,7 +312,7 @@ class _Distillation(torch.autograd.Function):
                 coef.data_ptr(), columns.data_ptr(), _native.ptr(logits), *after)
 
         d_hidden, d_w = _backward(x, k, x.w is not None and ctx.needs_input_grad[1], call)
-        return (d_hidden, d_w, *[None] * 13)
+        return (d_hidden, d_w, *[None] * 14)
 
 
 # ---- the reference impl -------------------------------------------------------------------------------------------
@@ -429,7 +430,7 @@ def token_logprobs(hidden: torch.Tensor, head: HeadRef, targets: torch.Tensor | 
         y = None if targets2 is None else targets2.contiguous()
         args = (y, int(ignore_index), top, temperature)
         nodes = _nodes(x)
-        parts = _TokenLogprobs.apply(*x, *args) if nodes is None else nodes.logprobs(*x, _forward_kind(x), _kept_bytes(x), *args)
+        parts = _TokenLogprobs.apply(*x, *args, torch.is_grad_enabled()) if nodes is None else nodes.logprobs(*x, _forward_kind(x), _kept_bytes(x), *args)
     *logprobs, entropy, top_lp, top_ids = parts   # (the node has none without targets)
     logprobs = logprobs[0] if logprobs else None
     return TokenLogprobs(None if logprobs is None else logprobs.view(leading), entropy.view(leading),
@@ -493,5 +494,5 @@ def distillation_loss(hidden: torch.Tensor, head: HeadRef, teacher_ids: torch.Te
         args = (ids2.contiguous(), _float(teacher2), None if mask2 is None else mask2.contiguous(), _KINDS[kind],
                 float(beta), temperature, int(renormalize), _REDUCTIONS[reduction])
         nodes = _nodes(x)
-        loss = _Distillation.apply(*x, *args) if nodes is None else nodes.distillation(*x, _forward_kind(x), _kept_bytes(x), *args)
+        loss = _Distillation.apply(*x, *args, torch.is_grad_enabled()) if nodes is None else nodes.distillation(*x, _forward_kind(x), _kept_bytes(x), *args)
     return loss.view(leading) if reduction == "none" else loss
