@@ -581,10 +581,10 @@ ScoreHead kept_head(torch::autograd::AutogradContext* ctx) {
   auto tensor = [&](const char* name) { return sd.count(name) ? sd[name].toTensor() : at::Tensor(); };
   return ScoreHead{tensor("w"), tensor("w_q"), tensor("scales"), tensor("biases"), tensor("owner"), sd["kind"].toInt(), 0, 0};
 }
-// Room for the logits of a call that has a backward to come, or none.
-at::Tensor kept_logits(const at::Tensor& hidden, const ScoreHead& h, const std::optional<at::Tensor>& w, const at::Tensor& owner) {
+// Room for the logits of a call that has a backward to come, or none. (A frozen head's weight may ask for a gradient: it gets none.)
+at::Tensor kept_logits(const at::Tensor& hidden, const ScoreHead& h, const std::optional<at::Tensor>& w) {
   // (inside a node's forward: whether its inputs ask for a gradient, and whether one is recorded)
-  const bool asked = hidden.requires_grad() || (w.has_value() && w->requires_grad()) || owner.requires_grad();
+  const bool asked = hidden.requires_grad() || (w.has_value() && w->requires_grad());
   return h.kept && asked && h.recorded ? at::empty({h.kept / 4}, hidden.options().dtype(at::kFloat)) : at::Tensor();
 }
 
@@ -598,7 +598,7 @@ struct LogprobsCall {
 struct Logprobs : torch::autograd::Function<Logprobs> {
   // hidden, w and owner: the inputs that may ask for a gradient
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& hidden,
-                                                const std::optional<at::Tensor>& w, const at::Tensor& owner,
+                                                const std::optional<at::Tensor>& w, const at::Tensor& /*owner*/,
                                                 const LogprobsCall& c) {
     const c10::DeviceGuard device(hidden.device());
     const int64_t n = hidden.size(0), d = hidden.size(1), v = c.head.vocab();
@@ -609,7 +609,7 @@ struct Logprobs : torch::autograd::Function<Logprobs> {
     float *lse = ptr<float>(kept), *tgt = c.targets.defined() ? lse + n : nullptr;
     if (c.targets.defined()) logprobs = at::empty({n}, opt);
     const at::Tensor top = at::empty({n, c.top}, opt), ids = at::empty({n, c.top}, opt.dtype(at::kLong));
-    const at::Tensor logits = kept_logits(hidden, c.head, w, owner);
+    const at::Tensor logits = kept_logits(hidden, c.head, w);
     const size_t bytes = (f32 ? g_api.logprobs_ws32 : g_api.logprobs_ws)(n, d, v, (int)c.head.fwd_kind, (int)c.top, logits.defined());
     const at::Tensor ws = bytes_like(hidden, bytes);
     const auto* y = c.targets.defined() ? ptr<int64_t>(c.targets) : nullptr;
@@ -674,7 +674,7 @@ struct DistillCall {
 
 struct Distillation : torch::autograd::Function<Distillation> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& hidden, const std::optional<at::Tensor>& w,
-                            const at::Tensor& owner, const DistillCall& c) {
+                            const at::Tensor& /*owner*/, const DistillCall& c) {
     const c10::DeviceGuard device(hidden.device());
     const int64_t n = hidden.size(0), d = hidden.size(1), v = c.head.vocab(), k = c.ids.size(1);
     const bool f32 = hidden.scalar_type() == at::kFloat;
@@ -683,7 +683,7 @@ struct Distillation : torch::autograd::Function<Distillation> {
     // lse, a factor per token, a factor and a column (int32) per slot, the scale
     const at::Tensor kept = at::empty({2 * n * (k + 1) + 1}, opt);
     float *lse = ptr<float>(kept), *rest = lse + n, *coef = rest + n, *columns = coef + n * k, *scale = columns + n * k;
-    const at::Tensor logits = kept_logits(hidden, c.head, w, owner);
+    const at::Tensor logits = kept_logits(hidden, c.head, w);
     const size_t bytes = (f32 ? g_api.distill_ws32 : g_api.distill_ws)(n, d, v, (int)c.head.fwd_kind, (int)k, logits.defined());
     const at::Tensor ws = bytes_like(hidden, bytes);
     const ScoreHead& h = c.head;

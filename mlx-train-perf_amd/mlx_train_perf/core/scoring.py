@@ -241,7 +241,7 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, w, w_q, scales, biases, kind, owner, targets, ignore_index, top, temperature, record=True):
         x = _Inputs(hidden, w, w_q, scales, biases, kind, owner)
-        logits = _kept_logits(x) if record and any(ctx.needs_input_grad) else None
+        logits = _kept_logits(x) if record and any(ctx.needs_input_grad[:2]) else None
         logprobs, entropy, top_lp, top_ids, lse, tgt = _score_forward(x, targets, ignore_index, top, temperature, logits)
         ctx.save_for_backward(hidden, targets, lse, entropy, tgt, logits)
         ctx.inputs, ctx.args = x._replace(hidden=None), (ignore_index, temperature)
@@ -284,7 +284,7 @@ class _Distillation(torch.autograd.Function):
         coef = torch.empty((n, k), dtype=torch.float32, device=dev)
         columns = torch.empty((n, k), dtype=torch.int32, device=dev)
         size = lib.mtp_distill_fwd_f32_workspace_bytes if f32 else lib.mtp_distill_fwd_workspace_bytes
-        logits = _kept_logits(x) if record and any(ctx.needs_input_grad) else None
+        logits = _kept_logits(x) if record and any(ctx.needs_input_grad[:2]) else None
         ws_bytes = size(n, d, x.v, fwd_kind, k, int(logits is not None))
         ws = _workspace(ws_bytes, hidden)
         with _native.on_device(hidden):

@@ -50,6 +50,7 @@ def test_logits_are_kept_for_a_gradient_alone(path, dtype, loss):
     assert held(True, False, False, grad=False) < _KEPT // 4
     assert held(False, True, True, grad=False) < _KEPT // 4
     assert held(False, False, False) < _KEPT // 4
+    assert held(False, True, False) < _KEPT // 4   # a frozen head's weight gets no gradient, whatever it asks for
 
 
 @pytest.mark.parametrize("n", [20, 200])
