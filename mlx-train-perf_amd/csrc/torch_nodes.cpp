@@ -596,9 +596,10 @@ struct LogprobsCall {
 };
 
 struct Logprobs : torch::autograd::Function<Logprobs> {
-  // hidden, w and owner: the inputs that may ask for a gradient
+  // hidden, w, scales, biases and owner: the inputs that may ask for a gradient
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& hidden,
-                                                const std::optional<at::Tensor>& w, const at::Tensor& /*owner*/,
+                                                const std::optional<at::Tensor>& w, const std::optional<at::Tensor>& /*scales*/,
+                                                const std::optional<at::Tensor>& /*biases*/, const at::Tensor& /*owner*/,
                                                 const LogprobsCall& c) {
     const c10::DeviceGuard device(hidden.device());
     const int64_t n = hidden.size(0), d = hidden.size(1), v = c.head.vocab();
@@ -661,7 +662,7 @@ struct Logprobs : torch::autograd::Function<Logprobs> {
                                opt_ptr<float>(d_entropy), ptr(p.d_hidden), opt_ptr(p.d_w), p.chunk, p.rows, ptr(p.ws), p.bytes,
                                stream_of(hidden)),
             "loss");
-    return once(grads, {p.d_hidden, p.d_w, at::Tensor(), at::Tensor()});
+    return once(grads, {p.d_hidden, p.d_w, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()});
   }
 };
 
@@ -674,6 +675,7 @@ struct DistillCall {
 
 struct Distillation : torch::autograd::Function<Distillation> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& hidden, const std::optional<at::Tensor>& w,
+                            const std::optional<at::Tensor>& /*scales*/, const std::optional<at::Tensor>& /*biases*/,
                             const at::Tensor& /*owner*/, const DistillCall& c) {
     const c10::DeviceGuard device(hidden.device());
     const int64_t n = hidden.size(0), d = hidden.size(1), v = c.head.vocab(), k = c.ids.size(1);
@@ -733,7 +735,7 @@ struct Distillation : torch::autograd::Function<Distillation> {
                               reinterpret_cast<const int32_t*>(columns), opt_ptr<float>(logits), ptr(p.d_hidden), opt_ptr(p.d_w), p.chunk, p.rows, ptr(p.ws),
                               p.bytes, stream_of(hidden)),
             "loss");
-    return once(grads, {p.d_hidden, p.d_w, at::Tensor(), at::Tensor()});
+    return once(grads, {p.d_hidden, p.d_w, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()});
   }
 };
 
@@ -804,7 +806,7 @@ std::vector<at::Tensor> logprobs(const at::Tensor& hidden, const std::optional<a
   const LogprobsCall call{{w.value_or(none), w_q.value_or(none), scales.value_or(none), biases.value_or(none), owner, kind, fwd_kind, kept,
                            at::GradMode::is_enabled()},
                           targets.value_or(none), ignore_index, top, temperature};
-  return apply_node([&] { return Logprobs::apply(hidden, w, owner, call); });
+  return apply_node([&] { return Logprobs::apply(hidden, w, scales, biases, owner, call); });
 }
 
 at::Tensor distillation(const at::Tensor& hidden, const std::optional<at::Tensor>& w, const std::optional<at::Tensor>& w_q,
@@ -816,7 +818,7 @@ at::Tensor distillation(const at::Tensor& hidden, const std::optional<at::Tensor
   const DistillCall call{{w.value_or(none), w_q.value_or(none), scales.value_or(none), biases.value_or(none), owner, kind, fwd_kind, kept,
                            at::GradMode::is_enabled()},
                          ids, teacher, mask.value_or(none), loss_kind, renormalize, reduction, beta, temperature};
-  return apply_node([&] { return Distillation::apply(hidden, w, owner, call); });
+  return apply_node([&] { return Distillation::apply(hidden, w, scales, biases, owner, call); });
 }
 
 void bind(const py::dict& entries, py::object check_fn) {

@@ -124,9 +124,9 @@ def _inputs(hidden2: torch.Tensor, head: HeadRef) -> _Inputs:
                    _native.HEAD_Q4, head.w_q)
 
 
-def _nodes(x: _Inputs):
-    """The C++ nodes, for plain tensors; None: the Python Functions serve the call, the same bits."""
-    plain = _native.plain(*(t for t in (x.hidden, x.w, x.w_q, x.scales, x.biases, x.owner) if t is not None))
+def _nodes(x: _Inputs, *others):
+    """The C++ nodes, where every tensor of the call is plain; None: the Python Functions serve it, the same bits."""
+    plain = _native.plain(*(t for t in (*x, *others) if isinstance(t, torch.Tensor)))
     return _native.nodes() if plain else None
 
 
@@ -429,7 +429,7 @@ def token_logprobs(hidden: torch.Tensor, head: HeadRef, targets: torch.Tensor | 
         x = _inputs(hidden2, head)
         y = None if targets2 is None else targets2.contiguous()
         args = (y, int(ignore_index), top, temperature)
-        nodes = _nodes(x)
+        nodes = _nodes(x, *args)
         parts = _TokenLogprobs.apply(*x, *args, torch.is_grad_enabled()) if nodes is None else nodes.logprobs(*x, _forward_kind(x), _kept_bytes(x), *args)
     *logprobs, entropy, top_lp, top_ids = parts   # (the node has none without targets)
     logprobs = logprobs[0] if logprobs else None
@@ -484,7 +484,7 @@ def distillation_loss(hidden: torch.Tensor, head: HeadRef, teacher_ids: torch.Te
         raise LossInputError(f"teacher_ids must be below V={v} (negative ones are empty slots)")
     hidden2 = hidden.reshape(-1, hidden.shape[-1])
     k = teacher_ids.shape[-1]
-    ids2, teacher2 = teacher_ids.reshape(-1, k), teacher_logprobs.detach().reshape(-1, k)
+    ids2, teacher2 = teacher_ids.reshape(-1, k), teacher_logprobs.reshape(-1, k)
     mask2 = None if mask is None else mask.reshape(-1)
     others = {"teacher_ids": teacher_ids, "teacher_logprobs": teacher_logprobs, "mask": mask}
     if _resolve(hidden2, head, others, impl, ("lists", k), allow_unverified_mlx) == "reference":
@@ -493,6 +493,6 @@ def distillation_loss(hidden: torch.Tensor, head: HeadRef, teacher_ids: torch.Te
         x = _inputs(hidden2, head)
         args = (ids2.contiguous(), _float(teacher2), None if mask2 is None else mask2.contiguous(), _KINDS[kind],
                 float(beta), temperature, int(renormalize), _REDUCTIONS[reduction])
-        nodes = _nodes(x)
+        nodes = _nodes(x, *args)
         loss = _Distillation.apply(*x, *args, torch.is_grad_enabled()) if nodes is None else nodes.distillation(*x, _forward_kind(x), _kept_bytes(x), *args)
     return loss.view(leading) if reduction == "none" else loss
