@@ -566,25 +566,22 @@ __global__ __launch_bounds__(256) void gather_groups_kernel(const int* __restric
   entries[atomicAdd(&cursor[groups[i]], 1)] = int2{(int)(i / k), (int)i};
 }
 
-// (Loaded and decided apart from the slot's own conditions: with the mask's test among them the compiler dropped the id of
-// every slot of a masked row that counts.)
-__device__ __forceinline__ bool row_counts_by(const uint8_t* mask, long row) { return (mask ? mask[row] : (uint8_t)1) != 0; }
-__device__ __forceinline__ bool listed(long long id, float lp, bool counts, long V) {
-  return (id >= 0) & (id < V) & (lp != kNegInf) & counts;
+__device__ __forceinline__ bool listed(long long id, float lp, const uint8_t* mask, long row, long V) {
+  return id >= 0 && id < V && lp != kNegInf && (!mask || mask[row]);
 }
 
 constexpr int kPerLane = kScoreTop / 64;
 
 // The column of slot lane + 64 i of row t's list, -1 where the slot is empty: not a token, nothing of the teacher's, or a column
 // that an earlier slot has.
-__device__ __forceinline__ void load_list(const int64_t* ids, const float* teacher, bool counts, long t, long V, int k, int lane,
+__device__ __forceinline__ void load_list(const int64_t* ids, const float* teacher, const uint8_t* mask, long t, long V, int k, int lane,
                                           int (&id)[kPerLane]) {
   bool on[kPerLane];
 #pragma unroll
   for (int i = 0; i < kPerLane; ++i) {
     const int s = lane + 64 * i;
     const long long y = s < k ? ids[t * k + s] : -1;
-    on[i] = listed(y, s < k ? teacher[t * k + s] : 0.f, counts, V);
+    on[i] = listed(y, s < k ? teacher[t * k + s] : 0.f, mask, t, V);
     id[i] = on[i] ? (int)y : -1;
   }
 #pragma unroll
@@ -608,7 +605,7 @@ __global__ __launch_bounds__(256) void sort_lists_kernel(const int64_t* __restri
   const long t = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (t >= n) return;
   int id[kPerLane];
-  load_list(ids, teacher, row_counts_by(mask, t), t, V, k, lane, id);
+  load_list(ids, teacher, mask, t, V, k, lane, id);
 #pragma unroll
   for (int i = 0; i < kPerLane; ++i) {
     const int s = lane + 64 * i;
@@ -901,7 +898,7 @@ __global__ __launch_bounds__(256) void distill_rows_kernel(RowParts parts, const
   // Which slots hold an outcome: a column of its own that the teacher gives something to.
   int id[kPerLane];
   if constexpr (FEW) {
-    load_list(ids, teacher, row_counts_by(mask, t), t, V, k, lane, id);
+    load_list(ids, teacher, mask, t, V, k, lane, id);
   } else {
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) {
