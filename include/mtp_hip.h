@@ -407,8 +407,8 @@ size_t mtp_logprobs_fwd_f32_workspace_bytes(int64_t n, int64_t d, int64_t v, int
 /* Per token: logprobs = x_y - lse of the target y (targets NULL: no targets, and logprobs and tgt may be NULL; a target outside
  * [0, v) counts as a logit of 0, as in mtp_lce_fwd), entropy = lse - sum p x, and the `top` largest logits (0 to
  * min(v, MTP_SCORE_MAX)), the lowest index first among equal ones: top_ids int64 [n][top], top_logprobs fp32 [n][top]. An
- * ignored target's row: 0, 0, ids -1, log probabilities -inf. lse, tgt (the target's logit before the temperature): fp32 [n],
- * for the backward. */
+ * ignored target's row: 0, 0, ids -1, log probabilities -inf. lse, tgt (the target's log probability): fp32 [n], for the
+ * backward. */
 int mtp_logprobs_fwd(const void* hidden, const void* w, const uint32_t* w_q, const void* scales, const void* biases,
                      const int64_t* targets, int64_t n, int64_t d, int64_t v, int32_t head_kind, int64_t ignore_index,
                      int32_t top, double temperature, float* logprobs, float* entropy, float* top_logprobs,

@@ -385,7 +385,7 @@ void lce32_fwd_kernel(const float* __restrict__ H, const float* __restrict__ W,
         }
       }
     }
-    if constexpr (STAT & kStatList) cursor.take<kT>(list, tokens, acc, v0, 64 * wa, h);
+    if constexpr (STAT & kStatList) cursor.take<kT, !(STAT & kStatEntropy)>(list, tokens, acc, v0, 64 * wa, h);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       float mz = kNegInf;
@@ -466,21 +466,6 @@ __device__ __forceinline__ float row_dot32(const float* __restrict__ h, const fl
     for (int d = lane; d < D; d += 64) dot = __builtin_fmaf(h[d], wr[d], dot);
   }
   return wave_sum(dot);
-}
-
-// Each token's target logit alone, 0 for a target outside the vocabulary; one wave per token.
-template <int Q4>
-__global__ __launch_bounds__(256) void lce32_target_kernel(const float* __restrict__ H, const float* __restrict__ W,
-                                                           const uint32_t* __restrict__ Wq, const float* __restrict__ Sc,
-                                                           const float* __restrict__ Bi, const int64_t* __restrict__ targets,
-                                                           int N, int D, int V, float* __restrict__ tgt) {
-  const int lane = threadIdx.x & 63;
-  const int t = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (t >= N) return;
-  const long long y = targets[t];
-  float dot = 0.f;
-  if (y >= 0 && y < (long long)V) dot = row_dot32<Q4>(H + (long)t * D, W, Wq, Sc, Bi, y, D, lane);
-  if (lane == 0) tgt[t] = dot;
 }
 
 // Per token (one wave each): merge the splits into lse, tgt = H_t . W_y as an fp32 dot product,
@@ -800,16 +785,11 @@ hipError_t launch_lce32_stats(const LceHead32& h, const float* H, int N, int D, 
   if (x.z && x.gmax) return lce32_fwd_tiles<kGroups | kStatKeep>(h, H, N, D, V, x, st);
   if (x.z && x.list.column) return lce32_fwd_tiles<kStatScaled | kStatList | kStatKeep>(h, H, N, D, V, x, st);
   if (x.z) return lce32_fwd_tiles<kEntropy | kStatKeep>(h, H, N, D, V, x, st);
+  if (x.gmax && x.list.column) return lce32_fwd_tiles<kGroups | kStatList>(h, H, N, D, V, x, st);
   if (x.gmax) return lce32_fwd_tiles<kGroups>(h, H, N, D, V, x, st);
+  if (x.u && x.list.column) return lce32_fwd_tiles<kEntropy | kStatList>(h, H, N, D, V, x, st);
   if (x.u) return lce32_fwd_tiles<kEntropy>(h, H, N, D, V, x, st);
   return lce32_fwd_tiles<kStatScaled | kStatList>(h, H, N, D, V, x, st);
-}
-
-hipError_t launch_lce32_target(const LceHead32& h, const float* H, const int64_t* targets, int N, int D, int V, float* tgt,
-                               hipStream_t st) {
-  auto kernel = h.q4 ? lce32_target_kernel<1> : lce32_target_kernel<0>;
-  hipLaunchKernelGGL(kernel, dim3((N + 3) / 4), dim3(256), 0, st, H, h.w, h.wq, h.sc, h.bi, targets, N, D, V, tgt);
-  return hipGetLastError();
 }
 
 hipError_t launch_lce32_gather(const LceHead32& h, const float* H, int D, int V, const GatherPlan& p, hipStream_t st) {

@@ -888,8 +888,8 @@ __device__ __forceinline__ bool xcd_rect_tile(int mtiles, int ntiles, int& m, in
 //
 // STAT (mtp_launch.hpp, kStat...) is what token scoring wants beside it: the softmax of z / temperature (scale2 =
 // log2(e) / temperature), the sum of 2^(x - m) (x - m) that the entropy is made of (an fma per logit), and the maximum of
-// every group of kGroup logits, which the tile's own maximum holds already; or the logits of a list of columns a row, which
-// then are in no statistic (ListCursor); with all logits themselves or without. 0 is the loss as it was.
+// every group of kGroup logits, which the tile's own maximum holds already; the logits of a list of columns a row (ListCursor),
+// which without the entropy are in no statistic; all logits themselves. 0 is the loss as it was.
 // ------------------------------------------------------------------------------------------
 template <int Q4, int STAT = 0>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
@@ -979,7 +979,7 @@ void lce_fwd_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
                 f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
       }
     }
-    if constexpr (STAT & kStatList) cursor.take<kTile>(list, tokens, acc, v0, 128 * wa, lhalf);
+    if constexpr (STAT & kStatList) cursor.take<kTile, !(STAT & kStatEntropy)>(list, tokens, acc, v0, 128 * wa, lhalf);
     // Four partial maxima and sums per token column, combined in a fixed order: four short
     // dependency chains instead of one 64 long (forward -1%).
     float pm[kNJ][4], ps[kNJ][4], pu[kNJ][4];
@@ -1237,29 +1237,6 @@ __global__ __launch_bounds__(256) void lce_fwd_finalize_kernel(
     tgt[t] = (ignored || !inrange) ? 0.f : dot;
     nll[t] = ignored ? 0.f : (l - ((!inrange) ? 0.f : dot));
   }
-}
-
-// Each token's target logit H_t . W_y alone (4-bit weights rounded to bf16, as in the product tiles), 0 for a target outside
-// the vocabulary; one wave per token.
-template <int Q4>
-__global__ __launch_bounds__(256) void lce_target_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
-                                                         const uint32_t* __restrict__ Wq, const bf16_t* __restrict__ Sc,
-                                                         const bf16_t* __restrict__ Bi, const int64_t* __restrict__ targets,
-                                                         int N, int D, int V, float* __restrict__ tgt) {
-  const int lane = threadIdx.x & 63;
-  const int t = blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (t >= N) return;
-  const long long y = targets[t];
-  float dot = 0.f;
-  if (y >= 0 && y < (long long)V) dot = row_dot<Q4, true>(H + (long)t * D, W, Wq, Sc, Bi, y, D, lane);
-  if (lane == 0) tgt[t] = dot;
-}
-
-hipError_t launch_lce_target(const LceHead& h, const bf16_t* H, const int64_t* targets, int N, int D, int V, float* tgt,
-                             hipStream_t stream) {
-  auto kernel = h.q4 ? lce_target_kernel<1> : lce_target_kernel<0>;
-  hipLaunchKernelGGL(kernel, dim3((N + 3) / 4), dim3(256), 0, stream, H, h.w, h.wq, h.sc, h.bi, targets, N, D, V, tgt);
-  return hipGetLastError();
 }
 
 // ------------------------------------------------------------------------------------------
@@ -2226,7 +2203,9 @@ hipError_t launch_lce_stats(const LceHead& h, const bf16_t* H, int N, int D, int
   if (x.z && x.gmax) return lce_fwd_tiles<kGroups | kStatKeep>(h, H, N, D, V, x, stage, stage_rows, stream);
   if (x.z && x.list.column) return lce_fwd_tiles<kStatScaled | kStatList | kStatKeep>(h, H, N, D, V, x, stage, stage_rows, stream);
   if (x.z) return lce_fwd_tiles<kEntropy | kStatKeep>(h, H, N, D, V, x, stage, stage_rows, stream);
+  if (x.gmax && x.list.column) return lce_fwd_tiles<kGroups | kStatList>(h, H, N, D, V, x, stage, stage_rows, stream);
   if (x.gmax) return lce_fwd_tiles<kGroups>(h, H, N, D, V, x, stage, stage_rows, stream);
+  if (x.u && x.list.column) return lce_fwd_tiles<kEntropy | kStatList>(h, H, N, D, V, x, stage, stage_rows, stream);
   if (x.u) return lce_fwd_tiles<kEntropy>(h, H, N, D, V, x, stage, stage_rows, stream);
   return lce_fwd_tiles<kStatScaled | kStatList>(h, H, N, D, V, x, stage, stage_rows, stream);
 }

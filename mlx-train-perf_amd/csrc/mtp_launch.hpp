@@ -59,7 +59,7 @@ hipError_t launch_lce_fwd(const LceHead& h, const bf16_t* H, const int64_t* targ
 // Token scoring (score_kernels.hip) takes the forward's tiles with more of their statistics. A forward's STAT is a sum of:
 enum { kStatScaled = 1, kStatEntropy = 2, kStatGroups = 4, kStatList = 8, kStatKeep = 16 };
 constexpr int kGroup = 128;  // consecutive logits whose maximum a forward keeps
-// Logits to put away of each row: ascending columns (kNoColumn past the last) to their places in z. The statistics leave them out.
+// Logits to put away of each row: ascending columns (kNoColumn past the last) to their places in z. Statistics without an entropy leave them out.
 constexpr int kNoColumn = 0x7fffffff;
 struct ScoreList {
   const int* column;  // [N][k], or null
@@ -78,8 +78,6 @@ struct ScoreStats {
 };
 hipError_t launch_lce_stats(const LceHead& h, const bf16_t* H, int N, int D, int V, const ScoreStats& st, bf16_t* stage,
                             long stage_rows, hipStream_t stream);
-hipError_t launch_lce_target(const LceHead& h, const bf16_t* H, const int64_t* targets, int N, int D, int V, float* tgt,
-                             hipStream_t stream);
 
 // The gradient of a loss of softmax(z / temperature) by the logits z that is p (alpha + beta z) but for k columns a row.
 // Rows with neither factor get zeros, whatever their hidden state holds.
@@ -180,8 +178,6 @@ hipError_t launch_lce32_bwd(const LceHead32& h, const float* H, const int64_t* t
                             float* dW, float* Gbuf, hipStream_t stream, const AffineGrad* affine = nullptr);
 hipError_t launch_lce32_stats(const LceHead32& h, const float* H, int N, int D, int V, const ScoreStats& st,
                               hipStream_t stream);  // [lce32_fwd_nsplit][N]
-hipError_t launch_lce32_target(const LceHead32& h, const float* H, const int64_t* targets, int N, int D, int V, float* tgt,
-                               hipStream_t stream);
 hipError_t launch_attn32_fwd(const AttnShape& sh, const float* q, const float* k, const float* v,
                              const int32_t* seg_start, float* o, float* lse, hipStream_t stream);
 hipError_t launch_attn32_dkv_reduce(const float* part, int ns, long plane, float* dk, float* dv, hipStream_t stream);

@@ -625,6 +625,15 @@ __global__ __launch_bounds__(256) void sort_lists_kernel(const int64_t* __restri
   }
 }
 
+// A target as its row's list of one.
+__global__ __launch_bounds__(256) void target_columns_kernel(const int64_t* __restrict__ targets, long long ignore_index, long n, long V,
+                                                             int* __restrict__ column) {
+  const long t = (long)blockIdx.x * 256 + threadIdx.x;
+  if (t >= n) return;
+  const long long y = targets[t];
+  column[t] = y != ignore_index && y >= 0 && y < V ? (int)y : kNoColumn;
+}
+
 // ------------------------------------------------------------------------------------------
 // Scoring, per token: the statistics of its row, the target's log probability, the groups to look into (and, where the logits
 // were kept, the alternatives themselves). One workgroup a token: bound by the chain of loads, barriers and counts where there are few tokens (12 us
@@ -677,13 +686,17 @@ __device__ __forceinline__ void merge_row(const RowParts& p, long t, float& m, f
   for (int i = 1; i < kPick / 64; ++i) lse2_merge(m, s, u, x[0][i], x[1][i], x[2][i]);
 }
 
+// The log probability of a logit z by norm = (m, log2 s) of its row: relative to the row's largest logit, so that it is right to the
+// digits of what it leaves of 0. As z / temperature - lse it had the last digits of a logit: 2e-6 at 32, 1 - p of 8.5e-5 off by 3%.
+__device__ __forceinline__ float log_p(float z, float c2, float2 norm) { return (__builtin_fmaf(z, c2, -norm.x) - norm.y) * kLn2; }
+
 // The K largest of a row's candidate logits, ngroups kGroup of them in LDS as keys, in order, with their log probabilities.
 // The groups ascend, so positions ascend with the index. `least`: the K-th largest of the groups' maxima (0 with fewer than K
 // groups), below which nothing is chosen: mostly a few more than K are left, and each one's place is its count of those before
-// it. A target among them takes its logit from here.
+// it. A target among them takes its log probability from here.
 template <int MC>
 __device__ __forceinline__ void write_top(const uint32_t* key, const int* group, int ngroups, int K, uint32_t least, int V,
-                                          float inv_t, float lse, long t, long long target, const LogprobsOut& out, PickScratch& s) {
+                                          float c2, float2 norm, long t, long long target, const LogprobsOut& out, PickScratch& s) {
   const int M = ngroups * kGroup;
   int n = list_from(key, M, least, s);
   if (n > kRanked || n < K) {  // many equal ones; or logits that are no numbers
@@ -694,13 +707,10 @@ __device__ __forceinline__ void write_top(const uint32_t* key, const int* group,
     const int rank = rank_of(s.list[i], n, s);
     if (rank >= K) continue;
     const int p = entry_at(s.list[i]), id = group[p / kGroup] * kGroup + p % kGroup;
-    const float z = key_value(entry_key(s.list[i])), lp = z * inv_t - lse;
+    const float lp = log_p(key_value(entry_key(s.list[i])), c2, norm);
     out.top_ids[t * K + rank] = id < V ? id : -1;
     out.top_logprobs[t * K + rank] = lp;
-    if (id == target) {
-      out.tgt[t] = z;
-      out.logprobs[t] = lp;
-    }
+    if (id == target) out.tgt[t] = out.logprobs[t] = lp;
   }
 }
 
@@ -711,10 +721,11 @@ template <bool KEPT, int MG, int MC>
 __global__ __launch_bounds__(kPick) void score_rows_kernel(RowParts parts, const float* __restrict__ gmax, int ngroups, int ldg,
                                                            const float* __restrict__ Z, long ldz,
                                                            const int64_t* __restrict__ targets, long long ignore_index, int V,
-                                                           float inv_t, int K, int take, LogprobsOut out,
+                                                           float c2, int K, int take, LogprobsOut out,
                                                            int* __restrict__ groups, int* __restrict__ counts,
-                                                           uint32_t* __restrict__ floors) {
+                                                           uint32_t* __restrict__ floors, float2* __restrict__ norms) {
   __shared__ float x[3][kPick / 64];
+  __shared__ float2 norm;
   __shared__ PickScratch scratch;
   __shared__ uint32_t key[MG > MC ? MG : MC > 0 ? MC : 1];
   __shared__ int group[kScoreTop];
@@ -736,16 +747,13 @@ __global__ __launch_bounds__(kPick) void score_rows_kernel(RowParts parts, const
   }
   float m, s, u;
   merge_row(parts, t, m, s, u, x);
-  const float lse = (m + fast_log2(s)) * kLn2;
   const bool in = y >= 0 && y < V;
   if (tid == 0) {
+    norm = float2{m, fast_log2(s)};
+    const float lse = (m + norm.y) * kLn2;
     out.lse[t] = lse;
-    out.entropy[t] = (fast_log2(s) - u / s) * kLn2;
-    if (targets) {
-      const float z = KEPT ? (in ? Z[t * ldz + y] : 0.f) : out.tgt[t];
-      out.tgt[t] = z;
-      out.logprobs[t] = in ? z * inv_t - lse : -lse;
-    }
+    out.entropy[t] = (norm.y - u / s) * kLn2;
+    if (targets) out.tgt[t] = out.logprobs[t] = in ? log_p(KEPT ? Z[t * ldz + y] : out.tgt[t], c2, norm) : -lse;
   }
   if constexpr (MG > 0) {
     each<5>(ngroups, [&](int i) { return gmax[t * ldg + i]; }, [&](int i, float x) { key[i] = order_key(x); });
@@ -756,11 +764,14 @@ __global__ __launch_bounds__(kPick) void score_rows_kernel(RowParts parts, const
       each<5>(take * kGroup, [&](int i) { return Z[t * ldz + (long)group[i / kGroup] * kGroup + i % kGroup]; },
               [&](int i, float x) { key[i] = group[i / kGroup] * kGroup + i % kGroup < V ? order_key(x) : 0u; });
       __syncthreads();
-      write_top<MC>(key, group, take, K, least, V, inv_t, lse, t, targets ? y : -1, out, scratch);
+      write_top<MC>(key, group, take, K, least, V, c2, norm, t, targets ? y : -1, out, scratch);
     } else if (tid < take) {
       groups[t * take + tid] = group[tid];
       atomicAdd(&counts[group[tid]], 1);
-      if (tid == 0) floors[t] = least;
+      if (tid == 0) {
+        floors[t] = least;
+        norms[t] = norm;
+      }
     }
   }
 }
@@ -768,8 +779,9 @@ __global__ __launch_bounds__(kPick) void score_rows_kernel(RowParts parts, const
 // After the gather: the alternatives from the chosen groups' logits [N][take][kGroup].
 template <int MC>
 __global__ __launch_bounds__(kPick) void score_top_kernel(const float* __restrict__ rows, const int* __restrict__ groups,
-                                                          const uint32_t* __restrict__ floors, const int64_t* __restrict__ targets, int V, float inv_t, int K,
-                                                          int take, LogprobsOut out) {
+                                                          const uint32_t* __restrict__ floors, const float2* __restrict__ norms,
+                                                          const int64_t* __restrict__ targets, int V, float c2, int K, int take,
+                                                          LogprobsOut out) {
   __shared__ PickScratch scratch;
   __shared__ uint32_t key[MC];
   __shared__ int group[kScoreTop];
@@ -779,7 +791,7 @@ __global__ __launch_bounds__(kPick) void score_top_kernel(const float* __restric
   for (int i = tid; i < take; i += kPick) group[i] = groups[t * take + i];
   each<4>(take * kGroup, [&](int i) { return rows[t * take * kGroup + i]; }, [&](int i, float x) { key[i] = order_key(x); });
   __syncthreads();
-  write_top<MC>(key, group, take, K, floors[t], V, inv_t, out.lse[t], t, targets ? targets[t] : -1, out, scratch);
+  write_top<MC>(key, group, take, K, floors[t], V, c2, norms[t], t, targets ? targets[t] : -1, out, scratch);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -1087,7 +1099,7 @@ __global__ __launch_bounds__(256) void logprobs_coef_kernel(const float* __restr
   const long long y = targets ? targets[t] : -1;
   const bool dead = targets && y == ignore_index, in = !dead && targets && y >= 0 && y < V;
   const float a = !dead && d_logprobs ? d_logprobs[t] : 0.f, b = !dead && d_entropy ? d_entropy[t] : 0.f;
-  const float up = lse[t] - entropy[t], l = in ? finite_exponent(tgt[t] * inv_t - lse[t]) : 0.f;
+  const float up = lse[t] - entropy[t], l = in ? finite_exponent(tgt[t]) : 0.f;
   alpha[t] = (b * up - a) * inv_t;
   beta[t] = -b * inv_t * inv_t;
   columns[t] = in ? (int)y : -1;
@@ -1186,6 +1198,7 @@ struct Scratch {
   float *m, *s, *u, *gmax, *z, *gs, *gu, *cand, *picks, *row_loss;
   int *chosen, *counts, *column, *slot, *row_counts;
   uint32_t* floors;
+  float2* norms;
   int2* entries;
   GatherTile* tiles;
   bf16_t* stage;
@@ -1235,6 +1248,7 @@ Scratch carve(const ScoreShape& sh, int f32, int q4, int top, int k_list, float*
     if (entries) {
       x.chosen = c.take<int>(entries);
       x.floors = c.take<uint32_t>(x.rows);
+      x.norms = c.take<float2>(x.rows);
       x.cand = c.take<float>(entries * kGroup);
       x.counts = c.take<int>(x.groups);
       x.entries = c.take<int2>(entries);
@@ -1242,6 +1256,7 @@ Scratch carve(const ScoreShape& sh, int f32, int q4, int top, int k_list, float*
       if (x.max_tiles > entries) x.max_tiles = (int)entries;
       x.tiles = c.take<GatherTile>(x.max_tiles);
     }
+    if (!k_list && !x.kept) x.column = c.take<int>(x.rows);  // the targets'
     if (k_list) {
       x.column = c.take<int>(x.rows * k_list);
       x.slot = c.take<int>(x.rows * k_list);
@@ -1315,9 +1330,10 @@ RowParts row_parts(const Scratch& x, const ScoreHead& h, long n, long v, float c
   return RowParts{x.m, x.s, x.u ? x.u : x.s, ns, n, 1, 1.f};
 }
 
-// The product over rows [r0, r0 + n) with its statistics.
-hipError_t tile_stats(const ScoreHead& h, const ScoreShape& sh, const Scratch& x, long r0, long n, float c2, int k, hipStream_t st) {
-  const ScoreStats stats{c2, x.m, x.s, x.u, x.gmax, x.ldg, x.kept ? x.z : nullptr, x.ldz, ScoreList{x.column, x.picks, k}};
+// The product over rows [r0, r0 + n) with its statistics; k columns a row to picks.
+hipError_t tile_stats(const ScoreHead& h, const ScoreShape& sh, const Scratch& x, long r0, long n, float c2, int k, float* picks,
+                      hipStream_t st) {
+  const ScoreStats stats{c2, x.m, x.s, x.u, x.gmax, x.ldg, x.kept ? x.z : nullptr, x.ldz, ScoreList{k ? x.column : nullptr, picks, k}};
   if (h.f32)
     return launch_lce32_stats(h.h32, static_cast<const float*>(h.hidden) + r0 * sh.d, (int)n, (int)sh.d, (int)sh.v, stats, st);
   return launch_lce_stats(h.h, static_cast<const bf16_t*>(h.hidden) + r0 * sh.d, (int)n, (int)sh.d, (int)sh.v, stats, x.stage,
@@ -1367,24 +1383,24 @@ hipError_t launch_logprobs_fwd(const ScoreHead& head, const ScoreShape& sh, cons
                           top ? o.top_ids + r0 * top : nullptr, o.lse + r0, o.tgt ? o.tgt + r0 : nullptr};
     const int64_t* y = targets ? targets + r0 : nullptr;
     if (x.kept) {
-      const hipError_t e = x.few ? few_logits(h, sh, x, c2, st) : tile_stats(h, sh, x, r0, n, c2, 0, st);
+      const hipError_t e = x.few ? few_logits(h, sh, x, c2, st) : tile_stats(h, sh, x, r0, n, c2, 0, nullptr, st);
       if (e != hipSuccess) return e;
       auto kernel = !top ? score_rows_kernel<true, 0, 0>
                     : x.take <= 16 && x.groups <= 2048 ? score_rows_kernel<true, 2048, 2048>
                     : x.take <= 64 && x.groups <= 2048 ? score_rows_kernel<true, 2048, 64 * kGroup>
                                                        : score_rows_kernel<true, kMaxGroups, kScoreTop * kGroup>;
       hipLaunchKernelGGL(kernel, dim3((unsigned)n), dim3(kPick), 0, st, row_parts(x, h, n, sh.v, c2), x.gmax, x.groups, x.ldg, x.z,
-                         x.ldz, y, ignore_index, V, sh.inv_t, top, x.take, out, nullptr, nullptr, nullptr);
+                         x.ldz, y, ignore_index, V, c2, top, x.take, out, nullptr, nullptr, nullptr, nullptr);
       MTP_LAUNCHED();
       continue;
     }
-    hipError_t e = tile_stats(h, sh, x, r0, n, c2, 0, st);
-    if (e != hipSuccess) return e;
+    hipError_t e;
     if (y) {
-      e = h.f32 ? launch_lce32_target(h.h32, static_cast<const float*>(h.hidden) + r0 * sh.d, y, (int)n, (int)sh.d, V, out.tgt, st)
-                : launch_lce_target(h.h, static_cast<const bf16_t*>(h.hidden) + r0 * sh.d, y, (int)n, (int)sh.d, V, out.tgt, st);
-      if (e != hipSuccess) return e;
+      hipLaunchKernelGGL(target_columns_kernel, dim3((unsigned)ceil_div(n, 256)), dim3(256), 0, st, y, ignore_index, n, sh.v, x.column);
+      MTP_LAUNCHED();
     }
+    e = tile_stats(h, sh, x, r0, n, c2, y ? 1 : 0, out.tgt, st);
+    if (e != hipSuccess) return e;
     if (top) {
       hipLaunchKernelGGL(zero_counts_kernel, dim3((unsigned)ceil_div(x.groups, 256)), dim3(256), 0, st, x.counts, x.groups);
       MTP_LAUNCHED();
@@ -1392,7 +1408,7 @@ hipError_t launch_logprobs_fwd(const ScoreHead& head, const ScoreShape& sh, cons
     auto rows = !top ? score_rows_kernel<false, 0, 0>
                      : x.groups <= 2048 ? score_rows_kernel<false, 2048, 0> : score_rows_kernel<false, kMaxGroups, 0>;
     hipLaunchKernelGGL(rows, dim3((unsigned)n), dim3(kPick), 0, st, row_parts(x, h, n, sh.v, c2), x.gmax, x.groups, x.ldg, nullptr, 0L, y,
-                       ignore_index, V, sh.inv_t, top, x.take, out, x.chosen, x.counts, x.floors);
+                       ignore_index, V, c2, top, x.take, out, x.chosen, x.counts, x.floors, x.norms);
     MTP_LAUNCHED();
     if (!top) continue;
     hipLaunchKernelGGL(gather_tiles_kernel, dim3(1), dim3(1024), 0, st, x.counts, x.groups, x.tiles, x.max_tiles);
@@ -1403,7 +1419,7 @@ hipError_t launch_logprobs_fwd(const ScoreHead& head, const ScoreShape& sh, cons
     e = gather(h, sh, x, r0, st);
     if (e != hipSuccess) return e;
     auto best = x.take <= 16 ? score_top_kernel<16 * kGroup> : x.take <= 64 ? score_top_kernel<64 * kGroup> : score_top_kernel<kScoreTop * kGroup>;
-    hipLaunchKernelGGL(best, dim3((unsigned)n), dim3(kPick), 0, st, x.cand, x.chosen, x.floors, y, V, sh.inv_t, top, x.take, out);
+    hipLaunchKernelGGL(best, dim3((unsigned)n), dim3(kPick), 0, st, x.cand, x.chosen, x.floors, x.norms, y, V, c2, top, x.take, out);
     MTP_LAUNCHED();
   }
   return hipSuccess;
@@ -1440,7 +1456,7 @@ hipError_t launch_distill_fwd(const ScoreHead& head, const ScoreShape& sh, const
                          x.slot);
       MTP_LAUNCHED();
     }
-    const hipError_t e = x.few ? few_logits(h, sh, x, c2, st) : tile_stats(h, sh, x, r0, n, c2, p.k, st);
+    const hipError_t e = x.few ? few_logits(h, sh, x, c2, st) : tile_stats(h, sh, x, r0, n, c2, p.k, x.picks, st);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(kernel, dim3((unsigned)ceil_div(n, 4)), dim3(256), 0, st, row_parts(x, h, n, sh.v, c2), x.column,
                        x.slot, x.picks, x.z, x.ldz, id, lp, see, n, sh.v, c2, p.inv_t, p.k, p.renormalize, p.beta, row_loss + r0,

@@ -235,7 +235,7 @@ def _score_forward(x: _Inputs, targets, ignore_index: int, top: int, temperature
 
 
 class _TokenLogprobs(torch.autograd.Function):
-    """Saves each token's log-sum-exp, entropy and target logit, and few enough logits; more of them the backward forms again.
+    """Saves each token's log-sum-exp, entropy and log probability, and few enough logits; more of them the backward forms again.
     record: whether autograd is (inside a forward it is off, and what asks for a gradient asks under no_grad too)."""
 
     @staticmethod
