@@ -1211,8 +1211,8 @@ struct Scratch {
 bool keep_logits(const ScoreShape& sh) { return 4 * sh.n * sh.v <= kKeptBytes; }
 // Tokens of one pass that does: a row is a whole number of groups, which a small vocabulary is far from.
 long kept_rows(long n, long ldz) {
-  const long most = kKeptBytes / (4 * ldz) / 256 * 256;
-  return n < most ? n : most > 256 ? most : 256;
+  const long most = kKeptBytes / (4 * ldz);
+  return n <= most ? n : most < 256 ? most : most / 256 * 256;
 }
 
 // k_list: length of a teacher's list (0: scoring, with `top` alternatives).

@@ -17,6 +17,15 @@ def test_workspaces(n, v):
             assert 0 < size(n, 64, v, _native.HEAD_DENSE, top, 0) <= 280 << 20
 
 
+@pytest.mark.parametrize(("n", "v"), [(1, 2 ** 21), (10, 2 ** 21), (32, 2 ** 21 - 1), (60, 2 ** 20), (511, 131000), (200, 300)])
+def test_no_more_than_the_tokens_that_there_are(n, v):
+    """fp32 hidden dims that no chunk of 4 divides: few tokens, tiles, their logits."""
+    lib = _native.load()
+    ldz = int(lib.mtp_score_logits_ld(v))
+    size = lib.mtp_logprobs_fwd_f32_workspace_bytes(n, 33, v, _native.HEAD_DENSE, 5, 0)
+    assert n * ldz * 4 <= size <= n * ldz * 4 + n * (ldz // 128 + 1) * 4 + (8 << 20)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 @pytest.mark.parametrize(("n", "v"), [(300001, 130), (600000, 5)])
