@@ -201,8 +201,8 @@ __device__ __forceinline__ uint32_t pick_few(const uint32_t* key, int M, int K, 
 // fragments straight from memory to registers, each loaded for the next slab as soon as its product has gone out (a whole slab in
 // flight a wave, 8 KiB of a dense head, 4 of a 4-bit one), the tokens' slab (NB blocks of 32) through LDS, one barrier a
 // slab. The registers and, up to 16 tokens, the LDS leave room for 5 workgroups a CU: all 1187 groups of 151936 run at once
-// (16 tokens over a 4-bit head, 4 workgroups and 5: 157 and 130 us). 4096 x 151936: a dense head's 1.24 GB in 245 us (5.1 TB/s, as
-// a library product of one row), a 4-bit head's 0.35 GB in 104, where the vector units are busy for some 60.
+// (16 tokens over a 4-bit head, 4 workgroups and 5: 157 and 130 us). 4096 x 151936: a dense head's 1.24 GB in 242 us (5.1 TB/s, as
+// a library product of one row), a 4-bit head's 0.35 GB in 108, where the vector units are busy for some 60.
 // ------------------------------------------------------------------------------------------
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base, long bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, bytes > 0x7fffffffL ? 0x7fffffff : (int)bytes, 0x00020000);
@@ -430,7 +430,7 @@ void lce_few_kernel(const T* __restrict__ H, const T* __restrict__ W, const uint
 // ------------------------------------------------------------------------------------------
 // The logits of a gather (GatherPlan): C[v][entry] = W_v . H_token, 128 x 128 a workgroup (4 waves of 64 x 64), 64-deep stages
 // through registers, a stage ahead. Bound by what it fetches again: the head once (nearly every group is wanted by some token) and
-// the hidden rows for every entry (2 D bytes each). 8 of 8192 x 4096 x 151936: 346 us, 250 of them the head's bytes.
+// the hidden rows for every entry (2 D bytes each). 8 of 8192 x 4096 x 151936: 344 us, 250 of them the head's bytes.
 // ------------------------------------------------------------------------------------------
 template <int Q4>
 __global__ __launch_bounds__(256) void lce_gather_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
@@ -637,7 +637,7 @@ __global__ __launch_bounds__(256) void target_columns_kernel(const int64_t* __re
 // ------------------------------------------------------------------------------------------
 // Scoring, per token: the statistics of its row, the target's log probability, the groups to look into (and, where the logits
 // were kept, the alternatives themselves). One workgroup a token: bound by the chain of loads, barriers and counts where there are few tokens (12 us
-// for 16 x 151936, 17 for 20 alternatives of one), by its vector instructions where there are many (8192: 51).
+// for 16 x 151936, 15 for 20 alternatives of one), by its vector instructions where there are many (8192: 50).
 // ------------------------------------------------------------------------------------------
 // Partials of one row: value i at base[i * stride]. m: of x in the log2 domain, or (few tokens) of z, times c2.
 struct RowParts {
@@ -803,7 +803,7 @@ __global__ __launch_bounds__(kPick) void score_top_kernel(const float* __restric
 //   jsd      b KL(t | m) + (1 - b) KL(q | m), m = b t + (1 - b) q:  f = (1 - b) log(q / m), f_R = (1 - b) log(R / m_R)
 // the gradient by a logit is p (f_R - F) off the list and q (f - F) on it, F = sum q f + R f_R. R and T (but in F) are at least
 // kTailFloor. From the partials on in 64 bits: T is a difference, and the products above are what take the time
-// (8192 lists of 64: 14 us, their sorting 38, the products 21.6 ms).
+// (8192 lists of 64: 16 us, their sorting 38, the products 21.7 ms).
 // ------------------------------------------------------------------------------------------
 __device__ __forceinline__ double wave_sum64(double v) {
 #pragma unroll

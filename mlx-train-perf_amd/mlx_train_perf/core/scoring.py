@@ -454,7 +454,8 @@ def distillation_loss(hidden: torch.Tensor, head: HeadRef, teacher_ids: torch.Te
     `renormalize`: the teacher's slots are logits, t = softmax(them / temperature) over the list, with nothing outside it (not
     with "reverse").
     `mask` (hidden's leading dims, bool or uint8) says which tokens count; those without any outcome in their list do
-    not. "mean" is over the tokens that count (0 without any); "none" gives them 0. The gradient goes to `hidden` and to a
+    not. "mean" is over the tokens that count (0 without any); "none" gives them 0. There is no factor of temperature squared: multiply
+    by it for gradients of one size at any temperature. The gradient goes to `hidden` and to a
     trainable dense head. `validate_ids` checks at one host sync that ids lie below V; unchecked, such slots are empty."""
     if reduction not in _REDUCTIONS:
         raise LossInputError(f"unknown reduction {reduction!r}; expected 'none', 'mean' or 'sum'")
