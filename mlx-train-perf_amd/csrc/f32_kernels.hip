@@ -350,7 +350,7 @@ void lce32_fwd_kernel(const float* __restrict__ H, const float* __restrict__ W,
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, wa = w & 1, wb = w >> 1, h = lane >> 5;
   RowSrc hb{H + (long)t0 * D, D, N - t0, D, aligned16(H) && D % 4 == 0};
   float m[2] = {kNegInf, kNegInf}, s[2] = {0.f, 0.f}, u[2] = {0.f, 0.f};
-  ListCursor<2> cursor;
+  std::conditional_t<(STAT & kStatEntropy) != 0, TargetCursor<2>, ListCursor<2>> cursor;
   const int tokens[2] = {t0 + 64 * wb + (lane & 31), t0 + 64 * wb + 32 + (lane & 31)};
   if constexpr (STAT & kStatList) cursor.start(list, tokens, N, vt0 * kT);
   for (int vt = vt0; vt < vt1; ++vt) {
@@ -385,7 +385,7 @@ void lce32_fwd_kernel(const float* __restrict__ H, const float* __restrict__ W,
         }
       }
     }
-    if constexpr (STAT & kStatList) cursor.take<kT, !(STAT & kStatEntropy)>(list, tokens, acc, v0, 64 * wa, h);
+    if constexpr (STAT & kStatList) cursor.template take<kT>(list, tokens, acc, v0, 64 * wa, h);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       float mz = kNegInf;

@@ -888,8 +888,8 @@ __device__ __forceinline__ bool xcd_rect_tile(int mtiles, int ntiles, int& m, in
 //
 // STAT (mtp_launch.hpp, kStat...) is what token scoring wants beside it: the softmax of z / temperature (scale2 =
 // log2(e) / temperature), the sum of 2^(x - m) (x - m) that the entropy is made of (an fma per logit), and the maximum of
-// every group of kGroup logits, which the tile's own maximum holds already; the logits of a list of columns a row (ListCursor),
-// which without the entropy are in no statistic; all logits themselves. 0 is the loss as it was.
+// every group of kGroup logits, which the tile's own maximum holds already; the logits of a list of columns a row, which then are
+// in no statistic (ListCursor), with the entropy those of a target a row, which are (TargetCursor); all logits themselves. 0 is the loss as it was.
 // ------------------------------------------------------------------------------------------
 template <int Q4, int STAT = 0>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
@@ -939,7 +939,7 @@ void lce_fwd_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
     u[j] = 0.f;
   }
 
-  ListCursor<kNJ> cursor;
+  std::conditional_t<(STAT & kStatEntropy) != 0, TargetCursor<kNJ>, ListCursor<kNJ>> cursor;
   int tokens[kNJ];
   if constexpr (STAT & kStatList) {
 #pragma unroll
@@ -979,7 +979,7 @@ void lce_fwd_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
                 f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
       }
     }
-    if constexpr (STAT & kStatList) cursor.take<kTile, !(STAT & kStatEntropy)>(list, tokens, acc, v0, 128 * wa, lhalf);
+    if constexpr (STAT & kStatList) cursor.template take<kTile>(list, tokens, acc, v0, 128 * wa, lhalf);
     // Four partial maxima and sums per token column, combined in a fixed order: four short
     // dependency chains instead of one 64 long (forward -1%).
     float pm[kNJ][4], ps[kNJ][4], pu[kNJ][4];

@@ -59,7 +59,8 @@ hipError_t launch_lce_fwd(const LceHead& h, const bf16_t* H, const int64_t* targ
 // Token scoring (score_kernels.hip) takes the forward's tiles with more of their statistics. A forward's STAT is a sum of:
 enum { kStatScaled = 1, kStatEntropy = 2, kStatGroups = 4, kStatList = 8, kStatKeep = 16 };
 constexpr int kGroup = 128;  // consecutive logits whose maximum a forward keeps
-// Logits to put away of each row: ascending columns (kNoColumn past the last) to their places in z. Statistics without an entropy leave them out.
+// Logits to put away of each row: ascending columns (kNoColumn past the last) to their places in z, and out of the statistics; with an entropy one
+// column a row (k = 1), which stays in them.
 constexpr int kNoColumn = 0x7fffffff;
 struct ScoreList {
   const int* column;  // [N][k], or null

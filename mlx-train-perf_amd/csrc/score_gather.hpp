@@ -34,7 +34,7 @@ __device__ __forceinline__ void store_gathered(const f32x16 (&acc)[NI][NJ], cons
 // listed column that no tile has passed, `at` its place. A tile's lanes hold the logits of column li = 32 i + 8 (r / 4) + 4 half
 // + r % 4 of their wave's part of it, so a listed one is in one lane and one of 16 NI registers: a tree of selects by the bits
 // of li finds it (16 NI of them) and a store puts it away. A teacher's list then leaves the tile (its registers become -inf), so
-// that the statistics are those of what no list has: what a list leaves of 1 is a sum of its own and no difference. A target stays.
+// that the statistics are those of what no list has: what a list leaves of 1 is a sum of its own and no difference.
 // Most tiles have none of a wave's tokens' columns, and the rest few.
 // ------------------------------------------------------------------------------------------
 // acc[BITS' registers from `first`], the one whose index has the bits of li: register bits 0, 1 are bits 0, 1 of li, the ones
@@ -71,8 +71,8 @@ struct ListCursor {
       if (lo < l.k) next[j] = row[lo];
     }
   }
-  // The tile [v0, v0 + SIZE): the wave holds its rows [part, part + 32 NI). OUT: what is put away leaves the tile.
-  template <int SIZE, bool OUT, int NI>
+  // The tile [v0, v0 + SIZE): the wave holds its rows [part, part + 32 NI).
+  template <int SIZE, int NI>
   __device__ __forceinline__ void take(const ScoreList& l, const int (&t)[NJ], f32x16 (&acc)[NI][NJ], int v0, int part, int half) {
     constexpr int kBits = NI == 4 ? 6 : 5, kWords = NI / 2;
     static_assert(NI == 4 || NI == 2, "16 NI registers");
@@ -85,11 +85,9 @@ struct ListCursor {
           const float z = select_logit<kBits>(acc, j, li, 0);
           if (li >= 0 && li < 32 * NI && ((li >> 2) & 1) == half) {
             l.z[(long)t[j] * l.k + at[j]] = z;
-            if constexpr (OUT) {
-              const int r = (li & 3) | (li >> 3) << 2;
+            const int r = (li & 3) | (li >> 3) << 2;
 #pragma unroll
-              for (int w = 0; w < kWords; ++w) taken[w] |= (r >> 5) == w ? 1u << (r & 31) : 0u;
-            }
+            for (int w = 0; w < kWords; ++w) taken[w] |= (r >> 5) == w ? 1u << (r & 31) : 0u;
           }
           ++at[j];
           next[j] = at[j] < l.k ? l.column[(long)t[j] * l.k + at[j]] : kNoColumn;
@@ -97,10 +95,32 @@ struct ListCursor {
       }
 #pragma unroll
       for (int w = 0; w < kWords; ++w)
-        if (OUT && __any(taken[w]))
+        if (__any(taken[w]))
 #pragma unroll
           for (int r = 0; r < 32; ++r)
             if (taken[w] >> r & 1) acc[2 * w + (r >> 4)][j][r & 15] = kNegInf;
+    }
+  }
+};
+
+// The same for lists of one, targets, which stay in the statistics: nothing to follow.
+template <int NJ>
+struct TargetCursor {
+  int column[NJ];
+  __device__ __forceinline__ void start(const ScoreList& l, const int (&t)[NJ], int N, int) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) column[j] = t[j] < N ? l.column[t[j]] : kNoColumn;
+  }
+  template <int SIZE, int NI>
+  __device__ __forceinline__ void take(const ScoreList& l, const int (&t)[NJ], const f32x16 (&acc)[NI][NJ], int v0, int part, int half) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const int li = column[j] - v0 - part;
+      const bool here = li >= 0 && li < 32 * NI && ((li >> 2) & 1) == half;
+      if (__any(here)) {
+        const float z = select_logit<NI == 4 ? 6 : 5>(acc, j, li, 0);
+        if (here) l.z[t[j]] = z;
+      }
     }
   }
 };
