@@ -217,9 +217,9 @@ def _score_forward(x: _Inputs, targets, ignore_index: int, top: int, temperature
     dev = x.hidden.device
     f32 = x.hidden.dtype == torch.float32
     kind = _forward_kind(x)
-    rows = torch.empty((4 if targets is not None else 2, n), dtype=torch.float32, device=dev)
-    entropy, lse = rows[0], rows[1]
-    logprobs, tgt = (rows[2], rows[3]) if targets is not None else (None, None)
+    # (results of their own, not views of one: a caller may change them in place)
+    entropy, lse = (torch.empty(n, dtype=torch.float32, device=dev) for _ in range(2))
+    logprobs, tgt = (torch.empty_like(lse) if targets is not None else None for _ in range(2))
     top_lp = torch.empty((n, top), dtype=torch.float32, device=dev)
     top_ids = torch.empty((n, top), dtype=torch.int64, device=dev)
     size = lib.mtp_logprobs_fwd_f32_workspace_bytes if f32 else lib.mtp_logprobs_fwd_workspace_bytes

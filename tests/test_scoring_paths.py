@@ -85,3 +85,28 @@ def test_a_4bit_heads_scales_and_biases(asks, nodes, monkeypatch):
             continue
         grads = torch.autograd.grad(out, list(t[k] for k in asks), allow_unused=True)
         assert all((g is not None) == (k == "hidden") for k, g in zip(asks, grads))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nodes", [True, False])
+def test_results_can_be_changed_in_place(nodes, monkeypatch):
+    """What a call hands out is not what its backward reads; of the entropy, which it does read, autograd says so."""
+    if not nodes:
+        monkeypatch.setattr(_native, "_nodes", False)
+    hidden, hd, _, _, _ = _tensors("cuda")
+    y = torch.arange(6, device="cuda")
+
+    def grad(change):
+        h = hidden.clone().requires_grad_(True)
+        r = token_logprobs(h, hd, y, top=2)
+        logprobs = change(r.logprobs)
+        r.top_logprobs.zero_()
+        r.top_ids.zero_()
+        return torch.autograd.grad(logprobs.sum() + r.entropy.sum(), h)[0]
+
+    assert torch.equal(grad(lambda x: x.mul_(2.0)), grad(lambda x: x * 2.0))
+    h = hidden.clone().requires_grad_(True)
+    entropy = token_logprobs(h, hd, y).entropy
+    entropy.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        entropy.sum().backward()
