@@ -587,7 +587,7 @@ __device__ __forceinline__ void load_list(const int64_t* ids, const float* teach
 #pragma unroll
   for (int i = 0; i < kPerLane; ++i)
     for (int j = 0; j < 64 && 64 * i + j < k; ++j) {
-      const int other = __shfl(id[i], j, 64);
+      const int other = __builtin_amdgcn_readlane(id[i], j);
 #pragma unroll
       for (int o = 0; o < kPerLane; ++o)
         if (64 * i + j < lane + 64 * o && other >= 0 && other == id[o]) on[o] = false;
@@ -614,7 +614,7 @@ __global__ __launch_bounds__(256) void sort_lists_kernel(const int64_t* __restri
 #pragma unroll
     for (int o = 0; o < kPerLane; ++o)
       for (int j = 0; j < 64 && 64 * o + j < k; ++j) {
-        const int other = __shfl(id[o], j, 64);
+        const int other = __builtin_amdgcn_readlane(id[o], j);
         const int their = other < 0 ? kNoColumn : other;
         place += their < key || (their == key && 64 * o + j < s);
       }
