@@ -1397,7 +1397,7 @@ __device__ __forceinline__ void store_lines(char* blk, const __amdgpu_buffer_rsr
 // The blocks lie past the two stages (dense head: 160 KB in all), or in the first stage's head tile, which the
 // 4-bit head's next tile fills only after its first barrier.
 // AFFINE: the gradient of any loss of the softmax that leaves G = p (alpha_t + beta_t z) but for a few columns a row
-// (lce_bwd_g_columns_kernel), p the softmax of z / temperature. Rows with neither factor are written as zeros, whatever their
+// (lce_bwd_g_columns_kernel), p the softmax of z / temperature; 2: without beta. Rows with neither factor are written as zeros, whatever their
 // hidden state holds.
 // ------------------------------------------------------------------------------------------
 template <int Q4, int AFFINE = 0>
@@ -1449,7 +1449,7 @@ void lce_bwd_g_persist_kernel(const bf16_t* __restrict__ H, const bf16_t* __rest
     if (t < N) {
       if constexpr (AFFINE) {
         coef[j] = rows.alpha[t];
-        if (rows.beta) slope[j] = rows.beta[t];
+        if constexpr (AFFINE == 1) slope[j] = rows.beta[t];
       } else {
         coef[j] = targets[t] == ignore_index ? 0.f : dnll[t];
       }
@@ -1535,7 +1535,7 @@ void lce_bwd_g_persist_kernel(const bf16_t* __restrict__ H, const bf16_t* __rest
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const float z = acc[i][j][4 * q + u];
-          gv[u] = fast_exp2(z * rows.scale2 - l2[j]) * __builtin_fmaf(slope[j], finite_exponent(z), coef[j]);
+          gv[u] = fast_exp2(z * rows.scale2 - l2[j]) * (AFFINE == 1 ? __builtin_fmaf(slope[j], finite_exponent(z), coef[j]) : coef[j]);
         }
         return u32x2{pack_bf16x2(gv[0], gv[1]) & keep, pack_bf16x2(gv[2], gv[3]) & keep};
       }
@@ -2342,8 +2342,9 @@ static hipError_t lce_bwd_rows(const LceHead& h, const bf16_t* H, const int64_t*
       // One resident workgroup per CU (160 KiB of LDS, all of it, with a dense head; 130 KiB with a 4-bit one).
       const int ns = lce_nsplit(N, (long)ctiles * kTile, 1);
       dim3 pgrid(rtiles * ns);
-      auto gradient = affine ? (gq4 ? lce_bwd_g_persist_kernel<1, 1> : lce_bwd_g_persist_kernel<0, 1>)
-                             : (gq4 ? lce_bwd_g_persist_kernel<1, 0> : lce_bwd_g_persist_kernel<0, 0>);
+      auto gradient = !affine ? (gq4 ? lce_bwd_g_persist_kernel<1, 0> : lce_bwd_g_persist_kernel<0, 0>)
+                      : affine->rows.beta ? (gq4 ? lce_bwd_g_persist_kernel<1, 1> : lce_bwd_g_persist_kernel<0, 1>)
+                                          : (gq4 ? lce_bwd_g_persist_kernel<1, 2> : lce_bwd_g_persist_kernel<0, 2>);
       hipLaunchKernelGGL(gradient, pgrid, block, 0, stream, H, gw, h.wq, h.sc, h.bi, targets, lse, dnll, ignore_index, N, D,
                          V, vb, ve, ctiles, ns, ldg, wrow0, Gbuf, affine ? affine->rows : AffineRows{});
       hipError_t pe = hipGetLastError();
