@@ -430,7 +430,7 @@ void lce_few_kernel(const T* __restrict__ H, const T* __restrict__ W, const uint
 // ------------------------------------------------------------------------------------------
 // The logits of a gather (GatherPlan): C[v][entry] = W_v . H_token, 128 x 128 a workgroup (4 waves of 64 x 64), 64-deep stages
 // through registers, a stage ahead. Bound by what it fetches again: the head once (nearly every group is wanted by some token) and
-// the hidden rows for every entry (2 D bytes each). 8 of 8192 x 4096 x 151936: 344 us, 250 of them the head's bytes.
+// the hidden rows for every entry (2 D bytes each). 8 of 8192 x 4096 x 151936: 343 us, 250 of them the head's bytes.
 // ------------------------------------------------------------------------------------------
 template <int Q4>
 __global__ __launch_bounds__(256) void lce_gather_kernel(const bf16_t* __restrict__ H, const bf16_t* __restrict__ W,
@@ -803,7 +803,7 @@ __global__ __launch_bounds__(kPick) void score_top_kernel(const float* __restric
 //   jsd      b KL(t | m) + (1 - b) KL(q | m), m = b t + (1 - b) q:  f = (1 - b) log(q / m), f_R = (1 - b) log(R / m_R)
 // the gradient by a logit is p (f_R - F) off the list and q (f - F) on it, F = sum q f + R f_R. R and T (but in F) are at least
 // kTailFloor. From the partials on in 64 bits: T is a difference, and the products above are what take the time
-// (8192 lists of 64: 16 us, their sorting 38, the products 21.7 ms).
+// (8192 lists of 64: 16 us, their sorting 35, the products 21.6 ms).
 // ------------------------------------------------------------------------------------------
 __device__ __forceinline__ double wave_sum64(double v) {
 #pragma unroll

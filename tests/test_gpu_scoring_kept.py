@@ -10,8 +10,8 @@ from mlx_train_perf import DenseHead, _native, distillation_loss, token_logprobs
 
 pytestmark = pytest.mark.gpu
 
-_N, _V = 200, 3000
-_KEPT = _N * 3072 * 4
+_N, _V = 200, 3200
+_KEPT = _N * _V * 4
 
 
 @pytest.fixture(params=[True, False], ids=["nodes", "functions"])
